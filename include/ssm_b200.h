@@ -37,7 +37,7 @@
 extern "C" {
 #endif
 
-#define SSM_B200_ABI_VERSION 5
+#define SSM_B200_ABI_VERSION 6
 
 #if defined(__GNUC__)
 #define SSM_API __attribute__((visibility("default")))
@@ -324,6 +324,73 @@ SSM_API int ssm_conv1d_bwd(int64_t B, int64_t L, int64_t D, int64_t K, ssm_view 
                    const float* weight, const float* bias, int32_t silu, ssm_view dout,
                    ssm_view dx, float* dweight, float* dbias,
                    void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------------
+ * Gated delta rule: the other recurrence of language models' token mixers.  No counterpart in
+ * the reference.  Per value head, with a state S (dk, dv):
+ *
+ *   S_t = e^(g_t) S_{t-1} + beta_t k_t (v_t - e^(g_t) S_{t-1}^T k_t)^T,   o_t = scale S_t^T q_t
+ *
+ * q, k: (B, L, Hk, dk); v, o: (B, L, Hv, dv), Hv a multiple of Hk (value head h uses key head
+ * h / (Hv / Hk)); all four in one dtype, SSM_F32 or SSM_BF16, with any batch, row and head
+ * strides.  g (log decay, <= 0; -inf resets the state) and beta: (B, L, Hv) float32 views, unit
+ * stride along the heads.  h0, last, dlast, dh0: (B, Hv, dk, dv) dense float32.  dk <= 128.
+ *
+ * ssm_gated_delta_fwd: h0 NULL = zeros; last may be NULL.  saved: NULL, or
+ * ssm_gated_delta_saved_size bytes that a training call keeps for ssm_gated_delta_bwd.
+ * ssm_gated_delta_bwd: gradients from d_o (like o, any strides) and dlast (NULL = zeros): d_q, d_k
+ * (summed over the value heads of a key head), d_v in the inputs' dtype; d_g, d_beta (B, L, Hv)
+ * dense float32; dh0 may be NULL.  Every sum has a fixed order: results are reproducible.
+ * workspace: ssm_gated_delta_workspace_size bytes (backward = 0 / 1).
+ * ------------------------------------------------------------------------------- */
+typedef struct {
+  const void* ptr;
+  int32_t dtype;          /* ssm_dtype */
+  int32_t reserved;
+  int64_t batch_stride;   /* in elements; the innermost stride is 1 */
+  int64_t row_stride;
+  int64_t head_stride;
+} ssm_heads;
+
+SSM_API int ssm_gated_delta_workspace_size(int64_t B, int64_t L, int64_t Hk, int64_t Hv, int64_t dk, int64_t dv,
+                                   int32_t dtype, int32_t backward, size_t* bytes);
+SSM_API int ssm_gated_delta_saved_size(int64_t B, int64_t L, int64_t Hk, int64_t Hv, int64_t dk, int64_t dv,
+                               int32_t dtype, size_t* bytes);
+SSM_API int ssm_gated_delta_fwd(int64_t B, int64_t L, int64_t Hk, int64_t Hv, int64_t dk, int64_t dv,
+                        ssm_heads q, ssm_heads k, ssm_heads v, ssm_view g, ssm_view beta, const float* h0, float scale,
+                        ssm_heads o, float* last, void* saved, void* workspace, size_t workspace_bytes, void* stream);
+SSM_API int ssm_gated_delta_bwd(int64_t B, int64_t L, int64_t Hk, int64_t Hv, int64_t dk, int64_t dv,
+                        ssm_heads q, ssm_heads k, ssm_heads v, ssm_view g, ssm_view beta, float scale,
+                        const void* saved, ssm_heads d_o, const float* dlast, ssm_heads d_q, ssm_heads d_k,
+                        ssm_heads d_v, float* d_g, float* d_beta, float* dh0,
+                        void* workspace, size_t workspace_bytes, void* stream);
+
+/* One token of the gated delta rule: state (B, Hv, dk, dv) dense float32, updated in place; q, k, v, o
+ * (row strides ignored), g, beta (B, Hv) (row strides ignored).  Capturable in a CUDA graph. */
+SSM_API int ssm_gated_delta_state_update(int64_t B, int64_t Hk, int64_t Hv, int64_t dk, int64_t dv, float* state,
+                                 ssm_heads q, ssm_heads k, ssm_heads v, ssm_view g, ssm_view beta, float scale,
+                                 ssm_heads o, void* stream);
+
+/* ---------------------------------------------------------------------------------
+ * Group norm, channels last, with an activation and a gate.  No counterpart in the reference.
+ *   n = (x - mean) rstd,   y = act(n weight + bias) silu(z)
+ * x, z, y: views (samples, positions, C) in one dtype, SSM_F32 or SSM_BF16.  mean (0 unless center)
+ * and rstd = 1 / sqrt(var + eps) over the positions * C / groups elements of a sample and group.  One
+ * position per sample is the norm of every head of every token.  weight, bias: (C) float32 or NULL (1, 0);
+ * silu != 0: act = SiLU, else the identity; z.ptr may be NULL (no gate).  stats: (samples, groups, 2)
+ * float32, mean and rstd, or NULL where no backward follows.
+ * Backward: dx, dz (iff z) in x's dtype, dweight and dbias (C) float32 or NULL, summed in a fixed order.
+ * workspace: ssm_group_norm_workspace_size bytes (backward = 0 / 1).
+ * ------------------------------------------------------------------------------- */
+SSM_API int ssm_group_norm_workspace_size(int64_t samples, int64_t positions, int64_t C, int64_t groups,
+                                  int32_t backward, size_t* bytes);
+SSM_API int ssm_group_norm_fwd(int64_t samples, int64_t positions, int64_t C, int64_t groups, ssm_view x,
+                       const float* weight, const float* bias, float eps, int32_t center, int32_t silu, ssm_view z,
+                       ssm_view y, float* stats, void* workspace, size_t workspace_bytes, void* stream);
+SSM_API int ssm_group_norm_bwd(int64_t samples, int64_t positions, int64_t C, int64_t groups, ssm_view x,
+                       const float* weight, const float* bias, int32_t center, int32_t silu, ssm_view z,
+                       const float* stats, ssm_view dy, ssm_view dx, float* dweight, float* dbias, ssm_view dz,
+                       void* workspace, size_t workspace_bytes, void* stream);
 
 /* ABI version of the loaded library (SSM_B200_ABI_VERSION). */
 SSM_API int ssm_abi_version(void);

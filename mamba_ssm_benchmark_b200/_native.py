@@ -17,7 +17,7 @@ SSM_OK, SSM_ERR_INVALID, SSM_ERR_DTYPE, SSM_ERR_WORKSPACE, SSM_ERR_CUDA, SSM_ERR
 SSM_F32, SSM_BF16 = 0, 1
 METHODS = {"zoh": 0, "euler": 1, "bilinear": 2}
 DTYPES = {torch.float32: SSM_F32, torch.bfloat16: SSM_BF16}
-ABI_VERSION = 5
+ABI_VERSION = 6
 
 # Every symbol include/ssm_b200.h declares (checked by the tests).
 EXPORTED = (
@@ -27,6 +27,8 @@ EXPORTED = (
     "ssm_scan_bwd_summary", "ssm_conv1d_fwd", "ssm_conv1d_bwd_workspace_size", "ssm_conv1d_bwd",
     "selective_scan_fwd", "selective_scan_bwd", "selective_state_update", "ssm_scan_fwd_ex", "ssm_scan_bwd_ex",
     "ssm_scan_bwd_plan", "ssm_compose_shards",
+    "ssm_gated_delta_workspace_size", "ssm_gated_delta_saved_size", "ssm_gated_delta_fwd", "ssm_gated_delta_bwd",
+    "ssm_gated_delta_state_update", "ssm_group_norm_workspace_size", "ssm_group_norm_fwd", "ssm_group_norm_bwd",
 )
 
 
@@ -46,7 +48,15 @@ class SsmDeltaOpts(ctypes.Structure):
                 ("dbias", ctypes.c_void_p)]
 
 
+class SsmHeads(ctypes.Structure):
+    """ssm_heads: a (B, rows, heads, width) tensor with unit stride along the width."""
+    _fields_ = [("ptr", ctypes.c_void_p), ("dtype", ctypes.c_int32), ("reserved", ctypes.c_int32),
+                ("batch_stride", ctypes.c_int64), ("row_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64)]
+
+
 _V = SsmView
+_H = SsmHeads
+_F = ctypes.c_float
 _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
 _I32 = ctypes.c_int32
@@ -77,6 +87,20 @@ _SIGNATURES = {
     "ssm_scan_bwd_noalloc": (ctypes.c_int, [_I64, _I64, _I64, _I64, _I32, _V, _V, _P, _V, _V, _P, _V, _P,
                                             _P, _V, _V, _P, _V, _V, _P, _V, _V, _P, _V, _P, _P]),
 }
+
+_DIMS = [_I64] * 6                  # B, L, Hk, Hv, dk, dv
+_SIGNATURES.update({
+    "ssm_gated_delta_workspace_size": (ctypes.c_int, _DIMS + [_I32, _I32, ctypes.POINTER(_SZ)]),
+    "ssm_gated_delta_saved_size": (ctypes.c_int, _DIMS + [_I32, ctypes.POINTER(_SZ)]),
+    "ssm_gated_delta_fwd": (ctypes.c_int, _DIMS + [_H, _H, _H, _V, _V, _P, _F, _H, _P, _P, _P, _SZ, _P]),
+    "ssm_gated_delta_bwd": (ctypes.c_int, _DIMS + [_H, _H, _H, _V, _V, _F, _P, _H, _P, _H, _H, _H, _P, _P, _P,
+                                                   _P, _SZ, _P]),
+    "ssm_gated_delta_state_update": (ctypes.c_int, [_I64] * 5 + [_P, _H, _H, _H, _V, _V, _F, _H, _P]),
+    "ssm_group_norm_workspace_size": (ctypes.c_int, [_I64] * 4 + [_I32, ctypes.POINTER(_SZ)]),
+    "ssm_group_norm_fwd": (ctypes.c_int, [_I64] * 4 + [_V, _P, _P, _F, _I32, _I32, _V, _V, _P, _P, _SZ, _P]),
+    "ssm_group_norm_bwd": (ctypes.c_int, [_I64] * 4 + [_V, _P, _P, _I32, _I32, _V, _P, _V, _V, _P, _P, _V,
+                                                       _P, _SZ, _P]),
+})
 
 _OPTS = ctypes.POINTER(SsmDeltaOpts)
 _SIGNATURES["ssm_scan_fwd_ex"] = (ctypes.c_int, _SIGNATURES["ssm_scan_fwd"][1][:17] + [_OPTS] +
@@ -145,6 +169,12 @@ def view2(t):
     return SsmView(t.data_ptr(), DTYPES[t.dtype], 0, t.stride(0), 0)
 
 
+def heads4(t):
+    """(B, rows, heads, width) tensor with unit inner stride -> ssm_heads."""
+    assert t.dim() == 4 and (t.stride(3) == 1 or t.shape[3] == 1), "inner dimension must be contiguous"
+    return SsmHeads(t.data_ptr(), DTYPES[t.dtype], 0, t.stride(0), t.stride(1), t.stride(2))
+
+
 def delta_opts(bias, softplus, dbias=None):
     """ssm_delta_opts for the _ex entry points, or None (plain delta)."""
     if not softplus:
@@ -184,6 +214,26 @@ def bwd_plan(B, L, D, N, dtype):
 def bwd_workspace_bytes(B, L, D, N):
     n = _SZ(0)
     check(lib().ssm_scan_bwd_workspace_size(B, L, D, N, ctypes.byref(n)), "ssm_scan_bwd_workspace_size")
+    return n.value
+
+
+def gated_delta_workspace_bytes(dims, dtype, backward):
+    n = _SZ(0)
+    check(lib().ssm_gated_delta_workspace_size(*dims, DTYPES[dtype], int(backward), ctypes.byref(n)),
+          "ssm_gated_delta_workspace_size")
+    return n.value
+
+
+def gated_delta_saved_bytes(dims, dtype):
+    n = _SZ(0)
+    check(lib().ssm_gated_delta_saved_size(*dims, DTYPES[dtype], ctypes.byref(n)), "ssm_gated_delta_saved_size")
+    return n.value
+
+
+def norm_workspace_bytes(samples, positions, C, groups, backward):
+    n = _SZ(0)
+    check(lib().ssm_group_norm_workspace_size(samples, positions, C, groups, int(backward), ctypes.byref(n)),
+          "ssm_group_norm_workspace_size")
     return n.value
 
 

@@ -33,6 +33,8 @@ namespace ssm {
 // Internal (not exported): lets other translation units set the message ssm_last_error_message
 // returns.
 int report_error(int code, const char* msg);
+// The current device's error word (see below), for kernels launched from other translation units.
+int* device_error_word();
 }  // namespace ssm
 
 // Device-side error word set by kernels whose bounded waits gave up.
@@ -438,6 +440,7 @@ int fwd_impl(int phase, int64_t B, int64_t L, int64_t D, int64_t N, int32_t meth
 }  // namespace
 
 int ssm::report_error(int code, const char* msg) { return fail(code, "%s", msg); }
+int* ssm::device_error_word() { return device_error_ptr(); }
 
 extern "C" {
 
