@@ -378,7 +378,8 @@ SSM_API int ssm_gated_delta_state_update(int64_t B, int64_t Hk, int64_t Hv, int6
  * and rstd = 1 / sqrt(var + eps) over the positions * C / groups elements of a sample and group.  One
  * position per sample is the norm of every head of every token.  weight, bias: (C) float32 or NULL (1, 0);
  * silu != 0: act = SiLU, else the identity; z.ptr may be NULL (no gate).  stats: (samples, groups, 2)
- * float32, mean and rstd, or NULL where no backward follows.
+ * float32, mean and rstd, or NULL; written with more than one position and read by the backward, which forms
+ * them again when it is given NULL.
  * Backward: dx, dz (iff z) in x's dtype, dweight and dbias (C) float32 or NULL, summed in a fixed order.
  * workspace: ssm_group_norm_workspace_size bytes (backward = 0 / 1).
  * ------------------------------------------------------------------------------- */
@@ -388,7 +389,7 @@ SSM_API int ssm_group_norm_fwd(int64_t samples, int64_t positions, int64_t C, in
                        const float* weight, const float* bias, float eps, int32_t center, int32_t silu, ssm_view z,
                        ssm_view y, float* stats, void* workspace, size_t workspace_bytes, void* stream);
 SSM_API int ssm_group_norm_bwd(int64_t samples, int64_t positions, int64_t C, int64_t groups, ssm_view x,
-                       const float* weight, const float* bias, int32_t center, int32_t silu, ssm_view z,
+                       const float* weight, const float* bias, float eps, int32_t center, int32_t silu, ssm_view z,
                        const float* stats, ssm_view dy, ssm_view dx, float* dweight, float* dbias, ssm_view dz,
                        void* workspace, size_t workspace_bytes, void* stream);
 

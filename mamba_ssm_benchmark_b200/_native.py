@@ -6,6 +6,7 @@ This module only loads the library and marshals torch tensors into the ABI's pla
 """
 
 import ctypes
+import functools
 import os
 import threading
 
@@ -98,7 +99,7 @@ _SIGNATURES.update({
     "ssm_gated_delta_state_update": (ctypes.c_int, [_I64] * 5 + [_P, _H, _H, _H, _V, _V, _F, _H, _P]),
     "ssm_group_norm_workspace_size": (ctypes.c_int, [_I64] * 4 + [_I32, ctypes.POINTER(_SZ)]),
     "ssm_group_norm_fwd": (ctypes.c_int, [_I64] * 4 + [_V, _P, _P, _F, _I32, _I32, _V, _V, _P, _P, _SZ, _P]),
-    "ssm_group_norm_bwd": (ctypes.c_int, [_I64] * 4 + [_V, _P, _P, _I32, _I32, _V, _P, _V, _V, _P, _P, _V,
+    "ssm_group_norm_bwd": (ctypes.c_int, [_I64] * 4 + [_V, _P, _P, _F, _I32, _I32, _V, _P, _V, _V, _P, _P, _V,
                                                        _P, _SZ, _P]),
 })
 
@@ -175,6 +176,12 @@ def heads4(t):
     return SsmHeads(t.data_ptr(), DTYPES[t.dtype], 0, t.stride(0), t.stride(1), t.stride(2))
 
 
+def heads3(t):
+    """(B, heads, width) tensor with unit inner stride -> ssm_heads with one row per batch entry."""
+    assert t.dim() == 3 and (t.stride(2) == 1 or t.shape[2] == 1), "inner dimension must be contiguous"
+    return SsmHeads(t.data_ptr(), DTYPES[t.dtype], 0, t.stride(0), 0, t.stride(1))
+
+
 def delta_opts(bias, softplus, dbias=None):
     """ssm_delta_opts for the _ex entry points, or None (plain delta)."""
     if not softplus:
@@ -189,6 +196,26 @@ def ptr(t):
 
 def stream_of(device):
     return torch.cuda.current_stream(device).cuda_stream
+
+
+# The stream handle without building a torch.cuda.Stream (about 1.5 us of a decode step's host time), where
+# this torch has it.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def call(name, dev, *args):
+    """Calls the entry point ``name`` with ``args`` and ``dev``'s current stream, on device ``dev``.  The device
+    is switched only where it is not current: the context manager costs more than a small launch."""
+    index = dev.index
+    stream = _raw_stream(index) if _raw_stream is not None else stream_of(dev)
+    fn = getattr(_lib or lib(), name)
+    if index == torch.cuda.current_device():
+        rc = fn(*args, stream)
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, stream)
+    if rc != SSM_OK:
+        check(rc, name)
 
 
 def conv_workspace_bytes(B, L, D, K):
@@ -217,6 +244,7 @@ def bwd_workspace_bytes(B, L, D, N):
     return n.value
 
 
+@functools.lru_cache(maxsize=4096)
 def gated_delta_workspace_bytes(dims, dtype, backward):
     n = _SZ(0)
     check(lib().ssm_gated_delta_workspace_size(*dims, DTYPES[dtype], int(backward), ctypes.byref(n)),
@@ -224,12 +252,14 @@ def gated_delta_workspace_bytes(dims, dtype, backward):
     return n.value
 
 
+@functools.lru_cache(maxsize=4096)
 def gated_delta_saved_bytes(dims, dtype):
     n = _SZ(0)
     check(lib().ssm_gated_delta_saved_size(*dims, DTYPES[dtype], ctypes.byref(n)), "ssm_gated_delta_saved_size")
     return n.value
 
 
+@functools.lru_cache(maxsize=4096)
 def norm_workspace_bytes(samples, positions, C, groups, backward):
     n = _SZ(0)
     check(lib().ssm_group_norm_workspace_size(samples, positions, C, groups, int(backward), ctypes.byref(n)),

@@ -70,39 +70,68 @@ __device__ __forceinline__ bool rows_aligned16(const Heads& h, int es) {
            (uintptr_t)(h.sh * es)) & 15) == 0;
 }
 
-template <typename T, int NP, int DKP>
-struct PrepSmem {
-  __nv_bfloat16 k[NP][kC * DKP], q[NP][kC * DKP];
-  float A[kC][kPitch], T_[kC][kPitch], P[kC][kPitch], tmp[32][36];
+template <int NP, int DKP>
+struct alignas(128) PrepSmem {
+  union {
+    struct {
+      __nv_bfloat16 k[NP][kC * DKP], q[NP][kC * DKP];
+    };
+    struct {                            // after the products: A, and T in its place
+      float T_[kC][kPitch], tmp[32][36];
+    };
+  };
   float gh[kC], gl[kC], beta[kC];
 };
 
 template <typename T, int NP, int DKP>
-__global__ void __launch_bounds__(128) delta_prep(const DeltaParams p) {
+__global__ void __launch_bounds__(128, NP == 1 ? 5 : 2) delta_prep(const __grid_constant__ DeltaParams p) {
   extern __shared__ __align__(128) unsigned char smem_raw[];
-  auto& s = *reinterpret_cast<PrepSmem<T, NP, DKP>*>(smem_raw);
+  auto& s = *reinterpret_cast<PrepSmem<NP, DKP>*>(smem_raw);
   const int ch = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int t0 = ch * kC, rows = min(kC, p.L - t0), hk = h / p.group;
   const size_t at = ((size_t)b * p.Hv + h) * p.n + ch;
   const size_t atk = ((size_t)b * p.Hk + hk) * p.n + ch;
 
-  // q and k in pieces: into shared memory and, once per key head, into the tiles the chain kernels load
-  {
-    const bool writer = h % p.group == 0;
-    const T* kb = static_cast<const T*>(p.k.ptr) + b * p.k.sb + t0 * p.k.sl + hk * p.k.sh;
-    const T* qb = static_cast<const T*>(p.q.ptr) + b * p.q.sb + t0 * p.q.sl + hk * p.q.sh;
-    const bool kv = rows_aligned16(p.k, sizeof(T)), qv = rows_aligned16(p.q, sizeof(T));
-    __nv_bfloat16* kg = writer ? p.kimg + atk * (NP * kC * DKP) : nullptr;
-    __nv_bfloat16* qg = writer ? p.qimg + atk * (NP * kC * DKP) : nullptr;
-    for (int e = tid; e < kC * DKP / 8; e += 128) {
-      const int r = e / (DKP / 8), grp = e % (DKP / 8), width = r < rows ? p.dkw : 0;
-      float x[8], y[8];
-      load8<T>(kb + (long long)r * p.k.sl, grp * 8, width, kv, x);
-      load8<T>(qb + (long long)r * p.q.sl, grp * 8, width, qv, y);
-      const int off = tile_off<DKP>(r, grp);
-      put_pieces<NP>(x, s.k[0], kg, off, kC * DKP);
-      put_pieces<NP>(y, s.q[0], qg, off, kC * DKP);
+  // q and k in pieces: into shared memory and, once per key head, into the tiles the other kernels load
+  const bool writer = h % p.group == 0;
+  const T* kbase = static_cast<const T*>(p.k.ptr) + b * p.k.sb + t0 * p.k.sl + hk * p.k.sh;
+  const T* qbase = static_cast<const T*>(p.q.ptr) + b * p.q.sb + t0 * p.q.sl + hk * p.q.sh;
+  const bool kv = rows_aligned16(p.k, sizeof(T)), qv = rows_aligned16(p.q, sizeof(T));
+  __nv_bfloat16* kg = p.kimg + atk * (NP * kC * DKP);
+  __nv_bfloat16* qg = p.qimg + atk * (NP * kC * DKP);
+  constexpr int kGroups = kC * DKP / 8 / 128;            // 8-element groups per thread and tensor
+  const bool direct = NP == 1 && kv && qv && p.dkw % 8 == 0;   // bf16 rows are the tile's rows as they are
+  if (direct) {
+#pragma unroll
+    for (int i = 0; i < kGroups; ++i) {
+      const int e = tid + 128 * i, r = e / (DKP / 8), grp = e % (DKP / 8), off = tile_off<DKP>(r, grp);
+      if (r < rows && grp * 8 < p.dkw) {
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(&s.k[0][off])), "l"(kbase + r * p.k.sl + grp * 8) : "memory");
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(&s.q[0][off])), "l"(qbase + r * p.q.sl + grp * 8) : "memory");
+      } else {
+        *reinterpret_cast<uint4*>(&s.k[0][off]) = make_uint4(0, 0, 0, 0);
+        *reinterpret_cast<uint4*>(&s.q[0][off]) = make_uint4(0, 0, 0, 0);
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  } else {
+    constexpr int kBatch = 4;                              // loads in flight before the first is used
+#pragma unroll 1
+    for (int i0 = 0; i0 < kGroups; i0 += kBatch) {
+      float x[kBatch][8], y[kBatch][8];
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const int e = tid + 128 * (i0 + i), r = e / (DKP / 8), grp = e % (DKP / 8), width = r < rows ? p.dkw : 0;
+        load8<T>(kbase + r * p.k.sl, grp * 8, width, kv, x[i]);
+        load8<T>(qbase + r * p.q.sl, grp * 8, width, qv, y[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const int e = tid + 128 * (i0 + i), off = tile_off<DKP>(e / (DKP / 8), e % (DKP / 8));
+        put_pieces<NP>(x[i], s.k[0], writer ? kg : nullptr, off, kC * DKP);
+        put_pieces<NP>(y[i], s.q[0], writer ? qg : nullptr, off, kC * DKP);
+      }
     }
   }
   // running sums of g.  In double and kept as two floats: differences of neighbours stay exact to fp32
@@ -112,9 +141,9 @@ __global__ void __launch_bounds__(128) delta_prep(const DeltaParams p) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int r = 2 * lane + i;
-      float g = r < rows ? p.g[b * p.gsb + (t0 + r) * p.gsl + h] : 0.0f;
-      g = g < -1000.0f ? -1000.0f : g;
-      acc[i] = (double)g * 1.4426950408889634;
+      float gate = r < rows ? p.g[b * p.gsb + (t0 + r) * p.gsl + h] : 0.0f;
+      gate = gate < -1000.0f ? -1000.0f : gate;
+      acc[i] = (double)gate * 1.4426950408889634;
       s.beta[r] = r < rows ? p.beta[b * p.bsb + (t0 + r) * p.bsl + h] : 0.0f;
     }
     acc[1] += acc[0];
@@ -140,12 +169,21 @@ __global__ void __launch_bounds__(128) delta_prep(const DeltaParams p) {
       vec[4 * kC + r] = lo;
     }
   }
-  for (int e = tid; e < kC * kPitch; e += 128) (&s.T_[0][0])[e] = 0.0f;
+  if (direct) asm volatile("cp.async.wait_group 0;" ::: "memory");
   __syncthreads();
+  if (direct && writer) {
+#pragma unroll
+    for (int i = 0; i < kGroups; ++i) {
+      const int e = tid + 128 * i;
+      reinterpret_cast<uint4*>(kg)[e] = reinterpret_cast<const uint4*>(s.k[0])[e];
+      reinterpret_cast<uint4*>(qg)[e] = reinterpret_cast<const uint4*>(s.q[0])[e];
+    }
+  }
 
   // k.k and q.k of the warp's 16 rows against the columns up to its own
+  float kk[kC / 8][4];
   {
-    float kk[kC / 8][4], qk[kC / 8][4];
+    float qk[kC / 8][4];
     zero(kk);
     zero(qk);
     const uint32_t sk = smem_u32(s.k[0]), sq = smem_u32(s.q[0]);
@@ -162,287 +200,426 @@ __global__ void __launch_bounds__(128) delta_prep(const DeltaParams p) {
         if (jp > warp) break;
 #pragma unroll
         for (int pb = 0; pb < NP; ++pb) {
-          uint32_t bf[4];
-          load_b<DKP>(bf, sk + pb * (kC * DKP * 2), 2 * jp, kb, lane);
-          mma_pieces<NP, 2>(kk[2 * jp], kk[2 * jp + 1], ak, bf, pb);
-          mma_pieces<NP, 2>(qk[2 * jp], qk[2 * jp + 1], aq, bf, pb);
+          uint32_t bf[1][4];
+          load_b<DKP>(bf[0], sk + pb * (kC * DKP * 2), 2 * jp, kb, lane);
+          mma_pieces<0, 2>(kk, 2 * jp, ak, bf, pb);
+          mma_pieces<0, 2>(qk, 2 * jp, aq, bf, pb);
         }
       }
     }
-    const int g = lane >> 2, t = lane & 3;
+    // P goes out as it is; A stays in registers until every warp is past the tiles that it replaces
 #pragma unroll
     for (int j = 0; j < kC / 8; ++j)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int i = 16 * warp + g + 8 * (e >> 1), c = 8 * j + 2 * t + (e & 1);
-        const float d = i >= c ? ex2((s.gh[i] - s.gh[c]) + (s.gl[i] - s.gl[c])) : 0.0f;
-        s.A[i][c] = i > c ? s.beta[i] * (d * kk[j][e]) : 0.0f;
-        s.P[i][c] = i >= c ? p.scale * (d * qk[j][e]) : 0.0f;
+      for (int r = 0; r < 2; ++r) {
+        const int i = 16 * warp + g + 8 * r, c = 8 * j + 2 * t;
+        float x[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float d = i >= c + e ? ex2((s.gh[i] - s.gh[c + e]) + (s.gl[i] - s.gl[c + e])) : 0.0f;
+          x[e] = i >= c + e ? p.scale * (d * qk[j][2 * r + e]) : 0.0f;
+          kk[j][2 * r + e] = i > c + e ? s.beta[i] * (d * kk[j][2 * r + e]) : 0.0f;
+        }
+        uint32_t q[3];
+        split<3>(x[0], x[1], q);
+        __nv_bfloat16* o = p.pimg + at * (3 * kTri) + tile_off<kC>(i, j) + 2 * t;
+#pragma unroll
+        for (int k = 0; k < 3; ++k) *reinterpret_cast<uint32_t*>(o + k * kTri) = q[k];
       }
   }
   __syncthreads();
+#pragma unroll
+  for (int j = 0; j < kC / 8; ++j)
+#pragma unroll
+    for (int r = 0; r < 2; ++r)
+      *reinterpret_cast<float2*>(&s.T_[16 * warp + g + 8 * r][8 * j + 2 * t]) = make_float2(kk[j][2 * r], kk[j][2 * r + 1]);
+  __syncthreads();
 
-  // T = (I + A)^-1 by forward substitution: the diagonal 16 x 16 blocks, then the blocks below them
-  // from the blocks beside: T21 = -T22 A21 T11.
-  if (lane < 16) {
-    const int r0 = 16 * warp;
-    float t[16];
+  // T = (I + A)^-1 in A's place by forward substitution: the diagonal 16 x 16 blocks, then the blocks below
+  // them from the blocks beside: T21 = -T22 A21 T11.
+  {
+    const int r0 = 16 * warp, col = lane & 15;
+    float x[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      float v = i == lane ? 1.0f : 0.0f;
+      float v[4] = {i == col ? 1.0f : 0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int m = 0; m < i; ++m) v = fmaf(-s.A[r0 + i][r0 + m], t[m], v);
-      t[i] = v;
-      s.T_[r0 + i][r0 + lane] = v;
+      for (int m0 = 0; m0 < i; m0 += 4) {
+        float a[4];
+        load4(&s.T_[r0 + i][r0 + m0], a);
+#pragma unroll
+        for (int m = 0; m < 4; ++m)
+          if (m0 + m < i) v[m] = fmaf(-a[m], x[m0 + m], v[m]);
+      }
+      x[i] = (v[0] + v[1]) + (v[2] + v[3]);
+    }
+    __syncwarp();
+    if (lane < 16) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s.T_[r0 + i][r0 + lane] = x[i];
     }
   }
   __syncthreads();
+  // y[0 .. W) of a row of F = (A or T block)[row][m] x G[m][c ..], m < M
+  auto block_row = [&](auto& y, int M, const float* frow, float sign, const float* grow, int pitch) {
+    constexpr int W = sizeof(y) / sizeof(float);
+#pragma unroll 8
+    for (int m = 0; m < M; ++m) {
+      const float a = sign * frow[m];
+#pragma unroll
+      for (int e = 0; e < W; e += 4) {
+        float x[4];
+        load4(grow + m * pitch + e, x);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) y[e + q] = fmaf(a, x[q], y[e + q]);
+      }
+    }
+  };
   {
     const int pr = 32 * (tid >> 6), r = (tid & 63) >> 2, c = 4 * (tid & 3);
-    float y[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int m = 0; m < 16; ++m) {
-      const float a = s.A[pr + 16 + r][pr + m];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) y[e] = fmaf(a, s.T_[pr + m][pr + c + e], y[e]);
-    }
+    float y[4] = {}, x[4] = {};
+    block_row(y, 16, &s.T_[pr + 16 + r][pr], 1.0f, &s.T_[pr][pr + c], kPitch);
 #pragma unroll
     for (int e = 0; e < 4; ++e) s.tmp[r][(pr >> 1) + c + e] = y[e];
-  }
-  __syncthreads();
-  {
-    const int pr = 32 * (tid >> 6), r = (tid & 63) >> 2, c = 4 * (tid & 3);
-    float y[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int m = 0; m < 16; ++m) {
-      const float a = s.T_[pr + 16 + r][pr + 16 + m];
+    __syncthreads();
+    block_row(x, 16, &s.T_[pr + 16 + r][pr + 16], -1.0f, &s.tmp[0][(pr >> 1) + c], 36);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) y[e] = fmaf(-a, s.tmp[m][(pr >> 1) + c + e], y[e]);
-    }
-#pragma unroll
-    for (int e = 0; e < 4; ++e) s.T_[pr + 16 + r][pr + c + e] = y[e];
+    for (int e = 0; e < 4; ++e) s.T_[pr + 16 + r][pr + c + e] = x[e];
   }
   __syncthreads();
   {
     const int r = tid >> 2, c = 8 * (tid & 3);
-    float y[8] = {};
-    for (int m = 0; m < 32; ++m) {
-      const float a = s.A[32 + r][m];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] = fmaf(a, s.T_[m][c + e], y[e]);
-    }
+    float y[8] = {}, x[8] = {};
+    block_row(y, 32, &s.T_[32 + r][0], 1.0f, &s.T_[0][c], kPitch);
 #pragma unroll
     for (int e = 0; e < 8; ++e) s.tmp[r][c + e] = y[e];
     __syncthreads();
+    block_row(x, 32, &s.T_[32 + r][32], -1.0f, &s.tmp[0][c], 36);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) y[e] = 0.0f;
-    for (int m = 0; m < 32; ++m) {
-      const float a = s.T_[32 + r][32 + m];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] = fmaf(-a, s.tmp[m][c + e], y[e]);
-    }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) s.T_[32 + r][c + e] = y[e];
+    for (int e = 0; e < 8; ++e) s.T_[32 + r][c + e] = x[e];
   }
   __syncthreads();
+#pragma unroll 2
   for (int e = tid; e < kC * kC / 8; e += 128) {
-    const int r = e / (kC / 8), grp = e % (kC / 8), off = tile_off<kC>(r, grp);
-    float x[8], y[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      x[i] = s.T_[r][grp * 8 + i];
-      y[i] = s.P[r][grp * 8 + i];
-    }
-    put_pieces<3>(x, nullptr, p.timg + at * (3 * kTri), off, kTri);
-    put_pieces<3>(y, nullptr, p.pimg + at * (3 * kTri), off, kTri);
+    const int r = e / (kC / 8), grp = e % (kC / 8);
+    float x[8];
+    load8<float>(s.T_[r], 8 * grp, kC, true, x);
+    put_pieces<3>(x, nullptr, p.timg + at * (3 * kTri), tile_off<kC>(r, grp), kTri);
   }
 }
 
 // ================================================================================================
-// The chain kernels' shared memory: the tiles of one chunk, loaded by bulk copies.
+// The chain kernels: a CTA carries NS strips of 16 value channels of one head's state through all chunks, four
+// warps per strip, and one more warp loads the chunks' tiles.  The chain from chunk to chunk is what takes
+// the time: it is cut four ways inside a strip (three exchanges per chunk, barriers of four warps), and the
+// strips of a CTA run freely, so that one's exchange hides behind another's products.
+// Tiles: K is used first and last in a chunk and has two buffers where they fit, like the vectors; Q, T and P have
+// one each, refilled as soon as every strip is past them.
 // ================================================================================================
-template <int NP, int DKP, int PP>     // PP: pieces of P
-struct alignas(128) ChainStage {
-  __nv_bfloat16 k[NP][kC * DKP], q[NP][kC * DKP];
-  __nv_bfloat16 t[3][kTri], pm[PP][kTri];
-  float vec[kVec];
+template <typename T, int DKP, int PU, int PO>       // pieces of the operands uf and of
+struct alignas(16) StripSmem {
+  uint4 sf[DKP / 16][3][32], xf[4][3][32], lf[4][3][32], uf[4][PU][32], of[PO ? 4 : 1][PO ? PO : 1][PO ? 32 : 1];
+  Strip<T> in, out;
 };
-template <int NP, int DKP, int PP>
-constexpr int chain_stages() {
-  return 2 * sizeof(ChainStage<NP, DKP, PP>) + 256 <= 227 * 1024 ? 2 : 1;
-}
-template <int NP, int DKP, int PP>
-constexpr size_t chain_smem() {
-  return chain_stages<NP, DKP, PP>() * sizeof(ChainStage<NP, DKP, PP>) + 128;
-}
+template <int NP, int DKP, int PP, typename StripT, int NS, int KB>
+struct alignas(128) ChainSmem {
+  __nv_bfloat16 k[KB][NP][kC * DKP], q[NP][kC * DKP];
+  __nv_bfloat16 t[3][kTri], pm[PP][kTri];
+  StripT strip[NS];
+  float vec[2][kVec];
+  uint64_t full[7], empty[7];             // by tile
+};
+enum { kTileK = 0, kTileV = 2, kTileQ = 4, kTileT = 5, kTileP = 6, kTiles = 7 };   // K, vectors: two each
 
-template <int NP, int DKP, int PP>
-__device__ __forceinline__ void chain_load(ChainStage<NP, DKP, PP>& s, const DeltaParams& p, int b, int h, int ch,
-                                           uint64_t* bar) {
-  const size_t at = ((size_t)b * p.Hv + h) * p.n + ch;
-  const size_t atk = ((size_t)b * p.Hk + h / p.group) * p.n + ch;
-  mbar_arrive_expect_tx(bar, sizeof(s.k) + sizeof(s.q) + sizeof(s.t) + sizeof(s.pm) + sizeof(s.vec));
-  bulk_load(s.k, p.kimg + atk * (NP * kC * DKP), sizeof(s.k), bar);
-  bulk_load(s.q, p.qimg + atk * (NP * kC * DKP), sizeof(s.q), bar);
-  bulk_load(s.t, p.timg + at * (3 * kTri), sizeof(s.t), bar);
-  bulk_load(s.pm, p.pimg + at * (3 * kTri), sizeof(s.pm), bar);
-  bulk_load(s.vec, p.vec + at * kVec, sizeof(s.vec), bar);
+// The tiles of one chunk after another, chunk index by order(i), as the strips release them.
+template <int NP, int DKP, int KB, typename Smem, typename F>
+__device__ void load_tiles(Smem& s, const DeltaParams& p, int b, int h, F order) {
+  const size_t at0 = ((size_t)b * p.Hv + h) * p.n, atk0 = ((size_t)b * p.Hk + h / p.group) * p.n;
+  auto freed = [&](int tile, int use) {
+    if (use > 0) mbar_wait(&s.empty[tile], (use - 1) & 1, p.err);
+  };
+  for (int i = 0; i < p.n; ++i) {
+    const int ch = order(i);
+    auto load_k = [&] {
+      const int buf = i % KB, tile = kTileK + buf;
+      freed(tile, i / KB);
+      mbar_arrive_expect_tx(&s.full[tile], sizeof(s.k[0]));
+      bulk_load(s.k[buf], p.kimg + (atk0 + ch) * (NP * kC * DKP), sizeof(s.k[0]), &s.full[tile]);
+    };
+    freed(kTileV + (i & 1), i >> 1);
+    mbar_arrive_expect_tx(&s.full[kTileV + (i & 1)], sizeof(s.vec[0]));
+    bulk_load(s.vec[i & 1], p.vec + (at0 + ch) * kVec, sizeof(s.vec[0]), &s.full[kTileV + (i & 1)]);
+    if (KB == 2) load_k();
+    freed(kTileQ, i);
+    mbar_arrive_expect_tx(&s.full[kTileQ], sizeof(s.q));
+    bulk_load(s.q, p.qimg + (atk0 + ch) * (NP * kC * DKP), sizeof(s.q), &s.full[kTileQ]);
+    if (KB == 1) load_k();
+    freed(kTileT, i);
+    mbar_arrive_expect_tx(&s.full[kTileT], sizeof(s.t));
+    bulk_load(s.t, p.timg + (at0 + ch) * (3 * kTri), sizeof(s.t), &s.full[kTileT]);
+    freed(kTileP, i);
+    mbar_arrive_expect_tx(&s.full[kTileP], sizeof(s.pm));
+    bulk_load(s.pm, p.pimg + (at0 + ch) * (3 * kTri), sizeof(s.pm), &s.full[kTileP]);
+  }
 }
+__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void strip_sync(int strip) { asm volatile("bar.sync %0, 128;" ::"r"(strip + 1) : "memory"); }
 
-// The state (dk, dv) of a head in global memory from / to the warp's accumulators of S^T.
+// A quarter of the state (dk, dv) of a head in global memory from / to accumulators of S^T.
 template <int NT>
-__device__ __forceinline__ void state_load(const float* base, int dk, int dv, int d0, int lane, float (&S)[NT][4]) {
+__device__ __forceinline__ void state_load(const float* base, int dk, int dv, int k0, int d0, int lane, float (&S)[NT][4]) {
   const int g = lane >> 2, t = lane & 3;
 #pragma unroll
   for (int j = 0; j < NT; ++j)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const int k = 8 * j + 2 * t + (e & 1), d = d0 + g + 8 * (e >> 1);
+      const int k = k0 + 8 * j + 2 * t + (e & 1), d = d0 + g + 8 * (e >> 1);
       S[j][e] = base != nullptr && k < dk && d < dv ? base[(size_t)k * dv + d] : 0.0f;
     }
 }
 template <int NT>
-__device__ __forceinline__ void state_store(float* base, int dk, int dv, int d0, int lane, const float (&S)[NT][4]) {
+__device__ __forceinline__ void state_store(float* base, int dk, int dv, int k0, int d0, int lane, const float (&S)[NT][4]) {
   const int g = lane >> 2, t = lane & 3;
 #pragma unroll
   for (int j = 0; j < NT; ++j)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const int k = 8 * j + 2 * t + (e & 1), d = d0 + g + 8 * (e >> 1);
+      const int k = k0 + 8 * j + 2 * t + (e & 1), d = d0 + g + 8 * (e >> 1);
       if (k < dk && d < dv) base[(size_t)k * dv + d] = S[j][e];
     }
 }
+// The warp's quarter of S in operand form for the strip.
+template <int DKP>
+__device__ __forceinline__ void put_state(uint4 (*sf)[3][32], const float (&S)[DKP / 32][4], int w, int lane) {
+#pragma unroll
+  for (int j = 0; j < DKP / 32; j += 2) {
+    uint32_t a[3][4];
+    acc_to_a<3>(S, j / 2, a);
+#pragma unroll
+    for (int i = 0; i < 3; ++i)
+      sf[(w * (DKP / 32) + j) / 2][i][lane] = make_uint4(a[i][0], a[i][1], a[i][2], a[i][3]);
+  }
+}
 
-// R^T (16 x kC) = M^T-side product with a triangular kC x kC tile: D[.][i] += sum_k a[.][k] L[i][k] (TR false,
-// L lower: tiles i >= k) or D[.][j] += sum_i a[.][i] L[i][j] (TR true: tiles j <= i).
+// The warp's two column tiles of d (16 x kC) += S times the transpose of a [c][dk] tile, and, with TWO, of d2
+// for a second tile with products up to index sum MAXI2.
+template <int NP, int DKP, bool TWO, int MAXI2>
+__device__ __forceinline__ void state_product(float (&d)[2][4], float (&d2)[2][4], const uint4 (*sf)[3][32], uint32_t tile,
+                                              uint32_t tile2, int w, int lane) {
+  float low[2][4], low2[2][4];
+  zero(low);
+  zero(low2);
+#pragma unroll 4
+  for (int kb = 0; kb < DKP / 16; ++kb) {
+    uint32_t a[3][4];
+#pragma unroll
+    for (int i = 0; i < 3; ++i) get_frag(a[i], sf[kb][i][lane]);
+#pragma unroll
+    for (int pb = 0; pb < NP; ++pb) {
+      uint32_t bf[1][4], cf[1][4];
+      load_b2<DKP>(bf[0], tile + pb * (kC * DKP * 2), w, kb, lane);
+      if (TWO && pb <= MAXI2) load_b2<DKP>(cf[0], tile2 + pb * (kC * DKP * 2), w, kb, lane);
+      mma_split<2>(d, low, 0, a, bf, pb);
+      if (TWO && pb <= MAXI2) mma_split<MAXI2>(d2, low2, 0, a, cf, pb);
+    }
+  }
+  add(d, low);
+  if (TWO) add(d2, low2);
+}
+
+// The warp's two column tiles of a product with a triangular kC x kC tile: d[.][i] += sum_k a[.][k] L[i][k] (TR
+// false, L lower: k blocks up to the column's) or d[.][j] += sum_i a[.][i] L[i][j] (TR true: k blocks from it).
+// a: the strip's operand in NA pieces; products up to index sum MAXI.
 template <int NA, int NB, int MAXI, bool TR>
-__device__ __forceinline__ void tri_product(float (&d)[kC / 8][4], const float (&a)[kC / 8][4], uint32_t tile, int lane) {
+__device__ __forceinline__ void tri_product(float (&d)[2][4], const uint4 (*f)[NA][32], uint32_t tile, int w, int lane) {
+  float low[2][4];
+  zero(low);
 #pragma unroll
   for (int kb = 0; kb < kC / 16; ++kb) {
-    uint32_t af[NA][4];
-    acc_to_a<NA>(a, kb, af);
+    const bool first = TR ? 2 * kb + 1 >= w : 2 * kb <= w;             // whether the tiles w and 7 - w need kb
+    const bool second = TR ? 2 * kb + 1 >= 7 - w : 2 * kb <= 7 - w;
+    if (!first && !second) continue;
+    uint32_t a[NA][4];
 #pragma unroll
-    for (int jp = 0; jp < kC / 16; ++jp) {
-      if (TR ? jp > kb : jp < kb) continue;
+    for (int i = 0; i < NA; ++i) get_frag(a[i], f[kb][i][lane]);
 #pragma unroll
-      for (int pb = 0; pb < NB; ++pb) {
-        uint32_t bf[4];
-        if (TR) load_bt<kC>(bf, tile + pb * (kTri * 2), 2 * jp, kb, lane);
-        else load_b<kC>(bf, tile + pb * (kTri * 2), 2 * jp, kb, lane);
-        mma_pieces<NA, MAXI>(d[2 * jp], d[2 * jp + 1], af, bf, pb);
+    for (int pb = 0; pb < NB && pb <= MAXI; ++pb) {
+      uint32_t bf[4];
+      if (TR) load_bt2<kC>(bf, tile + pb * (kTri * 2), w, kb, lane);
+      else load_b2<kC>(bf, tile + pb * (kTri * 2), w, kb, lane);
+#pragma unroll
+      for (int i = 0; i < NA; ++i) {
+        if (i + pb > MAXI) continue;
+        if (first) mma_bf16(i + pb ? low[0] : d[0], a[i], bf[0], bf[1]);
+        if (second) mma_bf16(i + pb ? low[1] : d[1], a[i], bf[2], bf[3]);
       }
     }
   }
+  add(d, low);
 }
 
-// S <- decay S + (a [.][c]) (tile [c][dk]) over kC positions.  The sum over the chunk is formed on its
-// own and added once, rounded to nearest: the tensor cores' accumulation truncates, and a state that
-// they accumulated over hundreds of chunks would drift.
+// The warp's quarter of S <- decay S + sign (a [.][c]) (tile [c][dk]) over kC positions.  The sum over the chunk is
+// formed on its own and added once, rounded to nearest: a state that the tensor cores accumulated over
+// hundreds of chunks, truncating each time, would drift.
 template <int NP, int DKP>
-__device__ __forceinline__ void state_add(float (&S)[DKP / 8][4], float decay, float sign, const float (&a)[kC / 8][4],
-                                          uint32_t tile, int lane) {
-  uint32_t af[kC / 16][3][4];
+__device__ __forceinline__ void state_add(float (&S)[DKP / 32][4], float decay, float sign, const uint4 (*f)[3][32],
+                                          uint32_t tile, int w, int lane) {
+  constexpr int NT = DKP / 32;
+  float d[NT][4], low[NT][4];
+  zero(d);
+  zero(low);
 #pragma unroll
-  for (int kb = 0; kb < kC / 16; ++kb) acc_to_a<3>(a, kb, af[kb]);
+  for (int kb = 0; kb < kC / 16; ++kb) {
+    uint32_t a[3][4];
 #pragma unroll
-  for (int jp = 0; jp < DKP / 16; ++jp) {
-    float d[2][4];
-    zero(d);
+    for (int i = 0; i < 3; ++i) get_frag(a[i], f[kb][i][lane]);
 #pragma unroll
-    for (int kb = 0; kb < kC / 16; ++kb)
+    for (int pb = 0; pb < NP; ++pb) {
+      uint32_t bf[NT / 2][4];
 #pragma unroll
-      for (int pb = 0; pb < NP; ++pb) {
-        uint32_t bf[4];
-        load_bt<DKP>(bf, tile + pb * (kC * DKP * 2), 2 * jp, kb, lane);
-        mma_pieces<3, 2>(d[0], d[1], af[kb], bf, pb);
-      }
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) S[2 * jp + h][e] = fmaf(decay, S[2 * jp + h][e], sign * d[h][e]);
+      for (int j = 0; j < NT / 2; ++j) load_bt<DKP>(bf[j], tile + pb * (kC * DKP * 2), w * NT + 2 * j, kb, lane);
+      mma_split<2>(d, low, 0, a, bf, pb);
+    }
   }
+#pragma unroll
+  for (int j = 0; j < NT; ++j)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) S[j][e] = fmaf(decay, S[j][e], sign * (d[j][e] + low[j][e]));
 }
 
-// ================================================================================================
-// Forward chain: a warp carries 16 value channels of one head's state through all chunks.
-// ================================================================================================
-template <typename T, int NP, int DKP, bool SAVE>
-__global__ void __launch_bounds__(256) delta_fwd(const __grid_constant__ DeltaParams p) {
-  constexpr int PP = NP == 1 ? 2 : 3;
-  using Stage = ChainStage<NP, DKP, PP>;
-  constexpr int kStages = chain_stages<NP, DKP, PP>();
-  extern __shared__ __align__(128) unsigned char smem_raw[];
-  Stage* stage = reinterpret_cast<Stage*>(smem_raw);
-  uint64_t* bar = reinterpret_cast<uint64_t*>(smem_raw + kStages * sizeof(Stage));
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, t = lane & 3;
-  const int h = blockIdx.y, b = blockIdx.z;
-  const int d0 = 16 * (blockIdx.x * (blockDim.x >> 5) + warp), cols = p.dvw - d0;
+// The per-position factors of the columns 2 t, 2 t + 1 of a column tile.
+__device__ __forceinline__ float2 at_cols(const float* v, int tile, int t) {
+  return *reinterpret_cast<const float2*>(v + 8 * tile + 2 * t);
+}
+// The warp's column tiles of a dense fp32 [channel][kC] block.
+__device__ __forceinline__ void store_cols(float* base, int w, int lane, const float (&c)[2][4]) {
+  const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    float* o = base + g * kC + 8 * col_tile(w, j) + 2 * t;
+    *reinterpret_cast<float2*>(o) = make_float2(c[j][0], c[j][1]);
+    *reinterpret_cast<float2*>(o + 8 * kC) = make_float2(c[j][2], c[j][3]);
+  }
+}
+template <typename Smem>
+__device__ __forceinline__ void init_tiles(Smem& s, int strips) {
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kStages; ++i) mbar_init(&bar[i], 1);
-    fence_mbar_init();
-    for (int i = 0; i < kStages && i < p.n; ++i) chain_load(stage[i], p, b, h, i, &bar[i]);
-  }
-  const size_t head = (size_t)b * p.Hv + h;
-  float S[DKP / 8][4];
-  state_load(p.h0 != nullptr ? p.h0 + head * p.dkw * p.dvw : nullptr, p.dkw, p.dvw, d0, lane, S);
-  __syncthreads();
-  for (int ch = 0; ch < p.n; ++ch) {
-    const int st = ch % kStages;
-    const Stage& s = stage[st];
-    const int rows = min(kC, p.L - ch * kC);
-    const long long t0 = (long long)ch * kC;
-    mbar_wait(&bar[st], (ch / kStages) & 1, p.err);
-    if (cols > 0) {
-      float V[kC / 8][4], X[kC / 8][4], O[kC / 8][4];
-      load_vt(static_cast<const T*>(p.v.ptr) + b * p.v.sb + t0 * p.v.sl + h * p.v.sh + d0, p.v.sl, rows, cols, lane, V);
-      if (SAVE) store_acc(p.states + ((head * p.n + ch) * p.dvp + d0) * DKP, DKP, lane, S);
-      // K S and Q S (transposed)
-      zero(X);
-      zero(O);
-      const uint32_t sk = smem_u32(s.k[0]), sq = smem_u32(s.q[0]);
-#pragma unroll
-      for (int kb = 0; kb < DKP / 16; ++kb) {
-        uint32_t a[3][4];
-        acc_to_a<3>(S, kb, a);
-#pragma unroll
-        for (int jp = 0; jp < kC / 16; ++jp)
-#pragma unroll
-          for (int pb = 0; pb < NP; ++pb) {
-            uint32_t bf[4];
-            load_b<DKP>(bf, sk + pb * (kC * DKP * 2), 2 * jp, kb, lane);
-            mma_pieces<3, 2>(X[2 * jp], X[2 * jp + 1], a, bf, pb);
-            load_b<DKP>(bf, sq + pb * (kC * DKP * 2), 2 * jp, kb, lane);
-            mma_pieces<3, NP == 1 ? 1 : 2>(O[2 * jp], O[2 * jp + 1], a, bf, pb);   // bf16 o: 16 bits of S
-          }
-      }
-#pragma unroll
-      for (int j = 0; j < kC / 8; ++j) {
-        const float2 eg = *reinterpret_cast<const float2*>(s.vec + 8 * j + 2 * t);
-        const float2 be = *reinterpret_cast<const float2*>(s.vec + 2 * kC + 8 * j + 2 * t);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float eg_ = e & 1 ? eg.y : eg.x;
-          X[j][e] = (e & 1 ? be.y : be.x) * fmaf(-eg_, X[j][e], V[j][e]);
-          O[j][e] *= p.scale * eg_;
-        }
-      }
-      float U[kC / 8][4];
-      zero(U);
-      tri_product<3, 3, 2, false>(U, X, smem_u32(s.t[0]), lane);
-      if (SAVE) store_acc(p.us + ((head * p.n + ch) * p.dvp + d0) * kC, kC, lane, U);
-      tri_product<PP, PP, PP - 1, false>(O, U, smem_u32(s.pm[0]), lane);
-      store_vt(static_cast<T*>(const_cast<void*>(p.o.ptr)) + b * p.o.sb + t0 * p.o.sl + h * p.o.sh + d0, p.o.sl, rows,
-               cols, lane, O);
-#pragma unroll
-      for (int j = 0; j < kC / 8; ++j) {
-        const float2 la = *reinterpret_cast<const float2*>(s.vec + kC + 8 * j + 2 * t);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) U[j][e] *= e & 1 ? la.y : la.x;
-      }
-      state_add<NP, DKP>(S, s.vec[kC - 1], 1.0f, U, sk, lane);
+    for (int i = 0; i < kTiles; ++i) {
+      mbar_init(&s.full[i], 1);
+      mbar_init(&s.empty[i], strips);
     }
-    __syncthreads();
-    if (threadIdx.x == 0 && ch + kStages < p.n) chain_load(stage[st], p, b, h, ch + kStages, &bar[st]);
+    fence_mbar_init();
   }
-  if (cols > 0 && p.last != nullptr) state_store(p.last + head * p.dkw * p.dvw, p.dkw, p.dvw, d0, lane, S);
+  __syncthreads();
+}
+
+template <typename T, int NP, int DKP, int NS>
+struct FwdChain {
+  static constexpr int PP = NP == 1 ? 2 : 3;      // pieces of P and of its U: a bf16 o keeps 16 bits
+  using StripT = StripSmem<T, DKP, PP, 0>;
+  template <int KB>
+  using Smem = ChainSmem<NP, DKP, PP, StripT, NS, KB>;
+  static constexpr int KB = sizeof(Smem<2>) <= 227 * 1024 ? 2 : 1;
+};
+template <typename T, int NP, int DKP, int NS>
+struct BwdChain {
+  using StripT = StripSmem<T, DKP, 3, NP>;
+  template <int KB>
+  using Smem = ChainSmem<NP, DKP, 3, StripT, NS, KB>;
+  static constexpr int KB = sizeof(Smem<2>) <= 227 * 1024 ? 2 : 1;
+};
+
+// ================================================================================================
+// Forward chain
+// ================================================================================================
+template <typename T, int NP, int DKP, int NS, bool SAVE>
+__global__ void __launch_bounds__(128 * NS + 32) delta_fwd(const __grid_constant__ DeltaParams p) {
+  using Form = FwdChain<T, NP, DKP, NS>;
+  constexpr int PP = Form::PP, KB = Form::KB, NT = DKP / 32;
+  using Smem = typename Form::template Smem<KB>;
+  extern __shared__ __align__(128) unsigned char smem_raw[];
+  Smem& s = *reinterpret_cast<Smem*>(smem_raw);
+  const int strip = threadIdx.x >> 7, w = (threadIdx.x >> 5) & 3, lane = threadIdx.x & 31, t = lane & 3;
+  const int h = blockIdx.y, b = blockIdx.z;
+  const int strips = min(NS, p.dvp / 16 - (int)blockIdx.x * NS);
+  init_tiles(s, strips);
+  if (strip >= NS) {
+    if (lane == 0) load_tiles<NP, DKP, KB>(s, p, b, h, [](int i) { return i; });
+    return;
+  }
+  if (strip >= strips) return;
+  const int d0 = 16 * (blockIdx.x * NS + strip), cols = p.dvw - d0;
+  auto& z = s.strip[strip];
+  const size_t head = (size_t)b * p.Hv + h;
+  float S[NT][4];
+  state_load(p.h0 != nullptr ? p.h0 + head * p.dkw * p.dvw : nullptr, p.dkw, p.dvw, 8 * NT * w, d0, lane, S);
+  const uint32_t sq = smem_u32(s.q[0]), stt = smem_u32(s.t[0]), sp = smem_u32(s.pm[0]);
+  const T* vbase = static_cast<const T*>(p.v.ptr) + b * p.v.sb + h * p.v.sh + d0;
+  T* obase = static_cast<T*>(const_cast<void*>(p.o.ptr)) + b * p.o.sb + h * p.o.sh + d0;
+  const bool vin = rows_aligned16(p.v, sizeof(T)), oout = rows_aligned16(p.o, sizeof(T));
+  const bool leader = w == 0 && lane == 0;
+  z.in.fetch(vbase, p.v.sl, min(kC, p.L), cols, vin, w, lane);
+  for (int ch = 0; ch < p.n; ++ch) {
+    const int buf = ch % KB, rows = min(kC, p.L - ch * kC);
+    const long long t0 = (long long)ch * kC;
+    const float* vec = s.vec[ch & 1];
+    const uint32_t sk = smem_u32(s.k[buf][0]);
+    put_state<DKP>(z.sf, S, w, lane);
+    if (SAVE) store_acc(p.states + ((head * p.n + ch) * p.dvp + d0) * DKP + 8 * NT * w, DKP, lane, S);
+    strip_sync(strip);                            // S is there; the last chunk is done with
+    if (leader && ch > 0) {
+      mbar_arrive(&s.empty[kTileP]);
+      mbar_arrive(&s.empty[kTileK + (ch - 1) % KB]);
+      mbar_arrive(&s.empty[kTileV + ((ch - 1) & 1)]);
+    }
+    float V[2][4], X[2][4], O[2][4], U[2][4];
+    z.in.arrive();
+    z.in.read(V, w, lane);
+    __syncwarp();
+    if (ch + 1 < p.n)
+      z.in.fetch(vbase + (t0 + kC) * p.v.sl, p.v.sl, min(kC, p.L - (ch + 1) * kC), cols, vin, w, lane);
+    zero(X);
+    zero(O);
+    zero(U);
+    mbar_wait(&s.full[kTileK + buf], (ch / KB) & 1, p.err);
+    mbar_wait(&s.full[kTileV + (ch & 1)], (ch >> 1) & 1, p.err);
+    mbar_wait(&s.full[kTileQ], ch & 1, p.err);
+    state_product<NP, DKP, true, PP - 1>(X, O, z.sf, sk, sq, w, lane);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const float2 eg = at_cols(vec, col_tile(w, j), t), be = at_cols(vec + 2 * kC, col_tile(w, j), t);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float eg_ = e & 1 ? eg.y : eg.x;
+        X[j][e] = (e & 1 ? be.y : be.x) * fmaf(-eg_, X[j][e], V[j][e]);
+        O[j][e] *= p.scale * eg_;
+      }
+      put_half<3>(z.xf, col_tile(w, j), X[j], lane);
+    }
+    strip_sync(strip);                            // X is there; Q is done with
+    if (leader) mbar_arrive(&s.empty[kTileQ]);
+    mbar_wait(&s.full[kTileT], ch & 1, p.err);
+    tri_product<3, 3, 2, false>(U, z.xf, stt, w, lane);
+    if (SAVE) store_cols(p.us + ((head * p.n + ch) * p.dvp + d0) * kC, w, lane, U);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      put_half<PP>(z.uf, col_tile(w, j), U[j], lane);
+      const float2 la = at_cols(vec + kC, col_tile(w, j), t);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) U[j][e] *= e & 1 ? la.y : la.x;
+      put_half<3>(z.lf, col_tile(w, j), U[j], lane);
+    }
+    strip_sync(strip);                            // U is there; T is done with
+    if (leader) mbar_arrive(&s.empty[kTileT]);
+    state_add<NP, DKP>(S, vec[kC - 1], 1.0f, z.lf, sk, w, lane);
+    mbar_wait(&s.full[kTileP], ch & 1, p.err);
+    tri_product<PP, PP, PP - 1, false>(O, z.uf, sp, w, lane);
+    z.out.write(O, w, lane);
+    z.out.flush(obase + t0 * p.o.sl, p.o.sl, rows, cols, oout, w, lane);
+  }
+  if (p.last != nullptr) state_store(p.last + head * p.dkw * p.dvw, p.dkw, p.dvw, 8 * NT * w, d0, lane, S);
 }
 
 // ================================================================================================
@@ -450,85 +627,105 @@ __global__ void __launch_bounds__(256) delta_fwd(const __grid_constant__ DeltaPa
 //   Y = e^(G_last - G) K dS' + P^T dO,  dX = T^T Y,  dV = beta dX
 //   dS = e^G_last dS' + (scale e^G Q)^T dO - (beta e^G K)^T dX
 // ================================================================================================
-template <typename T, int NP, int DKP>
-__global__ void __launch_bounds__(256) delta_bwd_chain(const __grid_constant__ DeltaParams p) {
-  using Stage = ChainStage<NP, DKP, 3>;
-  constexpr int kStages = chain_stages<NP, DKP, 3>();
+template <typename T, int NP, int DKP, int NS>
+__global__ void __launch_bounds__(128 * NS + 32) delta_bwd_chain(const __grid_constant__ DeltaParams p) {
+  using Form = BwdChain<T, NP, DKP, NS>;
+  constexpr int KB = Form::KB, NT = DKP / 32;
+  using Smem = typename Form::template Smem<KB>;
   extern __shared__ __align__(128) unsigned char smem_raw[];
-  Stage* stage = reinterpret_cast<Stage*>(smem_raw);
-  uint64_t* bar = reinterpret_cast<uint64_t*>(smem_raw + kStages * sizeof(Stage));
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, t = lane & 3;
+  Smem& s = *reinterpret_cast<Smem*>(smem_raw);
+  const int strip = threadIdx.x >> 7, w = (threadIdx.x >> 5) & 3, lane = threadIdx.x & 31, t = lane & 3;
   const int h = blockIdx.y, b = blockIdx.z;
-  const int d0 = 16 * (blockIdx.x * (blockDim.x >> 5) + warp), cols = p.dvw - d0;
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < kStages; ++i) mbar_init(&bar[i], 1);
-    fence_mbar_init();
-    for (int i = 0; i < kStages && i < p.n; ++i) chain_load(stage[i], p, b, h, p.n - 1 - i, &bar[i]);
+  const int strips = min(NS, p.dvp / 16 - (int)blockIdx.x * NS);
+  init_tiles(s, strips);
+  if (strip >= NS) {
+    const int last = p.n - 1;
+    if (lane == 0) load_tiles<NP, DKP, KB>(s, p, b, h, [last](int i) { return last - i; });
+    return;
   }
+  if (strip >= strips) return;
+  const int d0 = 16 * (blockIdx.x * NS + strip), cols = p.dvw - d0;
+  auto& z = s.strip[strip];
   const size_t head = (size_t)b * p.Hv + h;
-  float S[DKP / 8][4];
-  state_load(p.h0 != nullptr ? p.h0 + head * p.dkw * p.dvw : nullptr, p.dkw, p.dvw, d0, lane, S);
-  __syncthreads();
+  float S[NT][4];
+  state_load(p.h0 != nullptr ? p.h0 + head * p.dkw * p.dvw : nullptr, p.dkw, p.dvw, 8 * NT * w, d0, lane, S);
+  const uint32_t sq = smem_u32(s.q[0]), stt = smem_u32(s.t[0]), sp = smem_u32(s.pm[0]);
+  const T* gbase = static_cast<const T*>(p.o.ptr) + b * p.o.sb + h * p.o.sh + d0;
+  T* obase = static_cast<T*>(const_cast<void*>(p.dv.ptr)) + b * p.dv.sb + h * p.dv.sh + d0;
+  const bool gin = rows_aligned16(p.o, sizeof(T)), oout = rows_aligned16(p.dv, sizeof(T));
+  const bool leader = w == 0 && lane == 0;
+  z.in.fetch(gbase + (long long)(p.n - 1) * kC * p.o.sl, p.o.sl, p.L - (p.n - 1) * kC, cols, gin, w, lane);
   for (int it = 0; it < p.n; ++it) {
-    const int ch = p.n - 1 - it, st = it % kStages;
-    const Stage& s = stage[st];
-    const int rows = min(kC, p.L - ch * kC);
+    const int ch = p.n - 1 - it, buf = it % KB, rows = min(kC, p.L - ch * kC);
     const long long t0 = (long long)ch * kC;
-    mbar_wait(&bar[st], (it / kStages) & 1, p.err);
-    if (cols > 0) {
-      float dO[kC / 8][4], Y[kC / 8][4];
-      load_vt(static_cast<const T*>(p.o.ptr) + b * p.o.sb + t0 * p.o.sl + h * p.o.sh + d0, p.o.sl, rows, cols, lane, dO);
-      store_acc(p.dstates + ((head * p.n + ch) * p.dvp + d0) * DKP, DKP, lane, S);
-      zero(Y);
-      const uint32_t sk = smem_u32(s.k[0]), sq = smem_u32(s.q[0]);
+    const float* vec = s.vec[it & 1];
+    const uint32_t sk = smem_u32(s.k[buf][0]);
+    put_state<DKP>(z.sf, S, w, lane);
+    store_acc(p.dstates + ((head * p.n + ch) * p.dvp + d0) * DKP + 8 * NT * w, DKP, lane, S);
+    float dO[2][4], Y[2][4], X[2][4];
+    z.in.arrive();
+    z.in.read(dO, w, lane);
+    __syncwarp();
+    if (ch > 0) z.in.fetch(gbase + (t0 - kC) * p.o.sl, p.o.sl, kC, cols, gin, w, lane);
+    mbar_wait(&s.full[kTileV + (it & 1)], (it >> 1) & 1, p.err);
 #pragma unroll
-      for (int kb = 0; kb < DKP / 16; ++kb) {
-        uint32_t a[3][4];
-        acc_to_a<3>(S, kb, a);
+    for (int j = 0; j < 2; ++j) {
+      put_half<NP>(z.of, col_tile(w, j), dO[j], lane);
+      const float2 eg = at_cols(vec, col_tile(w, j), t);
 #pragma unroll
-        for (int jp = 0; jp < kC / 16; ++jp)
-#pragma unroll
-          for (int pb = 0; pb < NP; ++pb) {
-            uint32_t bf[4];
-            load_b<DKP>(bf, sk + pb * (kC * DKP * 2), 2 * jp, kb, lane);
-            mma_pieces<3, 2>(Y[2 * jp], Y[2 * jp + 1], a, bf, pb);
-          }
-      }
-#pragma unroll
-      for (int j = 0; j < kC / 8; ++j) {
-        const float2 la = *reinterpret_cast<const float2*>(s.vec + kC + 8 * j + 2 * t);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) Y[j][e] *= e & 1 ? la.y : la.x;
-      }
-      tri_product<NP, 3, 2, true>(Y, dO, smem_u32(s.pm[0]), lane);
-      float X[kC / 8][4];
-      zero(X);
-      tri_product<3, 3, 2, true>(X, Y, smem_u32(s.t[0]), lane);
-      store_acc(p.dxs + ((head * p.n + ch) * p.dvp + d0) * kC, kC, lane, X);
-#pragma unroll
-      for (int j = 0; j < kC / 8; ++j) {
-        const float2 eg = *reinterpret_cast<const float2*>(s.vec + 8 * j + 2 * t);
-        const float2 be = *reinterpret_cast<const float2*>(s.vec + 2 * kC + 8 * j + 2 * t);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          Y[j][e] = X[j][e] * (e & 1 ? be.y : be.x);
-          dO[j][e] *= p.scale * (e & 1 ? eg.y : eg.x);
-          X[j][e] = Y[j][e] * (e & 1 ? eg.y : eg.x);
-        }
-      }
-      store_vt(static_cast<T*>(const_cast<void*>(p.dv.ptr)) + b * p.dv.sb + t0 * p.dv.sl + h * p.dv.sh + d0, p.dv.sl,
-               rows, cols, lane, Y);
-      state_add<NP, DKP>(S, s.vec[kC - 1], 1.0f, dO, sq, lane);
-      state_add<NP, DKP>(S, 1.0f, -1.0f, X, sk, lane);
+      for (int e = 0; e < 4; ++e) dO[j][e] *= p.scale * (e & 1 ? eg.y : eg.x);
+      put_half<3>(z.uf, col_tile(w, j), dO[j], lane);
     }
-    __syncthreads();
-    if (threadIdx.x == 0 && it + kStages < p.n) chain_load(stage[st], p, b, h, p.n - 1 - it - kStages, &bar[st]);
+    zero(X);
+    zero(Y);
+    strip_sync(strip);                            // dS' and dO are there; the last chunk is done with
+    if (leader && it > 0) {
+      mbar_arrive(&s.empty[kTileK + (it - 1) % KB]);
+      mbar_arrive(&s.empty[kTileV + ((it - 1) & 1)]);
+    }
+    mbar_wait(&s.full[kTileK + buf], (it / KB) & 1, p.err);
+    state_product<NP, DKP, false, 0>(Y, Y, z.sf, sk, sk, w, lane);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const float2 la = at_cols(vec + kC, col_tile(w, j), t);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) Y[j][e] *= e & 1 ? la.y : la.x;
+    }
+    mbar_wait(&s.full[kTileP], it & 1, p.err);
+    tri_product<NP, 3, 2, true>(Y, z.of, sp, w, lane);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) put_half<3>(z.xf, col_tile(w, j), Y[j], lane);
+    mbar_wait(&s.full[kTileQ], it & 1, p.err);
+    state_add<NP, DKP>(S, vec[kC - 1], 1.0f, z.uf, sq, w, lane);
+    strip_sync(strip);                            // Y is there; P and Q are done with
+    if (leader) {
+      mbar_arrive(&s.empty[kTileQ]);
+      mbar_arrive(&s.empty[kTileP]);
+    }
+    mbar_wait(&s.full[kTileT], it & 1, p.err);
+    tri_product<3, 3, 2, true>(X, z.xf, stt, w, lane);
+    store_cols(p.dxs + ((head * p.n + ch) * p.dvp + d0) * kC, w, lane, X);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const float2 eg = at_cols(vec, col_tile(w, j), t), be = at_cols(vec + 2 * kC, col_tile(w, j), t);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        Y[j][e] = X[j][e] * (e & 1 ? be.y : be.x);
+        X[j][e] = Y[j][e] * (e & 1 ? eg.y : eg.x);
+      }
+      put_half<3>(z.lf, col_tile(w, j), X[j], lane);
+    }
+    strip_sync(strip);                            // dX is there; T is done with
+    if (leader) mbar_arrive(&s.empty[kTileT]);
+    state_add<NP, DKP>(S, 1.0f, -1.0f, z.lf, sk, w, lane);
+    z.out.write(Y, w, lane);
+    z.out.flush(obase + t0 * p.dv.sl, p.dv.sl, rows, cols, oout, w, lane);
   }
-  if (cols > 0 && p.last != nullptr) state_store(p.last + head * p.dkw * p.dvw, p.dkw, p.dvw, d0, lane, S);
+  if (p.last != nullptr) state_store(p.last + head * p.dkw * p.dvw, p.dkw, p.dvw, 8 * NT * w, d0, lane, S);
 }
 
 // ================================================================================================
-// Backward, all chunks at once: one CTA of eight warps per (chunk, value head, batch).  With
+// Backward, all chunks at once: one CTA of sixteen warps per (chunk, value head, batch).  With
 //   E1 = dO S^T,  E2 = dX S^T,  E3 = U dS'^T,  N = -tril(D dX U^T, -1),  M = scale tril(D dO U^T, -1),
 //   m_i = scale dO_i.U_i (the diagonal, where D = 1 has no gradient)
 //   H = N K - e^G E2                         (the gradient of beta k)
@@ -539,222 +736,283 @@ __global__ void __launch_bounds__(256) delta_bwd_chain(const __grid_constant__ D
 // after which dQ_i gets m_i k_i and dK_i gets m_i q_i;
 // dg is dG summed from the end of the chunk.  Every exponent's gradient is thus a row product of
 // gradients that are formed anyway; k.k and q.k are not needed again.
-// A warp takes 16 rows and half of the columns; dv is walked 32 channels at a time.
+// A warp takes 16 rows and a quarter of the columns.  dv is walked SL channels at a time: a bulk copy brings a slab of S,
+// dS', U and dX (fp32) while the last one is multiplied; all threads then split it into bf16 pieces once, in the
+// tiles that ldmatrix reads.
 // ================================================================================================
-constexpr int kSlab = 32;
-template <int NP, int DKP>
+template <int NP, int DKP, int SL>
+struct BwdSlab {
+  float S[SL * DKP], dS[SL * DKP], U[SL * kC], dX[SL * kC];                     // as they lie in global memory
+  __nv_bfloat16 pS[3][SL * DKP], pdS[3][SL * DKP], pU[3][SL * kC], pdX[3][SL * kC], pdO[NP][kC * SL];
+};
+struct BwdTri {
+  __nv_bfloat16 M[3][kTri], N[3][kTri], Nb[3][kTri];     // Nb: rows times beta
+};
+template <int NP, int DKP, int SL>
 struct alignas(128) BwdSmem {
+  union {
+    BwdSlab<NP, DKP, SL> slab;
+    BwdTri tri;                 // after the last slab
+  };
   __nv_bfloat16 k[NP][kC * DKP], q[NP][kC * DKP];
   float vec[kVec];
-  float S[kSlab][DKP + 4], dS[kSlab][DKP + 4];
-  float U[kSlab][kC + 4], dX[kSlab][kC + 4];
-  float dO[kC][kSlab + 8];
-  float N[kC][kC + 8], M[kC][kC + 8];
-  float dots[4][2][kC];         // q.dQ, k.H, k.C, e^(G_last - G) k.E3; by column half
-  float dxv[4][kC];             // dX.V by quarter of the slab
-  float sds[8];                 // <S, dS'> by warp
+  float dots[4][4][kC];         // q.dQ, k.H, k.C, e^(G_last - G) k.E3; by column quarter
+  float dxv[kC];                // dX.V
+  float sds[16];                 // <S, dS'> by warp
   float m[kC];                  // the diagonal of M
-  uint64_t bar;
+  uint64_t bar_kq, bar_slab;
 };
 
-// A operand (16 rows from row0, k block kb) in NA pieces from a float tile stored [m][k], rows `scale`d.
-template <int NA, int W>
-__device__ __forceinline__ void a_rows(const float (*m)[W], int row0, int k0, int lane, uint32_t (&a)[NA][4]) {
-  const int g = lane >> 2, t = lane & 3;
-#pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    const float2 x = *reinterpret_cast<const float2*>(&m[row0 + g + 8 * (r & 1)][k0 + 2 * t + 8 * (r >> 1)]);
-    uint32_t p[NA];
-    split<NA>(x.x, x.y, p);
-#pragma unroll
-    for (int i = 0; i < NA; ++i) a[i][r] = p[i];
-  }
-}
-// The same from a tile stored [k][m]; w (or null) scales position k.
-template <int NA, int W>
-__device__ __forceinline__ void a_cols(const float (*m)[W], int row0, int k0, int lane, const float* w,
-                                       uint32_t (&a)[NA][4]) {
-  const int g = lane >> 2, t = lane & 3;
-#pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    const int k = k0 + 2 * t + 8 * (r >> 1), i = row0 + g + 8 * (r & 1);
-    float x0 = m[k][i], x1 = m[k + 1][i];
-    if (w != nullptr) {
-      x0 *= w[k];
-      x1 *= w[k + 1];
-    }
-    uint32_t p[NA];
-    split<NA>(x0, x1, p);
-#pragma unroll
-    for (int i2 = 0; i2 < NA; ++i2) a[i2][r] = p[i2];
-  }
-}
-// B operand (k block from k0, n tile from n0) in three pieces from a float tile stored [k][n].
-template <int W>
-__device__ __forceinline__ void b_cols(const float (*m)[W], int k0, int n0, int lane, uint32_t (&b)[3][2]) {
-  const int g = lane >> 2, t = lane & 3;
-#pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    uint32_t p[3];
-    split<3>(m[k0 + 2 * t + 8 * r][n0 + g], m[k0 + 2 * t + 1 + 8 * r][n0 + g], p);
-#pragma unroll
-    for (int i = 0; i < 3; ++i) b[i][r] = p[i];
-  }
-}
-template <int NA>
-__device__ __forceinline__ void mma_all(float (&d)[4], const uint32_t (&a)[NA][4], const uint32_t (&b)[3][2]) {
-#pragma unroll
-  for (int i = 0; i < NA; ++i)
-#pragma unroll
-    for (int j = 0; j < 3; ++j)
-      if (i + j <= 2) mma_bf16(d, a[i], b[j][0], b[j][1]);
-}
-// d (tiles of 8 columns from col0) += a (kC positions, given by fragment loader) x tile [c][dk] in NP pieces
+// d += the products of A (given by frag(kb, piece, a)) over k blocks [kb0, kb1) with a [c][dk] tile of NP pieces, in the
+// warp's NT column tiles from col_tile0.
 template <int NP, int DKP, int NT, typename F>
-__device__ __forceinline__ void add_rows_times_tile(float (&d)[NT][4], uint32_t tile, int col_tile0, int kb0, int kb1,
-                                                    int lane, F frag) {
+__device__ __forceinline__ void add_tile_product(float (&d)[NT][4], uint32_t tile, int col_tile0, int kb0, int kb1,
+                                                 int lane, F frag) {
+  float lead[NT][4], low[NT][4];
+  zero(lead);
+  zero(low);
   for (int kb = kb0; kb < kb1; ++kb) {
     uint32_t a[3][4];
-    frag(kb, a);
 #pragma unroll
-    for (int jp = 0; jp < NT / 2; ++jp)
+    for (int i = 0; i < 3; ++i) frag(kb, i, a[i]);
 #pragma unroll
-      for (int pb = 0; pb < NP; ++pb) {
-        uint32_t bf[4];
-        load_bt<DKP>(bf, tile + pb * (kC * DKP * 2), col_tile0 + 2 * jp, kb, lane);
-        mma_pieces<3, 2>(d[2 * jp], d[2 * jp + 1], a, bf, pb);
-      }
+    for (int pb = 0; pb < NP; ++pb) {
+      uint32_t bf[NT / 2][4];
+#pragma unroll
+      for (int jp = 0; jp < NT / 2; ++jp) load_bt<DKP>(bf[jp], tile + pb * (kC * DKP * 2), col_tile0 + 2 * jp, kb, lane);
+      mma_split<2>(lead, low, 0, a, bf, pb);
+    }
   }
+  add(lead, low);
+  add(d, lead);
 }
 
-template <typename T, int NP, int DKP>
-__global__ void __launch_bounds__(256) delta_bwd_chunk(const __grid_constant__ DeltaParams p) {
+template <typename T, int NP, int DKP, int SL>
+__global__ void __launch_bounds__(512) delta_bwd_chunk(const __grid_constant__ DeltaParams p) {
   extern __shared__ __align__(128) unsigned char smem_raw[];
-  auto& s = *reinterpret_cast<BwdSmem<NP, DKP>*>(smem_raw);
-  constexpr int NT = DKP / 16;                    // n tiles of a warp's half of dk
+  auto& s = *reinterpret_cast<BwdSmem<NP, DKP, SL>*>(smem_raw);
+  constexpr int NT = DKP / 32, KS = SL / 16;      // n tiles of a warp's quarter of dk; k blocks of a slab
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  const int row0 = 16 * (warp & 3), half = warp >> 2;
+  const int w4 = warp & 3, row0 = 16 * w4, quarter = warp >> 2;
   const int ch = blockIdx.x, h = blockIdx.y, b = blockIdx.z, hk = h / p.group;
   const int rows = min(kC, p.L - ch * kC);
   const long long t0 = (long long)ch * kC;
   const size_t at = ((size_t)b * p.Hv + h) * p.n + ch;
   const size_t atk = ((size_t)b * p.Hk + hk) * p.n + ch;
+  auto fetch_slab = [&](int v0) {
+    const uint32_t vn = min(SL, p.dvp - v0);
+    mbar_arrive_expect_tx(&s.bar_slab, vn * (2 * DKP + 2 * kC) * 4);
+    bulk_load(s.slab.S, p.states + (at * p.dvp + v0) * DKP, vn * DKP * 4, &s.bar_slab);
+    bulk_load(s.slab.dS, p.dstates + (at * p.dvp + v0) * DKP, vn * DKP * 4, &s.bar_slab);
+    bulk_load(s.slab.U, p.us + (at * p.dvp + v0) * kC, vn * kC * 4, &s.bar_slab);
+    bulk_load(s.slab.dX, p.dxs + (at * p.dvp + v0) * kC, vn * kC * 4, &s.bar_slab);
+  };
   if (tid == 0) {
-    mbar_init(&s.bar, 1);
+    mbar_init(&s.bar_kq, 1);
+    mbar_init(&s.bar_slab, 1);
     fence_mbar_init();
-    mbar_arrive_expect_tx(&s.bar, sizeof(s.k) + sizeof(s.q) + sizeof(s.vec));
-    bulk_load(s.k, p.kimg + atk * (NP * kC * DKP), sizeof(s.k), &s.bar);
-    bulk_load(s.q, p.qimg + atk * (NP * kC * DKP), sizeof(s.q), &s.bar);
-    bulk_load(s.vec, p.vec + at * kVec, sizeof(s.vec), &s.bar);
+    fetch_slab(0);
+    mbar_arrive_expect_tx(&s.bar_kq, sizeof(s.k) + sizeof(s.q) + sizeof(s.vec));
+    bulk_load(s.k, p.kimg + atk * (NP * kC * DKP), sizeof(s.k), &s.bar_kq);
+    bulk_load(s.q, p.qimg + atk * (NP * kC * DKP), sizeof(s.q), &s.bar_kq);
+    bulk_load(s.vec, p.vec + at * kVec, sizeof(s.vec), &s.bar_kq);
   }
-  float E1[NT][4], E2[NT][4], E3[NT][4], XU[4][4], OU[4][4];
+  // dO and V of a slab: 8 channels of one position per thread and step
+  constexpr int kRowGroups = SL / 8;
+  const T* dOb = static_cast<const T*>(p.o.ptr) + b * p.o.sb + t0 * p.o.sl + h * p.o.sh;
+  const T* Vb = static_cast<const T*>(p.v.ptr) + b * p.v.sb + t0 * p.v.sl + h * p.v.sh;
+  const bool ovec = rows_aligned16(p.o, sizeof(T)), vvec = rows_aligned16(p.v, sizeof(T));
+  const bool loads = tid < kC * kRowGroups;
+  const int lc = tid / kRowGroups, lg = tid % kRowGroups;
+  static_assert(kC * kRowGroups <= 512, "a slab's dO is one step");
+  float xo[8], xv[8];
+  auto load_rows = [&](int v0) {
+    if (!loads) return;
+    const int width = lc < rows ? p.dvw : 0;
+    load8<T>(dOb + lc * p.o.sl, v0 + 8 * lg, width, ovec, xo);
+    load8<T>(Vb + lc * p.v.sl, v0 + 8 * lg, width, vvec, xv);
+  };
+  load_rows(0);
+  float E1[NT][4], E2[NT][4], E3[NT][4], XU[2][4], OU[2][4];
   zero(E1);
   zero(E2);
   zero(E3);
   zero(XU);
   zero(OU);
   float dot = 0.0f, dxv = 0.0f;
-  const T* dOb = static_cast<const T*>(p.o.ptr) + b * p.o.sb + t0 * p.o.sl + h * p.o.sh;
-  const T* Vb = static_cast<const T*>(p.v.ptr) + b * p.v.sb + t0 * p.v.sl + h * p.v.sh;
-  for (int v0 = 0; v0 < p.dvp; v0 += kSlab) {
-    const int vn = min(kSlab, p.dvp - v0);
-    __syncthreads();
-    for (int e = tid; e < kSlab * DKP / 4; e += 256) {
-      const int r = e / (DKP / 4), c = 4 * (e % (DKP / 4));
-      float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
+  __syncthreads();
+  for (int v0 = 0, it = 0; v0 < p.dvp; v0 += SL, ++it) {
+    const int vn = min(SL, p.dvp - v0);
+    mbar_wait(&s.bar_slab, it & 1, p.err);
+    // split the slab
+    for (int e = tid; e < SL * DKP / 8; e += 512) {
+      const int r = e / (DKP / 8), grp = e % (DKP / 8), off = tile_off<DKP>(r, grp);
+      float x[8], y[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = y[i] = 0.0f;
       if (r < vn) {
-        x = *reinterpret_cast<const float4*>(p.states + (at * p.dvp + v0 + r) * DKP + c);
-        y = *reinterpret_cast<const float4*>(p.dstates + (at * p.dvp + v0 + r) * DKP + c);
+        load8<float>(s.slab.S + r * DKP, 8 * grp, DKP, true, x);
+        load8<float>(s.slab.dS + r * DKP, 8 * grp, DKP, true, y);
       }
-      *reinterpret_cast<float4*>(&s.S[r][c]) = x;
-      *reinterpret_cast<float4*>(&s.dS[r][c]) = y;
-      dot = fmaf(x.x, y.x, fmaf(x.y, y.y, fmaf(x.z, y.z, fmaf(x.w, y.w, dot))));
+#pragma unroll
+      for (int i = 0; i < 8; ++i) dot = fmaf(x[i], y[i], dot);
+      put_pieces<3>(x, s.slab.pS[0], nullptr, off, SL * DKP);
+      put_pieces<3>(y, s.slab.pdS[0], nullptr, off, SL * DKP);
     }
-    for (int e = tid; e < kSlab * kC / 4; e += 256) {
-      const int r = e / (kC / 4), c = 4 * (e % (kC / 4));
-      float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
+    for (int e = tid; e < SL * kC / 8; e += 512) {
+      const int r = e / (kC / 8), grp = e % (kC / 8), off = tile_off<kC>(r, grp);
+      float x[8], y[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = y[i] = 0.0f;
       if (r < vn) {
-        x = *reinterpret_cast<const float4*>(p.us + (at * p.dvp + v0 + r) * kC + c);
-        y = *reinterpret_cast<const float4*>(p.dxs + (at * p.dvp + v0 + r) * kC + c);
+        load8<float>(s.slab.U + r * kC, 8 * grp, kC, true, x);
+        load8<float>(s.slab.dX + r * kC, 8 * grp, kC, true, y);
       }
-      *reinterpret_cast<float4*>(&s.U[r][c]) = x;
-      *reinterpret_cast<float4*>(&s.dX[r][c]) = y;
+      put_pieces<3>(x, s.slab.pU[0], nullptr, off, SL * kC);
+      put_pieces<3>(y, s.slab.pdX[0], nullptr, off, SL * kC);
     }
-    for (int e = tid; e < kC * kSlab; e += 256) {
-      const int c = e / kSlab, d = e % kSlab;
-      s.dO[c][d] = c < rows && v0 + d < p.dvw ? to_f32(dOb[c * p.o.sl + v0 + d]) : 0.0f;
+    if (loads) {
+      put_pieces<NP>(xo, s.slab.pdO[0], nullptr, tile_off<SL>(lc, lg), kC * SL);
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (8 * lg + i < vn) dxv = fmaf(s.slab.dX[(8 * lg + i) * kC + lc], xv[i], dxv);
     }
     __syncthreads();
-    {
-      const int c = tid & 63, d1 = (tid >> 6) * 8;
-      if (c < rows)
+    if (v0 + SL < p.dvp) {
+      if (tid == 0) fetch_slab(v0 + SL);
+      load_rows(v0 + SL);
+    }
+    // multiply.  The slab's small products, then its leading ones, in fresh accumulators that are added to the
+    // totals once, rounded to nearest.
+    uint32_t ao[KS][NP][4], ax[KS][3][4], au[KS][3][4];
+    const uint32_t tO = smem_u32(s.slab.pdO[0]), tX = smem_u32(s.slab.pdX[0]), tU = smem_u32(s.slab.pU[0]);
+    const uint32_t tS = smem_u32(s.slab.pS[0]), tdS = smem_u32(s.slab.pdS[0]);
 #pragma unroll
-        for (int d = d1; d < d1 + 8; ++d)
-          if (v0 + d < p.dvw) dxv = fmaf(s.dX[d][c], to_f32(Vb[c * p.v.sl + v0 + d]), dxv);
+    for (int k = 0; k < KS; ++k) {
+#pragma unroll
+      for (int i = 0; i < NP; ++i) load_a<SL>(ao[k][i], tO + i * (kC * SL * 2), row0, k, lane);
+#pragma unroll
+      for (int i = 0; i < 3; ++i) {
+        load_at<kC>(ax[k][i], tX + i * (SL * kC * 2), row0, k, lane);
+        load_at<kC>(au[k][i], tU + i * (SL * kC * 2), row0, k, lane);
+      }
     }
 #pragma unroll
-    for (int k0 = 0; k0 < kSlab; k0 += 16) {
-      uint32_t ao[NP][4], ax[3][4], au[3][4];
-      a_rows<NP>(s.dO, row0, k0, lane, ao);
-      a_cols<3>(s.dX, row0, k0, lane, nullptr, ax);
-      a_cols<3>(s.U, row0, k0, lane, nullptr, au);
+    for (int jp = 0; jp < NT / 2; ++jp) {
+      float d1[2][4], d2[2][4], d3[2][4];
+      zero(d1);
+      zero(d2);
+      zero(d3);
+      uint32_t bs[KS][1][4], bd[KS][1][4];
 #pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        uint32_t bf[3][2];
-        b_cols(s.S, k0, half * (DKP / 2) + 8 * j, lane, bf);
-        mma_all<NP>(E1[j], ao, bf);
-        mma_all<3>(E2[j], ax, bf);
-        b_cols(s.dS, k0, half * (DKP / 2) + 8 * j, lane, bf);
-        mma_all<3>(E3[j], au, bf);
-      }
-      if (row0 + 15 >= 32 * half) {
+      for (int pb = 2; pb >= 0; --pb)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          uint32_t bf[3][2];
-          b_cols(s.U, k0, 32 * half + 8 * j, lane, bf);
-          mma_all<3>(XU[j], ax, bf);
-          mma_all<NP>(OU[j], ao, bf);
+        for (int k = 0; k < KS; ++k) {
+          load_bt<DKP>(bs[k][0], tS + pb * (SL * DKP * 2), quarter * NT + 2 * jp, k, lane);
+          load_bt<DKP>(bd[k][0], tdS + pb * (SL * DKP * 2), quarter * NT + 2 * jp, k, lane);
+          mma_pieces<1, 2>(d1, 0, ao[k], bs[k], pb);
+          mma_pieces<1, 2>(d2, 0, ax[k], bs[k], pb);
+          mma_pieces<1, 2>(d3, 0, au[k], bd[k], pb);
         }
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        mma_pieces<0, 0>(d1, 0, ao[k], bs[k], 0);
+        mma_pieces<0, 0>(d2, 0, ax[k], bs[k], 0);
+        mma_pieces<0, 0>(d3, 0, au[k], bd[k], 0);
       }
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          E1[2 * jp + j][e] += d1[j][e];
+          E2[2 * jp + j][e] += d2[j][e];
+          E3[2 * jp + j][e] += d3[j][e];
+        }
     }
+    if (quarter <= w4) {
+      float d1[2][4], d2[2][4];
+      zero(d1);
+      zero(d2);
+      uint32_t bu[KS][1][4];
+#pragma unroll
+      for (int pb = 2; pb >= 0; --pb)
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+          load_bt<kC>(bu[k][0], tU + pb * (SL * kC * 2), 2 * quarter, k, lane);
+          mma_pieces<1, 2>(d1, 0, ao[k], bu[k], pb);
+          mma_pieces<1, 2>(d2, 0, ax[k], bu[k], pb);
+        }
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        mma_pieces<0, 0>(d1, 0, ao[k], bu[k], 0);
+        mma_pieces<0, 0>(d2, 0, ax[k], bu[k], 0);
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          OU[j][e] += d1[j][e];
+          XU[j][e] += d2[j][e];
+        }
+    }
+    __syncthreads();
   }
-  mbar_wait(&s.bar, 0, p.err);
-  // N and M
+  mbar_wait(&s.bar_kq, 0, p.err);
+  const float* beta = s.vec + 2 * kC;
+  // N, beta N and M in pieces, where the slab was
 #pragma unroll
-  for (int j = 0; j < 4; ++j)
+  for (int j = 0; j < 2; ++j)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int i = row0 + g + 8 * (e >> 1), c = 32 * half + 8 * j + 2 * t + (e & 1);
-      const float d = i >= c ? ex2((s.vec[3 * kC + i] - s.vec[3 * kC + c]) + (s.vec[4 * kC + i] - s.vec[4 * kC + c])) : 0.0f;
-      s.N[i][c] = i > c ? -d * XU[j][e] : 0.0f;
-      s.M[i][c] = i > c ? p.scale * d * OU[j][e] : 0.0f;
-      if (i == c) s.m[i] = p.scale * OU[j][e];
+    for (int r = 0; r < 2; ++r) {
+      const int i = row0 + g + 8 * r, c = 16 * quarter + 8 * j + 2 * t;
+      float n[2], m[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float d =
+            i > c + e ? ex2((s.vec[3 * kC + i] - s.vec[3 * kC + c + e]) + (s.vec[4 * kC + i] - s.vec[4 * kC + c + e])) : 0.0f;
+        n[e] = i > c + e ? -d * XU[j][2 * r + e] : 0.0f;
+        m[e] = i > c + e ? p.scale * d * OU[j][2 * r + e] : 0.0f;
+        if (i == c + e) s.m[i] = p.scale * OU[j][2 * r + e];
+      }
+      const int off = tile_off<kC>(i, c >> 3) + 2 * t;
+      uint32_t x[3];
+      auto put = [&](__nv_bfloat16 (&tile)[3][kTri], float v0, float v1) {
+        split<3>(v0, v1, x);
+#pragma unroll
+        for (int q = 0; q < 3; ++q) *reinterpret_cast<uint32_t*>(&tile[q][off]) = x[q];
+      };
+      put(s.tri.N, n[0], n[1]);
+      put(s.tri.Nb, beta[i] * n[0], beta[i] * n[1]);
+      put(s.tri.M, m[0], m[1]);
     }
-  s.dxv[tid >> 6][tid & 63] = dxv;
+  // dX.V over the threads of a position (kRowGroups neighbours)
+#pragma unroll
+  for (int m = 1; m < kRowGroups; m <<= 1) dxv += __shfl_xor_sync(0xffffffffu, dxv, m);
+  if (loads && lg == 0) s.dxv[lc] = dxv;
   dot = group_allreduce<32, 1>(dot);
   if (lane == 0) s.sds[warp] = dot;
   __syncthreads();
   const uint32_t sk = smem_u32(s.k[0]), sq = smem_u32(s.q[0]);
-  const int ct = half * NT;
-  const float* beta = s.vec + 2 * kC;
-  float eg[2], la[2], be[2];
+  const uint32_t tM = smem_u32(s.tri.M[0]), tN = smem_u32(s.tri.N[0]), tNb = smem_u32(s.tri.Nb[0]);
+  const int ct = quarter * NT;
+  float be[2];
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
-    eg[r] = s.vec[row0 + g + 8 * r];
-    la[r] = s.vec[kC + row0 + g + 8 * r];
-    be[r] = beta[row0 + g + 8 * r];
+    const int i = row0 + g + 8 * r;
+    const float eg = s.vec[i], la = s.vec[kC + i];
+    be[r] = beta[i];
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int e = 2 * r; e < 2 * r + 2; ++e) {
+        E1[j][e] *= p.scale * eg;
+        E2[j][e] *= -eg;
+        E3[j][e] *= la;
+      }
   }
-#pragma unroll
-  for (int j = 0; j < NT; ++j)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      E1[j][e] *= p.scale * eg[e >> 1];
-      E2[j][e] *= -eg[e >> 1];
-      E3[j][e] *= la[e >> 1];
-    }
-  // x.y of the warp's rows over its columns, from a tile in pieces
-  auto row_dot = [&](const float (&c)[NT][4], const __nv_bfloat16* tile, float (&out)[2]) {
-    out[0] = out[1] = 0.0f;
+  // x.y of the warp's rows over its columns, y a tile in pieces
+  auto put_dot = [&](int which, const float (&c)[NT][4], const __nv_bfloat16* tile) {
+    float out[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
@@ -762,63 +1020,69 @@ __global__ void __launch_bounds__(256) delta_bwd_chunk(const __grid_constant__ D
         const int off = tile_off<DKP>(row0 + g + 8 * r, ct + j) + 2 * t;
 #pragma unroll
         for (int i = 0; i < NP; ++i) {
-          const uint32_t w = *reinterpret_cast<const uint32_t*>(tile + i * (kC * DKP) + off);
-          out[r] = fmaf(lo_f32(w), c[j][2 * r], fmaf(hi_f32(w), c[j][2 * r + 1], out[r]));
+          const uint32_t x = *reinterpret_cast<const uint32_t*>(tile + i * (kC * DKP) + off);
+          out[r] = fmaf(lo_f32(x), c[j][2 * r], fmaf(hi_f32(x), c[j][2 * r + 1], out[r]));
         }
       }
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       out[r] += __shfl_xor_sync(0xffffffffu, out[r], 1);
       out[r] += __shfl_xor_sync(0xffffffffu, out[r], 2);
+      if (t == 0) s.dots[which][quarter][row0 + g + 8 * r] = out[r];
     }
   };
-  auto put_dot = [&](int which, const float (&c)[NT][4], const __nv_bfloat16* tile) {
-    float d[2];
-    row_dot(c, tile, d);
-    if (t == 0) {
-      s.dots[which][half][row0 + g] = d[0];
-      s.dots[which][half][row0 + g + 8] = d[1];
-    }
-  };
-  const int w4 = warp & 3;
   put_dot(3, E3, s.k[0]);
   // dQ = scale e^G E1 + M K
-  add_rows_times_tile<NP, DKP>(E1, sk, ct, 0, w4 + 1, lane,
-                               [&](int kb, uint32_t (&a)[3][4]) { a_rows<3>(s.M, row0, 16 * kb, lane, a); });
+  add_tile_product<NP, DKP>(E1, sk, ct, 0, w4 + 1, lane,
+                            [&](int kb, int i, uint32_t (&a)[4]) { load_a<kC>(a, tM + i * (kTri * 2), row0, kb, lane); });
   put_dot(0, E1, s.q[0]);
   // H = N K - e^G E2
-  add_rows_times_tile<NP, DKP>(E2, sk, ct, 0, w4 + 1, lane,
-                               [&](int kb, uint32_t (&a)[3][4]) { a_rows<3>(s.N, row0, 16 * kb, lane, a); });
+  add_tile_product<NP, DKP>(E2, sk, ct, 0, w4 + 1, lane,
+                            [&](int kb, int i, uint32_t (&a)[4]) { load_a<kC>(a, tN + i * (kTri * 2), row0, kb, lane); });
   put_dot(1, E2, s.k[0]);
   // C = N^T (beta K) + M^T Q + e^(G_last - G) E3
-  add_rows_times_tile<NP, DKP>(E3, sk, ct, w4, kC / 16, lane,
-                               [&](int kb, uint32_t (&a)[3][4]) { a_cols<3>(s.N, row0, 16 * kb, lane, beta, a); });
-  add_rows_times_tile<NP, DKP>(E3, sq, ct, w4, kC / 16, lane,
-                               [&](int kb, uint32_t (&a)[3][4]) { a_cols<3>(s.M, row0, 16 * kb, lane, nullptr, a); });
+  add_tile_product<NP, DKP>(E3, sk, ct, w4, kC / 16, lane,
+                            [&](int kb, int i, uint32_t (&a)[4]) { load_at<kC>(a, tNb + i * (kTri * 2), row0, kb, lane); });
+  add_tile_product<NP, DKP>(E3, sq, ct, w4, kC / 16, lane,
+                            [&](int kb, int i, uint32_t (&a)[4]) { load_at<kC>(a, tM + i * (kTri * 2), row0, kb, lane); });
   put_dot(2, E3, s.k[0]);
   // query and key gradients: to the tensors, or per value head where key heads are shared
 #pragma unroll
   for (int j = 0; j < NT; ++j)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int i = row0 + g + 8 * (e >> 1), c = 8 * (ct + j) + 2 * t + (e & 1);
-      if (i >= rows || c >= p.dkw) continue;
-      float kv = 0.0f, qv = 0.0f;
+    for (int r = 0; r < 2; ++r) {
+      const int i = row0 + g + 8 * r, c = 8 * (ct + j) + 2 * t;
+      float kv[2] = {0.0f, 0.0f}, qv[2] = {0.0f, 0.0f};
 #pragma unroll
       for (int x = 0; x < NP; ++x) {
-        const int off = x * (kC * DKP) + tile_off<DKP>(i, ct + j) + 2 * t + (e & 1);
-        kv += __bfloat162float(s.k[0][off]);
-        qv += __bfloat162float(s.q[0][off]);
+        const int off = x * (kC * DKP) + tile_off<DKP>(i, ct + j) + 2 * t;
+        const uint32_t kx = *reinterpret_cast<const uint32_t*>(s.k[0] + off);
+        const uint32_t qx = *reinterpret_cast<const uint32_t*>(s.q[0] + off);
+        kv[0] += lo_f32(kx);
+        kv[1] += hi_f32(kx);
+        qv[0] += lo_f32(qx);
+        qv[1] += hi_f32(qx);
       }
-      const float dq = fmaf(s.m[i], kv, E1[j][e]);
-      const float dk = fmaf(s.m[i], qv, fmaf(be[e >> 1], E2[j][e], E3[j][e]));
+      float dq[2], dk[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        dq[e] = fmaf(s.m[i], kv[e], E1[j][2 * r + e]);
+        dk[e] = fmaf(s.m[i], qv[e], fmaf(be[r], E2[j][2 * r + e], E3[j][2 * r + e]));
+      }
+      if (i >= rows || c >= p.dkw) continue;
       if (p.group > 1) {
-        const size_t o = (((size_t)b * p.L + t0 + i) * p.Hv + h) * p.dkw + c;
-        p.pdq[o] = dq;
-        p.pdk[o] = dk;
+        const size_t o = (((size_t)b * p.L + t0 + i) * p.Hv + h) * DKP + c;
+        *reinterpret_cast<float2*>(p.pdq + o) = make_float2(dq[0], dq[1]);
+        *reinterpret_cast<float2*>(p.pdk + o) = make_float2(dk[0], dk[1]);
       } else {
-        static_cast<T*>(const_cast<void*>(p.dq.ptr))[b * p.dq.sb + (t0 + i) * p.dq.sl + hk * p.dq.sh + c] = from_f32<T>(dq);
-        static_cast<T*>(const_cast<void*>(p.dk.ptr))[b * p.dk.sb + (t0 + i) * p.dk.sl + hk * p.dk.sh + c] = from_f32<T>(dk);
+        T* dqp = static_cast<T*>(const_cast<void*>(p.dq.ptr)) + b * p.dq.sb + (t0 + i) * p.dq.sl + hk * p.dq.sh + c;
+        T* dkp = static_cast<T*>(const_cast<void*>(p.dk.ptr)) + b * p.dk.sb + (t0 + i) * p.dk.sl + hk * p.dk.sh + c;
+        dqp[0] = from_f32<T>(dq[0]);
+        dkp[0] = from_f32<T>(dk[0]);
+        if (c + 1 < p.dkw) {
+          dqp[1] = from_f32<T>(dq[1]);
+          dkp[1] = from_f32<T>(dk[1]);
+        }
       }
     }
   __syncthreads();
@@ -827,17 +1091,16 @@ __global__ void __launch_bounds__(256) delta_bwd_chunk(const __grid_constant__ D
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int r = 2 * lane + i;
-      const float kH = s.dots[1][0][r] + s.dots[1][1][r];
-      dG[i] = (s.dots[0][0][r] + s.dots[0][1][r]) + beta[r] * kH - (s.dots[2][0][r] + s.dots[2][1][r]);
-      tail += s.dots[3][0][r] + s.dots[3][1][r];
-      if (r < rows)
-        p.dbeta[((size_t)b * p.L + t0 + r) * p.Hv + h] =
-            ((s.dxv[0][r] + s.dxv[1][r]) + (s.dxv[2][r] + s.dxv[3][r])) + kH;
+      auto sum = [&](int w) { return (s.dots[w][0][r] + s.dots[w][1][r]) + (s.dots[w][2][r] + s.dots[w][3][r]); };
+      const float kH = sum(1);
+      dG[i] = sum(0) + beta[r] * kH - sum(2);
+      tail += sum(3);
+      if (r < rows) p.dbeta[((size_t)b * p.L + t0 + r) * p.Hv + h] = s.dxv[r] + kH;
     }
     tail = group_allreduce<32, 1>(tail);
     float sds = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) sds += s.sds[i];
+    for (int i = 0; i < 16; ++i) sds += s.sds[i];
     tail = fmaf(s.vec[kC - 1], sds, tail);
     float run = dG[0] + dG[1];
 #pragma unroll
@@ -851,22 +1114,41 @@ __global__ void __launch_bounds__(256) delta_bwd_chunk(const __grid_constant__ D
   }
 }
 
-// dq, dk (B, L, Hk, dk): the value heads' parts summed in head order.
-template <typename T>
+// dq, dk (B, L, Hk, dk): the value heads' parts, (B, L, Hv, DKP) fp32, summed in head order.  A thread takes four
+// channels of one position and key head (blockIdx.x walks positions, blockIdx.y key heads).
+template <typename T, int DKP>
 __global__ void __launch_bounds__(256) delta_sum_heads(const __grid_constant__ DeltaParams p) {
-  const long long i = blockIdx.x * 256LL + threadIdx.x;
-  const long long total = (long long)p.B * p.L * p.Hk * p.dkw;
-  if (i >= total) return;
-  const int c = (int)(i % p.dkw), hk = (int)(i / p.dkw % p.Hk);
-  const long long row = i / p.dkw / p.Hk, b = row / p.L, l = row % p.L;
-  float dq = 0.0f, dk = 0.0f;
+  constexpr int kPer = 256 / (DKP / 4);              // positions per CTA
+  const int c = 4 * (threadIdx.x % (DKP / 4)), hk = blockIdx.y;
+  const long long row = (long long)blockIdx.x * kPer + threadIdx.x / (DKP / 4);
+  if (row >= (long long)p.B * p.L || c >= p.dkw) return;
+  const long long b = row / p.L, l = row - b * p.L;
+  float dq[4] = {}, dk[4] = {};
   for (int r = 0; r < p.group; ++r) {
-    const size_t o = ((size_t)row * p.Hv + hk * p.group + r) * p.dkw + c;
-    dq += p.pdq[o];
-    dk += p.pdk[o];
+    const size_t o = ((size_t)row * p.Hv + hk * p.group + r) * DKP + c;
+    float x[4], y[4];
+    load4(p.pdq + o, x);
+    load4(p.pdk + o, y);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      dq[e] += x[e];
+      dk[e] += y[e];
+    }
   }
-  static_cast<T*>(const_cast<void*>(p.dq.ptr))[b * p.dq.sb + l * p.dq.sl + hk * p.dq.sh + c] = from_f32<T>(dq);
-  static_cast<T*>(const_cast<void*>(p.dk.ptr))[b * p.dk.sb + l * p.dk.sl + hk * p.dk.sh + c] = from_f32<T>(dk);
+  T* dqp = static_cast<T*>(const_cast<void*>(p.dq.ptr)) + b * p.dq.sb + l * p.dq.sl + hk * p.dq.sh + c;
+  T* dkp = static_cast<T*>(const_cast<void*>(p.dk.ptr)) + b * p.dk.sb + l * p.dk.sl + hk * p.dk.sh + c;
+  constexpr int kBytes = 4 * (int)sizeof(T);
+  if (c + 4 <= p.dkw && ((reinterpret_cast<uintptr_t>(dqp) | reinterpret_cast<uintptr_t>(dkp)) & (kBytes - 1)) == 0) {
+    vec_store<T, 4>(dqp, dq);
+    vec_store<T, 4>(dkp, dk);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (c + e < p.dkw) {
+        dqp[e] = from_f32<T>(dq[e]);
+        dkp[e] = from_f32<T>(dk[e]);
+      }
+  }
 }
 
 // ================================================================================================
@@ -997,8 +1279,8 @@ size_t carve(const Shape& s, bool bwd, DeltaParams& p, unsigned char* base) {
     p.dstates = c.take<float>(chunks * s.dvp() * s.dkp());
     p.dxs = c.take<float>(chunks * s.dvp() * kC);
     if (s.Hv > s.Hk) {
-      p.pdq = c.take<float>((size_t)s.B * s.L * s.Hv * s.dk);
-      p.pdk = c.take<float>((size_t)s.B * s.L * s.Hv * s.dk);
+      p.pdq = c.take<float>((size_t)s.B * s.L * s.Hv * s.dkp());
+      p.pdk = c.take<float>((size_t)s.B * s.L * s.Hv * s.dkp());
     }
   }
   return c.used + 256;
@@ -1040,41 +1322,56 @@ cudaError_t launch(K kern, dim3 grid, int threads, size_t smem, const DeltaParam
   return cudaGetLastError();
 }
 
-// Warps per CTA of the chain kernels, 16 value channels each: up to eight, four where eight would leave
-// SMs without a CTA (a warp then has a scheduler to itself either way).
-int chain_warps(const Shape& s) {
-  const int64_t tiles = s.dvp() / 16;
-  int w = 1;
-  while (w < 8 && w < tiles) w *= 2;
-  return w == 8 && s.B * s.Hv * ((tiles + 7) / 8) < 148 ? 4 : w;
+// Strips per CTA of the chain kernels: one while every strip can have an SM of its own, then two, then four, which
+// load the chunks' tiles once for all.
+template <typename T, int NP, int DKP, int NS>
+cudaError_t run_chain_ns(const Shape& s, const DeltaParams& p, bool bwd, cudaStream_t st) {
+  const dim3 grid((unsigned)((s.dvp() / 16 + NS - 1) / NS), (unsigned)s.Hv, (unsigned)s.B);
+  constexpr int threads = 128 * NS + 32;
+  if (bwd) {
+    using Form = BwdChain<T, NP, DKP, NS>;
+    constexpr size_t smem = sizeof(typename Form::template Smem<Form::KB>);
+    if constexpr (smem > 227 * 1024) return cudaErrorInvalidValue;
+    else return launch(delta_bwd_chain<T, NP, DKP, NS>, grid, threads, smem, p, st);
+  } else {
+    using Form = FwdChain<T, NP, DKP, NS>;
+    constexpr size_t smem = sizeof(typename Form::template Smem<Form::KB>);
+    if constexpr (smem > 227 * 1024) return cudaErrorInvalidValue;
+    else
+      return p.states != nullptr ? launch(delta_fwd<T, NP, DKP, NS, true>, grid, threads, smem, p, st)
+                                 : launch(delta_fwd<T, NP, DKP, NS, false>, grid, threads, smem, p, st);
+  }
 }
-
 template <typename T, int NP, int DKP>
-cudaError_t run_fwd(const Shape& s, const DeltaParams& p, cudaStream_t st) {
+cudaError_t run_chain(const Shape& s, const DeltaParams& p, bool bwd, cudaStream_t st) {
+  const int64_t tiles = s.dvp() / 16, strips = s.B * s.Hv * tiles;
+  constexpr bool wide = NP == 3 && DKP == 128;       // six tiles of pieces leave room for one strip
+  if (wide || tiles == 1 || strips <= 148) return run_chain_ns<T, NP, DKP, 1>(s, p, bwd, st);
+  if constexpr (!wide) {
+    if (NP == 3 || tiles == 2 || strips <= 2 * 148) return run_chain_ns<T, NP, DKP, 2>(s, p, bwd, st);
+    if constexpr (NP == 1) return run_chain_ns<T, NP, DKP, 4>(s, p, bwd, st);
+  }
+  return cudaErrorInvalidValue;
+}
+template <typename T, int NP, int DKP>
+cudaError_t run_prep_and_chain(const Shape& s, const DeltaParams& p, bool bwd, cudaStream_t st) {
   const dim3 grid((unsigned)s.n(), (unsigned)s.Hv, (unsigned)s.B);
-  cudaError_t e = launch(delta_prep<T, NP, DKP>, grid, 128, sizeof(PrepSmem<T, NP, DKP>), p, st);
+  const cudaError_t e = launch(delta_prep<T, NP, DKP>, grid, 128, sizeof(PrepSmem<NP, DKP>), p, st);
   if (e != cudaSuccess) return e;
-  constexpr int PP = NP == 1 ? 2 : 3;
-  const int w = chain_warps(s);
-  const dim3 cg((unsigned)((s.dvp() / 16 + w - 1) / w), (unsigned)s.Hv, (unsigned)s.B);
-  constexpr size_t smem = chain_smem<NP, DKP, PP>();
-  return p.states != nullptr ? launch(delta_fwd<T, NP, DKP, true>, cg, 32 * w, smem, p, st)
-                             : launch(delta_fwd<T, NP, DKP, false>, cg, 32 * w, smem, p, st);
+  return run_chain<T, NP, DKP>(s, p, bwd, st);
 }
 
 template <typename T, int NP, int DKP>
 cudaError_t run_bwd(const Shape& s, const DeltaParams& p, cudaStream_t st) {
+  cudaError_t e = run_prep_and_chain<T, NP, DKP>(s, p, true, st);
+  if (e != cudaSuccess) return e;
   const dim3 grid((unsigned)s.n(), (unsigned)s.Hv, (unsigned)s.B);
-  cudaError_t e = launch(delta_prep<T, NP, DKP>, grid, 128, sizeof(PrepSmem<T, NP, DKP>), p, st);
-  if (e != cudaSuccess) return e;
-  const int w = chain_warps(s);
-  const dim3 cg((unsigned)((s.dvp() / 16 + w - 1) / w), (unsigned)s.Hv, (unsigned)s.B);
-  e = launch(delta_bwd_chain<T, NP, DKP>, cg, 32 * w, chain_smem<NP, DKP, 3>(), p, st);
-  if (e != cudaSuccess) return e;
-  e = launch(delta_bwd_chunk<T, NP, DKP>, grid, 256, sizeof(BwdSmem<NP, DKP>), p, st);
+  constexpr int SL = NP == 3 && DKP == 128 ? 16 : 32;     // what shared memory holds beside six tiles of pieces
+  e = launch(delta_bwd_chunk<T, NP, DKP, SL>, grid, 512, sizeof(BwdSmem<NP, DKP, SL>), p, st);
   if (e != cudaSuccess || p.group == 1) return e;
-  const long long total = (long long)p.B * p.L * p.Hk * p.dkw;
-  return launch(delta_sum_heads<T>, dim3((unsigned)((total + 255) / 256)), 256, 0, p, st);
+  constexpr int per = 256 / (DKP / 4);
+  const dim3 sg((unsigned)(((long long)p.B * p.L + per - 1) / per), (unsigned)p.Hk);
+  return launch(delta_sum_heads<T, DKP>, sg, 256, 0, p, st);
 }
 
 }  // namespace
@@ -1131,9 +1428,11 @@ int ssm_gated_delta_fwd(int64_t B, int64_t L, int64_t Hk, int64_t Hv, int64_t dk
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e;
   if (s.dtype == SSM_BF16)
-    e = s.dkp() == 64 ? run_fwd<__nv_bfloat16, 1, 64>(s, p, st) : run_fwd<__nv_bfloat16, 1, 128>(s, p, st);
+    e = s.dkp() == 64 ? run_prep_and_chain<__nv_bfloat16, 1, 64>(s, p, false, st)
+                      : run_prep_and_chain<__nv_bfloat16, 1, 128>(s, p, false, st);
   else
-    e = s.dkp() == 64 ? run_fwd<float, 3, 64>(s, p, st) : run_fwd<float, 3, 128>(s, p, st);
+    e = s.dkp() == 64 ? run_prep_and_chain<float, 3, 64>(s, p, false, st)
+                      : run_prep_and_chain<float, 3, 128>(s, p, false, st);
   if (e != cudaSuccess) return fail(SSM_ERR_CUDA, "gated delta rule forward: %s", cudaGetErrorString(e));
   return SSM_OK;
 }

@@ -11,9 +11,11 @@
 // are kept: six for float x float, three for float x bf16, one for bf16 x bf16.  That holds states,
 // gradients and their sums to fp32's own rounding, which one bf16 pass (2^-8) does not.
 //
-// The state is kept transposed, S^T (dv x dk), as accumulator fragments: a warp owns 16 rows (value
-// channels).  An accumulator tile pair is, lane by lane, the A operand of the next product, so the
-// chain S -> X -> U -> S' of a warp never leaves its registers and needs no barrier.
+// The state is kept transposed, S^T (dv x dk), as accumulator fragments: its rows (value channels) are
+// independent of one another.  Four warps share a strip of 16 rows: each owns a quarter of dk and two of
+// the eight 8-position column tiles of X, U and O.  An accumulator tile is, lane by lane, half of the A
+// operand of the next product, so what the warps exchange (the pieces of S, X, U) goes through shared
+// memory once, already in operand form.
 #pragma once
 
 #include "ssm_common.cuh"
@@ -30,22 +32,19 @@ struct Heads {                 // (B, L, H, width), unit stride along the width
 };
 
 __device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr)
-               : "memory");
+               : "r"(addr));
 }
 __device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr)
-               : "memory");
+               : "r"(addr));
 }
 // lo in the low half
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
@@ -73,7 +72,9 @@ __device__ __forceinline__ void split(float x0, float x1, uint32_t (&p)[NP]) {
 // groups are permuted by the row, so that the eight rows of an ldmatrix hit different banks.
 template <int W>
 __device__ __forceinline__ int tile_off(int row, int grp) {
-  return row * W + ((grp ^ (row & 7)) << 3);
+  static_assert(W == 16 || W == 32 || W >= 64, "rows of 32, 64 or a multiple of 128 bytes");
+  const int s = W >= 64 ? row & 7 : W == 32 ? (row >> 1) & 3 : (row >> 2) & 1;
+  return row * W + ((grp ^ s) << 3);
 }
 
 // B fragments of n tiles j, j + 1 (r[0..1], r[2..3]) and k block kb from a tile stored [n][k].
@@ -92,6 +93,12 @@ __device__ __forceinline__ void load_a(uint32_t (&r)[4], uint32_t tile, int row,
   ldsm4(r, tile + 2 * tile_off<W>(row + (lane & 15), 2 * kb + (lane >> 4)));
 }
 
+// The same from a tile stored [k][m].
+template <int W>
+__device__ __forceinline__ void load_at(uint32_t (&r)[4], uint32_t tile, int row, int kb, int lane) {
+  ldsm4t(r, tile + 2 * tile_off<W>(16 * kb + 8 * (lane >> 4) + (lane & 7), row / 8 + ((lane >> 3) & 1)));
+}
+
 // The A operand of k block kb from accumulator tiles 2 kb, 2 kb + 1, in NP pieces.
 template <int NP, int NT>
 __device__ __forceinline__ void acc_to_a(const float (&c)[NT][4], int kb, uint32_t (&a)[NP][4]) {
@@ -106,18 +113,38 @@ __device__ __forceinline__ void acc_to_a(const float (&c)[NT][4], int kb, uint32
     }
 }
 
-// d0, d1 += A (NA pieces) x the B fragments of piece pb, every product of pieces with index sum <= MAXI.
-template <int NA, int MAXI>
-__device__ __forceinline__ void mma_pieces(float (&d0)[4], float (&d1)[4], const uint32_t (&a)[NA][4],
-                                           const uint32_t (&b)[4], int pb) {
+// Tiles j0 .. j0 + 2 NJ - 1 of d += A (NA pieces) x NJ pairs of B fragments of piece pb: the products of pieces
+// with MINI <= index sum <= MAXI.  Consecutive instructions go to different accumulators.
+// The tensor cores truncate each sum to fp32.  So the small products (index sum >= 1) and the leading ones go to
+// accumulators of their own, added at the end: the many truncations of the small ones then count little.
+template <int MINI, int MAXI, int NJ, int NA, int NT>
+__device__ __forceinline__ void mma_pieces(float (&d)[NT][4], int j0, const uint32_t (&a)[NA][4],
+                                           const uint32_t (&b)[NJ][4], int pb) {
 #pragma unroll
   for (int i = 0; i < NA; ++i)
-    if (i + pb <= MAXI) {
-      mma_bf16(d0, a[i], b[0], b[1]);
-      mma_bf16(d1, a[i], b[2], b[3]);
+    if (i + pb >= MINI && i + pb <= MAXI) {
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        mma_bf16(d[j0 + 2 * j], a[i], b[j][0], b[j][1]);
+        mma_bf16(d[j0 + 2 * j + 1], a[i], b[j][2], b[j][3]);
+      }
     }
 }
+// lead += the leading products, low += the others up to index sum MAXI.
+template <int MAXI, int NJ, int NA, int NT>
+__device__ __forceinline__ void mma_split(float (&lead)[NT][4], float (&low)[NT][4], int j0, const uint32_t (&a)[NA][4],
+                                          const uint32_t (&b)[NJ][4], int pb) {
+  mma_pieces<1, MAXI>(low, j0, a, b, pb);
+  if (pb == 0) mma_pieces<0, 0>(lead, j0, a, b, 0);
+}
 
+template <int NT>
+__device__ __forceinline__ void add(float (&c)[NT][4], const float (&x)[NT][4]) {
+#pragma unroll
+  for (int j = 0; j < NT; ++j)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) c[j][e] += x[j][e];
+}
 template <int NT>
 __device__ __forceinline__ void zero(float (&c)[NT][4]) {
 #pragma unroll
@@ -126,30 +153,132 @@ __device__ __forceinline__ void zero(float (&c)[NT][4]) {
     for (int e = 0; e < 4; ++e) c[j][e] = 0.0f;
 }
 
-// (positions x value channels) of a head read in the accumulator layout of its transpose: element
-// (2 r + e) of tile j is position 8 j + 2 t + e, channel g + 8 r (g = lane / 4, t = lane % 4).
+// ---- strips: kC positions x 16 channels of a (positions, channels) tensor -----------------------------
+// Warp w of a strip works on the column tiles w and 7 - w, positions 8 w .. and 56 - 8 w .. (a pair that
+// carries the same triangular work for every w).  In the accumulator layout of the transpose element
+// (2 r + e) of a tile is position 2 t + e, channel g + 8 r (g = lane / 4, t = lane % 4): a gather of single
+// elements from global memory.  So a warp's rows pass through shared memory, 16 bytes at a time, in by
+// asynchronous copies a chunk ahead.  The 16-byte units of a row are permuted by the row so that the eight
+// rows of a transposing ldmatrix hit different banks.
+__device__ __forceinline__ int col_tile(int w, int i) { return i ? 7 - w : w; }
+
 template <typename T>
-__device__ __forceinline__ void load_vt(const T* base, long long sl, int rows, int cols, int lane, float (&v)[kC / 8][4]) {
-  const int g = lane >> 2, t = lane & 3;
+struct alignas(16) Strip {
+  T x[kC * 16];
+  static constexpr int kUnit = 16 / (int)sizeof(T);      // elements per unit
+  static constexpr int kUnits = 16 / kUnit;              // units per row
+  __device__ static int off(int row, int unit) {
+    const int s = sizeof(T) == 2 ? (row >> 2) & 1 : (row >> 1) & 3;
+    return (row * kUnits + (unit ^ s)) * kUnit;
+  }
+  __device__ static int row_of(int w, int i) { return 8 * col_tile(w, i >> 3) + (i & 7); }   // i-th of the warp's 16 rows
+  // Starts the copy of the warp's rows of `rows` x `cols` elements; the rest becomes zero.
+  __device__ void fetch(const T* base, long long sl, int rows, int cols, bool aligned, int w, int lane) {
 #pragma unroll
-  for (int j = 0; j < kC / 8; ++j)
+    for (int i = 0; i < kUnits / 2; ++i) {
+      const int u = lane + 32 * i, row = row_of(w, u / kUnits), unit = u % kUnits;
+      T* dst = x + off(row, unit);
+      if (aligned && cols >= 16 && row < rows) {
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)),
+                     "l"(base + row * sl + unit * kUnit)
+                     : "memory");
+      } else {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int c = 8 * j + 2 * t + (e & 1), d = g + 8 * (e >> 1);
-      v[j][e] = c < rows && d < cols ? to_f32(base[(long long)c * sl + d]) : 0.0f;
+        for (int e = 0; e < kUnit; ++e)
+          dst[e] = row < rows && unit * kUnit + e < cols ? base[row * sl + unit * kUnit + e] : from_f32<T>(0.0f);
+      }
     }
-}
-template <typename T>
-__device__ __forceinline__ void store_vt(T* base, long long sl, int rows, int cols, int lane, const float (&v)[kC / 8][4]) {
-  const int g = lane >> 2, t = lane & 3;
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  }
+  __device__ void arrive() {
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncwarp();
+  }
+  __device__ void read(float (&v)[2][4], int w, int lane) const {
+    if constexpr (sizeof(T) == 2) {
+      uint32_t r[4];
+      ldsm4t(r, smem_u32(x + off(8 * col_tile(w, lane >> 4) + (lane & 7), (lane >> 3) & 1)));
 #pragma unroll
-  for (int j = 0; j < kC / 8; ++j)
+      for (int h = 0; h < 4; ++h) {
+        v[h >> 1][2 * (h & 1)] = lo_f32(r[h]);
+        v[h >> 1][2 * (h & 1) + 1] = hi_f32(r[h]);
+      }
+    } else {
+      const int g = lane >> 2, t = lane & 3;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int c = 8 * j + 2 * t + (e & 1), d = g + 8 * (e >> 1);
-      if (c < rows && d < cols) base[(long long)c * sl + d] = from_f32<T>(v[j][e]);
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int c = 8 * col_tile(w, j) + 2 * t + (e & 1), d = g + 8 * (e >> 1);
+          v[j][e] = x[off(c, d >> 2) + (d & 3)];
+        }
     }
+  }
+  __device__ void write(const float (&v)[2][4], int w, int lane) {
+    if constexpr (sizeof(T) == 2) {
+      const uint32_t a = smem_u32(x + off(8 * col_tile(w, lane >> 4) + (lane & 7), (lane >> 3) & 1));
+      asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(a),
+                   "r"(pack_bf16(v[0][0], v[0][1])), "r"(pack_bf16(v[0][2], v[0][3])),
+                   "r"(pack_bf16(v[1][0], v[1][1])), "r"(pack_bf16(v[1][2], v[1][3]))
+                   : "memory");
+    } else {
+      const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int c = 8 * col_tile(w, j) + 2 * t + (e & 1), d = g + 8 * (e >> 1);
+          x[off(c, d >> 2) + (d & 3)] = v[j][e];
+        }
+    }
+    __syncwarp();
+  }
+  // Copies the warp's rows out; they may be written again after the next __syncwarp().
+  __device__ void flush(T* base, long long sl, int rows, int cols, bool aligned, int w, int lane) const {
+#pragma unroll
+    for (int i = 0; i < kUnits / 2; ++i) {
+      const int u = lane + 32 * i, row = row_of(w, u / kUnits), unit = u % kUnits;
+      const T* src = x + off(row, unit);
+      if (row >= rows) continue;
+      if (aligned && cols >= 16) {
+        *reinterpret_cast<uint4*>(base + row * sl + unit * kUnit) = *reinterpret_cast<const uint4*>(src);
+      } else {
+#pragma unroll
+        for (int e = 0; e < kUnit; ++e)
+          if (unit * kUnit + e < cols) base[row * sl + unit * kUnit + e] = src[e];
+      }
+    }
+    __syncwarp();
+  }
+};
+
+// ---- operands exchanged between the warps of a strip: [k block][piece][lane], 16 bytes a lane ------------
+// Half h (column tile 2 kb + h) of k block kb's A operand from an accumulator tile.
+template <int NP>
+__device__ __forceinline__ void put_half(uint4 (*f)[NP][32], int tile, const float (&c)[4], int lane) {
+  uint32_t a[NP], b[NP];
+  split<NP>(c[0], c[1], a);
+  split<NP>(c[2], c[3], b);
+#pragma unroll
+  for (int i = 0; i < NP; ++i)
+    reinterpret_cast<uint2*>(&f[tile >> 1][i][lane])[tile & 1] = make_uint2(a[i], b[i]);
 }
+__device__ __forceinline__ void get_frag(uint32_t (&a)[4], const uint4& f) {
+  a[0] = f.x;
+  a[1] = f.y;
+  a[2] = f.z;
+  a[3] = f.w;
+}
+// B fragments of the warp's two column tiles from a tile stored [n][k] / [k][n].
+template <int W>
+__device__ __forceinline__ void load_b2(uint32_t (&r)[4], uint32_t tile, int w, int kb, int lane) {
+  ldsm4(r, tile + 2 * tile_off<W>(8 * col_tile(w, lane >> 4) + (lane & 7), 2 * kb + ((lane >> 3) & 1)));
+}
+template <int W>
+__device__ __forceinline__ void load_bt2(uint32_t (&r)[4], uint32_t tile, int w, int kb, int lane) {
+  ldsm4t(r, tile + 2 * tile_off<W>(16 * kb + (lane & 15), col_tile(w, lane >> 4)));
+}
+
 // 16 rows of a dense fp32 [channel][W] tile from / to accumulators.
 template <int NT>
 __device__ __forceinline__ void store_acc(float* base, int W, int lane, const float (&c)[NT][4]) {
@@ -185,7 +314,7 @@ struct DeltaParams {
   float* us;                   // (B, Hv, n, dvp, kC): U^T
   float* dstates;              // the gradient of the state leaving the chunk, like states
   float* dxs;                  // dX^T, like us
-  float *pdq, *pdk;            // (B, L, Hv, dk) per value head, when value heads share key heads
+  float *pdq, *pdk;            // (B, L, Hv, DKP) per value head, when value heads share key heads
   int* err;
   int B, L, Hk, Hv, dkw, dvw, dvp, n, group;
   float scale;

@@ -9,13 +9,11 @@
 //   dz = dy a silu'(z);  dw = sum e n;  db = sum e
 //   dx = rstd (e w - (s1 + n s2) / M),  s1 = sum_group e w (0 unless centred), s2 = sum_group e w n
 //
-// A thread owns VEC consecutive channels (16 bytes where the layout allows, else one element); a warp
-// reads 32 consecutive vectors of a row.  Memory bounds every form; which launch does what:
-//   * one position, group = a power of two <= 32 vectors ("rows"): one kernel, every tensor moved
-//     once; the group sums are butterflies over the group's lanes, mean and variance two passes over
-//     registers.
-//   * one position, any other group width: a warp per (sample, group) for the sums, then the same
-//     element-wise kernels as below with a stride of one sample per row.
+// Memory bounds every form; which launch does what:
+//   * one position ("rows"): one kernel, every tensor moved once.  1 to 32 lanes, or eight warps, share
+//     a group, each lane holding K vectors of VEC channels in registers; sums are butterflies, mean and
+//     variance two passes over registers.  Groups that do not fit (above 8192 channels) take the last form
+//     with a warp per group for the sums.
 //   * more positions: per-(slab of rows, channel) partial sums, a combine per (sample, group), an
 //     element-wise pass (the tensors are read twice).
 // All sums are fp32 (the combines fp64) in a fixed order: no atomics, results are reproducible.
@@ -23,6 +21,7 @@
 
 #include <algorithm>
 #include <cstdio>
+#include <initializer_list>
 
 #include "ssm_b200.h"
 #include "ssm_vec.cuh"
@@ -112,104 +111,205 @@ __device__ __forceinline__ void write_partials(float* part, long long row, long 
   }
 }
 
-// ---- one position per sample, group = lpg lanes --------------------------------------------
-template <typename T, int VEC, int U>
-__global__ void __launch_bounds__(32 * kWarps) norm_rows_fwd(const NormParams p, int lpg) {
-  const long long c = ((long long)blockIdx.y * 32 + threadIdx.x) * VEC;
-  const bool live = c < p.C;
-  const float inv = 1.0f / (float)p.cg;
-  float w[VEC], b[VEC];
-  if (live) load_params<VEC>(p, c, w, b);
-  const long long r0 = (long long)blockIdx.x * kWarps * U + threadIdx.y;
-  float x[U][VEC], z[U][VEC];
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const long long r = r0 + u * kWarps;
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) x[u][v] = z[u][v] = 0.0f;
-    if (live && r < p.N) {
-      vec_load<T, VEC>(static_cast<const T*>(p.x) + r * p.xs + c, x[u]);
-      if (p.gate) vec_load<T, VEC>(static_cast<const T*>(p.z) + r * p.zs + c, z[u]);
+// ---- one position per sample ----------------------------------------------------------------
+// WPG = 1: lpg lanes (a power of two) share a group, the CTA's warps take different rows; blockIdx.y
+// selects 32 / lpg groups.  WPG = kWarps: the CTA shares one group, blockIdx.y selects it.
+// Vector i of a lane starts at channel (lane + i lpg) VEC of the group.
+template <int WPG>
+struct Place {
+  int lane;          // within the group
+  int lpg;
+  long long c0;      // first channel of the group
+  bool live;         // the group exists
+  long long row, step;
+  __device__ Place(const NormParams& p, int lpg_) {
+    long long group;
+    if (WPG == 1) {
+      lpg = lpg_;
+      lane = threadIdx.x & (lpg - 1);
+      group = (long long)blockIdx.y * (32 / lpg) + threadIdx.x / lpg;
+      row = (long long)blockIdx.x * kWarps + threadIdx.y;
+      step = (long long)gridDim.x * kWarps;
+    } else {
+      lpg = 32 * WPG;
+      lane = threadIdx.y * 32 + threadIdx.x;
+      group = blockIdx.y;
+      row = blockIdx.x;
+      step = gridDim.x;
     }
+    live = group < p.G;
+    c0 = group * p.cg;
   }
+};
+template <int WPG>
+__device__ __forceinline__ float group_sum(float x, int lpg) {
+  if (WPG == 1) {
+    for (int m = lpg >> 1; m >= 1; m >>= 1) x += __shfl_xor_sync(0xffffffffu, x, m);
+    return x;
+  }
+  __shared__ float red[kWarps];
+  x = ssm::group_allreduce<32, 1>(x);
+  __syncthreads();
+  if (threadIdx.x == 0) red[threadIdx.y] = x;
+  __syncthreads();
+  float s = 0.0f;
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const long long r = r0 + u * kWarps;
-    float mean = 0.0f, q = 0.0f;
-    if (p.center) {
+  for (int w = 0; w < kWarps; ++w) s += red[w];
+  return s;
+}
+
+// Mean (of the centred form) and rstd of the group whose lane holds x (zero past the group's end);
+// x becomes x - mean.
+template <int WPG, int VEC, int K>
+__device__ __forceinline__ float row_stats(const NormParams& p, const Place<WPG>& at, float (&x)[K][VEC]) {
+  const float inv = 1.0f / (float)p.cg;
+  if (p.center) {
+    float mean = 0.0f;
 #pragma unroll
-      for (int v = 0; v < VEC; ++v) mean += x[u][v];
-      for (int m = lpg >> 1; m >= 1; m >>= 1) mean += __shfl_xor_sync(0xffffffffu, mean, m);
-      mean *= inv;
+    for (int i = 0; i < K; ++i)
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) mean += x[i][v];
+    mean = group_sum<WPG>(mean, at.lpg) * inv;
+#pragma unroll
+    for (int i = 0; i < K; ++i)
+      if ((at.lane + i * at.lpg) * VEC < p.cg) {
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) x[i][v] -= mean;
+      }
+  }
+  float q = 0.0f;
+#pragma unroll
+  for (int i = 0; i < K; ++i)
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) q = fmaf(x[i][v], x[i][v], q);
+  return rsqrtf(fmaf(group_sum<WPG>(q, at.lpg), inv, p.eps));
+}
+
+// The number of rows is the same for all of a CTA's warps, so that group_sum's barriers match; rows past
+// the end work on zeros.
+template <typename T, int VEC, int K, int WPG>
+__global__ void __launch_bounds__(32 * kWarps) norm_rows_fwd(const NormParams p, int lpg) {
+  const Place<WPG> at(p, lpg);
+  for (long long r0 = 0; r0 < p.N; r0 += at.step) {
+    const long long r = r0 + at.row;
+    if (WPG > 1 && r >= p.N) return;
+    float x[K][VEC], z[K][VEC];
+    const bool ok = at.live && r < p.N;
+#pragma unroll
+    for (int i = 0; i < K; ++i) {
+      const int c = (at.lane + i * at.lpg) * VEC;
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) x[i][v] = z[i][v] = 0.0f;
+      if (ok && c < p.cg) {
+        vec_load<T, VEC>(static_cast<const T*>(p.x) + r * p.xs + at.c0 + c, x[i]);
+        if (p.gate) vec_load<T, VEC>(static_cast<const T*>(p.z) + r * p.zs + at.c0 + c, z[i]);
+      }
     }
+    const float rstd = row_stats<WPG, VEC, K>(p, at, x);
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) {
-      x[u][v] -= mean;
-      q = fmaf(x[u][v], x[u][v], q);
-    }
-    for (int m = lpg >> 1; m >= 1; m >>= 1) q += __shfl_xor_sync(0xffffffffu, q, m);
-    const float rstd = rsqrtf(fmaf(q, inv, p.eps));
-    if (live && r < p.N) {
-      float o[VEC];
+    for (int i = 0; i < K; ++i) {
+      const int c = (at.lane + i * at.lpg) * VEC;
+      if (ok && c < p.cg) {
+        float w[VEC], b[VEC], o[VEC];
+        load_params<VEC>(p, at.c0 + c, w, b);
 #pragma unroll
-      for (int v = 0; v < VEC; ++v) o[v] = norm_out(p, x[u][v] * rstd, w[v], b[v], z[u][v]);
-      vec_store<T, VEC>(static_cast<T*>(p.y) + r * p.ys + c, o);
-      if (p.stats != nullptr && threadIdx.x % lpg == 0)
-        *reinterpret_cast<float2*>(p.stats + (r * p.G + c / p.cg) * 2) = make_float2(mean, rstd);
+        for (int v = 0; v < VEC; ++v) o[v] = norm_out(p, x[i][v] * rstd, w[v], b[v], z[i][v]);
+        vec_store<T, VEC>(static_cast<T*>(p.y) + r * p.ys + at.c0 + c, o);
+      }
     }
   }
 }
 
-// Rows r = slab, slab + nslab, ... in steps of kWarps rows; parameter gradients stay in registers.
-template <typename T, int VEC>
+// Parameter gradients stay in registers over a CTA's rows; WPG = 1 adds its warps' at the end.
+template <typename T, int VEC, int K, int WPG>
 __global__ void __launch_bounds__(32 * kWarps) norm_rows_bwd(const NormParams p, int lpg) {
-  const long long c = ((long long)blockIdx.y * 32 + threadIdx.x) * VEC;
-  const bool live = c < p.C;
+  const Place<WPG> at(p, lpg);
   const float inv = 1.0f / (float)p.cg;
-  float w[VEC], b[VEC], dw[VEC], db[VEC];
+  float dw[K][VEC], db[K][VEC], w[K][VEC], b[K][VEC];
 #pragma unroll
-  for (int v = 0; v < VEC; ++v) w[v] = b[v] = dw[v] = db[v] = 0.0f;
-  if (live) load_params<VEC>(p, c, w, b);
-  for (long long r = (long long)blockIdx.x * kWarps + threadIdx.y; r < p.N; r += (long long)p.nslab * kWarps) {
-    float x[VEC], z[VEC], g[VEC], dz[VEC], n[VEC];
-    float2 st = make_float2(0.0f, 0.0f);
+  for (int i = 0; i < K; ++i) {
+    const int c = (at.lane + i * at.lpg) * VEC;
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) x[v] = z[v] = g[v] = 0.0f;
-    if (live) {
-      vec_load<T, VEC>(static_cast<const T*>(p.x) + r * p.xs + c, x);
-      vec_load<T, VEC>(static_cast<const T*>(p.dy) + r * p.gs + c, g);
-      if (p.gate) vec_load<T, VEC>(static_cast<const T*>(p.z) + r * p.zs + c, z);
-      st = *reinterpret_cast<const float2*>(p.stats + (r * p.G + c / p.cg) * 2);
+    for (int v = 0; v < VEC; ++v) dw[i][v] = db[i][v] = w[i][v] = b[i][v] = 0.0f;
+    if (at.live && c < p.cg) load_params<VEC>(p, at.c0 + c, w[i], b[i]);
+  }
+  for (long long r0 = 0; r0 < p.N; r0 += at.step) {
+    const long long r = r0 + at.row;
+    if (WPG > 1 && r >= p.N) break;
+    const bool ok = at.live && r < p.N;
+    float x[K][VEC], z[K][VEC], g[K][VEC];
+#pragma unroll
+    for (int i = 0; i < K; ++i) {
+      const int c = (at.lane + i * at.lpg) * VEC;
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) x[i][v] = z[i][v] = g[i][v] = 0.0f;
+      if (ok && c < p.cg) {
+        vec_load<T, VEC>(static_cast<const T*>(p.x) + r * p.xs + at.c0 + c, x[i]);
+        vec_load<T, VEC>(static_cast<const T*>(p.dy) + r * p.gs + at.c0 + c, g[i]);
+        if (p.gate) vec_load<T, VEC>(static_cast<const T*>(p.z) + r * p.zs + at.c0 + c, z[i]);
+      }
     }
+    const float rstd = row_stats<WPG, VEC, K>(p, at, x);
     float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) {
-      n[v] = (x[v] - st.x) * st.y;
-      g[v] = norm_grad(p, n[v], w[v], b[v], z[v], g[v], dz[v]);
-      dw[v] = fmaf(g[v], n[v], dw[v]);
-      db[v] += g[v];
-      g[v] *= w[v];
-      s1 += g[v];
-      s2 = fmaf(g[v], n[v], s2);
-    }
-    for (int m = lpg >> 1; m >= 1; m >>= 1) {
-      if (p.center) s1 += __shfl_xor_sync(0xffffffffu, s1, m);
-      s2 += __shfl_xor_sync(0xffffffffu, s2, m);
-    }
-    s1 = p.center ? s1 * inv : 0.0f;
-    s2 *= inv;
-    if (live) {
-      float o[VEC];
+    for (int i = 0; i < K; ++i)
 #pragma unroll
-      for (int v = 0; v < VEC; ++v) o[v] = st.y * (g[v] - fmaf(n[v], s2, s1));
-      vec_store<T, VEC>(static_cast<T*>(p.dx) + r * p.dxs + c, o);
-      if (p.gate) vec_store<T, VEC>(static_cast<T*>(p.dz) + r * p.dzs + c, dz);
+      for (int v = 0; v < VEC; ++v) {
+        x[i][v] *= rstd;
+        float dz = 0.0f;
+        const float e = norm_grad(p, x[i][v], w[i][v], b[i][v], z[i][v], g[i][v], dz);
+        z[i][v] = dz;
+        dw[i][v] = fmaf(e, x[i][v], dw[i][v]);
+        db[i][v] += e;
+        g[i][v] = e * w[i][v];
+        s1 += g[i][v];
+        s2 = fmaf(g[i][v], x[i][v], s2);
+      }
+    s1 = p.center ? group_sum<WPG>(s1, at.lpg) * inv : 0.0f;
+    s2 = group_sum<WPG>(s2, at.lpg) * inv;
+#pragma unroll
+    for (int i = 0; i < K; ++i) {
+      const int c = (at.lane + i * at.lpg) * VEC;
+      if (ok && c < p.cg) {
+        float o[VEC];
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) o[v] = rstd * (g[i][v] - fmaf(x[i][v], s2, s1));
+        vec_store<T, VEC>(static_cast<T*>(p.dx) + r * p.dxs + at.c0 + c, o);
+        if (p.gate) vec_store<T, VEC>(static_cast<T*>(p.dz) + r * p.dzs + at.c0 + c, z[i]);
+      }
     }
   }
-  write_partials<VEC>(p.part, blockIdx.x, p.C, c, live, dw, db);
+  float* part = p.part + (long long)blockIdx.x * 2 * p.C + at.c0;
+#pragma unroll
+  for (int i = 0; i < K; ++i) {
+    const int c = (at.lane + i * at.lpg) * VEC;
+    const bool ok = at.live && c < p.cg;
+    if (WPG == 1) {
+      __shared__ float red[kWarps][32][2 * VEC + 1];
+      __syncthreads();
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) {
+        red[threadIdx.y][threadIdx.x][v] = dw[i][v];
+        red[threadIdx.y][threadIdx.x][VEC + v] = db[i][v];
+      }
+      __syncthreads();
+      for (int j = threadIdx.y; j < 2 * VEC; j += kWarps) {
+        float s = 0.0f;
+#pragma unroll
+        for (int q = 0; q < kWarps; ++q) s += red[q][threadIdx.x][j];
+        if (ok) part[(j >= VEC ? p.C : 0) + c + j % VEC] = s;
+      }
+    } else if (ok) {
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) {
+        part[c + v] = dw[i][v];
+        part[p.C + c + v] = db[i][v];
+      }
+    }
+  }
 }
 
-// ---- one position per sample, any group width: a warp per (sample, group) ------------------
+// ---- one position per sample, groups too wide for registers: a warp per (sample, group) ------
 template <typename T, bool BWD>
 __global__ void __launch_bounds__(256) norm_group_sums(const NormParams p) {
   const long long i = ((long long)blockIdx.x * 256 + threadIdx.x) >> 5;
@@ -518,9 +618,18 @@ void plan_slabs(long long units, long long rows, long long C, int* nslab, long l
 
 size_t round256(size_t x) { return (x + 255) & ~size_t(255); }
 
-bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
-bool view_al(const ssm_view& v, int es) {
-  return v.ptr == nullptr || (al16(v.ptr) && (v.batch_stride * es) % 16 == 0 && (v.row_stride * es) % 16 == 0);
+// The widest vector (a power of two elements, at most 16 bytes) that divides cg channels and at which every row
+// of every view starts aligned.
+int rows_vec(int cg, int es, std::initializer_list<ssm_view> views) {
+  int vec = 16 / es;
+  while (cg % vec != 0) vec /= 2;
+  for (const ssm_view& v : views) {
+    if (v.ptr == nullptr) continue;
+    while (vec > 1 && (reinterpret_cast<uintptr_t>(v.ptr) % (vec * es) != 0 || v.batch_stride % vec != 0 ||
+                       v.row_stride % vec != 0))
+      vec /= 2;
+  }
+  return vec;
 }
 
 int check_shape(int64_t N, int64_t P, int64_t C, int64_t G) {
@@ -544,59 +653,96 @@ int check_act(const char* what, const ssm_view& v, int dtype, bool required) {
   return SSM_OK;
 }
 
-// Lanes per group when the one-kernel rows form applies, else 0.
-int rows_lanes(int64_t P, int cg, int vec) {
-  if (P != 1 || cg % vec != 0) return 0;
-  const int lanes = cg / vec;
-  return lanes <= 32 && (lanes & (lanes - 1)) == 0 ? lanes : 0;
+// How the rows kernels share a group of cg channels in vectors of vec: lanes (0: eight warps), vectors
+// per lane (a power of two, at most 32 channels in all); K = 0 where the group does not fit.
+struct RowsForm {
+  int lpg, k;
+};
+RowsForm rows_form(int cg, int vec) {
+  const int nvec = cg / vec, most = std::min(8, 32 / vec);
+  RowsForm f = {1, 1};
+  while (f.lpg < 32 && f.lpg < nvec) f.lpg *= 2;
+  while (f.k < most && f.lpg * f.k < nvec) f.k *= 2;
+  if (f.lpg * f.k >= nvec) return f;
+  f = {0, 1};
+  if (32 * kWarps < nvec) f.k = most;
+  if (32 * kWarps * f.k < nvec) f.k = 0;
+  return f;
+}
+
+template <typename T, int VEC, int K, int WPG>
+cudaError_t launch_rows(const NormParams& p, bool bwd, int lpg, cudaStream_t st) {
+  const dim3 block(32, kWarps);
+  const int per = WPG == 1 ? 32 / lpg : 1;                         // groups per CTA
+  const unsigned gy = (unsigned)ceil_div(p.G, per);
+  if (bwd) {
+    norm_rows_bwd<T, VEC, K, WPG><<<dim3((unsigned)p.nslab, gy), block, 0, st>>>(p, lpg);
+  } else {
+    // every warp (CTA) takes one row while that fills the GPU a few times over, then loops
+    const long long rows = WPG == 1 ? ceil_div(p.N, kWarps) : p.N;
+    const unsigned gx = (unsigned)std::min<long long>(rows, std::max<long long>(1, ceil_div(148 * 64, gy)));
+    norm_rows_fwd<T, VEC, K, WPG><<<dim3(gx, gy), block, 0, st>>>(p, lpg);
+  }
+  return cudaGetLastError();
+}
+template <typename T, int VEC>
+cudaError_t run_rows(const NormParams& p, bool bwd, RowsForm f, cudaStream_t st) {
+  constexpr int kMost = 32 / VEC < 8 ? 32 / VEC : 8;
+  if (f.lpg == 0) return f.k == 1 ? launch_rows<T, VEC, 1, kWarps>(p, bwd, 0, st) : launch_rows<T, VEC, kMost, kWarps>(p, bwd, 0, st);
+  if (f.k == 1) return launch_rows<T, VEC, 1, 1>(p, bwd, f.lpg, st);
+  if (f.k == 2) return launch_rows<T, VEC, 2, 1>(p, bwd, f.lpg, st);
+  if (f.k == 4) return launch_rows<T, VEC, 4, 1>(p, bwd, f.lpg, st);
+  if constexpr (kMost == 8) return launch_rows<T, VEC, 8, 1>(p, bwd, f.lpg, st);
+  return cudaErrorInvalidValue;
+}
+// The widest vector that divides a group and every row start.
+template <typename T>
+cudaError_t run_rows_any(const NormParams& p, bool bwd, int vec, RowsForm f, cudaStream_t st) {
+  if constexpr (sizeof(T) == 2)
+    if (vec == 8) return run_rows<T, 8>(p, bwd, f, st);
+  if (vec == 4) return run_rows<T, 4>(p, bwd, f, st);
+  if (vec == 2) return run_rows<T, 2>(p, bwd, f, st);
+  return run_rows<T, 1>(p, bwd, f, st);
+}
+
+// mean and rstd of every (sample, group) into p.stats
+template <typename T, int VEC>
+void run_stats(const NormParams& p, cudaStream_t st) {
+  if (p.P == 1) {
+    norm_group_sums<T, false><<<(unsigned)ceil_div(p.N * p.G, 8), 256, 0, st>>>(p);
+    return;
+  }
+  const dim3 grid((unsigned)(p.N * p.nslab), (unsigned)ceil_div(ceil_div(p.C, VEC), 32));
+  norm_col_stats<T, VEC><<<grid, dim3(32, kWarps), 0, st>>>(p);
+  norm_combine_stats<<<(unsigned)ceil_div(p.N * p.G, 8), 256, 0, st>>>(p);
 }
 
 template <typename T, int VEC>
 cudaError_t run_fwd(NormParams& p, cudaStream_t st) {
   const dim3 block(32, kWarps);
   const unsigned cols = (unsigned)ceil_div(ceil_div(p.C, VEC), 32);
-  if (const int lpg = rows_lanes(p.P, p.cg, VEC)) {
-    constexpr int U = 4;
-    norm_rows_fwd<T, VEC, U><<<dim3((unsigned)ceil_div(p.N, kWarps * U), cols), block, 0, st>>>(p, lpg);
-    return cudaGetLastError();
-  }
-  if (p.P == 1) {
-    norm_group_sums<T, false><<<(unsigned)ceil_div(p.N * p.G, 8), 256, 0, st>>>(p);
-    norm_apply_fwd<T, VEC, true><<<dim3((unsigned)p.nslab, cols), block, 0, st>>>(p);
-    return cudaGetLastError();
-  }
-  const dim3 grid((unsigned)(p.N * p.nslab), cols);
-  norm_col_stats<T, VEC><<<grid, block, 0, st>>>(p);
-  norm_combine_stats<<<(unsigned)ceil_div(p.N * p.G, 8), 256, 0, st>>>(p);
-  norm_apply_fwd<T, VEC, false><<<grid, block, 0, st>>>(p);
+  run_stats<T, VEC>(p, st);
+  if (p.P == 1) norm_apply_fwd<T, VEC, true><<<dim3((unsigned)p.nslab, cols), block, 0, st>>>(p);
+  else norm_apply_fwd<T, VEC, false><<<dim3((unsigned)(p.N * p.nslab), cols), block, 0, st>>>(p);
   return cudaGetLastError();
 }
 
 template <typename T, int VEC>
-cudaError_t run_bwd(NormParams& p, cudaStream_t st) {
+cudaError_t run_bwd(NormParams& p, bool stats_given, cudaStream_t st) {
   const dim3 block(32, kWarps);
   const unsigned cols = (unsigned)ceil_div(ceil_div(p.C, VEC), 32);
-  long long nparts = p.nslab;
-  if (const int lpg = rows_lanes(p.P, p.cg, VEC)) {
-    norm_rows_bwd<T, VEC><<<dim3((unsigned)p.nslab, cols), block, 0, st>>>(p, lpg);
-  } else if (p.P == 1) {
+  if (!stats_given) run_stats<T, VEC>(p, st);
+  if (p.P == 1) {
     norm_group_sums<T, true><<<(unsigned)ceil_div(p.N * p.G, 8), 256, 0, st>>>(p);
     norm_col_grads<T, VEC, true><<<dim3((unsigned)p.nslab, cols), block, 0, st>>>(p);
     norm_apply_bwd<T, VEC, true><<<dim3((unsigned)p.nslab, cols), block, 0, st>>>(p);
   } else {
-    nparts = p.N * p.nslab;
-    const dim3 grid((unsigned)nparts, cols);
+    const dim3 grid((unsigned)(p.N * p.nslab), cols);
     norm_col_grads<T, VEC, false><<<grid, block, 0, st>>>(p);
     norm_combine_sums<<<(unsigned)ceil_div(p.N * p.G, 8), 256, 0, st>>>(p);
     norm_apply_bwd<T, VEC, false><<<grid, block, 0, st>>>(p);
   }
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return e;
-  if (p.dw != nullptr || p.db != nullptr) {
-    norm_param_grads<<<dim3((unsigned)ceil_div(p.C, 32), 2), block, 0, st>>>(p, nparts);
-    e = cudaGetLastError();
-  }
-  return e;
+  return cudaGetLastError();
 }
 
 // Fills the shape and the slabs; returns the number of partial rows (each 2 C floats).
@@ -625,9 +771,26 @@ int ssm_group_norm_workspace_size(int64_t N, int64_t P, int64_t C, int64_t G, in
   NormParams p = {};
   const size_t part = round256((size_t)plan(p, N, P, C, G) * 2 * C * sizeof(float));
   const size_t groups = round256((size_t)N * G * 2 * sizeof(float));
-  if (backward) *bytes = part + groups + 256;
-  else *bytes = (P > 1 ? part : 0) + groups + 256;
+  // the rows kernels need none forward and only partial sums backward; single channels always fit worst
+  const bool rows = P == 1 && rows_form(p.cg, 1).k != 0;
+  if (backward) *bytes = part + (rows ? 0 : 2 * groups) + 256;
+  else *bytes = rows ? 0 : (P > 1 ? part : 0) + groups + 256;
   return SSM_OK;
+}
+
+static void set_inputs(NormParams& p, ssm_view x, const float* weight, const float* bias, int32_t center, int32_t silu,
+                       ssm_view z) {
+  p.x = x.ptr;
+  p.xs = x.batch_stride;
+  p.xp = x.row_stride;
+  p.z = z.ptr;
+  p.zs = z.batch_stride;
+  p.zp = z.row_stride;
+  p.w = weight;
+  p.b = bias;
+  p.center = center ? 1 : 0;
+  p.silu = silu ? 1 : 0;
+  p.gate = z.ptr != nullptr;
 }
 
 int ssm_group_norm_fwd(int64_t N, int64_t P, int64_t C, int64_t G, ssm_view x, const float* weight, const float* bias,
@@ -641,50 +804,45 @@ int ssm_group_norm_fwd(int64_t N, int64_t P, int64_t C, int64_t G, ssm_view x, c
   if ((rc = check_act("y", y, x.dtype, true))) return rc;
   size_t need = 0;
   ssm_group_norm_workspace_size(N, P, C, G, 0, &need);
-  if (workspace == nullptr || workspace_bytes < need)
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need))
     return fail(SSM_ERR_WORKSPACE, "group_norm: workspace of %lld bytes required, %lld given", (long long)need,
                 (long long)workspace_bytes);
   NormParams p = {};
   const long long parts = plan(p, N, P, C, G);
-  unsigned char* cur = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(workspace) + 255) & ~uintptr_t(255));
-  if (P > 1) {
-    p.part = reinterpret_cast<float*>(cur);
-    cur += round256((size_t)parts * 2 * C * sizeof(float));
-  }
-  p.stats = stats != nullptr ? stats : reinterpret_cast<float*>(cur);
-  p.x = x.ptr;
-  p.xs = x.batch_stride;
-  p.xp = x.row_stride;
-  p.z = z.ptr;
-  p.zs = z.batch_stride;
-  p.zp = z.row_stride;
+  set_inputs(p, x, weight, bias, center, silu, z);
   p.y = const_cast<void*>(y.ptr);
   p.ys = y.batch_stride;
   p.yp = y.row_stride;
-  p.w = weight;
-  p.b = bias;
   p.eps = eps;
-  p.center = center ? 1 : 0;
-  p.silu = silu ? 1 : 0;
-  p.gate = z.ptr != nullptr;
-  const int es = x.dtype == SSM_BF16 ? 2 : 4;
-  const bool vec = C % (16 / es) == 0 && view_al(x, es) && view_al(z, es) && view_al(y, es);
-  if (stats == nullptr && rows_lanes(P, p.cg, vec ? 16 / es : 1)) p.stats = nullptr;   // not needed, not written
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int es = x.dtype == SSM_BF16 ? 2 : 4;
   cudaError_t e;
-  if (x.dtype == SSM_BF16) e = vec ? run_fwd<__nv_bfloat16, 8>(p, st) : run_fwd<__nv_bfloat16, 1>(p, st);
-  else e = vec ? run_fwd<float, 4>(p, st) : run_fwd<float, 1>(p, st);
+  const int rv = rows_vec(p.cg, es, {x, z, y});
+  const RowsForm f = rows_form(p.cg, rv);
+  if (P == 1 && f.k != 0) {
+    e = es == 2 ? run_rows_any<__nv_bfloat16>(p, false, rv, f, st) : run_rows_any<float>(p, false, rv, f, st);
+  } else {
+    unsigned char* cur = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(workspace) + 255) & ~uintptr_t(255));
+    if (P > 1) {
+      p.part = reinterpret_cast<float*>(cur);
+      cur += round256((size_t)parts * 2 * C * sizeof(float));
+    }
+    p.stats = stats != nullptr ? stats : reinterpret_cast<float*>(cur);
+    const bool vec = C % (16 / es) == 0 && rows_vec(16 / es, es, {x, z, y}) == 16 / es;
+    if (es == 2) e = vec ? run_fwd<__nv_bfloat16, 8>(p, st) : run_fwd<__nv_bfloat16, 1>(p, st);
+    else e = vec ? run_fwd<float, 4>(p, st) : run_fwd<float, 1>(p, st);
+  }
   if (e != cudaSuccess) return fail(SSM_ERR_CUDA, "group_norm forward launch failed (error %lld)", (long long)e);
   return SSM_OK;
 }
 
 int ssm_group_norm_bwd(int64_t N, int64_t P, int64_t C, int64_t G, ssm_view x, const float* weight, const float* bias,
-                       int32_t center, int32_t silu, ssm_view z, const float* stats, ssm_view dy, ssm_view dx,
-                       float* dweight, float* dbias, ssm_view dz, void* workspace, size_t workspace_bytes,
+                       float eps, int32_t center, int32_t silu, ssm_view z, const float* stats, ssm_view dy,
+                       ssm_view dx, float* dweight, float* dbias, ssm_view dz, void* workspace, size_t workspace_bytes,
                        void* stream) {
   int rc = check_shape(N, P, C, G);
   if (rc) return rc;
-  if (x.ptr == nullptr || stats == nullptr) return fail(SSM_ERR_INVALID, "group_norm: x and stats are required");
+  if (x.ptr == nullptr) return fail(SSM_ERR_INVALID, "group_norm: x is required");
   if (x.dtype != SSM_F32 && x.dtype != SSM_BF16) return fail(SSM_ERR_DTYPE, "group_norm: x dtype %lld unsupported", x.dtype);
   if ((rc = check_act("z", z, x.dtype, false))) return rc;
   if ((rc = check_act("dy", dy, x.dtype, true))) return rc;
@@ -697,16 +855,8 @@ int ssm_group_norm_bwd(int64_t N, int64_t P, int64_t C, int64_t G, ssm_view x, c
                 (long long)workspace_bytes);
   NormParams p = {};
   const long long parts = plan(p, N, P, C, G);
-  unsigned char* cur = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(workspace) + 255) & ~uintptr_t(255));
-  p.part = reinterpret_cast<float*>(cur);
-  p.sums = reinterpret_cast<float*>(cur + round256((size_t)parts * 2 * C * sizeof(float)));
-  p.stats = const_cast<float*>(stats);
-  p.x = x.ptr;
-  p.xs = x.batch_stride;
-  p.xp = x.row_stride;
-  p.z = z.ptr;
-  p.zs = z.batch_stride;
-  p.zp = z.row_stride;
+  set_inputs(p, x, weight, bias, center, silu, z);
+  p.eps = eps;
   p.dy = dy.ptr;
   p.gs = dy.batch_stride;
   p.gp = dy.row_stride;
@@ -716,20 +866,33 @@ int ssm_group_norm_bwd(int64_t N, int64_t P, int64_t C, int64_t G, ssm_view x, c
   p.dz = const_cast<void*>(dz.ptr);
   p.dzs = dz.batch_stride;
   p.dzp = dz.row_stride;
-  p.w = weight;
-  p.b = bias;
   p.dw = dweight;
   p.db = dbias;
-  p.center = center ? 1 : 0;
-  p.silu = silu ? 1 : 0;
-  p.gate = z.ptr != nullptr;
-  const int es = x.dtype == SSM_BF16 ? 2 : 4;
-  const bool vec = C % (16 / es) == 0 && view_al(x, es) && view_al(z, es) && view_al(dy, es) && view_al(dx, es) &&
-                   view_al(dz, es);
+  unsigned char* cur = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(workspace) + 255) & ~uintptr_t(255));
+  p.part = reinterpret_cast<float*>(cur);
+  cur += round256((size_t)parts * 2 * C * sizeof(float));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int es = x.dtype == SSM_BF16 ? 2 : 4;
   cudaError_t e;
-  if (x.dtype == SSM_BF16) e = vec ? run_bwd<__nv_bfloat16, 8>(p, st) : run_bwd<__nv_bfloat16, 1>(p, st);
-  else e = vec ? run_bwd<float, 4>(p, st) : run_bwd<float, 1>(p, st);
+  long long nparts = parts;
+  const int rv = rows_vec(p.cg, es, {x, z, dy, dx, dz});
+  const RowsForm f = rows_form(p.cg, rv);
+  if (P == 1 && f.k != 0) {
+    nparts = p.nslab;
+    e = es == 2 ? run_rows_any<__nv_bfloat16>(p, true, rv, f, st) : run_rows_any<float>(p, true, rv, f, st);
+  } else {
+    p.sums = reinterpret_cast<float*>(cur);
+    cur += round256((size_t)N * G * 2 * sizeof(float));
+    p.stats = stats != nullptr ? const_cast<float*>(stats) : reinterpret_cast<float*>(cur);
+    const bool vec = C % (16 / es) == 0 && rows_vec(16 / es, es, {x, z, dy, dx, dz}) == 16 / es;
+    const bool given = stats != nullptr;
+    if (es == 2) e = vec ? run_bwd<__nv_bfloat16, 8>(p, given, st) : run_bwd<__nv_bfloat16, 1>(p, given, st);
+    else e = vec ? run_bwd<float, 4>(p, given, st) : run_bwd<float, 1>(p, given, st);
+  }
+  if (e == cudaSuccess && (dweight != nullptr || dbias != nullptr)) {
+    norm_param_grads<<<dim3((unsigned)ceil_div(C, 32), 2), dim3(32, kWarps), 0, st>>>(p, nparts);
+    e = cudaGetLastError();
+  }
   if (e != cudaSuccess) return fail(SSM_ERR_CUDA, "group_norm backward launch failed (error %lld)", (long long)e);
   return SSM_OK;
 }

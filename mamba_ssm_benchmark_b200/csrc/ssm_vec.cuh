@@ -1,4 +1,4 @@
-// ssm_vec.cuh — vectors of VEC consecutive elements (16 bytes, or one element) as float.
+// ssm_vec.cuh — vectors of VEC consecutive elements (up to 16 bytes, aligned to their size) as float.
 #pragma once
 
 #include "ssm_common.cuh"
@@ -7,13 +7,17 @@ namespace ssm {
 
 template <typename T, int VEC>
 __device__ __forceinline__ void vec_load(const T* src, float (&v)[VEC]) {
+  constexpr int kBytes = VEC * (int)sizeof(T);
+  static_assert(kBytes <= 16 && (VEC & (VEC - 1)) == 0, "a vector is one load");
   if constexpr (VEC == 1) {
     v[0] = to_f32(src[0]);
   } else if constexpr (sizeof(T) == 4) {
-    static_assert(VEC == 4, "fp32 vectors are 4 wide");
-    load4(src, v);
+    if constexpr (VEC == 4) load4(src, v);
+    else load2(src, v);
+  } else if constexpr (VEC <= 4) {
+    if constexpr (VEC == 4) load4(src, v);
+    else load2(src, v);
   } else {
-    static_assert(VEC == 8, "bf16 vectors are 8 wide");
     const uint4 q = *reinterpret_cast<const uint4*>(src);
     const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
@@ -29,13 +33,18 @@ __device__ __forceinline__ void vec_store(T* dst, const float (&v)[VEC]) {
   if constexpr (VEC == 1) {
     dst[0] = from_f32<T>(v[0]);
   } else if constexpr (sizeof(T) == 4) {
-    *reinterpret_cast<float4*>(dst) = make_float4(v[0], v[1], v[2], v[3]);
+    if constexpr (VEC == 4) *reinterpret_cast<float4*>(dst) = make_float4(v[0], v[1], v[2], v[3]);
+    else *reinterpret_cast<float2*>(dst) = make_float2(v[0], v[1]);
   } else {
-    uint4 q;
-    __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&q);
+    uint32_t w[VEC / 2];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) h[i] = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-    *reinterpret_cast<uint4*>(dst) = q;
+    for (int i = 0; i < VEC / 2; ++i) {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    if constexpr (VEC == 8) *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+    else if constexpr (VEC == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
+    else *reinterpret_cast<uint32_t*>(dst) = w[0];
   }
 }
 

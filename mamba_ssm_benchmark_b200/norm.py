@@ -18,31 +18,31 @@ import torch
 from . import _native as nat
 
 
-def _view(t, positions):
-    """ssm_view of a (samples, positions, C) tensor; a 2-D one has a single position."""
-    return nat.view2(t) if positions == 1 else nat.view3(t)
+def _dims(x):
+    return (x.shape[0], 1, x.shape[1]) if x.dim() == 2 else tuple(x.shape)
 
 
-def _workspace(shape, groups, backward, dev):
-    n = nat.norm_workspace_bytes(*shape, groups, backward)
-    return torch.empty(n, dtype=torch.uint8, device=dev), n
+def _views(positions, *tensors):
+    """ssm_views of (samples, positions, C) tensors; two-dimensional ones have a single position."""
+    view = nat.view2 if positions == 1 else nat.view3
+    return [view(t) for t in tensors]
+
+
+def _workspace(N, P, C, groups, backward, dev):
+    n = nat.norm_workspace_bytes(N, P, C, groups, backward)
+    return (torch.empty(n, dtype=torch.uint8, device=dev) if n else None), n
 
 
 def _forward(x, weight, bias, z, groups, eps, silu, center, want_stats):
+    """(y, stats): the statistics are kept for a backward where more than one position makes them costly."""
     (N, P, C), dev = _dims(x), x.device
-    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    stats = torch.empty((N, groups, 2), dtype=torch.float32, device=dev) if want_stats else None
-    ws, wsb = _workspace((N, P, C), groups, False, dev)
-    with torch.cuda.device(dev):
-        rc = nat.lib().ssm_group_norm_fwd(N, P, C, groups, _view(x, P), nat.ptr(weight), nat.ptr(bias), eps,
-                                          int(center), int(silu), _view(z, P), _view(y, P), nat.ptr(stats),
-                                          ws.data_ptr(), wsb, nat.stream_of(dev))
-    nat.check(rc, "ssm_group_norm_fwd")
+    y = torch.empty_like(x)
+    stats = torch.empty((N, groups, 2), dtype=torch.float32, device=dev) if want_stats and P > 1 else None
+    ws, wsb = _workspace(N, P, C, groups, False, dev)
+    xv, zv, yv = _views(P, x, z, y)
+    nat.call("ssm_group_norm_fwd", dev, N, P, C, groups, xv, nat.ptr(weight), nat.ptr(bias), eps, center, silu, zv, yv,
+             nat.ptr(stats), nat.ptr(ws), wsb)
     return y, stats
-
-
-def _dims(x):
-    return (x.shape[0], 1, x.shape[1]) if x.dim() == 2 else tuple(x.shape)
 
 
 class GroupNormFn(torch.autograd.Function):
@@ -50,40 +50,50 @@ class GroupNormFn(torch.autograd.Function):
     def forward(ctx, x, weight, bias, z, groups, eps, silu, center):
         y, stats = _forward(x, weight, bias, z, groups, eps, silu, center, True)
         ctx.save_for_backward(x, weight, bias, z, stats)
-        ctx.args = groups, silu, center
+        ctx.args = groups, eps, silu, center
         return y
 
     @staticmethod
     def backward(ctx, dy):
         x, weight, bias, z, stats = ctx.saved_tensors
-        groups, silu, center = ctx.args
+        groups, eps, silu, center = ctx.args
         (N, P, C), dev = _dims(x), x.device
-        dy = _dense(dy.to(x.dtype))
-        dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
-        dz = torch.empty(x.shape, dtype=x.dtype, device=dev) if z is not None else None
-        dw = torch.empty(C, dtype=torch.float32, device=dev) if weight is not None else None
-        db = torch.empty(C, dtype=torch.float32, device=dev) if bias is not None else None
-        ws, wsb = _workspace((N, P, C), groups, True, dev)
-        with torch.cuda.device(dev):
-            rc = nat.lib().ssm_group_norm_bwd(N, P, C, groups, _view(x, P), nat.ptr(weight), nat.ptr(bias), int(center),
-                                              int(silu), _view(z, P), nat.ptr(stats), _view(dy, P), _view(dx, P),
-                                              nat.ptr(dw), nat.ptr(db), _view(dz, P), ws.data_ptr(), wsb,
-                                              nat.stream_of(dev))
-        nat.check(rc, "ssm_group_norm_bwd")
+        dy = _dense(dy if dy.dtype == x.dtype else dy.to(x.dtype))
+        dx = torch.empty_like(x)
+        dz = None if z is None else torch.empty_like(z)
+        dw = None if weight is None else torch.empty_like(weight)
+        db = None if bias is None else torch.empty_like(bias)
+        ws, wsb = _workspace(N, P, C, groups, True, dev)
+        xv, zv, gv, dxv, dzv = _views(P, x, z, dy, dx, dz)
+        nat.call("ssm_group_norm_bwd", dev, N, P, C, groups, xv, nat.ptr(weight), nat.ptr(bias), eps, center, silu, zv,
+                 nat.ptr(stats), gv, dxv, nat.ptr(dw), nat.ptr(db), dzv, nat.ptr(ws), wsb)
         return dx, dw, db, dz, None, None, None, None
 
 
 def _dense(t):
-    """A layout the kernels read: unit stride along the channels, no negative or broadcast trouble."""
+    """A layout that the kernels read: unit stride along the channels."""
     return t if t is None or t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
 def _param(t, name, C):
     if t is None:
         return None
-    if tuple(t.shape) != (C,):
+    if t.dim() != 1 or t.shape[0] != C:
         raise ValueError(f"{name} must be ({C},), got {tuple(t.shape)}")
-    return t.to(torch.float32).contiguous()
+    return (t if t.dtype == torch.float32 else t.to(torch.float32)).contiguous()
+
+
+def _flat(t, dtype):
+    """(samples, C) or (samples, positions, C) in the kernels' type; one position is the two-dimensional case."""
+    if t is None:
+        return None
+    if t.dtype != dtype:
+        t = t.to(dtype)
+    if t.dim() > 2:
+        t = t.reshape(t.shape[0], -1, t.shape[-1])
+        if t.shape[1] == 1:
+            t = t[:, 0]
+    return _dense(t)
 
 
 def group_norm(x, groups, weight=None, bias=None, eps=1e-5, activation=None, z=None, center=True):
@@ -95,40 +105,34 @@ def group_norm(x, groups, weight=None, bias=None, eps=1e-5, activation=None, z=N
     Differentiable with respect to x, weight, bias and z."""
     if x.dim() < 2:
         raise ValueError(f"x must be (samples, ..., C), got {tuple(x.shape)}")
-    C = x.shape[-1]
-    if min(x.shape) < 1:
-        raise ValueError(f"x must have no empty axis, got {tuple(x.shape)}")
+    C, in_dtype, shape = x.shape[-1], x.dtype, x.shape
+    if x.numel() == 0:
+        raise ValueError(f"x must have no empty axis, got {tuple(shape)}")
     if not isinstance(groups, int) or groups < 1 or C % groups != 0:
         raise ValueError(f"groups must divide C={C}, got {groups!r}")
     if activation not in (None, "silu"):
         raise ValueError(f"activation must be 'silu' or None, got {activation!r}")
-    if z is not None and z.shape != x.shape:
-        raise ValueError(f"z must be shaped like x {tuple(x.shape)}, got {tuple(z.shape)}")
+    if z is not None and z.shape != shape:
+        raise ValueError(f"z must be shaped like x {tuple(shape)}, got {tuple(z.shape)}")
     if not eps >= 0.0:
         raise ValueError(f"eps must not be negative, got {eps!r}")
-    acts = [t for t in (x, z) if t is not None]
-    if any(t.dtype == torch.float64 for t in acts):
+    if in_dtype == torch.float64 or (z is not None and z.dtype == torch.float64):
         raise TypeError("float64 is not supported by the sm_100a kernels; use float32 or bfloat16")
     if not x.is_cuda:
         raise RuntimeError("the sm_100a group norm needs CUDA tensors (this package has no CPU path)")
-    if any(t is not None and t.device != x.device for t in (weight, bias, z)):
-        raise ValueError("all tensors must be on one device")
-    ct = x.dtype if x.dtype in nat.DTYPES and all(t.dtype == x.dtype for t in acts) else torch.float32
+    dev = x.device
+    for t in (weight, bias, z):
+        if t is not None and t.device != dev:
+            raise ValueError("all tensors must be on one device")
+    dtype = in_dtype if in_dtype in nat.DTYPES and (z is None or z.dtype == in_dtype) else torch.float32
+    x, z = _flat(x, dtype), _flat(z, dtype)
     weight, bias = _param(weight, "weight", C), _param(bias, "bias", C)
-
-    def flat(t):
-        if t is None:
-            return None
-        t = t.to(ct)
-        if t.dim() > 2:      # (samples, positions, C); one position is the two-dimensional case
-            t = t.reshape(t.shape[0], -1, C)
-            t = t[:, 0] if t.shape[1] == 1 else t
-        return _dense(t)
-
-    xf, zf = flat(x), flat(z)
-    tensors = [t for t in (xf, weight, bias, zf) if t is not None]
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
-        y = GroupNormFn.apply(xf, weight, bias, zf, groups, float(eps), activation == "silu", bool(center))
+    silu = activation == "silu"
+    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or
+                                    (bias is not None and bias.requires_grad) or (z is not None and z.requires_grad)):
+        y = GroupNormFn.apply(x, weight, bias, z, groups, float(eps), silu, bool(center))
     else:
-        y, _ = _forward(xf, weight, bias, zf, groups, float(eps), activation == "silu", bool(center), False)
-    return y.reshape(x.shape).to(x.dtype)
+        y = _forward(x, weight, bias, z, groups, float(eps), silu, bool(center), False)[0]
+    if y.shape != shape:
+        y = y.reshape(shape)
+    return y if in_dtype == dtype else y.to(in_dtype)

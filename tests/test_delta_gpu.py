@@ -256,7 +256,7 @@ def test_refusals():
         bad(q=torch.zeros(1, 8, 1, 129, device=DEV), k=torch.zeros(1, 8, 1, 129, device=DEV), h0=None)
     with pytest.raises(ValueError, match="empty"):
         bad(q=d["q"][:, :0], k=d["k"][:, :0], v=d["v"][:, :0], g=d["g"][:, :0], beta=d["beta"][:, :0])
-    with pytest.raises(ValueError, match="g must"):
+    with pytest.raises(ValueError, match="g and beta must"):
         bad(g=d["g"][..., 0])
     with pytest.raises(ValueError, match="h0 must"):
         bad(h0=d["h0"].transpose(0, 1))
