@@ -12,6 +12,7 @@
 
 #include "ssm_b200.h"
 #include "ssm_delta.cuh"
+#include "ssm_launch.cuh"
 #include "ssm_vec.cuh"
 
 namespace ssm {
@@ -736,13 +737,16 @@ __global__ void __launch_bounds__(128 * NS + 32) delta_bwd_chain(const __grid_co
 // after which dQ_i gets m_i k_i and dK_i gets m_i q_i;
 // dg is dG summed from the end of the chunk.  Every exponent's gradient is thus a row product of
 // gradients that are formed anyway; k.k and q.k are not needed again.
-// A warp takes 16 rows and a quarter of the columns.  dv is walked SL channels at a time: a bulk copy brings a slab of S,
-// dS', U and dX (fp32) while the last one is multiplied; all threads then split it into bf16 pieces once, in the
-// tiles that ldmatrix reads.
+// A warp takes 16 rows and a quarter of the columns.  dv is walked SL channels at a time: bulk copies bring slabs of
+// S, dS', U and dX (fp32) one ahead of the one in work, across chunks too (a CTA walks over many); all threads
+// split a slab into bf16 pieces once, in the tiles that ldmatrix reads.
 // ================================================================================================
+template <int DKP, int SL>
+struct alignas(128) BwdSlab {   // as it lies in global memory
+  float S[SL * DKP], dS[SL * DKP], U[SL * kC], dX[SL * kC];
+};
 template <int NP, int DKP, int SL>
-struct BwdSlab {
-  float S[SL * DKP], dS[SL * DKP], U[SL * kC], dX[SL * kC];                     // as they lie in global memory
+struct BwdPieces {
   __nv_bfloat16 pS[3][SL * DKP], pdS[3][SL * DKP], pU[3][SL * kC], pdX[3][SL * kC], pdO[NP][kC * SL];
 };
 struct BwdTri {
@@ -750,17 +754,19 @@ struct BwdTri {
 };
 template <int NP, int DKP, int SL>
 struct alignas(128) BwdSmem {
+  BwdSlab<DKP, SL> slab[2];
   union {
-    BwdSlab<NP, DKP, SL> slab;
+    BwdPieces<NP, DKP, SL> x;
     BwdTri tri;                 // after the last slab
   };
-  __nv_bfloat16 k[NP][kC * DKP], q[NP][kC * DKP];
+  alignas(128) __nv_bfloat16 k[NP][kC * DKP];
+  __nv_bfloat16 q[NP][kC * DKP];
   float vec[kVec];
   float dots[4][4][kC];         // q.dQ, k.H, k.C, e^(G_last - G) k.E3; by column quarter
   float dxv[kC];                // dX.V
-  float sds[16];                 // <S, dS'> by warp
+  float sds[16];                // <S, dS'> by warp
   float m[kC];                  // the diagonal of M
-  uint64_t bar_kq, bar_slab;
+  uint64_t bar_kq, bar_slab[2];
 };
 
 // d += the products of A (given by frag(kb, piece, a)) over k blocks [kb0, kb1) with a [c][dk] tile of NP pieces, in the
@@ -794,323 +800,337 @@ __global__ void __launch_bounds__(512) delta_bwd_chunk(const __grid_constant__ D
   constexpr int NT = DKP / 32, KS = SL / 16;      // n tiles of a warp's quarter of dk; k blocks of a slab
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int w4 = warp & 3, row0 = 16 * w4, quarter = warp >> 2;
-  const int ch = blockIdx.x, h = blockIdx.y, b = blockIdx.z, hk = h / p.group;
-  const int rows = min(kC, p.L - ch * kC);
-  const long long t0 = (long long)ch * kC;
-  const size_t at = ((size_t)b * p.Hv + h) * p.n + ch;
-  const size_t atk = ((size_t)b * p.Hk + hk) * p.n + ch;
-  auto fetch_slab = [&](int v0) {
+  const int items = p.n * p.Hv * p.B, per_item = (p.dvp + SL - 1) / SL;    // (chunk, head, batch); slabs of each
+  // slab number `it` of this CTA, counted over its items
+  auto fetch_slab = [&](int it) {
+    const size_t at = blockIdx.x + (size_t)(it / per_item) * gridDim.x;    // chunk innermost, like the buffers
+    if (at >= (size_t)items) return;
+    const int v0 = it % per_item * SL;
     const uint32_t vn = min(SL, p.dvp - v0);
-    mbar_arrive_expect_tx(&s.bar_slab, vn * (2 * DKP + 2 * kC) * 4);
-    bulk_load(s.slab.S, p.states + (at * p.dvp + v0) * DKP, vn * DKP * 4, &s.bar_slab);
-    bulk_load(s.slab.dS, p.dstates + (at * p.dvp + v0) * DKP, vn * DKP * 4, &s.bar_slab);
-    bulk_load(s.slab.U, p.us + (at * p.dvp + v0) * kC, vn * kC * 4, &s.bar_slab);
-    bulk_load(s.slab.dX, p.dxs + (at * p.dvp + v0) * kC, vn * kC * 4, &s.bar_slab);
+    auto& d = s.slab[it & 1];
+    uint64_t* bar = &s.bar_slab[it & 1];
+    mbar_arrive_expect_tx(bar, vn * (2 * DKP + 2 * kC) * 4);
+    bulk_load(d.S, p.states + (at * p.dvp + v0) * DKP, vn * DKP * 4, bar);
+    bulk_load(d.dS, p.dstates + (at * p.dvp + v0) * DKP, vn * DKP * 4, bar);
+    bulk_load(d.U, p.us + (at * p.dvp + v0) * kC, vn * kC * 4, bar);
+    bulk_load(d.dX, p.dxs + (at * p.dvp + v0) * kC, vn * kC * 4, bar);
   };
   if (tid == 0) {
     mbar_init(&s.bar_kq, 1);
-    mbar_init(&s.bar_slab, 1);
+    mbar_init(&s.bar_slab[0], 1);
+    mbar_init(&s.bar_slab[1], 1);
     fence_mbar_init();
     fetch_slab(0);
-    mbar_arrive_expect_tx(&s.bar_kq, sizeof(s.k) + sizeof(s.q) + sizeof(s.vec));
-    bulk_load(s.k, p.kimg + atk * (NP * kC * DKP), sizeof(s.k), &s.bar_kq);
-    bulk_load(s.q, p.qimg + atk * (NP * kC * DKP), sizeof(s.q), &s.bar_kq);
-    bulk_load(s.vec, p.vec + at * kVec, sizeof(s.vec), &s.bar_kq);
+    fetch_slab(1);
   }
-  // dO and V of a slab: 8 channels of one position per thread and step
+  __syncthreads();
+  // dO and V of a slab: 8 channels of one position per thread
   constexpr int kRowGroups = SL / 8;
-  const T* dOb = static_cast<const T*>(p.o.ptr) + b * p.o.sb + t0 * p.o.sl + h * p.o.sh;
-  const T* Vb = static_cast<const T*>(p.v.ptr) + b * p.v.sb + t0 * p.v.sl + h * p.v.sh;
+  static_assert(kC * kRowGroups <= 512, "a slab's dO is one step");
   const bool ovec = rows_aligned16(p.o, sizeof(T)), vvec = rows_aligned16(p.v, sizeof(T));
   const bool loads = tid < kC * kRowGroups;
   const int lc = tid / kRowGroups, lg = tid % kRowGroups;
-  static_assert(kC * kRowGroups <= 512, "a slab's dO is one step");
-  float xo[8], xv[8];
-  auto load_rows = [&](int v0) {
-    if (!loads) return;
-    const int width = lc < rows ? p.dvw : 0;
-    load8<T>(dOb + lc * p.o.sl, v0 + 8 * lg, width, ovec, xo);
-    load8<T>(Vb + lc * p.v.sl, v0 + 8 * lg, width, vvec, xv);
-  };
-  load_rows(0);
-  float E1[NT][4], E2[NT][4], E3[NT][4], XU[2][4], OU[2][4];
-  zero(E1);
-  zero(E2);
-  zero(E3);
-  zero(XU);
-  zero(OU);
-  float dot = 0.0f, dxv = 0.0f;
-  __syncthreads();
-  for (int v0 = 0, it = 0; v0 < p.dvp; v0 += SL, ++it) {
-    const int vn = min(SL, p.dvp - v0);
-    mbar_wait(&s.bar_slab, it & 1, p.err);
-    // split the slab
-    for (int e = tid; e < SL * DKP / 8; e += 512) {
-      const int r = e / (DKP / 8), grp = e % (DKP / 8), off = tile_off<DKP>(r, grp);
-      float x[8], y[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = y[i] = 0.0f;
-      if (r < vn) {
-        load8<float>(s.slab.S + r * DKP, 8 * grp, DKP, true, x);
-        load8<float>(s.slab.dS + r * DKP, 8 * grp, DKP, true, y);
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) dot = fmaf(x[i], y[i], dot);
-      put_pieces<3>(x, s.slab.pS[0], nullptr, off, SL * DKP);
-      put_pieces<3>(y, s.slab.pdS[0], nullptr, off, SL * DKP);
+  int it = 0;
+#pragma unroll 1
+  for (int item = blockIdx.x, turn = 0; item < items; item += gridDim.x, ++turn) {
+    const int ch = item % p.n, h = item / p.n % p.Hv, b = item / p.n / p.Hv, hk = h / p.group;
+    const int rows = min(kC, p.L - ch * kC);
+    const long long t0 = (long long)ch * kC;
+    if (tid == 0) {
+      const size_t at = item, atk = ((size_t)b * p.Hk + hk) * p.n + ch;
+      mbar_arrive_expect_tx(&s.bar_kq, sizeof(s.k) + sizeof(s.q) + sizeof(s.vec));
+      bulk_load(s.k, p.kimg + atk * (NP * kC * DKP), sizeof(s.k), &s.bar_kq);
+      bulk_load(s.q, p.qimg + atk * (NP * kC * DKP), sizeof(s.q), &s.bar_kq);
+      bulk_load(s.vec, p.vec + at * kVec, sizeof(s.vec), &s.bar_kq);
     }
-    for (int e = tid; e < SL * kC / 8; e += 512) {
-      const int r = e / (kC / 8), grp = e % (kC / 8), off = tile_off<kC>(r, grp);
-      float x[8], y[8];
+    const T* dOb = static_cast<const T*>(p.o.ptr) + b * p.o.sb + t0 * p.o.sl + h * p.o.sh;
+    const T* Vb = static_cast<const T*>(p.v.ptr) + b * p.v.sb + t0 * p.v.sl + h * p.v.sh;
+    float xo[8], xv[8];
+    auto load_rows = [&](int v0) {
+      if (!loads) return;
+      const int width = lc < rows ? p.dvw : 0;
+      load8<T>(dOb + lc * p.o.sl, v0 + 8 * lg, width, ovec, xo);
+      load8<T>(Vb + lc * p.v.sl, v0 + 8 * lg, width, vvec, xv);
+    };
+    load_rows(0);
+    float E1[NT][4], E2[NT][4], E3[NT][4], XU[2][4], OU[2][4];
+    zero(E1);
+    zero(E2);
+    zero(E3);
+    zero(XU);
+    zero(OU);
+    float dot = 0.0f, dxv = 0.0f;
+    for (int v0 = 0; v0 < p.dvp; v0 += SL, ++it) {
+      const int vn = min(SL, p.dvp - v0);
+      const auto& raw = s.slab[it & 1];
+      mbar_wait(&s.bar_slab[it & 1], (it >> 1) & 1, p.err);
+      // split the slab
+      for (int e = tid; e < SL * DKP / 8; e += 512) {
+        const int r = e / (DKP / 8), grp = e % (DKP / 8), off = tile_off<DKP>(r, grp);
+        float x[8], y[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = y[i] = 0.0f;
-      if (r < vn) {
-        load8<float>(s.slab.U + r * kC, 8 * grp, kC, true, x);
-        load8<float>(s.slab.dX + r * kC, 8 * grp, kC, true, y);
-      }
-      put_pieces<3>(x, s.slab.pU[0], nullptr, off, SL * kC);
-      put_pieces<3>(y, s.slab.pdX[0], nullptr, off, SL * kC);
-    }
-    if (loads) {
-      put_pieces<NP>(xo, s.slab.pdO[0], nullptr, tile_off<SL>(lc, lg), kC * SL);
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (8 * lg + i < vn) dxv = fmaf(s.slab.dX[(8 * lg + i) * kC + lc], xv[i], dxv);
-    }
-    __syncthreads();
-    if (v0 + SL < p.dvp) {
-      if (tid == 0) fetch_slab(v0 + SL);
-      load_rows(v0 + SL);
-    }
-    // multiply.  The slab's small products, then its leading ones, in fresh accumulators that are added to the
-    // totals once, rounded to nearest.
-    uint32_t ao[KS][NP][4], ax[KS][3][4], au[KS][3][4];
-    const uint32_t tO = smem_u32(s.slab.pdO[0]), tX = smem_u32(s.slab.pdX[0]), tU = smem_u32(s.slab.pU[0]);
-    const uint32_t tS = smem_u32(s.slab.pS[0]), tdS = smem_u32(s.slab.pdS[0]);
-#pragma unroll
-    for (int k = 0; k < KS; ++k) {
-#pragma unroll
-      for (int i = 0; i < NP; ++i) load_a<SL>(ao[k][i], tO + i * (kC * SL * 2), row0, k, lane);
-#pragma unroll
-      for (int i = 0; i < 3; ++i) {
-        load_at<kC>(ax[k][i], tX + i * (SL * kC * 2), row0, k, lane);
-        load_at<kC>(au[k][i], tU + i * (SL * kC * 2), row0, k, lane);
-      }
-    }
-#pragma unroll
-    for (int jp = 0; jp < NT / 2; ++jp) {
-      float d1[2][4], d2[2][4], d3[2][4];
-      zero(d1);
-      zero(d2);
-      zero(d3);
-      uint32_t bs[KS][1][4], bd[KS][1][4];
-#pragma unroll
-      for (int pb = 2; pb >= 0; --pb)
-#pragma unroll
-        for (int k = 0; k < KS; ++k) {
-          load_bt<DKP>(bs[k][0], tS + pb * (SL * DKP * 2), quarter * NT + 2 * jp, k, lane);
-          load_bt<DKP>(bd[k][0], tdS + pb * (SL * DKP * 2), quarter * NT + 2 * jp, k, lane);
-          mma_pieces<1, 2>(d1, 0, ao[k], bs[k], pb);
-          mma_pieces<1, 2>(d2, 0, ax[k], bs[k], pb);
-          mma_pieces<1, 2>(d3, 0, au[k], bd[k], pb);
+        for (int i = 0; i < 8; ++i) x[i] = y[i] = 0.0f;
+        if (r < vn) {
+          load8<float>(raw.S + r * DKP, 8 * grp, DKP, true, x);
+          load8<float>(raw.dS + r * DKP, 8 * grp, DKP, true, y);
         }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) dot = fmaf(x[i], y[i], dot);
+        put_pieces<3>(x, s.x.pS[0], nullptr, off, SL * DKP);
+        put_pieces<3>(y, s.x.pdS[0], nullptr, off, SL * DKP);
+      }
+      for (int e = tid; e < SL * kC / 8; e += 512) {
+        const int r = e / (kC / 8), grp = e % (kC / 8), off = tile_off<kC>(r, grp);
+        float x[8], y[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = y[i] = 0.0f;
+        if (r < vn) {
+          load8<float>(raw.U + r * kC, 8 * grp, kC, true, x);
+          load8<float>(raw.dX + r * kC, 8 * grp, kC, true, y);
+        }
+        put_pieces<3>(x, s.x.pU[0], nullptr, off, SL * kC);
+        put_pieces<3>(y, s.x.pdX[0], nullptr, off, SL * kC);
+      }
+      if (loads) {
+        put_pieces<NP>(xo, s.x.pdO[0], nullptr, tile_off<SL>(lc, lg), kC * SL);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (8 * lg + i < vn) dxv = fmaf(raw.dX[(8 * lg + i) * kC + lc], xv[i], dxv);
+      }
+      __syncthreads();
+      if (tid == 0) fetch_slab(it + 2);
+      if (v0 + SL < p.dvp) load_rows(v0 + SL);
+      // multiply.  The slab's small products, then its leading ones, in fresh accumulators that are added to the
+      // totals once, rounded to nearest.
+      uint32_t ao[KS][NP][4], ax[KS][3][4], au[KS][3][4];
+      const uint32_t tO = smem_u32(s.x.pdO[0]), tX = smem_u32(s.x.pdX[0]), tU = smem_u32(s.x.pU[0]);
+      const uint32_t tS = smem_u32(s.x.pS[0]), tdS = smem_u32(s.x.pdS[0]);
 #pragma unroll
       for (int k = 0; k < KS; ++k) {
-        mma_pieces<0, 0>(d1, 0, ao[k], bs[k], 0);
-        mma_pieces<0, 0>(d2, 0, ax[k], bs[k], 0);
-        mma_pieces<0, 0>(d3, 0, au[k], bd[k], 0);
+#pragma unroll
+        for (int i = 0; i < NP; ++i) load_a<SL>(ao[k][i], tO + i * (kC * SL * 2), row0, k, lane);
+#pragma unroll
+        for (int i = 0; i < 3; ++i) {
+          load_at<kC>(ax[k][i], tX + i * (SL * kC * 2), row0, k, lane);
+          load_at<kC>(au[k][i], tU + i * (SL * kC * 2), row0, k, lane);
+        }
       }
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
+      for (int jp = 0; jp < NT / 2; ++jp) {
+        float d1[2][4], d2[2][4], d3[2][4];
+        zero(d1);
+        zero(d2);
+        zero(d3);
+        uint32_t bs[KS][1][4], bd[KS][1][4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          E1[2 * jp + j][e] += d1[j][e];
-          E2[2 * jp + j][e] += d2[j][e];
-          E3[2 * jp + j][e] += d3[j][e];
-        }
-    }
-    if (quarter <= w4) {
-      float d1[2][4], d2[2][4];
-      zero(d1);
-      zero(d2);
-      uint32_t bu[KS][1][4];
+        for (int pb = 2; pb >= 0; --pb)
 #pragma unroll
-      for (int pb = 2; pb >= 0; --pb)
+          for (int k = 0; k < KS; ++k) {
+            load_bt<DKP>(bs[k][0], tS + pb * (SL * DKP * 2), quarter * NT + 2 * jp, k, lane);
+            load_bt<DKP>(bd[k][0], tdS + pb * (SL * DKP * 2), quarter * NT + 2 * jp, k, lane);
+            mma_pieces<1, 2>(d1, 0, ao[k], bs[k], pb);
+            mma_pieces<1, 2>(d2, 0, ax[k], bs[k], pb);
+            mma_pieces<1, 2>(d3, 0, au[k], bd[k], pb);
+          }
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
-          load_bt<kC>(bu[k][0], tU + pb * (SL * kC * 2), 2 * quarter, k, lane);
-          mma_pieces<1, 2>(d1, 0, ao[k], bu[k], pb);
-          mma_pieces<1, 2>(d2, 0, ax[k], bu[k], pb);
+          mma_pieces<0, 0>(d1, 0, ao[k], bs[k], 0);
+          mma_pieces<0, 0>(d2, 0, ax[k], bs[k], 0);
+          mma_pieces<0, 0>(d3, 0, au[k], bd[k], 0);
         }
 #pragma unroll
-      for (int k = 0; k < KS; ++k) {
-        mma_pieces<0, 0>(d1, 0, ao[k], bu[k], 0);
-        mma_pieces<0, 0>(d2, 0, ax[k], bu[k], 0);
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            E1[2 * jp + j][e] += d1[j][e];
+            E2[2 * jp + j][e] += d2[j][e];
+            E3[2 * jp + j][e] += d3[j][e];
+          }
       }
+      if (quarter <= w4) {
+        float d1[2][4], d2[2][4];
+        zero(d1);
+        zero(d2);
+        uint32_t bu[KS][1][4];
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
+        for (int pb = 2; pb >= 0; --pb)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          OU[j][e] += d1[j][e];
-          XU[j][e] += d2[j][e];
+          for (int k = 0; k < KS; ++k) {
+            load_bt<kC>(bu[k][0], tU + pb * (SL * kC * 2), 2 * quarter, k, lane);
+            mma_pieces<1, 2>(d1, 0, ao[k], bu[k], pb);
+            mma_pieces<1, 2>(d2, 0, ax[k], bu[k], pb);
+          }
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+          mma_pieces<0, 0>(d1, 0, ao[k], bu[k], 0);
+          mma_pieces<0, 0>(d2, 0, ax[k], bu[k], 0);
         }
-    }
-    __syncthreads();
-  }
-  mbar_wait(&s.bar_kq, 0, p.err);
-  const float* beta = s.vec + 2 * kC;
-  // N, beta N and M in pieces, where the slab was
 #pragma unroll
-  for (int j = 0; j < 2; ++j)
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            OU[j][e] += d1[j][e];
+            XU[j][e] += d2[j][e];
+          }
+      }
+      __syncthreads();
+    }
+    mbar_wait(&s.bar_kq, turn & 1, p.err);
+    const float* beta = s.vec + 2 * kC;
+    // N, beta N and M in pieces, where the slab was
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const int i = row0 + g + 8 * r, c = 16 * quarter + 8 * j + 2 * t;
+        float n[2], m[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float d =
+              i > c + e ? ex2((s.vec[3 * kC + i] - s.vec[3 * kC + c + e]) + (s.vec[4 * kC + i] - s.vec[4 * kC + c + e])) : 0.0f;
+          n[e] = i > c + e ? -d * XU[j][2 * r + e] : 0.0f;
+          m[e] = i > c + e ? p.scale * d * OU[j][2 * r + e] : 0.0f;
+          if (i == c + e) s.m[i] = p.scale * OU[j][2 * r + e];
+        }
+        const int off = tile_off<kC>(i, c >> 3) + 2 * t;
+        uint32_t x[3];
+        auto put = [&](__nv_bfloat16 (&tile)[3][kTri], float v0, float v1) {
+          split<3>(v0, v1, x);
+#pragma unroll
+          for (int q = 0; q < 3; ++q) *reinterpret_cast<uint32_t*>(&tile[q][off]) = x[q];
+        };
+        put(s.tri.N, n[0], n[1]);
+        put(s.tri.Nb, beta[i] * n[0], beta[i] * n[1]);
+        put(s.tri.M, m[0], m[1]);
+      }
+    // dX.V over the threads of a position (kRowGroups neighbours)
+#pragma unroll
+    for (int m = 1; m < kRowGroups; m <<= 1) dxv += __shfl_xor_sync(0xffffffffu, dxv, m);
+    if (loads && lg == 0) s.dxv[lc] = dxv;
+    dot = group_allreduce<32, 1>(dot);
+    if (lane == 0) s.sds[warp] = dot;
+    __syncthreads();
+    const uint32_t sk = smem_u32(s.k[0]), sq = smem_u32(s.q[0]);
+    const uint32_t tM = smem_u32(s.tri.M[0]), tN = smem_u32(s.tri.N[0]), tNb = smem_u32(s.tri.Nb[0]);
+    const int ct = quarter * NT;
+    float be[2];
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      const int i = row0 + g + 8 * r, c = 16 * quarter + 8 * j + 2 * t;
-      float n[2], m[2];
+      const int i = row0 + g + 8 * r;
+      const float eg = s.vec[i], la = s.vec[kC + i];
+      be[r] = beta[i];
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const float d =
-            i > c + e ? ex2((s.vec[3 * kC + i] - s.vec[3 * kC + c + e]) + (s.vec[4 * kC + i] - s.vec[4 * kC + c + e])) : 0.0f;
-        n[e] = i > c + e ? -d * XU[j][2 * r + e] : 0.0f;
-        m[e] = i > c + e ? p.scale * d * OU[j][2 * r + e] : 0.0f;
-        if (i == c + e) s.m[i] = p.scale * OU[j][2 * r + e];
-      }
-      const int off = tile_off<kC>(i, c >> 3) + 2 * t;
-      uint32_t x[3];
-      auto put = [&](__nv_bfloat16 (&tile)[3][kTri], float v0, float v1) {
-        split<3>(v0, v1, x);
+      for (int j = 0; j < NT; ++j)
 #pragma unroll
-        for (int q = 0; q < 3; ++q) *reinterpret_cast<uint32_t*>(&tile[q][off]) = x[q];
-      };
-      put(s.tri.N, n[0], n[1]);
-      put(s.tri.Nb, beta[i] * n[0], beta[i] * n[1]);
-      put(s.tri.M, m[0], m[1]);
+        for (int e = 2 * r; e < 2 * r + 2; ++e) {
+          E1[j][e] *= p.scale * eg;
+          E2[j][e] *= -eg;
+          E3[j][e] *= la;
+        }
     }
-  // dX.V over the threads of a position (kRowGroups neighbours)
+    // x.y of the warp's rows over its columns, y a tile in pieces
+    auto put_dot = [&](int which, const float (&c)[NT][4], const __nv_bfloat16* tile) {
+      float out[2] = {0.0f, 0.0f};
 #pragma unroll
-  for (int m = 1; m < kRowGroups; m <<= 1) dxv += __shfl_xor_sync(0xffffffffu, dxv, m);
-  if (loads && lg == 0) s.dxv[lc] = dxv;
-  dot = group_allreduce<32, 1>(dot);
-  if (lane == 0) s.sds[warp] = dot;
-  __syncthreads();
-  const uint32_t sk = smem_u32(s.k[0]), sq = smem_u32(s.q[0]);
-  const uint32_t tM = smem_u32(s.tri.M[0]), tN = smem_u32(s.tri.N[0]), tNb = smem_u32(s.tri.Nb[0]);
-  const int ct = quarter * NT;
-  float be[2];
+      for (int j = 0; j < NT; ++j)
 #pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    const int i = row0 + g + 8 * r;
-    const float eg = s.vec[i], la = s.vec[kC + i];
-    be[r] = beta[i];
+        for (int r = 0; r < 2; ++r) {
+          const int off = tile_off<DKP>(row0 + g + 8 * r, ct + j) + 2 * t;
 #pragma unroll
-    for (int j = 0; j < NT; ++j)
+          for (int i = 0; i < NP; ++i) {
+            const uint32_t x = *reinterpret_cast<const uint32_t*>(tile + i * (kC * DKP) + off);
+            out[r] = fmaf(lo_f32(x), c[j][2 * r], fmaf(hi_f32(x), c[j][2 * r + 1], out[r]));
+          }
+        }
 #pragma unroll
-      for (int e = 2 * r; e < 2 * r + 2; ++e) {
-        E1[j][e] *= p.scale * eg;
-        E2[j][e] *= -eg;
-        E3[j][e] *= la;
+      for (int r = 0; r < 2; ++r) {
+        out[r] += __shfl_xor_sync(0xffffffffu, out[r], 1);
+        out[r] += __shfl_xor_sync(0xffffffffu, out[r], 2);
+        if (t == 0) s.dots[which][quarter][row0 + g + 8 * r] = out[r];
       }
-  }
-  // x.y of the warp's rows over its columns, y a tile in pieces
-  auto put_dot = [&](int which, const float (&c)[NT][4], const __nv_bfloat16* tile) {
-    float out[2] = {0.0f, 0.0f};
+    };
+    put_dot(3, E3, s.k[0]);
+    // dQ = scale e^G E1 + M K
+    add_tile_product<NP, DKP>(E1, sk, ct, 0, w4 + 1, lane,
+                              [&](int kb, int i, uint32_t (&a)[4]) { load_a<kC>(a, tM + i * (kTri * 2), row0, kb, lane); });
+    put_dot(0, E1, s.q[0]);
+    // H = N K - e^G E2
+    add_tile_product<NP, DKP>(E2, sk, ct, 0, w4 + 1, lane,
+                              [&](int kb, int i, uint32_t (&a)[4]) { load_a<kC>(a, tN + i * (kTri * 2), row0, kb, lane); });
+    put_dot(1, E2, s.k[0]);
+    // C = N^T (beta K) + M^T Q + e^(G_last - G) E3
+    add_tile_product<NP, DKP>(E3, sk, ct, w4, kC / 16, lane,
+                              [&](int kb, int i, uint32_t (&a)[4]) { load_at<kC>(a, tNb + i * (kTri * 2), row0, kb, lane); });
+    add_tile_product<NP, DKP>(E3, sq, ct, w4, kC / 16, lane,
+                              [&](int kb, int i, uint32_t (&a)[4]) { load_at<kC>(a, tM + i * (kTri * 2), row0, kb, lane); });
+    put_dot(2, E3, s.k[0]);
+    // query and key gradients: to the tensors, or per value head where key heads are shared
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        const int off = tile_off<DKP>(row0 + g + 8 * r, ct + j) + 2 * t;
+        const int i = row0 + g + 8 * r, c = 8 * (ct + j) + 2 * t;
+        float kv[2] = {0.0f, 0.0f}, qv[2] = {0.0f, 0.0f};
 #pragma unroll
-        for (int i = 0; i < NP; ++i) {
-          const uint32_t x = *reinterpret_cast<const uint32_t*>(tile + i * (kC * DKP) + off);
-          out[r] = fmaf(lo_f32(x), c[j][2 * r], fmaf(hi_f32(x), c[j][2 * r + 1], out[r]));
+        for (int x = 0; x < NP; ++x) {
+          const int off = x * (kC * DKP) + tile_off<DKP>(i, ct + j) + 2 * t;
+          const uint32_t kx = *reinterpret_cast<const uint32_t*>(s.k[0] + off);
+          const uint32_t qx = *reinterpret_cast<const uint32_t*>(s.q[0] + off);
+          kv[0] += lo_f32(kx);
+          kv[1] += hi_f32(kx);
+          qv[0] += lo_f32(qx);
+          qv[1] += hi_f32(qx);
+        }
+        float dq[2], dk[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          dq[e] = fmaf(s.m[i], kv[e], E1[j][2 * r + e]);
+          dk[e] = fmaf(s.m[i], qv[e], fmaf(be[r], E2[j][2 * r + e], E3[j][2 * r + e]));
+        }
+        if (i >= rows || c >= p.dkw) continue;
+        if (p.group > 1) {
+          const size_t o = (((size_t)b * p.L + t0 + i) * p.Hv + h) * DKP + c;
+          *reinterpret_cast<float2*>(p.pdq + o) = make_float2(dq[0], dq[1]);
+          *reinterpret_cast<float2*>(p.pdk + o) = make_float2(dk[0], dk[1]);
+        } else {
+          T* dqp = static_cast<T*>(const_cast<void*>(p.dq.ptr)) + b * p.dq.sb + (t0 + i) * p.dq.sl + hk * p.dq.sh + c;
+          T* dkp = static_cast<T*>(const_cast<void*>(p.dk.ptr)) + b * p.dk.sb + (t0 + i) * p.dk.sl + hk * p.dk.sh + c;
+          dqp[0] = from_f32<T>(dq[0]);
+          dkp[0] = from_f32<T>(dk[0]);
+          if (c + 1 < p.dkw) {
+            dqp[1] = from_f32<T>(dq[1]);
+            dkp[1] = from_f32<T>(dk[1]);
+          }
         }
       }
+    __syncthreads();
+    if (warp == 0) {
+      float dG[2], tail = 0.0f;
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      out[r] += __shfl_xor_sync(0xffffffffu, out[r], 1);
-      out[r] += __shfl_xor_sync(0xffffffffu, out[r], 2);
-      if (t == 0) s.dots[which][quarter][row0 + g + 8 * r] = out[r];
-    }
-  };
-  put_dot(3, E3, s.k[0]);
-  // dQ = scale e^G E1 + M K
-  add_tile_product<NP, DKP>(E1, sk, ct, 0, w4 + 1, lane,
-                            [&](int kb, int i, uint32_t (&a)[4]) { load_a<kC>(a, tM + i * (kTri * 2), row0, kb, lane); });
-  put_dot(0, E1, s.q[0]);
-  // H = N K - e^G E2
-  add_tile_product<NP, DKP>(E2, sk, ct, 0, w4 + 1, lane,
-                            [&](int kb, int i, uint32_t (&a)[4]) { load_a<kC>(a, tN + i * (kTri * 2), row0, kb, lane); });
-  put_dot(1, E2, s.k[0]);
-  // C = N^T (beta K) + M^T Q + e^(G_last - G) E3
-  add_tile_product<NP, DKP>(E3, sk, ct, w4, kC / 16, lane,
-                            [&](int kb, int i, uint32_t (&a)[4]) { load_at<kC>(a, tNb + i * (kTri * 2), row0, kb, lane); });
-  add_tile_product<NP, DKP>(E3, sq, ct, w4, kC / 16, lane,
-                            [&](int kb, int i, uint32_t (&a)[4]) { load_at<kC>(a, tM + i * (kTri * 2), row0, kb, lane); });
-  put_dot(2, E3, s.k[0]);
-  // query and key gradients: to the tensors, or per value head where key heads are shared
-#pragma unroll
-  for (int j = 0; j < NT; ++j)
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const int i = row0 + g + 8 * r, c = 8 * (ct + j) + 2 * t;
-      float kv[2] = {0.0f, 0.0f}, qv[2] = {0.0f, 0.0f};
-#pragma unroll
-      for (int x = 0; x < NP; ++x) {
-        const int off = x * (kC * DKP) + tile_off<DKP>(i, ct + j) + 2 * t;
-        const uint32_t kx = *reinterpret_cast<const uint32_t*>(s.k[0] + off);
-        const uint32_t qx = *reinterpret_cast<const uint32_t*>(s.q[0] + off);
-        kv[0] += lo_f32(kx);
-        kv[1] += hi_f32(kx);
-        qv[0] += lo_f32(qx);
-        qv[1] += hi_f32(qx);
+      for (int i = 0; i < 2; ++i) {
+        const int r = 2 * lane + i;
+        auto sum = [&](int w) { return (s.dots[w][0][r] + s.dots[w][1][r]) + (s.dots[w][2][r] + s.dots[w][3][r]); };
+        const float kH = sum(1);
+        dG[i] = sum(0) + beta[r] * kH - sum(2);
+        tail += sum(3);
+        if (r < rows) p.dbeta[((size_t)b * p.L + t0 + r) * p.Hv + h] = s.dxv[r] + kH;
       }
-      float dq[2], dk[2];
+      tail = group_allreduce<32, 1>(tail);
+      float sds = 0.0f;
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        dq[e] = fmaf(s.m[i], kv[e], E1[j][2 * r + e]);
-        dk[e] = fmaf(s.m[i], qv[e], fmaf(be[r], E2[j][2 * r + e], E3[j][2 * r + e]));
+      for (int i = 0; i < 16; ++i) sds += s.sds[i];
+      tail = fmaf(s.vec[kC - 1], sds, tail);
+      float run = dG[0] + dG[1];
+#pragma unroll
+      for (int m = 1; m < 32; m <<= 1) {
+        const float down = __shfl_down_sync(0xffffffffu, run, m);
+        if (lane + m < 32) run += down;
       }
-      if (i >= rows || c >= p.dkw) continue;
-      if (p.group > 1) {
-        const size_t o = (((size_t)b * p.L + t0 + i) * p.Hv + h) * DKP + c;
-        *reinterpret_cast<float2*>(p.pdq + o) = make_float2(dq[0], dq[1]);
-        *reinterpret_cast<float2*>(p.pdk + o) = make_float2(dk[0], dk[1]);
-      } else {
-        T* dqp = static_cast<T*>(const_cast<void*>(p.dq.ptr)) + b * p.dq.sb + (t0 + i) * p.dq.sl + hk * p.dq.sh + c;
-        T* dkp = static_cast<T*>(const_cast<void*>(p.dk.ptr)) + b * p.dk.sb + (t0 + i) * p.dk.sl + hk * p.dk.sh + c;
-        dqp[0] = from_f32<T>(dq[0]);
-        dkp[0] = from_f32<T>(dk[0]);
-        if (c + 1 < p.dkw) {
-          dqp[1] = from_f32<T>(dq[1]);
-          dkp[1] = from_f32<T>(dk[1]);
-        }
-      }
+      run += tail;
+      if (2 * lane < rows) p.dg[((size_t)b * p.L + t0 + 2 * lane) * p.Hv + h] = run;
+      if (2 * lane + 1 < rows) p.dg[((size_t)b * p.L + t0 + 2 * lane + 1) * p.Hv + h] = run - dG[0];
     }
-  __syncthreads();
-  if (warp == 0) {
-    float dG[2], tail = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int r = 2 * lane + i;
-      auto sum = [&](int w) { return (s.dots[w][0][r] + s.dots[w][1][r]) + (s.dots[w][2][r] + s.dots[w][3][r]); };
-      const float kH = sum(1);
-      dG[i] = sum(0) + beta[r] * kH - sum(2);
-      tail += sum(3);
-      if (r < rows) p.dbeta[((size_t)b * p.L + t0 + r) * p.Hv + h] = s.dxv[r] + kH;
-    }
-    tail = group_allreduce<32, 1>(tail);
-    float sds = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) sds += s.sds[i];
-    tail = fmaf(s.vec[kC - 1], sds, tail);
-    float run = dG[0] + dG[1];
-#pragma unroll
-    for (int m = 1; m < 32; m <<= 1) {
-      const float down = __shfl_down_sync(0xffffffffu, run, m);
-      if (lane + m < 32) run += down;
-    }
-    run += tail;
-    if (2 * lane < rows) p.dg[((size_t)b * p.L + t0 + 2 * lane) * p.Hv + h] = run;
-    if (2 * lane + 1 < rows) p.dg[((size_t)b * p.L + t0 + 2 * lane + 1) * p.Hv + h] = run - dG[0];
+    __syncthreads();              // the next item writes over all of this
   }
 }
 
@@ -1239,7 +1259,7 @@ int check_shape(const Shape& s) {
     return fail(SSM_ERR_INVALID, "gated delta rule: %lld value heads are not a multiple of %lld key heads",
                 (long long)s.Hv, (long long)s.Hk);
   if (s.dk > 128) return fail(SSM_ERR_UNSUPPORTED, "gated delta rule: key width %lld above 128", (long long)s.dk);
-  if (s.B > 65535 || s.Hv > 65535 || s.dv > (1 << 20) || s.L > (1LL << 30))
+  if (s.B > 65535 || s.Hv > 65535 || s.dv > (1 << 20) || s.L > (1LL << 30) || s.B * s.Hv * s.n() > (1LL << 31) - 1024)
     return fail(SSM_ERR_INVALID, "gated delta rule: shape out of range (B=%lld, L=%lld)", (long long)s.B, (long long)s.L);
   if (s.dtype != SSM_F32 && s.dtype != SSM_BF16) return fail(SSM_ERR_DTYPE, "gated delta rule: dtype %d unsupported", s.dtype);
   return SSM_OK;
@@ -1312,13 +1332,10 @@ void fill(DeltaParams& p, const Shape& s, ssm_heads q, ssm_heads k, ssm_heads v,
   p.err = device_error_word();
 }
 
-template <typename K>
-cudaError_t launch(K kern, dim3 grid, int threads, size_t smem, const DeltaParams& p, cudaStream_t st) {
-  if (smem > 48 * 1024) {
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return e;
-  }
-  kern<<<grid, threads, smem, st>>>(p);
+template <auto Kern>
+cudaError_t launch(dim3 grid, int threads, size_t smem, const DeltaParams& p, cudaStream_t st) {
+  if (smem > 48 * 1024) ctas_per_sm<Kern>(threads, smem);
+  Kern<<<grid, threads, smem, st>>>(p);
   return cudaGetLastError();
 }
 
@@ -1332,14 +1349,14 @@ cudaError_t run_chain_ns(const Shape& s, const DeltaParams& p, bool bwd, cudaStr
     using Form = BwdChain<T, NP, DKP, NS>;
     constexpr size_t smem = sizeof(typename Form::template Smem<Form::KB>);
     if constexpr (smem > 227 * 1024) return cudaErrorInvalidValue;
-    else return launch(delta_bwd_chain<T, NP, DKP, NS>, grid, threads, smem, p, st);
+    else return launch<delta_bwd_chain<T, NP, DKP, NS>>(grid, threads, smem, p, st);
   } else {
     using Form = FwdChain<T, NP, DKP, NS>;
     constexpr size_t smem = sizeof(typename Form::template Smem<Form::KB>);
     if constexpr (smem > 227 * 1024) return cudaErrorInvalidValue;
     else
-      return p.states != nullptr ? launch(delta_fwd<T, NP, DKP, NS, true>, grid, threads, smem, p, st)
-                                 : launch(delta_fwd<T, NP, DKP, NS, false>, grid, threads, smem, p, st);
+      return p.states != nullptr ? launch<delta_fwd<T, NP, DKP, NS, true>>(grid, threads, smem, p, st)
+                                 : launch<delta_fwd<T, NP, DKP, NS, false>>(grid, threads, smem, p, st);
   }
 }
 template <typename T, int NP, int DKP>
@@ -1356,7 +1373,7 @@ cudaError_t run_chain(const Shape& s, const DeltaParams& p, bool bwd, cudaStream
 template <typename T, int NP, int DKP>
 cudaError_t run_prep_and_chain(const Shape& s, const DeltaParams& p, bool bwd, cudaStream_t st) {
   const dim3 grid((unsigned)s.n(), (unsigned)s.Hv, (unsigned)s.B);
-  const cudaError_t e = launch(delta_prep<T, NP, DKP>, grid, 128, sizeof(PrepSmem<NP, DKP>), p, st);
+  const cudaError_t e = launch<delta_prep<T, NP, DKP>>(grid, 128, sizeof(PrepSmem<NP, DKP>), p, st);
   if (e != cudaSuccess) return e;
   return run_chain<T, NP, DKP>(s, p, bwd, st);
 }
@@ -1365,13 +1382,13 @@ template <typename T, int NP, int DKP>
 cudaError_t run_bwd(const Shape& s, const DeltaParams& p, cudaStream_t st) {
   cudaError_t e = run_prep_and_chain<T, NP, DKP>(s, p, true, st);
   if (e != cudaSuccess) return e;
-  const dim3 grid((unsigned)s.n(), (unsigned)s.Hv, (unsigned)s.B);
   constexpr int SL = NP == 3 && DKP == 128 ? 16 : 32;     // what shared memory holds beside six tiles of pieces
-  e = launch(delta_bwd_chunk<T, NP, DKP, SL>, grid, 512, sizeof(BwdSmem<NP, DKP, SL>), p, st);
+  const dim3 bg((unsigned)std::min<int64_t>(s.n() * s.Hv * s.B, 148));       // one CTA per SM walks over the chunks
+  e = launch<delta_bwd_chunk<T, NP, DKP, SL>>(bg, 512, sizeof(BwdSmem<NP, DKP, SL>), p, st);
   if (e != cudaSuccess || p.group == 1) return e;
   constexpr int per = 256 / (DKP / 4);
   const dim3 sg((unsigned)(((long long)p.B * p.L + per - 1) / per), (unsigned)p.Hk);
-  return launch(delta_sum_heads<T, DKP>, sg, 256, 0, p, st);
+  return launch<delta_sum_heads<T, DKP>>(sg, 256, 0, p, st);
 }
 
 }  // namespace
@@ -1495,8 +1512,8 @@ int ssm_gated_delta_state_update(int64_t B, int64_t Hk, int64_t Hv, int64_t dk, 
   p.last = state;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const dim3 grid((unsigned)((dv + 31) / 32), (unsigned)Hv, (unsigned)B);
-  const cudaError_t e = s.dtype == SSM_BF16 ? launch(delta_step<__nv_bfloat16>, grid, 256, 0, p, st)
-                                            : launch(delta_step<float>, grid, 256, 0, p, st);
+  const cudaError_t e = s.dtype == SSM_BF16 ? launch<delta_step<__nv_bfloat16>>(grid, 256, 0, p, st)
+                                            : launch<delta_step<float>>(grid, 256, 0, p, st);
   if (e != cudaSuccess) return fail(SSM_ERR_CUDA, "gated delta state update: %s", cudaGetErrorString(e));
   return SSM_OK;
 }

@@ -24,6 +24,7 @@
 #include <initializer_list>
 
 #include "ssm_b200.h"
+#include "ssm_launch.cuh"
 #include "ssm_vec.cuh"
 
 namespace ssm {
@@ -36,7 +37,6 @@ using ssm::vec_load;
 using ssm::vec_store;
 
 constexpr int kWarps = 8;           // warps per CTA: rows taken side by side
-constexpr int kTargetCtas = 148 * 4;
 
 struct NormParams {
   const void *x, *z, *dy;
@@ -58,30 +58,55 @@ struct NormParams {
 
 __device__ __forceinline__ float dsilu(float z, float s) { return s * fmaf(z, 1.0f - s, 1.0f); }
 
-// y from the normalised value
-__device__ __forceinline__ float norm_out(const NormParams& p, float n, float w, float b, float z) {
-  float a = fmaf(n, w, b);
-  if (p.silu) a *= ssm::sigmoid(a);
-  return p.gate ? a * (z * ssm::sigmoid(z)) : a;
-}
-// e = d loss / d (n w + b), and dz
-__device__ __forceinline__ float norm_grad(const NormParams& p, float n, float w, float b, float z, float dy,
-                                           float& dz) {
-  const float pre = fmaf(n, w, b);
-  float a = pre, e = dy;
+// y from the normalised values.  The activation and the gate are branched on once per vector, not per element
+// (per element they made 39 instructions of 13).
+template <int VEC>
+__device__ __forceinline__ void norm_out(const NormParams& p, const float (&n)[VEC], const float (&w)[VEC],
+                                         const float (&b)[VEC], const float (&z)[VEC], float (&y)[VEC]) {
+#pragma unroll
+  for (int v = 0; v < VEC; ++v) y[v] = fmaf(n[v], w[v], b[v]);
   if (p.silu) {
-    const float s = ssm::sigmoid(pre);
-    a = pre * s;
-    e *= dsilu(pre, s);
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) y[v] *= ssm::sigmoid(y[v]);
   }
   if (p.gate) {
-    const float s = ssm::sigmoid(z);
-    e *= z * s;
-    dz = dy * a * dsilu(z, s);
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) y[v] *= z[v] * ssm::sigmoid(z[v]);
   }
-  return e;
+}
+// e = d loss / d (n w + b) in dy's place, and dz in z's.
+template <int VEC>
+__device__ __forceinline__ void norm_grad(const NormParams& p, const float (&n)[VEC], const float (&w)[VEC],
+                                          const float (&b)[VEC], float (&z)[VEC], float (&dy)[VEC]) {
+  float a[VEC], d[VEC];                  // act and act' of n w + b
+#pragma unroll
+  for (int v = 0; v < VEC; ++v) {
+    a[v] = fmaf(n[v], w[v], b[v]);
+    d[v] = 1.0f;
+  }
+  if (p.silu) {
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) {
+      const float s = ssm::sigmoid(a[v]);
+      d[v] = dsilu(a[v], s);
+      a[v] *= s;
+    }
+  }
+  if (p.gate) {
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) {
+      const float s = ssm::sigmoid(z[v]), g = dy[v];
+      dy[v] = g * (z[v] * s);
+      z[v] = g * a[v] * dsilu(z[v], s);
+    }
+  }
+  if (p.silu) {
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) dy[v] *= d[v];
+  }
 }
 
+// weight and bias of VEC channels from c on (both arrays may start anywhere)
 template <int VEC>
 __device__ __forceinline__ void load_params(const NormParams& p, long long c, float (&w)[VEC], float (&b)[VEC]) {
 #pragma unroll
@@ -185,35 +210,82 @@ __device__ __forceinline__ float row_stats(const NormParams& p, const Place<WPG>
   return rsqrtf(fmaf(group_sum<WPG>(q, at.lpg), inv, p.eps));
 }
 
+// Rows ahead of the one in work: kDepth rows of every tensor, copied asynchronously into slots of shared memory
+// that only the thread itself reads, so no barrier is needed and depth costs no registers.  (A prefetch of one
+// row in registers kept 22 KB per SM in flight and reached half the bandwidth.)
+template <typename T, int VEC, int K, bool BWD>
+struct RowQueue {
+  using Vec = ssm::Raw<T, VEC>;
+  static constexpr int kTensors = BWD ? 3 : 2, kRow = kTensors * K * 32 * kWarps * (int)sizeof(Vec);
+  static constexpr int kDepth = kRow * 4 <= 48 * 1024 ? 4 : 2;
+  static constexpr size_t kBytes = (size_t)kDepth * kRow;
+  Vec* slots;
+  int tid;
+  __device__ RowQueue(unsigned char* smem) : slots(reinterpret_cast<Vec*>(smem)), tid(threadIdx.y * 32 + threadIdx.x) {}
+  __device__ Vec* slot(int stage, int tensor, int i) { return slots + ((stage * kTensors + tensor) * K + i) * 32 * kWarps + tid; }
+  __device__ void copy(Vec* dst, const T* src, bool ok) {
+    if constexpr (sizeof(Vec) >= 4) {
+      asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(ssm::smem_u32(dst)), "l"(src),
+                   "n"((int)sizeof(Vec)), "r"(ok ? (int)sizeof(Vec) : 0)
+                   : "memory");
+    } else {
+      if (ok) dst->load(src);
+      else dst->zero();
+    }
+  }
+  template <int WPG>
+  __device__ void fetch(const NormParams& p, const Place<WPG>& at, long long r, int stage) {
+#pragma unroll
+    for (int i = 0; i < K; ++i) {
+      const int c = (at.lane + i * at.lpg) * VEC;
+      const bool ok = at.live && r < p.N && c < p.cg;
+      const long long rr = ok ? r : 0, cc = ok ? at.c0 + c : 0;
+      copy(slot(stage, 0, i), static_cast<const T*>(p.x) + rr * p.xs + cc, ok);
+      if (p.gate) copy(slot(stage, 1, i), static_cast<const T*>(p.z) + rr * p.zs + cc, ok);
+      if (BWD) copy(slot(stage, 2, i), static_cast<const T*>(p.dy) + rr * p.gs + cc, ok);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  }
+  __device__ void wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory"); }
+};
+
 // The number of rows is the same for all of a CTA's warps, so that group_sum's barriers match; rows past
 // the end work on zeros.
 template <typename T, int VEC, int K, int WPG>
-__global__ void __launch_bounds__(32 * kWarps) norm_rows_fwd(const NormParams p, int lpg) {
+__global__ void __launch_bounds__(32 * kWarps) norm_rows_fwd(const __grid_constant__ NormParams p, int lpg) {
+  extern __shared__ __align__(16) unsigned char smem[];
   const Place<WPG> at(p, lpg);
+  RowQueue<T, VEC, K, false> queue(smem);
+#pragma unroll
+  for (int d = 0; d < queue.kDepth; ++d) queue.fetch(p, at, at.row + d * at.step, d);
+  float w[K][VEC], b[K][VEC];
+#pragma unroll
+  for (int i = 0; i < K; ++i) {
+    const int c = (at.lane + i * at.lpg) * VEC;
+    if (at.live && c < p.cg) load_params<VEC>(p, at.c0 + c, w[i], b[i]);
+  }
+  int stage = 0;
   for (long long r0 = 0; r0 < p.N; r0 += at.step) {
     const long long r = r0 + at.row;
     if (WPG > 1 && r >= p.N) return;
     float x[K][VEC], z[K][VEC];
-    const bool ok = at.live && r < p.N;
+    queue.wait();
 #pragma unroll
     for (int i = 0; i < K; ++i) {
-      const int c = (at.lane + i * at.lpg) * VEC;
-#pragma unroll
-      for (int v = 0; v < VEC; ++v) x[i][v] = z[i][v] = 0.0f;
-      if (ok && c < p.cg) {
-        vec_load<T, VEC>(static_cast<const T*>(p.x) + r * p.xs + at.c0 + c, x[i]);
-        if (p.gate) vec_load<T, VEC>(static_cast<const T*>(p.z) + r * p.zs + at.c0 + c, z[i]);
-      }
+      queue.slot(stage, 0, i)->widen(x[i]);
+      if (p.gate) queue.slot(stage, 1, i)->widen(z[i]);
     }
+    queue.fetch(p, at, r + queue.kDepth * at.step, stage);
+    stage = stage + 1 == queue.kDepth ? 0 : stage + 1;
     const float rstd = row_stats<WPG, VEC, K>(p, at, x);
 #pragma unroll
     for (int i = 0; i < K; ++i) {
       const int c = (at.lane + i * at.lpg) * VEC;
-      if (ok && c < p.cg) {
-        float w[VEC], b[VEC], o[VEC];
-        load_params<VEC>(p, at.c0 + c, w, b);
+      if (at.live && r < p.N && c < p.cg) {
+        float o[VEC];
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) o[v] = norm_out(p, x[i][v] * rstd, w[v], b[v], z[i][v]);
+        for (int v = 0; v < VEC; ++v) x[i][v] *= rstd;
+        norm_out(p, x[i], w[i], b[i], z[i], o);
         vec_store<T, VEC>(static_cast<T*>(p.y) + r * p.ys + at.c0 + c, o);
       }
     }
@@ -222,8 +294,12 @@ __global__ void __launch_bounds__(32 * kWarps) norm_rows_fwd(const NormParams p,
 
 // Parameter gradients stay in registers over a CTA's rows; WPG = 1 adds its warps' at the end.
 template <typename T, int VEC, int K, int WPG>
-__global__ void __launch_bounds__(32 * kWarps) norm_rows_bwd(const NormParams p, int lpg) {
+__global__ void __launch_bounds__(32 * kWarps) norm_rows_bwd(const __grid_constant__ NormParams p, int lpg) {
+  extern __shared__ __align__(16) unsigned char smem[];
   const Place<WPG> at(p, lpg);
+  RowQueue<T, VEC, K, true> queue(smem);
+#pragma unroll
+  for (int d = 0; d < queue.kDepth; ++d) queue.fetch(p, at, at.row + d * at.step, d);
   const float inv = 1.0f / (float)p.cg;
   float dw[K][VEC], db[K][VEC], w[K][VEC], b[K][VEC];
 #pragma unroll
@@ -233,38 +309,37 @@ __global__ void __launch_bounds__(32 * kWarps) norm_rows_bwd(const NormParams p,
     for (int v = 0; v < VEC; ++v) dw[i][v] = db[i][v] = w[i][v] = b[i][v] = 0.0f;
     if (at.live && c < p.cg) load_params<VEC>(p, at.c0 + c, w[i], b[i]);
   }
+  int stage = 0;
   for (long long r0 = 0; r0 < p.N; r0 += at.step) {
     const long long r = r0 + at.row;
     if (WPG > 1 && r >= p.N) break;
     const bool ok = at.live && r < p.N;
     float x[K][VEC], z[K][VEC], g[K][VEC];
+    queue.wait();
 #pragma unroll
     for (int i = 0; i < K; ++i) {
-      const int c = (at.lane + i * at.lpg) * VEC;
-#pragma unroll
-      for (int v = 0; v < VEC; ++v) x[i][v] = z[i][v] = g[i][v] = 0.0f;
-      if (ok && c < p.cg) {
-        vec_load<T, VEC>(static_cast<const T*>(p.x) + r * p.xs + at.c0 + c, x[i]);
-        vec_load<T, VEC>(static_cast<const T*>(p.dy) + r * p.gs + at.c0 + c, g[i]);
-        if (p.gate) vec_load<T, VEC>(static_cast<const T*>(p.z) + r * p.zs + at.c0 + c, z[i]);
-      }
+      queue.slot(stage, 0, i)->widen(x[i]);
+      if (p.gate) queue.slot(stage, 1, i)->widen(z[i]);
+      queue.slot(stage, 2, i)->widen(g[i]);
     }
+    queue.fetch(p, at, r + queue.kDepth * at.step, stage);
+    stage = stage + 1 == queue.kDepth ? 0 : stage + 1;
     const float rstd = row_stats<WPG, VEC, K>(p, at, x);
     float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
-    for (int i = 0; i < K; ++i)
+    for (int i = 0; i < K; ++i) {
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) x[i][v] *= rstd;
+      norm_grad(p, x[i], w[i], b[i], z[i], g[i]);
 #pragma unroll
       for (int v = 0; v < VEC; ++v) {
-        x[i][v] *= rstd;
-        float dz = 0.0f;
-        const float e = norm_grad(p, x[i][v], w[i][v], b[i][v], z[i][v], g[i][v], dz);
-        z[i][v] = dz;
-        dw[i][v] = fmaf(e, x[i][v], dw[i][v]);
-        db[i][v] += e;
-        g[i][v] = e * w[i][v];
+        dw[i][v] = fmaf(g[i][v], x[i][v], dw[i][v]);
+        db[i][v] += g[i][v];
+        g[i][v] *= w[i][v];
         s1 += g[i][v];
         s2 = fmaf(g[i][v], x[i][v], s2);
       }
+    }
     s1 = p.center ? group_sum<WPG>(s1, at.lpg) * inv : 0.0f;
     s2 = group_sum<WPG>(s2, at.lpg) * inv;
 #pragma unroll
@@ -311,7 +386,7 @@ __global__ void __launch_bounds__(32 * kWarps) norm_rows_bwd(const NormParams p,
 
 // ---- one position per sample, groups too wide for registers: a warp per (sample, group) ------
 template <typename T, bool BWD>
-__global__ void __launch_bounds__(256) norm_group_sums(const NormParams p) {
+__global__ void __launch_bounds__(256) norm_group_sums(const __grid_constant__ NormParams p) {
   const long long i = ((long long)blockIdx.x * 256 + threadIdx.x) >> 5;
   const int lane = threadIdx.x & 31;
   if (i >= p.N * p.G) return;
@@ -337,12 +412,13 @@ __global__ void __launch_bounds__(256) norm_group_sums(const NormParams p) {
     const float2 st = *reinterpret_cast<const float2*>(p.stats + i * 2);
     float s1 = 0.0f, s2 = 0.0f;
     for (int j = lane; j < p.cg; j += 32) {
-      float w[1], b[1], dz;
+      float w[1], b[1], e[1] = {ssm::to_f32(dy[j])}, zj[1] = {p.gate ? ssm::to_f32(z[j]) : 0.0f};
       load_params<1>(p, c0 + j, w, b);
-      const float nn = (ssm::to_f32(x[j]) - st.x) * st.y;
-      const float e = norm_grad(p, nn, w[0], b[0], p.gate ? ssm::to_f32(z[j]) : 0.0f, ssm::to_f32(dy[j]), dz) * w[0];
-      s1 += e;
-      s2 = fmaf(e, nn, s2);
+      const float n1[1] = {(ssm::to_f32(x[j]) - st.x) * st.y};
+      norm_grad(p, n1, w, b, zj, e);
+      e[0] *= w[0];
+      s1 += e[0];
+      s2 = fmaf(e[0], n1[0], s2);
     }
     s1 = ssm::group_allreduce<32, 1>(s1);
     s2 = ssm::group_allreduce<32, 1>(s2);
@@ -373,7 +449,7 @@ __device__ __forceinline__ long long row_at(long long n, long long r, long long 
 // Per (sample, slab, channel): mean and sum of squared deviations of the slab's rows, summed about the
 // slab's first row so that a large common offset costs no digits.
 template <typename T, int VEC>
-__global__ void __launch_bounds__(32 * kWarps) norm_col_stats(const NormParams p) {
+__global__ void __launch_bounds__(32 * kWarps) norm_col_stats(const __grid_constant__ NormParams p) {
   const long long c = ((long long)blockIdx.y * 32 + threadIdx.x) * VEC;
   const bool live = c < p.C;
   const Rows s = rows_of<false>(p);
@@ -418,36 +494,49 @@ __global__ void __launch_bounds__(32 * kWarps) norm_col_stats(const NormParams p
   }
 }
 
-// A warp per (sample, group): mean and rstd from the slabs' per-channel means and squared deviations.
-__global__ void __launch_bounds__(256) norm_combine_stats(const NormParams p) {
-  const long long i = ((long long)blockIdx.x * 256 + threadIdx.x) >> 5;
-  const int lane = threadIdx.x & 31;
-  if (i >= p.N * p.G) return;
-  const long long n = i / p.G, c0 = (i % p.G) * p.cg;
-  const long long cells = (long long)p.nslab * p.cg;
+// Sum of a double over a CTA of 128 threads, in a fixed order, to all of them.
+__device__ __forceinline__ double cta_sum(double x) {
+  __shared__ double red[4];
+  for (int k = 16; k >= 1; k >>= 1) x += __shfl_xor_sync(0xffffffffu, x, k);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = x;
+  __syncthreads();
+  return (red[0] + red[1]) + (red[2] + red[3]);
+}
+// f(slab, channel of the group) for this thread's share of a sample's slabs x a group's channels.
+template <typename F>
+__device__ __forceinline__ void for_cells(const NormParams& p, F f) {
+  const int cells = p.nslab * p.cg;
+#pragma unroll 4
+  for (int e = threadIdx.x; e < cells; e += 128) f(e / p.cg, e % p.cg);
+}
+
+// A CTA per (sample, group): mean and rstd from the slabs' per-channel means and squared deviations.
+__global__ void __launch_bounds__(128) norm_combine_stats(const __grid_constant__ NormParams p) {
+  const long long n = blockIdx.x / p.G;
+  const float* part = p.part + n * p.nslab * 2 * p.C + (long long)(blockIdx.x % p.G) * p.cg;
   const double m = (double)p.P * p.cg;
-  double mean = 0.0, q = 0.0;
-  auto at = [&](long long e) { return ((n * p.nslab + e / p.cg) * 2) * p.C + c0 + e % p.cg; };
-  auto rows = [&](long long e) {
-    const long long r0 = e / p.cg * p.slab;
+  auto rows = [&](int slab) {
+    const long long r0 = slab * p.slab;
     return (double)((r0 + p.slab < p.P ? r0 + p.slab : p.P) - r0);
   };
+  double mean = 0.0, q = 0.0;
   if (p.center) {
-    for (long long e = lane; e < cells; e += 32) mean += rows(e) * p.part[at(e)];
-    for (int k = 16; k >= 1; k >>= 1) mean += __shfl_xor_sync(0xffffffffu, mean, k);
-    mean /= m;
+    for_cells(p, [&](int slab, int c) { mean += rows(slab) * part[(long long)slab * 2 * p.C + c]; });
+    mean = cta_sum(mean) / m;
   }
-  for (long long e = lane; e < cells; e += 32) {
-    const double d = p.part[at(e)] - mean;
-    q += p.part[at(e) + p.C] + rows(e) * d * d;
-  }
-  for (int k = 16; k >= 1; k >>= 1) q += __shfl_xor_sync(0xffffffffu, q, k);
-  if (lane == 0)
-    *reinterpret_cast<float2*>(p.stats + i * 2) = make_float2((float)mean, (float)(1.0 / sqrt(q / m + (double)p.eps)));
+  for_cells(p, [&](int slab, int c) {
+    const float* at = part + (long long)slab * 2 * p.C + c;
+    const double d = at[0] - mean;
+    q += at[p.C] + rows(slab) * d * d;
+  });
+  q = cta_sum(q);
+  if (threadIdx.x == 0)
+    *reinterpret_cast<float2*>(p.stats + blockIdx.x * 2LL) = make_float2((float)mean, (float)(1.0 / sqrt(q / m + (double)p.eps)));
 }
 
 template <typename T, int VEC, bool ROWS>
-__global__ void __launch_bounds__(32 * kWarps) norm_apply_fwd(const NormParams p) {
+__global__ void __launch_bounds__(32 * kWarps) norm_apply_fwd(const __grid_constant__ NormParams p) {
   const long long c = ((long long)blockIdx.y * 32 + threadIdx.x) * VEC;
   if (c >= p.C) return;
   const Rows s = rows_of<ROWS>(p);
@@ -464,19 +553,20 @@ __global__ void __launch_bounds__(32 * kWarps) norm_apply_fwd(const NormParams p
   if (!ROWS) stats(s.n);
 #pragma unroll 4
   for (long long r = s.r0 + threadIdx.y; r < s.r1; r += kWarps) {
-    float x[VEC], z[VEC], o[VEC];
+    float x[VEC], z[VEC] = {}, o[VEC];
     vec_load<T, VEC>(static_cast<const T*>(p.x) + row_at<ROWS>(s.n, r, p.xs, p.xp) + c, x);
     if (p.gate) vec_load<T, VEC>(static_cast<const T*>(p.z) + row_at<ROWS>(s.n, r, p.zs, p.zp) + c, z);
     if (ROWS) stats(r);
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) o[v] = norm_out(p, (x[v] - mean[v]) * rstd[v], w[v], b[v], p.gate ? z[v] : 0.0f);
+    for (int v = 0; v < VEC; ++v) x[v] = (x[v] - mean[v]) * rstd[v];
+    norm_out(p, x, w, b, z, o);
     vec_store<T, VEC>(static_cast<T*>(p.y) + row_at<ROWS>(s.n, r, p.ys, p.yp) + c, o);
   }
 }
 
 // Per (sample, slab, channel) (ROWS: per (slab, channel)): sums of e n and of e.
 template <typename T, int VEC, bool ROWS>
-__global__ void __launch_bounds__(32 * kWarps) norm_col_grads(const NormParams p) {
+__global__ void __launch_bounds__(32 * kWarps) norm_col_grads(const __grid_constant__ NormParams p) {
   const long long c = ((long long)blockIdx.y * 32 + threadIdx.x) * VEC;
   const bool live = c < p.C;
   const Rows s = rows_of<ROWS>(p);
@@ -496,48 +586,44 @@ __global__ void __launch_bounds__(32 * kWarps) norm_col_grads(const NormParams p
     if (!ROWS) stats(s.n);
 #pragma unroll 2
     for (long long r = s.r0 + threadIdx.y; r < s.r1; r += kWarps) {
-      float x[VEC], z[VEC], g[VEC], dz;
+      float x[VEC], z[VEC] = {}, g[VEC];
       vec_load<T, VEC>(static_cast<const T*>(p.x) + row_at<ROWS>(s.n, r, p.xs, p.xp) + c, x);
       vec_load<T, VEC>(static_cast<const T*>(p.dy) + row_at<ROWS>(s.n, r, p.gs, p.gp) + c, g);
       if (p.gate) vec_load<T, VEC>(static_cast<const T*>(p.z) + row_at<ROWS>(s.n, r, p.zs, p.zp) + c, z);
       if (ROWS) stats(r);
 #pragma unroll
+      for (int v = 0; v < VEC; ++v) x[v] = (x[v] - mean[v]) * rstd[v];
+      norm_grad(p, x, w, b, z, g);
+#pragma unroll
       for (int v = 0; v < VEC; ++v) {
-        const float n = (x[v] - mean[v]) * rstd[v];
-        const float e = norm_grad(p, n, w[v], b[v], p.gate ? z[v] : 0.0f, g[v], dz);
-        dw[v] = fmaf(e, n, dw[v]);
-        db[v] += e;
+        dw[v] = fmaf(g[v], x[v], dw[v]);
+        db[v] += g[v];
       }
     }
   }
   write_partials<VEC>(p.part, blockIdx.x, p.C, c, live, dw, db);
 }
 
-// A warp per (sample, group): s1 / M and s2 / M from the channels' sums.
-__global__ void __launch_bounds__(256) norm_combine_sums(const NormParams p) {
-  const long long i = ((long long)blockIdx.x * 256 + threadIdx.x) >> 5;
-  const int lane = threadIdx.x & 31;
-  if (i >= p.N * p.G) return;
-  const long long n = i / p.G, c0 = (i % p.G) * p.cg;
-  const long long cells = (long long)p.nslab * p.cg;
+// A CTA per (sample, group): s1 / M and s2 / M from the channels' sums.
+__global__ void __launch_bounds__(128) norm_combine_sums(const __grid_constant__ NormParams p) {
+  const long long n = blockIdx.x / p.G, c0 = (long long)(blockIdx.x % p.G) * p.cg;
+  const float* part = p.part + n * p.nslab * 2 * p.C + c0;
   double s1 = 0.0, s2 = 0.0;
-  for (long long e = lane; e < cells; e += 32) {
-    const long long c = c0 + e % p.cg, o = ((n * p.nslab + e / p.cg) * 2) * p.C + c;
-    const double w = p.w != nullptr ? p.w[c] : 1.0f;
-    s2 += w * p.part[o];
-    s1 += w * p.part[o + p.C];
-  }
-  for (int k = 16; k >= 1; k >>= 1) {
-    s1 += __shfl_xor_sync(0xffffffffu, s1, k);
-    s2 += __shfl_xor_sync(0xffffffffu, s2, k);
-  }
+  for_cells(p, [&](int slab, int c) {
+    const float* at = part + (long long)slab * 2 * p.C + c;
+    const double w = p.w != nullptr ? p.w[c0 + c] : 1.0f;
+    s2 += w * at[0];
+    s1 += w * at[p.C];
+  });
+  s2 = cta_sum(s2);
+  s1 = cta_sum(s1);
   const double m = (double)p.P * p.cg;
-  if (lane == 0)
-    *reinterpret_cast<float2*>(p.sums + i * 2) = make_float2(p.center ? (float)(s1 / m) : 0.0f, (float)(s2 / m));
+  if (threadIdx.x == 0)
+    *reinterpret_cast<float2*>(p.sums + blockIdx.x * 2LL) = make_float2(p.center ? (float)(s1 / m) : 0.0f, (float)(s2 / m));
 }
 
 template <typename T, int VEC, bool ROWS>
-__global__ void __launch_bounds__(32 * kWarps) norm_apply_bwd(const NormParams p) {
+__global__ void __launch_bounds__(32 * kWarps) norm_apply_bwd(const __grid_constant__ NormParams p) {
   const long long c = ((long long)blockIdx.y * 32 + threadIdx.x) * VEC;
   if (c >= p.C) return;
   const Rows s = rows_of<ROWS>(p);
@@ -558,25 +644,24 @@ __global__ void __launch_bounds__(32 * kWarps) norm_apply_bwd(const NormParams p
   if (!ROWS) stats(s.n);
 #pragma unroll 2
   for (long long r = s.r0 + threadIdx.y; r < s.r1; r += kWarps) {
-    float x[VEC], z[VEC], g[VEC], dz[VEC], o[VEC];
+    float x[VEC], z[VEC] = {}, g[VEC], o[VEC];
     vec_load<T, VEC>(static_cast<const T*>(p.x) + row_at<ROWS>(s.n, r, p.xs, p.xp) + c, x);
     vec_load<T, VEC>(static_cast<const T*>(p.dy) + row_at<ROWS>(s.n, r, p.gs, p.gp) + c, g);
     if (p.gate) vec_load<T, VEC>(static_cast<const T*>(p.z) + row_at<ROWS>(s.n, r, p.zs, p.zp) + c, z);
     if (ROWS) stats(r);
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) {
-      const float n = (x[v] - mean[v]) * rstd[v];
-      const float e = norm_grad(p, n, w[v], b[v], p.gate ? z[v] : 0.0f, g[v], dz[v]) * w[v];
-      o[v] = rstd[v] * (e - fmaf(n, s2[v], s1[v]));
-    }
+    for (int v = 0; v < VEC; ++v) x[v] = (x[v] - mean[v]) * rstd[v];
+    norm_grad(p, x, w, b, z, g);
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) o[v] = rstd[v] * (g[v] * w[v] - fmaf(x[v], s2[v], s1[v]));
     vec_store<T, VEC>(static_cast<T*>(p.dx) + row_at<ROWS>(s.n, r, p.dxs, p.dxp) + c, o);
-    if (p.gate) vec_store<T, VEC>(static_cast<T*>(p.dz) + row_at<ROWS>(s.n, r, p.dzs, p.dzp) + c, dz);
+    if (p.gate) vec_store<T, VEC>(static_cast<T*>(p.dz) + row_at<ROWS>(s.n, r, p.dzs, p.dzp) + c, z);
   }
 }
 
 // dw and db: the partial rows summed in a fixed order (a warp takes every kWarps-th row, the warps'
 // sums are added in warp order).
-__global__ void __launch_bounds__(32 * kWarps) norm_param_grads(const NormParams p, long long nparts) {
+__global__ void __launch_bounds__(32 * kWarps) norm_param_grads(const __grid_constant__ NormParams p, long long nparts) {
   __shared__ float red[kWarps][32];
   const long long c = (long long)blockIdx.x * 32 + threadIdx.x;
   const int which = blockIdx.y;
@@ -605,12 +690,12 @@ int fail(int code, const char* fmt, long long a = 0, long long b = 0) {
 
 long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
 
-// Slabs of rows: enough CTAs to fill the GPU a few times, at least 4 rows per warp in each.  Sized for
-// 16-byte fp32 vectors whatever the type, so that the workspace size needs no type.
-void plan_slabs(long long units, long long rows, long long C, int* nslab, long long* slab) {
+// Slabs of rows: `ctas` CTAs in all, at least 2 rows per warp in each.  Sized for fp32 vectors whatever the type, so
+// that the workspace size needs no type.
+void plan_slabs(long long ctas, long long units, long long rows, long long C, int* nslab, long long* slab) {
   const long long col_tiles = ceil_div(C, 128);
-  long long n = ceil_div(kTargetCtas, units * col_tiles);
-  n = std::min(n, ceil_div(rows, 4 * kWarps));
+  long long n = ceil_div(ctas, units * col_tiles);
+  n = std::min(n, ceil_div(rows, 2 * kWarps));
   n = std::max<long long>(n, 1);
   *slab = ceil_div(rows, n);
   *nslab = (int)ceil_div(rows, *slab);
@@ -671,22 +756,29 @@ RowsForm rows_form(int cg, int vec) {
 }
 
 template <typename T, int VEC, int K, int WPG>
-cudaError_t launch_rows(const NormParams& p, bool bwd, int lpg, cudaStream_t st) {
+cudaError_t launch_rows(NormParams& p, bool bwd, int lpg, cudaStream_t st) {
   const dim3 block(32, kWarps);
   const int per = WPG == 1 ? 32 / lpg : 1;                         // groups per CTA
   const unsigned gy = (unsigned)ceil_div(p.G, per);
+  // one wave: rows ahead are on their way while a CTA works, so more CTAs than fit only start the queue again
+  const long long rows = WPG == 1 ? ceil_div(p.N, kWarps) : p.N;
+  auto ctas = [&](int fit, long long most) {
+    return std::max<long long>(1, std::min({rows, most, (long long)148 * std::max(fit, 1) / gy}));
+  };
   if (bwd) {
-    norm_rows_bwd<T, VEC, K, WPG><<<dim3((unsigned)p.nslab, gy), block, 0, st>>>(p, lpg);
+    constexpr size_t smem = RowQueue<T, VEC, K, true>::kBytes;
+    constexpr auto kern = norm_rows_bwd<T, VEC, K, WPG>;
+    p.nslab = (int)ctas(ssm::ctas_per_sm<kern>(32 * kWarps, smem), p.nslab);
+    kern<<<dim3((unsigned)p.nslab, gy), block, smem, st>>>(p, lpg);
   } else {
-    // every warp (CTA) takes one row while that fills the GPU a few times over, then loops
-    const long long rows = WPG == 1 ? ceil_div(p.N, kWarps) : p.N;
-    const unsigned gx = (unsigned)std::min<long long>(rows, std::max<long long>(1, ceil_div(148 * 64, gy)));
-    norm_rows_fwd<T, VEC, K, WPG><<<dim3(gx, gy), block, 0, st>>>(p, lpg);
+    constexpr size_t smem = RowQueue<T, VEC, K, false>::kBytes;
+    constexpr auto kern = norm_rows_fwd<T, VEC, K, WPG>;
+    kern<<<dim3((unsigned)ctas(ssm::ctas_per_sm<kern>(32 * kWarps, smem), rows), gy), block, smem, st>>>(p, lpg);
   }
   return cudaGetLastError();
 }
 template <typename T, int VEC>
-cudaError_t run_rows(const NormParams& p, bool bwd, RowsForm f, cudaStream_t st) {
+cudaError_t run_rows(NormParams& p, bool bwd, RowsForm f, cudaStream_t st) {
   constexpr int kMost = 32 / VEC < 8 ? 32 / VEC : 8;
   if (f.lpg == 0) return f.k == 1 ? launch_rows<T, VEC, 1, kWarps>(p, bwd, 0, st) : launch_rows<T, VEC, kMost, kWarps>(p, bwd, 0, st);
   if (f.k == 1) return launch_rows<T, VEC, 1, 1>(p, bwd, f.lpg, st);
@@ -697,7 +789,7 @@ cudaError_t run_rows(const NormParams& p, bool bwd, RowsForm f, cudaStream_t st)
 }
 // The widest vector that divides a group and every row start.
 template <typename T>
-cudaError_t run_rows_any(const NormParams& p, bool bwd, int vec, RowsForm f, cudaStream_t st) {
+cudaError_t run_rows_any(NormParams& p, bool bwd, int vec, RowsForm f, cudaStream_t st) {
   if constexpr (sizeof(T) == 2)
     if (vec == 8) return run_rows<T, 8>(p, bwd, f, st);
   if (vec == 4) return run_rows<T, 4>(p, bwd, f, st);
@@ -714,7 +806,7 @@ void run_stats(const NormParams& p, cudaStream_t st) {
   }
   const dim3 grid((unsigned)(p.N * p.nslab), (unsigned)ceil_div(ceil_div(p.C, VEC), 32));
   norm_col_stats<T, VEC><<<grid, dim3(32, kWarps), 0, st>>>(p);
-  norm_combine_stats<<<(unsigned)ceil_div(p.N * p.G, 8), 256, 0, st>>>(p);
+  norm_combine_stats<<<(unsigned)(p.N * p.G), 128, 0, st>>>(p);
 }
 
 template <typename T, int VEC>
@@ -739,10 +831,19 @@ cudaError_t run_bwd(NormParams& p, bool stats_given, cudaStream_t st) {
   } else {
     const dim3 grid((unsigned)(p.N * p.nslab), cols);
     norm_col_grads<T, VEC, false><<<grid, block, 0, st>>>(p);
-    norm_combine_sums<<<(unsigned)ceil_div(p.N * p.G, 8), 256, 0, st>>>(p);
+    norm_combine_sums<<<(unsigned)(p.N * p.G), 128, 0, st>>>(p);
     norm_apply_bwd<T, VEC, false><<<grid, block, 0, st>>>(p);
   }
   return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t run_slabs(NormParams& p, bool bwd, bool stats_given, int vec, cudaStream_t st) {
+  if constexpr (sizeof(T) == 2)
+    if (vec == 8) return bwd ? run_bwd<T, 8>(p, stats_given, st) : run_fwd<T, 8>(p, st);
+  if (vec == 4) return bwd ? run_bwd<T, 4>(p, stats_given, st) : run_fwd<T, 4>(p, st);
+  if (vec == 2) return bwd ? run_bwd<T, 2>(p, stats_given, st) : run_fwd<T, 2>(p, st);
+  return bwd ? run_bwd<T, 1>(p, stats_given, st) : run_fwd<T, 1>(p, st);
 }
 
 // Fills the shape and the slabs; returns the number of partial rows (each 2 C floats).
@@ -753,10 +854,10 @@ long long plan(NormParams& p, int64_t N, int64_t P, int64_t C, int64_t G) {
   p.G = (int)G;
   p.cg = (int)(C / G);
   if (P == 1) {
-    plan_slabs(1, N, C, &p.nslab, &p.slab);
+    plan_slabs(148 * 6, 1, N, C, &p.nslab, &p.slab);
     return p.nslab;
   }
-  plan_slabs(N, P, C, &p.nslab, &p.slab);
+  plan_slabs(148 * 12, N, P, C, &p.nslab, &p.slab);
   return N * p.nslab;
 }
 
@@ -828,9 +929,8 @@ int ssm_group_norm_fwd(int64_t N, int64_t P, int64_t C, int64_t G, ssm_view x, c
       cur += round256((size_t)parts * 2 * C * sizeof(float));
     }
     p.stats = stats != nullptr ? stats : reinterpret_cast<float*>(cur);
-    const bool vec = C % (16 / es) == 0 && rows_vec(16 / es, es, {x, z, y}) == 16 / es;
-    if (es == 2) e = vec ? run_fwd<__nv_bfloat16, 8>(p, st) : run_fwd<__nv_bfloat16, 1>(p, st);
-    else e = vec ? run_fwd<float, 4>(p, st) : run_fwd<float, 1>(p, st);
+    const int vec = rows_vec((int)C, es, {x, z, y});
+    e = es == 2 ? run_slabs<__nv_bfloat16>(p, false, true, vec, st) : run_slabs<float>(p, false, true, vec, st);
   }
   if (e != cudaSuccess) return fail(SSM_ERR_CUDA, "group_norm forward launch failed (error %lld)", (long long)e);
   return SSM_OK;
@@ -878,16 +978,15 @@ int ssm_group_norm_bwd(int64_t N, int64_t P, int64_t C, int64_t G, ssm_view x, c
   const int rv = rows_vec(p.cg, es, {x, z, dy, dx, dz});
   const RowsForm f = rows_form(p.cg, rv);
   if (P == 1 && f.k != 0) {
-    nparts = p.nslab;
     e = es == 2 ? run_rows_any<__nv_bfloat16>(p, true, rv, f, st) : run_rows_any<float>(p, true, rv, f, st);
+    nparts = p.nslab;
   } else {
     p.sums = reinterpret_cast<float*>(cur);
     cur += round256((size_t)N * G * 2 * sizeof(float));
     p.stats = stats != nullptr ? const_cast<float*>(stats) : reinterpret_cast<float*>(cur);
-    const bool vec = C % (16 / es) == 0 && rows_vec(16 / es, es, {x, z, dy, dx, dz}) == 16 / es;
+    const int vec = rows_vec((int)C, es, {x, z, dy, dx, dz});
     const bool given = stats != nullptr;
-    if (es == 2) e = vec ? run_bwd<__nv_bfloat16, 8>(p, given, st) : run_bwd<__nv_bfloat16, 1>(p, given, st);
-    else e = vec ? run_bwd<float, 4>(p, given, st) : run_bwd<float, 1>(p, given, st);
+    e = es == 2 ? run_slabs<__nv_bfloat16>(p, true, given, vec, st) : run_slabs<float>(p, true, given, vec, st);
   }
   if (e == cudaSuccess && (dweight != nullptr || dbias != nullptr)) {
     norm_param_grads<<<dim3((unsigned)ceil_div(C, 32), 2), dim3(32, kWarps), 0, st>>>(p, nparts);

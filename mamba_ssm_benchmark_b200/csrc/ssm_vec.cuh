@@ -48,4 +48,19 @@ __device__ __forceinline__ void vec_store(T* dst, const float (&v)[VEC]) {
   }
 }
 
+// VEC elements as they lie in memory: loaded now, widened later (a prefetch in half the registers).
+template <typename T, int VEC>
+struct alignas(VEC * sizeof(T)) Raw {
+  T x[VEC];
+  __device__ __forceinline__ void load(const T* src) { *this = *reinterpret_cast<const Raw*>(src); }
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) x[i] = from_f32<T>(0.0f);
+  }
+  __device__ __forceinline__ void widen(float (&v)[VEC]) const {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) v[i] = to_f32(x[i]);
+  }
+};
+
 }  // namespace ssm
