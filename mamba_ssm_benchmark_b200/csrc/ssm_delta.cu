@@ -1173,57 +1173,84 @@ __global__ void __launch_bounds__(256) delta_sum_heads(const __grid_constant__ D
 
 // ================================================================================================
 // One token: S <- a S, e = beta (v - S^T k), S <- S + k e^T, o = scale S^T q.
-// A CTA of 256 threads takes 32 value channels (lanes) of one head; its warps share the dk rows.  Two
-// passes over rows held in registers: the state is read and written once, which bounds the kernel.
+// A CTA of eight warps takes 32 VEC value channels of one head: a lane has VEC of them, a warp every eighth row
+// of dk, ROWS in all.  The rows stay in registers between the two passes over them, so the state is read and
+// written once, which bounds the kernel.
 // ================================================================================================
-constexpr int kStepRows = 16;                     // dk rows per warp: 8 warps cover dk <= 128
-template <typename T>
+template <typename T, int VEC, int ROWS>
 __global__ void __launch_bounds__(256) delta_step(const __grid_constant__ DeltaParams p) {
-  __shared__ float red[2][8][32];
+  __shared__ float red[2][8][32 * VEC], kq[2][8 * ROWS];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int h = blockIdx.y, b = blockIdx.z, hk = h / p.group;
-  const int d = blockIdx.x * 32 + lane;
+  const int d = (blockIdx.x * 32 + lane) * VEC;
   const bool live = d < p.dvw;
   float* S = p.last + ((size_t)b * p.Hv + h) * p.dkw * p.dvw + d;
-  const T* kp = static_cast<const T*>(p.k.ptr) + b * p.k.sb + hk * p.k.sh;
-  const T* qp = static_cast<const T*>(p.q.ptr) + b * p.q.sb + hk * p.q.sh;
-  float x[kStepRows], kr[kStepRows], part = 0.0f;
+  float x[ROWS][VEC], part[VEC], e[VEC];
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) {
+    const int r = warp + 8 * i;
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) x[i][v] = 0.0f;
+    if (live && r < p.dkw) vec_load<float, VEC>(S + (size_t)r * p.dvw, x[i]);
+  }
   const float alpha = expf(p.g[b * p.gsb + h]), beta = p.beta[b * p.bsb + h];
-#pragma unroll
-  for (int i = 0; i < kStepRows; ++i) {
-    const int r = warp + 8 * i;
-    x[i] = live && r < p.dkw ? S[(size_t)r * p.dvw] : 0.0f;
-    kr[i] = r < p.dkw ? to_f32(kp[r]) : 0.0f;
+  for (int i = threadIdx.x; i < 16 * ROWS; i += 256) {
+    const int which = i / (8 * ROWS), r = i % (8 * ROWS);
+    const Heads& src = which ? p.q : p.k;
+    kq[which][r] = r < p.dkw ? to_f32(static_cast<const T*>(src.ptr)[b * src.sb + hk * src.sh + r]) : 0.0f;
   }
 #pragma unroll
-  for (int i = 0; i < kStepRows; ++i) {
-    x[i] *= alpha;
-    part = fmaf(x[i], kr[i], part);
+  for (int v = 0; v < VEC; ++v) {
+    part[v] = 0.0f;
+    e[v] = live ? to_f32(static_cast<const T*>(p.v.ptr)[b * p.v.sb + h * p.v.sh + d + v]) : 0.0f;
   }
-  red[0][warp][lane] = part;
   __syncthreads();
-  float dot = 0.0f;
 #pragma unroll
-  for (int w = 0; w < 8; ++w) dot += red[0][w][lane];
-  const float v = live ? to_f32(static_cast<const T*>(p.v.ptr)[b * p.v.sb + h * p.v.sh + d]) : 0.0f;
-  const float e = beta * (v - dot);
-  part = 0.0f;
+  for (int i = 0; i < ROWS; ++i) {
+    const float k = kq[0][warp + 8 * i];
 #pragma unroll
-  for (int i = 0; i < kStepRows; ++i) {
-    const int r = warp + 8 * i;
-    x[i] = fmaf(kr[i], e, x[i]);
-    if (r < p.dkw) {
-      part = fmaf(x[i], to_f32(qp[r]), part);
-      if (live) S[(size_t)r * p.dvw] = x[i];
+    for (int v = 0; v < VEC; ++v) {
+      x[i][v] *= alpha;
+      part[v] = fmaf(x[i][v], k, part[v]);
     }
   }
-  red[1][warp][lane] = part;
+  vec_store<float, VEC>(&red[0][warp][lane * VEC], part);
+  __syncthreads();
+  float dot[VEC] = {};
+#pragma unroll
+  for (int w = 0; w < 8; ++w) {
+    float y[VEC];
+    vec_load<float, VEC>(&red[0][w][lane * VEC], y);
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) dot[v] += y[v];
+  }
+#pragma unroll
+  for (int v = 0; v < VEC; ++v) {
+    e[v] = beta * (e[v] - dot[v]);
+    part[v] = 0.0f;
+  }
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) {
+    const int r = warp + 8 * i;
+    const float k = kq[0][r], q = kq[1][r];
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) {
+      x[i][v] = fmaf(k, e[v], x[i][v]);
+      part[v] = fmaf(x[i][v], q, part[v]);
+    }
+    if (live && r < p.dkw) vec_store<float, VEC>(S + (size_t)r * p.dvw, x[i]);
+  }
+  vec_store<float, VEC>(&red[1][warp][lane * VEC], part);
   __syncthreads();
   if (warp == 0 && live) {
-    float o = 0.0f;
+    T* o = static_cast<T*>(const_cast<void*>(p.o.ptr)) + b * p.o.sb + h * p.o.sh + d;
 #pragma unroll
-    for (int w = 0; w < 8; ++w) o += red[1][w][lane];
-    static_cast<T*>(const_cast<void*>(p.o.ptr))[b * p.o.sb + h * p.o.sh + d] = from_f32<T>(p.scale * o);
+    for (int v = 0; v < VEC; ++v) {
+      float s = 0.0f;
+#pragma unroll
+      for (int w = 0; w < 8; ++w) s += red[1][w][lane * VEC + v];
+      o[v] = from_f32<T>(p.scale * s);
+    }
   }
 }
 
@@ -1391,6 +1418,19 @@ cudaError_t run_bwd(const Shape& s, const DeltaParams& p, cudaStream_t st) {
   return launch<delta_sum_heads<T, DKP>>(sg, 256, 0, p, st);
 }
 
+// Four value channels a lane (16-byte accesses) where the state's rows allow it and that still gives every SM a CTA,
+// else one, in four times the CTAs.
+template <typename T>
+cudaError_t run_step(const Shape& s, const DeltaParams& p, cudaStream_t st) {
+  const bool aligned = s.dv % 4 == 0 && reinterpret_cast<uintptr_t>(p.last) % 16 == 0;
+  const bool wide = aligned && s.B * s.Hv * ((s.dv + 127) / 128) >= 148;
+  const int per = wide ? 128 : 32;
+  const dim3 grid((unsigned)((s.dv + per - 1) / per), (unsigned)s.Hv, (unsigned)s.B);
+  if (s.dk <= 64)
+    return wide ? launch<delta_step<T, 4, 8>>(grid, 256, 0, p, st) : launch<delta_step<T, 1, 8>>(grid, 256, 0, p, st);
+  return wide ? launch<delta_step<T, 4, 16>>(grid, 256, 0, p, st) : launch<delta_step<T, 1, 16>>(grid, 256, 0, p, st);
+}
+
 }  // namespace
 
 extern "C" {
@@ -1511,9 +1551,7 @@ int ssm_gated_delta_state_update(int64_t B, int64_t Hk, int64_t Hv, int64_t dk, 
   p.o = heads(o);
   p.last = state;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const dim3 grid((unsigned)((dv + 31) / 32), (unsigned)Hv, (unsigned)B);
-  const cudaError_t e = s.dtype == SSM_BF16 ? launch<delta_step<__nv_bfloat16>>(grid, 256, 0, p, st)
-                                            : launch<delta_step<float>>(grid, 256, 0, p, st);
+  const cudaError_t e = s.dtype == SSM_BF16 ? run_step<__nv_bfloat16>(s, p, st) : run_step<float>(s, p, st);
   if (e != cudaSuccess) return fail(SSM_ERR_CUDA, "gated delta state update: %s", cudaGetErrorString(e));
   return SSM_OK;
 }

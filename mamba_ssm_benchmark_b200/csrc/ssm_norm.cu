@@ -136,6 +136,34 @@ __device__ __forceinline__ void write_partials(float* part, long long row, long 
   }
 }
 
+// Rows ahead of the one in work: kDepth rows of every tensor, copied asynchronously into slots of shared memory
+// that only the thread itself reads, so no barrier is needed and depth costs no registers.  (A prefetch of one
+// row in registers kept 22 KB per SM in flight and reached half the bandwidth.)
+template <typename T, int VEC, int K, int TENSORS>
+struct Slots {
+  using Vec = ssm::Raw<T, VEC>;
+  static constexpr int kRow = TENSORS * K * 32 * kWarps * (int)sizeof(Vec);
+  static constexpr int kDepth = kRow * 4 <= 48 * 1024 ? 4 : 2;
+  static constexpr size_t kBytes = (size_t)kDepth * kRow;
+  Vec* slots;
+  int tid;
+  __device__ Slots(unsigned char* smem) : slots(reinterpret_cast<Vec*>(smem)), tid(threadIdx.y * 32 + threadIdx.x) {}
+  __device__ Vec* slot(int stage, int tensor, int i = 0) { return slots + ((stage * TENSORS + tensor) * K + i) * 32 * kWarps + tid; }
+  // src may be anything readable where ok is false: the slot becomes zero
+  __device__ void copy(Vec* dst, const void* src, bool ok) {
+    if constexpr (sizeof(Vec) >= 4) {
+      asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(ssm::smem_u32(dst)), "l"(src),
+                   "n"((int)sizeof(Vec)), "r"(ok ? (int)sizeof(Vec) : 0)
+                   : "memory");
+    } else {
+      if (ok) dst->load(static_cast<const T*>(src));
+      else dst->zero();
+    }
+  }
+  __device__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+  __device__ void wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory"); }
+};
+
 // ---- one position per sample ----------------------------------------------------------------
 // WPG = 1: lpg lanes (a power of two) share a group, the CTA's warps take different rows; blockIdx.y
 // selects 32 / lpg groups.  WPG = kWarps: the CTA shares one group, blockIdx.y selects it.
@@ -210,29 +238,10 @@ __device__ __forceinline__ float row_stats(const NormParams& p, const Place<WPG>
   return rsqrtf(fmaf(group_sum<WPG>(q, at.lpg), inv, p.eps));
 }
 
-// Rows ahead of the one in work: kDepth rows of every tensor, copied asynchronously into slots of shared memory
-// that only the thread itself reads, so no barrier is needed and depth costs no registers.  (A prefetch of one
-// row in registers kept 22 KB per SM in flight and reached half the bandwidth.)
 template <typename T, int VEC, int K, bool BWD>
-struct RowQueue {
-  using Vec = ssm::Raw<T, VEC>;
-  static constexpr int kTensors = BWD ? 3 : 2, kRow = kTensors * K * 32 * kWarps * (int)sizeof(Vec);
-  static constexpr int kDepth = kRow * 4 <= 48 * 1024 ? 4 : 2;
-  static constexpr size_t kBytes = (size_t)kDepth * kRow;
-  Vec* slots;
-  int tid;
-  __device__ RowQueue(unsigned char* smem) : slots(reinterpret_cast<Vec*>(smem)), tid(threadIdx.y * 32 + threadIdx.x) {}
-  __device__ Vec* slot(int stage, int tensor, int i) { return slots + ((stage * kTensors + tensor) * K + i) * 32 * kWarps + tid; }
-  __device__ void copy(Vec* dst, const T* src, bool ok) {
-    if constexpr (sizeof(Vec) >= 4) {
-      asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(ssm::smem_u32(dst)), "l"(src),
-                   "n"((int)sizeof(Vec)), "r"(ok ? (int)sizeof(Vec) : 0)
-                   : "memory");
-    } else {
-      if (ok) dst->load(src);
-      else dst->zero();
-    }
-  }
+struct RowQueue : Slots<T, VEC, K, BWD ? 3 : 2> {
+  using Base = Slots<T, VEC, K, BWD ? 3 : 2>;
+  using Base::Base;
   template <int WPG>
   __device__ void fetch(const NormParams& p, const Place<WPG>& at, long long r, int stage) {
 #pragma unroll
@@ -240,13 +249,12 @@ struct RowQueue {
       const int c = (at.lane + i * at.lpg) * VEC;
       const bool ok = at.live && r < p.N && c < p.cg;
       const long long rr = ok ? r : 0, cc = ok ? at.c0 + c : 0;
-      copy(slot(stage, 0, i), static_cast<const T*>(p.x) + rr * p.xs + cc, ok);
-      if (p.gate) copy(slot(stage, 1, i), static_cast<const T*>(p.z) + rr * p.zs + cc, ok);
-      if (BWD) copy(slot(stage, 2, i), static_cast<const T*>(p.dy) + rr * p.gs + cc, ok);
+      this->copy(this->slot(stage, 0, i), static_cast<const T*>(p.x) + rr * p.xs + cc, ok);
+      if (p.gate) this->copy(this->slot(stage, 1, i), static_cast<const T*>(p.z) + rr * p.zs + cc, ok);
+      if (BWD) this->copy(this->slot(stage, 2, i), static_cast<const T*>(p.dy) + rr * p.gs + cc, ok);
     }
-    asm volatile("cp.async.commit_group;" ::: "memory");
+    this->commit();
   }
-  __device__ void wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory"); }
 };
 
 // The number of rows is the same for all of a CTA's warps, so that group_sum's barriers match; rows past
@@ -446,10 +454,43 @@ __device__ __forceinline__ long long row_at(long long n, long long r, long long 
   return ROWS ? r * ss : n * ss + r * ps;
 }
 
+// A thread's rows of a slab, kWarps apart, in order: x, and where wanted dy and z.
+template <typename T, int VEC, bool ROWS, bool GRAD>
+struct SlabQueue : Slots<T, VEC, 1, GRAD ? 3 : 2> {
+  using Base = Slots<T, VEC, 1, GRAD ? 3 : 2>;
+  __device__ SlabQueue(unsigned char* smem) : Base(smem) {}
+  __device__ void fetch(const NormParams& p, const Rows& s, long long c, long long r, bool z, int stage) {
+    const bool ok = r < s.r1;
+    const long long rr = ok ? r : s.r0;
+    this->copy(this->slot(stage, 0), static_cast<const T*>(p.x) + row_at<ROWS>(s.n, rr, p.xs, p.xp) + c, ok);
+    if (z) this->copy(this->slot(stage, 1), static_cast<const T*>(p.z) + row_at<ROWS>(s.n, rr, p.zs, p.zp) + c, ok);
+    if (GRAD) this->copy(this->slot(stage, 2), static_cast<const T*>(p.dy) + row_at<ROWS>(s.n, rr, p.gs, p.gp) + c, ok);
+    this->commit();
+  }
+  // f(row, x, z, dy) for every row
+  template <typename F>
+  __device__ void each(const NormParams& p, const Rows& s, long long c, bool gate, F f) {
+#pragma unroll
+    for (int d = 0; d < Base::kDepth; ++d) fetch(p, s, c, s.r0 + threadIdx.y + d * kWarps, gate, d);
+    int stage = 0;
+    for (long long r = s.r0 + threadIdx.y; r < s.r1; r += kWarps) {
+      float x[VEC], z[VEC] = {}, g[VEC] = {};
+      this->wait();
+      this->slot(stage, 0)->widen(x);
+      if (gate) this->slot(stage, 1)->widen(z);
+      if (GRAD) this->slot(stage, 2)->widen(g);
+      fetch(p, s, c, r + Base::kDepth * kWarps, gate, stage);
+      stage = stage + 1 == Base::kDepth ? 0 : stage + 1;
+      f(r, x, z, g);
+    }
+  }
+};
+
 // Per (sample, slab, channel): mean and sum of squared deviations of the slab's rows, summed about the
 // slab's first row so that a large common offset costs no digits.
 template <typename T, int VEC>
 __global__ void __launch_bounds__(32 * kWarps) norm_col_stats(const __grid_constant__ NormParams p) {
+  extern __shared__ __align__(16) unsigned char smem[];
   const long long c = ((long long)blockIdx.y * 32 + threadIdx.x) * VEC;
   const bool live = c < p.C;
   const Rows s = rows_of<false>(p);
@@ -459,17 +500,14 @@ __global__ void __launch_bounds__(32 * kWarps) norm_col_stats(const __grid_const
   for (int v = 0; v < VEC; ++v) k[v] = a[v] = q[v] = 0.0f;
   if (live) {
     vec_load<T, VEC>(x + s.r0 * p.xp, k);
-#pragma unroll 4
-    for (long long r = s.r0 + threadIdx.y; r < s.r1; r += kWarps) {
-      float t[VEC];
-      vec_load<T, VEC>(x + r * p.xp, t);
+    SlabQueue<T, VEC, false, false>(smem).each(p, s, c, false, [&](long long, float (&t)[VEC], float (&)[VEC], float (&)[VEC]) {
 #pragma unroll
       for (int v = 0; v < VEC; ++v) {
         const float d = t[v] - k[v];
         a[v] += d;
         q[v] = fmaf(d, d, q[v]);
       }
-    }
+    });
   }
   __shared__ float red[kWarps][32][2 * VEC + 1];
 #pragma unroll
@@ -494,25 +532,25 @@ __global__ void __launch_bounds__(32 * kWarps) norm_col_stats(const __grid_const
   }
 }
 
-// Sum of a double over a CTA of 128 threads, in a fixed order, to all of them.
+// Sum of a double over a CTA of 256 threads, in a fixed order, to all of them.
 __device__ __forceinline__ double cta_sum(double x) {
-  __shared__ double red[4];
+  __shared__ double red[8];
   for (int k = 16; k >= 1; k >>= 1) x += __shfl_xor_sync(0xffffffffu, x, k);
   __syncthreads();
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = x;
   __syncthreads();
-  return (red[0] + red[1]) + (red[2] + red[3]);
+  return ((red[0] + red[1]) + (red[2] + red[3])) + ((red[4] + red[5]) + (red[6] + red[7]));
 }
 // f(slab, channel of the group) for this thread's share of a sample's slabs x a group's channels.
 template <typename F>
 __device__ __forceinline__ void for_cells(const NormParams& p, F f) {
   const int cells = p.nslab * p.cg;
 #pragma unroll 4
-  for (int e = threadIdx.x; e < cells; e += 128) f(e / p.cg, e % p.cg);
+  for (int e = threadIdx.x; e < cells; e += 256) f(e / p.cg, e % p.cg);
 }
 
 // A CTA per (sample, group): mean and rstd from the slabs' per-channel means and squared deviations.
-__global__ void __launch_bounds__(128) norm_combine_stats(const __grid_constant__ NormParams p) {
+__global__ void __launch_bounds__(256) norm_combine_stats(const __grid_constant__ NormParams p) {
   const long long n = blockIdx.x / p.G;
   const float* part = p.part + n * p.nslab * 2 * p.C + (long long)(blockIdx.x % p.G) * p.cg;
   const double m = (double)p.P * p.cg;
@@ -537,6 +575,7 @@ __global__ void __launch_bounds__(128) norm_combine_stats(const __grid_constant_
 
 template <typename T, int VEC, bool ROWS>
 __global__ void __launch_bounds__(32 * kWarps) norm_apply_fwd(const __grid_constant__ NormParams p) {
+  extern __shared__ __align__(16) unsigned char smem[];
   const long long c = ((long long)blockIdx.y * 32 + threadIdx.x) * VEC;
   if (c >= p.C) return;
   const Rows s = rows_of<ROWS>(p);
@@ -551,22 +590,20 @@ __global__ void __launch_bounds__(32 * kWarps) norm_apply_fwd(const __grid_const
     }
   };
   if (!ROWS) stats(s.n);
-#pragma unroll 4
-  for (long long r = s.r0 + threadIdx.y; r < s.r1; r += kWarps) {
-    float x[VEC], z[VEC] = {}, o[VEC];
-    vec_load<T, VEC>(static_cast<const T*>(p.x) + row_at<ROWS>(s.n, r, p.xs, p.xp) + c, x);
-    if (p.gate) vec_load<T, VEC>(static_cast<const T*>(p.z) + row_at<ROWS>(s.n, r, p.zs, p.zp) + c, z);
+  SlabQueue<T, VEC, ROWS, false>(smem).each(p, s, c, p.gate, [&](long long r, float (&x)[VEC], float (&z)[VEC], float (&)[VEC]) {
     if (ROWS) stats(r);
+    float o[VEC];
 #pragma unroll
     for (int v = 0; v < VEC; ++v) x[v] = (x[v] - mean[v]) * rstd[v];
     norm_out(p, x, w, b, z, o);
     vec_store<T, VEC>(static_cast<T*>(p.y) + row_at<ROWS>(s.n, r, p.ys, p.yp) + c, o);
-  }
+  });
 }
 
 // Per (sample, slab, channel) (ROWS: per (slab, channel)): sums of e n and of e.
 template <typename T, int VEC, bool ROWS>
 __global__ void __launch_bounds__(32 * kWarps) norm_col_grads(const __grid_constant__ NormParams p) {
+  extern __shared__ __align__(16) unsigned char smem[];
   const long long c = ((long long)blockIdx.y * 32 + threadIdx.x) * VEC;
   const bool live = c < p.C;
   const Rows s = rows_of<ROWS>(p);
@@ -584,12 +621,7 @@ __global__ void __launch_bounds__(32 * kWarps) norm_col_grads(const __grid_const
       }
     };
     if (!ROWS) stats(s.n);
-#pragma unroll 2
-    for (long long r = s.r0 + threadIdx.y; r < s.r1; r += kWarps) {
-      float x[VEC], z[VEC] = {}, g[VEC];
-      vec_load<T, VEC>(static_cast<const T*>(p.x) + row_at<ROWS>(s.n, r, p.xs, p.xp) + c, x);
-      vec_load<T, VEC>(static_cast<const T*>(p.dy) + row_at<ROWS>(s.n, r, p.gs, p.gp) + c, g);
-      if (p.gate) vec_load<T, VEC>(static_cast<const T*>(p.z) + row_at<ROWS>(s.n, r, p.zs, p.zp) + c, z);
+    SlabQueue<T, VEC, ROWS, true>(smem).each(p, s, c, p.gate, [&](long long r, float (&x)[VEC], float (&z)[VEC], float (&g)[VEC]) {
       if (ROWS) stats(r);
 #pragma unroll
       for (int v = 0; v < VEC; ++v) x[v] = (x[v] - mean[v]) * rstd[v];
@@ -599,13 +631,13 @@ __global__ void __launch_bounds__(32 * kWarps) norm_col_grads(const __grid_const
         dw[v] = fmaf(g[v], x[v], dw[v]);
         db[v] += g[v];
       }
-    }
+    });
   }
   write_partials<VEC>(p.part, blockIdx.x, p.C, c, live, dw, db);
 }
 
 // A CTA per (sample, group): s1 / M and s2 / M from the channels' sums.
-__global__ void __launch_bounds__(128) norm_combine_sums(const __grid_constant__ NormParams p) {
+__global__ void __launch_bounds__(256) norm_combine_sums(const __grid_constant__ NormParams p) {
   const long long n = blockIdx.x / p.G, c0 = (long long)(blockIdx.x % p.G) * p.cg;
   const float* part = p.part + n * p.nslab * 2 * p.C + c0;
   double s1 = 0.0, s2 = 0.0;
@@ -624,6 +656,7 @@ __global__ void __launch_bounds__(128) norm_combine_sums(const __grid_constant__
 
 template <typename T, int VEC, bool ROWS>
 __global__ void __launch_bounds__(32 * kWarps) norm_apply_bwd(const __grid_constant__ NormParams p) {
+  extern __shared__ __align__(16) unsigned char smem[];
   const long long c = ((long long)blockIdx.y * 32 + threadIdx.x) * VEC;
   if (c >= p.C) return;
   const Rows s = rows_of<ROWS>(p);
@@ -642,13 +675,9 @@ __global__ void __launch_bounds__(32 * kWarps) norm_apply_bwd(const __grid_const
     }
   };
   if (!ROWS) stats(s.n);
-#pragma unroll 2
-  for (long long r = s.r0 + threadIdx.y; r < s.r1; r += kWarps) {
-    float x[VEC], z[VEC] = {}, g[VEC], o[VEC];
-    vec_load<T, VEC>(static_cast<const T*>(p.x) + row_at<ROWS>(s.n, r, p.xs, p.xp) + c, x);
-    vec_load<T, VEC>(static_cast<const T*>(p.dy) + row_at<ROWS>(s.n, r, p.gs, p.gp) + c, g);
-    if (p.gate) vec_load<T, VEC>(static_cast<const T*>(p.z) + row_at<ROWS>(s.n, r, p.zs, p.zp) + c, z);
+  SlabQueue<T, VEC, ROWS, true>(smem).each(p, s, c, p.gate, [&](long long r, float (&x)[VEC], float (&z)[VEC], float (&g)[VEC]) {
     if (ROWS) stats(r);
+    float o[VEC];
 #pragma unroll
     for (int v = 0; v < VEC; ++v) x[v] = (x[v] - mean[v]) * rstd[v];
     norm_grad(p, x, w, b, z, g);
@@ -656,7 +685,7 @@ __global__ void __launch_bounds__(32 * kWarps) norm_apply_bwd(const __grid_const
     for (int v = 0; v < VEC; ++v) o[v] = rstd[v] * (g[v] * w[v] - fmaf(x[v], s2[v], s1[v]));
     vec_store<T, VEC>(static_cast<T*>(p.dx) + row_at<ROWS>(s.n, r, p.dxs, p.dxp) + c, o);
     if (p.gate) vec_store<T, VEC>(static_cast<T*>(p.dz) + row_at<ROWS>(s.n, r, p.dzs, p.dzp) + c, z);
-  }
+  });
 }
 
 // dw and db: the partial rows summed in a fixed order (a warp takes every kWarps-th row, the warps'
@@ -797,6 +826,12 @@ cudaError_t run_rows_any(NormParams& p, bool bwd, int vec, RowsForm f, cudaStrea
   return run_rows<T, 1>(p, bwd, f, st);
 }
 
+template <auto Kern, typename Queue>
+void launch_slabs(dim3 grid, const NormParams& p, cudaStream_t st) {
+  if (Queue::kBytes > 24 * 1024) ssm::ctas_per_sm<Kern>(32 * kWarps, Queue::kBytes);   // beside static shared memory
+  Kern<<<grid, dim3(32, kWarps), Queue::kBytes, st>>>(p);
+}
+
 // mean and rstd of every (sample, group) into p.stats
 template <typename T, int VEC>
 void run_stats(const NormParams& p, cudaStream_t st) {
@@ -805,34 +840,32 @@ void run_stats(const NormParams& p, cudaStream_t st) {
     return;
   }
   const dim3 grid((unsigned)(p.N * p.nslab), (unsigned)ceil_div(ceil_div(p.C, VEC), 32));
-  norm_col_stats<T, VEC><<<grid, dim3(32, kWarps), 0, st>>>(p);
-  norm_combine_stats<<<(unsigned)(p.N * p.G), 128, 0, st>>>(p);
+  launch_slabs<norm_col_stats<T, VEC>, Slots<T, VEC, 1, 2>>(grid, p, st);
+  norm_combine_stats<<<(unsigned)(p.N * p.G), 256, 0, st>>>(p);
 }
 
 template <typename T, int VEC>
 cudaError_t run_fwd(NormParams& p, cudaStream_t st) {
-  const dim3 block(32, kWarps);
   const unsigned cols = (unsigned)ceil_div(ceil_div(p.C, VEC), 32);
   run_stats<T, VEC>(p, st);
-  if (p.P == 1) norm_apply_fwd<T, VEC, true><<<dim3((unsigned)p.nslab, cols), block, 0, st>>>(p);
-  else norm_apply_fwd<T, VEC, false><<<dim3((unsigned)(p.N * p.nslab), cols), block, 0, st>>>(p);
+  if (p.P == 1) launch_slabs<norm_apply_fwd<T, VEC, true>, Slots<T, VEC, 1, 2>>(dim3((unsigned)p.nslab, cols), p, st);
+  else launch_slabs<norm_apply_fwd<T, VEC, false>, Slots<T, VEC, 1, 2>>(dim3((unsigned)(p.N * p.nslab), cols), p, st);
   return cudaGetLastError();
 }
 
 template <typename T, int VEC>
 cudaError_t run_bwd(NormParams& p, bool stats_given, cudaStream_t st) {
-  const dim3 block(32, kWarps);
   const unsigned cols = (unsigned)ceil_div(ceil_div(p.C, VEC), 32);
   if (!stats_given) run_stats<T, VEC>(p, st);
   if (p.P == 1) {
     norm_group_sums<T, true><<<(unsigned)ceil_div(p.N * p.G, 8), 256, 0, st>>>(p);
-    norm_col_grads<T, VEC, true><<<dim3((unsigned)p.nslab, cols), block, 0, st>>>(p);
-    norm_apply_bwd<T, VEC, true><<<dim3((unsigned)p.nslab, cols), block, 0, st>>>(p);
+    launch_slabs<norm_col_grads<T, VEC, true>, Slots<T, VEC, 1, 3>>(dim3((unsigned)p.nslab, cols), p, st);
+    launch_slabs<norm_apply_bwd<T, VEC, true>, Slots<T, VEC, 1, 3>>(dim3((unsigned)p.nslab, cols), p, st);
   } else {
     const dim3 grid((unsigned)(p.N * p.nslab), cols);
-    norm_col_grads<T, VEC, false><<<grid, block, 0, st>>>(p);
-    norm_combine_sums<<<(unsigned)(p.N * p.G), 128, 0, st>>>(p);
-    norm_apply_bwd<T, VEC, false><<<grid, block, 0, st>>>(p);
+    launch_slabs<norm_col_grads<T, VEC, false>, Slots<T, VEC, 1, 3>>(grid, p, st);
+    norm_combine_sums<<<(unsigned)(p.N * p.G), 256, 0, st>>>(p);
+    launch_slabs<norm_apply_bwd<T, VEC, false>, Slots<T, VEC, 1, 3>>(grid, p, st);
   }
   return cudaGetLastError();
 }
@@ -857,7 +890,7 @@ long long plan(NormParams& p, int64_t N, int64_t P, int64_t C, int64_t G) {
     plan_slabs(148 * 6, 1, N, C, &p.nslab, &p.slab);
     return p.nslab;
   }
-  plan_slabs(148 * 12, N, P, C, &p.nslab, &p.slab);
+  plan_slabs(148 * 8, N, P, C, &p.nslab, &p.slab);
   return N * p.nslab;
 }
 
