@@ -337,7 +337,8 @@ SSM_API int ssm_conv1d_bwd(int64_t B, int64_t L, int64_t D, int64_t K, ssm_view 
  * stride along the heads.  h0, last, dlast, dh0: (B, Hv, dk, dv) dense float32.  dk <= 128.
  *
  * ssm_gated_delta_fwd: h0 NULL = zeros; last may be NULL.  saved: NULL, or
- * ssm_gated_delta_saved_size bytes that a training call keeps for ssm_gated_delta_bwd.
+ * ssm_gated_delta_saved_size bytes that a training call keeps for ssm_gated_delta_bwd (the forward then
+ * needs no workspace): the chunks' tiles, the state entering every 64 positions, the corrected values.
  * ssm_gated_delta_bwd: gradients from d_o (like o, any strides) and dlast (NULL = zeros): d_q, d_k
  * (summed over the value heads of a key head), d_v in the inputs' dtype; d_g, d_beta (B, L, Hv)
  * dense float32; dh0 may be NULL.  Every sum has a fixed order: results are reproducible.

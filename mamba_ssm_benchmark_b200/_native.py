@@ -172,14 +172,16 @@ def view2(t):
 
 def heads4(t):
     """(B, rows, heads, width) tensor with unit inner stride -> ssm_heads."""
-    assert t.dim() == 4 and (t.stride(3) == 1 or t.shape[3] == 1), "inner dimension must be contiguous"
-    return SsmHeads(t.data_ptr(), DTYPES[t.dtype], 0, t.stride(0), t.stride(1), t.stride(2))
+    sb, sl, sh, inner = t.stride()
+    assert inner == 1 or t.shape[3] == 1, "inner dimension must be contiguous"
+    return SsmHeads(t.data_ptr(), DTYPES[t.dtype], 0, sb, sl, sh)
 
 
 def heads3(t):
     """(B, heads, width) tensor with unit inner stride -> ssm_heads with one row per batch entry."""
-    assert t.dim() == 3 and (t.stride(2) == 1 or t.shape[2] == 1), "inner dimension must be contiguous"
-    return SsmHeads(t.data_ptr(), DTYPES[t.dtype], 0, t.stride(0), 0, t.stride(1))
+    sb, sh, inner = t.stride()
+    assert inner == 1 or t.shape[2] == 1, "inner dimension must be contiguous"
+    return SsmHeads(t.data_ptr(), DTYPES[t.dtype], 0, sb, 0, sh)
 
 
 def delta_opts(bias, softplus, dbias=None):

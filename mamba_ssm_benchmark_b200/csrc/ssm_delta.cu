@@ -1,9 +1,8 @@
 // ssm_delta.cu — the gated delta rule: chunked forward and backward, one-token state update.
 // The formulas are in ssm_delta.cuh.  Forward: delta_prep (everything that does not need the state, all
-// chunks at once), delta_fwd (the state from chunk to chunk, and the output).  Backward: delta_prep,
-// delta_bwd_chain (the state's gradient from the last chunk to the first), delta_bwd_chunk (all other
-// gradients, all chunks at once), delta_sum_heads (query and key gradients over the value heads that
-// share a key head).
+// chunks at once), delta_fwd (the state from chunk to chunk, and the output).  Backward: delta_bwd_chain (the
+// state's gradient from the last chunk to the first), delta_bwd_chunk (all other gradients, all chunks at
+// once), delta_sum_heads (query and key gradients over the value heads that share a key head).
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -50,6 +49,22 @@ __device__ __forceinline__ void load8(const T* row, int c0, int width, bool vec,
     for (int i = 0; i < 8; ++i) x[i] = c0 + i < width ? to_f32(row[c0 + i]) : 0.0f;
   }
 }
+
+// The same as they lie in memory.
+template <typename T>
+struct alignas(16) Row8 {
+  T x[8];
+  __device__ __forceinline__ void load(const T* row, int c0, int width, bool vec) {
+    if (vec && c0 + 8 <= width) {
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(T) / 2; ++i)
+        reinterpret_cast<uint4*>(x)[i] = reinterpret_cast<const uint4*>(row + c0)[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = c0 + i < width ? row[c0 + i] : from_f32<T>(0.0f);
+    }
+  }
+};
 
 // Splits 8 values into NP pieces and writes 16 bytes of each at `off` of the tiles `stride` apart.
 template <int NP>
@@ -435,30 +450,33 @@ __device__ __forceinline__ void state_product(float (&d)[2][4], float (&d2)[2][4
 // a: the strip's operand in NA pieces; products up to index sum MAXI.
 template <int NA, int NB, int MAXI, bool TR>
 __device__ __forceinline__ void tri_product(float (&d)[2][4], const uint4 (*f)[NA][32], uint32_t tile, int w, int lane) {
-  float low[2][4];
-  zero(low);
+  float low[3][2][4];                    // by piece of the tile: six chains of products instead of two
+#pragma unroll
+  for (int pb = 0; pb < 3; ++pb) zero(low[pb]);
 #pragma unroll
   for (int kb = 0; kb < kC / 16; ++kb) {
     const bool first = TR ? 2 * kb + 1 >= w : 2 * kb <= w;             // whether the tiles w and 7 - w need kb
     const bool second = TR ? 2 * kb + 1 >= 7 - w : 2 * kb <= 7 - w;
     if (!first && !second) continue;
-    uint32_t a[NA][4];
+    uint32_t a[NA][4], bf[NB][4];
 #pragma unroll
     for (int i = 0; i < NA; ++i) get_frag(a[i], f[kb][i][lane]);
 #pragma unroll
     for (int pb = 0; pb < NB && pb <= MAXI; ++pb) {
-      uint32_t bf[4];
-      if (TR) load_bt2<kC>(bf, tile + pb * (kTri * 2), w, kb, lane);
-      else load_b2<kC>(bf, tile + pb * (kTri * 2), w, kb, lane);
-#pragma unroll
-      for (int i = 0; i < NA; ++i) {
-        if (i + pb > MAXI) continue;
-        if (first) mma_bf16(i + pb ? low[0] : d[0], a[i], bf[0], bf[1]);
-        if (second) mma_bf16(i + pb ? low[1] : d[1], a[i], bf[2], bf[3]);
-      }
+      if (TR) load_bt2<kC>(bf[pb], tile + pb * (kTri * 2), w, kb, lane);
+      else load_b2<kC>(bf[pb], tile + pb * (kTri * 2), w, kb, lane);
     }
+#pragma unroll
+    for (int i = 0; i < NA; ++i)
+#pragma unroll
+      for (int pb = 0; pb < NB; ++pb) {
+        if (i + pb > MAXI) continue;
+        if (first) mma_bf16(i + pb ? low[pb][0] : d[0], a[i], bf[pb][0], bf[pb][1]);
+        if (second) mma_bf16(i + pb ? low[pb][1] : d[1], a[i], bf[pb][2], bf[pb][3]);
+      }
   }
-  add(d, low);
+#pragma unroll
+  for (int pb = 0; pb < NB && pb <= MAXI; ++pb) add(d, low[pb]);
 }
 
 // The warp's quarter of S <- decay S + sign (a [.][c]) (tile [c][dk]) over kC positions.  The sum over the chunk is
@@ -614,9 +632,9 @@ __global__ void __launch_bounds__(128 * NS + 32) delta_fwd(const __grid_constant
     }
     strip_sync(strip);                            // U is there; T is done with
     if (leader) mbar_arrive(&s.empty[kTileT]);
-    state_add<NP, DKP>(S, vec[kC - 1], 1.0f, z.lf, sk, w, lane);
     mbar_wait(&s.full[kTileP], ch & 1, p.err);
     tri_product<PP, PP, PP - 1, false>(O, z.uf, sp, w, lane);
+    state_add<NP, DKP>(S, vec[kC - 1], 1.0f, z.lf, sk, w, lane);
     z.out.write(O, w, lane);
     z.out.flush(obase + t0 * p.o.sl, p.o.sl, rows, cols, oout, w, lane);
   }
@@ -763,7 +781,7 @@ struct alignas(128) BwdSmem {
   __nv_bfloat16 q[NP][kC * DKP];
   float vec[kVec];
   float dots[4][4][kC];         // q.dQ, k.H, k.C, e^(G_last - G) k.E3; by column quarter
-  float dxv[kC];                // dX.V
+  float dxv[SL / 8][kC];        // dX.V by 8 channels of a slab
   float sds[16];                // <S, dS'> by warp
   float m[kC];                  // the diagonal of M
   uint64_t bar_kq, bar_slab[2];
@@ -815,6 +833,15 @@ __global__ void __launch_bounds__(512) delta_bwd_chunk(const __grid_constant__ D
     bulk_load(d.U, p.us + (at * p.dvp + v0) * kC, vn * kC * 4, bar);
     bulk_load(d.dX, p.dxs + (at * p.dvp + v0) * kC, vn * kC * 4, bar);
   };
+  auto fetch_tiles = [&](int item) {
+    if (item >= items) return;
+    const int h = item / p.n % p.Hv, b = item / p.n / p.Hv;
+    const size_t at = item, atk = ((size_t)b * p.Hk + h / p.group) * p.n + item % p.n;
+    mbar_arrive_expect_tx(&s.bar_kq, sizeof(s.k) + sizeof(s.q) + sizeof(s.vec));
+    bulk_load(s.k, p.kimg + atk * (NP * kC * DKP), sizeof(s.k), &s.bar_kq);
+    bulk_load(s.q, p.qimg + atk * (NP * kC * DKP), sizeof(s.q), &s.bar_kq);
+    bulk_load(s.vec, p.vec + at * kVec, sizeof(s.vec), &s.bar_kq);
+  };
   if (tid == 0) {
     mbar_init(&s.bar_kq, 1);
     mbar_init(&s.bar_slab[0], 1);
@@ -822,35 +849,29 @@ __global__ void __launch_bounds__(512) delta_bwd_chunk(const __grid_constant__ D
     fence_mbar_init();
     fetch_slab(0);
     fetch_slab(1);
+    fetch_tiles(blockIdx.x);
   }
   __syncthreads();
-  // dO and V of a slab: 8 channels of one position per thread
-  constexpr int kRowGroups = SL / 8;
-  static_assert(kC * kRowGroups <= 512, "a slab's dO is one step");
+  // A slab's dO and V, 8 channels of one position per thread: dO by the first threads, neighbours along a row; V,
+  // which only meets dX (stored [channel][position]) in dX.V, by the next ones, neighbours along the positions.
+  constexpr int kRowGroups = SL / 8, kLoaders = kC * kRowGroups;
+  static_assert(2 * kLoaders <= 512, "a slab's dO and V are one step");
   const bool ovec = rows_aligned16(p.o, sizeof(T)), vvec = rows_aligned16(p.v, sizeof(T));
-  const bool loads = tid < kC * kRowGroups;
-  const int lc = tid / kRowGroups, lg = tid % kRowGroups;
+  const bool loads_o = tid < kLoaders, loads_v = !loads_o && tid < 2 * kLoaders;
+  const int lc = loads_o ? tid / kRowGroups : tid % kC, lg = loads_o ? tid % kRowGroups : tid / kC % kRowGroups;
   int it = 0;
 #pragma unroll 1
   for (int item = blockIdx.x, turn = 0; item < items; item += gridDim.x, ++turn) {
     const int ch = item % p.n, h = item / p.n % p.Hv, b = item / p.n / p.Hv, hk = h / p.group;
     const int rows = min(kC, p.L - ch * kC);
     const long long t0 = (long long)ch * kC;
-    if (tid == 0) {
-      const size_t at = item, atk = ((size_t)b * p.Hk + hk) * p.n + ch;
-      mbar_arrive_expect_tx(&s.bar_kq, sizeof(s.k) + sizeof(s.q) + sizeof(s.vec));
-      bulk_load(s.k, p.kimg + atk * (NP * kC * DKP), sizeof(s.k), &s.bar_kq);
-      bulk_load(s.q, p.qimg + atk * (NP * kC * DKP), sizeof(s.q), &s.bar_kq);
-      bulk_load(s.vec, p.vec + at * kVec, sizeof(s.vec), &s.bar_kq);
-    }
     const T* dOb = static_cast<const T*>(p.o.ptr) + b * p.o.sb + t0 * p.o.sl + h * p.o.sh;
     const T* Vb = static_cast<const T*>(p.v.ptr) + b * p.v.sb + t0 * p.v.sl + h * p.v.sh;
-    float xo[8], xv[8];
+    Row8<T> ahead;
     auto load_rows = [&](int v0) {
-      if (!loads) return;
       const int width = lc < rows ? p.dvw : 0;
-      load8<T>(dOb + lc * p.o.sl, v0 + 8 * lg, width, ovec, xo);
-      load8<T>(Vb + lc * p.v.sl, v0 + 8 * lg, width, vvec, xv);
+      if (loads_o) ahead.load(dOb + lc * p.o.sl, v0 + 8 * lg, width, ovec);
+      else if (loads_v) ahead.load(Vb + lc * p.v.sl, v0 + 8 * lg, width, vvec);
     };
     load_rows(0);
     float E1[NT][4], E2[NT][4], E3[NT][4], XU[2][4], OU[2][4];
@@ -891,11 +912,15 @@ __global__ void __launch_bounds__(512) delta_bwd_chunk(const __grid_constant__ D
         put_pieces<3>(x, s.x.pU[0], nullptr, off, SL * kC);
         put_pieces<3>(y, s.x.pdX[0], nullptr, off, SL * kC);
       }
-      if (loads) {
-        put_pieces<NP>(xo, s.x.pdO[0], nullptr, tile_off<SL>(lc, lg), kC * SL);
+      if (loads_o) {
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = to_f32(ahead.x[i]);
+        put_pieces<NP>(x, s.x.pdO[0], nullptr, tile_off<SL>(lc, lg), kC * SL);
+      } else if (loads_v) {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-          if (8 * lg + i < vn) dxv = fmaf(raw.dX[(8 * lg + i) * kC + lc], xv[i], dxv);
+          if (8 * lg + i < vn) dxv = fmaf(raw.dX[(8 * lg + i) * kC + lc], to_f32(ahead.x[i]), dxv);
       }
       __syncthreads();
       if (tid == 0) fetch_slab(it + 2);
@@ -1003,10 +1028,7 @@ __global__ void __launch_bounds__(512) delta_bwd_chunk(const __grid_constant__ D
         put(s.tri.Nb, beta[i] * n[0], beta[i] * n[1]);
         put(s.tri.M, m[0], m[1]);
       }
-    // dX.V over the threads of a position (kRowGroups neighbours)
-#pragma unroll
-    for (int m = 1; m < kRowGroups; m <<= 1) dxv += __shfl_xor_sync(0xffffffffu, dxv, m);
-    if (loads && lg == 0) s.dxv[lc] = dxv;
+    if (loads_v) s.dxv[lg][lc] = dxv;
     dot = group_allreduce<32, 1>(dot);
     if (lane == 0) s.sds[warp] = dot;
     __syncthreads();
@@ -1095,11 +1117,16 @@ __global__ void __launch_bounds__(512) delta_bwd_chunk(const __grid_constant__ D
         } else {
           T* dqp = static_cast<T*>(const_cast<void*>(p.dq.ptr)) + b * p.dq.sb + (t0 + i) * p.dq.sl + hk * p.dq.sh + c;
           T* dkp = static_cast<T*>(const_cast<void*>(p.dk.ptr)) + b * p.dk.sb + (t0 + i) * p.dk.sl + hk * p.dk.sh + c;
-          dqp[0] = from_f32<T>(dq[0]);
-          dkp[0] = from_f32<T>(dk[0]);
-          if (c + 1 < p.dkw) {
-            dqp[1] = from_f32<T>(dq[1]);
-            dkp[1] = from_f32<T>(dk[1]);
+          if (c + 1 < p.dkw && ((reinterpret_cast<uintptr_t>(dqp) | reinterpret_cast<uintptr_t>(dkp)) & (2 * sizeof(T) - 1)) == 0) {
+            vec_store<T, 2>(dqp, dq);
+            vec_store<T, 2>(dkp, dk);
+          } else {
+            dqp[0] = from_f32<T>(dq[0]);
+            dkp[0] = from_f32<T>(dk[0]);
+            if (c + 1 < p.dkw) {
+              dqp[1] = from_f32<T>(dq[1]);
+              dkp[1] = from_f32<T>(dk[1]);
+            }
           }
         }
       }
@@ -1113,7 +1140,10 @@ __global__ void __launch_bounds__(512) delta_bwd_chunk(const __grid_constant__ D
         const float kH = sum(1);
         dG[i] = sum(0) + beta[r] * kH - sum(2);
         tail += sum(3);
-        if (r < rows) p.dbeta[((size_t)b * p.L + t0 + r) * p.Hv + h] = s.dxv[r] + kH;
+        float xv = 0.0f;
+#pragma unroll
+        for (int k = 0; k < kRowGroups; ++k) xv += s.dxv[k][r];
+        if (r < rows) p.dbeta[((size_t)b * p.L + t0 + r) * p.Hv + h] = xv + kH;
       }
       tail = group_allreduce<32, 1>(tail);
       float sds = 0.0f;
@@ -1129,8 +1159,11 @@ __global__ void __launch_bounds__(512) delta_bwd_chunk(const __grid_constant__ D
       run += tail;
       if (2 * lane < rows) p.dg[((size_t)b * p.L + t0 + 2 * lane) * p.Hv + h] = run;
       if (2 * lane + 1 < rows) p.dg[((size_t)b * p.L + t0 + 2 * lane + 1) * p.Hv + h] = run - dG[0];
+      // every warp is past the tiles (the barrier above)
+      __syncwarp();
+      if (lane == 0) fetch_tiles(item + gridDim.x);
     }
-    __syncthreads();              // the next item writes over all of this
+    __syncthreads();          // measured 5 % faster than letting the others run ahead of warp 0
   }
 }
 
@@ -1313,22 +1346,38 @@ struct Carver {
   }
 };
 
-// The workspace's parts; with base null only its size is of use.
-size_t carve(const Shape& s, bool bwd, DeltaParams& p, unsigned char* base) {
-  Carver c{base};
+// The parts of a buffer; with base null only its size is of use.  Everything delta_prep writes:
+void carve_prep(const Shape& s, DeltaParams& p, Carver& c) {
   const size_t chunks_k = (size_t)s.B * s.Hk * s.n(), chunks = (size_t)s.B * s.Hv * s.n();
   p.kimg = c.take<__nv_bfloat16>(chunks_k * s.np() * kC * s.dkp());
   p.qimg = c.take<__nv_bfloat16>(chunks_k * s.np() * kC * s.dkp());
   p.timg = c.take<__nv_bfloat16>(chunks * 3 * kTri);
   p.pimg = c.take<__nv_bfloat16>(chunks * 3 * kTri);
   p.vec = c.take<float>(chunks * kVec);
-  if (bwd) {
-    p.dstates = c.take<float>(chunks * s.dvp() * s.dkp());
-    p.dxs = c.take<float>(chunks * s.dvp() * kC);
-    if (s.Hv > s.Hk) {
-      p.pdq = c.take<float>((size_t)s.B * s.L * s.Hv * s.dkp());
-      p.pdk = c.take<float>((size_t)s.B * s.L * s.Hv * s.dkp());
-    }
+}
+// What a training forward leaves for the backward: that (again computing it took 10 % of a training pass), the
+// states and the corrected values.
+size_t carve_saved(const Shape& s, DeltaParams& p, unsigned char* base) {
+  Carver c{base};
+  carve_prep(s, p, c);
+  const size_t chunks = (size_t)s.B * s.Hv * s.n();
+  p.states = c.take<float>(chunks * s.dvp() * s.dkp());
+  p.us = c.take<float>(chunks * s.dvp() * kC);
+  return c.used + 256;
+}
+size_t carve_fwd(const Shape& s, DeltaParams& p, unsigned char* base) {
+  Carver c{base};
+  carve_prep(s, p, c);
+  return c.used + 256;
+}
+size_t carve_bwd(const Shape& s, DeltaParams& p, unsigned char* base) {
+  Carver c{base};
+  const size_t chunks = (size_t)s.B * s.Hv * s.n();
+  p.dstates = c.take<float>(chunks * s.dvp() * s.dkp());
+  p.dxs = c.take<float>(chunks * s.dvp() * kC);
+  if (s.Hv > s.Hk) {
+    p.pdq = c.take<float>((size_t)s.B * s.L * s.Hv * s.dkp());
+    p.pdk = c.take<float>((size_t)s.B * s.L * s.Hv * s.dkp());
   }
   return c.used + 256;
 }
@@ -1398,16 +1447,15 @@ cudaError_t run_chain(const Shape& s, const DeltaParams& p, bool bwd, cudaStream
   return cudaErrorInvalidValue;
 }
 template <typename T, int NP, int DKP>
-cudaError_t run_prep_and_chain(const Shape& s, const DeltaParams& p, bool bwd, cudaStream_t st) {
+cudaError_t run_fwd(const Shape& s, const DeltaParams& p, cudaStream_t st) {
   const dim3 grid((unsigned)s.n(), (unsigned)s.Hv, (unsigned)s.B);
   const cudaError_t e = launch<delta_prep<T, NP, DKP>>(grid, 128, sizeof(PrepSmem<NP, DKP>), p, st);
-  if (e != cudaSuccess) return e;
-  return run_chain<T, NP, DKP>(s, p, bwd, st);
+  return e != cudaSuccess ? e : run_chain<T, NP, DKP>(s, p, false, st);
 }
 
 template <typename T, int NP, int DKP>
 cudaError_t run_bwd(const Shape& s, const DeltaParams& p, cudaStream_t st) {
-  cudaError_t e = run_prep_and_chain<T, NP, DKP>(s, p, true, st);
+  cudaError_t e = run_chain<T, NP, DKP>(s, p, true, st);
   if (e != cudaSuccess) return e;
   constexpr int SL = NP == 3 && DKP == 128 ? 16 : 32;     // what shared memory holds beside six tiles of pieces
   const dim3 bg((unsigned)std::min<int64_t>(s.n() * s.Hv * s.B, 148));       // one CTA per SM walks over the chunks
@@ -1442,7 +1490,8 @@ int ssm_gated_delta_workspace_size(int64_t B, int64_t L, int64_t Hk, int64_t Hv,
   int rc = check_shape(s);
   if (rc) return rc;
   DeltaParams p;
-  *bytes = carve(s, backward != 0, p, nullptr);
+  memset(&p, 0, sizeof(p));
+  *bytes = backward ? carve_bwd(s, p, nullptr) : carve_fwd(s, p, nullptr);
   return SSM_OK;
 }
 
@@ -1452,13 +1501,10 @@ int ssm_gated_delta_saved_size(int64_t B, int64_t L, int64_t Hk, int64_t Hv, int
   const Shape s{B, L, Hk, Hv, dk, dv, dtype};
   int rc = check_shape(s);
   if (rc) return rc;
-  *bytes = (size_t)B * Hv * s.n() * s.dvp() * (s.dkp() + kC) * sizeof(float) + 256;
+  DeltaParams p;
+  memset(&p, 0, sizeof(p));
+  *bytes = carve_saved(s, p, nullptr);
   return SSM_OK;
-}
-
-static void saved_parts(const Shape& s, void* saved, DeltaParams& p) {
-  p.states = reinterpret_cast<float*>(align256(saved));
-  p.us = p.states + (size_t)s.B * s.Hv * s.n() * s.dvp() * s.dkp();
 }
 
 int ssm_gated_delta_fwd(int64_t B, int64_t L, int64_t Hk, int64_t Hv, int64_t dk, int64_t dv, ssm_heads q, ssm_heads k,
@@ -1472,24 +1518,27 @@ int ssm_gated_delta_fwd(int64_t B, int64_t L, int64_t Hk, int64_t Hv, int64_t dk
     return rc;
   DeltaParams p;
   memset(&p, 0, sizeof(p));
-  const size_t need = carve(s, false, p, nullptr);
-  if (workspace == nullptr || workspace_bytes < need)
-    return fail(SSM_ERR_WORKSPACE, "gated delta rule: forward workspace of %zu bytes required, %zu given", need,
-                workspace_bytes);
-  carve(s, false, p, align256(workspace));
+  if (saved != nullptr) {          // a training call needs no workspace beside it
+    carve_saved(s, p, align256(saved));
+  } else {
+    const size_t need = carve_fwd(s, p, nullptr);
+    if (workspace == nullptr || workspace_bytes < need)
+      return fail(SSM_ERR_WORKSPACE, "gated delta rule: forward workspace of %zu bytes required, %zu given", need,
+                  workspace_bytes);
+    carve_fwd(s, p, align256(workspace));
+  }
   fill(p, s, q, k, v, g, beta, scale);
   p.o = heads(o);
   p.h0 = h0;
   p.last = last;
-  if (saved != nullptr) saved_parts(s, saved, p);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e;
   if (s.dtype == SSM_BF16)
-    e = s.dkp() == 64 ? run_prep_and_chain<__nv_bfloat16, 1, 64>(s, p, false, st)
-                      : run_prep_and_chain<__nv_bfloat16, 1, 128>(s, p, false, st);
+    e = s.dkp() == 64 ? run_fwd<__nv_bfloat16, 1, 64>(s, p, st)
+                      : run_fwd<__nv_bfloat16, 1, 128>(s, p, st);
   else
-    e = s.dkp() == 64 ? run_prep_and_chain<float, 3, 64>(s, p, false, st)
-                      : run_prep_and_chain<float, 3, 128>(s, p, false, st);
+    e = s.dkp() == 64 ? run_fwd<float, 3, 64>(s, p, st)
+                      : run_fwd<float, 3, 128>(s, p, st);
   if (e != cudaSuccess) return fail(SSM_ERR_CUDA, "gated delta rule forward: %s", cudaGetErrorString(e));
   return SSM_OK;
 }
@@ -1510,13 +1559,13 @@ int ssm_gated_delta_bwd(int64_t B, int64_t L, int64_t Hk, int64_t Hv, int64_t dk
     return fail(SSM_ERR_INVALID, "gated delta rule: saved, dg and dbeta are required");
   DeltaParams p;
   memset(&p, 0, sizeof(p));
-  const size_t need = carve(s, true, p, nullptr);
+  const size_t need = carve_bwd(s, p, nullptr);
   if (workspace == nullptr || workspace_bytes < need)
     return fail(SSM_ERR_WORKSPACE, "gated delta rule: backward workspace of %zu bytes required, %zu given", need,
                 workspace_bytes);
-  carve(s, true, p, align256(workspace));
+  carve_bwd(s, p, align256(workspace));
   fill(p, s, q, k, v, g, beta, scale);
-  saved_parts(s, const_cast<void*>(saved), p);
+  carve_saved(s, p, align256(const_cast<void*>(saved)));
   p.o = heads(d_o);
   p.dq = heads(d_q);
   p.dk = heads(d_k);

@@ -70,19 +70,19 @@ def _bytes(n, dev):
 def _forward(dims, q, k, v, g, beta, h0, scale, save):
     B, L, Hk, Hv, dk, dv = dims
     dev, dtype = q.device, q.dtype
-    o = torch.empty((B, L, Hv, dv), dtype=dtype, device=dev)
-    last = torch.empty((B, Hv, dk, dv), dtype=torch.float32, device=dev)
+    o = v.new_empty((B, L, Hv, dv))
+    last = g.new_empty((B, Hv, dk, dv))
     saved = _bytes(nat.gated_delta_saved_bytes(dims, dtype), dev) if save else None
-    wsb = nat.gated_delta_workspace_bytes(dims, dtype, False)
-    ws = _bytes(wsb, dev)
+    wsb = 0 if save else nat.gated_delta_workspace_bytes(dims, dtype, False)
+    ws = None if save else _bytes(wsb, dev)
     nat.call("ssm_gated_delta_fwd", dev, *dims, nat.heads4(q), nat.heads4(k), nat.heads4(v), nat.view3(g),
-             nat.view3(beta), nat.ptr(h0), scale, nat.heads4(o), last.data_ptr(), nat.ptr(saved), ws.data_ptr(), wsb)
+             nat.view3(beta), nat.ptr(h0), scale, nat.heads4(o), last.data_ptr(), nat.ptr(saved), nat.ptr(ws), wsb)
     return o, last, saved
 
 
 class GatedDeltaFn(torch.autograd.Function):
-    """(o, last) of the gated delta rule.  Keeps the state entering every 64 positions and the chunks'
-    corrected values for the backward."""
+    """(o, last) of the gated delta rule.  Keeps the state entering every 64 positions, the chunks' triangular
+    factors and corrected values for the backward."""
 
     @staticmethod
     def forward(ctx, q, k, v, g, beta, h0, scale, dims):
@@ -99,8 +99,8 @@ class GatedDeltaFn(torch.autograd.Function):
         do = _act(do, dtype)
         if dlast is not None:
             dlast = dlast.to(torch.float32).contiguous()
-        dq, dk, dv = (torch.empty(t.shape, dtype=dtype, device=dev) for t in (q, k, v))
-        dg, dbeta = (torch.empty(g.shape, dtype=torch.float32, device=dev) for _ in range(2))
+        dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
+        dg, dbeta = g.new_empty(g.shape), g.new_empty(g.shape)
         dh0 = None if h0 is None else torch.empty_like(h0)
         wsb = nat.gated_delta_workspace_bytes(dims, dtype, True)
         ws = _bytes(wsb, dev)
@@ -142,7 +142,7 @@ def gated_delta_state_update(state, q, k, v, g, beta, scale=None, out=None):
     q, k, v = _act(q, ct), _act(k, ct), _act(v, ct)
     g, beta = _act(g, torch.float32), _act(beta, torch.float32)
     if out is None:
-        o = torch.empty((B, Hv, dv), dtype=ct, device=dev)
+        o = v.new_empty((B, Hv, dv))
     else:
         if out.shape != (B, Hv, dv) or out.dtype != ct or out.device != dev or (out.stride(-1) != 1 and dv != 1):
             raise ValueError(f"out must be a ({B}, {Hv}, {dv}) {ct} tensor with unit inner stride")
