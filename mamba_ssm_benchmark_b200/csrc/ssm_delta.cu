@@ -11,6 +11,7 @@
 
 #include "ssm_b200.h"
 #include "ssm_delta.cuh"
+#include "ssm_delta_tc.cuh"
 #include "ssm_launch.cuh"
 #include "ssm_vec.cuh"
 
@@ -887,7 +888,7 @@ __global__ void __launch_bounds__(512) delta_bwd_chunk(const __grid_constant__ D
       mbar_wait(&s.bar_slab[it & 1], (it >> 1) & 1, p.err);
       // split the slab
       for (int e = tid; e < SL * DKP / 8; e += 512) {
-        const int r = e / (DKP / 8), grp = e % (DKP / 8), off = tile_off<DKP>(r, grp);
+        const int r = e / (DKP / 8), grp = e % (DKP / 8), off = tile_off<DKP, SL>(r, grp);
         float x[8], y[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] = y[i] = 0.0f;
@@ -901,7 +902,7 @@ __global__ void __launch_bounds__(512) delta_bwd_chunk(const __grid_constant__ D
         put_pieces<3>(y, s.x.pdS[0], nullptr, off, SL * DKP);
       }
       for (int e = tid; e < SL * kC / 8; e += 512) {
-        const int r = e / (kC / 8), grp = e % (kC / 8), off = tile_off<kC>(r, grp);
+        const int r = e / (kC / 8), grp = e % (kC / 8), off = tile_off<kC, SL>(r, grp);
         float x[8], y[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] = y[i] = 0.0f;
@@ -936,8 +937,8 @@ __global__ void __launch_bounds__(512) delta_bwd_chunk(const __grid_constant__ D
         for (int i = 0; i < NP; ++i) load_a<SL>(ao[k][i], tO + i * (kC * SL * 2), row0, k, lane);
 #pragma unroll
         for (int i = 0; i < 3; ++i) {
-          load_at<kC>(ax[k][i], tX + i * (SL * kC * 2), row0, k, lane);
-          load_at<kC>(au[k][i], tU + i * (SL * kC * 2), row0, k, lane);
+          load_at<kC, SL>(ax[k][i], tX + i * (SL * kC * 2), row0, k, lane);
+          load_at<kC, SL>(au[k][i], tU + i * (SL * kC * 2), row0, k, lane);
         }
       }
 #pragma unroll
@@ -951,8 +952,8 @@ __global__ void __launch_bounds__(512) delta_bwd_chunk(const __grid_constant__ D
         for (int pb = 2; pb >= 0; --pb)
 #pragma unroll
           for (int k = 0; k < KS; ++k) {
-            load_bt<DKP>(bs[k][0], tS + pb * (SL * DKP * 2), quarter * NT + 2 * jp, k, lane);
-            load_bt<DKP>(bd[k][0], tdS + pb * (SL * DKP * 2), quarter * NT + 2 * jp, k, lane);
+            load_bt<DKP, SL>(bs[k][0], tS + pb * (SL * DKP * 2), quarter * NT + 2 * jp, k, lane);
+            load_bt<DKP, SL>(bd[k][0], tdS + pb * (SL * DKP * 2), quarter * NT + 2 * jp, k, lane);
             mma_pieces<1, 2>(d1, 0, ao[k], bs[k], pb);
             mma_pieces<1, 2>(d2, 0, ax[k], bs[k], pb);
             mma_pieces<1, 2>(d3, 0, au[k], bd[k], pb);
@@ -981,7 +982,7 @@ __global__ void __launch_bounds__(512) delta_bwd_chunk(const __grid_constant__ D
         for (int pb = 2; pb >= 0; --pb)
 #pragma unroll
           for (int k = 0; k < KS; ++k) {
-            load_bt<kC>(bu[k][0], tU + pb * (SL * kC * 2), 2 * quarter, k, lane);
+            load_bt<kC, SL>(bu[k][0], tU + pb * (SL * kC * 2), 2 * quarter, k, lane);
             mma_pieces<1, 2>(d1, 0, ao[k], bu[k], pb);
             mma_pieces<1, 2>(d2, 0, ax[k], bu[k], pb);
           }
@@ -1436,9 +1437,20 @@ cudaError_t run_chain_ns(const Shape& s, const DeltaParams& p, bool bwd, cudaStr
   }
 }
 template <typename T, int NP, int DKP>
+cudaError_t run_chain_tc(const Shape& s, const DeltaParams& p, bool bwd, cudaStream_t st) {
+  const dim3 grid((unsigned)((s.dv + 127) / 128), (unsigned)s.Hv, (unsigned)s.B);
+  constexpr size_t fwd = sizeof(TcSmem<NP, DKP, NP == 1 ? 2 : 3>) + 1024, back = sizeof(TcSmem<NP, DKP, 3>) + 1024;
+  static_assert(back <= 227 * 1024, "two stages of tiles");
+  if (bwd) return launch<delta_bwd_tc<T, NP, DKP>>(grid, kTcThreads, back, p, st);
+  return p.states != nullptr ? launch<delta_fwd_tc<T, NP, DKP, true>>(grid, kTcThreads, fwd, p, st)
+                             : launch<delta_fwd_tc<T, NP, DKP, false>>(grid, kTcThreads, fwd, p, st);
+}
+template <typename T, int NP, int DKP>
 cudaError_t run_chain(const Shape& s, const DeltaParams& p, bool bwd, cudaStream_t st) {
   const int64_t tiles = s.dvp() / 16, strips = s.B * s.Hv * tiles;
   constexpr bool wide = NP == 3 && DKP == 128;       // six tiles of pieces leave room for one strip
+  if constexpr (!wide)
+    if (strips > 148) return run_chain_tc<T, NP, DKP>(s, p, bwd, st);
   if (wide || tiles == 1 || strips <= 148) return run_chain_ns<T, NP, DKP, 1>(s, p, bwd, st);
   if constexpr (!wide) {
     if (NP == 3 || tiles == 2 || strips <= 2 * 148) return run_chain_ns<T, NP, DKP, 2>(s, p, bwd, st);

@@ -68,35 +68,37 @@ __device__ __forceinline__ void split(float x0, float x1, uint32_t (&p)[NP]) {
   }
 }
 
-// Element offset of 8-element column group `grp` of row `row` in a (rows x W) bf16 tile whose 16-byte
-// groups are permuted by the row, so that the eight rows of an ldmatrix hit different banks.
-template <int W>
+// Element offset of 8-element column group `grp` of row `row` in a (ROWS x W) bf16 tile.  Its 16-byte groups are
+// permuted by the row, so that the eight rows of an ldmatrix hit different banks; a tile of 128 columns is two of 64
+// behind one another.  For ROWS = 64 that is the 128-byte swizzle that tcgen05's descriptors name.
+template <int W, int ROWS = kC>
 __device__ __forceinline__ int tile_off(int row, int grp) {
-  static_assert(W == 16 || W == 32 || W >= 64, "rows of 32, 64 or a multiple of 128 bytes");
-  const int s = W >= 64 ? row & 7 : W == 32 ? (row >> 1) & 3 : (row >> 2) & 1;
+  static_assert(W == 16 || W == 32 || W == 64 || W == 128, "rows of 32, 64 or 128 bytes, or two of these");
+  if (W == 128) return (grp >> 3) * (ROWS * 64) + row * 64 + (((grp & 7) ^ (row & 7)) << 3);
+  const int s = W == 64 ? row & 7 : W == 32 ? (row >> 1) & 3 : (row >> 2) & 1;
   return row * W + ((grp ^ s) << 3);
 }
 
 // B fragments of n tiles j, j + 1 (r[0..1], r[2..3]) and k block kb from a tile stored [n][k].
-template <int W>
+template <int W, int ROWS = kC>
 __device__ __forceinline__ void load_b(uint32_t (&r)[4], uint32_t tile, int j, int kb, int lane) {
-  ldsm4(r, tile + 2 * tile_off<W>(8 * (j + (lane >> 4)) + (lane & 7), 2 * kb + ((lane >> 3) & 1)));
+  ldsm4(r, tile + 2 * tile_off<W, ROWS>(8 * (j + (lane >> 4)) + (lane & 7), 2 * kb + ((lane >> 3) & 1)));
 }
 // The same from a tile stored [k][n].
-template <int W>
+template <int W, int ROWS = kC>
 __device__ __forceinline__ void load_bt(uint32_t (&r)[4], uint32_t tile, int j, int kb, int lane) {
-  ldsm4t(r, tile + 2 * tile_off<W>(16 * kb + (lane & 15), j + (lane >> 4)));
+  ldsm4t(r, tile + 2 * tile_off<W, ROWS>(16 * kb + (lane & 15), j + (lane >> 4)));
 }
 // A fragment of the 16 rows from `row` and k block kb from a tile stored [m][k].
-template <int W>
+template <int W, int ROWS = kC>
 __device__ __forceinline__ void load_a(uint32_t (&r)[4], uint32_t tile, int row, int kb, int lane) {
-  ldsm4(r, tile + 2 * tile_off<W>(row + (lane & 15), 2 * kb + (lane >> 4)));
+  ldsm4(r, tile + 2 * tile_off<W, ROWS>(row + (lane & 15), 2 * kb + (lane >> 4)));
 }
 
 // The same from a tile stored [k][m].
-template <int W>
+template <int W, int ROWS = kC>
 __device__ __forceinline__ void load_at(uint32_t (&r)[4], uint32_t tile, int row, int kb, int lane) {
-  ldsm4t(r, tile + 2 * tile_off<W>(16 * kb + 8 * (lane >> 4) + (lane & 7), row / 8 + ((lane >> 3) & 1)));
+  ldsm4t(r, tile + 2 * tile_off<W, ROWS>(16 * kb + 8 * (lane >> 4) + (lane & 7), row / 8 + ((lane >> 3) & 1)));
 }
 
 // The A operand of k block kb from accumulator tiles 2 kb, 2 kb + 1, in NP pieces.
@@ -270,13 +272,13 @@ __device__ __forceinline__ void get_frag(uint32_t (&a)[4], const uint4& f) {
   a[3] = f.w;
 }
 // B fragments of the warp's two column tiles from a tile stored [n][k] / [k][n].
-template <int W>
+template <int W, int ROWS = kC>
 __device__ __forceinline__ void load_b2(uint32_t (&r)[4], uint32_t tile, int w, int kb, int lane) {
-  ldsm4(r, tile + 2 * tile_off<W>(8 * col_tile(w, lane >> 4) + (lane & 7), 2 * kb + ((lane >> 3) & 1)));
+  ldsm4(r, tile + 2 * tile_off<W, ROWS>(8 * col_tile(w, lane >> 4) + (lane & 7), 2 * kb + ((lane >> 3) & 1)));
 }
-template <int W>
+template <int W, int ROWS = kC>
 __device__ __forceinline__ void load_bt2(uint32_t (&r)[4], uint32_t tile, int w, int kb, int lane) {
-  ldsm4t(r, tile + 2 * tile_off<W>(16 * kb + (lane & 15), col_tile(w, lane >> 4)));
+  ldsm4t(r, tile + 2 * tile_off<W, ROWS>(16 * kb + (lane & 15), col_tile(w, lane >> 4)));
 }
 
 // 16 rows of a dense fp32 [channel][W] tile from / to accumulators.

@@ -61,6 +61,8 @@ def _compare(got, want):
 SHAPES = [
     (1, 1, 1, 1, 64, 64), (2, 2, 1, 2, 16, 8), (1, 63, 2, 2, 64, 48), (2, 64, 2, 4, 32, 16), (1, 65, 1, 3, 128, 33),
     (2, 130, 2, 2, 17, 80), (1, 200, 2, 4, 65, 17), (3, 129, 1, 1, 1, 1), (1, 96, 2, 2, 128, 160), (1, 320, 1, 1, 100, 7),
+    # enough heads to fill the GPU
+    (5, 70, 4, 8, 64, 64), (3, 200, 8, 16, 100, 80), (2, 65, 5, 10, 128, 160), (20, 33, 4, 8, 16, 16), (40, 130, 2, 4, 48, 33),
 ]
 
 
