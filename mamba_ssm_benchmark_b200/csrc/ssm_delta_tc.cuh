@@ -32,13 +32,16 @@ __device__ __forceinline__ void tc_commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
                : "memory");
 }
-// D (128 x N, fp32) (+)= A (128 x 16 bf16, tensor memory) x B (16 x N bf16, shared memory)
+// D (128 x N, fp32) (+)= A (128 x 16 bf16, tensor memory) x B (16 x N bf16, shared memory), issued by the lane whose
+// `issue` is set.  The whole warp calls it with the same operands, which thus stay in uniform registers: from a
+// branch that one lane takes, each instruction cost 53 clocks to issue.
 __device__ __forceinline__ void tc_mma(uint32_t d, uint32_t a, uint32_t b, uint32_t b_high, uint32_t idesc,
-                                       bool accumulate) {
+                                       bool accumulate, uint32_t issue) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\tsetp.ne.b32 p, %5, 0;\n\tmov.b64 b, {%2, %3};\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}" ::"r"(d),
-      "r"(a), "r"(b), "r"(b_high), "r"(idesc), "r"((uint32_t)accumulate)
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 b;\n\tsetp.ne.b32 p, %5, 0;\n\tsetp.ne.b32 q, %6, 0;\n\t"
+      "mov.b64 b, {%2, %3};\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(b_high), "r"(idesc), "r"((uint32_t)accumulate), "r"(issue)
       : "memory");
 }
 // 32 columns of this warp's 32 lanes
@@ -144,7 +147,7 @@ struct TcWait {
   }
 };
 
-// ---- products, issued by one thread -----------------------------------------------------------
+// ---- products, issued by one warp -------------------------------------------------------------
 // Which products of pieces: LOW: index sums 1 .. MAXI; else the leading one.
 // d (N columns) += A (NA pieces, K / 2 columns apart) x tile of NB pieces, over K / 16 steps.
 //   FULL   B [n][k] of 64 rows, K = DKP: both halves of a (kC x DKP) tile
@@ -152,7 +155,8 @@ struct TcWait {
 //   LOWER  B [n][k], K = 64, N = 64, zero above the diagonal;  UPPER  the same read across, [k][n]
 enum TcForm { kFull, kAcross, kLower, kUpper };
 template <TcForm FORM, int NA, int NB, int MAXI, int DKP>
-__device__ __forceinline__ void tc_product(uint32_t d, uint32_t a, uint32_t tile, bool lead, bool& started) {
+__device__ __forceinline__ void tc_product(uint32_t d, uint32_t a, uint32_t tile, bool lead, bool& started,
+                                           uint32_t issue) {
   constexpr int kSteps = (FORM == kFull ? DKP : kC) / 16, kTile = (FORM == kLower || FORM == kUpper ? kTri : kC * DKP) * 2;
   const uint32_t base = tc_desc(tile, FORM == kAcross ? kC * 64 * 2 : 16);
 #pragma unroll
@@ -165,22 +169,22 @@ __device__ __forceinline__ void tc_product(uint32_t d, uint32_t a, uint32_t tile
         const int s = FORM == kUpper ? kSteps - 1 - s0 : s0;       // the step that covers all columns comes first
         const uint32_t as = a + i * (kSteps * 8) + s * 8, bt = base + j * (kTile / 16);
         if (FORM == kFull)
-          tc_mma(d, as, bt + ((s >> 2) * (kC * 64 * 2) + (s & 3) * 32) / 16, kTcDescHigh, tc_idesc<false>(64), started);
+          tc_mma(d, as, bt + ((s >> 2) * (kC * 64 * 2) + (s & 3) * 32) / 16, kTcDescHigh, tc_idesc<false>(64), started, issue);
         else if (FORM == kAcross)
-          tc_mma(d, as, bt + s * (2048 / 16), kTcDescHigh, tc_idesc<true>(DKP), started);
+          tc_mma(d, as, bt + s * (2048 / 16), kTcDescHigh, tc_idesc<true>(DKP), started, issue);
         else if (FORM == kLower)         // columns from 16 s
-          tc_mma(d + 16 * s, as, bt + s * ((2048 + 32) / 16), kTcDescHigh, tc_idesc<false>(kC - 16 * s), started);
+          tc_mma(d + 16 * s, as, bt + s * ((2048 + 32) / 16), kTcDescHigh, tc_idesc<false>(kC - 16 * s), started, issue);
         else                             // columns below 16 (s + 1)
-          tc_mma(d, as, bt + s * (2048 / 16), kTcDescHigh, tc_idesc<true>(16 * (s + 1)), started);
+          tc_mma(d, as, bt + s * (2048 / 16), kTcDescHigh, tc_idesc<true>(16 * (s + 1)), started, issue);
         started = true;
       }
     }
 }
 template <TcForm FORM, int NA, int NB, int MAXI, int DKP>
-__device__ __forceinline__ void tc_full_product(uint32_t d, uint32_t a, uint32_t tile) {
+__device__ __forceinline__ void tc_full_product(uint32_t d, uint32_t a, uint32_t tile, uint32_t issue) {
   bool started = false;
-  tc_product<FORM, NA, NB, MAXI, DKP>(d, a, tile, false, started);
-  tc_product<FORM, NA, NB, MAXI, DKP>(d, a, tile, true, started);
+  tc_product<FORM, NA, NB, MAXI, DKP>(d, a, tile, false, started, issue);
+  tc_product<FORM, NA, NB, MAXI, DKP>(d, a, tile, true, started, issue);
 }
 
 template <int NP, int DKP, int PP>
@@ -286,33 +290,32 @@ __global__ void __launch_bounds__(kTcThreads, 1) delta_fwd_tc(const __grid_const
   Smem& s = tc_smem<Smem>();
   const int h = blockIdx.y, b = blockIdx.z, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   tc_init(s);
-  const uint32_t tm = s.tmem;
+  const uint32_t tm = __shfl_sync(0xffffffffu, s.tmem, 0);
   TcWait wait{p.err};
   if (warp == 8) {
-    if (lane == 0) {
-      for (int i = 0; i < 2 && i < p.n; ++i) tc_load_stage(s, p, b, h, i, i);
-      for (int ch = 0; ch < p.n; ++ch) {
-        const int st = ch & 1, par = ch & 1;
-        auto& g = s.stage[st];
-        const uint32_t sk = smem_u32(g.k), sq = smem_u32(g.q), stt = smem_u32(g.t), sp = smem_u32(g.pm);
-        wait(&s.full[st], (ch >> 1) & 1);
-        wait(&s.ready[0], par);
-        tc_fence_after();
-        tc_full_product<kFull, 3, NP, 2, DKP>(tm + kTcD, tm + kTcS, sk);
-        tc_full_product<kFull, 3, NP, PP - 1, DKP>(tm + kTcO, tm + kTcS, sq);
-        tc_commit(&s.done[0]);
-        // every thread is past the last chunk, whose stage is free
-        if (ch >= 1 && ch + 1 < p.n) tc_load_stage(s, p, b, h, ch + 1, st ^ 1);
-        wait(&s.ready[1], par);
-        tc_fence_after();
-        tc_full_product<kLower, 3, 3, 2, DKP>(tm + kTcD, tm + kTcX, stt);
-        tc_commit(&s.done[1]);
-        wait(&s.ready[2], par);
-        tc_fence_after();
-        tc_full_product<kAcross, 3, NP, 2, DKP>(tm + kTcD, tm + kTcLU, sk);
-        tc_full_product<kLower, PP, PP, PP - 1, DKP>(tm + kTcX, tm + kTcU, sp);
-        tc_commit(&s.done[2]);
-      }
+    const uint32_t issue = lane == 0;
+    for (int i = 0; issue && i < 2 && i < p.n; ++i) tc_load_stage(s, p, b, h, i, i);
+    for (int ch = 0; ch < p.n; ++ch) {
+      const int st = ch & 1, par = ch & 1;
+      auto& g = s.stage[st];
+      const uint32_t sk = smem_u32(g.k), sq = smem_u32(g.q), stt = smem_u32(g.t), sp = smem_u32(g.pm);
+      wait(&s.full[st], (ch >> 1) & 1);
+      wait(&s.ready[0], par);
+      tc_fence_after();
+      tc_full_product<kFull, 3, NP, 2, DKP>(tm + kTcD, tm + kTcS, sk, issue);
+      tc_full_product<kFull, 3, NP, PP - 1, DKP>(tm + kTcO, tm + kTcS, sq, issue);
+      if (issue) tc_commit(&s.done[0]);
+      // every thread is past the last chunk, whose stage is free
+      if (issue && ch >= 1 && ch + 1 < p.n) tc_load_stage(s, p, b, h, ch + 1, st ^ 1);
+      wait(&s.ready[1], par);
+      tc_fence_after();
+      tc_full_product<kLower, 3, 3, 2, DKP>(tm + kTcD, tm + kTcX, stt, issue);
+      if (issue) tc_commit(&s.done[1]);
+      wait(&s.ready[2], par);
+      tc_fence_after();
+      tc_full_product<kAcross, 3, NP, 2, DKP>(tm + kTcD, tm + kTcLU, sk, issue);
+      tc_full_product<kLower, PP, PP, PP - 1, DKP>(tm + kTcX, tm + kTcU, sp, issue);
+      if (issue) tc_commit(&s.done[2]);
     }
     __syncwarp();
   } else {
@@ -399,35 +402,34 @@ __global__ void __launch_bounds__(kTcThreads, 1) delta_bwd_tc(const __grid_const
   Smem& s = tc_smem<Smem>();
   const int h = blockIdx.y, b = blockIdx.z, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   tc_init(s);
-  const uint32_t tm = s.tmem;
+  const uint32_t tm = __shfl_sync(0xffffffffu, s.tmem, 0);
   TcWait wait{p.err};
   if (warp == 8) {
-    if (lane == 0) {
-      for (int i = 0; i < 2 && i < p.n; ++i) tc_load_stage(s, p, b, h, p.n - 1 - i, i);
-      for (int it = 0; it < p.n; ++it) {
-        const int st = it & 1, par = it & 1;
-        auto& g = s.stage[st];
-        const uint32_t sk = smem_u32(g.k), sq = smem_u32(g.q), stt = smem_u32(g.t), sp = smem_u32(g.pm);
-        wait(&s.full[st], (it >> 1) & 1);
-        wait(&s.ready[0], par);
-        tc_fence_after();
-        tc_full_product<kFull, 3, NP, 2, DKP>(tm + kTcD, tm + kTcS, sk);
-        tc_full_product<kUpper, NP, 3, 2, DKP>(tm + kTcD2, tm + kTcO, sp);
-        tc_commit(&s.done[0]);
-        if (it >= 1 && it + 1 < p.n) tc_load_stage(s, p, b, h, p.n - 2 - it, st ^ 1);
-        wait(&s.ready[1], par);
-        tc_fence_after();
-        tc_full_product<kUpper, 3, 3, 2, DKP>(tm + kTcD, tm + kTcU, stt);
-        tc_commit(&s.done[1]);
-        wait(&s.ready[2], par);
-        tc_fence_after();
-        bool started = false;
-        tc_product<kAcross, 3, NP, 2, DKP>(tm + kTcD, tm + kTcG, sq, false, started);
-        tc_product<kAcross, 3, NP, 2, DKP>(tm + kTcD, tm + kTcLU, sk, false, started);
-        tc_product<kAcross, 3, NP, 2, DKP>(tm + kTcD, tm + kTcG, sq, true, started);
-        tc_product<kAcross, 3, NP, 2, DKP>(tm + kTcD, tm + kTcLU, sk, true, started);
-        tc_commit(&s.done[2]);
-      }
+    const uint32_t issue = lane == 0;
+    for (int i = 0; issue && i < 2 && i < p.n; ++i) tc_load_stage(s, p, b, h, p.n - 1 - i, i);
+    for (int it = 0; it < p.n; ++it) {
+      const int st = it & 1, par = it & 1;
+      auto& g = s.stage[st];
+      const uint32_t sk = smem_u32(g.k), sq = smem_u32(g.q), stt = smem_u32(g.t), sp = smem_u32(g.pm);
+      wait(&s.full[st], (it >> 1) & 1);
+      wait(&s.ready[0], par);
+      tc_fence_after();
+      tc_full_product<kFull, 3, NP, 2, DKP>(tm + kTcD, tm + kTcS, sk, issue);
+      tc_full_product<kUpper, NP, 3, 2, DKP>(tm + kTcD2, tm + kTcO, sp, issue);
+      if (issue) tc_commit(&s.done[0]);
+      if (issue && it >= 1 && it + 1 < p.n) tc_load_stage(s, p, b, h, p.n - 2 - it, st ^ 1);
+      wait(&s.ready[1], par);
+      tc_fence_after();
+      tc_full_product<kUpper, 3, 3, 2, DKP>(tm + kTcD, tm + kTcU, stt, issue);
+      if (issue) tc_commit(&s.done[1]);
+      wait(&s.ready[2], par);
+      tc_fence_after();
+      bool started = false;
+      tc_product<kAcross, 3, NP, 2, DKP>(tm + kTcD, tm + kTcG, sq, false, started, issue);
+      tc_product<kAcross, 3, NP, 2, DKP>(tm + kTcD, tm + kTcLU, sk, false, started, issue);
+      tc_product<kAcross, 3, NP, 2, DKP>(tm + kTcD, tm + kTcG, sq, true, started, issue);
+      tc_product<kAcross, 3, NP, 2, DKP>(tm + kTcD, tm + kTcLU, sk, true, started, issue);
+      if (issue) tc_commit(&s.done[2]);
     }
     __syncwarp();
   } else {
