@@ -326,10 +326,12 @@ __global__ void __launch_bounds__(128, NP == 1 ? 5 : 2) delta_prep(const __grid_
 }
 
 // ================================================================================================
-// The chain kernels: a CTA carries NS strips of 16 value channels of one head's state through all chunks, four
-// warps per strip, and one more warp loads the chunks' tiles.  The chain from chunk to chunk is what takes
-// the time: it is cut four ways inside a strip (three exchanges per chunk, barriers of four warps), and the
-// strips of a CTA run freely, so that one's exchange hides behind another's products.
+// The chain kernels: a CTA carries NS (one or two) strips of 16 value channels of one head's state through all
+// chunks, four warps per strip, and one more warp loads the chunks' tiles.  The chain from chunk to chunk is what
+// takes the time: it is cut four ways inside a strip (three exchanges per chunk, barriers of four warps), and the
+// strips of a CTA run freely, so that one's exchange hides behind another's products.  A chunk takes 2.3 us with
+// one strip per SM (bf16, dk 128), of which the tensor pipe is busy 0.7: waits for operands and for one another's
+// results bound it.  Where heads are many, ssm_delta_tc.cuh is faster.
 // Tiles: K is used first and last in a chunk and has two buffers where they fit, like the vectors; Q, T and P have
 // one each, refilled as soon as every strip is past them.
 // ================================================================================================
@@ -1416,8 +1418,6 @@ cudaError_t launch(dim3 grid, int threads, size_t smem, const DeltaParams& p, cu
   return cudaGetLastError();
 }
 
-// Strips per CTA of the chain kernels: one while every strip can have an SM of its own, then two, then four, which
-// load the chunks' tiles once for all.
 template <typename T, int NP, int DKP, int NS>
 cudaError_t run_chain_ns(const Shape& s, const DeltaParams& p, bool bwd, cudaStream_t st) {
   const dim3 grid((unsigned)((s.dvp() / 16 + NS - 1) / NS), (unsigned)s.Hv, (unsigned)s.B);
@@ -1425,15 +1425,14 @@ cudaError_t run_chain_ns(const Shape& s, const DeltaParams& p, bool bwd, cudaStr
   if (bwd) {
     using Form = BwdChain<T, NP, DKP, NS>;
     constexpr size_t smem = sizeof(typename Form::template Smem<Form::KB>);
-    if constexpr (smem > 227 * 1024) return cudaErrorInvalidValue;
-    else return launch<delta_bwd_chain<T, NP, DKP, NS>>(grid, threads, smem, p, st);
+    static_assert(smem <= 227 * 1024, "shared memory");
+    return launch<delta_bwd_chain<T, NP, DKP, NS>>(grid, threads, smem, p, st);
   } else {
     using Form = FwdChain<T, NP, DKP, NS>;
     constexpr size_t smem = sizeof(typename Form::template Smem<Form::KB>);
-    if constexpr (smem > 227 * 1024) return cudaErrorInvalidValue;
-    else
-      return p.states != nullptr ? launch<delta_fwd<T, NP, DKP, NS, true>>(grid, threads, smem, p, st)
-                                 : launch<delta_fwd<T, NP, DKP, NS, false>>(grid, threads, smem, p, st);
+    static_assert(smem <= 227 * 1024, "shared memory");
+    return p.states != nullptr ? launch<delta_fwd<T, NP, DKP, NS, true>>(grid, threads, smem, p, st)
+                               : launch<delta_fwd<T, NP, DKP, NS, false>>(grid, threads, smem, p, st);
   }
 }
 template <typename T, int NP, int DKP>
@@ -1445,18 +1444,26 @@ cudaError_t run_chain_tc(const Shape& s, const DeltaParams& p, bool bwd, cudaStr
   return p.states != nullptr ? launch<delta_fwd_tc<T, NP, DKP, true>>(grid, kTcThreads, fwd, p, st)
                              : launch<delta_fwd_tc<T, NP, DKP, false>>(grid, kTcThreads, fwd, p, st);
 }
+// Which chain kernel: strips, one or two to a CTA, or tcgen05.  All three keep an SM to a CTA, so a call takes waves of
+// 148 CTAs; what a wave takes, in units of one strip per CTA, was measured over 4 to 600 strips (1024 positions,
+// forward / backward in us):
+//                         bf16, dk 128     bf16, dk 64      fp32, dk 64
+//   one strip             42 / 50          33 / 37          46 / 49
+//   two strips            65 / 71          59 / 60          80 / 80
+//   tcgen05, 128 rows     118 / 160        93 / 120         113 / 134
+// (fp32 keys above 64 channels leave shared memory for one strip only.)
 template <typename T, int NP, int DKP>
 cudaError_t run_chain(const Shape& s, const DeltaParams& p, bool bwd, cudaStream_t st) {
-  const int64_t tiles = s.dvp() / 16, strips = s.B * s.Hv * tiles;
-  constexpr bool wide = NP == 3 && DKP == 128;       // six tiles of pieces leave room for one strip
-  if constexpr (!wide)
-    if (strips > 148) return run_chain_tc<T, NP, DKP>(s, p, bwd, st);
-  if (wide || tiles == 1 || strips <= 148) return run_chain_ns<T, NP, DKP, 1>(s, p, bwd, st);
-  if constexpr (!wide) {
-    if (NP == 3 || tiles == 2 || strips <= 2 * 148) return run_chain_ns<T, NP, DKP, 2>(s, p, bwd, st);
-    if constexpr (NP == 1) return run_chain_ns<T, NP, DKP, 4>(s, p, bwd, st);
+  if constexpr (NP == 3 && DKP == 128) {
+    return run_chain_ns<T, NP, DKP, 1>(s, p, bwd, st);
+  } else {
+    const int64_t heads = s.B * s.Hv, tiles = s.dvp() / 16;
+    auto waves = [heads](int64_t ctas_per_head) { return (double)((heads * ctas_per_head + 147) / 148); };
+    const double one = waves(tiles), two = waves((tiles + 1) / 2) * (NP == 3 || DKP == 64 ? 1.7 : 1.5);
+    const double tc = waves((s.dv + 127) / 128) * (NP == 3 ? 2.5 : bwd ? 3.2 : 2.8);
+    if (tc < one && tc < two) return run_chain_tc<T, NP, DKP>(s, p, bwd, st);
+    return two < one ? run_chain_ns<T, NP, DKP, 2>(s, p, bwd, st) : run_chain_ns<T, NP, DKP, 1>(s, p, bwd, st);
   }
-  return cudaErrorInvalidValue;
 }
 template <typename T, int NP, int DKP>
 cudaError_t run_fwd(const Shape& s, const DeltaParams& p, cudaStream_t st) {
