@@ -9,6 +9,7 @@ Public API (reference interface it replaces in parentheses):
     gated_delta_rule         (the gated delta rule over a sequence; no counterpart in the reference)
     gated_delta_state_update (one token of it, the state updated in place)
     group_norm               (channels last, with an activation and a gate: the norm behind the heads)
+``mixer.MambaMixer``, ``delta_mixer.GatedDeltaMixer`` and ``mixer.MambaLM`` put them together.
 The kernels live in libssm_b200.so (C ABI: include/ssm_b200.h); this package only marshals
 torch tensors into it.  Build it with ``python -m mamba_ssm_benchmark_b200.build``.
 """

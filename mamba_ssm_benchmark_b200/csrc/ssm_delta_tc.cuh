@@ -333,8 +333,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) delta_fwd_tc(const __grid_const
       const int k = half * HK + i;
       S[i / 32][i % 32] = h0 != nullptr && live && k < p.dkw ? h0[(size_t)k * p.dvw] : 0.0f;
     }
+    const int c0 = 32 * half;
     for (int ch = 0; ch < p.n; ++ch) {
-      const int st = ch & 1, par = ch & 1, rows = min(kC, p.L - ch * kC), c0 = 32 * half;
+      const int st = ch & 1, par = ch & 1, rows = min(kC, p.L - ch * kC);
       const float* vec = s.stage[st].vec;
       const long long t0 = (long long)ch * kC + c0;
 #pragma unroll
@@ -467,7 +468,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) delta_bwd_tc(const __grid_const
       tc_each(vec + c0, [&](int i, float eg) { x[i] *= p.scale * eg; });
       tc_put<3>(my + kTcG + c0 / 2, kC / 2, x);
       tc_ready(&s.ready[0]);
-      if (ch > 0) fetch(ch - 1);
+      if (NP == 3 && ch > 0) fetch(ch - 1);
       float* dst = p.dstates + ((head * p.n + ch) * p.dvp + d - lane) * DKP + half * HK;
 #pragma unroll
       for (int i = 0; i < HK / 32; ++i) tc_store_rows<Smem::kRowUnits>(s.rows[warp], dst + 32 * i, DKP, kept, S[i], lane);
@@ -479,6 +480,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) delta_bwd_tc(const __grid_const
       tc_each(vec + kC + c0, [&](int i, float la) { x[i] = fmaf(la, x[i], y[i]); });
       tc_put<3>(my + kTcU + c0 / 2, kC / 2, x);
       tc_ready(&s.ready[1]);
+      if (NP == 1 && ch > 0) fetch(ch - 1);      // behind the shorter wait; 32-bit values would spill (76 -> 84 us)
       wait(&s.done[1], par);
       tc_fence_after();
       tc_load_f32(my + kTcD + c0, x);

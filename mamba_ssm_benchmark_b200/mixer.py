@@ -221,14 +221,22 @@ class RMSNorm(nn.Module):
         return F.rms_norm(x.float(), (x.shape[-1],), eps=self.eps).to(x.dtype) * self.weight
 
 
-class MambaBlock(nn.Module):
-    """x + mixer(norm1(x)): a pre-norm residual block with a Mamba mixer and no MLP."""
+def _delta_mixer(*args, **kw):
+    from .delta_mixer import GatedDeltaMixer        # which builds on this module
+    return GatedDeltaMixer(*args, **kw)
 
-    def __init__(self, d_model, **mixer_kw):
+
+class MambaBlock(nn.Module):
+    """x + mixer(norm1(x)): a pre-norm residual block without an MLP, around a Mamba mixer or, with
+    ``mixer="delta"``, a gated delta-rule mixer."""
+
+    def __init__(self, d_model, mixer="mamba", **mixer_kw):
         super().__init__()
-        self.kind = "M"
+        if mixer not in ("mamba", "delta"):
+            raise ValueError(f"mixer must be 'mamba' or 'delta', got {mixer!r}")
+        self.kind = "M" if mixer == "mamba" else "D"
         self.norm1 = RMSNorm(d_model)
-        self.mixer = MambaMixer(d_model, **mixer_kw)
+        self.mixer = MambaMixer(d_model, **mixer_kw) if mixer == "mamba" else _delta_mixer(d_model, **mixer_kw)
         self.mlp = None
 
     def forward(self, x, state=None, pos=0):
@@ -249,15 +257,18 @@ def _sample(logits, temperature, top_k):
 
 class MambaLM(nn.Module):
     """Byte-level LM: embedding, n_layers Mamba blocks, final RMSNorm, head tied to the embedding
-    (the reference's "mamba" preset is 11 blocks at d_model 256)."""
+    (the reference's "mamba" preset is 11 blocks at d_model 256).  With ``mixer="delta"`` the blocks are
+    gated delta-rule mixers with value heads of ``head_dim`` channels; d_state, discretization, selective and
+    a_mode then have no meaning."""
 
     def __init__(self, n_layers=11, vocab_size=256, d_model=256, d_state=16, expand=2, d_conv=4,
-                 discretization="zoh", selective=True, a_mode="s4d"):
+                 discretization="zoh", selective=True, a_mode="s4d", mixer="mamba", head_dim=64):
         super().__init__()
         self.n_layers = n_layers
         self.embed = nn.Embedding(vocab_size, d_model)
-        self.blocks = nn.ModuleList(MambaBlock(d_model, d_state=d_state, expand=expand, d_conv=d_conv,
-                                               discretization=discretization, selective=selective, a_mode=a_mode)
+        kw = dict(d_state=d_state, discretization=discretization, selective=selective, a_mode=a_mode) \
+            if mixer == "mamba" else dict(head_dim=head_dim)
+        self.blocks = nn.ModuleList(MambaBlock(d_model, mixer=mixer, expand=expand, d_conv=d_conv, **kw)
                                     for _ in range(n_layers))
         self.norm_f = RMSNorm(d_model)
         self.head = nn.Linear(d_model, vocab_size, bias=False)
@@ -274,7 +285,7 @@ class MambaLM(nn.Module):
         for block in self.blocks:
             m = block.mixer
             m.in_proj.weight.normal_(0.0, 0.02)
-            if m.selective:
+            if getattr(m, "selective", False):
                 m.x_proj.weight.normal_(0.0, 0.02)
             m.out_proj.weight.normal_(0.0, residual_std)
 

@@ -76,7 +76,9 @@ def _entering(t, dy, groups, silu, center):
 
 
 TOKENS = [((1, 64), 1), ((7, 512), 8), ((33, 96), 3), ((5, 40), 5), ((300, 1024), 8), ((9, 330), 11), ((4, 4096), 2),
-          ((1000, 72), 9), ((2, 5120), 40)]
+          ((1000, 72), 9), ((2, 5120), 40),
+          # groups that eight warps share, and that no registers hold
+          ((70, 2100), 1), ((3, 4098), 2), ((9, 2099), 1), ((5, 16400), 1)]
 SEQUENCES = [((2, 17, 64), 4), ((1, 1, 64), 8), ((3, 101, 30), 5), ((2, 6, 7, 48), 3), ((1, 700, 96), 1), ((5, 2, 24), 24)]
 
 
