@@ -6,12 +6,13 @@ This module only loads the library and marshals torch tensors into the ABI's pla
 """
 
 import ctypes
-import functools
+import importlib.util
 import os
 import threading
 
 import torch
 
+GLUE_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_C", "_glue.so")
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_C", "libssm_b200.so")
 
 SSM_OK, SSM_ERR_INVALID, SSM_ERR_DTYPE, SSM_ERR_WORKSPACE, SSM_ERR_CUDA, SSM_ERR_UNSUPPORTED = range(6)
@@ -170,20 +171,6 @@ def view2(t):
     return SsmView(t.data_ptr(), DTYPES[t.dtype], 0, t.stride(0), 0)
 
 
-def heads4(t):
-    """(B, rows, heads, width) tensor with unit inner stride -> ssm_heads."""
-    sb, sl, sh, inner = t.stride()
-    assert inner == 1 or t.shape[3] == 1, "inner dimension must be contiguous"
-    return SsmHeads(t.data_ptr(), DTYPES[t.dtype], 0, sb, sl, sh)
-
-
-def heads3(t):
-    """(B, heads, width) tensor with unit inner stride -> ssm_heads with one row per batch entry."""
-    sb, sh, inner = t.stride()
-    assert inner == 1 or t.shape[2] == 1, "inner dimension must be contiguous"
-    return SsmHeads(t.data_ptr(), DTYPES[t.dtype], 0, sb, 0, sh)
-
-
 def delta_opts(bias, softplus, dbias=None):
     """ssm_delta_opts for the _ex entry points, or None (plain delta)."""
     if not softplus:
@@ -200,24 +187,30 @@ def stream_of(device):
     return torch.cuda.current_stream(device).cuda_stream
 
 
-# The stream handle without building a torch.cuda.Stream (about 1.5 us of a decode step's host time), where
-# this torch has it.
-_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_glue = None
 
 
-def call(name, dev, *args):
-    """Calls the entry point ``name`` with ``args`` and ``dev``'s current stream, on device ``dev``.  The device
-    is switched only where it is not current: the context manager costs more than a small launch."""
-    index = dev.index
-    stream = _raw_stream(index) if _raw_stream is not None else stream_of(dev)
-    fn = getattr(_lib or lib(), name)
-    if index == torch.cuda.current_device():
-        rc = fn(*args, stream)
-    else:
-        with torch.cuda.device(dev):
-            rc = fn(*args, stream)
-    if rc != SSM_OK:
-        check(rc, name)
+def glue():
+    """The module _C/_glue.so (csrc/torch_glue.cpp): torch tensors and autograd over the library, in C++."""
+    global _glue
+    if _glue is None:
+        handle = lib()                       # the checks and messages of the library come first
+        with _lock:
+            if _glue is None:
+                if not os.path.exists(GLUE_PATH):
+                    raise NativeLibraryError(
+                        f"{GLUE_PATH} is not built; run `python -m mamba_ssm_benchmark_b200.build` "
+                        "(this package has no non-CUDA fallback)")
+                spec = importlib.util.spec_from_file_location("_glue", GLUE_PATH)
+                module = importlib.util.module_from_spec(spec)
+                try:
+                    spec.loader.exec_module(module)
+                except ImportError as e:
+                    raise NativeLibraryError(f"cannot load {GLUE_PATH}: {e}") from e
+                if module.abi_version() != handle.ssm_abi_version():
+                    raise NativeLibraryError(f"{GLUE_PATH} was built for ABI {module.abi_version()}")
+                _glue = module
+    return _glue
 
 
 def conv_workspace_bytes(B, L, D, K):
@@ -243,29 +236,6 @@ def bwd_plan(B, L, D, N, dtype):
 def bwd_workspace_bytes(B, L, D, N):
     n = _SZ(0)
     check(lib().ssm_scan_bwd_workspace_size(B, L, D, N, ctypes.byref(n)), "ssm_scan_bwd_workspace_size")
-    return n.value
-
-
-@functools.lru_cache(maxsize=4096)
-def gated_delta_workspace_bytes(dims, dtype, backward):
-    n = _SZ(0)
-    check(lib().ssm_gated_delta_workspace_size(*dims, DTYPES[dtype], int(backward), ctypes.byref(n)),
-          "ssm_gated_delta_workspace_size")
-    return n.value
-
-
-@functools.lru_cache(maxsize=4096)
-def gated_delta_saved_bytes(dims, dtype):
-    n = _SZ(0)
-    check(lib().ssm_gated_delta_saved_size(*dims, DTYPES[dtype], ctypes.byref(n)), "ssm_gated_delta_saved_size")
-    return n.value
-
-
-@functools.lru_cache(maxsize=4096)
-def norm_workspace_bytes(samples, positions, C, groups, backward):
-    n = _SZ(0)
-    check(lib().ssm_group_norm_workspace_size(samples, positions, C, groups, int(backward), ctypes.byref(n)),
-          "ssm_group_norm_workspace_size")
     return n.value
 
 

@@ -6,6 +6,8 @@
 Each .cu file under csrc/ is compiled by nvcc in parallel into _build/, then linked into
 mamba_ssm_benchmark_b200/_C/libssm_b200.so with the CUDA runtime linked statically, so the
 library needs only the driver at run time.  nvcc cross-compiles: no GPU is needed to build.
+csrc/torch_glue.cpp (torch tensors and autograd over that library) becomes _C/_glue.so, compiled
+by the host compiler against the installed torch at the same time.
 """
 
 import argparse
@@ -22,6 +24,8 @@ INCLUDE = os.path.join(ROOT, "include")
 BUILD = os.path.join(ROOT, "_build")
 OUT_DIR = os.path.join(PKG, "_C")
 LIB = os.path.join(OUT_DIR, "libssm_b200.so")
+GLUE_SRC = os.path.join(CSRC, "torch_glue.cpp")
+GLUE = os.path.join(OUT_DIR, "_glue.so")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",
@@ -53,8 +57,38 @@ def _compile(src, obj, verbose):
     return r.stderr
 
 
+def _compile_glue(obj):
+    """torch_glue.cpp against the installed torch (headers only; linked by _link_glue)."""
+    import sysconfig
+
+    import torch
+    from torch.utils.cpp_extension import include_paths
+    cuda = os.path.join(os.path.dirname(os.path.dirname(nvcc())), "include")
+    paths = [INCLUDE, sysconfig.get_paths()["include"], cuda] + include_paths()
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-DTORCH_EXTENSION_NAME=_glue",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+    cmd += [f for path in paths for f in ("-isystem", path)] + ["-c", GLUE_SRC, "-o", obj]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"the host compiler failed for torch_glue.cpp:\n{r.stderr[-8000:]}")
+    return r.stderr
+
+
+def _link_glue(obj):
+    import torch
+    tmp = GLUE + ".tmp"
+    cmd = [os.environ.get("CXX", "g++"), "-shared", "-o", tmp, obj, "-L" + os.path.join(os.path.dirname(torch.__file__), "lib"),
+           "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python", "-L" + OUT_DIR, "-l:" + os.path.basename(LIB),
+           "-Wl,-rpath,$ORIGIN"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"link failed:\n{r.stderr[-8000:]}")
+    os.replace(tmp, GLUE)
+
+
 def build(force=False, verbose=False, jobs=None):
-    """Compiles every CUDA source for sm_100a and links the shared library; returns its path."""
+    """Compiles every CUDA source for sm_100a and the torch glue, and links both libraries; returns the path of
+    libssm_b200.so."""
     os.makedirs(BUILD, exist_ok=True)
     os.makedirs(OUT_DIR, exist_ok=True)
     newest_header = max(os.path.getmtime(h) for h in _headers())
@@ -64,10 +98,15 @@ def build(force=False, verbose=False, jobs=None):
         objs.append(obj)
         if force or not os.path.exists(obj) or os.path.getmtime(obj) < max(os.path.getmtime(src), newest_header):
             todo.append((src, obj))
-    if todo:
-        jobs = jobs or min(len(todo), os.cpu_count() or 4)
+    glue_obj = os.path.join(BUILD, "torch_glue.o")
+    glue = force or not os.path.exists(glue_obj) or os.path.getmtime(glue_obj) < max(os.path.getmtime(GLUE_SRC),
+                                                                                     newest_header)
+    if todo or glue:
+        jobs = jobs or min(len(todo) + 1, os.cpu_count() or 4)
         with cf.ThreadPoolExecutor(jobs) as ex:
             futs = {ex.submit(_compile, s, o, verbose): s for s, o in todo}
+            if glue:
+                futs[ex.submit(_compile_glue, glue_obj)] = GLUE_SRC
             for f in cf.as_completed(futs):
                 log = f.result()
                 if verbose and log:
@@ -79,6 +118,8 @@ def build(force=False, verbose=False, jobs=None):
         if r.returncode != 0:
             raise RuntimeError(f"link failed:\n{r.stderr[-8000:]}")
         os.replace(tmp, LIB)
+    if glue or not os.path.exists(GLUE) or os.path.getmtime(GLUE) < os.path.getmtime(glue_obj):
+        _link_glue(glue_obj)
     return LIB
 
 

@@ -63,53 +63,6 @@ def _common_dtype(q, k, v):
     return q.dtype if q.dtype in nat.DTYPES and k.dtype == q.dtype and v.dtype == q.dtype else torch.float32
 
 
-def _bytes(n, dev):
-    return torch.empty(n, dtype=torch.uint8, device=dev)
-
-
-def _forward(dims, q, k, v, g, beta, h0, scale, save):
-    B, L, Hk, Hv, dk, dv = dims
-    dev, dtype = q.device, q.dtype
-    o = v.new_empty((B, L, Hv, dv))
-    last = g.new_empty((B, Hv, dk, dv))
-    saved = _bytes(nat.gated_delta_saved_bytes(dims, dtype), dev) if save else None
-    wsb = 0 if save else nat.gated_delta_workspace_bytes(dims, dtype, False)
-    ws = None if save else _bytes(wsb, dev)
-    nat.call("ssm_gated_delta_fwd", dev, *dims, nat.heads4(q), nat.heads4(k), nat.heads4(v), nat.view3(g),
-             nat.view3(beta), nat.ptr(h0), scale, nat.heads4(o), last.data_ptr(), nat.ptr(saved), nat.ptr(ws), wsb)
-    return o, last, saved
-
-
-class GatedDeltaFn(torch.autograd.Function):
-    """(o, last) of the gated delta rule.  Keeps the state entering every 64 positions, the chunks' triangular
-    factors and corrected values for the backward."""
-
-    @staticmethod
-    def forward(ctx, q, k, v, g, beta, h0, scale, dims):
-        o, last, saved = _forward(dims, q, k, v, g, beta, h0, scale, True)
-        ctx.save_for_backward(q, k, v, g, beta, h0, saved)
-        ctx.args = scale, dims
-        return o, last
-
-    @staticmethod
-    def backward(ctx, do, dlast):
-        q, k, v, g, beta, h0, saved = ctx.saved_tensors
-        scale, dims = ctx.args
-        dev, dtype = q.device, q.dtype
-        do = _act(do, dtype)
-        if dlast is not None:
-            dlast = dlast.to(torch.float32).contiguous()
-        dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
-        dg, dbeta = g.new_empty(g.shape), g.new_empty(g.shape)
-        dh0 = None if h0 is None else torch.empty_like(h0)
-        wsb = nat.gated_delta_workspace_bytes(dims, dtype, True)
-        ws = _bytes(wsb, dev)
-        nat.call("ssm_gated_delta_bwd", dev, *dims, nat.heads4(q), nat.heads4(k), nat.heads4(v), nat.view3(g),
-                 nat.view3(beta), scale, saved.data_ptr(), nat.heads4(do), nat.ptr(dlast), nat.heads4(dq),
-                 nat.heads4(dk), nat.heads4(dv), dg.data_ptr(), dbeta.data_ptr(), nat.ptr(dh0), ws.data_ptr(), wsb)
-        return dq, dk, dv, dg, dbeta, dh0, None, None
-
-
 def gated_delta_rule(q, k, v, g, beta, h0=None, scale=None):
     """Returns (o, last): o (B, L, Hv, dv) in v's dtype, last (B, Hv, dk, dv) float32.
 
@@ -117,16 +70,14 @@ def gated_delta_rule(q, k, v, g, beta, h0=None, scale=None):
     head h); g: (B, L, Hv), the log of the decay (at most 0; -inf resets the state); beta: (B, L, Hv), the
     step of the correction; h0: (B, Hv, dk, dv) or None (zeros); scale: of o, default dk ** -0.5.
     Any strides.  Differentiable with respect to all six tensors."""
-    dims = _check(q, k, v, g, beta, h0, "h0", 4)
+    _check(q, k, v, g, beta, h0, "h0", 4)
     scale = float(q.shape[-1] ** -0.5 if scale is None else scale)
     out_dtype, ct = v.dtype, _common_dtype(q, k, v)
     q, k, v = _act(q, ct), _act(k, ct), _act(v, ct)
     g, beta = _act(g, torch.float32), _act(beta, torch.float32)
-    h0 = None if h0 is None else h0.to(torch.float32).contiguous()
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, g, beta, h0)):
-        o, last = GatedDeltaFn.apply(q, k, v, g, beta, h0, scale, dims)
-    else:
-        o, last, _ = _forward(dims, q, k, v, g, beta, h0, scale, False)
+    if h0 is not None:
+        h0 = _act(h0, torch.float32).contiguous()
+    o, last = nat.glue().gated_delta(q, k, v, g, beta, h0, scale)
     return (o if out_dtype == ct else o.to(out_dtype)), last
 
 
@@ -134,19 +85,15 @@ def gated_delta_state_update(state, q, k, v, g, beta, scale=None, out=None):
     """One token; ``state`` (B, Hv, dk, dv) float32 is updated in place.  q, k: (B, Hk, dk); v: (B, Hv, dv);
     g, beta: (B, Hv).  Returns o (B, Hv, dv) in v's dtype (``out`` if given: that shape, q, k and v's common
     type).  No synchronisation; capturable in a CUDA graph."""
-    B, _, Hk, Hv, dk, dv = _check(q, k, v, g, beta, state, "state", 3)
+    B, _, _, Hv, dk, dv = _check(q, k, v, g, beta, state, "state", 3)
     if state.dtype != torch.float32 or not state.is_contiguous():
         raise ValueError("state must be a contiguous float32 (B, Hv, dk, dv) tensor")
     scale = float(dk ** -0.5 if scale is None else scale)
-    out_dtype, ct, dev = v.dtype, _common_dtype(q, k, v), state.device
+    out_dtype, ct = v.dtype, _common_dtype(q, k, v)
     q, k, v = _act(q, ct), _act(k, ct), _act(v, ct)
     g, beta = _act(g, torch.float32), _act(beta, torch.float32)
-    if out is None:
-        o = v.new_empty((B, Hv, dv))
-    else:
-        if out.shape != (B, Hv, dv) or out.dtype != ct or out.device != dev or (out.stride(-1) != 1 and dv != 1):
-            raise ValueError(f"out must be a ({B}, {Hv}, {dv}) {ct} tensor with unit inner stride")
-        o = out
-    nat.call("ssm_gated_delta_state_update", dev, B, Hk, Hv, dk, dv, state.data_ptr(), nat.heads3(q), nat.heads3(k),
-             nat.heads3(v), nat.view2(g), nat.view2(beta), scale, nat.heads3(o))
+    if out is not None and (out.shape != (B, Hv, dv) or out.dtype != ct or out.device != state.device or
+                            (out.stride(-1) != 1 and dv != 1)):
+        raise ValueError(f"out must be a ({B}, {Hv}, {dv}) {ct} tensor with unit inner stride")
+    o = nat.glue().gated_delta_step(state, q, k, v, g, beta, scale, out)
     return o if out is not None or out_dtype == ct else o.to(out_dtype)

@@ -18,58 +18,6 @@ import torch
 from . import _native as nat
 
 
-def _dims(x):
-    return (x.shape[0], 1, x.shape[1]) if x.dim() == 2 else tuple(x.shape)
-
-
-def _views(positions, *tensors):
-    """ssm_views of (samples, positions, C) tensors; two-dimensional ones have a single position."""
-    view = nat.view2 if positions == 1 else nat.view3
-    return [view(t) for t in tensors]
-
-
-def _workspace(N, P, C, groups, backward, dev):
-    n = nat.norm_workspace_bytes(N, P, C, groups, backward)
-    return (torch.empty(n, dtype=torch.uint8, device=dev) if n else None), n
-
-
-def _forward(x, weight, bias, z, groups, eps, silu, center, want_stats):
-    """(y, stats): the statistics are kept for a backward where more than one position makes them costly."""
-    (N, P, C), dev = _dims(x), x.device
-    y = torch.empty_like(x)
-    stats = torch.empty((N, groups, 2), dtype=torch.float32, device=dev) if want_stats and P > 1 else None
-    ws, wsb = _workspace(N, P, C, groups, False, dev)
-    xv, zv, yv = _views(P, x, z, y)
-    nat.call("ssm_group_norm_fwd", dev, N, P, C, groups, xv, nat.ptr(weight), nat.ptr(bias), eps, center, silu, zv, yv,
-             nat.ptr(stats), nat.ptr(ws), wsb)
-    return y, stats
-
-
-class GroupNormFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, z, groups, eps, silu, center):
-        y, stats = _forward(x, weight, bias, z, groups, eps, silu, center, True)
-        ctx.save_for_backward(x, weight, bias, z, stats)
-        ctx.args = groups, eps, silu, center
-        return y
-
-    @staticmethod
-    def backward(ctx, dy):
-        x, weight, bias, z, stats = ctx.saved_tensors
-        groups, eps, silu, center = ctx.args
-        (N, P, C), dev = _dims(x), x.device
-        dy = _dense(dy if dy.dtype == x.dtype else dy.to(x.dtype))
-        dx = torch.empty_like(x)
-        dz = None if z is None else torch.empty_like(z)
-        dw = None if weight is None else torch.empty_like(weight)
-        db = None if bias is None else torch.empty_like(bias)
-        ws, wsb = _workspace(N, P, C, groups, True, dev)
-        xv, zv, gv, dxv, dzv = _views(P, x, z, dy, dx, dz)
-        nat.call("ssm_group_norm_bwd", dev, N, P, C, groups, xv, nat.ptr(weight), nat.ptr(bias), eps, center, silu, zv,
-                 nat.ptr(stats), gv, dxv, nat.ptr(dw), nat.ptr(db), dzv, nat.ptr(ws), wsb)
-        return dx, dw, db, dz, None, None, None, None
-
-
 def _dense(t):
     """A layout that the kernels read: unit stride along the channels."""
     return t if t is None or t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
@@ -114,6 +62,7 @@ def group_norm(x, groups, weight=None, bias=None, eps=1e-5, activation=None, z=N
         raise ValueError(f"activation must be 'silu' or None, got {activation!r}")
     if z is not None and z.shape != shape:
         raise ValueError(f"z must be shaped like x {tuple(shape)}, got {tuple(z.shape)}")
+    eps, center = float(eps), bool(center)
     if not eps >= 0.0:
         raise ValueError(f"eps must not be negative, got {eps!r}")
     if in_dtype == torch.float64 or (z is not None and z.dtype == torch.float64):
@@ -127,12 +76,7 @@ def group_norm(x, groups, weight=None, bias=None, eps=1e-5, activation=None, z=N
     dtype = in_dtype if in_dtype in nat.DTYPES and (z is None or z.dtype == in_dtype) else torch.float32
     x, z = _flat(x, dtype), _flat(z, dtype)
     weight, bias = _param(weight, "weight", C), _param(bias, "bias", C)
-    silu = activation == "silu"
-    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or
-                                    (bias is not None and bias.requires_grad) or (z is not None and z.requires_grad)):
-        y = GroupNormFn.apply(x, weight, bias, z, groups, float(eps), silu, bool(center))
-    else:
-        y = _forward(x, weight, bias, z, groups, float(eps), silu, bool(center), False)[0]
+    y = nat.glue().group_norm(x, groups, weight, bias, z, eps, activation == "silu", center)
     if y.shape != shape:
         y = y.reshape(shape)
     return y if in_dtype == dtype else y.to(in_dtype)
