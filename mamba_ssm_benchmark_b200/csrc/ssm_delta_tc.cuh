@@ -11,6 +11,10 @@
 // A chunk is three dependent rounds of products with a register pass after each; a warp of its own issues them:
 //   forward   S -> [K S, Q S] -> X -> [T X] -> U -> [P U, K^T U]
 //   backward  dS' -> [K dS', P^T dO] -> Y -> [T^T Y] -> dX -> [Q^T dO, K^T dX]
+//
+// 80 heads of 128 x 128, 4096 positions, bf16, training: 459 us forward (14 thousand clocks a chunk) and 559 us
+// backward; the strips take 856 and 1146.  The rounds' products take 2.4, 1.7 and 1.8 thousand clocks, about 53 an
+// instruction whatever its N up to 64; the register passes and the saved states' stores take the rest.
 #pragma once
 
 #include "ssm_delta.cuh"

@@ -2,7 +2,7 @@
 // which calls the C entry points of libssm_b200.so (include/ssm_b200.h).
 //
 // These operators are small enough in training and decoding that the host decides: as Python autograd functions
-// over ctypes a head norm of 8192 x 512 took 135 us forward and backward, 33 of them on the GPU.  Arguments are
+// over ctypes a head norm of 8192 x 512 took 135 us forward and backward, 33 of them on the GPU; through here 85.  Arguments are
 // checked by the Python layer (delta.py, norm.py); what arrives here has the right shapes, one device and unit
 // inner strides, except gradients, which autograd hands over as they are.
 #include <c10/cuda/CUDAGuard.h>
@@ -52,6 +52,11 @@ Tensor dense(const Tensor& t, at::ScalarType type) {
 Tensor bytes(size_t n, const Tensor& like) { return at::empty({(int64_t)n}, like.options().dtype(at::kByte)); }
 void* stream(const Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
 
+// The kernels write gradients that have no history of their own.
+void once(const char* what) {
+  TORCH_CHECK(!at::GradMode::is_enabled(), what, " is differentiable once: create_graph=True is not supported");
+}
+
 // ---- group norm -------------------------------------------------------------------------------
 struct NormArgs {
   int64_t groups;
@@ -91,6 +96,7 @@ struct GroupNorm : torch::autograd::Function<GroupNorm> {
     return y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    once("group_norm");
     const variable_list saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &weight = saved[1], &bias = saved[2], &z = saved[3], &stats = saved[4];
     const int64_t groups = ctx->saved_data["groups"].toInt(), form = ctx->saved_data["form"].toInt();
@@ -164,6 +170,7 @@ struct GatedDelta : torch::autograd::Function<GatedDelta> {
     return {o, last};
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    once("gated_delta_rule");
     const variable_list saved = ctx->get_saved_variables();
     const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &g = saved[3], &beta = saved[4], &h0 = saved[5];
     const c10::cuda::CUDAGuard guard(q.device());

@@ -246,6 +246,25 @@ def test_state_update_resets_and_replays_in_a_graph():
     assert _err(o, want_o[:, 0]) <= F32_TOL and _err(state, want_s) <= F32_TOL
 
 
+def test_partial_gradients():
+    """A loss on o alone, or on the last state alone, and inputs that want no gradient."""
+    t, do, dlast = _inputs(1, 70, 1, 2, 32, 16, seed=15)
+    for which, dout in (("o", do), ("last", dlast)):
+        lv = {n: x.to(DEV).requires_grad_(n in ("k", "g")) for n, x in t.items()}
+        got = torch.autograd.grad(gated_delta_rule(**lv)[which == "last"], [lv["k"], lv["g"]], dout.to(DEV))
+        rv = {n: x.double().requires_grad_() for n, x in t.items()}
+        want = torch.autograd.grad(O.gated_delta_rule(**rv)[which == "last"], [rv["k"], rv["g"]], dout.double())
+        for a, b in zip(got, want):
+            assert _err(a, b) <= F32_TOL, which
+
+
+def test_second_derivatives_are_refused():
+    t, do, _ = _inputs(1, 8, 1, 1, 16, 16, seed=1)
+    lv = {n: x.to(DEV).requires_grad_() for n, x in t.items()}
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad(gated_delta_rule(**lv)[0], lv["k"], do.to(DEV), create_graph=True)
+
+
 def test_refusals():
     t, *_ = _inputs(1, 8, 1, 2, 16, 16, seed=1)
     d = {n: x.to(DEV) for n, x in t.items()}
