@@ -11,9 +11,9 @@
 
 #include "ssm_b200.h"
 #include "ssm_delta.cuh"
+#include "ssm_delta_chunk.cuh"
 #include "ssm_delta_tc.cuh"
 #include "ssm_launch.cuh"
-#include "ssm_vec.cuh"
 
 namespace ssm {
 int report_error(int code, const char* msg);
@@ -31,64 +31,6 @@ constexpr int kPitch = kC + 4;
 // products, a triangular inverse) bound it, so CTAs are small, 33 KB of shared memory in bf16, five to an SM.
 // 5120 chunks of 64 x 128 (bf16): 140 us; in 90 KB, with rows loaded through registers: 252 us.
 // ================================================================================================
-// 8 columns of a row as float; zero outside.
-template <typename T>
-__device__ __forceinline__ void load8(const T* row, int c0, int width, bool vec, float (&x)[8]) {
-  if (vec && c0 + 8 <= width) {
-    if constexpr (sizeof(T) == 2) {
-      vec_load<T, 8>(row + c0, x);
-    } else {
-      float a[4], b[4];
-      load4(row + c0, a);
-      load4(row + c0 + 4, b);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        x[i] = a[i];
-        x[4 + i] = b[i];
-      }
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = c0 + i < width ? to_f32(row[c0 + i]) : 0.0f;
-  }
-}
-
-// The same as they lie in memory.
-template <typename T>
-struct alignas(16) Row8 {
-  T x[8];
-  __device__ __forceinline__ void load(const T* row, int c0, int width, bool vec) {
-    if (vec && c0 + 8 <= width) {
-#pragma unroll
-      for (int i = 0; i < (int)sizeof(T) / 2; ++i)
-        reinterpret_cast<uint4*>(x)[i] = reinterpret_cast<const uint4*>(row + c0)[i];
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = c0 + i < width ? row[c0 + i] : from_f32<T>(0.0f);
-    }
-  }
-};
-
-// Splits 8 values into NP pieces and writes 16 bytes of each at `off` of the tiles `stride` apart.
-template <int NP>
-__device__ __forceinline__ void put_pieces(const float (&x)[8], __nv_bfloat16* shared, __nv_bfloat16* global, int off,
-                                           int stride) {
-  uint32_t p[4][NP];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) split<NP>(x[2 * i], x[2 * i + 1], p[i]);
-#pragma unroll
-  for (int i = 0; i < NP; ++i) {
-    const uint4 w = make_uint4(p[0][i], p[1][i], p[2][i], p[3][i]);
-    if (shared != nullptr) *reinterpret_cast<uint4*>(shared + i * stride + off) = w;
-    if (global != nullptr) *reinterpret_cast<uint4*>(global + i * stride + off) = w;
-  }
-}
-
-__device__ __forceinline__ bool rows_aligned16(const Heads& h, int es) {
-  return ((reinterpret_cast<uintptr_t>(h.ptr) | (uintptr_t)(h.sb * es) | (uintptr_t)(h.sl * es) |
-           (uintptr_t)(h.sh * es)) & 15) == 0;
-}
-
 template <int NP, int DKP>
 struct alignas(128) PrepSmem {
   union {
@@ -748,432 +690,6 @@ __global__ void __launch_bounds__(128 * NS + 32) delta_bwd_chain(const __grid_co
   if (p.last != nullptr) state_store(p.last + head * p.dkw * p.dvw, p.dkw, p.dvw, 8 * NT * w, d0, lane, S);
 }
 
-// ================================================================================================
-// Backward, all chunks at once: one CTA of sixteen warps per (chunk, value head, batch).  With
-//   E1 = dO S^T,  E2 = dX S^T,  E3 = U dS'^T,  N = -tril(D dX U^T, -1),  M = scale tril(D dO U^T, -1),
-//   m_i = scale dO_i.U_i (the diagonal, where D = 1 has no gradient)
-//   H = N K - e^G E2                         (the gradient of beta k)
-//   dQ = scale e^G E1 + M K,   dK = beta H + C,  C = N^T (beta K) + M^T Q + e^(G_last - G) E3
-//   dbeta_i = dX_i.V_i + k_i.H_i
-//   dG_i = q_i.dQ_i + beta_i k_i.H_i - k_i.C_i;  the last position also gets
-//          sum_i e^(G_last - G_i) k_i.E3_i + e^G_last <S, dS'>
-// after which dQ_i gets m_i k_i and dK_i gets m_i q_i;
-// dg is dG summed from the end of the chunk.  Every exponent's gradient is thus a row product of
-// gradients that are formed anyway; k.k and q.k are not needed again.
-// A warp takes 16 rows and a quarter of the columns.  dv is walked SL channels at a time: bulk copies bring slabs of
-// S, dS', U and dX (fp32) one ahead of the one in work, across chunks too (a CTA walks over many); all threads
-// split a slab into bf16 pieces once, in the tiles that ldmatrix reads.  5120 chunks of 128 x 128 (bf16): 1.02 ms, 7 us
-// or 55 thousand clocks a CTA and chunk: 29 for the products (20 of them the tensor pipe), 8 for splitting, 18 for what
-// follows the last slab.  Splitting by each warp that uses an operand, instead of once: 2.14 ms.
-// ================================================================================================
-template <int DKP, int SL>
-struct alignas(128) BwdSlab {   // as it lies in global memory
-  float S[SL * DKP], dS[SL * DKP], U[SL * kC], dX[SL * kC];
-};
-template <int NP, int DKP, int SL>
-struct BwdPieces {
-  __nv_bfloat16 pS[3][SL * DKP], pdS[3][SL * DKP], pU[3][SL * kC], pdX[3][SL * kC], pdO[NP][kC * SL];
-};
-struct BwdTri {
-  __nv_bfloat16 M[3][kTri], N[3][kTri], Nb[3][kTri];     // Nb: rows times beta
-};
-template <int NP, int DKP, int SL>
-struct alignas(128) BwdSmem {
-  BwdSlab<DKP, SL> slab[2];
-  union {
-    BwdPieces<NP, DKP, SL> x;
-    BwdTri tri;                 // after the last slab
-  };
-  alignas(128) __nv_bfloat16 k[NP][kC * DKP];
-  __nv_bfloat16 q[NP][kC * DKP];
-  float vec[kVec];
-  float dots[4][4][kC];         // q.dQ, k.H, k.C, e^(G_last - G) k.E3; by column quarter
-  float dxv[SL / 8][kC];        // dX.V by 8 channels of a slab
-  float sds[16];                // <S, dS'> by warp
-  float m[kC];                  // the diagonal of M
-  uint64_t bar_kq, bar_slab[2];
-};
-
-// d += the products of A (given by frag(kb, piece, a)) over k blocks [kb0, kb1) with a [c][dk] tile of NP pieces, in the
-// warp's NT column tiles from col_tile0.
-template <int NP, int DKP, int NT, typename F>
-__device__ __forceinline__ void add_tile_product(float (&d)[NT][4], uint32_t tile, int col_tile0, int kb0, int kb1,
-                                                 int lane, F frag) {
-  float lead[NT][4], low[NT][4];
-  zero(lead);
-  zero(low);
-  for (int kb = kb0; kb < kb1; ++kb) {
-    uint32_t a[3][4];
-#pragma unroll
-    for (int i = 0; i < 3; ++i) frag(kb, i, a[i]);
-#pragma unroll
-    for (int pb = 0; pb < NP; ++pb) {
-      uint32_t bf[NT / 2][4];
-#pragma unroll
-      for (int jp = 0; jp < NT / 2; ++jp) load_bt<DKP>(bf[jp], tile + pb * (kC * DKP * 2), col_tile0 + 2 * jp, kb, lane);
-      mma_split<2>(lead, low, 0, a, bf, pb);
-    }
-  }
-  add(lead, low);
-  add(d, lead);
-}
-
-template <typename T, int NP, int DKP, int SL>
-__global__ void __launch_bounds__(512) delta_bwd_chunk(const __grid_constant__ DeltaParams p) {
-  extern __shared__ __align__(128) unsigned char smem_raw[];
-  auto& s = *reinterpret_cast<BwdSmem<NP, DKP, SL>*>(smem_raw);
-  constexpr int NT = DKP / 32, KS = SL / 16;      // n tiles of a warp's quarter of dk; k blocks of a slab
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  const int w4 = warp & 3, row0 = 16 * w4, quarter = warp >> 2;
-  const int items = p.n * p.Hv * p.B, per_item = (p.dvp + SL - 1) / SL;    // (chunk, head, batch); slabs of each
-  // slab number `it` of this CTA, counted over its items
-  auto fetch_slab = [&](int it) {
-    const size_t at = blockIdx.x + (size_t)(it / per_item) * gridDim.x;    // chunk innermost, like the buffers
-    if (at >= (size_t)items) return;
-    const int v0 = it % per_item * SL;
-    const uint32_t vn = min(SL, p.dvp - v0);
-    auto& d = s.slab[it & 1];
-    uint64_t* bar = &s.bar_slab[it & 1];
-    mbar_arrive_expect_tx(bar, vn * (2 * DKP + 2 * kC) * 4);
-    bulk_load(d.S, p.states + (at * p.dvp + v0) * DKP, vn * DKP * 4, bar);
-    bulk_load(d.dS, p.dstates + (at * p.dvp + v0) * DKP, vn * DKP * 4, bar);
-    bulk_load(d.U, p.us + (at * p.dvp + v0) * kC, vn * kC * 4, bar);
-    bulk_load(d.dX, p.dxs + (at * p.dvp + v0) * kC, vn * kC * 4, bar);
-  };
-  auto fetch_tiles = [&](int item) {
-    if (item >= items) return;
-    const int h = item / p.n % p.Hv, b = item / p.n / p.Hv;
-    const size_t at = item, atk = ((size_t)b * p.Hk + h / p.group) * p.n + item % p.n;
-    mbar_arrive_expect_tx(&s.bar_kq, sizeof(s.k) + sizeof(s.q) + sizeof(s.vec));
-    bulk_load(s.k, p.kimg + atk * (NP * kC * DKP), sizeof(s.k), &s.bar_kq);
-    bulk_load(s.q, p.qimg + atk * (NP * kC * DKP), sizeof(s.q), &s.bar_kq);
-    bulk_load(s.vec, p.vec + at * kVec, sizeof(s.vec), &s.bar_kq);
-  };
-  if (tid == 0) {
-    mbar_init(&s.bar_kq, 1);
-    mbar_init(&s.bar_slab[0], 1);
-    mbar_init(&s.bar_slab[1], 1);
-    fence_mbar_init();
-    fetch_slab(0);
-    fetch_slab(1);
-    fetch_tiles(blockIdx.x);
-  }
-  __syncthreads();
-  // A slab's dO and V, 8 channels of one position per thread: dO by the first threads, neighbours along a row; V,
-  // which only meets dX (stored [channel][position]) in dX.V, by the next ones, neighbours along the positions.
-  constexpr int kRowGroups = SL / 8, kLoaders = kC * kRowGroups;
-  static_assert(2 * kLoaders <= 512, "a slab's dO and V are one step");
-  const bool ovec = rows_aligned16(p.o, sizeof(T)), vvec = rows_aligned16(p.v, sizeof(T));
-  const bool loads_o = tid < kLoaders, loads_v = !loads_o && tid < 2 * kLoaders;
-  const int lc = loads_o ? tid / kRowGroups : tid % kC, lg = loads_o ? tid % kRowGroups : tid / kC % kRowGroups;
-  int it = 0;
-#pragma unroll 1
-  for (int item = blockIdx.x, turn = 0; item < items; item += gridDim.x, ++turn) {
-    const int ch = item % p.n, h = item / p.n % p.Hv, b = item / p.n / p.Hv, hk = h / p.group;
-    const int rows = min(kC, p.L - ch * kC);
-    const long long t0 = (long long)ch * kC;
-    const T* dOb = static_cast<const T*>(p.o.ptr) + b * p.o.sb + t0 * p.o.sl + h * p.o.sh;
-    const T* Vb = static_cast<const T*>(p.v.ptr) + b * p.v.sb + t0 * p.v.sl + h * p.v.sh;
-    Row8<T> ahead;
-    auto load_rows = [&](int v0) {
-      const int width = lc < rows ? p.dvw : 0;
-      if (loads_o) ahead.load(dOb + lc * p.o.sl, v0 + 8 * lg, width, ovec);
-      else if (loads_v) ahead.load(Vb + lc * p.v.sl, v0 + 8 * lg, width, vvec);
-    };
-    load_rows(0);
-    float E1[NT][4], E2[NT][4], E3[NT][4], XU[2][4], OU[2][4];
-    zero(E1);
-    zero(E2);
-    zero(E3);
-    zero(XU);
-    zero(OU);
-    float dot = 0.0f, dxv = 0.0f;
-    for (int v0 = 0; v0 < p.dvp; v0 += SL, ++it) {
-      const int vn = min(SL, p.dvp - v0);
-      const auto& raw = s.slab[it & 1];
-      mbar_wait(&s.bar_slab[it & 1], (it >> 1) & 1, p.err);
-      // split the slab
-      for (int e = tid; e < SL * DKP / 8; e += 512) {
-        const int r = e / (DKP / 8), grp = e % (DKP / 8), off = tile_off<DKP, SL>(r, grp);
-        float x[8], y[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = y[i] = 0.0f;
-        if (r < vn) {
-          load8<float>(raw.S + r * DKP, 8 * grp, DKP, true, x);
-          load8<float>(raw.dS + r * DKP, 8 * grp, DKP, true, y);
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) dot = fmaf(x[i], y[i], dot);
-        put_pieces<3>(x, s.x.pS[0], nullptr, off, SL * DKP);
-        put_pieces<3>(y, s.x.pdS[0], nullptr, off, SL * DKP);
-      }
-      for (int e = tid; e < SL * kC / 8; e += 512) {
-        const int r = e / (kC / 8), grp = e % (kC / 8), off = tile_off<kC, SL>(r, grp);
-        float x[8], y[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = y[i] = 0.0f;
-        if (r < vn) {
-          load8<float>(raw.U + r * kC, 8 * grp, kC, true, x);
-          load8<float>(raw.dX + r * kC, 8 * grp, kC, true, y);
-        }
-        put_pieces<3>(x, s.x.pU[0], nullptr, off, SL * kC);
-        put_pieces<3>(y, s.x.pdX[0], nullptr, off, SL * kC);
-      }
-      if (loads_o) {
-        float x[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = to_f32(ahead.x[i]);
-        put_pieces<NP>(x, s.x.pdO[0], nullptr, tile_off<SL>(lc, lg), kC * SL);
-      } else if (loads_v) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (8 * lg + i < vn) dxv = fmaf(raw.dX[(8 * lg + i) * kC + lc], to_f32(ahead.x[i]), dxv);
-      }
-      __syncthreads();
-      if (tid == 0) fetch_slab(it + 2);
-      if (v0 + SL < p.dvp) load_rows(v0 + SL);
-      // multiply.  The slab's small products, then its leading ones, in fresh accumulators that are added to the
-      // totals once, rounded to nearest.
-      uint32_t ao[KS][NP][4], ax[KS][3][4], au[KS][3][4];
-      const uint32_t tO = smem_u32(s.x.pdO[0]), tX = smem_u32(s.x.pdX[0]), tU = smem_u32(s.x.pU[0]);
-      const uint32_t tS = smem_u32(s.x.pS[0]), tdS = smem_u32(s.x.pdS[0]);
-#pragma unroll
-      for (int k = 0; k < KS; ++k) {
-#pragma unroll
-        for (int i = 0; i < NP; ++i) load_a<SL>(ao[k][i], tO + i * (kC * SL * 2), row0, k, lane);
-#pragma unroll
-        for (int i = 0; i < 3; ++i) {
-          load_at<kC, SL>(ax[k][i], tX + i * (SL * kC * 2), row0, k, lane);
-          load_at<kC, SL>(au[k][i], tU + i * (SL * kC * 2), row0, k, lane);
-        }
-      }
-#pragma unroll
-      for (int jp = 0; jp < NT / 2; ++jp) {
-        float d1[2][4], d2[2][4], d3[2][4];
-        zero(d1);
-        zero(d2);
-        zero(d3);
-        uint32_t bs[KS][1][4], bd[KS][1][4];
-#pragma unroll
-        for (int pb = 2; pb >= 0; --pb)
-#pragma unroll
-          for (int k = 0; k < KS; ++k) {
-            load_bt<DKP, SL>(bs[k][0], tS + pb * (SL * DKP * 2), quarter * NT + 2 * jp, k, lane);
-            load_bt<DKP, SL>(bd[k][0], tdS + pb * (SL * DKP * 2), quarter * NT + 2 * jp, k, lane);
-            mma_pieces<1, 2>(d1, 0, ao[k], bs[k], pb);
-            mma_pieces<1, 2>(d2, 0, ax[k], bs[k], pb);
-            mma_pieces<1, 2>(d3, 0, au[k], bd[k], pb);
-          }
-#pragma unroll
-        for (int k = 0; k < KS; ++k) {
-          mma_pieces<0, 0>(d1, 0, ao[k], bs[k], 0);
-          mma_pieces<0, 0>(d2, 0, ax[k], bs[k], 0);
-          mma_pieces<0, 0>(d3, 0, au[k], bd[k], 0);
-        }
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            E1[2 * jp + j][e] += d1[j][e];
-            E2[2 * jp + j][e] += d2[j][e];
-            E3[2 * jp + j][e] += d3[j][e];
-          }
-      }
-      if (quarter <= w4) {
-        float d1[2][4], d2[2][4];
-        zero(d1);
-        zero(d2);
-        uint32_t bu[KS][1][4];
-#pragma unroll
-        for (int pb = 2; pb >= 0; --pb)
-#pragma unroll
-          for (int k = 0; k < KS; ++k) {
-            load_bt<kC, SL>(bu[k][0], tU + pb * (SL * kC * 2), 2 * quarter, k, lane);
-            mma_pieces<1, 2>(d1, 0, ao[k], bu[k], pb);
-            mma_pieces<1, 2>(d2, 0, ax[k], bu[k], pb);
-          }
-#pragma unroll
-        for (int k = 0; k < KS; ++k) {
-          mma_pieces<0, 0>(d1, 0, ao[k], bu[k], 0);
-          mma_pieces<0, 0>(d2, 0, ax[k], bu[k], 0);
-        }
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            OU[j][e] += d1[j][e];
-            XU[j][e] += d2[j][e];
-          }
-      }
-      __syncthreads();
-    }
-    mbar_wait(&s.bar_kq, turn & 1, p.err);
-    const float* beta = s.vec + 2 * kC;
-    // N, beta N and M in pieces, where the slab was
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const int i = row0 + g + 8 * r, c = 16 * quarter + 8 * j + 2 * t;
-        float n[2], m[2];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float d =
-              i > c + e ? ex2((s.vec[3 * kC + i] - s.vec[3 * kC + c + e]) + (s.vec[4 * kC + i] - s.vec[4 * kC + c + e])) : 0.0f;
-          n[e] = i > c + e ? -d * XU[j][2 * r + e] : 0.0f;
-          m[e] = i > c + e ? p.scale * d * OU[j][2 * r + e] : 0.0f;
-          if (i == c + e) s.m[i] = p.scale * OU[j][2 * r + e];
-        }
-        const int off = tile_off<kC>(i, c >> 3) + 2 * t;
-        uint32_t x[3];
-        auto put = [&](__nv_bfloat16 (&tile)[3][kTri], float v0, float v1) {
-          split<3>(v0, v1, x);
-#pragma unroll
-          for (int q = 0; q < 3; ++q) *reinterpret_cast<uint32_t*>(&tile[q][off]) = x[q];
-        };
-        put(s.tri.N, n[0], n[1]);
-        put(s.tri.Nb, beta[i] * n[0], beta[i] * n[1]);
-        put(s.tri.M, m[0], m[1]);
-      }
-    if (loads_v) s.dxv[lg][lc] = dxv;
-    dot = group_allreduce<32, 1>(dot);
-    if (lane == 0) s.sds[warp] = dot;
-    __syncthreads();
-    const uint32_t sk = smem_u32(s.k[0]), sq = smem_u32(s.q[0]);
-    const uint32_t tM = smem_u32(s.tri.M[0]), tN = smem_u32(s.tri.N[0]), tNb = smem_u32(s.tri.Nb[0]);
-    const int ct = quarter * NT;
-    float be[2];
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const int i = row0 + g + 8 * r;
-      const float eg = s.vec[i], la = s.vec[kC + i];
-      be[r] = beta[i];
-#pragma unroll
-      for (int j = 0; j < NT; ++j)
-#pragma unroll
-        for (int e = 2 * r; e < 2 * r + 2; ++e) {
-          E1[j][e] *= p.scale * eg;
-          E2[j][e] *= -eg;
-          E3[j][e] *= la;
-        }
-    }
-    // x.y of the warp's rows over its columns, y a tile in pieces
-    auto put_dot = [&](int which, const float (&c)[NT][4], const __nv_bfloat16* tile) {
-      float out[2] = {0.0f, 0.0f};
-#pragma unroll
-      for (int j = 0; j < NT; ++j)
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const int off = tile_off<DKP>(row0 + g + 8 * r, ct + j) + 2 * t;
-#pragma unroll
-          for (int i = 0; i < NP; ++i) {
-            const uint32_t x = *reinterpret_cast<const uint32_t*>(tile + i * (kC * DKP) + off);
-            out[r] = fmaf(lo_f32(x), c[j][2 * r], fmaf(hi_f32(x), c[j][2 * r + 1], out[r]));
-          }
-        }
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        out[r] += __shfl_xor_sync(0xffffffffu, out[r], 1);
-        out[r] += __shfl_xor_sync(0xffffffffu, out[r], 2);
-        if (t == 0) s.dots[which][quarter][row0 + g + 8 * r] = out[r];
-      }
-    };
-    put_dot(3, E3, s.k[0]);
-    // dQ = scale e^G E1 + M K
-    add_tile_product<NP, DKP>(E1, sk, ct, 0, w4 + 1, lane,
-                              [&](int kb, int i, uint32_t (&a)[4]) { load_a<kC>(a, tM + i * (kTri * 2), row0, kb, lane); });
-    put_dot(0, E1, s.q[0]);
-    // H = N K - e^G E2
-    add_tile_product<NP, DKP>(E2, sk, ct, 0, w4 + 1, lane,
-                              [&](int kb, int i, uint32_t (&a)[4]) { load_a<kC>(a, tN + i * (kTri * 2), row0, kb, lane); });
-    put_dot(1, E2, s.k[0]);
-    // C = N^T (beta K) + M^T Q + e^(G_last - G) E3
-    add_tile_product<NP, DKP>(E3, sk, ct, w4, kC / 16, lane,
-                              [&](int kb, int i, uint32_t (&a)[4]) { load_at<kC>(a, tNb + i * (kTri * 2), row0, kb, lane); });
-    add_tile_product<NP, DKP>(E3, sq, ct, w4, kC / 16, lane,
-                              [&](int kb, int i, uint32_t (&a)[4]) { load_at<kC>(a, tM + i * (kTri * 2), row0, kb, lane); });
-    put_dot(2, E3, s.k[0]);
-    // query and key gradients: to the tensors, or per value head where key heads are shared
-#pragma unroll
-    for (int j = 0; j < NT; ++j)
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const int i = row0 + g + 8 * r, c = 8 * (ct + j) + 2 * t;
-        float kv[2] = {0.0f, 0.0f}, qv[2] = {0.0f, 0.0f};
-#pragma unroll
-        for (int x = 0; x < NP; ++x) {
-          const int off = x * (kC * DKP) + tile_off<DKP>(i, ct + j) + 2 * t;
-          const uint32_t kx = *reinterpret_cast<const uint32_t*>(s.k[0] + off);
-          const uint32_t qx = *reinterpret_cast<const uint32_t*>(s.q[0] + off);
-          kv[0] += lo_f32(kx);
-          kv[1] += hi_f32(kx);
-          qv[0] += lo_f32(qx);
-          qv[1] += hi_f32(qx);
-        }
-        float dq[2], dk[2];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          dq[e] = fmaf(s.m[i], kv[e], E1[j][2 * r + e]);
-          dk[e] = fmaf(s.m[i], qv[e], fmaf(be[r], E2[j][2 * r + e], E3[j][2 * r + e]));
-        }
-        if (i >= rows || c >= p.dkw) continue;
-        if (p.group > 1) {
-          const size_t o = (((size_t)b * p.L + t0 + i) * p.Hv + h) * DKP + c;
-          *reinterpret_cast<float2*>(p.pdq + o) = make_float2(dq[0], dq[1]);
-          *reinterpret_cast<float2*>(p.pdk + o) = make_float2(dk[0], dk[1]);
-        } else {
-          T* dqp = static_cast<T*>(const_cast<void*>(p.dq.ptr)) + b * p.dq.sb + (t0 + i) * p.dq.sl + hk * p.dq.sh + c;
-          T* dkp = static_cast<T*>(const_cast<void*>(p.dk.ptr)) + b * p.dk.sb + (t0 + i) * p.dk.sl + hk * p.dk.sh + c;
-          if (c + 1 < p.dkw && ((reinterpret_cast<uintptr_t>(dqp) | reinterpret_cast<uintptr_t>(dkp)) & (2 * sizeof(T) - 1)) == 0) {
-            vec_store<T, 2>(dqp, dq);
-            vec_store<T, 2>(dkp, dk);
-          } else {
-            dqp[0] = from_f32<T>(dq[0]);
-            dkp[0] = from_f32<T>(dk[0]);
-            if (c + 1 < p.dkw) {
-              dqp[1] = from_f32<T>(dq[1]);
-              dkp[1] = from_f32<T>(dk[1]);
-            }
-          }
-        }
-      }
-    __syncthreads();
-    if (warp == 0) {
-      float dG[2], tail = 0.0f;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int r = 2 * lane + i;
-        auto sum = [&](int w) { return (s.dots[w][0][r] + s.dots[w][1][r]) + (s.dots[w][2][r] + s.dots[w][3][r]); };
-        const float kH = sum(1);
-        dG[i] = sum(0) + beta[r] * kH - sum(2);
-        tail += sum(3);
-        float xv = 0.0f;
-#pragma unroll
-        for (int k = 0; k < kRowGroups; ++k) xv += s.dxv[k][r];
-        if (r < rows) p.dbeta[((size_t)b * p.L + t0 + r) * p.Hv + h] = xv + kH;
-      }
-      tail = group_allreduce<32, 1>(tail);
-      float sds = 0.0f;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) sds += s.sds[i];
-      tail = fmaf(s.vec[kC - 1], sds, tail);
-      float run = dG[0] + dG[1];
-#pragma unroll
-      for (int m = 1; m < 32; m <<= 1) {
-        const float down = __shfl_down_sync(0xffffffffu, run, m);
-        if (lane + m < 32) run += down;
-      }
-      run += tail;
-      if (2 * lane < rows) p.dg[((size_t)b * p.L + t0 + 2 * lane) * p.Hv + h] = run;
-      if (2 * lane + 1 < rows) p.dg[((size_t)b * p.L + t0 + 2 * lane + 1) * p.Hv + h] = run - dG[0];
-      // every warp is past the tiles (the barrier above)
-      __syncwarp();
-      if (lane == 0) fetch_tiles(item + gridDim.x);
-    }
-    __syncthreads();          // measured 5 % faster than letting the others run ahead of warp 0
-  }
-}
-
 // dq, dk (B, L, Hk, dk): the value heads' parts, (B, L, Hv, DKP) fp32, summed in head order.  A thread takes four
 // channels of one position and key head (blockIdx.x walks positions, blockIdx.y key heads).  Memory bounds it: 8192
 // positions x 40 heads of 128 in 68 us, 6.2 TB/s.
@@ -1481,9 +997,10 @@ template <typename T, int NP, int DKP>
 cudaError_t run_bwd(const Shape& s, const DeltaParams& p, cudaStream_t st) {
   cudaError_t e = run_chain<T, NP, DKP>(s, p, true, st);
   if (e != cudaSuccess) return e;
-  constexpr int SL = NP == 3 && DKP == 128 ? 16 : 32;     // what shared memory holds beside six tiles of pieces
   const dim3 bg((unsigned)std::min<int64_t>(s.n() * s.Hv * s.B, 148));       // one CTA per SM walks over the chunks
-  e = launch<delta_bwd_chunk<T, NP, DKP, SL>>(bg, 512, sizeof(BwdSmem<NP, DKP, SL>), p, st);
+  constexpr size_t smem = sizeof(ChunkSmem<NP, DKP>) + 1024;
+  static_assert(smem <= 227 * 1024 && smem > 114 * 1024, "one CTA per SM, which takes all tensor memory");
+  e = launch<delta_bwd_chunk<T, NP, DKP>>(bg, kChunkThreads, smem, p, st);
   if (e != cudaSuccess || p.group == 1) return e;
   constexpr int per = 256 / (DKP / 4);
   const dim3 sg((unsigned)(((long long)p.B * p.L + per - 1) / per), (unsigned)p.Hk);

@@ -19,6 +19,7 @@
 #pragma once
 
 #include "ssm_common.cuh"
+#include "ssm_vec.cuh"
 
 namespace ssm {
 
@@ -70,13 +71,12 @@ __device__ __forceinline__ void split(float x0, float x1, uint32_t (&p)[NP]) {
 
 // Element offset of 8-element column group `grp` of row `row` in a (ROWS x W) bf16 tile.  Its 16-byte groups are
 // permuted by the row, so that the eight rows of an ldmatrix hit different banks; a tile of 128 columns is two of 64
-// behind one another.  For ROWS = 64 that is the 128-byte swizzle that tcgen05's descriptors name.
+// behind one another.  That is the 128-byte swizzle that tcgen05's descriptors name.
 template <int W, int ROWS = kC>
 __device__ __forceinline__ int tile_off(int row, int grp) {
-  static_assert(W == 16 || W == 32 || W == 64 || W == 128, "rows of 32, 64 or 128 bytes, or two of these");
+  static_assert(W == 64 || W == 128, "rows of 128 bytes, or two of these");
   if (W == 128) return (grp >> 3) * (ROWS * 64) + row * 64 + (((grp & 7) ^ (row & 7)) << 3);
-  const int s = W == 64 ? row & 7 : W == 32 ? (row >> 1) & 3 : (row >> 2) & 1;
-  return row * W + ((grp ^ s) << 3);
+  return row * 64 + ((grp ^ (row & 7)) << 3);
 }
 
 // B fragments of n tiles j, j + 1 (r[0..1], r[2..3]) and k block kb from a tile stored [n][k].
@@ -93,12 +93,6 @@ __device__ __forceinline__ void load_bt(uint32_t (&r)[4], uint32_t tile, int j, 
 template <int W, int ROWS = kC>
 __device__ __forceinline__ void load_a(uint32_t (&r)[4], uint32_t tile, int row, int kb, int lane) {
   ldsm4(r, tile + 2 * tile_off<W, ROWS>(row + (lane & 15), 2 * kb + (lane >> 4)));
-}
-
-// The same from a tile stored [k][m].
-template <int W, int ROWS = kC>
-__device__ __forceinline__ void load_at(uint32_t (&r)[4], uint32_t tile, int row, int kb, int lane) {
-  ldsm4t(r, tile + 2 * tile_off<W, ROWS>(16 * kb + 8 * (lane >> 4) + (lane & 7), row / 8 + ((lane >> 3) & 1)));
 }
 
 // The A operand of k block kb from accumulator tiles 2 kb, 2 kb + 1, in NP pieces.
@@ -290,6 +284,64 @@ __device__ __forceinline__ void store_acc(float* base, int W, int lane, const fl
     *reinterpret_cast<float2*>(base + (size_t)g * W + 8 * j + 2 * t) = make_float2(c[j][0], c[j][1]);
     *reinterpret_cast<float2*>(base + (size_t)(g + 8) * W + 8 * j + 2 * t) = make_float2(c[j][2], c[j][3]);
   }
+}
+
+// 8 columns of a row as float; zero outside.
+template <typename T>
+__device__ __forceinline__ void load8(const T* row, int c0, int width, bool vec, float (&x)[8]) {
+  if (vec && c0 + 8 <= width) {
+    if constexpr (sizeof(T) == 2) {
+      vec_load<T, 8>(row + c0, x);
+    } else {
+      float a[4], b[4];
+      load4(row + c0, a);
+      load4(row + c0 + 4, b);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        x[i] = a[i];
+        x[4 + i] = b[i];
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = c0 + i < width ? to_f32(row[c0 + i]) : 0.0f;
+  }
+}
+
+// The same as they lie in memory.
+template <typename T>
+struct alignas(16) Row8 {
+  T x[8];
+  __device__ __forceinline__ void load(const T* row, int c0, int width, bool vec) {
+    if (vec && c0 + 8 <= width) {
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(T) / 2; ++i)
+        reinterpret_cast<uint4*>(x)[i] = reinterpret_cast<const uint4*>(row + c0)[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = c0 + i < width ? row[c0 + i] : from_f32<T>(0.0f);
+    }
+  }
+};
+
+// Splits 8 values into NP pieces and writes 16 bytes of each at `off` of the tiles `stride` apart.
+template <int NP>
+__device__ __forceinline__ void put_pieces(const float (&x)[8], __nv_bfloat16* shared, __nv_bfloat16* global, int off,
+                                           int stride) {
+  uint32_t p[4][NP];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) split<NP>(x[2 * i], x[2 * i + 1], p[i]);
+#pragma unroll
+  for (int i = 0; i < NP; ++i) {
+    const uint4 w = make_uint4(p[0][i], p[1][i], p[2][i], p[3][i]);
+    if (shared != nullptr) *reinterpret_cast<uint4*>(shared + i * stride + off) = w;
+    if (global != nullptr) *reinterpret_cast<uint4*>(global + i * stride + off) = w;
+  }
+}
+
+__device__ __forceinline__ bool rows_aligned16(const Heads& h, int es) {
+  return ((reinterpret_cast<uintptr_t>(h.ptr) | (uintptr_t)(h.sb * es) | (uintptr_t)(h.sl * es) |
+           (uintptr_t)(h.sh * es)) & 15) == 0;
 }
 
 // Bulk copy global -> shared, completion on bar; 16-byte aligned, a multiple of 16 bytes.

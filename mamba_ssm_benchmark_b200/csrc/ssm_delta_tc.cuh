@@ -75,6 +75,19 @@ __device__ __forceinline__ void tc_load_f32(uint32_t addr, float (&v)[32]) {
 #pragma unroll
   for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
+__device__ __forceinline__ void tc_load_f32(uint32_t addr, float (&v)[16]) {
+  uint32_t r[16];
+  __syncwarp();
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(addr)
+      : "memory");
+  tc_wait_load();
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
 // 32 values as NP pieces of 16 packed columns each, `stride` columns apart
 template <int NP>
 __device__ __forceinline__ void tc_put(uint32_t addr, int stride, const float (&v)[32]) {
@@ -148,6 +161,10 @@ struct TcWait {
       if (mbar_try_wait(bar, parity)) return;
     if (err) atomicOr(err, 1);
     dead = true;
+  }
+  // Before the kernel ends: after a wait that gave up, time for its copies and products in flight to land.
+  __device__ void drain() const {
+    for (int i = 0; dead && i < 1000; ++i) __nanosleep(1000);
   }
 };
 
@@ -223,22 +240,24 @@ __device__ __forceinline__ void tc_init(Smem& s) {
   __syncthreads();
   tc_fence_after();
 }
+__device__ __forceinline__ void tc_arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
 // This thread's part of a round's operands is written (and what it read of the last round's results is read).
 __device__ __forceinline__ void tc_ready(uint64_t* bar) {
   tc_wait_store();
   tc_fence_before();
   __syncwarp();
-  if ((threadIdx.x & 31) == 0)
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+  if ((threadIdx.x & 31) == 0) tc_arrive(bar);
 }
 
-// The warp's 32 rows of 32 floats to a dense [row][pitch] array.  A thread holds a row, and 32 rows at a time are 32
+// The warp's 32 rows of N floats to a dense [row][pitch] array.  A thread holds a row, and 32 rows at a time are 32
 // lines of memory per store; through shared memory (units permuted by the row) a store covers U units of 32 / U rows.
-template <int U>
-__device__ __forceinline__ void tc_store_rows(float4* buf, float* base, int pitch, int rows, const float (&v)[32], int lane) {
+template <int U, int N>
+__device__ __forceinline__ void tc_store_rows(float4* buf, float* base, int pitch, int rows, const float (&v)[N], int lane) {
   auto at = [](int r, int u) { return r * U + (u ^ (U == 8 ? r & 7 : (r >> 1) & 3)); };
 #pragma unroll
-  for (int p0 = 0; p0 < 32; p0 += 4 * U) {
+  for (int p0 = 0; p0 < N; p0 += 4 * U) {
 #pragma unroll
     for (int u = 0; u < U; ++u)
       buf[at(lane, u)] = make_float4(v[p0 + 4 * u], v[p0 + 4 * u + 1], v[p0 + 4 * u + 2], v[p0 + 4 * u + 3]);
@@ -395,6 +414,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) delta_fwd_tc(const __grid_const
     }
     tc_fence_before();
   }
+  wait.drain();
   __syncthreads();
   if (warp == 8) tc_free(tm, kTcCols);
 }
@@ -515,6 +535,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) delta_bwd_tc(const __grid_const
     }
     tc_fence_before();
   }
+  wait.drain();
   __syncthreads();
   if (warp == 8) tc_free(tm, kTcCols);
 }
