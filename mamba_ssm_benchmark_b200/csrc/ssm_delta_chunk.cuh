@@ -14,7 +14,7 @@
 // one warp multiplies them, and one copies and does the last sums along a chunk.  The 128 rows of a product are two operands of 64 positions on top of one
 // another: [dO; dX] [S | U]^T, [0; U] dS'^T, then [M; N] K and [0; (beta N)^T] K + [0; M^T] Q; so a thread meets H and C
 // of one position, or dQ.  Sums of small products and of leading ones are kept apart where tensor memory has the
-// columns for it (E3 at dk > 64 has not).  5120 chunks of 128 x 128 (bf16): 597 us; on mma.sync, 1020.
+// columns for it (E3 at dk > 64 has not).  5120 chunks of 128 x 128 (bf16): 584 us; on mma.sync, 1020.
 #pragma once
 
 #include "ssm_delta_tc.cuh"
@@ -45,7 +45,7 @@ struct alignas(1024) ChunkSmem {
   };
   __nv_bfloat16 k[NP][kC * DKP], q[NP][kC * DKP];
   ChunkSlab<DKP> slab[RB];
-  float vec[kVec];
+  alignas(16) float vec[kVec];
   float dots[4][4][kC];                          // q.dQ, k.H, k.C, e^(G_last - G) k.E3; by quarter of dk
   float dxv[2][kC];                              // dX.V by half of a slab
   float sds[16];                                 // <S, dS'> by warp
@@ -55,12 +55,15 @@ struct alignas(1024) ChunkSmem {
 };
 constexpr int kChunkThreads = 512 + 64;
 
-// Columns of tensor memory: [E1; E2] and beside it [dO; dX] U^T, small sums and, kLead further, leading ones; then E3.
-// [M; N] K and what makes C take their place.
-template <int DKP>
+// Columns of tensor memory: E3; then [E1; E2] and beside it [dO; dX] U^T, small sums and, kLead further, leading ones.
+// [M; N] K and what makes C take the latter's place.  With kStacked the pieces of K (or Q) are one wide operand and
+// their products lie kStacked columns apart, by index sum: half the instructions (1024 chunks, fp32, dk 64: 113 -> 102 us).
+template <int NP, int DKP>
 struct ChunkCols {
-  enum : uint32_t { kE = 0, kU = DKP, kLead = DKP + kC, kE3 = 2 * kLead, kE3Lead = kE3 + DKP, kMNK = 0, kCC = DKP };
-  static_assert(kE3 + (DKP == 64 ? 2 : 1) * DKP <= kTcCols, "tensor memory");
+  static constexpr int kStacked = NP == 3 && DKP == 64 ? 64 : 0;
+  enum : uint32_t { kE3 = 0, kE3Lead = 64, kE = 128, kU = kE + DKP, kLead = DKP + kC, kMNK = 128 };
+  static constexpr uint32_t kCC = kMNK + (kStacked ? 3 * kStacked : DKP);
+  static_assert(kE + 2 * kLead <= kTcCols && kCC + (kStacked ? 3 * kStacked : DKP) <= kTcCols, "tensor memory");
 };
 
 __device__ __forceinline__ void tc_mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t high, uint32_t idesc, bool accumulate,
@@ -76,10 +79,23 @@ constexpr uint32_t kTcAcrossA = 1u << 15;        // A read across its rows, [k][
 // The low descriptor word of two 64-row blocks of A, the upper one at `low`.
 __device__ __forceinline__ uint32_t tc_pair(uint32_t low, uint32_t high) { return tc_desc(low, high - low); }
 
+// Two or four neighbours in three pieces, `stride` apart.
+template <int N>
+__device__ __forceinline__ void put_values(const float (&v)[N], __nv_bfloat16* o, int stride) {
+  uint32_t q[N / 2][3];
+#pragma unroll
+  for (int e = 0; e < N / 2; ++e) split<3>(v[2 * e], v[2 * e + 1], q[e]);
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    if constexpr (N == 4) *reinterpret_cast<uint2*>(o + k * stride) = make_uint2(q[0][k], q[1][k]);
+    else *reinterpret_cast<uint32_t*>(o + k * stride) = q[0][k];
+  }
+}
+
 template <typename T, int NP, int DKP>
 __global__ void __launch_bounds__(kChunkThreads, 1) delta_bwd_chunk(const __grid_constant__ DeltaParams p) {
   using Smem = ChunkSmem<NP, DKP>;
-  using Cols = ChunkCols<DKP>;
+  using Cols = ChunkCols<NP, DKP>;
   constexpr int RB = Smem::RB, QK = DKP / 4;
   constexpr bool kApart = DKP == 64;             // E3's small sums have columns of their own
   Smem& s = tc_smem<Smem>();
@@ -213,24 +229,43 @@ __global__ void __launch_bounds__(kChunkThreads, 1) delta_bwd_chunk(const __grid
       tc_fence_after();
       const uint32_t tMN = smem_u32(s.tri.MN), tNb = smem_u32(s.tri.Nb), sk = smem_u32(s.k), sq = smem_u32(s.q);
       constexpr uint32_t kTile = kTri * 2, kKey = kC * DKP * 2;
-      bool mn = false, c = false;
+      const uint32_t kAcrossA = tc_idesc<true>(DKP) | kTcAcrossA;
+      if constexpr (Cols::kStacked != 0) {
 #pragma unroll
-      for (int lead = 0; lead < 2; ++lead)
+        for (int a = 0; a < 3; ++a)              // pieces 0 .. 2 - a of K and Q
 #pragma unroll
-        for (int a = 0; a < 3; ++a)
-#pragma unroll
-          for (int b = 0; b < NP; ++b) {
-            if (a + b > 2 || (a + b == 0) != (lead == 1)) continue;
-#pragma unroll
-            for (int st = 0; st < kC / 16; ++st) {
-              const uint32_t bk = tc_desc(sk + b * kKey + st * 2048, kC * 64 * 2), bq = tc_desc(sq + b * kKey + st * 2048, kC * 64 * 2);
-              tc_mma_ss(tm + Cols::kMNK, tc_desc(tMN + 2 * a * kTile + st * 32, 16), bk, kTcDescHigh, tc_idesc<true>(DKP), mn, issue);
-              tc_mma_ss(tm + Cols::kCC, tc_pair(zero, tNb + a * kTile + st * 2048), bk, kTcDescHigh, tc_idesc<true>(DKP) | kTcAcrossA, c, issue);
-              tc_mma_ss(tm + Cols::kCC, tc_pair(zero, tMN + 2 * a * kTile + st * 2048), bq, kTcDescHigh, tc_idesc<true>(DKP) | kTcAcrossA,
-                        true, issue);
-              mn = c = true;
-            }
+          for (int st = 0; st < kC / 16; ++st) {
+            constexpr uint32_t kBlock = kC * 64 * 2;
+            const uint32_t bk = tc_desc(sk + st * 2048, kBlock), bq = tc_desc(sq + st * 2048, kBlock);
+            const uint32_t idesc = tc_idesc<true>((3 - a) * DKP), to = a * Cols::kStacked;
+            const bool more = a + st > 0;
+            tc_mma_ss(tm + Cols::kMNK + to, tc_desc(tMN + 2 * a * kTile + st * 32, 16), bk, kTcDescHigh, idesc, more, issue);
+            tc_mma_ss(tm + Cols::kCC + to, tc_pair(zero, tNb + a * kTile + st * 2048), bk, kTcDescHigh, idesc | kTcAcrossA, more,
+                      issue);
+            tc_mma_ss(tm + Cols::kCC + to, tc_pair(zero, tMN + 2 * a * kTile + st * 2048), bq, kTcDescHigh, idesc | kTcAcrossA,
+                      true, issue);
           }
+      } else {
+        bool more = false;
+#pragma unroll
+        for (int lead = 0; lead < 2; ++lead)
+#pragma unroll
+          for (int a = 0; a < 3; ++a)
+#pragma unroll
+            for (int b = 0; b < NP; ++b) {
+              if (a + b > 2 || (a + b == 0) != (lead == 1)) continue;
+#pragma unroll
+              for (int st = 0; st < kC / 16; ++st) {
+                const uint32_t at = b * kKey + st * 2048;
+                const uint32_t bk = tc_desc(sk + at, kC * 64 * 2), bq = tc_desc(sq + at, kC * 64 * 2);
+                tc_mma_ss(tm + Cols::kMNK, tc_desc(tMN + 2 * a * kTile + st * 32, 16), bk, kTcDescHigh, tc_idesc<true>(DKP), more,
+                          issue);
+                tc_mma_ss(tm + Cols::kCC, tc_pair(zero, tNb + a * kTile + st * 2048), bk, kTcDescHigh, kAcrossA, more, issue);
+                tc_mma_ss(tm + Cols::kCC, tc_pair(zero, tMN + 2 * a * kTile + st * 2048), bq, kTcDescHigh, kAcrossA, true, issue);
+                more = true;
+              }
+            }
+      }
       if (issue) tc_commit(&s.done_tri);
     }
     __syncwarp();
@@ -268,25 +303,20 @@ __global__ void __launch_bounds__(kChunkThreads, 1) delta_bwd_chunk(const __grid
           vec_load<float, kN>(raw.dS + tid * kN, c);
 #pragma unroll
           for (int e = 0; e < kN; ++e) dot = fmaf(a[e], c[e], dot);
-          auto put = [&](const float (&v)[kN], __nv_bfloat16* tile, int stride) {
-            uint32_t q[kN / 2][3];
-#pragma unroll
-            for (int e = 0; e < kN / 2; ++e) split<3>(v[2 * e], v[2 * e + 1], q[e]);
-            __nv_bfloat16* o = tile + tile_off<DKP, kSL>(r, col >> 3) + in8;
-#pragma unroll
-            for (int k = 0; k < 3; ++k) {
-              if constexpr (kN == 4) *reinterpret_cast<uint2*>(o + k * stride) = make_uint2(q[0][k], q[1][k]);
-              else *reinterpret_cast<uint32_t*>(o + k * stride) = q[0][k];
-            }
-          };
-          put(a, x.SU[0], kSL * (DKP + kC));
-          put(c, x.dS[0], kSL * DKP);
+          const int off = tile_off<DKP, kSL>(r, col >> 3) + in8;
+          put_values(a, x.SU[0] + off, kSL * (DKP + kC));
+          put_values(c, x.dS[0] + off, kSL * DKP);
         }
         if (role < 2) {
-          const int at = tid & 127, r = at / (kC / 8), grp = at % (kC / 8), off = tile_off<kC, kSL>(r, grp);
-          float a[8];
-          load8<float>((role ? raw.dX : raw.U) + r * kC, 8 * grp, kC, true, a);
-          put_pieces<3>(a, role ? x.dX[0] : x.SU[0] + kSL * DKP, nullptr, off, role ? kSL * kC : kSL * (DKP + kC));
+          const float* src = role ? raw.dX : raw.U;
+          __nv_bfloat16* dst = role ? x.dX[0] : x.SU[0] + kSL * DKP;
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            const int at = (tid & 127) + 128 * q, r = at / (kC / 4), grp = at % (kC / 4);
+            float a[4];
+            load4(src + 4 * at, a);
+            put_values(a, dst + tile_off<kC, kSL>(r, grp >> 1) + 4 * (grp & 1), role ? kSL * kC : kSL * (DKP + kC));
+          }
         } else {
           if (role == 2) {
 #pragma unroll
@@ -325,12 +355,17 @@ __global__ void __launch_bounds__(kChunkThreads, 1) delta_bwd_chunk(const __grid
         tc_load_f32(my + Cols::kU + Cols::kLead + c0, y);
         const float gh = vec[3 * kC + i], gl = vec[4 * kC + i], f = upper ? -1.0f : p.scale;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int c = c0 + e;
-          x[e] += y[e];
-          if (!upper && c == i) s.m[i] = p.scale * x[e];
-          const float d = i > c ? ex2((gh - vec[3 * kC + c]) + (gl - vec[4 * kC + c])) : 0.0f;
-          x[e] = i > c ? f * d * x[e] : 0.0f;
+        for (int e0 = 0; e0 < 16; e0 += 4) {
+          float h4[4], l4[4];
+          load4(vec + 3 * kC + c0 + e0, h4);
+          load4(vec + 4 * kC + c0 + e0, l4);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int e = e0 + q, c = c0 + e;
+            x[e] += y[e];
+            if (!upper && c == i) s.m[i] = p.scale * x[e];
+            x[e] = i > c ? f * ex2((gh - h4[q]) + (gl - l4[q])) * x[e] : 0.0f;
+          }
         }
 #pragma unroll
         for (int g8 = 0; g8 < 2; ++g8) {
@@ -358,6 +393,16 @@ __global__ void __launch_bounds__(kChunkThreads, 1) delta_bwd_chunk(const __grid
       asm volatile("bar.sync 1, 512;" ::: "memory");       // m is there
       wait(&s.done_tri, turn & 1);
       tc_fence_after();
+      auto load_sums = [&](uint32_t at, float (&v)[16]) {
+        tc_load_f32(my + at, v);
+        if constexpr (Cols::kStacked != 0) {
+          float a[16], b[16];
+          tc_load_f32(my + at + Cols::kStacked, a);
+          tc_load_f32(my + at + 2 * Cols::kStacked, b);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) v[e] += a[e] + b[e];
+        }
+      };
       float qd = 0.0f, kh = 0.0f, kc = 0.0f, ke = 0.0f;
       const float m = s.m[i];
       auto row_of = [&](const __nv_bfloat16* tile, int col, float (&v)[16]) {       // of K or Q, 16 columns, whole
@@ -381,7 +426,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) delta_bwd_chunk(const __grid
         const int col = quarter * QK + 16 * j;
         float* o = E + 16 * j;
         float y[16], z[16], v[16];
-        tc_load_f32(my + Cols::kMNK + col, y);
+        load_sums(Cols::kMNK + col, y);
 #pragma unroll
         for (int e = 0; e < 16; ++e) o[e] += y[e];
         if (upper) {
@@ -392,7 +437,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) delta_bwd_chunk(const __grid
 #pragma unroll
             for (int e = 0; e < 16; ++e) y[e] += z[e];
           }
-          tc_load_f32(my + Cols::kCC + col, z);
+          load_sums(Cols::kCC + col, z);
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
             y[e] *= la;
