@@ -971,7 +971,7 @@ cudaError_t run_chain_tc(const Shape& s, const DeltaParams& p, bool bwd, cudaStr
 //                         bf16, dk 128     bf16, dk 64      fp32, dk 64
 //   one strip             42 / 50          33 / 37          46 / 49
 //   two strips            65 / 71          59 / 60          80 / 80
-//   tcgen05, 128 rows     118 / 145        93 / 110         113 / 134
+//   tcgen05, 128 rows     121 / 125        82 / 97          118 / 125
 // (fp32 keys above 64 channels leave shared memory for one strip only.)
 template <typename T, int NP, int DKP>
 cudaError_t run_chain(const Shape& s, const DeltaParams& p, bool bwd, cudaStream_t st) {
@@ -981,7 +981,7 @@ cudaError_t run_chain(const Shape& s, const DeltaParams& p, bool bwd, cudaStream
     const int64_t heads = s.B * s.Hv, tiles = s.dvp() / 16;
     auto waves = [heads](int64_t ctas_per_head) { return (double)((heads * ctas_per_head + 147) / 148); };
     const double one = waves(tiles), two = waves((tiles + 1) / 2) * (NP == 3 || DKP == 64 ? 1.7 : 1.5);
-    const double tc = waves((s.dv + 127) / 128) * (NP == 3 ? 2.5 : 2.9);
+    const double tc = waves((s.dv + 127) / 128) * (NP == 3 ? 2.5 : DKP == 64 ? 2.4 : 2.6);
     if (tc < one && tc < two) return run_chain_tc<T, NP, DKP>(s, p, bwd, st);
     return two < one ? run_chain_ns<T, NP, DKP, 2>(s, p, bwd, st) : run_chain_ns<T, NP, DKP, 1>(s, p, bwd, st);
   }

@@ -2,8 +2,8 @@
 //
 // The strips of ssm_delta.cu cut a chunk's chain finely, which wins while they do not fill the GPU.  With more
 // heads the tensor pipe decides, and mma.sync has a quarter of its rate.  Here one CTA carries 128 value
-// channels of a head (the M of tcgen05.mma): S^T lies across 256 threads, a thread holding one channel and
-// half of dk in registers.  Each product takes its left operand (pieces of S, X, U: three bf16 each) from tensor
+// channels of a head (the M of tcgen05.mma): S^T lies across 512 threads, a thread holding one channel and a
+// quarter of dk in registers.  Each product takes its left operand (pieces of S, X, U: three bf16 each) from tensor
 // memory, where the threads put it, and its right one from shared memory, where a bulk copy put the tile; the
 // accumulators are read back, combined and split for the next product.  Small products of pieces come before the
 // leading ones in every sum, so that the accumulators' truncations count only at the end.
@@ -12,9 +12,10 @@
 //   forward   S -> [K S, Q S] -> X -> [T X] -> U -> [P U, K^T U]
 //   backward  dS' -> [K dS', P^T dO] -> Y -> [T^T Y] -> dX -> [Q^T dO, K^T dX]
 //
-// 80 heads of 128 x 128, 4096 positions, bf16, training: 459 us forward (14 thousand clocks a chunk) and 559 us
-// backward; the strips take 856 and 1146.  The rounds' products take 2.4, 1.7 and 1.8 thousand clocks, about 53 an
-// instruction whatever its N up to 64; the register passes and the saved states' stores take the rest.
+// 80 heads of 128 x 128, 4096 positions, bf16, training: 478 us forward (14 thousand clocks a chunk) and 472 us
+// backward; the strips take 856 and 1146, and with half the threads these kernels 456 and 562 (fp32, dk 64: 67 and 77
+// instead of 63 and 67).  The rounds' products take 2.4, 1.7 and 1.8 thousand clocks, about 53 an instruction whatever
+// its N up to 64; the register passes and the saved states' stores take the rest.
 #pragma once
 
 #include "ssm_delta.cuh"
@@ -48,18 +49,6 @@ __device__ __forceinline__ void tc_mma(uint32_t d, uint32_t a, uint32_t b, uint3
       "r"(a), "r"(b), "r"(b_high), "r"(idesc), "r"((uint32_t)accumulate), "r"(issue)
       : "memory");
 }
-// 32 columns of this warp's 32 lanes
-__device__ __forceinline__ void tc_load32(uint32_t addr, uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
-      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(addr)
-      : "memory");
-}
 __device__ __forceinline__ void tc_wait_load() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tc_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tc_store8(uint32_t addr, const uint32_t (&r)[8]) {
@@ -67,14 +56,7 @@ __device__ __forceinline__ void tc_store8(uint32_t addr, const uint32_t (&r)[8])
                "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
                : "memory");
 }
-__device__ __forceinline__ void tc_load_f32(uint32_t addr, float (&v)[32]) {
-  uint32_t r[32];
-  __syncwarp();
-  tc_load32(addr, r);
-  tc_wait_load();
-#pragma unroll
-  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
-}
+// 16 columns of this warp's 32 lanes
 __device__ __forceinline__ void tc_load_f32(uint32_t addr, float (&v)[16]) {
   uint32_t r[16];
   __syncwarp();
@@ -88,23 +70,20 @@ __device__ __forceinline__ void tc_load_f32(uint32_t addr, float (&v)[16]) {
 #pragma unroll
   for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
 }
-// 32 values as NP pieces of 16 packed columns each, `stride` columns apart
+// 16 values as NP pieces of 8 packed columns each, `stride` columns apart
 template <int NP>
-__device__ __forceinline__ void tc_put(uint32_t addr, int stride, const float (&v)[32]) {
+__device__ __forceinline__ void tc_put(uint32_t addr, int stride, const float (&v)[16]) {
   __syncwarp();
+  uint32_t r[NP][8];
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    uint32_t r[NP][8];
+  for (int i = 0; i < 8; ++i) {
+    uint32_t x[NP];
+    split<NP>(v[2 * i], v[2 * i + 1], x);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      uint32_t x[NP];
-      split<NP>(v[16 * h + 2 * i], v[16 * h + 2 * i + 1], x);
-#pragma unroll
-      for (int k = 0; k < NP; ++k) r[k][i] = x[k];
-    }
-#pragma unroll
-    for (int k = 0; k < NP; ++k) tc_store8(addr + k * stride + 8 * h, r[k]);
+    for (int k = 0; k < NP; ++k) r[k][i] = x[k];
   }
+#pragma unroll
+  for (int k = 0; k < NP; ++k) tc_store8(addr + k * stride, r[k]);
 }
 
 // Shared memory descriptors of the 128-byte-swizzled tiles (rows of 64 bf16): read along the rows, [n][k] (stride
@@ -141,15 +120,15 @@ struct alignas(1024) TcStage {
 };
 template <int NP, int DKP, int PP>
 struct alignas(1024) TcSmem {
-  static constexpr int kRowUnits = NP == 1 ? 8 : 4;      // 16-byte units of a row that pass at a time
+  static constexpr int kRowUnits = NP == 1 ? 4 : 2;      // 16-byte units of a row that pass at a time
   TcStage<NP, DKP, PP> stage[2];
-  float4 rows[8][32 * kRowUnits];                        // per warp, see tc_store_rows
+  float4 rows[16][32 * kRowUnits];                       // per warp, see tc_store_rows
   uint64_t full[2];              // a stage's tiles are there
   uint64_t ready[3], done[3];    // operands of a round are in tensor memory; its products are finished
   uint32_t tmem;
 };
 
-constexpr int kTcThreads = 256 + 32;
+constexpr int kTcThreads = 512 + 32;
 
 // Waits like mbar_wait; after one that gave up the others do not wait any more, so that the kernel ends.
 struct TcWait {
@@ -230,12 +209,12 @@ __device__ __forceinline__ void tc_init(Smem& s) {
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) mbar_init(&s.full[i], 1);
     for (int i = 0; i < 3; ++i) {
-      mbar_init(&s.ready[i], 8);
+      mbar_init(&s.ready[i], 16);
       mbar_init(&s.done[i], 1);
     }
     fence_mbar_init();
   }
-  if (threadIdx.x >= 256) tc_alloc(&s.tmem, kTcCols);
+  if (threadIdx.x >= 512) tc_alloc(&s.tmem, kTcCols);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -255,7 +234,7 @@ __device__ __forceinline__ void tc_ready(uint64_t* bar) {
 // lines of memory per store; through shared memory (units permuted by the row) a store covers U units of 32 / U rows.
 template <int U, int N>
 __device__ __forceinline__ void tc_store_rows(float4* buf, float* base, int pitch, int rows, const float (&v)[N], int lane) {
-  auto at = [](int r, int u) { return r * U + (u ^ (U == 8 ? r & 7 : (r >> 1) & 3)); };
+  auto at = [](int r, int u) { return r * U + (u ^ (U == 8 ? r & 7 : U == 4 ? (r >> 1) & 3 : (r >> 2) & 1)); };
 #pragma unroll
   for (int p0 = 0; p0 < N; p0 += 4 * U) {
 #pragma unroll
@@ -270,33 +249,33 @@ __device__ __forceinline__ void tc_store_rows(float4* buf, float* base, int pitc
     __syncwarp();
   }
 }
-// 32 positions of one channel from / to a (positions, channels) tensor; neighbouring lanes are neighbouring channels.
+// 16 positions of one channel from / to a (positions, channels) tensor; neighbouring lanes are neighbouring channels.
 template <typename T>
-__device__ __forceinline__ void tc_load_col(const T* src, long long sl, int rows, bool live, T (&v)[32]) {
-  if (rows >= 32 && live) {
+__device__ __forceinline__ void tc_load_col(const T* src, long long sl, int rows, bool live, T (&v)[16]) {
+  if (rows >= 16 && live) {
 #pragma unroll
-    for (int i = 0; i < 32; ++i, src += sl) v[i] = *src;
+    for (int i = 0; i < 16; ++i, src += sl) v[i] = *src;
   } else {
 #pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = live && i < rows ? src[i * sl] : from_f32<T>(0.0f);
+    for (int i = 0; i < 16; ++i) v[i] = live && i < rows ? src[i * sl] : from_f32<T>(0.0f);
   }
 }
 template <typename T>
-__device__ __forceinline__ void tc_store_col(T* dst, long long sl, int rows, bool live, const float (&v)[32]) {
-  if (rows >= 32 && live) {
+__device__ __forceinline__ void tc_store_col(T* dst, long long sl, int rows, bool live, const float (&v)[16]) {
+  if (rows >= 16 && live) {
 #pragma unroll
-    for (int i = 0; i < 32; ++i, dst += sl) *dst = from_f32<T>(v[i]);
+    for (int i = 0; i < 16; ++i, dst += sl) *dst = from_f32<T>(v[i]);
   } else {
 #pragma unroll
-    for (int i = 0; i < 32; ++i)
+    for (int i = 0; i < 16; ++i)
       if (live && i < rows) dst[i * sl] = from_f32<T>(v[i]);
   }
 }
-// f(i, vec[i]) for 32 consecutive factors, read four at a time
+// f(i, vec[i]) for 16 consecutive factors, read four at a time
 template <typename F>
 __device__ __forceinline__ void tc_each(const float* vec, F f) {
 #pragma unroll
-  for (int i = 0; i < 32; i += 4) {
+  for (int i = 0; i < 16; i += 4) {
     const float4 x = *reinterpret_cast<const float4*>(vec + i);
     f(i, x.x);
     f(i + 1, x.y);
@@ -308,14 +287,14 @@ __device__ __forceinline__ void tc_each(const float* vec, F f) {
 // ---- forward ------------------------------------------------------------------------------------
 template <typename T, int NP, int DKP, bool SAVE>
 __global__ void __launch_bounds__(kTcThreads, 1) delta_fwd_tc(const __grid_constant__ DeltaParams p) {
-  constexpr int PP = NP == 1 ? 2 : 3, HK = DKP / 2;
+  constexpr int PP = NP == 1 ? 2 : 3, QK = DKP / 4;
   using Smem = TcSmem<NP, DKP, PP>;
   Smem& s = tc_smem<Smem>();
   const int h = blockIdx.y, b = blockIdx.z, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   tc_init(s);
   const uint32_t tm = __shfl_sync(0xffffffffu, s.tmem, 0);
   TcWait wait{p.err};
-  if (warp == 8) {
+  if (warp == 16) {
     const uint32_t issue = lane == 0;
     for (int i = 0; issue && i < 2 && i < p.n; ++i) tc_load_stage(s, p, b, h, i, i);
     for (int ch = 0; ch < p.n; ++ch) {
@@ -342,39 +321,39 @@ __global__ void __launch_bounds__(kTcThreads, 1) delta_fwd_tc(const __grid_const
     }
     __syncwarp();
   } else {
-    const int half = warp >> 2, row = 32 * (warp & 3) + lane, d = 128 * blockIdx.x + row;
+    const int quarter = warp >> 2, row = 32 * (warp & 3) + lane, d = 128 * blockIdx.x + row;
     const bool live = d < p.dvw;
     const int kept = p.dvp - (d - lane);           // rows of this warp that the saved arrays have
     const uint32_t my = tm + ((uint32_t)(32 * (warp & 3)) << 16);
     const size_t head = (size_t)b * p.Hv + h;
     const T* vb = static_cast<const T*>(p.v.ptr) + b * p.v.sb + h * p.v.sh + d;
     T* ob = static_cast<T*>(const_cast<void*>(p.o.ptr)) + b * p.o.sb + h * p.o.sh + d;
-    float S[HK / 32][32];
+    float S[QK / 16][16];
     const float* h0 = p.h0 != nullptr ? p.h0 + head * p.dkw * p.dvw + d : nullptr;
 #pragma unroll
-    for (int i = 0; i < HK; ++i) {
-      const int k = half * HK + i;
-      S[i / 32][i % 32] = h0 != nullptr && live && k < p.dkw ? h0[(size_t)k * p.dvw] : 0.0f;
+    for (int i = 0; i < QK; ++i) {
+      const int k = quarter * QK + i;
+      S[i / 16][i % 16] = h0 != nullptr && live && k < p.dkw ? h0[(size_t)k * p.dvw] : 0.0f;
     }
-    const int c0 = 32 * half;
+    const int c0 = 16 * quarter;
     for (int ch = 0; ch < p.n; ++ch) {
       const int st = ch & 1, par = ch & 1, rows = min(kC, p.L - ch * kC);
       const float* vec = s.stage[st].vec;
       const long long t0 = (long long)ch * kC + c0;
 #pragma unroll
-      for (int i = 0; i < HK / 32; ++i) tc_put<3>(my + kTcS + half * (HK / 2) + 16 * i, DKP / 2, S[i]);
+      for (int i = 0; i < QK / 16; ++i) tc_put<3>(my + kTcS + quarter * (QK / 2) + 8 * i, DKP / 2, S[i]);
       tc_ready(&s.ready[0]);
-      T vr[32];
+      T vr[16];
       tc_load_col(vb + t0 * p.v.sl, p.v.sl, rows - c0, live, vr);
       if (SAVE) {
-        float* o = p.states + ((head * p.n + ch) * p.dvp + d - lane) * DKP + half * HK;
+        float* o = p.states + ((head * p.n + ch) * p.dvp + d - lane) * DKP + quarter * QK;
 #pragma unroll
-        for (int i = 0; i < HK / 32; ++i) tc_store_rows<Smem::kRowUnits>(s.rows[warp], o + 32 * i, DKP, kept, S[i], lane);
+        for (int i = 0; i < QK / 16; ++i) tc_store_rows<Smem::kRowUnits>(s.rows[warp], o + 16 * i, DKP, kept, S[i], lane);
       }
       wait(&s.full[st], (ch >> 1) & 1);
       wait(&s.done[0], par);
       tc_fence_after();
-      float x[32];
+      float x[16];
       tc_load_f32(my + kTcD + c0, x);
       tc_each(vec + c0, [&](int i, float eg) { x[i] = fmaf(-eg, x[i], to_f32(vr[i])); });
       tc_each(vec + 2 * kC + c0, [&](int i, float be) { x[i] *= be; });
@@ -384,7 +363,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) delta_fwd_tc(const __grid_const
       tc_fence_after();
       tc_load_f32(my + kTcD + c0, x);
       tc_put<PP>(my + kTcU + c0 / 2, kC / 2, x);
-      float y[32];
+      float y[16];
       tc_each(vec + kC + c0, [&](int i, float la) { y[i] = x[i] * la; });
       tc_put<3>(my + kTcLU + c0 / 2, kC / 2, y);
       tc_ready(&s.ready[2]);
@@ -394,10 +373,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) delta_fwd_tc(const __grid_const
       tc_fence_after();
       const float keep = vec[kC - 1];
 #pragma unroll
-      for (int j = 0; j < HK / 32; ++j) {
-        tc_load_f32(my + kTcD + half * HK + 32 * j, x);
+      for (int j = 0; j < QK / 16; ++j) {
+        tc_load_f32(my + kTcD + quarter * QK + 16 * j, x);
 #pragma unroll
-        for (int i = 0; i < 32; ++i) S[j][i] = fmaf(keep, S[j][i], x[i]);
+        for (int i = 0; i < 16; ++i) S[j][i] = fmaf(keep, S[j][i], x[i]);
       }
       tc_load_f32(my + kTcO + c0, y);
       tc_load_f32(my + kTcX + c0, x);
@@ -407,29 +386,29 @@ __global__ void __launch_bounds__(kTcThreads, 1) delta_fwd_tc(const __grid_const
     if (p.last != nullptr && live) {
       float* last = p.last + head * p.dkw * p.dvw + d;
 #pragma unroll
-      for (int i = 0; i < HK; ++i) {
-        const int k = half * HK + i;
-        if (k < p.dkw) last[(size_t)k * p.dvw] = S[i / 32][i % 32];
+      for (int i = 0; i < QK; ++i) {
+        const int k = quarter * QK + i;
+        if (k < p.dkw) last[(size_t)k * p.dvw] = S[i / 16][i % 16];
       }
     }
     tc_fence_before();
   }
   wait.drain();
   __syncthreads();
-  if (warp == 8) tc_free(tm, kTcCols);
+  if (warp == 16) tc_free(tm, kTcCols);
 }
 
 // ---- backward, chunks in reverse ------------------------------------------------------------------
 template <typename T, int NP, int DKP>
 __global__ void __launch_bounds__(kTcThreads, 1) delta_bwd_tc(const __grid_constant__ DeltaParams p) {
-  constexpr int HK = DKP / 2;
+  constexpr int QK = DKP / 4;
   using Smem = TcSmem<NP, DKP, 3>;
   Smem& s = tc_smem<Smem>();
   const int h = blockIdx.y, b = blockIdx.z, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   tc_init(s);
   const uint32_t tm = __shfl_sync(0xffffffffu, s.tmem, 0);
   TcWait wait{p.err};
-  if (warp == 8) {
+  if (warp == 16) {
     const uint32_t issue = lane == 0;
     for (int i = 0; issue && i < 2 && i < p.n; ++i) tc_load_stage(s, p, b, h, p.n - 1 - i, i);
     for (int it = 0; it < p.n; ++it) {
@@ -458,57 +437,63 @@ __global__ void __launch_bounds__(kTcThreads, 1) delta_bwd_tc(const __grid_const
     }
     __syncwarp();
   } else {
-    const int half = warp >> 2, row = 32 * (warp & 3) + lane, d = 128 * blockIdx.x + row;
+    const int quarter = warp >> 2, row = 32 * (warp & 3) + lane, d = 128 * blockIdx.x + row;
     const bool live = d < p.dvw;
     const int kept = p.dvp - (d - lane);           // rows of this warp that the saved arrays have
     const uint32_t my = tm + ((uint32_t)(32 * (warp & 3)) << 16);
     const size_t head = (size_t)b * p.Hv + h;
     const T* gb = static_cast<const T*>(p.o.ptr) + b * p.o.sb + h * p.o.sh + d;
     T* ob = static_cast<T*>(const_cast<void*>(p.dv.ptr)) + b * p.dv.sb + h * p.dv.sh + d;
-    const int c0 = 32 * half;
-    float S[HK / 32][32];
+    const int c0 = 16 * quarter;
+    float S[QK / 16][16];
     const float* h0 = p.h0 != nullptr ? p.h0 + head * p.dkw * p.dvw + d : nullptr;
 #pragma unroll
-    for (int i = 0; i < HK; ++i) {
-      const int k = half * HK + i;
-      S[i / 32][i % 32] = h0 != nullptr && live && k < p.dkw ? h0[(size_t)k * p.dvw] : 0.0f;
+    for (int i = 0; i < QK; ++i) {
+      const int k = quarter * QK + i;
+      S[i / 16][i % 16] = h0 != nullptr && live && k < p.dkw ? h0[(size_t)k * p.dvw] : 0.0f;
     }
-    T gr[32];
+    T gr[16];
     auto fetch = [&](int ch) {
       tc_load_col(gb + ((long long)ch * kC + c0) * p.o.sl, p.o.sl, p.L - ch * kC - c0, live, gr);
     };
+    auto put_grad = [&] {
+      float x[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[i] = to_f32(gr[i]);
+      tc_put<NP>(my + kTcO + c0 / 2, kC / 2, x);
+    };
     fetch(p.n - 1);
+    put_grad();
     for (int it = 0; it < p.n; ++it) {
       const int ch = p.n - 1 - it, st = it & 1, par = it & 1, rows = min(kC, p.L - ch * kC);
       const float* vec = s.stage[st].vec;
       const long long t0 = (long long)ch * kC + c0;
-      float x[32];
+      float x[16];
 #pragma unroll
-      for (int i = 0; i < HK / 32; ++i) tc_put<3>(my + kTcS + half * (HK / 2) + 16 * i, DKP / 2, S[i]);
+      for (int i = 0; i < QK / 16; ++i) tc_put<3>(my + kTcS + quarter * (QK / 2) + 8 * i, DKP / 2, S[i]);
 #pragma unroll
-      for (int i = 0; i < 32; ++i) x[i] = to_f32(gr[i]);
-      tc_put<NP>(my + kTcO + c0 / 2, kC / 2, x);
+      for (int i = 0; i < 16; ++i) x[i] = to_f32(gr[i]);
       wait(&s.full[st], (it >> 1) & 1);
       tc_each(vec + c0, [&](int i, float eg) { x[i] *= p.scale * eg; });
       tc_put<3>(my + kTcG + c0 / 2, kC / 2, x);
       tc_ready(&s.ready[0]);
       if (NP == 3 && ch > 0) fetch(ch - 1);
-      float* dst = p.dstates + ((head * p.n + ch) * p.dvp + d - lane) * DKP + half * HK;
+      float* dst = p.dstates + ((head * p.n + ch) * p.dvp + d - lane) * DKP + quarter * QK;
 #pragma unroll
-      for (int i = 0; i < HK / 32; ++i) tc_store_rows<Smem::kRowUnits>(s.rows[warp], dst + 32 * i, DKP, kept, S[i], lane);
+      for (int i = 0; i < QK / 16; ++i) tc_store_rows<Smem::kRowUnits>(s.rows[warp], dst + 16 * i, DKP, kept, S[i], lane);
       wait(&s.done[0], par);
       tc_fence_after();
-      float y[32];
+      float y[16];
       tc_load_f32(my + kTcD + c0, x);
       tc_load_f32(my + kTcD2 + c0, y);
       tc_each(vec + kC + c0, [&](int i, float la) { x[i] = fmaf(la, x[i], y[i]); });
       tc_put<3>(my + kTcU + c0 / 2, kC / 2, x);
       tc_ready(&s.ready[1]);
-      if (NP == 1 && ch > 0) fetch(ch - 1);      // behind the shorter wait; 32-bit values would spill (76 -> 84 us)
+      if (NP == 1 && ch > 0) fetch(ch - 1);      // behind the shorter wait; 32-bit values would spill (67 -> 72 us)
       wait(&s.done[1], par);
       tc_fence_after();
       tc_load_f32(my + kTcD + c0, x);
-      float z[32];
+      float z[16];
       tc_each(vec + 2 * kC + c0, [&](int i, float be) { z[i] = x[i] * be; });
       tc_each(vec + c0, [&](int i, float eg) { y[i] = -eg * z[i]; });
       tc_put<3>(my + kTcLU + c0 / 2, kC / 2, y);
@@ -516,28 +501,29 @@ __global__ void __launch_bounds__(kTcThreads, 1) delta_bwd_tc(const __grid_const
       tc_store_rows<Smem::kRowUnits>(s.rows[warp], p.dxs + ((head * p.n + ch) * p.dvp + d - lane) * kC + c0, kC, kept, x, lane);
       tc_store_col(ob + t0 * p.dv.sl, p.dv.sl, rows - c0, live, z);
       const float keep = vec[kC - 1];
+      if (ch > 0) put_grad();
       wait(&s.done[2], par);
       tc_fence_after();
 #pragma unroll
-      for (int j = 0; j < HK / 32; ++j) {
-        tc_load_f32(my + kTcD + half * HK + 32 * j, x);
+      for (int j = 0; j < QK / 16; ++j) {
+        tc_load_f32(my + kTcD + quarter * QK + 16 * j, x);
 #pragma unroll
-        for (int i = 0; i < 32; ++i) S[j][i] = fmaf(keep, S[j][i], x[i]);
+        for (int i = 0; i < 16; ++i) S[j][i] = fmaf(keep, S[j][i], x[i]);
       }
     }
     if (p.last != nullptr && live) {
       float* last = p.last + head * p.dkw * p.dvw + d;
 #pragma unroll
-      for (int i = 0; i < HK; ++i) {
-        const int k = half * HK + i;
-        if (k < p.dkw) last[(size_t)k * p.dvw] = S[i / 32][i % 32];
+      for (int i = 0; i < QK; ++i) {
+        const int k = quarter * QK + i;
+        if (k < p.dkw) last[(size_t)k * p.dvw] = S[i / 16][i % 16];
       }
     }
     tc_fence_before();
   }
   wait.drain();
   __syncthreads();
-  if (warp == 8) tc_free(tm, kTcCols);
+  if (warp == 16) tc_free(tm, kTcCols);
 }
 
 }  // namespace ssm
