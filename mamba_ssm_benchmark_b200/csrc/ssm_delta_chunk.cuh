@@ -11,10 +11,14 @@
 //
 // One CTA per SM walks over (chunk, head, batch).  dv is walked 16 channels at a time: bulk copies bring slabs of S,
 // dS', U and dX (fp32) ahead; sixteen warps split them into bf16 pieces in 128-byte-swizzled tiles, two slabs' worth,
-// one warp multiplies them, and one copies and does the last sums along a chunk.  The 128 rows of a product are two operands of 64 positions on top of one
-// another: [dO; dX] [S | U]^T, [0; U] dS'^T, then [M; N] K and [0; (beta N)^T] K + [0; M^T] Q; so a thread meets H and C
-// of one position, or dQ.  Sums of small products and of leading ones are kept apart where tensor memory has the
-// columns for it (E3 at dk > 64 has not).  5120 chunks of 128 x 128 (bf16): 584 us; on mma.sync, 1020.
+// one warp multiplies them, and one copies and does the last sums along a chunk.  The 128 rows of a product are two
+// operands of 64 positions on top of one another: [dO; dX] [S | U]^T, [0; U] dS'^T, then [M; N] K and
+// [0; (beta N)^T] K + [0; M^T] Q; so a thread meets H and C of one position, or dQ.  Sums of small products and of
+// leading ones are kept apart where tensor memory has the columns for it (E3 at dk > 64 has not).
+//
+// 5120 chunks of 128 x 128 (bf16): 584 us, on mma.sync 1020.  Of 29 thousand clocks a chunk the slabs take 16, where
+// pieces written and operands read fill shared memory's bandwidth; the 13 behind the last slab are overlapped by
+// nothing, as the accumulators fill tensor memory.
 #pragma once
 
 #include "ssm_delta_tc.cuh"

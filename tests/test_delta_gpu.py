@@ -80,6 +80,20 @@ def test_forward_and_gradients(shape, dtype, h0):
     assert torch.equal(o, got["o"]) and torch.equal(last, got["last"])
 
 
+@pytest.mark.parametrize("shape", [(10, 260, 4, 8, 128, 16), (30, 70, 3, 6, 40, 24), (12, 200, 6, 6, 128, 65),
+                                   (8, 250, 5, 10, 64, 144)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_gradients_of_several_chunks_per_sm(shape, dtype):
+    """More chunks than the GPU has SMs, of one to nine slabs of 16 channels each; the same again, bit by bit."""
+    t, do, dlast = _inputs(*shape, dtype=dtype, seed=sum(shape))
+    got = _run(gated_delta_rule, t, do, dlast, lambda x: x.to(DEV))
+    _compare(got, _run(O.gated_delta_rule, t, do, dlast, lambda x: x.double()))
+    for _ in range(3):
+        again = _run(gated_delta_rule, t, do, dlast, lambda x: x.to(DEV))
+        for n, x in got.items():
+            assert torch.equal(again[n], x), n
+
+
 def test_gradients_against_differences():
     """<grad, d> against central differences of the float64 definition along random directions d: with steps of 1e-5
     the difference quotient is exact to about 1e-9 of the terms' size."""
