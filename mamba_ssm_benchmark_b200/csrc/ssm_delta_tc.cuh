@@ -12,9 +12,9 @@
 //   forward   S -> [K S, Q S] -> X -> [T X] -> U -> [P U, K^T U]
 //   backward  dS' -> [K dS', P^T dO] -> Y -> [T^T Y] -> dX -> [Q^T dO, K^T dX]
 //
-// 80 heads of 128 x 128, 4096 positions, bf16, training: 478 us forward (14 thousand clocks a chunk) and 472 us
+// 80 heads of 128 x 128, 4096 positions, bf16, training: 452 us forward (14 thousand clocks a chunk) and 472 us
 // backward; the strips take 856 and 1146, and with half the threads these kernels 456 and 562 (fp32, dk 64: 67 and 77
-// instead of 63 and 67).  The rounds' products take 2.4, 1.7 and 1.8 thousand clocks, about 53 an instruction whatever
+// instead of 62 and 67).  The rounds' products take 2.4, 1.7 and 1.8 thousand clocks, about 53 an instruction whatever
 // its N up to 64; the register passes and the saved states' stores take the rest.
 #pragma once
 
@@ -345,11 +345,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) delta_fwd_tc(const __grid_const
       tc_ready(&s.ready[0]);
       T vr[16];
       tc_load_col(vb + t0 * p.v.sl, p.v.sl, rows - c0, live, vr);
-      if (SAVE) {
-        float* o = p.states + ((head * p.n + ch) * p.dvp + d - lane) * DKP + quarter * QK;
-#pragma unroll
-        for (int i = 0; i < QK / 16; ++i) tc_store_rows<Smem::kRowUnits>(s.rows[warp], o + 16 * i, DKP, kept, S[i], lane);
-      }
+      auto save = [&](int i) {                   // 16 columns of S, behind a round of products each: 478 -> 452 us
+        if (SAVE)
+          tc_store_rows<Smem::kRowUnits>(
+              s.rows[warp], p.states + ((head * p.n + ch) * p.dvp + d - lane) * DKP + quarter * QK + 16 * i, DKP, kept, S[i], lane);
+      };
+      if (QK == 32) save(0);
       wait(&s.full[st], (ch >> 1) & 1);
       wait(&s.done[0], par);
       tc_fence_after();
@@ -359,6 +360,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) delta_fwd_tc(const __grid_const
       tc_each(vec + 2 * kC + c0, [&](int i, float be) { x[i] *= be; });
       tc_put<3>(my + kTcX + c0 / 2, kC / 2, x);
       tc_ready(&s.ready[1]);
+      save(QK / 16 - 1);
       wait(&s.done[1], par);
       tc_fence_after();
       tc_load_f32(my + kTcD + c0, x);
