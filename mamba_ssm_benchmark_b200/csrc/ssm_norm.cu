@@ -259,7 +259,7 @@ struct RowQueue : Slots<T, VEC, K, BWD ? 3 : 2> {
 };
 
 // The number of rows is the same for all of a CTA's warps, so that group_sum's barriers match; rows past
-// the end work on zeros.  16384 x 5120 bf16 in 40 groups with a gate: 89 us, 5.6 TB/s of the tensors' bytes; issue
+// the end work on zeros, and what comes of that (NaN where eps is 0) goes nowhere.  16384 x 5120 bf16 in 40 groups with a gate: 89 us, 5.6 TB/s of the tensors' bytes; issue
 // slots are 78 % taken (13 operations an element, 16 of every 32 elements' special functions).
 template <typename T, int VEC, int K, int WPG>
 __global__ void __launch_bounds__(32 * kWarps) norm_rows_fwd(const __grid_constant__ NormParams p, int lpg) {
@@ -343,10 +343,15 @@ __global__ void __launch_bounds__(32 * kWarps) norm_rows_bwd(const __grid_consta
 #pragma unroll
       for (int v = 0; v < VEC; ++v) x[i][v] *= rstd;
       norm_grad(p, x[i], w[i], b[i], z[i], g[i]);
+      if (ok) {                          // a row past the end is not a zero to the sums: with eps = 0 it is NaN
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+          dw[i][v] = fmaf(g[i][v], x[i][v], dw[i][v]);
+          db[i][v] += g[i][v];
+        }
+      }
 #pragma unroll
       for (int v = 0; v < VEC; ++v) {
-        dw[i][v] = fmaf(g[i][v], x[i][v], dw[i][v]);
-        db[i][v] += g[i][v];
         g[i][v] *= w[i][v];
         s1 += g[i][v];
         s2 = fmaf(g[i][v], x[i][v], s2);
