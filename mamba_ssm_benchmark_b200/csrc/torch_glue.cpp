@@ -49,6 +49,9 @@ Tensor dense(const Tensor& t, at::ScalarType type) {
   Tensor r = t.scalar_type() == type ? t : t.to(type);
   return r.stride(-1) == 1 || r.size(-1) == 1 ? r : r.contiguous();
 }
+// Results are dense whatever the layout of the input: torch's *_like follow its strides, and for rows that overlap
+// (sliding windows) choose some that are not unit along the channels.
+Tensor dense_like(const Tensor& t) { return at::empty(t.sizes(), t.options()); }
 Tensor bytes(size_t n, const Tensor& like) { return at::empty({(int64_t)n}, like.options().dtype(at::kByte)); }
 void* stream(const Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
 
@@ -73,7 +76,7 @@ std::tuple<Tensor, Tensor> norm_forward(const Tensor& x, const Tensor& weight, c
                                         const NormArgs& a, bool keep) {
   const c10::cuda::CUDAGuard guard(x.device());
   const NormDims d(x);
-  const Tensor y = at::empty_like(x);
+  const Tensor y = dense_like(x);
   Tensor stats, ws;
   if (keep && d.p > 1) stats = at::empty({d.n, a.groups, 2}, x.options().dtype(at::kFloat));
   size_t need = 0;
@@ -103,11 +106,11 @@ struct GroupNorm : torch::autograd::Function<GroupNorm> {
     const double eps = ctx->saved_data["eps"].toDouble();
     const c10::cuda::CUDAGuard guard(x.device());
     const NormDims d(x);
-    const Tensor dy = dense(grads[0], x.scalar_type()), dx = at::empty_like(x);
+    const Tensor dy = dense(grads[0], x.scalar_type()), dx = dense_like(x);
     Tensor dz, dw, db;
-    if (z.defined()) dz = at::empty_like(z);
-    if (weight.defined()) dw = at::empty_like(weight);
-    if (bias.defined()) db = at::empty_like(bias);
+    if (z.defined()) dz = dense_like(z);
+    if (weight.defined()) dw = dense_like(weight);
+    if (bias.defined()) db = dense_like(bias);
     size_t need = 0;
     check(ssm_group_norm_workspace_size(d.n, d.p, d.c, groups, 1, &need), "ssm_group_norm_workspace_size");
     const Tensor ws = bytes(need, x);
@@ -179,7 +182,7 @@ struct GatedDelta : torch::autograd::Function<GatedDelta> {
                                           : at::zeros({d.B, d.L, d.Hv, d.dv}, v.options());
     Tensor dlast, dh0;
     if (grads[1].defined()) dlast = grads[1].to(at::kFloat).contiguous();
-    if (h0.defined()) dh0 = at::empty_like(h0);
+    if (h0.defined()) dh0 = dense_like(h0);
     const Tensor dq = at::empty(q.sizes(), q.options()), dk = at::empty(k.sizes(), k.options()),
                  dv = at::empty(v.sizes(), v.options()), dg = at::empty(g.sizes(), g.options()),
                  dbeta = at::empty(g.sizes(), g.options());

@@ -38,3 +38,39 @@ def test_eps_of_zero(shape, groups, silu, gate):
                lambda x: x.to(DEV))
     want = _run(lambda x, **kw: O.group_norm(x, groups, eps=0.0, silu=silu, **kw), t, dy, lambda x: x.double())
     _hold(got, want, _entering(t, dy, groups, silu, True))
+
+
+def _windows(t, C):
+    return t.unfold(0, C, 1)                 # rows that overlap: strides (1, 1)
+
+
+@pytest.mark.parametrize("which", ["x", "z", "both"])
+def test_overlapping_rows(which):
+    """x, z or both as sliding windows over one array: results and gradients are those of the rows, each for itself."""
+    rows, C, groups = 37, 64, 4
+    t, dy = _inputs((rows, C), torch.float32, seed=11, gate=True)
+    gen = torch.Generator().manual_seed(12)
+    long = {n: torch.randn(rows + C - 1, generator=gen) for n in ("x", "z")}
+    for n in long:
+        if which in (n, "both"):
+            t[n] = _windows(long[n], C)
+    want = _run(lambda x, **kw: O.group_norm(x, groups, **kw), t, dy, lambda x: x.double().contiguous())
+    leaves = {n: (_windows(long[n].to(DEV), C) if which in (n, "both") and n in long else x.to(DEV)).requires_grad_()
+              for n, x in t.items()}
+    assert any(x.stride() == (1, 1) for x in leaves.values())
+    y = group_norm(leaves["x"], groups, leaves["weight"], leaves["bias"], z=leaves["z"])
+    grads = torch.autograd.grad(y, list(leaves.values()), dy.to(DEV))
+    _hold({"y": y.detach(), **{"d" + n: g for n, g in zip(leaves, grads)}}, want, _entering(t, dy, groups, False, True))
+
+
+def test_overlapping_positions():
+    """The same with more than one position: strides (5, 3, 1)."""
+    base = torch.randn(5 * 2 + 3 * 8 + 64, generator=torch.Generator().manual_seed(13))
+    shape, strides = (3, 9, 64), (5, 3, 1)
+    t, dy = _inputs(shape, torch.float32, seed=14, gate=False)
+    t["x"] = base.as_strided(shape, strides)
+    want = _run(lambda x, **kw: O.group_norm(x, 4, **kw), t, dy, lambda x: x.double().contiguous())
+    leaves = {n: (base.to(DEV).as_strided(shape, strides) if n == "x" else x.to(DEV)).requires_grad_() for n, x in t.items()}
+    y = group_norm(leaves["x"], 4, leaves["weight"], leaves["bias"])
+    grads = torch.autograd.grad(y, list(leaves.values()), dy.to(DEV))
+    _hold({"y": y.detach(), **{"d" + n: g for n, g in zip(leaves, grads)}}, want, _entering(t, dy, 4, False, True))
