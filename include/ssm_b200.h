@@ -37,7 +37,7 @@
 extern "C" {
 #endif
 
-#define SSM_B200_ABI_VERSION 6
+#define SSM_B200_ABI_VERSION 7
 
 #if defined(__GNUC__)
 #define SSM_API __attribute__((visibility("default")))
@@ -357,6 +357,10 @@ SSM_API int ssm_gated_delta_workspace_size(int64_t B, int64_t L, int64_t Hk, int
                                    int32_t dtype, int32_t backward, size_t* bytes);
 SSM_API int ssm_gated_delta_saved_size(int64_t B, int64_t L, int64_t Hk, int64_t Hv, int64_t dk, int64_t dv,
                                int32_t dtype, size_t* bytes);
+/* How a call takes the state from chunk to chunk: `channels` value channels of a head to a CTA, 16 or 32 (strips on
+ * mma.sync) or 128 (tcgen05). */
+SSM_API int ssm_gated_delta_plan(int64_t B, int64_t L, int64_t Hk, int64_t Hv, int64_t dk, int64_t dv,
+                         int32_t dtype, int32_t backward, int32_t* channels);
 SSM_API int ssm_gated_delta_fwd(int64_t B, int64_t L, int64_t Hk, int64_t Hv, int64_t dk, int64_t dv,
                         ssm_heads q, ssm_heads k, ssm_heads v, ssm_view g, ssm_view beta, const float* h0, float scale,
                         ssm_heads o, float* last, void* saved, void* workspace, size_t workspace_bytes, void* stream);

@@ -19,7 +19,7 @@ SSM_OK, SSM_ERR_INVALID, SSM_ERR_DTYPE, SSM_ERR_WORKSPACE, SSM_ERR_CUDA, SSM_ERR
 SSM_F32, SSM_BF16 = 0, 1
 METHODS = {"zoh": 0, "euler": 1, "bilinear": 2}
 DTYPES = {torch.float32: SSM_F32, torch.bfloat16: SSM_BF16}
-ABI_VERSION = 6
+ABI_VERSION = 7
 
 # Every symbol include/ssm_b200.h declares (checked by the tests).
 EXPORTED = (
@@ -29,8 +29,8 @@ EXPORTED = (
     "ssm_scan_bwd_summary", "ssm_conv1d_fwd", "ssm_conv1d_bwd_workspace_size", "ssm_conv1d_bwd",
     "selective_scan_fwd", "selective_scan_bwd", "selective_state_update", "ssm_scan_fwd_ex", "ssm_scan_bwd_ex",
     "ssm_scan_bwd_plan", "ssm_compose_shards",
-    "ssm_gated_delta_workspace_size", "ssm_gated_delta_saved_size", "ssm_gated_delta_fwd", "ssm_gated_delta_bwd",
-    "ssm_gated_delta_state_update", "ssm_group_norm_workspace_size", "ssm_group_norm_fwd", "ssm_group_norm_bwd",
+    "ssm_gated_delta_workspace_size", "ssm_gated_delta_saved_size", "ssm_gated_delta_plan", "ssm_gated_delta_fwd",
+    "ssm_gated_delta_bwd", "ssm_gated_delta_state_update", "ssm_group_norm_workspace_size", "ssm_group_norm_fwd", "ssm_group_norm_bwd",
 )
 
 
@@ -94,6 +94,7 @@ _DIMS = [_I64] * 6                  # B, L, Hk, Hv, dk, dv
 _SIGNATURES.update({
     "ssm_gated_delta_workspace_size": (ctypes.c_int, _DIMS + [_I32, _I32, ctypes.POINTER(_SZ)]),
     "ssm_gated_delta_saved_size": (ctypes.c_int, _DIMS + [_I32, ctypes.POINTER(_SZ)]),
+    "ssm_gated_delta_plan": (ctypes.c_int, _DIMS + [_I32, _I32, ctypes.POINTER(_I32)]),
     "ssm_gated_delta_fwd": (ctypes.c_int, _DIMS + [_H, _H, _H, _V, _V, _P, _F, _H, _P, _P, _P, _SZ, _P]),
     "ssm_gated_delta_bwd": (ctypes.c_int, _DIMS + [_H, _H, _H, _V, _V, _F, _P, _H, _P, _H, _H, _H, _P, _P, _P,
                                                    _P, _SZ, _P]),
@@ -231,6 +232,14 @@ def bwd_plan(B, L, D, N, dtype):
     code = SSM_BF16 if dtype == torch.bfloat16 else SSM_F32
     check(lib().ssm_scan_bwd_plan(B, L, D, N, code, ctypes.byref(S), ctypes.byref(n)), "ssm_scan_bwd_plan")
     return S.value, n.value
+
+
+def delta_channels(B, L, Hk, Hv, dk, dv, dtype, backward=False):
+    """Value channels of a head that a CTA of the gated delta rule's chain takes: 16 or 32 (strips), 128 (tcgen05)."""
+    n = _I32(0)
+    code = SSM_BF16 if dtype == torch.bfloat16 else SSM_F32
+    check(lib().ssm_gated_delta_plan(B, L, Hk, Hv, dk, dv, code, int(backward), ctypes.byref(n)), "ssm_gated_delta_plan")
+    return n.value
 
 
 def bwd_workspace_bytes(B, L, D, N):

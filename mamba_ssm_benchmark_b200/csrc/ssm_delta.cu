@@ -973,18 +973,25 @@ cudaError_t run_chain_tc(const Shape& s, const DeltaParams& p, bool bwd, cudaStr
 //   two strips            65 / 71          59 / 60          80 / 80
 //   tcgen05, 128 rows     121 / 125        82 / 97          118 / 125
 // (fp32 keys above 64 channels leave shared memory for one strip only.)
+// Returns the value channels that a CTA takes: 16 or 32 (strips), 128 (tcgen05).
+int chain_rows(const Shape& s) {
+  const bool wide = s.dkp() == 128;
+  if (s.np() == 3 && wide) return 16;
+  const int64_t heads = s.B * s.Hv, tiles = s.dvp() / 16;
+  auto waves = [heads](int64_t ctas_per_head) { return (double)((heads * ctas_per_head + 147) / 148); };
+  const double one = waves(tiles), two = waves((tiles + 1) / 2) * (s.np() == 3 || !wide ? 1.7 : 1.5);
+  const double tc = waves((s.dv + 127) / 128) * (s.np() == 3 ? 2.5 : !wide ? 2.4 : 2.6);
+  if (tc < one && tc < two) return 128;
+  return two < one ? 32 : 16;
+}
 template <typename T, int NP, int DKP>
 cudaError_t run_chain(const Shape& s, const DeltaParams& p, bool bwd, cudaStream_t st) {
-  if constexpr (NP == 3 && DKP == 128) {
-    return run_chain_ns<T, NP, DKP, 1>(s, p, bwd, st);
-  } else {
-    const int64_t heads = s.B * s.Hv, tiles = s.dvp() / 16;
-    auto waves = [heads](int64_t ctas_per_head) { return (double)((heads * ctas_per_head + 147) / 148); };
-    const double one = waves(tiles), two = waves((tiles + 1) / 2) * (NP == 3 || DKP == 64 ? 1.7 : 1.5);
-    const double tc = waves((s.dv + 127) / 128) * (NP == 3 ? 2.5 : DKP == 64 ? 2.4 : 2.6);
-    if (tc < one && tc < two) return run_chain_tc<T, NP, DKP>(s, p, bwd, st);
-    return two < one ? run_chain_ns<T, NP, DKP, 2>(s, p, bwd, st) : run_chain_ns<T, NP, DKP, 1>(s, p, bwd, st);
+  if constexpr (NP == 1 || DKP == 64) {
+    const int rows = chain_rows(s);
+    if (rows == 128) return run_chain_tc<T, NP, DKP>(s, p, bwd, st);
+    if (rows == 32) return run_chain_ns<T, NP, DKP, 2>(s, p, bwd, st);
   }
+  return run_chain_ns<T, NP, DKP, 1>(s, p, bwd, st);
 }
 template <typename T, int NP, int DKP>
 cudaError_t run_fwd(const Shape& s, const DeltaParams& p, cudaStream_t st) {
@@ -1045,6 +1052,17 @@ int ssm_gated_delta_saved_size(int64_t B, int64_t L, int64_t Hk, int64_t Hv, int
   DeltaParams p;
   memset(&p, 0, sizeof(p));
   *bytes = carve_saved(s, p, nullptr);
+  return SSM_OK;
+}
+
+int ssm_gated_delta_plan(int64_t B, int64_t L, int64_t Hk, int64_t Hv, int64_t dk, int64_t dv, int32_t dtype,
+                         int32_t backward, int32_t* channels) {
+  if (channels == nullptr) return fail(SSM_ERR_INVALID, "gated delta rule: channels is NULL");
+  const Shape s{B, L, Hk, Hv, dk, dv, dtype};
+  int rc = check_shape(s);
+  if (rc) return rc;
+  (void)backward;                  // both directions go by the same rule
+  *channels = chain_rows(s);
   return SSM_OK;
 }
 
