@@ -8,7 +8,9 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/extension.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
+#include <initializer_list>
 #include <optional>
 #include <string>
 #include <tuple>
@@ -58,6 +60,14 @@ void* stream(const Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.device(
 // The kernels write gradients that have no history of their own.
 void once(const char* what) {
   TORCH_CHECK(!at::GradMode::is_enabled(), what, " is differentiable once: create_graph=True is not supported");
+}
+
+// What a call would drop without a word: the tangent of a forward-mode derivative, which the kernels do not form, and the
+// launch itself under torch.jit.trace, which records the allocation of a result and not what fills it.
+void plain(const char* what, std::initializer_list<Tensor> inputs) {
+  for (const Tensor& t : inputs)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(0).defined(), what, " has no forward-mode derivative");
+  TORCH_CHECK(!torch::jit::tracer::isTracing(), what, " cannot be traced by torch.jit.trace");
 }
 
 // ---- group norm -------------------------------------------------------------------------------
@@ -127,6 +137,7 @@ bool wants(const Maybe& t) { return t.has_value() && t->requires_grad(); }
 
 Tensor group_norm(const Tensor& x, int64_t groups, const Maybe& weight, const Maybe& bias, const Maybe& z, double eps,
                   bool silu, bool center) {
+  plain("group_norm", {x, value(weight), value(bias), value(z)});
   if (at::GradMode::is_enabled() && (wants(x) || wants(weight) || wants(bias) || wants(z)))
     return GroupNorm::apply(x, weight, bias, z, groups, eps, silu, center);
   return std::get<0>(norm_forward(x, value(weight), value(bias), value(z), NormArgs{groups, eps, silu, center}, false));
@@ -201,6 +212,7 @@ struct GatedDelta : torch::autograd::Function<GatedDelta> {
 
 std::tuple<Tensor, Tensor> gated_delta(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, const Tensor& beta,
                                        const Maybe& h0, double scale) {
+  plain("gated_delta_rule", {q, k, v, g, beta, value(h0)});
   if (at::GradMode::is_enabled() && (wants(q) || wants(k) || wants(v) || wants(g) || wants(beta) || wants(h0))) {
     const variable_list r = GatedDelta::apply(q, k, v, g, beta, h0, scale);
     return {r[0], r[1]};
@@ -212,6 +224,7 @@ std::tuple<Tensor, Tensor> gated_delta(const Tensor& q, const Tensor& k, const T
 // One token: q, k (B, Hk, dk), v (B, Hv, dv), g, beta (B, Hv); the state in place.
 Tensor gated_delta_step(const Tensor& state, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g,
                         const Tensor& beta, double scale, const Maybe& out) {
+  plain("gated_delta_state_update", {state, q, k, v, g, beta});
   const c10::cuda::CUDAGuard guard(q.device());
   const Tensor o = out.has_value() ? *out : at::empty(v.sizes(), v.options());
   check(ssm_gated_delta_state_update(q.size(0), q.size(1), v.size(1), q.size(2), v.size(2), f32(state), heads(q), heads(k),
