@@ -7,6 +7,7 @@ output needs no copy) and fuse the bias and the SiLU.
 """
 
 import torch
+import torch.autograd.forward_ad as fwAD
 
 from . import _native as nat
 
@@ -91,8 +92,10 @@ def causal_conv1d(x, weight, bias=None, activation="silu", conv_state=None, upda
     w = _weight2d(weight, D)
     b = None if bias is None else bias.to(torch.float32).contiguous()
     if conv_state is None:
+        # the autograd function also refuses what it has no rule for (forward mode) and is what a trace records
         if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or
-                                        (bias is not None and bias.requires_grad)):
+                                        (bias is not None and bias.requires_grad)) or \
+                torch.jit.is_tracing() or any(t is not None and fwAD.unpack_dual(t).tangent is not None for t in (x, w, b)):
             out = CausalConv1dFn.apply(x, w, b, silu)
         else:
             out = _fwd(x, w, b, silu)
