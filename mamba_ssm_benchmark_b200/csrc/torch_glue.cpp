@@ -178,22 +178,23 @@ struct GatedDelta : torch::autograd::Function<GatedDelta> {
   static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g,
                                const Tensor& beta, const Maybe& h0, double scale) {
     const auto [o, last, saved] = delta_forward(q, k, v, g, beta, value(h0), scale, true);
-    ctx->save_for_backward({q, k, v, g, beta, value(h0), saved});
+    ctx->save_for_backward({q, k, v, g, beta, saved});      // the first state is in `saved`: h0 may be updated in place
     ctx->saved_data["scale"] = scale;
+    ctx->saved_data["h0"] = h0.has_value();
     ctx->set_materialize_grads(false);
     return {o, last};
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     once("gated_delta_rule");
     const variable_list saved = ctx->get_saved_variables();
-    const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &g = saved[3], &beta = saved[4], &h0 = saved[5];
+    const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &g = saved[3], &beta = saved[4], &tiles = saved[5];
     const c10::cuda::CUDAGuard guard(q.device());
     const DeltaDims d(q, v);
     const Tensor d_o = grads[0].defined() ? dense(grads[0], v.scalar_type())
                                           : at::zeros({d.B, d.L, d.Hv, d.dv}, v.options());
     Tensor dlast, dh0;
     if (grads[1].defined()) dlast = grads[1].to(at::kFloat).contiguous();
-    if (h0.defined()) dh0 = dense_like(h0);
+    if (ctx->saved_data["h0"].toBool()) dh0 = at::empty({d.B, d.Hv, d.dk, d.dv}, g.options());
     const Tensor dq = at::empty(q.sizes(), q.options()), dk = at::empty(k.sizes(), k.options()),
                  dv = at::empty(v.sizes(), v.options()), dg = at::empty(g.sizes(), g.options()),
                  dbeta = at::empty(g.sizes(), g.options());
@@ -202,7 +203,7 @@ struct GatedDelta : torch::autograd::Function<GatedDelta> {
           "ssm_gated_delta_workspace_size");
     const Tensor ws = bytes(need, q);
     check(ssm_gated_delta_bwd(d.B, d.L, d.Hk, d.Hv, d.dk, d.dv, heads(q), heads(k), heads(v), view(g), view(beta),
-                              (float)ctx->saved_data["scale"].toDouble(), saved[6].const_data_ptr(), heads(d_o), f32(dlast),
+                              (float)ctx->saved_data["scale"].toDouble(), tiles.const_data_ptr(), heads(d_o), f32(dlast),
                               heads(dq), heads(dk), heads(dv), f32(dg), f32(dbeta), f32(dh0), ws.mutable_data_ptr(), need,
                               stream(q)),
           "ssm_gated_delta_bwd");

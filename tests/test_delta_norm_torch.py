@@ -55,3 +55,23 @@ def test_tracing_is_refused():
             torch.jit.trace(fn, (t["q"],), check_trace=False)
     with pytest.raises(RuntimeError, match="traced"):
         torch.jit.trace(lambda x: group_norm(x, 4), (n["x"],), check_trace=False)
+
+
+def test_state_updated_in_place_before_the_backward():
+    """Truncated back-propagation: the state buffer takes the last state while the graph of the call that read it is alive."""
+    t = _delta()
+    t["q"].requires_grad_()
+    o, last = gated_delta_rule(**t)
+    (want,) = torch.autograd.grad(o.sum() + last.sum(), t["q"], retain_graph=True)
+    t["h0"].copy_(last.detach())
+    (got,) = torch.autograd.grad(o.sum() + last.sum(), t["q"])
+    assert torch.equal(got, want)
+
+
+def test_gradient_of_the_first_state():
+    t = {n: x.requires_grad_() for n, x in _delta().items()}
+    o, last = gated_delta_rule(**{**t, "h0": t["h0"].transpose(2, 3).contiguous().transpose(2, 3)})
+    (a,) = torch.autograd.grad(o.sum() + last.sum(), t["h0"])
+    o, last = gated_delta_rule(**{**t, "h0": t["h0"]})
+    (b,) = torch.autograd.grad(o.sum() + last.sum(), t["h0"])
+    assert a.shape == t["h0"].shape and torch.equal(a, b)
