@@ -561,28 +561,30 @@ __device__ __forceinline__ void for_cells(const NormParams& p, F f) {
   for (int e = threadIdx.x; e < cells; e += 256) f(e / p.cg, e % p.cg);
 }
 
-// A CTA per (sample, group): mean and rstd from the slabs' per-channel means and squared deviations.
+// A CTA per (sample, group), or several in turn where there are more of them than a grid holds: mean and rstd from the
+// slabs' per-channel means and squared deviations.
 __global__ void __launch_bounds__(256) norm_combine_stats(const __grid_constant__ NormParams p) {
-  const long long n = blockIdx.x / p.G;
-  const float* part = p.part + n * p.nslab * 2 * p.C + (long long)(blockIdx.x % p.G) * p.cg;
   const double m = (double)p.P * p.cg;
   auto rows = [&](int slab) {
     const long long r0 = slab * p.slab;
     return (double)((r0 + p.slab < p.P ? r0 + p.slab : p.P) - r0);
   };
-  double mean = 0.0, q = 0.0;
-  if (p.center) {
-    for_cells(p, [&](int slab, int c) { mean += rows(slab) * part[(long long)slab * 2 * p.C + c]; });
-    mean = cta_sum(mean) / m;
+  for (long long i = blockIdx.x; i < p.N * p.G; i += gridDim.x) {
+    const float* part = p.part + i / p.G * p.nslab * 2 * p.C + i % p.G * p.cg;
+    double mean = 0.0, q = 0.0;
+    if (p.center) {
+      for_cells(p, [&](int slab, int c) { mean += rows(slab) * part[(long long)slab * 2 * p.C + c]; });
+      mean = cta_sum(mean) / m;
+    }
+    for_cells(p, [&](int slab, int c) {
+      const float* at = part + (long long)slab * 2 * p.C + c;
+      const double d = at[0] - mean;
+      q += at[p.C] + rows(slab) * d * d;
+    });
+    q = cta_sum(q);
+    if (threadIdx.x == 0)
+      *reinterpret_cast<float2*>(p.stats + i * 2) = make_float2((float)mean, (float)(1.0 / sqrt(q / m + (double)p.eps)));
   }
-  for_cells(p, [&](int slab, int c) {
-    const float* at = part + (long long)slab * 2 * p.C + c;
-    const double d = at[0] - mean;
-    q += at[p.C] + rows(slab) * d * d;
-  });
-  q = cta_sum(q);
-  if (threadIdx.x == 0)
-    *reinterpret_cast<float2*>(p.stats + blockIdx.x * 2LL) = make_float2((float)mean, (float)(1.0 / sqrt(q / m + (double)p.eps)));
 }
 
 template <typename T, int VEC, bool ROWS>
@@ -648,22 +650,24 @@ __global__ void __launch_bounds__(32 * kWarps) norm_col_grads(const __grid_const
   write_partials<VEC>(p.part, blockIdx.x, p.C, c, live, dw, db);
 }
 
-// A CTA per (sample, group): s1 / M and s2 / M from the channels' sums.
+// s1 / M and s2 / M from the channels' sums; CTAs as in norm_combine_stats.
 __global__ void __launch_bounds__(256) norm_combine_sums(const __grid_constant__ NormParams p) {
-  const long long n = blockIdx.x / p.G, c0 = (long long)(blockIdx.x % p.G) * p.cg;
-  const float* part = p.part + n * p.nslab * 2 * p.C + c0;
-  double s1 = 0.0, s2 = 0.0;
-  for_cells(p, [&](int slab, int c) {
-    const float* at = part + (long long)slab * 2 * p.C + c;
-    const double w = p.w != nullptr ? p.w[c0 + c] : 1.0f;
-    s2 += w * at[0];
-    s1 += w * at[p.C];
-  });
-  s2 = cta_sum(s2);
-  s1 = cta_sum(s1);
   const double m = (double)p.P * p.cg;
-  if (threadIdx.x == 0)
-    *reinterpret_cast<float2*>(p.sums + blockIdx.x * 2LL) = make_float2(p.center ? (float)(s1 / m) : 0.0f, (float)(s2 / m));
+  for (long long i = blockIdx.x; i < p.N * p.G; i += gridDim.x) {
+    const long long c0 = i % p.G * p.cg;
+    const float* part = p.part + i / p.G * p.nslab * 2 * p.C + c0;
+    double s1 = 0.0, s2 = 0.0;
+    for_cells(p, [&](int slab, int c) {
+      const float* at = part + (long long)slab * 2 * p.C + c;
+      const double w = p.w != nullptr ? p.w[c0 + c] : 1.0f;
+      s2 += w * at[0];
+      s1 += w * at[p.C];
+    });
+    s2 = cta_sum(s2);
+    s1 = cta_sum(s1);
+    if (threadIdx.x == 0)
+      *reinterpret_cast<float2*>(p.sums + i * 2) = make_float2(p.center ? (float)(s1 / m) : 0.0f, (float)(s2 / m));
+  }
 }
 
 template <typename T, int VEC, bool ROWS>
@@ -761,7 +765,8 @@ int rows_vec(int cg, int es, std::initializer_list<ssm_view> views) {
 int check_shape(int64_t N, int64_t P, int64_t C, int64_t G) {
   if (N < 1 || P < 1 || C < 1) return fail(SSM_ERR_INVALID, "group_norm: samples, positions and channels must be positive");
   if (G < 1 || C % G != 0) return fail(SSM_ERR_INVALID, "group_norm: %lld channels do not split into %lld groups", C, G);
-  if (N > (1LL << 30) || P > (1LL << 30) || C > (1LL << 20))
+  // 2^40 elements are more than a GPU holds; below that the grids over slabs of rows fit
+  if (N > (1LL << 30) || P > (1LL << 30) || C > (1LL << 20) || N * C > (1LL << 40) || P > (1LL << 40) / (N * C))
     return fail(SSM_ERR_INVALID, "group_norm: shape out of range (samples %lld, channels %lld)", N, C);
   return SSM_OK;
 }
@@ -844,6 +849,8 @@ void launch_slabs(dim3 grid, const NormParams& p, cudaStream_t st) {
   Kern<<<grid, dim3(32, kWarps), Queue::kBytes, st>>>(p);
 }
 
+unsigned groups_grid(const NormParams& p) { return (unsigned)std::min<long long>(p.N * p.G, (1LL << 31) - 1); }
+
 // mean and rstd of every (sample, group) into p.stats
 template <typename T, int VEC>
 void run_stats(const NormParams& p, cudaStream_t st) {
@@ -853,7 +860,7 @@ void run_stats(const NormParams& p, cudaStream_t st) {
   }
   const dim3 grid((unsigned)(p.N * p.nslab), (unsigned)ceil_div(ceil_div(p.C, VEC), 32));
   launch_slabs<norm_col_stats<T, VEC>, Slots<T, VEC, 1, 2>>(grid, p, st);
-  norm_combine_stats<<<(unsigned)(p.N * p.G), 256, 0, st>>>(p);
+  norm_combine_stats<<<groups_grid(p), 256, 0, st>>>(p);
 }
 
 template <typename T, int VEC>
@@ -876,7 +883,7 @@ cudaError_t run_bwd(NormParams& p, bool stats_given, cudaStream_t st) {
   } else {
     const dim3 grid((unsigned)(p.N * p.nslab), cols);
     launch_slabs<norm_col_grads<T, VEC, false>, Slots<T, VEC, 1, 3>>(grid, p, st);
-    norm_combine_sums<<<(unsigned)(p.N * p.G), 256, 0, st>>>(p);
+    norm_combine_sums<<<groups_grid(p), 256, 0, st>>>(p);
     launch_slabs<norm_apply_bwd<T, VEC, false>, Slots<T, VEC, 1, 3>>(grid, p, st);
   }
   return cudaGetLastError();

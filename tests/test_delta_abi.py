@@ -88,3 +88,13 @@ def test_group_norm_refusals():
     assert fwd(x, z=V(P, nat.SSM_BF16, 0, 64, 64)) == nat.SSM_ERR_DTYPE and "z must" in _message()
     assert fwd(x, y=none) == nat.SSM_ERR_INVALID and "y is required" in _message()
     assert fwd(x, positions=5) == nat.SSM_ERR_WORKSPACE
+
+
+def test_group_norm_shapes_out_of_range():
+    """More elements than a GPU holds are refused before a grid is cut off; 2^32 (sample, group) pairs are not."""
+    n = ctypes.c_size_t(0)
+    size = lambda *a: nat.lib().ssm_group_norm_workspace_size(*a, ctypes.byref(n))
+    assert size(2 ** 30, 2 ** 30, 2 ** 20, 1, 0) == nat.SSM_ERR_INVALID and "range" in _message()
+    assert size(2 ** 30, 2 ** 10, 2, 1, 0) == nat.SSM_ERR_INVALID and "range" in _message()
+    assert size(2 ** 30, 1, 2 ** 11, 1, 0) == nat.SSM_ERR_INVALID and "range" in _message()
+    assert size(2 ** 22, 2, 1024, 1024, 1) == nat.SSM_OK

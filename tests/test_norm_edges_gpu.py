@@ -74,3 +74,33 @@ def test_overlapping_positions():
     y = group_norm(leaves["x"], 4, leaves["weight"], leaves["bias"])
     grads = torch.autograd.grad(y, list(leaves.values()), dy.to(DEV))
     _hold({"y": y.detach(), **{"d" + n: g for n, g in zip(leaves, grads)}}, want, _entering(t, dy, 4, False, True))
+
+
+def test_more_groups_than_a_grid_holds():
+    """2^31 (sample, group) pairs: every one has its statistics, in both directions.  Samples are independent, so slices of
+    the results are held against the definition of the same slice; dx is exact 0 up to rounding with two elements a group,
+    so the groups here are one channel at two positions with a weight, and dx is held against the size of what enters."""
+    N, P, C = 2 ** 21, 2, 1024
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < 130 * 2 ** 30:
+        pytest.skip("needs 130 GB")
+    gen = torch.Generator(device=DEV).manual_seed(21)
+    x = torch.empty(N, P, C, dtype=torch.bfloat16, device=DEV).normal_(generator=gen)
+    w = (1.0 + 0.1 * torch.randn(C, generator=gen, device=DEV)).requires_grad_()
+    slices = (slice(0, 3), slice(N // 2 - 1, N // 2 + 2), slice(N - 3, N))
+    dy = torch.zeros_like(x)
+    for sl in slices:
+        dy[sl].normal_(generator=gen)
+    x.requires_grad_()
+    y = group_norm(x, C, w)
+    dx, dw = torch.autograd.grad(y, [x, w], dy)
+    want_dw = torch.zeros(C, dtype=torch.float64)
+    for sl in slices:
+        t = {"x": x.detach()[sl].cpu(), "weight": w.detach().cpu(), "bias": torch.zeros(C)}
+        want = _run(lambda x, **kw: O.group_norm(x, C, **kw), t, dy[sl].cpu(), lambda x: x.double())
+        want_dw += want["dweight"]
+        _hold({"y": y.detach()[sl], "dx": dx[sl]}, {n: want[n] for n in ("y", "dx")}, _entering(t, dy[sl].cpu(), C, False, True))
+    off = float((dw.cpu().double() - want_dw).norm())
+    assert off <= F32_TOL * float(want_dw.norm())
+    del x, y, dx, dy
+    torch.cuda.empty_cache()
