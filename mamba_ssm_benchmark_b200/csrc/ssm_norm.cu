@@ -16,7 +16,8 @@
 //     with a warp per group for the sums.
 //   * more positions: per-(slab of rows, channel) partial sums, a combine per (sample, group), an
 //     element-wise pass (the tensors are read twice).
-// All sums are fp32 (the combines fp64) in a fixed order: no atomics, results are reproducible.
+// Sums over at most kChain rows in a row are fp32, what joins them is fp64, all in a fixed order: no atomics, results are
+// reproducible.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -37,6 +38,9 @@ using ssm::vec_load;
 using ssm::vec_store;
 
 constexpr int kWarps = 8;           // warps per CTA: rows taken side by side
+// Rows that one fp32 sum takes: its roundings stay below kChain 2^-24 = 1.5e-5 of the sum of its terms' sizes however long
+// the batch is (8192 rows in a row, as a batch of 65536 short samples had, came to 8e-5).
+constexpr int kChain = 256;
 
 struct NormParams {
   const void *x, *z, *dy;
@@ -705,24 +709,24 @@ __global__ void __launch_bounds__(32 * kWarps) norm_apply_bwd(const __grid_const
 }
 
 // dw and db: the partial rows summed in a fixed order (a warp takes every kWarps-th row, the warps'
-// sums are added in warp order).
+// sums are added in warp order), in fp64: there are as many as samples where these are short.
 __global__ void __launch_bounds__(32 * kWarps) norm_param_grads(const __grid_constant__ NormParams p, long long nparts) {
-  __shared__ float red[kWarps][32];
+  __shared__ double red[kWarps][32];
   const long long c = (long long)blockIdx.x * 32 + threadIdx.x;
   const int which = blockIdx.y;
   float* out = which ? p.db : p.dw;
-  float s = 0.0f;
+  double s = 0.0;
   if (c < p.C) {
-#pragma unroll 4
-    for (long long q = threadIdx.y; q < nparts; q += kWarps) s += p.part[(q * 2 + which) * p.C + c];
+#pragma unroll 8
+    for (long long q = threadIdx.y; q < nparts; q += kWarps) s += (double)p.part[(q * 2 + which) * p.C + c];
   }
   red[threadIdx.y][threadIdx.x] = s;
   __syncthreads();
   if (threadIdx.y == 0 && c < p.C && out != nullptr) {
-    float t = 0.0f;
+    double t = 0.0;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) t += red[w][threadIdx.x];
-    out[c] = t;
+    out[c] = (float)t;
   }
 }
 
@@ -735,13 +739,13 @@ int fail(int code, const char* fmt, long long a = 0, long long b = 0) {
 
 long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
 
-// Slabs of rows: `ctas` CTAs in all, at least 2 rows per warp in each.  Sized for fp32 vectors whatever the type, so
-// that the workspace size needs no type.
-void plan_slabs(long long ctas, long long units, long long rows, long long C, int* nslab, long long* slab) {
+// Slabs of rows: `ctas` CTAs in all, at least 2 rows per warp in each, and at most kChain rows after one another, `side` of
+// which are taken side by side.  Sized for fp32 vectors whatever the type, so that the workspace size needs no type.
+void plan_slabs(long long ctas, long long units, long long rows, long long C, int side, int* nslab, long long* slab) {
   const long long col_tiles = ceil_div(C, 128);
   long long n = ceil_div(ctas, units * col_tiles);
   n = std::min(n, ceil_div(rows, 2 * kWarps));
-  n = std::max<long long>(n, 1);
+  n = std::max<long long>({n, ceil_div(rows, side * kChain), 1});
   *slab = ceil_div(rows, n);
   *nslab = (int)ceil_div(rows, *slab);
 }
@@ -814,7 +818,9 @@ cudaError_t launch_rows(NormParams& p, bool bwd, int lpg, cudaStream_t st) {
   if (bwd) {
     constexpr size_t smem = RowQueue<T, VEC, K, true>::kBytes;
     constexpr auto kern = norm_rows_bwd<T, VEC, K, WPG>;
-    p.nslab = (int)ctas(ssm::ctas_per_sm<kern>(32 * kWarps, smem), p.nslab);
+    // as many waves as kChain asks for (the plan has room for that many partial rows)
+    const long long one = ctas(ssm::ctas_per_sm<kern>(32 * kWarps, smem), p.nslab);
+    p.nslab = (int)std::min<long long>(p.nslab, one * ceil_div(rows, one * kChain));
     kern<<<dim3((unsigned)p.nslab, gy), block, smem, st>>>(p, lpg);
   } else {
     constexpr size_t smem = RowQueue<T, VEC, K, false>::kBytes;
@@ -906,10 +912,10 @@ long long plan(NormParams& p, int64_t N, int64_t P, int64_t C, int64_t G) {
   p.G = (int)G;
   p.cg = (int)(C / G);
   if (P == 1) {
-    plan_slabs(148 * 6, 1, N, C, &p.nslab, &p.slab);
+    plan_slabs(148 * 6, 1, N, C, 1, &p.nslab, &p.slab);
     return p.nslab;
   }
-  plan_slabs(148 * 8, N, P, C, &p.nslab, &p.slab);
+  plan_slabs(148 * 8, N, P, C, kWarps, &p.nslab, &p.slab);
   return N * p.nslab;
 }
 

@@ -104,3 +104,21 @@ def test_more_groups_than_a_grid_holds():
     assert off <= F32_TOL * float(want_dw.norm())
     del x, y, dx, dy
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("shape", [(65536, 2, 64), (1 << 24, 8), (1, 1 << 22, 8), (3001, 4100)])
+def test_parameter_gradients_of_many_rows(shape):
+    """A constant gradient: every rounding of a running sum may go the same way.  One fp32 sum has at most 256 rows, and a
+    dozen more roundings follow before fp64: 270 * 2^-24 of the terms' sizes; dbias has terms of one sign."""
+    x = torch.randn(*shape, generator=torch.Generator(device=DEV).manual_seed(31), device=DEV)
+    w, b = (torch.ones(shape[-1], device=DEV, requires_grad=True) for _ in range(2))
+    dy = torch.full_like(x, 1.3)
+    dw, db = torch.autograd.grad(group_norm(x, 1, w, b, center=False), [w, b], dy)
+    bound = 270 * 2.0 ** -24
+    n = x.double()
+    n = n / (n.square().mean(dim=tuple(range(1, x.dim())), keepdim=True) + 1e-5).sqrt()
+    over = tuple(range(x.dim() - 1))
+    want = float(dy[(0,) * x.dim()].double()) * (x.numel() // shape[-1])
+    assert float((db.double() - want).abs().max()) <= bound * want
+    scale = float(dy[(0,) * x.dim()].double())
+    assert bool(((dw.double() - scale * n.sum(over)).abs() <= (bound + F32_TOL) * scale * n.abs().sum(over)).all())
