@@ -19,17 +19,19 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from .conv import causal_conv1d
-from .delta import gated_delta_rule, gated_delta_state_update
+from .delta import MAX_KEY_WIDTH, gated_delta_rule, gated_delta_state_update
 from .mixer import _Holder, _softplus_inverse
 from .norm import group_norm
 
 
 class GatedDeltaMixer(nn.Module):
     """d_model: width of the input; expand * d_model channels inside, in value heads of head_dim channels that
-    share key_heads key heads (default half as many) of the same width."""
+    share key_heads key heads (default half as many) of the same width, at most MAX_KEY_WIDTH."""
 
     def __init__(self, d_model, head_dim=64, key_heads=None, expand=2, d_conv=4, dt_min=1e-3, dt_max=0.1):
         super().__init__()
+        if not 1 <= head_dim <= MAX_KEY_WIDTH:
+            raise ValueError(f"head_dim must be 1 to {MAX_KEY_WIDTH} for the sm_100a kernels, got {head_dim}")
         self.d_inner, self.head_dim, self.d_conv = expand * d_model, head_dim, d_conv
         if self.d_inner % head_dim != 0:
             raise ValueError(f"the inner width {self.d_inner} must be a multiple of head_dim={head_dim}")

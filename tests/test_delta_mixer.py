@@ -113,3 +113,11 @@ def test_training_lowers_the_loss():
         opt.step()
         losses.append(float(loss.detach()))
     assert losses[-1] < 0.8 * losses[0]
+
+
+@pytest.mark.parametrize("make", [lambda d: GatedDeltaMixer(256, head_dim=d), lambda d: MambaLM(n_layers=1, d_model=256, mixer="delta", head_dim=d)])
+def test_head_widths_without_a_kernel_are_refused_at_once(make):
+    assert make(128) is not None
+    for d in (0, 256):
+        with pytest.raises(ValueError, match="head_dim must be"):
+            make(d)
