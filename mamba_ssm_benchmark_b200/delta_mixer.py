@@ -52,6 +52,12 @@ class GatedDeltaMixer(nn.Module):
         self.register_buffer("unit", torch.full((2 * self.d_key,), head_dim ** -0.5), persistent=False)
         self.reset_parameters(dt_min, dt_max)
 
+    def _apply(self, fn, recurse=True):
+        super()._apply(fn, recurse)
+        # moved with the module but not cast with it: rounded to bf16, keys would be up to 0.2 % off length 1
+        self.unit = torch.full_like(self.unit, self.head_dim ** -0.5, dtype=torch.float32)
+        return self
+
     @torch.no_grad()
     def reset_parameters(self, dt_min=1e-3, dt_max=0.1):
         """Decay rates in [1, 16], step sizes log-uniform in [dt_min, dt_max] through softplus; projections and

@@ -121,3 +121,24 @@ def test_head_widths_without_a_kernel_are_refused_at_once(make):
     for d in (0, 256):
         with pytest.raises(ValueError, match="head_dim must be"):
             make(d)
+
+
+def test_a_cast_leaves_the_key_scale():
+    """x / rms(x) times head_dim^-1/2: that factor in float32 whatever the model's type."""
+    for cast in (lambda m: m.bfloat16(), lambda m: m.half(), lambda m: m.bfloat16().float(), lambda m: m.to("meta").to_empty(device="cpu")):
+        m = cast(GatedDeltaMixer(128, head_dim=32))
+        assert m.unit.dtype == torch.float32 and torch.equal(m.unit, torch.full((2 * m.d_key,), 32 ** -0.5)), m.unit
+
+
+@pytest.mark.gpu
+def test_bf16_mixer_against_its_definition():
+    """A mixer in bfloat16 on its own (rounded) parameters: four operators and two projections in a row each round their
+    result (2^-8 of every element, unrelated to one another), the products before the gate pass one of them on twice."""
+    torch.manual_seed(5)
+    m = GatedDeltaMixer(64, head_dim=32).bfloat16()
+    u = torch.randn(2, 75, 64).bfloat16()
+    with torch.no_grad():
+        want = _definition(m, {n: t.detach().double() for n, t in m.named_parameters()}, u.double())
+        got = m.to(DEV)(u.to(DEV))
+    assert got.dtype == torch.bfloat16
+    assert float((got.cpu().double() - want).norm() / want.norm()) <= 8 * 2.0 ** -8
