@@ -503,7 +503,8 @@ struct SlabQueue : Slots<T, VEC, 1, GRAD ? 3 : 2> {
 
 // The passes over a slab (8 x 8192 x 512 bf16: statistics 16 us, apply 29 us; x is read twice, 67 MB each time) are
 // bound by memory.  Per (sample, slab, channel): mean and sum of squared deviations of the slab's rows, summed about the
-// slab's first row so that a large common offset costs no digits.
+// slab's first row so that a large common offset costs no digits; not centred, 0 and the sum of squares (about 0 that is
+// infinite and not NaN where an element is infinite).
 template <typename T, int VEC>
 __global__ void __launch_bounds__(32 * kWarps) norm_col_stats(const __grid_constant__ NormParams p) {
   extern __shared__ __align__(16) unsigned char smem[];
@@ -515,7 +516,7 @@ __global__ void __launch_bounds__(32 * kWarps) norm_col_stats(const __grid_const
 #pragma unroll
   for (int v = 0; v < VEC; ++v) k[v] = a[v] = q[v] = 0.0f;
   if (live) {
-    vec_load<T, VEC>(x + s.r0 * p.xp, k);
+    if (p.center) vec_load<T, VEC>(x + s.r0 * p.xp, k);
     SlabQueue<T, VEC, false, false>(smem).each(p, s, c, false, [&](long long, float (&t)[VEC], float (&)[VEC], float (&)[VEC]) {
 #pragma unroll
       for (int v = 0; v < VEC; ++v) {
@@ -542,8 +543,8 @@ __global__ void __launch_bounds__(32 * kWarps) norm_col_stats(const __grid_const
         sq += red[w][threadIdx.x][VEC + v];
       }
       float* o = p.part + ((long long)blockIdx.x * 2) * p.C + c + v;
-      o[0] = fmaf(sa, inv, k[v]);
-      o[p.C] = fmaxf(sq - sa * sa * inv, 0.0f);
+      o[0] = p.center ? fmaf(sa, inv, k[v]) : 0.0f;
+      o[p.C] = p.center ? fmaxf(sq - sa * sa * inv, 0.0f) : sq;
     }
   }
 }

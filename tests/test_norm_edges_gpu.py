@@ -122,3 +122,18 @@ def test_parameter_gradients_of_many_rows(shape):
     assert float((db.double() - want).abs().max()) <= bound * want
     scale = float(dy[(0,) * x.dim()].double())
     assert bool(((dw.double() - scale * n.sum(over)).abs() <= (bound + F32_TOL) * scale * n.abs().sum(over)).all())
+
+
+@pytest.mark.parametrize("shape,groups", [((3, 300, 64), 4), ((40, 64), 4), ((3, 2100), 1), ((3, 16400), 1)])
+def test_infinite_elements_without_centring(shape, groups):
+    """x / rms with an infinite element in a group: rms is infinite, so the element itself gives NaN and its group's others 0;
+    in the first row, in a later one, and of both signs at once.  Other groups are what they are."""
+    x = torch.randn(*shape, generator=torch.Generator().manual_seed(41))
+    x.view(shape[0], -1)[0, 3], x[1].view(-1)[-1] = float("inf"), float("-inf")
+    x[2].view(-1)[0], x[2].view(-1)[5] = float("inf"), float("-inf")
+    want = O.group_norm(x.double(), groups, center=False)
+    y = group_norm(x.to(DEV), groups, center=False).cpu()
+    assert int(want.isnan().sum()) == 4 and torch.equal(y.isnan(), want.isnan())
+    assert torch.equal(y == 0, want == 0)
+    fine = ~want.isnan()
+    assert float((y[fine] - want[fine]).norm()) <= F32_TOL * float(want[fine].norm())
