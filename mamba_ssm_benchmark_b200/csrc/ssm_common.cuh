@@ -289,7 +289,7 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
-// Bounded wait: gives up after ~2^24 polls (seconds), records the failure in *err and
+// Bounded wait: gives up after 2^24 polls (2 us each that runs out, half a minute), records the failure in *err and
 // returns, so a copy that never lands ends the kernel with an error flag instead of a hang.
 __device__ __forceinline__ void mbar_wait(uint64_t* bar, uint32_t parity, int* err) {
   for (uint32_t it = 0; it < (1u << 24); ++it) {

@@ -283,6 +283,7 @@ template <typename T, int DKP, int PU, int PO>       // pieces of the operands u
 struct alignas(16) StripSmem {
   uint4 sf[DKP / 16][3][32], xf[4][3][32], lf[4][3][32], uf[4][PU][32], of[PO ? 4 : 1][PO ? PO : 1][PO ? 32 : 1];
   Strip<T> in, out;
+  int stop;                               // a wait gave up, as the strip's leader saw it between two barriers
 };
 template <int NP, int DKP, int PP, typename StripT, int NS, int KB>
 struct alignas(128) ChainSmem {
@@ -291,17 +292,34 @@ struct alignas(128) ChainSmem {
   StripT strip[NS];
   float vec[2][kVec];
   uint64_t full[7], empty[7];             // by tile
+  int dead;                               // a wait gave up
 };
 enum { kTileK = 0, kTileV = 2, kTileQ = 4, kTileT = 5, kTileP = 6, kTiles = 7 };   // K, vectors: two each
+
+// A bounded wait that tells the CTA when it gave up: the strips then stop behind the chunk (z.stop, the same for
+// a strip's four warps), and no copy is started any more.  (Asked inside the wait, the flag costs the long prompt 4 %, a flag
+// per thread, as in Wait, 12 %.)
+template <typename Smem>
+__device__ __forceinline__ void chain_wait(Smem& s, uint64_t* bar, uint32_t parity, int* err) {
+  for (uint32_t it = 0; it < kPolls; ++it)
+    if (mbar_try_wait(bar, parity)) return;
+  *static_cast<volatile int*>(&s.dead) = 1;
+  if (err) atomicOr(err, 1);
+}
+// Before the kernel ends: after a wait that gave up, time for its copies in flight to land.
+template <typename Smem>
+__device__ __forceinline__ void chain_drain(Smem& s) {
+  for (int i = 0; *static_cast<volatile int*>(&s.dead) && i < 1000; ++i) __nanosleep(1000);
+}
 
 // The tiles of one chunk after another, chunk index by order(i), as the strips release them.
 template <int NP, int DKP, int KB, typename Smem, typename F>
 __device__ void load_tiles(Smem& s, const DeltaParams& p, int b, int h, F order) {
   const size_t at0 = ((size_t)b * p.Hv + h) * p.n, atk0 = ((size_t)b * p.Hk + h / p.group) * p.n;
   auto freed = [&](int tile, int use) {
-    if (use > 0) mbar_wait(&s.empty[tile], (use - 1) & 1, p.err);
+    if (use > 0) chain_wait(s, &s.empty[tile], (use - 1) & 1, p.err);
   };
-  for (int i = 0; i < p.n; ++i) {
+  for (int i = 0; i < p.n && !*static_cast<volatile int*>(&s.dead); ++i) {
     const int ch = order(i);
     auto load_k = [&] {
       const int buf = i % KB, tile = kTileK + buf;
@@ -324,6 +342,7 @@ __device__ void load_tiles(Smem& s, const DeltaParams& p, int b, int h, F order)
     mbar_arrive_expect_tx(&s.full[kTileP], sizeof(s.pm));
     bulk_load(s.pm, p.pimg + (at0 + ch) * (3 * kTri), sizeof(s.pm), &s.full[kTileP]);
   }
+  chain_drain(s);
 }
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
@@ -476,6 +495,7 @@ __device__ __forceinline__ void init_tiles(Smem& s, int strips) {
       mbar_init(&s.full[i], 1);
       mbar_init(&s.empty[i], strips);
     }
+    s.dead = 0;
     fence_mbar_init();
   }
   __syncthreads();
@@ -497,11 +517,16 @@ struct BwdChain {
   static constexpr int KB = sizeof(Smem<2>) <= 227 * 1024 ? 2 : 1;
 };
 
+// CTAs that shared memory lets on an SM: registers are shared out accordingly (the compiler's own choice, 128 a thread, made the
+// long prompt 3 % slower).
+template <int NP, int DKP, int NS>
+constexpr int kChainCtas = NP == 1 && DKP == 64 && NS == 1 ? 2 : 1;
+
 // ================================================================================================
 // Forward chain
 // ================================================================================================
 template <typename T, int NP, int DKP, int NS, bool SAVE>
-__global__ void __launch_bounds__(128 * NS + 32) delta_fwd(const __grid_constant__ DeltaParams p) {
+__global__ void __launch_bounds__(128 * NS + 32, kChainCtas<NP, DKP, NS>) delta_fwd(const __grid_constant__ DeltaParams p) {
   using Form = FwdChain<T, NP, DKP, NS>;
   constexpr int PP = Form::PP, KB = Form::KB, NT = DKP / 32;
   using Smem = typename Form::template Smem<KB>;
@@ -535,6 +560,7 @@ __global__ void __launch_bounds__(128 * NS + 32) delta_fwd(const __grid_constant
     put_state<DKP>(z.sf, S, w, lane);
     if (SAVE) store_acc(p.states + ((head * p.n + ch) * p.dvp + d0) * DKP + 8 * NT * w, DKP, lane, S);
     strip_sync(strip);                            // S is there; the last chunk is done with
+    if (leader) *static_cast<volatile int*>(&z.stop) = *static_cast<volatile int*>(&s.dead);
     if (leader && ch > 0) {
       mbar_arrive(&s.empty[kTileP]);
       mbar_arrive(&s.empty[kTileK + (ch - 1) % KB]);
@@ -549,9 +575,9 @@ __global__ void __launch_bounds__(128 * NS + 32) delta_fwd(const __grid_constant
     zero(X);
     zero(O);
     zero(U);
-    mbar_wait(&s.full[kTileK + buf], (ch / KB) & 1, p.err);
-    mbar_wait(&s.full[kTileV + (ch & 1)], (ch >> 1) & 1, p.err);
-    mbar_wait(&s.full[kTileQ], ch & 1, p.err);
+    chain_wait(s, &s.full[kTileK + buf], (ch / KB) & 1, p.err);
+    chain_wait(s, &s.full[kTileV + (ch & 1)], (ch >> 1) & 1, p.err);
+    chain_wait(s, &s.full[kTileQ], ch & 1, p.err);
     state_product<NP, DKP, true, PP - 1>(X, O, z.sf, sk, sq, w, lane);
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
@@ -566,7 +592,7 @@ __global__ void __launch_bounds__(128 * NS + 32) delta_fwd(const __grid_constant
     }
     strip_sync(strip);                            // X is there; Q is done with
     if (leader) mbar_arrive(&s.empty[kTileQ]);
-    mbar_wait(&s.full[kTileT], ch & 1, p.err);
+    chain_wait(s, &s.full[kTileT], ch & 1, p.err);
     tri_product<3, 3, 2, false>(U, z.xf, stt, w, lane);
     if (SAVE) store_cols(p.us + ((head * p.n + ch) * p.dvp + d0) * kC, w, lane, U);
 #pragma unroll
@@ -579,13 +605,15 @@ __global__ void __launch_bounds__(128 * NS + 32) delta_fwd(const __grid_constant
     }
     strip_sync(strip);                            // U is there; T is done with
     if (leader) mbar_arrive(&s.empty[kTileT]);
-    mbar_wait(&s.full[kTileP], ch & 1, p.err);
+    chain_wait(s, &s.full[kTileP], ch & 1, p.err);
     tri_product<PP, PP, PP - 1, false>(O, z.uf, sp, w, lane);
     state_add<NP, DKP>(S, vec[kC - 1], 1.0f, z.lf, sk, w, lane);
     z.out.write(O, w, lane);
     z.out.flush(obase + t0 * p.o.sl, p.o.sl, rows, cols, oout, w, lane);
+    if (*static_cast<volatile int*>(&z.stop)) break;
   }
   if (p.last != nullptr) state_store(p.last + head * p.dkw * p.dvw, p.dkw, p.dvw, 8 * NT * w, d0, lane, S);
+  chain_drain(s);
 }
 
 // ================================================================================================
@@ -594,7 +622,7 @@ __global__ void __launch_bounds__(128 * NS + 32) delta_fwd(const __grid_constant
 //   dS = e^G_last dS' + (scale e^G Q)^T dO - (beta e^G K)^T dX
 // ================================================================================================
 template <typename T, int NP, int DKP, int NS>
-__global__ void __launch_bounds__(128 * NS + 32) delta_bwd_chain(const __grid_constant__ DeltaParams p) {
+__global__ void __launch_bounds__(128 * NS + 32, kChainCtas<NP, DKP, NS>) delta_bwd_chain(const __grid_constant__ DeltaParams p) {
   using Form = BwdChain<T, NP, DKP, NS>;
   constexpr int KB = Form::KB, NT = DKP / 32;
   using Smem = typename Form::template Smem<KB>;
@@ -633,7 +661,7 @@ __global__ void __launch_bounds__(128 * NS + 32) delta_bwd_chain(const __grid_co
     z.in.read(dO, w, lane);
     __syncwarp();
     if (ch > 0) z.in.fetch(gbase + (t0 - kC) * p.o.sl, p.o.sl, kC, cols, gin, w, lane);
-    mbar_wait(&s.full[kTileV + (it & 1)], (it >> 1) & 1, p.err);
+    chain_wait(s, &s.full[kTileV + (it & 1)], (it >> 1) & 1, p.err);
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       put_half<NP>(z.of, col_tile(w, j), dO[j], lane);
@@ -645,11 +673,12 @@ __global__ void __launch_bounds__(128 * NS + 32) delta_bwd_chain(const __grid_co
     zero(X);
     zero(Y);
     strip_sync(strip);                            // dS' and dO are there; the last chunk is done with
+    if (leader) *static_cast<volatile int*>(&z.stop) = *static_cast<volatile int*>(&s.dead);
     if (leader && it > 0) {
       mbar_arrive(&s.empty[kTileK + (it - 1) % KB]);
       mbar_arrive(&s.empty[kTileV + ((it - 1) & 1)]);
     }
-    mbar_wait(&s.full[kTileK + buf], (it / KB) & 1, p.err);
+    chain_wait(s, &s.full[kTileK + buf], (it / KB) & 1, p.err);
     state_product<NP, DKP, false, 0>(Y, Y, z.sf, sk, sk, w, lane);
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
@@ -657,18 +686,18 @@ __global__ void __launch_bounds__(128 * NS + 32) delta_bwd_chain(const __grid_co
 #pragma unroll
       for (int e = 0; e < 4; ++e) Y[j][e] *= e & 1 ? la.y : la.x;
     }
-    mbar_wait(&s.full[kTileP], it & 1, p.err);
+    chain_wait(s, &s.full[kTileP], it & 1, p.err);
     tri_product<NP, 3, 2, true>(Y, z.of, sp, w, lane);
 #pragma unroll
     for (int j = 0; j < 2; ++j) put_half<3>(z.xf, col_tile(w, j), Y[j], lane);
-    mbar_wait(&s.full[kTileQ], it & 1, p.err);
+    chain_wait(s, &s.full[kTileQ], it & 1, p.err);
     state_add<NP, DKP>(S, vec[kC - 1], 1.0f, z.uf, sq, w, lane);
     strip_sync(strip);                            // Y is there; P and Q are done with
     if (leader) {
       mbar_arrive(&s.empty[kTileQ]);
       mbar_arrive(&s.empty[kTileP]);
     }
-    mbar_wait(&s.full[kTileT], it & 1, p.err);
+    chain_wait(s, &s.full[kTileT], it & 1, p.err);
     tri_product<3, 3, 2, true>(X, z.xf, stt, w, lane);
     store_cols(p.dxs + ((head * p.n + ch) * p.dvp + d0) * kC, w, lane, X);
 #pragma unroll
@@ -686,8 +715,10 @@ __global__ void __launch_bounds__(128 * NS + 32) delta_bwd_chain(const __grid_co
     state_add<NP, DKP>(S, 1.0f, -1.0f, z.lf, sk, w, lane);
     z.out.write(Y, w, lane);
     z.out.flush(obase + t0 * p.dv.sl, p.dv.sl, rows, cols, oout, w, lane);
+    if (*static_cast<volatile int*>(&z.stop)) break;
   }
   if (p.last != nullptr) state_store(p.last + head * p.dkw * p.dvw, p.dkw, p.dvw, 8 * NT * w, d0, lane, S);
+  chain_drain(s);
 }
 
 // dq, dk (B, L, Hk, dk): the value heads' parts, (B, L, Hv, DKP) fp32, summed in head order.  A thread takes four

@@ -352,6 +352,27 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
                : "memory");
 }
 
+// What these kernels wait for comes within microseconds.  A poll that runs out takes 3.9 thousand clocks: about a second.
+constexpr uint32_t kPolls = 1u << 19;
+
+// A bounded wait; after one that gave up the same thread waits no more, so that the kernel ends (one limit, not one per
+// chunk), and starts no copies.
+struct Wait {
+  int* err;
+  bool dead = false;
+  __device__ void operator()(uint64_t* bar, uint32_t parity) {
+    if (dead) return;
+    for (uint32_t it = 0; it < kPolls; ++it)
+      if (mbar_try_wait(bar, parity)) return;
+    if (err) atomicOr(err, 1);
+    dead = true;
+  }
+  // Before the kernel ends: after a wait that gave up, time for its copies and products in flight to land.
+  __device__ void drain() const {
+    for (int i = 0; dead && i < 1000; ++i) __nanosleep(1000);
+  }
+};
+
 struct DeltaParams {
   Heads q, k, v, o;            // o: the forward's output / the backward's incoming gradient of it
   Heads dq, dk, dv;

@@ -127,13 +127,13 @@ __global__ void __launch_bounds__(kChunkThreads, 1) delta_bwd_chunk(const __grid
   __syncthreads();
   tc_fence_after();
   const uint32_t tm = __shfl_sync(0xffffffffu, s.tmem, 0);
-  TcWait wait{p.err};
+  Wait wait{p.err};
 
   if (warp == 17) {
     // ---- copies; dbeta and dg ----
     auto fetch_slab = [&](int it) {              // slab number `it` of this CTA, counted over its items
       const size_t at = blockIdx.x + (size_t)(it / slabs) * gridDim.x;
-      if (lane != 0 || at >= (size_t)items) return;
+      if (lane != 0 || wait.dead || at >= (size_t)items) return;
       const size_t row = at * p.dvp + it % slabs * kSL;
       auto& d = s.slab[it % RB];
       uint64_t* bar = &s.full_slab[it % RB];
@@ -144,7 +144,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) delta_bwd_chunk(const __grid
       bulk_load(d.dX, p.dxs + row * kC, sizeof(d.dX), bar);
     };
     auto fetch_tiles = [&](int item) {
-      if (lane != 0 || item >= items) return;
+      if (lane != 0 || wait.dead || item >= items) return;
       const int h = item / p.n % p.Hv, b = item / p.n / p.Hv;
       const size_t atk = ((size_t)b * p.Hk + h / p.group) * p.n + item % p.n;
       mbar_arrive_expect_tx(&s.full_tiles, sizeof(s.k) + sizeof(s.q) + sizeof(s.vec));

@@ -130,23 +130,6 @@ struct alignas(1024) TcSmem {
 
 constexpr int kTcThreads = 512 + 32;
 
-// Waits like mbar_wait; after one that gave up the others do not wait any more, so that the kernel ends.
-struct TcWait {
-  int* err;
-  bool dead = false;
-  __device__ void operator()(uint64_t* bar, uint32_t parity) {
-    if (dead) return;
-    for (uint32_t it = 0; it < (1u << 24); ++it)
-      if (mbar_try_wait(bar, parity)) return;
-    if (err) atomicOr(err, 1);
-    dead = true;
-  }
-  // Before the kernel ends: after a wait that gave up, time for its copies and products in flight to land.
-  __device__ void drain() const {
-    for (int i = 0; dead && i < 1000; ++i) __nanosleep(1000);
-  }
-};
-
 // ---- products, issued by one warp -------------------------------------------------------------
 // Which products of pieces: LOW: index sums 1 .. MAXI; else the leading one.
 // d (N columns) += A (NA pieces, K / 2 columns apart) x tile of NB pieces, over K / 16 steps.
@@ -293,7 +276,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) delta_fwd_tc(const __grid_const
   const int h = blockIdx.y, b = blockIdx.z, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   tc_init(s);
   const uint32_t tm = __shfl_sync(0xffffffffu, s.tmem, 0);
-  TcWait wait{p.err};
+  Wait wait{p.err};
   if (warp == 16) {
     const uint32_t issue = lane == 0;
     for (int i = 0; issue && i < 2 && i < p.n; ++i) tc_load_stage(s, p, b, h, i, i);
@@ -308,7 +291,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) delta_fwd_tc(const __grid_const
       tc_full_product<kFull, 3, NP, PP - 1, DKP>(tm + kTcO, tm + kTcS, sq, issue);
       if (issue) tc_commit(&s.done[0]);
       // every thread is past the last chunk, whose stage is free
-      if (issue && ch >= 1 && ch + 1 < p.n) tc_load_stage(s, p, b, h, ch + 1, st ^ 1);
+      if (issue && !wait.dead && ch >= 1 && ch + 1 < p.n) tc_load_stage(s, p, b, h, ch + 1, st ^ 1);
       wait(&s.ready[1], par);
       tc_fence_after();
       tc_full_product<kLower, 3, 3, 2, DKP>(tm + kTcD, tm + kTcX, stt, issue);
@@ -409,7 +392,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) delta_bwd_tc(const __grid_const
   const int h = blockIdx.y, b = blockIdx.z, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   tc_init(s);
   const uint32_t tm = __shfl_sync(0xffffffffu, s.tmem, 0);
-  TcWait wait{p.err};
+  Wait wait{p.err};
   if (warp == 16) {
     const uint32_t issue = lane == 0;
     for (int i = 0; issue && i < 2 && i < p.n; ++i) tc_load_stage(s, p, b, h, p.n - 1 - i, i);
@@ -423,7 +406,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) delta_bwd_tc(const __grid_const
       tc_full_product<kFull, 3, NP, 2, DKP>(tm + kTcD, tm + kTcS, sk, issue);
       tc_full_product<kUpper, NP, 3, 2, DKP>(tm + kTcD2, tm + kTcO, sp, issue);
       if (issue) tc_commit(&s.done[0]);
-      if (issue && it >= 1 && it + 1 < p.n) tc_load_stage(s, p, b, h, p.n - 2 - it, st ^ 1);
+      if (issue && !wait.dead && it >= 1 && it + 1 < p.n) tc_load_stage(s, p, b, h, p.n - 2 - it, st ^ 1);
       wait(&s.ready[1], par);
       tc_fence_after();
       tc_full_product<kUpper, 3, 3, 2, DKP>(tm + kTcD, tm + kTcU, stt, issue);
