@@ -996,31 +996,41 @@ cudaError_t run_chain_tc(const Shape& s, const DeltaParams& p, bool bwd, cudaStr
   return p.states != nullptr ? launch<delta_fwd_tc<T, NP, DKP, true>>(grid, kTcThreads, fwd, p, st)
                              : launch<delta_fwd_tc<T, NP, DKP, false>>(grid, kTcThreads, fwd, p, st);
 }
-// Which chain kernel: strips, one or two to a CTA, or tcgen05.  All three keep an SM to a CTA, so a call takes waves of
-// 148 CTAs; what a wave takes, in units of one strip per CTA, was measured over 4 to 600 strips (1024 positions,
-// forward / backward in us):
-//                         bf16, dk 128     bf16, dk 64      fp32, dk 64
-//   one strip             42 / 50          33 / 37          46 / 49
-//   two strips            65 / 71          59 / 60          80 / 80
-//   tcgen05, 128 rows     121 / 125        82 / 97          118 / 125
-// (fp32 keys above 64 channels leave shared memory for one strip only.)
+// Which chain kernel: strips, one or two to a CTA, or tcgen05.  One CTA of each fills an SM's shared memory (of the bf16 ones
+// with one strip and dk up to 64, two do), so a call takes waves of 148 CTAs.  What a wave takes was measured over 4 to
+// 1184 strips in 4 to 385 heads (us for 1024 positions, 1965 MHz; forward, the mean of inference and training / backward):
+//                         bf16, dk 128     bf16, dk 64                    fp32, dk 64
+//   one strip             41 / 48          46 / 54 (up to 148: 40 / 43)   43 / 50
+//   two strips            60 / 69          47 / 55                        64 / 68
+//   tcgen05, 128 rows     112 / 121        84 / 99                        115 / 122
+// By these, the slowest of 198 choices is 11 % behind the best of the three measured, eleven are over 6 %.  Two strips never pay in
+// bf16 at dk 64; fp32 keys above 64 channels leave shared memory for one strip only.
 // Returns the value channels that a CTA takes: 16 or 32 (strips), 128 (tcgen05).
-int chain_rows(const Shape& s) {
-  const bool wide = s.dkp() == 128;
-  if (s.np() == 3 && wide) return 16;
-  const int64_t heads = s.B * s.Hv, tiles = s.dvp() / 16;
+int chain_rows(const Shape& s, bool bwd) {
+  const bool wide = s.dkp() == 128, f32 = s.np() == 3;
+  if (f32 && wide) return 16;
+  const int64_t heads = s.B * s.Hv, strips = s.dvp() / 16, pairs = (strips + 1) / 2;
   auto waves = [heads](int64_t ctas_per_head) { return (double)((heads * ctas_per_head + 147) / 148); };
-  const double one = waves(tiles), two = waves((tiles + 1) / 2) * (s.np() == 3 || !wide ? 1.7 : 1.5);
-  const double tc = waves((s.dv + 127) / 128) * (s.np() == 3 ? 2.5 : !wide ? 2.4 : 2.6);
+  const double tc = waves((s.dv + 127) / 128) * (wide ? (bwd ? 121 : 112) : f32 ? (bwd ? 122 : 115) : (bwd ? 99 : 84));
+  if (!wide && !f32) {
+    const int64_t full = heads * strips / 296, rest = heads * strips % 296;
+    const double wave = bwd ? 54 : 46;
+    const double one = (double)full * wave + (rest == 0 ? 0.0 : rest > 148 ? wave : bwd ? 43.0 : 40.0);
+    return tc < one ? 128 : 16;
+  }
+  const double strip = wide ? (bwd ? 48 : 41) : (bwd ? 50 : 43), pair = wide ? (bwd ? 69 : 60) : (bwd ? 68 : 64);
+  const double one = waves(strips) * strip;
+  const double two = waves(pairs) * ((double)(strips / 2) * pair + (double)(strips % 2) * strip) / (double)pairs;
   if (tc < one && tc < two) return 128;
   return two < one ? 32 : 16;
 }
 template <typename T, int NP, int DKP>
 cudaError_t run_chain(const Shape& s, const DeltaParams& p, bool bwd, cudaStream_t st) {
   if constexpr (NP == 1 || DKP == 64) {
-    const int rows = chain_rows(s);
+    const int rows = chain_rows(s, bwd);
     if (rows == 128) return run_chain_tc<T, NP, DKP>(s, p, bwd, st);
-    if (rows == 32) return run_chain_ns<T, NP, DKP, 2>(s, p, bwd, st);
+    if constexpr (NP == 3 || DKP == 128)
+      if (rows == 32) return run_chain_ns<T, NP, DKP, 2>(s, p, bwd, st);
   }
   return run_chain_ns<T, NP, DKP, 1>(s, p, bwd, st);
 }
@@ -1092,8 +1102,7 @@ int ssm_gated_delta_plan(int64_t B, int64_t L, int64_t Hk, int64_t Hv, int64_t d
   const Shape s{B, L, Hk, Hv, dk, dv, dtype};
   int rc = check_shape(s);
   if (rc) return rc;
-  (void)backward;                  // both directions go by the same rule
-  *channels = chain_rows(s);
+  *channels = chain_rows(s, backward != 0);
   return SSM_OK;
 }
 

@@ -20,7 +20,8 @@ F32, BF16 = torch.float32, torch.bfloat16
 # (B, L, Hk, Hv, dk, dv), types, channels a CTA: lengths that end inside a chunk, widths that fill no tile
 FORMS = [
     ((1, 130, 2, 4, 64, 48), (F32, BF16), 16), ((2, 70, 2, 2, 100, 40), (F32, BF16), 16), ((16, 70, 4, 8, 128, 128), (F32,), 16),
-    ((5, 130, 4, 8, 64, 64), (F32, BF16), 32), ((5, 130, 4, 8, 100, 50), (BF16,), 32),
+    ((5, 130, 4, 8, 64, 64), (F32,), 32), ((5, 130, 4, 8, 100, 50), (BF16,), 32), ((8, 70, 7, 21, 128, 48), (BF16,), 32),
+    ((5, 130, 4, 8, 64, 64), (BF16,), 16), ((16, 70, 4, 16, 48, 16), (BF16,), 16),
     ((16, 130, 4, 8, 64, 128), (F32, BF16), 128), ((8, 199, 8, 16, 48, 100), (F32, BF16), 128),
     ((16, 65, 8, 8, 64, 144), (F32, BF16), 128), ((16, 130, 4, 8, 128, 128), (BF16,), 128),
     ((8, 70, 5, 15, 100, 90), (BF16,), 128), ((150, 1, 1, 1, 33, 112), (F32, BF16), 128),
@@ -31,6 +32,15 @@ CASES = [(shape, dtype, channels) for shape, dtypes, channels in FORMS for dtype
 @pytest.mark.parametrize("shape,dtype,channels", CASES)
 def test_choice(shape, dtype, channels):
     assert [nat.delta_channels(*shape, dtype, backward) for backward in (False, True)] == [channels] * 2
+
+
+@pytest.mark.parametrize("heads,dk,dv,dtype,channels", [
+    (385, 128, 48, BF16, (32, 32)), (200, 64, 48, BF16, (16, 16)), (385, 64, 48, BF16, (16, 16)), (100, 128, 48, BF16, (32, 32)),
+    (200, 64, 48, F32, (32, 32)), (148, 128, 128, BF16, (128, 128)), (50, 64, 128, BF16, (128, 16)),
+])
+def test_choice_is_the_fastest_measured(heads, dk, dv, dtype, channels):
+    """Shapes at which another choice took at least 8 % more for 1024 positions."""
+    assert tuple(nat.delta_channels(1, 1024, heads, heads, dk, dv, dtype, backward) for backward in (False, True)) == channels
 
 
 def test_choice_refusals():
