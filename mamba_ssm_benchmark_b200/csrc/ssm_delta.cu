@@ -115,7 +115,8 @@ __global__ void __launch_bounds__(128, NP == 1 ? 5 : 2) delta_prep(const __grid_
       if (lane >= m) run += up;
     }
     const double total = __shfl_sync(0xffffffffu, run, 31);
-    const double G[2] = {run - (acc[1] - acc[0]), run};
+    const double before = __shfl_up_sync(0xffffffffu, run, 1);
+    const double G[2] = {lane > 0 ? before + acc[0] : acc[0], run};      // of its own position and those before, also where one is NaN
     float* vec = p.vec + at * kVec;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -221,12 +222,14 @@ __global__ void __launch_bounds__(128, NP == 1 ? 5 : 2) delta_prep(const __grid_
     }
   }
   __syncthreads();
-  // y[0 .. W) of a row of F = (A or T block)[row][m] x G[m][c ..], m < M
-  auto block_row = [&](auto& y, int M, const float* frow, float sign, const float* grow, int pitch) {
+  // y[0 .. W) of a row of F = (A or T block)[row][m] x G[m][c ..], m < M; of T's rows (`upto` their number) only up to the
+  // diagonal: behind it stand zeros, which would make NaN of a later position's values that are not finite
+  auto block_row = [&](auto& y, int M, int upto, const float* frow, float sign, const float* grow, int pitch) {
     constexpr int W = sizeof(y) / sizeof(float);
 #pragma unroll 8
     for (int m = 0; m < M; ++m) {
       const float a = sign * frow[m];
+      if (m > upto) continue;
 #pragma unroll
       for (int e = 0; e < W; e += 4) {
         float x[4];
@@ -239,11 +242,11 @@ __global__ void __launch_bounds__(128, NP == 1 ? 5 : 2) delta_prep(const __grid_
   {
     const int pr = 32 * (tid >> 6), r = (tid & 63) >> 2, c = 4 * (tid & 3);
     float y[4] = {}, x[4] = {};
-    block_row(y, 16, &s.T_[pr + 16 + r][pr], 1.0f, &s.T_[pr][pr + c], kPitch);
+    block_row(y, 16, 16, &s.T_[pr + 16 + r][pr], 1.0f, &s.T_[pr][pr + c], kPitch);
 #pragma unroll
     for (int e = 0; e < 4; ++e) s.tmp[r][(pr >> 1) + c + e] = y[e];
     __syncthreads();
-    block_row(x, 16, &s.T_[pr + 16 + r][pr + 16], -1.0f, &s.tmp[0][(pr >> 1) + c], 36);
+    block_row(x, 16, r, &s.T_[pr + 16 + r][pr + 16], -1.0f, &s.tmp[0][(pr >> 1) + c], 36);
 #pragma unroll
     for (int e = 0; e < 4; ++e) s.T_[pr + 16 + r][pr + c + e] = x[e];
   }
@@ -251,11 +254,11 @@ __global__ void __launch_bounds__(128, NP == 1 ? 5 : 2) delta_prep(const __grid_
   {
     const int r = tid >> 2, c = 8 * (tid & 3);
     float y[8] = {}, x[8] = {};
-    block_row(y, 32, &s.T_[32 + r][0], 1.0f, &s.T_[0][c], kPitch);
+    block_row(y, 32, 32, &s.T_[32 + r][0], 1.0f, &s.T_[0][c], kPitch);
 #pragma unroll
     for (int e = 0; e < 8; ++e) s.tmp[r][c + e] = y[e];
     __syncthreads();
-    block_row(x, 32, &s.T_[32 + r][32], -1.0f, &s.tmp[0][c], 36);
+    block_row(x, 32, r, &s.T_[32 + r][32], -1.0f, &s.tmp[0][c], 36);
 #pragma unroll
     for (int e = 0; e < 8; ++e) s.T_[32 + r][c + e] = x[e];
   }
@@ -265,6 +268,8 @@ __global__ void __launch_bounds__(128, NP == 1 ? 5 : 2) delta_prep(const __grid_
     const int r = e / (kC / 8), grp = e % (kC / 8);
     float x[8];
     load8<float>(s.T_[r], 8 * grp, kC, true, x);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = is_bad(x[i]) ? 0.0f : x[i];       // of a row whose X is not finite either, see is_bad
     put_pieces<3>(x, nullptr, p.timg + at * (3 * kTri), tile_off<kC>(r, grp), kTri);
   }
 }
@@ -283,6 +288,7 @@ template <typename T, int DKP, int PU, int PO>       // pieces of the operands u
 struct alignas(16) StripSmem {
   uint4 sf[DKP / 16][3][32], xf[4][3][32], lf[4][3][32], uf[4][PU][32], of[PO ? 4 : 1][PO ? PO : 1][PO ? 32 : 1];
   Strip<T> in, out;
+  int first[2][16];                       // by chunk parity: a channel's first position that is not finite, or kC
   int stop;                               // a wait gave up, as the strip's leader saw it between two barriers
 };
 template <int NP, int DKP, int PP, typename StripT, int NS, int KB>
@@ -488,6 +494,30 @@ __device__ __forceinline__ void store_cols(float* base, int w, int lane, const f
     *reinterpret_cast<float2*>(o + 8 * kC) = make_float2(c[j][2], c[j][3]);
   }
 }
+// See is_bad: values of the warp's column tiles, positions by column, channels by row.  What is not finite becomes 0 and is
+// noted in `first`, by channel.
+__device__ __forceinline__ void note_bad(float (&x)[2][4], int* first, int w, int lane) {
+  const float big = max3_abs(max3_abs(x[0][0], x[0][1], x[0][2]), max3_abs(x[0][3], x[1][0], x[1][1]), max3_abs(x[1][2], x[1][3], 0.0f));
+  if (!is_bad(big)) return;
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (is_bad(x[j][e])) {
+        atomicMin(first + (lane >> 2) + 8 * (e >> 1), 8 * col_tile(w, j) + 2 * (lane & 3) + (e & 1));
+        x[j][e] = 0.0f;
+      }
+}
+// NaN from a channel's first position that is not finite.
+__device__ __forceinline__ void set_from(float (&x)[2][4], const int* first, int w, int lane) {
+  const int f0 = first[lane >> 2], f1 = first[(lane >> 2) + 8];
+  if (min(f0, f1) >= kC) return;
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (8 * col_tile(w, j) + 2 * (lane & 3) + (e & 1) >= (e >> 1 ? f1 : f0)) x[j][e] = quiet_nan();
+}
 template <typename Smem>
 __device__ __forceinline__ void init_tiles(Smem& s, int strips) {
   if (threadIdx.x == 0) {
@@ -551,6 +581,7 @@ __global__ void __launch_bounds__(128 * NS + 32, kChainCtas<NP, DKP, NS>) delta_
   T* obase = static_cast<T*>(const_cast<void*>(p.o.ptr)) + b * p.o.sb + h * p.o.sh + d0;
   const bool vin = rows_aligned16(p.v, sizeof(T)), oout = rows_aligned16(p.o, sizeof(T));
   const bool leader = w == 0 && lane == 0;
+  if (w == 0) z.first[lane >> 4][lane & 15] = kC;
   z.in.fetch(vbase, p.v.sl, min(kC, p.L), cols, vin, w, lane);
   for (int ch = 0; ch < p.n; ++ch) {
     const int buf = ch % KB, rows = min(kC, p.L - ch * kC);
@@ -566,6 +597,8 @@ __global__ void __launch_bounds__(128 * NS + 32, kChainCtas<NP, DKP, NS>) delta_
       mbar_arrive(&s.empty[kTileK + (ch - 1) % KB]);
       mbar_arrive(&s.empty[kTileV + ((ch - 1) & 1)]);
     }
+    int* first = z.first[ch & 1];
+    if (w == 0 && lane < 16) z.first[(ch + 1) & 1][lane] = kC;
     float V[2][4], X[2][4], O[2][4], U[2][4];
     z.in.arrive();
     z.in.read(V, w, lane);
@@ -588,16 +621,23 @@ __global__ void __launch_bounds__(128 * NS + 32, kChainCtas<NP, DKP, NS>) delta_
         X[j][e] = (e & 1 ? be.y : be.x) * fmaf(-eg_, X[j][e], V[j][e]);
         O[j][e] *= p.scale * eg_;
       }
-      put_half<3>(z.xf, col_tile(w, j), X[j], lane);
     }
+    note_bad(X, first, w, lane);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) put_half<3>(z.xf, col_tile(w, j), X[j], lane);
     strip_sync(strip);                            // X is there; Q is done with
     if (leader) mbar_arrive(&s.empty[kTileQ]);
     chain_wait(s, &s.full[kTileT], ch & 1, p.err);
     tri_product<3, 3, 2, false>(U, z.xf, stt, w, lane);
-    if (SAVE) store_cols(p.us + ((head * p.n + ch) * p.dvp + d0) * kC, w, lane, U);
+    if (SAVE) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) put_half<PP>(z.uf, col_tile(w, j), U[j], lane);
+      set_from(U, first, w, lane);
+      store_cols(p.us + ((head * p.n + ch) * p.dvp + d0) * kC, w, lane, U);
+    }
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      put_half<PP>(z.uf, col_tile(w, j), U[j], lane);
+      if (!SAVE) put_half<PP>(z.uf, col_tile(w, j), U[j], lane);
       const float2 la = at_cols(vec + kC, col_tile(w, j), t);
 #pragma unroll
       for (int e = 0; e < 4; ++e) U[j][e] *= e & 1 ? la.y : la.x;
@@ -608,9 +648,18 @@ __global__ void __launch_bounds__(128 * NS + 32, kChainCtas<NP, DKP, NS>) delta_
     chain_wait(s, &s.full[kTileP], ch & 1, p.err);
     tri_product<PP, PP, PP - 1, false>(O, z.uf, sp, w, lane);
     state_add<NP, DKP>(S, vec[kC - 1], 1.0f, z.lf, sk, w, lane);
+    const int stop = *static_cast<volatile int*>(&z.stop), f0 = first[lane >> 2], f1 = first[(lane >> 2) + 8];
+    if (__any_sync(0xffffffffu, min(f0, f1) < kC)) {
+      set_from(O, first, w, lane);
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if ((e >> 1 ? f1 : f0) < kC) S[j][e] = quiet_nan();
+    }
     z.out.write(O, w, lane);
     z.out.flush(obase + t0 * p.o.sl, p.o.sl, rows, cols, oout, w, lane);
-    if (*static_cast<volatile int*>(&z.stop)) break;
+    if (stop) break;
   }
   if (p.last != nullptr) state_store(p.last + head * p.dkw * p.dvw, p.dkw, p.dvw, 8 * NT * w, d0, lane, S);
   chain_drain(s);

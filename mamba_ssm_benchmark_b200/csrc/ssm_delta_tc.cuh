@@ -123,6 +123,7 @@ struct alignas(1024) TcSmem {
   static constexpr int kRowUnits = NP == 1 ? 4 : 2;      // 16-byte units of a row that pass at a time
   TcStage<NP, DKP, PP> stage[2];
   float4 rows[16][32 * kRowUnits];                       // per warp, see tc_store_rows
+  int first[2][128];             // by chunk parity: a channel's first position that is not finite, or kC
   uint64_t full[2];              // a stage's tiles are there
   uint64_t ready[3], done[3];    // operands of a round are in tensor memory; its products are finished
   uint32_t tmem;
@@ -267,6 +268,25 @@ __device__ __forceinline__ void tc_each(const float* vec, F f) {
   }
 }
 
+// See is_bad: 16 positions from c0 of a channel.  What is not finite becomes 0, the first one is noted.
+__device__ __forceinline__ void tc_note_bad(float (&x)[16], int* first, int c0) {
+  float big = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 16; i += 2) big = max3_abs(big, x[i], x[i + 1]);
+  if (!is_bad(big)) return;
+#pragma unroll
+  for (int i = 15; i >= 0; --i)
+    if (is_bad(x[i])) {
+      atomicMin(first, c0 + i);
+      x[i] = 0.0f;
+    }
+}
+__device__ __forceinline__ void tc_set_from(float (&x)[16], int first, int c0) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+    if (c0 + i >= first) x[i] = quiet_nan();
+}
+
 // ---- forward ------------------------------------------------------------------------------------
 template <typename T, int NP, int DKP, bool SAVE>
 __global__ void __launch_bounds__(kTcThreads, 1) delta_fwd_tc(const __grid_constant__ DeltaParams p) {
@@ -319,7 +339,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) delta_fwd_tc(const __grid_const
       S[i / 16][i % 16] = h0 != nullptr && live && k < p.dkw ? h0[(size_t)k * p.dvw] : 0.0f;
     }
     const int c0 = 16 * quarter;
+    if (quarter == 0) s.first[0][row] = kC;        // the others read and write it behind the first round of products
     for (int ch = 0; ch < p.n; ++ch) {
+      int* first = &s.first[ch & 1][row];
       const int st = ch & 1, par = ch & 1, rows = min(kC, p.L - ch * kC);
       const float* vec = s.stage[st].vec;
       const long long t0 = (long long)ch * kC + c0;
@@ -341,13 +363,17 @@ __global__ void __launch_bounds__(kTcThreads, 1) delta_fwd_tc(const __grid_const
       tc_load_f32(my + kTcD + c0, x);
       tc_each(vec + c0, [&](int i, float eg) { x[i] = fmaf(-eg, x[i], to_f32(vr[i])); });
       tc_each(vec + 2 * kC + c0, [&](int i, float be) { x[i] *= be; });
+      if (quarter == 0) s.first[(ch + 1) & 1][row] = kC;       // whose readers of the chunk before are done
+      tc_note_bad(x, first, c0);
       tc_put<3>(my + kTcX + c0 / 2, kC / 2, x);
       tc_ready(&s.ready[1]);
       save(QK / 16 - 1);
       wait(&s.done[1], par);
       tc_fence_after();
       tc_load_f32(my + kTcD + c0, x);
+      const int bad = *first;
       tc_put<PP>(my + kTcU + c0 / 2, kC / 2, x);
+      if (bad < kC) tc_set_from(x, bad, c0);
       float y[16];
       tc_each(vec + kC + c0, [&](int i, float la) { y[i] = x[i] * la; });
       tc_put<3>(my + kTcLU + c0 / 2, kC / 2, y);
@@ -366,6 +392,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) delta_fwd_tc(const __grid_const
       tc_load_f32(my + kTcO + c0, y);
       tc_load_f32(my + kTcX + c0, x);
       tc_each(vec + c0, [&](int i, float eg) { x[i] = fmaf(p.scale * eg, y[i], x[i]); });
+      if (bad < kC) tc_set_from(x, bad, c0);
       tc_store_col(ob + t0 * p.o.sl, p.o.sl, rows - c0, live, x);
     }
     if (p.last != nullptr && live) {

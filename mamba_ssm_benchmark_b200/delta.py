@@ -69,7 +69,8 @@ def gated_delta_rule(q, k, v, g, beta, h0=None, scale=None):
     q, k: (B, L, Hk, dk); v: (B, L, Hv, dv), Hv a multiple of Hk (key head h // (Hv // Hk) serves value
     head h); g: (B, L, Hv), the log of the decay (at most 0; -inf resets the state); beta: (B, L, Hv), the
     step of the correction; h0: (B, Hv, dk, dv) or None (zeros); scale: of o, default dk ** -0.5.
-    Any strides.  Differentiable with respect to all six tensors."""
+    Any strides.  Differentiable once with respect to all six tensors.  A value that is not finite reaches no
+    output before its position; gradients are defined for finite inputs."""
     _check(q, k, v, g, beta, h0, "h0", 4)
     scale = float(q.shape[-1] ** -0.5 if scale is None else scale)
     out_dtype, ct = v.dtype, _common_dtype(q, k, v)
