@@ -341,7 +341,8 @@ SSM_API int ssm_conv1d_bwd(int64_t B, int64_t L, int64_t D, int64_t K, ssm_view 
  * needs no workspace): the chunks' tiles, the state entering every 64 positions, the corrected values.
  * ssm_gated_delta_bwd: gradients from d_o (like o, any strides) and dlast (NULL = zeros): d_q, d_k
  * (summed over the value heads of a key head), d_v in the inputs' dtype; d_g, d_beta (B, L, Hv)
- * dense float32; dh0 may be NULL.  Every sum has a fixed order: results are reproducible.
+ * dense float32; dh0 may be NULL.  Every sum has a fixed order: results are reproducible.  h0 may change
+ * before the backward.  A value that is not finite reaches no output before its position.
  * workspace: ssm_gated_delta_workspace_size bytes (backward = 0 / 1).
  * ------------------------------------------------------------------------------- */
 typedef struct {

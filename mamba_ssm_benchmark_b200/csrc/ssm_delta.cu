@@ -29,7 +29,7 @@ constexpr int kPitch = kC + 4;
 // ================================================================================================
 // Chunk preparation: one CTA of four warps per (chunk, value head, batch).  Short dependent steps (sums of g, two
 // products, a triangular inverse) bound it, so CTAs are small, 33 KB of shared memory in bf16, five to an SM.
-// 5120 chunks of 64 x 128 (bf16): 140 us; in 90 KB, with rows loaded through registers: 252 us.
+// 5120 chunks of 64 x 128 (bf16): 130 us; in 90 KB, with rows loaded through registers: 252 us.
 // ================================================================================================
 template <int NP, int DKP>
 struct alignas(128) PrepSmem {
@@ -533,7 +533,9 @@ __device__ __forceinline__ void init_tiles(Smem& s, int strips) {
 
 template <typename T, int NP, int DKP, int NS>
 struct FwdChain {
-  static constexpr int PP = NP == 1 ? 2 : 3;      // pieces of P and of its U: a bf16 o keeps 16 bits
+  // Pieces of P and of its U (and index sums of Q S): a bf16 o is kept to 16 bits before it is rounded to 8.  One value in 400
+  // then rounds the other way than from 24 bits; o's error against 64 bits is that rounding's, 1.659e-3, either way.
+  static constexpr int PP = NP == 1 ? 2 : 3;
   using StripT = StripSmem<T, DKP, PP, 0>;
   template <int KB>
   using Smem = ChainSmem<NP, DKP, PP, StripT, NS, KB>;
@@ -772,7 +774,7 @@ __global__ void __launch_bounds__(128 * NS + 32, kChainCtas<NP, DKP, NS>) delta_
 
 // dq, dk (B, L, Hk, dk): the value heads' parts, (B, L, Hv, DKP) fp32, summed in head order.  A thread takes four
 // channels of one position and key head (blockIdx.x walks positions, blockIdx.y key heads).  Memory bounds it: 8192
-// positions x 40 heads of 128 in 68 us, 6.2 TB/s.
+// positions x 40 heads of 128 in 72 us, 5.8 TB/s.
 template <typename T, int DKP>
 __global__ void __launch_bounds__(256) delta_sum_heads(const __grid_constant__ DeltaParams p) {
   constexpr int kPer = 256 / (DKP / 4);              // positions per CTA

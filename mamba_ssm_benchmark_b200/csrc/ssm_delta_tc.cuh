@@ -12,9 +12,9 @@
 //   forward   S -> [K S, Q S] -> X -> [T X] -> U -> [P U, K^T U]
 //   backward  dS' -> [K dS', P^T dO] -> Y -> [T^T Y] -> dX -> [Q^T dO, K^T dX]
 //
-// 80 heads of 128 x 128, 4096 positions, bf16, training: 452 us forward (14 thousand clocks a chunk) and 472 us
+// 80 heads of 128 x 128, 4096 positions, bf16, training: 452 us forward (14 thousand clocks a chunk) and 463 us
 // backward; the strips take 856 and 1146, and with half the threads these kernels 456 and 562 (fp32, dk 64: 67 and 77
-// instead of 62 and 67).  The rounds' products take 2.4, 1.7 and 1.8 thousand clocks, about 53 an instruction whatever
+// instead of 60 and 63).  The rounds' products take 2.4, 1.7 and 1.8 thousand clocks, about 53 an instruction whatever
 // its N up to 64; the register passes and the saved states' stores take the rest.
 #pragma once
 
