@@ -268,8 +268,13 @@ __global__ void __launch_bounds__(128, NP == 1 ? 5 : 2) delta_prep(const __grid_
     const int r = e / (kC / 8), grp = e % (kC / 8);
     float x[8];
     load8<float>(s.T_[r], 8 * grp, kC, true, x);
+    bool bad = false;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = is_bad(x[i]) ? 0.0f : x[i];       // of a row whose X is not finite either, see is_bad
+    for (int i = 0; i < 8; ++i) {
+      bad |= is_bad(x[i]);
+      x[i] = is_bad(x[i]) ? 0.0f : x[i];
+    }
+    if (bad) p.vec[at * kVec + 2 * kC + r] = quiet_nan();      // its X then is not finite and says so, see is_bad
     put_pieces<3>(x, nullptr, p.timg + at * (3 * kTri), tile_off<kC>(r, grp), kTri);
   }
 }

@@ -52,3 +52,26 @@ def test_outputs_before_a_non_finite_input(shape, dtype, channels, name, value, 
         later, state = later[:1], later[:1]
     assert not torch.isfinite(later).any() and not torch.isfinite(state).any()
     assert nat.read_device_error() == 0
+
+
+@pytest.mark.parametrize("shape,dtype,channels", FORMS)
+def test_divergence_is_not_hidden(shape, dtype, channels):
+    """Keys far longer than 1: the state grows by a factor of up to beta |k|^2 a position and overflows, in the triangular
+    inverse first.  Once the recurrence (in float64) is beyond float32's range, outputs are not finite, and never something
+    finite instead.  (Up to 15 outputs in front of an overflow inside a chunk may go with it.)"""
+    t, *_ = _inputs(*shape, dtype=dtype, h0=False, seed=sum(shape))
+    t["k"] = t["k"] * 100
+    t["g"], t["beta"] = torch.zeros_like(t["g"]), torch.ones_like(t["beta"])
+    t = {n: x if x is None else x[:1].to(DEV).expand(shape[0], *x.shape[1:]).contiguous() for n, x in t.items()}
+    with torch.no_grad():
+        o, last = gated_delta_rule(**t)
+        S = torch.zeros(shape[3], shape[4], shape[5], dtype=torch.float64, device=DEV)
+        group, size = shape[3] // shape[2], []
+        for i in range(shape[1]):
+            k = t["k"][0, i].double().repeat_interleave(group, 0)
+            S = S + k[..., None] * (t["v"][0, i].double() - (S * k[..., None]).sum(1))[:, None]
+            size.append(S.abs().amax(1).amin())              # of the smallest channel
+    size = torch.stack(size)
+    over = ~(size <= 1e42)                                   # float64 overflows too
+    assert int(over.sum()) > 20
+    assert not torch.isfinite(o[:, over]).any() and not torch.isfinite(last).any()
