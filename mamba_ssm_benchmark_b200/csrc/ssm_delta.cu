@@ -222,14 +222,12 @@ __global__ void __launch_bounds__(128, NP == 1 ? 5 : 2) delta_prep(const __grid_
     }
   }
   __syncthreads();
-  // y[0 .. W) of a row of F = (A or T block)[row][m] x G[m][c ..], m < M; of T's rows (`upto` their number) only up to the
-  // diagonal: behind it stand zeros, which would make NaN of a later position's values that are not finite
-  auto block_row = [&](auto& y, int M, int upto, const float* frow, float sign, const float* grow, int pitch) {
+  // y[0 .. W) of a row of F = (A or T block)[row][m] x G[m][c ..], m < M
+  auto block_row = [&](auto& y, int M, const float* frow, float sign, const float* grow, int pitch) {
     constexpr int W = sizeof(y) / sizeof(float);
 #pragma unroll 8
     for (int m = 0; m < M; ++m) {
       const float a = sign * frow[m];
-      if (m > upto) continue;
 #pragma unroll
       for (int e = 0; e < W; e += 4) {
         float x[4];
@@ -239,14 +237,25 @@ __global__ void __launch_bounds__(128, NP == 1 ? 5 : 2) delta_prep(const __grid_
       }
     }
   };
+  // What is not finite becomes 0, and row r's X NaN (see is_bad): the next product has zeros beside it, above T's diagonal.
+  auto finite = [&](auto& y, int r) {
+    constexpr int W = sizeof(y) / sizeof(float);
+    float big = max3_abs(y[0], y[1], max3_abs(y[2], y[3], 0.0f));
+    if constexpr (W == 8) big = max3_abs(big, max3_abs(y[4], y[5], 0.0f), max3_abs(y[6], y[7], 0.0f));
+    if (!is_bad(big)) return;
+    p.vec[at * kVec + 2 * kC + r] = quiet_nan();
+#pragma unroll
+    for (int e = 0; e < W; ++e) y[e] = is_bad(y[e]) ? 0.0f : y[e];
+  };
   {
     const int pr = 32 * (tid >> 6), r = (tid & 63) >> 2, c = 4 * (tid & 3);
     float y[4] = {}, x[4] = {};
-    block_row(y, 16, 16, &s.T_[pr + 16 + r][pr], 1.0f, &s.T_[pr][pr + c], kPitch);
+    block_row(y, 16, &s.T_[pr + 16 + r][pr], 1.0f, &s.T_[pr][pr + c], kPitch);
+    finite(y, pr + 16 + r);
 #pragma unroll
     for (int e = 0; e < 4; ++e) s.tmp[r][(pr >> 1) + c + e] = y[e];
     __syncthreads();
-    block_row(x, 16, r, &s.T_[pr + 16 + r][pr + 16], -1.0f, &s.tmp[0][(pr >> 1) + c], 36);
+    block_row(x, 16, &s.T_[pr + 16 + r][pr + 16], -1.0f, &s.tmp[0][(pr >> 1) + c], 36);
 #pragma unroll
     for (int e = 0; e < 4; ++e) s.T_[pr + 16 + r][pr + c + e] = x[e];
   }
@@ -254,11 +263,12 @@ __global__ void __launch_bounds__(128, NP == 1 ? 5 : 2) delta_prep(const __grid_
   {
     const int r = tid >> 2, c = 8 * (tid & 3);
     float y[8] = {}, x[8] = {};
-    block_row(y, 32, 32, &s.T_[32 + r][0], 1.0f, &s.T_[0][c], kPitch);
+    block_row(y, 32, &s.T_[32 + r][0], 1.0f, &s.T_[0][c], kPitch);
+    finite(y, 32 + r);
 #pragma unroll
     for (int e = 0; e < 8; ++e) s.tmp[r][c + e] = y[e];
     __syncthreads();
-    block_row(x, 32, r, &s.T_[32 + r][32], -1.0f, &s.tmp[0][c], 36);
+    block_row(x, 32, &s.T_[32 + r][32], -1.0f, &s.tmp[0][c], 36);
 #pragma unroll
     for (int e = 0; e < 8; ++e) s.T_[32 + r][c + e] = x[e];
   }
@@ -268,13 +278,7 @@ __global__ void __launch_bounds__(128, NP == 1 ? 5 : 2) delta_prep(const __grid_
     const int r = e / (kC / 8), grp = e % (kC / 8);
     float x[8];
     load8<float>(s.T_[r], 8 * grp, kC, true, x);
-    bool bad = false;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      bad |= is_bad(x[i]);
-      x[i] = is_bad(x[i]) ? 0.0f : x[i];
-    }
-    if (bad) p.vec[at * kVec + 2 * kC + r] = quiet_nan();      // its X then is not finite and says so, see is_bad
+    finite(x, r);
     put_pieces<3>(x, nullptr, p.timg + at * (3 * kTri), tile_off<kC>(r, grp), kTri);
   }
 }
@@ -460,7 +464,7 @@ __device__ __forceinline__ void tri_product(float (&d)[2][4], const uint4 (*f)[N
 // formed on its own and added once, rounded to nearest: a state that the tensor cores accumulated over
 // hundreds of chunks, truncating each time, would drift.
 template <int NP, int DKP>
-__device__ __forceinline__ void state_add(float (&S)[DKP / 32][4], float decay, float sign, const uint4 (*f)[3][32],
+__device__ __forceinline__ void state_add(float (&S)[DKP / 32][4], float2 decay, float sign, const uint4 (*f)[3][32],
                                           uint32_t tile, int w, int lane) {
   constexpr int NT = DKP / 32;
   float d[NT][4], low[NT][4];
@@ -482,7 +486,7 @@ __device__ __forceinline__ void state_add(float (&S)[DKP / 32][4], float decay, 
 #pragma unroll
   for (int j = 0; j < NT; ++j)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) S[j][e] = fmaf(decay, S[j][e], sign * (d[j][e] + low[j][e]));
+    for (int e = 0; e < 4; ++e) S[j][e] = fmaf(e >> 1 ? decay.y : decay.x, S[j][e], sign * (d[j][e] + low[j][e]));
 }
 
 // The per-position factors of the columns 2 t, 2 t + 1 of a column tile.
@@ -651,19 +655,17 @@ __global__ void __launch_bounds__(128 * NS + 32, kChainCtas<NP, DKP, NS>) delta_
       put_half<3>(z.lf, col_tile(w, j), U[j], lane);
     }
     strip_sync(strip);                            // U is there; T is done with
+    const int f0 = first[lane >> 2], f1 = first[(lane >> 2) + 8];
     if (leader) mbar_arrive(&s.empty[kTileT]);
     chain_wait(s, &s.full[kTileP], ch & 1, p.err);
     tri_product<PP, PP, PP - 1, false>(O, z.uf, sp, w, lane);
-    state_add<NP, DKP>(S, vec[kC - 1], 1.0f, z.lf, sk, w, lane);
-    const int stop = *static_cast<volatile int*>(&z.stop), f0 = first[lane >> 2], f1 = first[(lane >> 2) + 8];
-    if (__any_sync(0xffffffffu, min(f0, f1) < kC)) {
-      set_from(O, first, w, lane);
+    state_add<NP, DKP>(S, make_float2(f0 < kC ? quiet_nan() : vec[kC - 1], f1 < kC ? quiet_nan() : vec[kC - 1]), 1.0f, z.lf, sk, w, lane);
+    const int stop = *static_cast<volatile int*>(&z.stop);
 #pragma unroll
-      for (int j = 0; j < NT; ++j)
+    for (int j = 0; j < 2; ++j)
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if ((e >> 1 ? f1 : f0) < kC) S[j][e] = quiet_nan();
-    }
+      for (int e = 0; e < 4; ++e)
+        O[j][e] = 8 * col_tile(w, j) + 2 * t + (e & 1) >= (e >> 1 ? f1 : f0) ? quiet_nan() : O[j][e];
     z.out.write(O, w, lane);
     z.out.flush(obase + t0 * p.o.sl, p.o.sl, rows, cols, oout, w, lane);
     if (stop) break;
@@ -747,7 +749,7 @@ __global__ void __launch_bounds__(128 * NS + 32, kChainCtas<NP, DKP, NS>) delta_
 #pragma unroll
     for (int j = 0; j < 2; ++j) put_half<3>(z.xf, col_tile(w, j), Y[j], lane);
     chain_wait(s, &s.full[kTileQ], it & 1, p.err);
-    state_add<NP, DKP>(S, vec[kC - 1], 1.0f, z.uf, sq, w, lane);
+    state_add<NP, DKP>(S, make_float2(vec[kC - 1], vec[kC - 1]), 1.0f, z.uf, sq, w, lane);
     strip_sync(strip);                            // Y is there; P and Q are done with
     if (leader) {
       mbar_arrive(&s.empty[kTileQ]);
@@ -768,10 +770,11 @@ __global__ void __launch_bounds__(128 * NS + 32, kChainCtas<NP, DKP, NS>) delta_
     }
     strip_sync(strip);                            // dX is there; T is done with
     if (leader) mbar_arrive(&s.empty[kTileT]);
-    state_add<NP, DKP>(S, 1.0f, -1.0f, z.lf, sk, w, lane);
+    state_add<NP, DKP>(S, make_float2(1.0f, 1.0f), -1.0f, z.lf, sk, w, lane);
+    const int stop = *static_cast<volatile int*>(&z.stop);
     z.out.write(Y, w, lane);
     z.out.flush(obase + t0 * p.dv.sl, p.dv.sl, rows, cols, oout, w, lane);
-    if (*static_cast<volatile int*>(&z.stop)) break;
+    if (stop) break;
   }
   if (p.last != nullptr) state_store(p.last + head * p.dkw * p.dvw, p.dkw, p.dvw, 8 * NT * w, d0, lane, S);
   chain_drain(s);
@@ -1059,8 +1062,9 @@ cudaError_t run_chain_tc(const Shape& s, const DeltaParams& p, bool bwd, cudaStr
 //   one strip             41 / 48          46 / 54 (up to 148: 40 / 43)   43 / 50
 //   two strips            60 / 69          47 / 55                        64 / 68
 //   tcgen05, 128 rows     112 / 121        84 / 99                        115 / 122
-// By these, the slowest of 198 choices is 11 % behind the best of the three measured, eleven are over 6 %.  Two strips never pay in
-// bf16 at dk 64; fp32 keys above 64 channels leave shared memory for one strip only.
+// Heads with an odd number of strips give CTAs of two and of one: about the work's share of 148 SMs and half a pair more, unless
+// all run at once.  By this, the slowest of 198 choices is 11 % behind the best of the three measured, eight are over 6 %.  Two
+// strips never pay in bf16 at dk 64; fp32 keys above 64 channels leave shared memory for one strip only.
 // Returns the value channels that a CTA takes: 16 or 32 (strips), 128 (tcgen05).
 int chain_rows(const Shape& s, bool bwd) {
   const bool wide = s.dkp() == 128, f32 = s.np() == 3;
@@ -1076,7 +1080,10 @@ int chain_rows(const Shape& s, bool bwd) {
   }
   const double strip = wide ? (bwd ? 48 : 41) : (bwd ? 50 : 43), pair = wide ? (bwd ? 69 : 60) : (bwd ? 68 : 64);
   const double one = waves(strips) * strip;
-  const double two = waves(pairs) * ((double)(strips / 2) * pair + (double)(strips % 2) * strip) / (double)pairs;
+  double two = waves(pairs) * pair;
+  if (strips == 1) two = one;
+  else if (strips % 2 != 0 && heads * pairs > 148)
+    two = (double)heads * ((double)(strips / 2) * pair + strip) / 148.0 + 0.5 * pair;
   if (tc < one && tc < two) return 128;
   return two < one ? 32 : 16;
 }

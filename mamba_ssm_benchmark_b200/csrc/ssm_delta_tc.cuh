@@ -373,7 +373,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) delta_fwd_tc(const __grid_const
       tc_load_f32(my + kTcD + c0, x);
       const int bad = *first;
       tc_put<PP>(my + kTcU + c0 / 2, kC / 2, x);
-      if (bad < kC) tc_set_from(x, bad, c0);
+      tc_set_from(x, bad, c0);
       float y[16];
       tc_each(vec + kC + c0, [&](int i, float la) { y[i] = x[i] * la; });
       tc_put<3>(my + kTcLU + c0 / 2, kC / 2, y);

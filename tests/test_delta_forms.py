@@ -37,6 +37,7 @@ def test_choice(shape, dtype, channels):
 @pytest.mark.parametrize("heads,dk,dv,dtype,channels", [
     (385, 128, 48, BF16, (32, 32)), (200, 64, 48, BF16, (16, 16)), (385, 64, 48, BF16, (16, 16)), (100, 128, 48, BF16, (32, 32)),
     (200, 64, 48, F32, (32, 32)), (148, 128, 128, BF16, (128, 128)), (50, 64, 128, BF16, (128, 16)),
+    (128, 128, 48, BF16, (128, 128)), (128, 64, 48, F32, (128, 128)), (4, 128, 48, BF16, (16, 16)),
 ])
 def test_choice_is_the_fastest_measured(heads, dk, dv, dtype, channels):
     """Shapes at which another choice took at least 8 % more for 1024 positions."""
