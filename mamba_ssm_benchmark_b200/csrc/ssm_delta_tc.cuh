@@ -12,7 +12,7 @@
 //   forward   S -> [K S, Q S] -> X -> [T X] -> U -> [P U, K^T U]
 //   backward  dS' -> [K dS', P^T dO] -> Y -> [T^T Y] -> dX -> [Q^T dO, K^T dX]
 //
-// 80 heads of 128 x 128, 4096 positions, bf16, training: 452 us forward (14 thousand clocks a chunk) and 463 us
+// 80 heads of 128 x 128, 4096 positions, bf16, training: 439 us forward (14 thousand clocks a chunk) and 463 us
 // backward; the strips take 856 and 1146, and with half the threads these kernels 456 and 562 (fp32, dk 64: 67 and 77
 // instead of 60 and 63).  The rounds' products take 2.4, 1.7 and 1.8 thousand clocks, about 53 an instruction whatever
 // its N up to 64; the register passes and the saved states' stores take the rest.
@@ -373,7 +373,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) delta_fwd_tc(const __grid_const
       tc_load_f32(my + kTcD + c0, x);
       const int bad = *first;
       tc_put<PP>(my + kTcU + c0 / 2, kC / 2, x);
-      tc_set_from(x, bad, c0);
+      // Without the branch where dk is 128 and states are saved (wide training 455 -> 439 us), with it elsewhere (128 heads of
+      // 64 x 128: 176 -> 170, inference of 128 x 128: 193 -> 185): the schedules differ.
+      if ((SAVE && DKP == 128) || bad < kC) tc_set_from(x, bad, c0);
       float y[16];
       tc_each(vec + kC + c0, [&](int i, float la) { y[i] = x[i] * la; });
       tc_put<3>(my + kTcLU + c0 / 2, kC / 2, y);
