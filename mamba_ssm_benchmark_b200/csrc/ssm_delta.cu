@@ -29,7 +29,7 @@ constexpr int kPitch = kC + 4;
 // ================================================================================================
 // Chunk preparation: one CTA of four warps per (chunk, value head, batch).  Short dependent steps (sums of g, two
 // products, a triangular inverse) bound it, so CTAs are small, 33 KB of shared memory in bf16, five to an SM.
-// 5120 chunks of 64 x 128 (bf16): 130 us; in 90 KB, with rows loaded through registers: 252 us.
+// 5120 chunks of 64 x 128 (bf16): 135 us; in 90 KB, with rows loaded through registers: 252 us.
 // ================================================================================================
 template <int NP, int DKP>
 struct alignas(128) PrepSmem {
@@ -1063,7 +1063,7 @@ cudaError_t run_chain_tc(const Shape& s, const DeltaParams& p, bool bwd, cudaStr
 //   two strips            60 / 69          47 / 55                        64 / 68
 //   tcgen05, 128 rows     112 / 121        84 / 99                        115 / 122
 // Heads with an odd number of strips give CTAs of two and of one: about the work's share of 148 SMs and half a pair more, unless
-// all run at once.  By this, the slowest of 198 choices is 11 % behind the best of the three measured, eight are over 6 %.  Two
+// all run at once.  By this, the slowest of 198 choices is 8 % behind the best of the three measured, six are over 6 %.  Two
 // strips never pay in bf16 at dk 64; fp32 keys above 64 channels leave shared memory for one strip only.
 // Returns the value channels that a CTA takes: 16 or 32 (strips), 128 (tcgen05).
 int chain_rows(const Shape& s, bool bwd) {

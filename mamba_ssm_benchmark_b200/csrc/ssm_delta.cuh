@@ -378,8 +378,8 @@ struct Wait {
 // 0 for such values of X and T, a channel's first such position is noted, and at the end of the chunk its outputs from
 // there on and its state become NaN: as the recurrence has them, since a state that once is not finite stays so.  A row of
 // T with such values, which may come of an overflow as well, makes its X NaN.  Above kBig a float rounds to an infinite bf16
-// piece.  On the strips all this is selects and no branch behind X (long prompt 655 us, with branches at the products 683,
-// without any of it 657).
+// piece.  On the strips all this is selects and no branch behind X (long prompt 650 us, with branches at the products 683,
+// without any of it 655).
 constexpr float kBig = 3.3895313e38f;            // the largest bf16
 __device__ __forceinline__ float max3_abs(float a, float b, float c) {       // NaN if one of them is
   float r;
