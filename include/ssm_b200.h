@@ -37,7 +37,7 @@
 extern "C" {
 #endif
 
-#define SSM_B200_ABI_VERSION 7
+#define SSM_B200_ABI_VERSION 8
 
 #if defined(__GNUC__)
 #define SSM_API __attribute__((visibility("default")))
@@ -399,12 +399,65 @@ SSM_API int ssm_group_norm_bwd(int64_t samples, int64_t positions, int64_t C, in
                        const float* stats, ssm_view dy, ssm_view dx, float* dweight, float* dbias, ssm_view dz,
                        void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---------------------------------------------------------------------------------
+ * Around the mixers of a language model.  No counterparts in the reference, whose LM calls torch.  Tensors of rows are
+ * ssm_views whose batch_stride is the row's stride (row_stride is ignored).
+ *
+ * Embedding: y[t] = scale weight[idx[t]]; weight (V, C) and y (T, C) in one dtype, SSM_F32 or SSM_BF16; idx T dense ids of
+ * idx_bytes 4 or 8.  Backward: dweight[v] = scale sum of dy[t] over the t with idx[t] = v, every row written, sums in
+ * fp32 and above in a fixed order.  An id outside 0 .. V-1 gives a row of NaN and no gradient, and sets bit 1 (value 2)
+ * of the device error word.  workspace: ssm_embedding_bwd_workspace_size bytes.
+ * ------------------------------------------------------------------------------- */
+SSM_API int ssm_embedding_fwd(int64_t T, int64_t V, int64_t C, const void* idx, int32_t idx_bytes, ssm_view weight,
+                      float scale, ssm_view y, void* stream);
+SSM_API int ssm_embedding_bwd_workspace_size(int64_t T, int64_t V, int64_t C, size_t* bytes);
+SSM_API int ssm_embedding_bwd(int64_t T, int64_t V, int64_t C, const void* idx, int32_t idx_bytes, float scale, ssm_view dy,
+                      ssm_view dweight, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Root-mean-square norm with a residual:
+ *   total = x + residual,   y = total / sqrt(mean(total^2) + eps) * weight        over a row's C values
+ * x and y in one dtype, SSM_F32 or SSM_BF16; residual (ptr NULL: none) and total SSM_F32 or x's dtype; what is normed is
+ * total as it is kept.  weight: (C) in SSM_F32 or SSM_BF16 (weight_dtype), or NULL (1).
+ * ssm_rms_norm_fp8: y in 8 bits (e4m3): y8 = round(y / scale), scale[row] = max(max |y|, 1e-30) / 448; norm == 0: y = total.
+ * Backward, from total (x where there was no residual), dy and dtotal (ptr NULL: zeros): dx in dy's dtype, dresidual (the
+ * same values in total's dtype, ptr NULL: not wanted) and dweight in weight_dtype (or NULL), summed in a fixed order.
+ * workspace: ssm_rms_norm_bwd_workspace_size bytes. */
+SSM_API int ssm_rms_norm_fwd(int64_t rows, int64_t C, ssm_view x, ssm_view residual, const void* weight,
+                     int32_t weight_dtype, float eps, ssm_view y, ssm_view total, void* stream);
+SSM_API int ssm_rms_norm_fp8(int64_t rows, int64_t C, ssm_view x, ssm_view residual, const void* weight,
+                     int32_t weight_dtype, float eps, int32_t norm, void* y8, int64_t y8_stride, float* scale, ssm_view total,
+                     void* stream);
+SSM_API int ssm_rms_norm_bwd_workspace_size(int64_t rows, int64_t C, size_t* bytes);
+SSM_API int ssm_rms_norm_bwd(int64_t rows, int64_t C, ssm_view total, const void* weight, int32_t weight_dtype, float eps,
+                     ssm_view dy, ssm_view dtotal, ssm_view dx, ssm_view dresidual, void* dweight, void* workspace,
+                     size_t workspace_bytes, void* stream);
+
+/* Product of 8-bit rows:  y[m, n] = act(x_scale[m] w_scale[n] sum_k x8[m, k] w8[n, k] + bias[n]) + residual[m, n]
+ * x8 (tokens, K), w8 (channels, K): e4m3, rows of any length that start at multiples of 16 bytes; scales dense float32 by row;
+ * bias (channels) float32 or NULL; silu != 0: act = SiLU, else the identity; residual (ptr NULL: none) in y's dtype,
+ * SSM_F32 or SSM_BF16; y may be the residual itself.  Sums are fp32. */
+SSM_API int ssm_linear_fp8(int64_t tokens, int64_t channels, int64_t K, const void* x8, int64_t x_stride,
+                   const float* x_scale, const void* w8, int64_t w_stride, const float* w_scale, const float* bias,
+                   int32_t silu, ssm_view residual, ssm_view y, void* stream);
+
+/* The next token of every row of logits (B, V), SSM_F32 or SSM_BF16, V at most 2^20, from uniforms (B) in [0, 1).  Of
+ * w = exp((l - max) / temperature): the top_k largest are kept (0 or less: all); of these, largest first, as many as it takes
+ * to reach top_p of their sum (1 or more: all; at least one); of these what is at least min_p (0: all).  The token is the
+ * first, by index, where the running sum of the kept weights passes uniforms[b] times their sum.  Equal logits rank by
+ * index, the lowest first.  temperature <= 0: the largest logit.  A row without a logit above -inf, with a NaN or with a
+ * NaN temperature gives -1.  Settings by row (dense, B values) or, where that pointer is NULL, one value for all.
+ * Sums are whole numbers in units of 2^-42 of the largest weight: the token does not depend on how the row is split. */
+SSM_API int ssm_sample_tokens(int64_t B, int64_t V, ssm_view logits, const float* uniforms, const double* temperature,
+                      double temperature0, const int64_t* top_k, int64_t top_k0, const double* top_p, double top_p0,
+                      const double* min_p, double min_p0, int64_t* tokens, void* stream);
+
 /* ABI version of the loaded library (SSM_B200_ABI_VERSION). */
 SSM_API int ssm_abi_version(void);
 /* Message for the most recent non-OK status returned on this thread. */
 SSM_API const char* ssm_last_error_message(void);
 /* Reads and clears the device-side error word of the current device: nonzero when a
- * kernel gave up on a bounded wait (a TMA copy that never landed).  Synchronises
+ * kernel gave up on a bounded wait (bit 0: a TMA copy that never landed) or met an id
+ * outside its table (bit 1: ssm_embedding_fwd).  Synchronises
  * the device; intended for tests and debugging, not for the hot path. */
 SSM_API int ssm_read_device_error(int32_t* flags);
 

@@ -19,7 +19,7 @@ SSM_OK, SSM_ERR_INVALID, SSM_ERR_DTYPE, SSM_ERR_WORKSPACE, SSM_ERR_CUDA, SSM_ERR
 SSM_F32, SSM_BF16 = 0, 1
 METHODS = {"zoh": 0, "euler": 1, "bilinear": 2}
 DTYPES = {torch.float32: SSM_F32, torch.bfloat16: SSM_BF16}
-ABI_VERSION = 7
+ABI_VERSION = 8
 
 # Every symbol include/ssm_b200.h declares (checked by the tests).
 EXPORTED = (
@@ -31,6 +31,8 @@ EXPORTED = (
     "ssm_scan_bwd_plan", "ssm_compose_shards",
     "ssm_gated_delta_workspace_size", "ssm_gated_delta_saved_size", "ssm_gated_delta_plan", "ssm_gated_delta_fwd",
     "ssm_gated_delta_bwd", "ssm_gated_delta_state_update", "ssm_group_norm_workspace_size", "ssm_group_norm_fwd", "ssm_group_norm_bwd",
+    "ssm_embedding_fwd", "ssm_embedding_bwd_workspace_size", "ssm_embedding_bwd", "ssm_rms_norm_fwd", "ssm_rms_norm_fp8",
+    "ssm_rms_norm_bwd_workspace_size", "ssm_rms_norm_bwd", "ssm_linear_fp8", "ssm_sample_tokens",
 )
 
 
@@ -103,6 +105,19 @@ _SIGNATURES.update({
     "ssm_group_norm_fwd": (ctypes.c_int, [_I64] * 4 + [_V, _P, _P, _F, _I32, _I32, _V, _V, _P, _P, _SZ, _P]),
     "ssm_group_norm_bwd": (ctypes.c_int, [_I64] * 4 + [_V, _P, _P, _F, _I32, _I32, _V, _P, _V, _V, _P, _P, _V,
                                                        _P, _SZ, _P]),
+})
+
+_D = ctypes.c_double
+_SIGNATURES.update({
+    "ssm_embedding_fwd": (ctypes.c_int, [_I64] * 3 + [_P, _I32, _V, _F, _V, _P]),
+    "ssm_embedding_bwd_workspace_size": (ctypes.c_int, [_I64] * 3 + [ctypes.POINTER(_SZ)]),
+    "ssm_embedding_bwd": (ctypes.c_int, [_I64] * 3 + [_P, _I32, _F, _V, _V, _P, _SZ, _P]),
+    "ssm_rms_norm_fwd": (ctypes.c_int, [_I64] * 2 + [_V, _V, _P, _I32, _F, _V, _V, _P]),
+    "ssm_rms_norm_fp8": (ctypes.c_int, [_I64] * 2 + [_V, _V, _P, _I32, _F, _I32, _P, _I64, _P, _V, _P]),
+    "ssm_rms_norm_bwd_workspace_size": (ctypes.c_int, [_I64] * 2 + [ctypes.POINTER(_SZ)]),
+    "ssm_rms_norm_bwd": (ctypes.c_int, [_I64] * 2 + [_V, _P, _I32, _F, _V, _V, _V, _V, _P, _P, _SZ, _P]),
+    "ssm_linear_fp8": (ctypes.c_int, [_I64] * 3 + [_P, _I64, _P, _P, _I64, _P, _P, _I32, _V, _V, _P]),
+    "ssm_sample_tokens": (ctypes.c_int, [_I64] * 2 + [_V, _P, _P, _D, _P, _I64, _P, _D, _P, _D, _P, _P]),
 })
 
 _OPTS = ctypes.POINTER(SsmDeltaOpts)

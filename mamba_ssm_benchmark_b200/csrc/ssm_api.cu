@@ -35,6 +35,7 @@ namespace ssm {
 int report_error(int code, const char* msg);
 // The current device's error word (see below), for kernels launched from other translation units.
 int* device_error_word();
+bool encode_rows8(CUtensorMap* map, const void* ptr, int64_t rows, int64_t cols, int64_t stride, int box_rows);
 }  // namespace ssm
 
 // Device-side error word set by kernels whose bounded waits gave up.
@@ -441,6 +442,18 @@ int fwd_impl(int phase, int64_t B, int64_t L, int64_t D, int64_t N, int32_t meth
 
 int ssm::report_error(int code, const char* msg) { return fail(code, "%s", msg); }
 int* ssm::device_error_word() { return device_error_ptr(); }
+// Tensor map over (rows, cols) bytes, `stride` bytes from row to row, in boxes of 128 columns and box_rows rows whose
+// 16-byte groups are permuted as tcgen05's 128-byte swizzle has them.  Bytes past an edge read as zero.
+bool ssm::encode_rows8(CUtensorMap* map, const void* ptr, int64_t rows, int64_t cols, int64_t stride, int box_rows) {
+  EncodeTiledFn enc = encode_fn();
+  if (enc == nullptr) return false;
+  if (rows <= 1) stride = (cols + 15) / 16 * 16;       // addresses nothing then; any legal value
+  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)stride};
+  const cuuint32_t box[2] = {128, (cuuint32_t)box_rows}, es[2] = {1, 1};
+  return enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), dims, strides, box, es,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
 
 extern "C" {
 

@@ -1,0 +1,442 @@
+// ssm_embedding.cu — rows of a table by token, scaled, and the table's gradient.
+//
+//   y[t] = scale W[idx[t]],   dW[v] = scale sum over t with idx[t] = v of dy[t]
+// Both directions are bound by memory: the rows that are read and written.  The gradient's places are sorted by token
+// (stable, so that a token's places stay in order), cut into chunks of equal length whatever the tokens' frequencies,
+// and summed chunk by chunk: fp32 within a chunk, fp64 over the chunks that a frequent token spans.  No atomics on
+// floats, a fixed order: results are reproducible.  Rows that no token names are zeroed by CTAs of the same launch.
+//
+// A token outside 0 .. V-1 gives a row of NaN and no gradient, and sets bit 1 of the device error word.
+#include <cooperative_groups.h>
+
+#include <algorithm>
+#include <cstdio>
+
+#include "ssm_b200.h"
+#include "ssm_launch.cuh"
+#include "ssm_vec.cuh"
+
+namespace cg = cooperative_groups;
+
+namespace ssm {
+int report_error(int code, const char* msg);
+int* device_error_word();
+}  // namespace ssm
+
+namespace {
+
+using ssm::Raw;
+using ssm::from_f32;
+using ssm::to_f32;
+using ssm::vec_store;
+
+constexpr int kBadToken = 2;        // bit of the device error word
+
+struct EmbedParams {
+  const void* idx;
+  int idx8;                         // 64-bit ids
+  const void* w;                    // table, or the gradient of the rows
+  void* y;                          // rows, or the gradient of the table
+  long long ws, ys;                 // row strides
+  long long T, V;
+  int C;
+  float scale;
+  int* err;
+  // backward
+  const uint2* sorted;              // (token, place) by token
+  float* part;                      // (chunks, 2, C)
+  long long chunks;
+  int len;                          // places to a chunk
+  int slabs;                        // CTAs over the channels
+};
+
+__device__ __forceinline__ long long token_at(const EmbedParams& p, long long t) {
+  return p.idx8 ? static_cast<const long long*>(p.idx)[t] : (long long)static_cast<const int*>(p.idx)[t];
+}
+
+// ---- forward ----------------------------------------------------------------------------------
+// A warp takes kAhead vectors a lane of one row, so that as many loads are on their way; a row has `pieces` warps.
+constexpr int kAhead = 4;
+template <typename T, int VEC, bool SCALE>
+__global__ void __launch_bounds__(256) embed_fwd(const __grid_constant__ EmbedParams p, int pieces) {
+  const long long item = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const long long t = item / pieces;
+  if (t >= p.T) return;
+  const int lane = threadIdx.x & 31, c0 = ((int)(item - t * pieces) * kAhead * 32 + lane) * VEC;
+  const long long v = token_at(p, t);
+  const bool bad = v < 0 || v >= p.V;
+  T* out = static_cast<T*>(p.y) + t * p.ys;
+  if (bad) {
+    if (lane == 0 && p.err != nullptr) atomicOr(p.err, kBadToken);
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k)
+      for (int i = 0; i < VEC; ++i)
+        if (c0 + k * 32 * VEC + i < p.C) out[c0 + k * 32 * VEC + i] = from_f32<T>(__int_as_float(0x7fc00000));
+    return;
+  }
+  const T* row = static_cast<const T*>(p.w) + v * p.ws;
+  Raw<T, VEC> raw[kAhead];
+#pragma unroll
+  for (int k = 0; k < kAhead; ++k)
+    if (c0 + k * 32 * VEC < p.C) raw[k].load(row + c0 + k * 32 * VEC);
+#pragma unroll
+  for (int k = 0; k < kAhead; ++k) {
+    const int c = c0 + k * 32 * VEC;
+    if (c >= p.C) continue;
+    if constexpr (SCALE) {
+      float x[VEC];
+      raw[k].widen(x);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) x[i] *= p.scale;
+      vec_store<T, VEC>(out + c, x);
+    } else {
+      *reinterpret_cast<Raw<T, VEC>*>(out + c) = raw[k];
+    }
+  }
+}
+
+// ---- places by token ----------------------------------------------------------------------------
+// A stable radix sort, kDigit bits a pass, by one cluster: with a launch a step it would be six launches.  A warp
+// owns consecutive places; counts are kept by warp, so that its places land in order behind those of the warps before it.
+constexpr int kDigit = 9, kBins = 1 << kDigit, kSortWarps = 32;
+struct SortSmem {
+  uint32_t count[kSortWarps][kBins];   // by warp: counts, then where its next place of a bin goes
+  uint32_t total[kBins];               // of this CTA
+  uint32_t base[kBins];
+  uint32_t warp_sum[kSortWarps];
+};
+
+__global__ void __launch_bounds__(1024) embed_sort(const __grid_constant__ EmbedParams p, uint2* a, uint2* b, int passes) {
+  extern __shared__ __align__(16) unsigned char raw[];
+  SortSmem& s = *reinterpret_cast<SortSmem*>(raw);
+  cg::cluster_group cluster = cg::this_cluster();
+  const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // places of this warp: a multiple of 32 to each
+  const long long per = ((p.T + ctas * kSortWarps - 1) / (ctas * kSortWarps) + 31) / 32 * 32;
+  const long long first = min(p.T, (long long)(rank * kSortWarps + warp) * per), last = min(p.T, first + per);
+  for (int pass = 0; pass < passes; ++pass) {
+    const int shift = pass * kDigit;
+    const uint2* src = pass & 1 ? a : b;               // from the second pass on
+    uint2* dst = pass & 1 ? b : a;
+    auto item = [&](long long t) {
+      if (pass > 0) return src[t];
+      const long long v = token_at(p, t);
+      return make_uint2((uint32_t)(v < 0 || v >= p.V ? p.V : v), (uint32_t)t);
+    };
+    for (int i = threadIdx.x; i < kSortWarps * kBins; i += 1024) (&s.count[0][0])[i] = 0;
+    __syncthreads();
+    for (long long t = first + lane; t < last; t += 32) atomicAdd(&s.count[warp][item(t).x >> shift & (kBins - 1)], 1u);
+    __syncthreads();
+    // by bin: this CTA's total
+    uint32_t mine = 0;
+    if (threadIdx.x < kBins) {
+      for (int w = 0; w < kSortWarps; ++w) mine += s.count[w][threadIdx.x];
+      s.total[threadIdx.x] = mine;
+    }
+    cluster.sync();
+    // by bin: what the CTAs before have of it, and all CTAs have
+    uint32_t before = 0, all = 0;
+    if (threadIdx.x < kBins)
+      for (int r = 0; r < ctas; ++r) {
+        const uint32_t n = cluster.map_shared_rank(s.total, r)[threadIdx.x];
+        if (r < rank) before += n;
+        all += n;
+      }
+    uint32_t run = all;                                // inclusive sum over the bins
+#pragma unroll
+    for (int m = 1; m < 32; m *= 2) {
+      const uint32_t up = __shfl_up_sync(0xffffffffu, run, m);
+      if (lane >= m) run += up;
+    }
+    if (lane == 31) s.warp_sum[warp] = run;
+    __syncthreads();
+    if (threadIdx.x < kBins) {
+      uint32_t at = run - all + before;
+      for (int w = 0; w < warp; ++w) at += s.warp_sum[w];
+      for (int w = 0; w < kSortWarps; ++w) {
+        const uint32_t n = s.count[w][threadIdx.x];
+        s.count[w][threadIdx.x] = at;
+        at += n;
+      }
+    }
+    __syncthreads();
+    for (long long t0 = first; t0 < last; t0 += 32) {
+      const bool live = t0 + lane < last;
+      const uint2 x = live ? item(t0 + lane) : make_uint2(0, 0);
+      const uint32_t bin = live ? x.x >> shift & (kBins - 1) : kBins;      // lanes past the end share a bin of their own
+      const uint32_t same = __match_any_sync(0xffffffffu, bin);
+      const uint32_t place = live ? s.count[warp][bin] + __popc(same & ((1u << lane) - 1)) : 0;
+      __syncwarp();
+      if (live && lane == __ffs(same) - 1) s.count[warp][bin] += __popc(same);
+      __syncwarp();
+      if (live) dst[place] = x;
+    }
+    __threadfence();
+    cluster.sync();                                    // the next pass reads what every CTA wrote, and counts anew
+  }
+}
+
+// ---- sums of the sorted places ---------------------------------------------------------------------
+constexpr int kSumThreads = 128, kLongest = 64, kRows = 8, kFill = 32;
+
+// The sum of a run of equal tokens goes to the table where the chunk holds all of it, else to the chunk's partial
+// rows: 0 where the run comes from the chunk before, 1 where it starts here and goes on.
+template <typename T, int VEC>
+__global__ void __launch_bounds__(kSumThreads) embed_sum(const __grid_constant__ EmbedParams p) {
+  __shared__ uint2 at[kLongest];
+  __shared__ uint32_t outer[2];                        // the tokens before and behind the chunk
+  const int c = ((int)(blockIdx.x % p.slabs) * kSumThreads + threadIdx.x) * VEC;
+  const long long chunk = blockIdx.x / p.slabs;
+  constexpr uint32_t kNone = 0xffffffffu;
+  if (chunk >= p.chunks) {                             // rows without a token
+    const long long v0 = (chunk - p.chunks) * kFill;
+    if (threadIdx.x < kFill) {
+      const long long v = v0 + threadIdx.x;
+      long long lo = 0, hi = p.T;                      // the first place whose token is v or above
+      while (lo < hi) {
+        const long long mid = (lo + hi) >> 1;
+        if (p.sorted[mid].x < v) lo = mid + 1;
+        else hi = mid;
+      }
+      at[threadIdx.x].x = v < p.V && (lo == p.T || p.sorted[lo].x != v);
+    }
+    __syncthreads();
+    const float zero[VEC] = {};
+    if (c < p.C)
+      for (int i = 0; i < kFill; ++i)
+        if (at[i].x) vec_store<T, VEC>(static_cast<T*>(p.y) + (v0 + i) * p.ys + c, zero);
+    return;
+  }
+  const long long t0 = chunk * p.len;
+  const int n = (int)min((long long)p.len, p.T - t0);
+  if (threadIdx.x < n) at[threadIdx.x] = p.sorted[t0 + threadIdx.x];
+  if (threadIdx.x == 64) outer[0] = t0 > 0 ? p.sorted[t0 - 1].x : kNone;
+  if (threadIdx.x == 65) outer[1] = t0 + n < p.T ? p.sorted[t0 + n].x : kNone;
+  __syncthreads();
+  if (c >= p.C) return;
+  float acc[VEC] = {};
+  int start = 0;                                       // of the run
+  auto flush = [&](int end) {
+    const uint32_t v = at[start].x;
+    if (v < p.V) {
+      const bool from = start == 0 && outer[0] == v, to = end == n && outer[1] == v;
+      if (!from && !to) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) acc[i] *= p.scale;
+        vec_store<T, VEC>(static_cast<T*>(p.y) + (long long)v * p.ys + c, acc);
+      } else {
+        float* out = p.part + ((size_t)chunk * 2 + (from ? 0 : 1)) * p.C + c;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) out[i] = acc[i];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) acc[i] = 0.0f;
+    start = end;
+  };
+  for (int i0 = 0; i0 < n; i0 += kRows) {
+    Raw<T, VEC> raw[kRows];
+#pragma unroll
+    for (int i = 0; i < kRows; ++i)
+      if (i0 + i < n) raw[i].load(static_cast<const T*>(p.w) + (long long)at[i0 + i].y * p.ws + c);
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+      if (i0 + i >= n) break;
+      if (at[i0 + i].x != at[start].x) flush(i0 + i);
+      float x[VEC];
+      raw[i].widen(x);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) acc[j] += x[j];
+    }
+  }
+  flush(n);
+}
+
+// Runs that span chunks: the chunk where one starts adds what the next ones have of it.
+template <typename T>
+__global__ void __launch_bounds__(kSumThreads) embed_join(const __grid_constant__ EmbedParams p) {
+  const long long chunk = blockIdx.x / p.slabs, end = (chunk + 1) * p.len;
+  if (end >= p.T) return;
+  const uint32_t v = p.sorted[end - 1].x;
+  if (v >= p.V || p.sorted[end].x != v) return;
+  if (p.sorted[chunk * p.len].x == v && chunk > 0 && p.sorted[chunk * p.len - 1].x == v) return;      // starts before
+  long long more = chunk + 1;                          // chunks behind that go on with the run
+  while (more + 1 < p.chunks && p.sorted[(more + 1) * p.len].x == v) ++more;
+  for (int c = (int)(blockIdx.x % p.slabs) * kSumThreads + threadIdx.x; c < p.C; c += p.slabs * kSumThreads) {
+    double s = (double)p.part[((size_t)chunk * 2 + 1) * p.C + c];
+#pragma unroll 4
+    for (long long q = chunk + 1; q <= more; ++q) s += (double)p.part[(size_t)q * 2 * p.C + c];
+    static_cast<T*>(p.y)[(long long)v * p.ys + c] = from_f32<T>((float)(s * (double)p.scale));
+  }
+}
+
+// ---- host -----------------------------------------------------------------------------------
+int fail(int code, const char* fmt, long long a = 0, long long b = 0) {
+  char msg[256];
+  snprintf(msg, sizeof(msg), fmt, a, b);
+  return ssm::report_error(code, msg);
+}
+long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
+size_t round256(size_t x) { return (x + 255) & ~size_t(255); }
+
+int check_shape(int64_t T, int64_t V, int64_t C) {
+  if (T < 1 || V < 1 || C < 1) return fail(SSM_ERR_INVALID, "embedding: tokens, vocabulary and channels must be positive");
+  if (T > (1LL << 30) || V > (1LL << 30) || C > (1LL << 20))
+    return fail(SSM_ERR_INVALID, "embedding: shape out of range (tokens %lld, vocabulary %lld)", T, V);
+  return SSM_OK;
+}
+int check_side(const char* what, const ssm_view& v) {
+  char msg[128];
+  if (v.ptr == nullptr) {
+    snprintf(msg, sizeof(msg), "embedding: %s is required", what);
+    return ssm::report_error(SSM_ERR_INVALID, msg);
+  }
+  if (v.dtype != SSM_F32 && v.dtype != SSM_BF16) {
+    snprintf(msg, sizeof(msg), "embedding: %s must be float32 or bfloat16", what);
+    return ssm::report_error(SSM_ERR_DTYPE, msg);
+  }
+  return SSM_OK;
+}
+// The widest vector, at most 16 bytes, that divides the channels and at which the rows of both tensors start aligned.
+int width(int64_t C, int es, const ssm_view& a, const ssm_view& b) {
+  int vec = 16 / es;
+  auto fits = [&](const ssm_view& v) {
+    return reinterpret_cast<uintptr_t>(v.ptr) % (vec * es) == 0 && v.batch_stride % vec == 0;
+  };
+  while (vec > 1 && (C % vec != 0 || !fits(a) || !fits(b))) vec /= 2;
+  return vec;
+}
+
+template <typename T, int VEC>
+cudaError_t run_fwd(const EmbedParams& p, cudaStream_t st) {
+  const int pieces = (int)ceil_div(p.C, 32 * VEC * kAhead);
+  const unsigned grid = (unsigned)ceil_div(p.T * pieces, 8);
+  if (p.scale == 1.0f) embed_fwd<T, VEC, false><<<grid, 256, 0, st>>>(p, pieces);
+  else embed_fwd<T, VEC, true><<<grid, 256, 0, st>>>(p, pieces);
+  return cudaGetLastError();
+}
+template <typename T, int VEC>
+cudaError_t run_bwd(EmbedParams p, cudaStream_t st) {
+  p.slabs = (int)ceil_div(p.C, kSumThreads * VEC);
+  embed_sum<T, VEC><<<(unsigned)((p.chunks + ceil_div(p.V, kFill)) * p.slabs), kSumThreads, 0, st>>>(p);
+  p.slabs = (int)std::min<long long>(ceil_div(p.C, kSumThreads), 8);
+  embed_join<T><<<(unsigned)(p.chunks * p.slabs), kSumThreads, 0, st>>>(p);
+  return cudaGetLastError();
+}
+template <typename T>
+cudaError_t run(const EmbedParams& p, bool bwd, int vec, cudaStream_t st) {
+  if constexpr (sizeof(T) == 2)
+    if (vec == 8) return bwd ? run_bwd<T, 8>(p, st) : run_fwd<T, 8>(p, st);
+  if (vec == 4) return bwd ? run_bwd<T, 4>(p, st) : run_fwd<T, 4>(p, st);
+  if (vec == 2) return bwd ? run_bwd<T, 2>(p, st) : run_fwd<T, 2>(p, st);
+  return bwd ? run_bwd<T, 1>(p, st) : run_fwd<T, 1>(p, st);
+}
+
+// Places to a chunk: as many as leave every SM a dozen CTAs, 8 to kLongest.
+int chunk_len(int64_t T, int64_t C) {
+  const long long slabs = ceil_div(C, kSumThreads * 4);
+  return (int)std::max<long long>(8, std::min<long long>(kLongest, T * slabs / (148 * 12)));
+}
+
+int run_sort(const EmbedParams& p, uint2* a, uint2* b, int passes, cudaStream_t st) {
+  // the barriers of a cluster cost more than its CTAs save while one CTA's warps take a few dozen places each
+  const int ctas = p.T <= 4096 ? 1 : 8;
+  ssm::ctas_per_sm<embed_sort>(1024, sizeof(SortSmem));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(1024);
+  cfg.dynamicSmemBytes = sizeof(SortSmem);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = ctas;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, embed_sort, p, a, b, passes);
+  return e == cudaSuccess ? SSM_OK : fail(SSM_ERR_CUDA, "embedding: the sort's launch failed (error %lld)", (long long)e);
+}
+
+}  // namespace
+
+extern "C" {
+
+int ssm_embedding_fwd(int64_t T, int64_t V, int64_t C, const void* idx, int32_t idx_bytes, ssm_view weight, float scale,
+                      ssm_view y, void* stream) {
+  if (int rc = check_shape(T, V, C)) return rc;
+  if (idx == nullptr || (idx_bytes != 4 && idx_bytes != 8))
+    return fail(idx == nullptr ? SSM_ERR_INVALID : SSM_ERR_DTYPE, "embedding: the ids are required, in 32 or 64 bits");
+  if (int rc = check_side("weight", weight)) return rc;
+  if (int rc = check_side("y", y)) return rc;
+  if (weight.dtype != y.dtype) return fail(SSM_ERR_DTYPE, "embedding: y must have the weight's dtype");
+  EmbedParams p = {};
+  p.idx = idx;
+  p.idx8 = idx_bytes == 8;
+  p.w = weight.ptr;
+  p.ws = weight.batch_stride;
+  p.y = const_cast<void*>(y.ptr);
+  p.ys = y.batch_stride;
+  p.T = T;
+  p.V = V;
+  p.C = (int)C;
+  p.scale = scale;
+  p.err = ssm::device_error_word();
+  const int es = weight.dtype == SSM_BF16 ? 2 : 4, vec = width(C, es, weight, y);
+  if (ceil_div(T * ceil_div(C, 32 * vec * kAhead), 8) > 0x7fffffffLL)
+    return fail(SSM_ERR_INVALID, "embedding: shape out of range (tokens %lld, channels %lld)", T, C);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const cudaError_t e = es == 2 ? run<__nv_bfloat16>(p, false, vec, st) : run<float>(p, false, vec, st);
+  return e == cudaSuccess ? SSM_OK : fail(SSM_ERR_CUDA, "embedding forward launch failed (error %lld)", (long long)e);
+}
+
+int ssm_embedding_bwd_workspace_size(int64_t T, int64_t V, int64_t C, size_t* bytes) {
+  if (bytes == nullptr) return fail(SSM_ERR_INVALID, "embedding: bytes is NULL");
+  if (int rc = check_shape(T, V, C)) return rc;
+  *bytes = 2 * round256((size_t)T * sizeof(uint2)) + (size_t)ceil_div(T, chunk_len(T, C)) * 2 * C * sizeof(float) + 256;
+  return SSM_OK;
+}
+
+int ssm_embedding_bwd(int64_t T, int64_t V, int64_t C, const void* idx, int32_t idx_bytes, float scale, ssm_view dy,
+                      ssm_view dweight, void* workspace, size_t workspace_bytes, void* stream) {
+  if (int rc = check_shape(T, V, C)) return rc;
+  if (idx == nullptr || (idx_bytes != 4 && idx_bytes != 8))
+    return fail(idx == nullptr ? SSM_ERR_INVALID : SSM_ERR_DTYPE, "embedding: the ids are required, in 32 or 64 bits");
+  if (int rc = check_side("dy", dy)) return rc;
+  if (int rc = check_side("dweight", dweight)) return rc;
+  if (dy.dtype != dweight.dtype) return fail(SSM_ERR_DTYPE, "embedding: dweight must have dy's dtype");
+  size_t need = 0;
+  ssm_embedding_bwd_workspace_size(T, V, C, &need);
+  if (workspace == nullptr || workspace_bytes < need)
+    return fail(SSM_ERR_WORKSPACE, "embedding: workspace of %lld bytes required, %lld given", (long long)need,
+                (long long)workspace_bytes);
+  EmbedParams p = {};
+  p.idx = idx;
+  p.idx8 = idx_bytes == 8;
+  p.w = dy.ptr;
+  p.ws = dy.batch_stride;
+  p.y = const_cast<void*>(dweight.ptr);
+  p.ys = dweight.batch_stride;
+  p.T = T;
+  p.V = V;
+  p.C = (int)C;
+  p.scale = scale;
+  p.len = chunk_len(T, C);
+  p.chunks = ceil_div(T, p.len);
+  const int es = dy.dtype == SSM_BF16 ? 2 : 4, vec = width(C, es, dy, dweight);
+  if ((p.chunks + ceil_div(V, kFill)) * std::max<long long>(8, ceil_div(C, kSumThreads * vec)) > 0x7fffffffLL)
+    return fail(SSM_ERR_INVALID, "embedding: shape out of range (tokens %lld, channels %lld)", T, C);
+  unsigned char* at = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(workspace) + 255) & ~uintptr_t(255));
+  uint2* a = reinterpret_cast<uint2*>(at);
+  uint2* b = reinterpret_cast<uint2*>(at + round256((size_t)T * sizeof(uint2)));
+  p.part = reinterpret_cast<float*>(at + 2 * round256((size_t)T * sizeof(uint2)));
+  int passes = 1;                                      // of kDigit bits, for the ids 0 .. V (V: outside)
+  while (passes * kDigit < 32 && (V >> (passes * kDigit)) > 0) ++passes;
+  p.sorted = passes & 1 ? a : b;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (int rc = run_sort(p, a, b, passes, st)) return rc;
+  const cudaError_t e = es == 2 ? run<__nv_bfloat16>(p, true, vec, st) : run<float>(p, true, vec, st);
+  return e == cudaSuccess ? SSM_OK : fail(SSM_ERR_CUDA, "embedding backward launch failed (error %lld)", (long long)e);
+}
+
+}  // extern "C"

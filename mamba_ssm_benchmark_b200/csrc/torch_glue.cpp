@@ -1,9 +1,10 @@
-// torch_glue.cpp — torch tensors and autograd for the gated delta rule and the group norm: the module _C/_glue.so,
-// which calls the C entry points of libssm_b200.so (include/ssm_b200.h).
+// torch_glue.cpp — torch tensors and autograd for the operators whose host time counts: the gated delta rule, the group
+// norm and the operators around the mixers (embedding, RMS norm, 8-bit products, sampling).  The module _C/_glue.so, which
+// calls the C entry points of libssm_b200.so (include/ssm_b200.h).
 //
 // These operators are small enough in training and decoding that the host decides: as Python autograd functions
 // over ctypes a head norm of 8192 x 512 took 135 us forward and backward, 33 of them on the GPU; through here 85.  Arguments are
-// checked by the Python layer (delta.py, norm.py); what arrives here has the right shapes, one device and unit
+// checked by the Python layer (delta.py, norm.py and so on); what arrives here has the right shapes, one device and unit
 // inner strides, except gradients, which autograd hands over as they are.
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -234,6 +235,164 @@ Tensor gated_delta_step(const Tensor& state, const Tensor& q, const Tensor& k, c
   return o;
 }
 
+// ---- embedding ------------------------------------------------------------------------------------
+// idx: T dense ids; the result is (T, C).
+Tensor embedding_forward(const Tensor& idx, const Tensor& weight, double scale) {
+  const c10::cuda::CUDAGuard guard(weight.device());
+  const Tensor y = at::empty({idx.numel(), weight.size(1)}, weight.options());
+  check(ssm_embedding_fwd(idx.numel(), weight.size(0), weight.size(1), idx.const_data_ptr(), (int)idx.element_size(),
+                          view(weight), (float)scale, view(y), stream(weight)),
+        "ssm_embedding_fwd");
+  return y;
+}
+
+struct Embedding : torch::autograd::Function<Embedding> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& weight, const Tensor& idx, double scale) {
+    ctx->save_for_backward({idx});
+    ctx->saved_data["vocab"] = weight.size(0);
+    ctx->saved_data["scale"] = scale;
+    return embedding_forward(idx, weight, scale);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    once("embedding");
+    const Tensor idx = ctx->get_saved_variables()[0];
+    const int64_t V = ctx->saved_data["vocab"].toInt();
+    const c10::cuda::CUDAGuard guard(grads[0].device());
+    const Tensor dy = dense(grads[0], grads[0].scalar_type()), dw = at::empty({V, dy.size(1)}, dy.options());
+    size_t need = 0;
+    check(ssm_embedding_bwd_workspace_size(dy.size(0), V, dy.size(1), &need), "ssm_embedding_bwd_workspace_size");
+    const Tensor ws = bytes(need, dy);
+    check(ssm_embedding_bwd(dy.size(0), V, dy.size(1), idx.const_data_ptr(), (int)idx.element_size(),
+                            (float)ctx->saved_data["scale"].toDouble(), view(dy), view(dw), ws.mutable_data_ptr(), need,
+                            stream(dy)),
+          "ssm_embedding_bwd");
+    return {dw, Tensor(), Tensor()};
+  }
+};
+
+Tensor embedding(const Tensor& idx, const Tensor& weight, double scale) {
+  plain("embedding", {weight});
+  return at::GradMode::is_enabled() && wants(weight) ? Embedding::apply(weight, idx, scale)
+                                                     : embedding_forward(idx, weight, scale);
+}
+
+// ---- root-mean-square norm --------------------------------------------------------------------------
+// x, residual: (rows, C).  (y, total), total undefined without a residual.
+std::tuple<Tensor, Tensor> rms_forward(const Tensor& x, const Tensor& residual, const Tensor& weight, double eps) {
+  const c10::cuda::CUDAGuard guard(x.device());
+  const Tensor y = dense_like(x);
+  Tensor total;
+  if (residual.defined()) total = dense_like(residual);
+  check(ssm_rms_norm_fwd(x.size(0), x.size(1), view(x), view(residual), data(weight), weight.defined() ? code(weight) : SSM_F32,
+                         (float)eps, view(y), view(total), stream(x)),
+        "ssm_rms_norm_fwd");
+  return {y, total};
+}
+
+struct RmsNorm : torch::autograd::Function<RmsNorm> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Maybe& residual, const Maybe& weight, double eps) {
+    const auto [y, total] = rms_forward(x, value(residual), value(weight), eps);
+    ctx->save_for_backward({total.defined() ? total : x, value(weight)});
+    ctx->saved_data["eps"] = eps;
+    ctx->saved_data["bf16"] = x.scalar_type() == at::kBFloat16;
+    ctx->saved_data["residual"] = total.defined();
+    ctx->set_materialize_grads(false);
+    return total.defined() ? variable_list{y, total} : variable_list{y};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    once("rms_norm");
+    const variable_list saved = ctx->get_saved_variables();
+    const Tensor &total = saved[0], &weight = saved[1];
+    const bool residual = ctx->saved_data["residual"].toBool();
+    const at::ScalarType type = ctx->saved_data["bf16"].toBool() ? at::kBFloat16 : at::kFloat;
+    const c10::cuda::CUDAGuard guard(total.device());
+    Tensor dtotal;
+    if (residual && grads[1].defined()) dtotal = dense(grads[1], total.scalar_type());
+    if (!grads[0].defined()) {                       // only the sum was used
+      Tensor dw;
+      if (weight.defined()) dw = at::zeros(weight.sizes(), weight.options());
+      return {dtotal.defined() ? dtotal.to(type) : Tensor(), dtotal, dw, Tensor()};
+    }
+    const Tensor dy = dense(grads[0], type), dx = at::empty(total.sizes(), total.options().dtype(type));
+    Tensor dr, dw;
+    if (residual && total.scalar_type() != type) dr = dense_like(total);
+    if (weight.defined()) dw = dense_like(weight);
+    size_t need = 0;
+    check(ssm_rms_norm_bwd_workspace_size(dy.size(0), dy.size(1), &need), "ssm_rms_norm_bwd_workspace_size");
+    const Tensor ws = bytes(need, dy);
+    check(ssm_rms_norm_bwd(dy.size(0), dy.size(1), view(total), data(weight), weight.defined() ? code(weight) : SSM_F32,
+                           (float)ctx->saved_data["eps"].toDouble(), view(dy), view(dtotal), view(dx), view(dr),
+                           dw.defined() ? dw.mutable_data_ptr() : nullptr, ws.mutable_data_ptr(), need, stream(dy)),
+          "ssm_rms_norm_bwd");
+    // in one type the two inputs' gradients are one tensor, as those of a sum of two tensors are
+    return {dx, !residual ? Tensor() : dr.defined() ? dr : dx, dw, Tensor()};
+  }
+};
+
+variable_list rms_norm(const Tensor& x, const Maybe& residual, const Maybe& weight, double eps) {
+  plain("rms_norm", {x, value(residual), value(weight)});
+  if (at::GradMode::is_enabled() && (wants(x) || wants(residual) || wants(weight))) return RmsNorm::apply(x, residual, weight, eps);
+  const auto [y, total] = rms_forward(x, value(residual), value(weight), eps);
+  return total.defined() ? variable_list{y, total} : variable_list{y};
+}
+
+// Rows of 8 bits start at multiples of 16 bytes, as ssm_linear_fp8 reads them.
+Tensor rows8(int64_t rows, int64_t C, const Tensor& like) {
+  const Tensor t = at::empty({rows, (C + 15) / 16 * 16}, like.options().dtype(at::kFloat8_e4m3fn));
+  return t.size(1) == C ? t : t.narrow(1, 0, C);
+}
+
+// (y8, scale) or (y8, scale, total)
+variable_list rms_norm_fp8(const Tensor& x, const Maybe& residual, const Maybe& weight, double eps, bool norm) {
+  plain(norm ? "rms_norm_fp8" : "quantize_fp8", {x, value(residual), value(weight)});
+  const c10::cuda::CUDAGuard guard(x.device());
+  const Tensor r = value(residual), w = value(weight);
+  const Tensor y8 = rows8(x.size(0), x.size(1), x), scale = at::empty({x.size(0)}, x.options().dtype(at::kFloat));
+  Tensor total;
+  if (r.defined()) total = dense_like(r);
+  check(ssm_rms_norm_fp8(x.size(0), x.size(1), view(x), view(r), data(w), w.defined() ? code(w) : SSM_F32, (float)eps, norm,
+                         y8.mutable_data_ptr(), y8.stride(0), f32(scale), view(total), stream(x)),
+        "ssm_rms_norm_fp8");
+  return total.defined() ? variable_list{y8, scale, total} : variable_list{y8, scale};
+}
+
+// ---- 8-bit products -----------------------------------------------------------------------------------
+Tensor linear_fp8(const Tensor& x8, const Tensor& x_scale, const Tensor& w8, const Tensor& w_scale, const Maybe& bias,
+                  const Maybe& residual, bool silu, bool bf16) {
+  plain("linear_fp8", {x8, x_scale, w8, w_scale, value(bias), value(residual)});
+  const c10::cuda::CUDAGuard guard(x8.device());
+  auto rows = [](const Tensor& t) {                  // rows that start at multiples of 16 bytes
+    const bool fits = (t.stride(1) == 1 || t.size(1) == 1) && (t.size(0) == 1 || (t.stride(0) % 16 == 0 && t.stride(0) >= t.size(1))) &&
+                      reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0;
+    if (fits) return t;
+    const Tensor u = rows8(t.size(0), t.size(1), t);
+    u.copy_(t);
+    return u;
+  };
+  auto stride = [](const Tensor& t) { return t.size(0) == 1 ? (t.size(1) + 15) / 16 * 16 : t.stride(0); };
+  const Tensor x = rows(x8), w = rows(w8);
+  const Tensor y = at::empty({x.size(0), w.size(0)}, x_scale.options().dtype(bf16 ? at::kBFloat16 : at::kFloat));
+  check(ssm_linear_fp8(x.size(0), w.size(0), x.size(1), x.const_data_ptr(), stride(x), f32(x_scale), w.const_data_ptr(),
+                       stride(w), f32(w_scale), f32(value(bias)), silu, view(value(residual)), view(y), stream(x)),
+        "ssm_linear_fp8");
+  return y;
+}
+
+// ---- sampling -------------------------------------------------------------------------------------
+// Settings: (B) float64 (top_k: int64) tensors, or the numbers beside them.
+Tensor sample_tokens(const Tensor& logits, const Tensor& uniforms, const Maybe& temperature, double temperature0, const Maybe& top_k,
+                     int64_t top_k0, const Maybe& top_p, double top_p0, const Maybe& min_p, double min_p0) {
+  plain("sample_tokens", {logits, uniforms});
+  const c10::cuda::CUDAGuard guard(logits.device());
+  const Tensor tokens = at::empty({logits.size(0)}, logits.options().dtype(at::kLong));
+  auto by_row = [](const Maybe& t) { return t.has_value() ? t->const_data_ptr<double>() : nullptr; };
+  check(ssm_sample_tokens(logits.size(0), logits.size(1), view(logits), uniforms.const_data_ptr<float>(), by_row(temperature),
+                          temperature0, top_k.has_value() ? top_k->const_data_ptr<int64_t>() : nullptr, top_k0, by_row(top_p),
+                          top_p0, by_row(min_p), min_p0, tokens.mutable_data_ptr<int64_t>(), stream(logits)),
+        "ssm_sample_tokens");
+  return tokens;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -241,4 +400,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("group_norm", &group_norm, py::call_guard<py::gil_scoped_release>());
   m.def("gated_delta", &gated_delta, py::call_guard<py::gil_scoped_release>());
   m.def("gated_delta_step", &gated_delta_step, py::call_guard<py::gil_scoped_release>());
+  m.def("embedding", &embedding, py::call_guard<py::gil_scoped_release>());
+  m.def("rms_norm", &rms_norm, py::call_guard<py::gil_scoped_release>());
+  m.def("rms_norm_fp8", &rms_norm_fp8, py::call_guard<py::gil_scoped_release>());
+  m.def("linear_fp8", &linear_fp8, py::call_guard<py::gil_scoped_release>());
+  m.def("sample_tokens", &sample_tokens, py::call_guard<py::gil_scoped_release>());
 }
