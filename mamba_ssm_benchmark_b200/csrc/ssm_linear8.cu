@@ -84,13 +84,11 @@ __device__ __forceinline__ float peer_load(uint32_t addr, uint32_t rank) {
   return v;
 }
 
-// y's value from an accumulator; scale is the token's times the channel's.
-template <typename TY>
-__device__ __forceinline__ void finish(const LinearParams& p, float acc, float w_scale, float bias, int m, int n) {
-  float v = fmaf(acc, w_scale * p.x_scale[m], bias);
+// y's value from an accumulator, the token's scale and the residual.
+__device__ __forceinline__ float finish(const LinearParams& p, float acc, float w_scale, float x_scale, float bias, float res) {
+  float v = fmaf(acc, w_scale * x_scale, bias);
   if (p.silu) v = v / (1.0f + __expf(-v));
-  if (p.res != nullptr) v += to_f32(static_cast<const TY*>(p.res)[m * p.rs + n]);
-  static_cast<TY*>(p.y)[m * p.ys + n] = from_f32<TY>(v);
+  return v + res;
 }
 
 // SPLIT: a cluster takes one tile, its CTAs a part of K each.
@@ -180,18 +178,38 @@ __global__ void __launch_bounds__(kLinThreads) linear_e4m3(const __grid_constant
       wait.dead = __any_sync(0xffffffffu, wait.dead);
       if (!SPLIT && wait.dead) break;
       tc_fence_after();
+      if constexpr (SPLIT) {                             // [column][row], over the stages: all products are done
+        float* part = reinterpret_cast<float*>(smem);
 #pragma unroll
-      for (int c = 0; c < TN; c += 16) {
-        float v[16];
-        tc_load_f32(my + buf * TN + c, v);
-        if (SPLIT) {                                     // [column][row], over the stages: all products are done
-          float* part = reinterpret_cast<float*>(smem);
+        for (int c = 0; c < TN; c += 16) {
+          float v[16];
+          tc_load_f32(my + buf * TN + c, v);
 #pragma unroll
           for (int i = 0; i < 16; ++i) part[(c + i) * kRowsW + row] = wait.dead ? quiet_nan() : v[i];
-        } else if (live) {
+        }
+      } else {
+        // 16 tokens at a time, the next ones' residuals on their way
+        const TY* rp = static_cast<const TY*>(p.res) + (long long)m0 * p.rs + n;
+        TY* yp = static_cast<TY*>(p.y) + (long long)m0 * p.ys + n;
+        const bool adds = p.res != nullptr && live;
+        TY next[16];
+        auto fetch = [&](int c) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) next[i] = adds && m0 + c + i < p.tokens ? rp[(long long)(c + i) * p.rs] : from_f32<TY>(0.0f);
+        };
+        fetch(0);
+#pragma unroll 2
+        for (int c = 0; c < TN; c += 16) {
+          const float xs = m0 + c + (lane & 15) < p.tokens ? p.x_scale[m0 + c + (lane & 15)] : 0.0f;
+          float v[16];
+          tc_load_f32(my + buf * TN + c, v);
 #pragma unroll
           for (int i = 0; i < 16; ++i)
-            if (m0 + c + i < p.tokens) finish<TY>(p, v[i], ws, bias, m0 + c + i, n);
+            v[i] = finish(p, v[i], ws, __shfl_sync(0xffffffffu, xs, i), bias, to_f32(next[i]));
+          if (c + 16 < TN) fetch(c + 16);
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (live && m0 + c + i < p.tokens) yp[(long long)(c + i) * p.ys] = from_f32<TY>(v[i]);
         }
       }
       tc_fence_before();
@@ -211,7 +229,9 @@ __global__ void __launch_bounds__(kLinThreads) linear_e4m3(const __grid_constant
           const uint32_t at = smem_u32(smem) + (c * kRowsW + 32 * warp + lane) * 4;
           float v = peer_load(at, 0);
           for (int q = 1; q < parts; ++q) v += peer_load(at, q);
-          finish<TY>(p, v, ws, bias, m0 + c, n);
+          const long long m = m0 + c;
+          const float res = p.res != nullptr ? to_f32(static_cast<const TY*>(p.res)[m * p.rs + n]) : 0.0f;
+          static_cast<TY*>(p.y)[m * p.ys + n] = from_f32<TY>(finish(p, v, ws, p.x_scale[m], bias, res));
         }
       }
     }
