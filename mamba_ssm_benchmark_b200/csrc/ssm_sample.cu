@@ -8,7 +8,7 @@
 // units of 2^-42, formed in double, and every sum is a 64-bit whole number, exact in any order (up to 2^20 tokens).  A weight
 // is off by at most 2^-43 of the largest; what rounds to zero is never drawn.
 //
-// Up to kList tokens: a thread each, sorted by rank in registers.  More: a cluster of up to eight CTAs shares a row, a slice
+// Up to kFew tokens: a thread each, sorted by rank in registers.  More: a cluster of up to eight CTAs shares a row, a slice
 // of tokens each, kept in shared memory where it fits.  A histogram of the logits' distance to the largest says which
 // bins can hold the border of top_k (exactly) or of top_p (the bins' masses to a part in ten thousand); the few tokens
 // of these bins are sorted by one CTA, against exact sums of what lies before them.  Where a bin holds more than kList
@@ -43,26 +43,31 @@ struct SampleParams {
   long long* token;
   int V, bf16;
   int slice;                          // tokens of a CTA
+  int wide;                           // rows start where four logits are one load
   int cached;                         // its logits are kept in shared memory
 };
 
 constexpr int kBits = 42;
 constexpr u64 kOne = 1ull << kBits;
-constexpr int kTable = 64;            // steps of the table of 2^x
-
-constexpr int kList = 1024;           // tokens that are sorted: one to a thread
-constexpr int kBins = 2048;           // two to a thread
+constexpr int kTable = 1024;          // steps of the table of 2^x
+constexpr int kFew = 1024;            // tokens that one CTA takes, one to a thread
+constexpr int kThreads = 512;         // of a CTA that shares a row: two of them to an SM, so that one waits while one works
+constexpr int kWarps = kThreads / 32;
+constexpr int kList = kThreads;       // tokens that are sorted: one to a thread
+constexpr int kPer = 4, kBins = kPer * kThreads;
 constexpr int kMargins = 4;
 
 struct SampleSmem {
   double exp2[kTable];
   u64 part[32], slot[2];
   u64 list[kList];
-  uint32_t count[kBins];
+  u64 kept[kWarps];                   // by warp: the weight of its kept tokens
+  u64 slot2[2];
+  uint32_t count[kBins], upto[kBins];
   int size;                           // of the list
   int first[1 + 2 * kMargins];        // the first bin at which a sum over the bins passes a value
   u64 cut;
-  float logits[1];                    // the slice
+  alignas(16) float logits[4];        // the slice
 };
 
 // A whole number that orders floats as they compare (-0 as 0); the index decides among equal ones, the lowest first.
@@ -75,39 +80,37 @@ __device__ __forceinline__ float key_logit(u64 key) {
   return __uint_as_float(b & 0x80000000u ? b & 0x7fffffffu : ~b);
 }
 
-// 2^42 exp((l - top) rate / log2(e)).  2^y = 2^k 2^(j/64) 2^f, |f| <= 1/128: the Taylor polynomial of degree 5 is within
-// (ln 2 / 128)^6 / 720 = 4e-17 of 2^f.
+// A weight in whole units: 2^42 2^y, y = (l - top) rate.  2^y = 2^k 2^(j/1024) 2^r, |r| <= 2^-11: the Taylor polynomial of
+// degree 3 is within (ln 2 / 2048)^4 / 24 = 6e-16 of 2^r.  No branch: y is held above -60, where the weight is zero (a NaN,
+// of infinities, is too), and the largest logit's weight is set.  Ten operations in double, a quarter of the instructions.
 struct Weights {
   const double* table;
   float top;                          // the largest logit
-  double rate;                        // log2(e) / temperature
-  __device__ double operator()(float l) const {
-    if (l == top) return (double)kOne;
-    const double y = ((double)l - (double)top) * rate;
-    if (!(y > -(double)(kBits + 2))) return 0.0;           // below a quarter of a unit; also l = -inf
-    constexpr double kShift = 6755399441055744.0 / kTable;   // 1.5 2^52 / 64: y is rounded to 64ths
+  double top2, rate;                  // the same; log2(e) / temperature
+  __device__ u64 operator()(float l) const {
+    constexpr double kLn2 = 0.69314718055994531, kC2 = kLn2 * kLn2 / 2, kC3 = kLn2 * kLn2 * kLn2 / 6;
+    constexpr double kShift = 6755399441055744.0 / kTable;   // 1.5 2^52 / 1024: y is rounded to 1024ths
+    const double y = fmax(((double)l - top2) * rate, -60.0);
     const double t = y + kShift;
-    const int i = __double2loint(t);                       // 64 y, rounded
-    const double f = (y - (t - kShift)) * 0.6931471805599453;
-    double q = fma(f, 1.0 / 120, 1.0 / 24);
-    q = fma(f, q, 1.0 / 6);
-    q = fma(f, q, 0.5);
-    q = fma(f, q, 1.0);
-    q = fma(f, q, 1.0);
-    const double scale = __hiloint2double((1023 + kBits + (i >> 6)) << 20, 0);
-    return q * table[i & (kTable - 1)] * scale;
+    const int i = __double2loint(t);                       // 1024 y, rounded
+    const double r = y - (t - kShift);
+    const double q = fma(r, fma(r, fma(r, kC3, kC2), kLn2), 1.0);
+    const double step = table[i & (kTable - 1)];
+    const double scaled = __hiloint2double(__double2hiint(step) + (((i >> 10) + kBits) << 20), __double2loint(step));
+    const u64 units = (u64)__double_as_longlong(fma(scaled, q, 4503599627370496.0)) & ((1ull << 52) - 1);
+    return l == top ? kOne : units;
   }
 };
-__device__ __forceinline__ u64 units(double w) { return (u64)__double_as_longlong(w + 4503599627370496.0) & ((1ull << 52) - 1); }
 
 struct Settings {
-  double temperature, top_p, least;   // least: 2^42 min_p
+  double temperature, top_p;
+  u64 least;                          // min_p
   long long top_k;
   float u;
   __device__ Settings(const SampleParams& p, int row) {
     temperature = p.temperature != nullptr ? p.temperature[row] : p.temperature0;
     top_p = p.top_p != nullptr ? p.top_p[row] : p.top_p0;
-    least = fmin(fmax(p.min_p != nullptr ? p.min_p[row] : p.min_p0, 0.0), 1.0) * (double)kOne;
+    least = (u64)ceil(fmin(fmax(p.min_p != nullptr ? p.min_p[row] : p.min_p0, 0.0), 1.0) * (double)kOne);
     top_k = p.top_k != nullptr ? p.top_k[row] : p.top_k0;
     u = p.u[row];
   }
@@ -123,10 +126,6 @@ struct Settings {
   }
 };
 
-__device__ __forceinline__ float load_logit(const SampleParams& p, int row, int i) {
-  return p.bf16 ? ssm::to_f32(static_cast<const __nv_bfloat16*>(p.logits)[row * p.stride + i])
-                : static_cast<const float*>(p.logits)[row * p.stride + i];
-}
 // The rank of a logit as it came: a NaN above all.
 __device__ __forceinline__ u64 raw_key(float l, int i) { return l != l ? ~0ull : rank_key(l, i); }
 __device__ __forceinline__ int key_token(u64 key) { return (int)(0xffffffffu - (uint32_t)key); }
@@ -188,14 +187,13 @@ __device__ __forceinline__ u64 block_sort(u64 v, u64* buf, int n) {
   return v;
 }
 
-// Up to kList tokens, one to a thread.
-__global__ void __launch_bounds__(kList) sample_few(const __grid_constant__ SampleParams p) {
-  __shared__ u64 part[32], buf[kList];
-  __shared__ double table[kTable];
+// Up to kFew tokens, one to a thread.
+template <typename T>
+__global__ void __launch_bounds__(kFew) sample_few(const __grid_constant__ SampleParams p) {
+  __shared__ u64 part[32], buf[kFew];
   const int row = (int)blockIdx.x, i = threadIdx.x;
   const Settings set(p, row);
-  if (i < kTable) table[i] = exp2((double)i / kTable);
-  const float l = i < p.V ? load_logit(p, row, i) : 0.0f;
+  const float l = i < p.V ? ssm::to_f32(static_cast<const T*>(p.logits)[row * p.stride + i]) : 0.0f;
   u64 key = i < p.V ? raw_key(l, i) : 0;
   const u64 best = block_max(key, part);
   const bool none = no_token(best, set.temperature);
@@ -203,57 +201,85 @@ __global__ void __launch_bounds__(kList) sample_few(const __grid_constant__ Samp
     if (i == 0) p.token[row] = none ? -1 : key_token(best);
     return;
   }
-  const Weights weight{table, key_logit(best), 1.4426950408889634 / set.temperature};
+  const double top = key_logit(best), rate = 1.4426950408889634 / set.temperature;
+  auto weight = [&](float v) {                            // as in Weights, by the library's function: no table to make
+    const double y = ((double)v - top) * rate;
+    return v == key_logit(best) ? kOne : y > -60.0 ? (u64)__double2ll_rn(exp2(y) * (double)kOne) : 0;
+  };
   u64 total, w = 0;
   const bool top_k = set.top_k > 0 && set.top_k < p.V;
   if (top_k || set.top_p < 1.0) {
     key = block_sort(key, buf, (int)blockDim.x);
-    const double exact = key != 0 && (!top_k || i < set.top_k) ? weight(key_logit(key)) : 0.0;
-    w = units(exact);
+    w = key != 0 && (!top_k || i < set.top_k) ? weight(key_logit(key)) : 0;
     const u64 run = block_scan(w, part, &total);
-    if (key != 0) buf[key_token(key)] = run - w < set.reach(total) && exact >= set.least ? w : 0;
+    if (key != 0) buf[key_token(key)] = run - w < set.reach(total) && w >= set.least ? w : 0;
     __syncthreads();
     w = i < p.V ? buf[i] : 0;
   } else if (i < p.V) {
-    const double exact = weight(l);
-    w = exact >= set.least ? units(exact) : 0;
+    w = weight(l);
+    if (w < set.least) w = 0;
   }
   const u64 run = block_scan(w, part, &total), target = set.draw(total);
   if (run > target && run - w <= target) p.token[row] = i;
 }
 
 // ---- a cluster's threads, many tokens each --------------------------------------------------------------
+template <typename T>
 struct Sampler {
   const SampleParams& p;
   SampleSmem& s;
   cg::cluster_group cluster;
-  int row, ctas, lane, warp, base, first, last, turn;
+  const T* logits;                    // of the row
+  int row, ctas, lane, warp, base, per, first, last, turn;
   Weights weight;
   float bin_rate;                     // bins to a logit
 
   __device__ Sampler(const SampleParams& p_, SampleSmem& s_) : p(p_), s(s_), cluster(cg::this_cluster()), turn(0) {
     ctas = (int)cluster.num_blocks();
     row = (int)blockIdx.x / ctas;
+    logits = static_cast<const T*>(p.logits) + row * p.stride;
     lane = threadIdx.x & 31;
     warp = threadIdx.x >> 5;
-    // a warp's tokens are neighbours, so that warps in order are tokens in order
+    // a warp's tokens are neighbours, so that warps in order are tokens in order; four to a lane and step
     base = min(p.V, (int)cluster.block_rank() * p.slice);
-    const int end = min(p.V, base + p.slice), per = ((end - base + 31) / 32 + 31) & ~31;
+    const int end = min(p.V, base + p.slice);
+    per = ((end - base + kWarps - 1) / kWarps + 127) & ~127;
     first = min(end, base + warp * per);
     last = min(end, first + per);
     weight.table = s.exp2;
   }
-  __device__ float logit(int i) const { return p.cached ? s.logits[i - base] : load_logit(p, row, i); }
+  // Four logits from i on; -inf past the warp's last.
+  __device__ void load(int i, float (&l)[4]) const {
+    if (p.wide && i + 4 <= last) {
+      ssm::load4(logits + i, l);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) l[j] = i + j < last ? ssm::to_f32(logits[i + j]) : -__int_as_float(0x7f800000);
+    }
+  }
+  // f(i, l[4]) for this lane's tokens
+  template <typename F>
+  __device__ __forceinline__ void each(F f) {
+    for (int i = first + 4 * lane; i < last; i += 128) {
+      float l[4];
+      if (p.cached) ssm::load4(s.logits + (i - base), l);
+      else load(i, l);
+      f(i, l);
+    }
+  }
 
-  // The sum (or maximum) over the cluster's threads, for all of them.
-  template <bool MAX>
+  // The sum (or maximum, or HALVES: the maxima of the two halves) over the cluster's threads, for all of them.
+  template <bool MAX, bool HALVES = false>
   __device__ u64 join(u64 v) {
-    auto f = [](u64 a, u64 b) { return MAX ? max(a, b) : a + b; };
+    auto f = [](u64 a, u64 b) {
+      if (HALVES) return (u64)max((uint32_t)(a >> 32), (uint32_t)(b >> 32)) << 32 | max((uint32_t)a, (uint32_t)b);
+      return MAX ? max(a, b) : a + b;
+    };
 #pragma unroll
     for (int m = 16; m >= 1; m /= 2) v = f(v, __shfl_xor_sync(0xffffffffu, v, m));
     if (lane == 0) s.part[warp] = v;
     __syncthreads();
-    v = s.part[lane];
+    v = lane < kWarps ? s.part[lane] : 0;
 #pragma unroll
     for (int m = 16; m >= 1; m /= 2) v = f(v, __shfl_xor_sync(0xffffffffu, v, m));
     if (ctas == 1) {
@@ -266,6 +292,23 @@ struct Sampler {
     for (int r = 0; r < ctas; ++r) v = f(v, *cluster.map_shared_rank(&s.slot[turn], r));
     turn ^= 1;
     return v;
+  }
+  // Two sums at once.
+  __device__ void join2(u64& x, u64& y) {
+    u64 all;
+    block_scan(x, s.part, &all);
+    x = all;
+    block_scan(y, s.part, &all);
+    y = all;
+    if (ctas == 1) return;
+    if (threadIdx.x == 0) s.slot[turn] = x, s.slot2[turn] = y;
+    cluster.sync();
+    x = y = 0;
+    for (int r = 0; r < ctas; ++r) {
+      x += *cluster.map_shared_rank(&s.slot[turn], r);
+      y += *cluster.map_shared_rank(&s.slot2[turn], r);
+    }
+    turn ^= 1;
   }
   __device__ void sync() {
     if (ctas == 1) __syncthreads();
@@ -283,10 +326,11 @@ struct Sampler {
   __device__ u64 above(u64 cut, u64 key) {
     u64 n = 0;
     const u64 least = max(cut, key);
-    for (int i = first + lane; i < last; i += 32) {
-      const float l = logit(i);
-      if (rank_key(l, i) >= least) n += MASS ? units(weight(l)) : 1;
-    }
+    each([&](int i, const float (&l)[4]) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (i + j < last && rank_key(l[j], i + j) >= least) n += MASS ? weight(l[j]) : 1;
+    });
     return join<false>(n);
   }
   // The key of the token, by rank, at which the count (or weight) of those that rank at least as high as `cut`
@@ -302,40 +346,50 @@ struct Sampler {
     return lo;
   }
 
-  // Every bin's count over the cluster, in registers: bins 2 t and 2 t + 1 of thread t.
-  __device__ void count_bins(uint32_t (&n)[2]) {
-    for (int b = threadIdx.x; b < kBins; b += kList) s.count[b] = 0;
+  // Every bin's count over the cluster, in registers: kPer bins to a thread.
+  __device__ void count_bins(uint32_t (&n)[kPer]) {
+    for (int b = threadIdx.x; b < kBins; b += kThreads) s.count[b] = 0;
     if (threadIdx.x < 1 + 2 * kMargins) s.first[threadIdx.x] = kBins - 1;
     if (threadIdx.x == 0) s.size = 0;
     __syncthreads();
-    for (int i = first + lane; i < last; i += 32) {
-      const int b = bin(logit(i));
-      if (b < kBins) atomicAdd(&s.count[b], 1u);
-    }
+    each([&](int, const float (&l)[4]) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int b = bin(l[j]);
+        if (b < kBins) atomicAdd(&s.count[b], 1u);
+      }
+    });
     sync();
-    n[0] = n[1] = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) n[i] = 0;
     for (int r = 0; r < ctas; ++r) {
-      const uint2 c = *reinterpret_cast<const uint2*>(cluster.map_shared_rank(s.count, r) + 2 * threadIdx.x);
+      const uint4 c = *reinterpret_cast<const uint4*>(cluster.map_shared_rank(s.count, r) + kPer * threadIdx.x);
       n[0] += c.x;
       n[1] += c.y;
+      n[2] += c.z;
+      n[3] += c.w;
     }
   }
-  // The tokens of bins lo .. hi that rank at least as high as `cut`, in the first CTA's list (in any order); f(l, bin,
-  // in) is called for each token.
+  // The tokens of bins lo .. hi that rank at least as high as `cut`, in the first CTA's list (in any order); f(l, bin, in)
+  // for four tokens at a time, `in` where they rank so.
   template <typename F>
   __device__ void gather(int lo, int hi, u64 cut, F f) {
     int* size = cluster.map_shared_rank(&s.size, 0);
     u64* list = cluster.map_shared_rank(s.list, 0);
-    for (int i = first + lane; i < last; i += 32) {
-      const float l = logit(i);
-      const int b = bin(l);
-      const u64 key = rank_key(l, i);
-      if (b >= lo && b <= hi && key >= cut) {
-        const int at = atomicAdd(size, 1);
-        if (at < kList) list[at] = key;
+    each([&](int i, const float (&l)[4]) {
+      int b[4];
+      bool in[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        b[j] = bin(l[j]);
+        in[j] = b[j] < kBins && (cut == 0 || rank_key(l[j], i + j) >= cut);
+        if (b[j] >= lo && b[j] <= hi && in[j]) {
+          const int at = atomicAdd(size, 1);
+          if (at < kList) list[at] = rank_key(l[j], i + j);
+        }
       }
-      f(l, b, key);
-    }
+      f(l, b, in);
+    });
   }
   // This thread's token of the first CTA's list, largest first (0: none); for all CTAs of the cluster to call.
   __device__ u64 sorted() {
@@ -349,86 +403,97 @@ struct Sampler {
   }
 };
 
-__global__ void __launch_bounds__(kList) sample_many(const __grid_constant__ SampleParams p) {
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 2) sample_many(const __grid_constant__ SampleParams p) {
   extern __shared__ __align__(16) unsigned char raw[];
   SampleSmem& s = *reinterpret_cast<SampleSmem*>(raw);
-  Sampler a(p, s);
+  Sampler<T> a(p, s);
   const Settings set(p, a.row);
   const int t = threadIdx.x;
   const bool leader = a.cluster.block_rank() == 0;
-  if (t < kTable) s.exp2[t] = exp2((double)t / kTable);
-  u64 best = 0, worst = 0;                                // the lowest as the highest of the negated
-  const float inf = __int_as_float(0x7f800000);
+  for (int i = t; i < kTable; i += kThreads) s.exp2[i] = exp2((double)i / kTable);
+  constexpr float kInf = __builtin_huge_valf();
+  float high = -kInf, low = kInf;                         // of the logits above -inf
+  bool nan = false;
 #pragma unroll 4
-  for (int i = a.first + a.lane; i < a.last; i += 32) {
-    const float l = load_logit(p, a.row, i);
-    if (p.cached) s.logits[i - a.base] = l;
-    best = max(best, raw_key(l, i));
-    if (l != -inf) worst = max(worst, raw_key(-l, i));
+  for (int i = a.first + 4 * a.lane; i < a.last; i += 128) {
+    float l[4];
+    a.load(i, l);
+    if (p.cached) *reinterpret_cast<float4*>(s.logits + (i - a.base)) = make_float4(l[0], l[1], l[2], l[3]);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      high = fmaxf(high, l[j]);
+      low = fminf(low, l[j] > -kInf ? l[j] : kInf);
+      nan |= l[j] != l[j];
+    }
   }
-  best = a.join<true>(best);
-  const bool none = no_token(best, set.temperature);
+  // both in one: the largest, and the smallest as the largest of the negated
+  const u64 ends = a.template join<true, true>(nan ? ~0ull : (rank_key(high, 0) >> 32) << 32 | rank_key(-low, 0) >> 32);
+  const bool none = no_token(ends, set.temperature);
+  a.weight.top = key_logit(ends);
   if (none || !(set.temperature > 0.0)) {                 // the same for the whole cluster
+    u64 best = 0;
+    if (!none)
+      a.each([&](int i, const float (&l)[4]) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (i + j < a.last) best = max(best, rank_key(l[j], i + j));
+      });
+    best = a.template join<true>(best);
     if (t == 0 && leader) p.token[a.row] = none ? -1 : key_token(best);
     a.sync();                                             // peers read this CTA's slots until here
     return;
   }
-  a.weight.top = key_logit(best);
+  a.weight.top2 = a.weight.top;
   a.weight.rate = 1.4426950408889634 / set.temperature;
   const bool top_k = set.top_k > 0 && set.top_k < p.V, top_p = set.top_p < 1.0;
   u64 cut = 0;
+  bool summed = false;                                    // s.kept is known
   if (top_k || top_p) {
-    worst = a.join<true>(worst);
     // 31 temperatures below the largest a weight is zero
-    const float range = fminf(31.0f * (float)set.temperature, a.weight.top + key_logit(worst));
+    const float range = fminf(31.0f * (float)set.temperature, a.weight.top + key_logit(ends << 32));
     a.bin_rate = ((float)kBins - 0.01f) / range;
-    uint32_t n[2];
+    uint32_t n[kPer];
     a.count_bins(n);
-    u64 all;
-    const u64 count1 = block_scan((u64)n[0] + n[1], s.part, &all), count0 = count1 - n[1];   // up to bin 2 t + 1, 2 t
+    u64 all, run = block_scan((u64)n[0] + n[1] + n[2] + n[3], s.part, &all) - n[0] - n[1] - n[2] - n[3];
+    const int b0 = kPer * t;                              // this thread's first bin
     int last = kBins - 1;                                 // the bin of the top_k-th token
-    u64 listed = all;                                     // tokens up to it
-    if (top_k && (u64)set.top_k < all) {
-      const u64 k = (u64)set.top_k;
-      if (count1 >= k && count1 - n[0] - n[1] < k) s.first[0] = count0 >= k ? 2 * t : 2 * t + 1;
-      __syncthreads();
-      last = s.first[0];
-      if (last >> 1 == t) s.slot[a.turn] = last & 1 ? count1 : count0;
-      __syncthreads();
-      listed = s.slot[a.turn];
-      __syncthreads();
+    const bool borders = top_k && (u64)set.top_k < all;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      if (borders && run < (u64)set.top_k && run + n[i] >= (u64)set.top_k) s.first[0] = b0 + i;
+      s.upto[b0 + i] = (uint32_t)(run += n[i]);
     }
+    __syncthreads();
+    if (borders) last = s.first[0];
+    const int listed = (int)s.upto[last];                 // tokens up to it
     if (listed <= kList) {                                // what is kept of the top_k: all in the list
-      a.gather(0, last, 0, [](float, int, u64) {});
+      a.gather(0, last, 0, [](const float (&)[4], const int (&)[4], const bool (&)[4]) {});
       u64 key = a.sorted();
       a.sync();
       if (!leader) return;
       const long long k = top_k ? set.top_k : p.V;
-      const double exact = key != 0 && t < k ? a.weight(key_logit(key)) : 0.0;
-      u64 w = units(exact), total;
-      u64 run = block_scan(w, s.part, &total);
+      u64 w = key != 0 && t < k ? a.weight(key_logit(key)) : 0, total;
+      run = block_scan(w, s.part, &total);
       // by index: the token in the high half, its logit's order in the low one
-      key = w != 0 && run - w < set.reach(total) && exact >= set.least ? key << 32 | key >> 32 : 0;
+      key = w != 0 && run - w < set.reach(total) && w >= set.least ? key << 32 | key >> 32 : 0;
       int pow2 = 32;
-      while (pow2 < (int)listed) pow2 *= 2;
+      while (pow2 < listed) pow2 *= 2;
       key = block_sort(key, s.list, pow2);
-      w = key != 0 ? units(a.weight(key_logit(key << 32 | key >> 32))) : 0;
+      w = key != 0 ? a.weight(key_logit(key << 32 | key >> 32)) : 0;
       run = block_scan(w, s.part, &total);
       const u64 target = set.draw(total);
       if (run > target && run - w <= target) p.token[a.row] = key_token(key >> 32);
       return;
     }
-    if (top_k && (u64)set.top_k < all) {                  // the border of top_k lies in bin `last`
-      if (last >> 1 == t) s.slot[a.turn] = last & 1 ? count0 : count0 - n[0];
-      __syncthreads();
-      const u64 before = s.slot[a.turn];
-      __syncthreads();
+    if (borders) {                                        // the border of top_k lies in bin `last`
+      const int before = last > 0 ? (int)s.upto[last - 1] : 0;
       if (listed - before > kList) {
-        cut = a.bisect<false>(0, (u64)set.top_k);
+        cut = a.template bisect<false>(0, (u64)set.top_k);
       } else {
-        a.gather(last, last, 0, [](float, int, u64) {});
+        a.gather(last, last, 0, [](const float (&)[4], const int (&)[4], const bool (&)[4]) {});
         const u64 key = a.sorted();
-        if (leader && t == (int)((u64)set.top_k - before) - 1) s.cut = key;
+        if (leader && t == (int)set.top_k - before - 1) s.cut = key;
         a.sync();
         cut = *a.cluster.map_shared_rank(&s.cut, 0);
         if (t == 0) s.size = 0;
@@ -438,73 +503,98 @@ __global__ void __launch_bounds__(kList) sample_many(const __grid_constant__ Sam
     if (top_p) {
       // the bins' masses, about: as many weights as it has tokens, from its middle
       const float step = range / ((float)kBins - 0.01f) / (float)set.temperature;
-      const int b = 2 * t;
-      const float m0 = b <= last ? (float)n[0] * __expf(-step * ((float)b + 0.5f)) : 0.0f;
-      const float m1 = b < last ? (float)n[1] * __expf(-step * ((float)b + 1.5f)) : 0.0f;
-      u64 mass;
-      const u64 unit0 = (u64)(m0 * 16777216.0f), unit1 = (u64)(m1 * 16777216.0f);
-      const u64 run1 = block_scan(unit0 + unit1, s.part, &mass), run0 = run1 - unit1, run = run0 - unit0;
-      // the bins between (top_p - margin) and (top_p + margin) of the mass, for the widest margin whose tokens fit
-      const double margins[kMargins] = {0.008, 0.001, 0.0001, 0.0};
-      auto mark = [&](int at, u64 value) {                // the first bin at which the sum is above `value`
-        if (run <= value && run1 > value) s.first[at] = run0 > value ? b : b + 1;
-      };
+      u64 unit[kPer], mass, upto = 0;
 #pragma unroll
-      for (int i = 0; i < kMargins; ++i) {
-        mark(1 + 2 * i, (u64)fmax(0.0, (set.top_p - margins[i]) * (double)mass));
-        mark(2 + 2 * i, (u64)fmax(0.0, (set.top_p + margins[i]) * (double)mass));
+      for (int i = 0; i < kPer; ++i) {
+        if (borders && b0 + i == last) n[i] = (uint32_t)set.top_k - (last > 0 ? s.upto[last - 1] : 0);
+        unit[i] = b0 + i <= last ? (u64)((float)n[i] * __expf(-step * ((float)(b0 + i) + 0.5f)) * 16777216.0f) : 0;
+        upto += unit[i];
       }
-      // tokens up to every bin; the histogram's own counts are not needed again
-      a.sync();
-      s.count[b] = (uint32_t)count0;
-      s.count[b + 1] = (uint32_t)count1;
+      upto = block_scan(upto, s.part, &mass) - upto;      // before the first of this thread's bins
+      // the first bin at which the sum is above (top_p - margin), and (top_p + margin), of the mass
+      const double margins[kMargins] = {0.008, 0.001, 0.0001, 0.0};
+#pragma unroll
+      for (int i = 0; i < 2 * kMargins; ++i) {
+        const double share = set.top_p + (i & 1 ? margins[i / 2] : -margins[i / 2]);
+        const u64 value = (u64)fmax(0.0, share * (double)mass);
+        u64 at = upto;
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+          if (at <= value && at + unit[j] > value) s.first[1 + i] = b0 + j;
+          at += unit[j];
+        }
+      }
       __syncthreads();
-      int lo = 0, hi = 0;
-      bool fits = false;
-      for (int i = 0; i < kMargins && !fits; ++i) {
-        lo = s.first[1 + 2 * i];
-        hi = min(last, s.first[2 + 2 * i]);
-        fits = s.count[hi] - (lo > 0 ? s.count[lo - 1] : 0) <= kList;
-      }
-      u64 total = 0, before = 0;
-      if (fits) {
-        a.gather(lo, hi, cut, [&](float l, int bin, u64 key) {
-          if (bin >= kBins || key < cut) return;
-          const u64 w = units(a.weight(l));
-          total += w;
-          if (bin < lo) before += w;
+      // the widest margin with few tokens; where the border is not between them after all, with as many as fit
+      bool found = false;
+      u64 total = 0;
+      for (int most = kList / 4; most <= kList && !found; most *= 4) {
+        int lo = 0, hi = 0;
+        bool fits = false;
+        for (int i = 0; i < kMargins && !fits; ++i) {
+          lo = s.first[1 + 2 * i];
+          hi = min(last, s.first[2 + 2 * i]);
+          fits = (int)(s.upto[hi] - (lo > 0 ? s.upto[lo - 1] : 0)) <= most;
+        }
+        if (!fits) continue;
+        total = 0;
+        u64 before = 0;
+        a.gather(lo, hi, cut, [&](const float (&l)[4], const int (&bin)[4], const bool (&in)[4]) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const u64 w = a.weight(l[j]);
+            total += in[j] ? w : 0;
+            before += in[j] && bin[j] < lo ? w : 0;
+          }
         });
-        const u64 key = a.sorted();
-        total = a.join<false>(total);
-        before = a.join<false>(before);
-        const u64 reach = set.reach(total), w = key != 0 ? units(a.weight(key_logit(key))) : 0;
+        u64 mine = before;                                // of this warp
+#pragma unroll
+        for (int m = 16; m >= 1; m /= 2) mine += __shfl_xor_sync(0xffffffffu, mine, m);
+        if (a.lane == 0) s.kept[a.warp] = mine;
+        u64 key = a.sorted();
+        a.join2(total, before);
+        const u64 reach = set.reach(total), w = key != 0 ? a.weight(key_logit(key)) : 0;
         u64 sum;
-        const u64 upto = before + block_scan(w, s.part, &sum);
+        upto = before + block_scan(w, s.part, &sum);
         // the border is in the list: the last token that the sum before it leaves short
-        if (t == 0) s.cut = 0;
+        if (t == 0) s.cut = s.size = 0;
+        s.list[t] = key;
         __syncthreads();
         if (leader && key != 0 && upto - w < reach && upto >= reach) s.cut = key;
         a.sync();
-        const u64 found = *a.cluster.map_shared_rank(&s.cut, 0);
-        fits = found != 0;
-        if (fits) cut = found;
-      } else {
-        total = a.above<true>(cut, 0);
+        const u64 border = *a.cluster.map_shared_rank(&s.cut, 0);
+        found = border != 0;
+        if (found) {
+          cut = border;
+          key = a.cluster.map_shared_rank(s.list, 0)[t];
+          const int at = key_token(key) - a.base;
+          if (key >= cut && at >= 0 && at < p.slice) atomicAdd(&s.kept[at / a.per], a.weight(key_logit(key)));
+          summed = a.weight(key_logit(cut)) >= set.least;  // min_p cuts nothing off
+        }
+        a.sync();
       }
-      if (!fits) cut = max(cut, a.bisect<true>(cut, set.reach(total)));
+      if (!found) {
+        total = a.template above<true>(cut, 0);
+        cut = max(cut, a.template bisect<true>(cut, set.reach(total)));
+      }
     }
   }
-  auto kept = [&](int i) -> u64 {
-    const float l = a.logit(i);
-    if (rank_key(l, i) < cut) return 0;
-    const double w = a.weight(l);
-    return w >= set.least ? units(w) : 0;
+  auto kept = [&](int i, float l) -> u64 {
+    const u64 w = a.weight(l);
+    return i < a.last && (cut == 0 || rank_key(l, i) >= cut) && w >= set.least ? w : 0;
   };
   u64 sum = 0;
-  for (int i = a.first + a.lane; i < a.last; i += 32) sum += kept(i);
-  // what the warps and CTAs before have
+  if (summed) {
+    sum = s.kept[a.warp];
+  } else {
+    a.each([&](int i, const float (&l)[4]) {
 #pragma unroll
-  for (int m = 16; m >= 1; m /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, m);
+      for (int j = 0; j < 4; ++j) sum += kept(i + j, l[j]);
+    });
+#pragma unroll
+    for (int m = 16; m >= 1; m /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, m);
+  }
+  // what the warps and CTAs before have
   u64 cta;
   u64 before = block_scan(a.lane == 31 ? sum : 0, s.part, &cta), total = cta;
   before = __shfl_sync(0xffffffffu, before, 31) - sum;
@@ -520,8 +610,21 @@ __global__ void __launch_bounds__(kList) sample_many(const __grid_constant__ Sam
   }
   const u64 target = set.draw(total);
   if (before <= target && target < before + sum) {        // one warp of the cluster
-    for (int i0 = a.first; i0 < a.last; i0 += 32) {
-      u64 run = i0 + a.lane < a.last ? kept(i0 + a.lane) : 0;
+    for (int i0 = a.first; i0 < a.last; i0 += 128) {
+      const int i = i0 + 4 * a.lane;
+      float l[4];
+      if (i >= a.last) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) l[j] = -kInf;
+      } else if (p.cached) {
+        ssm::load4(s.logits + (i - a.base), l);
+      } else {
+        a.load(i, l);
+      }
+      u64 w[4], mine = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) mine += w[j] = kept(i + j, l[j]);
+      u64 run = mine;
 #pragma unroll
       for (int m = 1; m < 32; m *= 2) {
         const u64 up = __shfl_up_sync(0xffffffffu, run, m);
@@ -529,7 +632,12 @@ __global__ void __launch_bounds__(kList) sample_many(const __grid_constant__ Sam
       }
       const uint32_t passed = __ballot_sync(0xffffffffu, before + run > target);
       if (passed != 0) {
-        if (a.lane == 0) p.token[a.row] = i0 + __ffs(passed) - 1;
+        if (a.lane == __ffs(passed) - 1) {
+          u64 at = before + run - mine;
+          int j = 0;
+          while (j < 3 && at + w[j] <= target) at += w[j++];
+          p.token[a.row] = i + j;
+        }
         break;
       }
       before += __shfl_sync(0xffffffffu, run, 31);
@@ -544,7 +652,8 @@ int fail(int code, const char* fmt, long long a = 0, long long b = 0) {
   snprintf(msg, sizeof(msg), fmt, a, b);
   return ssm::report_error(code, msg);
 }
-constexpr int kCached = 48 * 1024;    // logits that a CTA keeps
+constexpr int kCached = 45 * 1024;    // logits that a CTA keeps (180 KB)
+constexpr int kTwo = 19 * 1024;       // logits that each of two CTAs on an SM keeps
 
 }  // namespace
 
@@ -574,23 +683,28 @@ extern "C" int ssm_sample_tokens(int64_t B, int64_t V, ssm_view logits, const fl
   p.token = reinterpret_cast<long long*>(tokens);
   p.V = (int)V;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (V <= kList) {
-    int threads = kTable;                                  // a power of two: one token to a thread
+  if (V <= kFew) {
+    int threads = 64;                                      // a power of two: one token to a thread
     while (threads < V) threads *= 2;
-    sample_few<<<(unsigned)B, threads, 0, st>>>(p);
+    if (p.bf16) sample_few<__nv_bfloat16><<<(unsigned)B, threads, 0, st>>>(p);
+    else sample_few<float><<<(unsigned)B, threads, 0, st>>>(p);
     const cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? SSM_OK : fail(SSM_ERR_CUDA, "sample_tokens launch failed (error %lld)", (long long)e);
   }
-  // CTAs to a row: what keeps the slices in shared memory, and more where few rows leave SMs idle
+  // CTAs to a row: what lets two on an SM keep their slices in shared memory, and more where few rows leave SMs idle
   int ctas = 1;
-  while (ctas < 8 && V > (int64_t)ctas * kCached) ctas *= 2;
-  while (ctas < 8 && V >= (int64_t)ctas * 8192 && B * ctas * 2 <= 148) ctas *= 2;
-  p.slice = (int)((V + ctas - 1) / ctas);
+  while (ctas < 8 && V > (int64_t)ctas * kTwo) ctas *= 2;
+  while (ctas < 8 && V >= (int64_t)ctas * 4096 && B * ctas * 2 <= 148) ctas *= 2;
+  p.slice = (int)((V + ctas - 1) / ctas + 3) & ~3;
   p.cached = p.slice <= kCached;
-  ssm::ctas_per_sm<sample_many>(kList, sizeof(SampleSmem) + kCached * sizeof(float));
+  const int unit = p.bf16 ? 8 : 16;                        // bytes of four logits
+  p.wide = reinterpret_cast<uintptr_t>(p.logits) % unit == 0 && p.stride % 4 == 0;
+  const size_t most = sizeof(SampleSmem) + kCached * sizeof(float);
+  if (p.bf16) ssm::ctas_per_sm<sample_many<__nv_bfloat16>>(kThreads, most);
+  else ssm::ctas_per_sm<sample_many<float>>(kThreads, most);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(B * ctas));
-  cfg.blockDim = dim3(kList);
+  cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = sizeof(SampleSmem) + (p.cached ? p.slice * sizeof(float) : 0);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
@@ -599,6 +713,7 @@ extern "C" int ssm_sample_tokens(int64_t B, int64_t V, ssm_view logits, const fl
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, sample_many, p);
+  const cudaError_t e = p.bf16 ? cudaLaunchKernelEx(&cfg, sample_many<__nv_bfloat16>, p)
+                                : cudaLaunchKernelEx(&cfg, sample_many<float>, p);
   return e == cudaSuccess ? SSM_OK : fail(SSM_ERR_CUDA, "sample_tokens launch failed (error %lld)", (long long)e);
 }
