@@ -2,8 +2,8 @@
 //
 //   y[t] = scale W[idx[t]],   dW[v] = scale sum over t with idx[t] = v of dy[t]
 // Both directions are bound by memory: the rows that are read and written.  The gradient's places are sorted by token
-// (stable, so that a token's places stay in order), cut into chunks of equal length whatever the tokens' frequencies,
-// and summed chunk by chunk: fp32 within a chunk, fp64 over the chunks that a frequent token spans.  No atomics on
+// (stable, so that a token's places stay in order), cut into chunks of nearly equal length whatever the tokens'
+// frequencies, and summed chunk by chunk: fp32 within a chunk, fp64 over the chunks that a frequent token spans.  No atomics on
 // floats, a fixed order: results are reproducible.  Rows that no token names are zeroed by CTAs of the same launch.
 //
 // A token outside 0 .. V-1 gives a row of NaN and no gradient, and sets bit 1 of the device error word.
@@ -48,6 +48,8 @@ struct EmbedParams {
   long long chunks;
   int len;                          // places to a chunk
   int slabs;                        // CTAs over the channels
+  int* joins;                       // how many chunks a run goes on from, then which
+  uint32_t* named;                  // a bit for every token: it occurs
 };
 
 __device__ __forceinline__ long long token_at(const EmbedParams& p, long long t) {
@@ -98,7 +100,7 @@ __global__ void __launch_bounds__(256) embed_fwd(const __grid_constant__ EmbedPa
 // ---- places by token ----------------------------------------------------------------------------
 // A stable radix sort, kDigit bits a pass, by one cluster: with a launch a step it would be six launches.  A warp
 // owns consecutive places; counts are kept by warp, so that its places land in order behind those of the warps before it.
-constexpr int kDigit = 9, kBins = 1 << kDigit, kSortWarps = 32;
+constexpr int kDigit = 9, kBins = 1 << kDigit, kSortWarps = 32, kHeld = 8;
 struct SortSmem {
   uint32_t count[kSortWarps][kBins];   // by warp: counts, then where its next place of a bin goes
   uint32_t total[kBins];               // of this CTA
@@ -112,6 +114,9 @@ __global__ void __launch_bounds__(1024) embed_sort(const __grid_constant__ Embed
   cg::cluster_group cluster = cg::this_cluster();
   const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (rank == 0 && threadIdx.x == 0) p.joins[0] = 0;
+  for (long long w = rank * 1024 + threadIdx.x; w < (p.V + 31) / 32; w += ctas * 1024) p.named[w] = 0;
+  cluster.sync();
   // places of this warp: a multiple of 32 to each
   const long long per = ((p.T + ctas * kSortWarps - 1) / (ctas * kSortWarps) + 31) / 32 * 32;
   const long long first = min(p.T, (long long)(rank * kSortWarps + warp) * per), last = min(p.T, first + per);
@@ -124,9 +129,28 @@ __global__ void __launch_bounds__(1024) embed_sort(const __grid_constant__ Embed
       const long long v = token_at(p, t);
       return make_uint2((uint32_t)(v < 0 || v >= p.V ? p.V : v), (uint32_t)t);
     };
-    for (int i = threadIdx.x; i < kSortWarps * kBins; i += 1024) (&s.count[0][0])[i] = 0;
+    // up to kHeld places a lane stay in registers, loaded at once
+    const bool held = per <= 32 * kHeld;
+    uint2 x[kHeld];
+    if (held) {
+#pragma unroll
+      for (int i = 0; i < kHeld; ++i)
+        if (first + 32 * i + lane < last) x[i] = item(first + 32 * i + lane);
+    }
+    for (int i = threadIdx.x; i < kSortWarps * kBins / 4; i += 1024) reinterpret_cast<uint4*>(s.count)[i] = make_uint4(0, 0, 0, 0);
     __syncthreads();
-    for (long long t = first + lane; t < last; t += 32) atomicAdd(&s.count[warp][item(t).x >> shift & (kBins - 1)], 1u);
+    auto count = [&](uint32_t token) {
+      atomicAdd(&s.count[warp][token >> shift & (kBins - 1)], 1u);
+      if (pass == 0 && token < p.V) atomicOr(p.named + (token >> 5), 1u << (token & 31));
+    };
+    if (held) {
+#pragma unroll
+      for (int i = 0; i < kHeld; ++i)
+        if (first + 32 * i + lane < last) count(x[i].x);
+    } else {
+#pragma unroll 4
+      for (long long t = first + lane; t < last; t += 32) count(item(t).x);
+    }
     __syncthreads();
     // by bin: this CTA's total
     uint32_t mine = 0;
@@ -161,16 +185,25 @@ __global__ void __launch_bounds__(1024) embed_sort(const __grid_constant__ Embed
       }
     }
     __syncthreads();
-    for (long long t0 = first; t0 < last; t0 += 32) {
-      const bool live = t0 + lane < last;
-      const uint2 x = live ? item(t0 + lane) : make_uint2(0, 0);
-      const uint32_t bin = live ? x.x >> shift & (kBins - 1) : kBins;      // lanes past the end share a bin of their own
+    auto place = [&](bool live, uint2 v) {
+      const uint32_t bin = live ? v.x >> shift & (kBins - 1) : kBins;      // lanes past the end share a bin of their own
       const uint32_t same = __match_any_sync(0xffffffffu, bin);
-      const uint32_t place = live ? s.count[warp][bin] + __popc(same & ((1u << lane) - 1)) : 0;
+      const uint32_t to = live ? s.count[warp][bin] + __popc(same & ((1u << lane) - 1)) : 0;
       __syncwarp();
       if (live && lane == __ffs(same) - 1) s.count[warp][bin] += __popc(same);
       __syncwarp();
-      if (live) dst[place] = x;
+      if (live) dst[to] = v;
+    };
+    if (held) {
+#pragma unroll
+      for (int i = 0; i < kHeld; ++i)
+        if (first + 32 * i < last) place(first + 32 * i + lane < last, x[i]);
+    } else {
+#pragma unroll 2
+      for (long long t0 = first; t0 < last; t0 += 32) {
+        const bool live = t0 + lane < last;
+        place(live, live ? item(t0 + lane) : make_uint2(0, 0));
+      }
     }
     __threadfence();
     cluster.sync();                                    // the next pass reads what every CTA wrote, and counts anew
@@ -178,42 +211,53 @@ __global__ void __launch_bounds__(1024) embed_sort(const __grid_constant__ Embed
 }
 
 // ---- sums of the sorted places ---------------------------------------------------------------------
-constexpr int kSumThreads = 128, kLongest = 64, kRows = 8, kFill = 32;
+constexpr int kSumThreads = 256, kLongest = 64, kRows = 8, kFill = 32;      // kFill: a word of `named`
 
+// Chunk q starts at the first place from q len on where another token begins, or at q len inside a run of more than len.
 // The sum of a run of equal tokens goes to the table where the chunk holds all of it, else to the chunk's partial
 // rows: 0 where the run comes from the chunk before, 1 where it starts here and goes on.
 template <typename T, int VEC>
 __global__ void __launch_bounds__(kSumThreads) embed_sum(const __grid_constant__ EmbedParams p) {
-  __shared__ uint2 at[kLongest];
-  __shared__ uint32_t outer[2];                        // the tokens before and behind the chunk
-  const int c = ((int)(blockIdx.x % p.slabs) * kSumThreads + threadIdx.x) * VEC;
-  const long long chunk = blockIdx.x / p.slabs;
+  __shared__ uint2 near[2 * kLongest + 1];             // from the place before the chunk's first possible one
+  __shared__ int bound[2];
+  const int c = ((int)(blockIdx.x % p.slabs) * blockDim.x + threadIdx.x) * VEC;
+  const long long item = blockIdx.x / p.slabs;
   constexpr uint32_t kNone = 0xffffffffu;
-  if (chunk >= p.chunks) {                             // rows without a token
-    const long long v0 = (chunk - p.chunks) * kFill;
-    if (threadIdx.x < kFill) {
-      const long long v = v0 + threadIdx.x;
-      long long lo = 0, hi = p.T;                      // the first place whose token is v or above
-      while (lo < hi) {
-        const long long mid = (lo + hi) >> 1;
-        if (p.sorted[mid].x < v) lo = mid + 1;
-        else hi = mid;
-      }
-      at[threadIdx.x].x = v < p.V && (lo == p.T || p.sorted[lo].x != v);
-    }
-    __syncthreads();
+  // Chunks to sum and rows to zero take turns, so that reads and writes mix.
+  const long long fills = (p.V + kFill - 1) / kFill, items = p.chunks + fills;
+  const long long fill = item * fills / items, chunk = item - fill;
+  if ((item + 1) * fills / items > fill) {             // rows without a token
+    const uint32_t named = p.named[fill];
+    const int rows = (int)min((long long)kFill, p.V - fill * kFill);
     const float zero[VEC] = {};
     if (c < p.C)
-      for (int i = 0; i < kFill; ++i)
-        if (at[i].x) vec_store<T, VEC>(static_cast<T*>(p.y) + (v0 + i) * p.ys + c, zero);
+      for (int i = 0; i < rows; ++i)
+        if (!(named >> i & 1)) vec_store<T, VEC>(static_cast<T*>(p.y) + (fill * kFill + i) * p.ys + c, zero);
     return;
   }
   const long long t0 = chunk * p.len;
-  const int n = (int)min((long long)p.len, p.T - t0);
-  if (threadIdx.x < n) at[threadIdx.x] = p.sorted[t0 + threadIdx.x];
-  if (threadIdx.x == 64) outer[0] = t0 > 0 ? p.sorted[t0 - 1].x : kNone;
-  if (threadIdx.x == 65) outer[1] = t0 + n < p.T ? p.sorted[t0 + n].x : kNone;
+  for (int i = threadIdx.x; i < 2 * p.len + 1; i += blockDim.x)
+    near[i] = t0 - 1 + i >= 0 && t0 - 1 + i < p.T ? p.sorted[t0 - 1 + i] : make_uint2(kNone, 0);
   __syncthreads();
+  // where this chunk and the next one start, from t0 on
+  for (int side = 0; side < 2; ++side) {
+    const int from = side * p.len, left = (int)min((long long)p.len, p.T - t0 - from);     // places that may start it
+    if ((int)threadIdx.x < 32) {
+      int at = kLongest;
+      for (int i = threadIdx.x; i < left; i += 32)
+        if (near[from + i].x != near[from + i + 1].x) at = min(at, i);
+      at = __reduce_min_sync(0xffffffffu, at);
+      if (threadIdx.x == 0) bound[side] = from + (t0 + from == 0 || at == kLongest ? 0 : at);
+    }
+  }
+  __syncthreads();
+  const int first = bound[0], n = (int)min((long long)bound[1], p.T - t0) - first;
+  const uint2* at = near + 1 + first;                  // the chunk's places
+  const uint32_t outer[2] = {at[-1].x, first + n < 2 * p.len && t0 + first + n < p.T ? at[n].x : kNone};
+  if (threadIdx.x == 0 && blockIdx.x % p.slabs == 0) {
+    const uint32_t v = at[n - 1].x;
+    if (v < p.V && outer[1] == v && !(at[0].x == v && outer[0] == v)) p.joins[1 + atomicAdd(p.joins, 1)] = (int)chunk;
+  }
   if (c >= p.C) return;
   float acc[VEC] = {};
   int start = 0;                                       // of the run
@@ -253,21 +297,43 @@ __global__ void __launch_bounds__(kSumThreads) embed_sum(const __grid_constant__
   flush(n);
 }
 
-// Runs that span chunks: the chunk where one starts adds what the next ones have of it.
+// Runs that span chunks: the chunk where one starts is in the list (in any order), and adds what the next ones have of it.
+// A warp has a partial row's 128 channels, the CTA's warps every eighth of the chunks, whose sums are added in order.
+constexpr int kJoinWarps = 8;
 template <typename T>
-__global__ void __launch_bounds__(kSumThreads) embed_join(const __grid_constant__ EmbedParams p) {
-  const long long chunk = blockIdx.x / p.slabs, end = (chunk + 1) * p.len;
-  if (end >= p.T) return;
-  const uint32_t v = p.sorted[end - 1].x;
-  if (v >= p.V || p.sorted[end].x != v) return;
-  if (p.sorted[chunk * p.len].x == v && chunk > 0 && p.sorted[chunk * p.len - 1].x == v) return;      // starts before
-  long long more = chunk + 1;                          // chunks behind that go on with the run
-  while (more + 1 < p.chunks && p.sorted[(more + 1) * p.len].x == v) ++more;
-  for (int c = (int)(blockIdx.x % p.slabs) * kSumThreads + threadIdx.x; c < p.C; c += p.slabs * kSumThreads) {
-    double s = (double)p.part[((size_t)chunk * 2 + 1) * p.C + c];
+__global__ void __launch_bounds__(32 * kJoinWarps) embed_join(const __grid_constant__ EmbedParams p) {
+  __shared__ double red[kJoinWarps][128];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, pieces = (p.C + 127) / 128;
+  const long long items = (long long)p.joins[0] * pieces;
+  for (long long item = blockIdx.x; item < items; item += gridDim.x) {
+    const long long chunk = p.joins[1 + item / pieces];
+    const int c0 = (int)(item % pieces) * 128;
+    const uint32_t v = p.sorted[(chunk + 1) * p.len].x;
+    long long end = chunk + 1;                         // the first chunk that does not start inside the run
+    for (bool all = true; all;) {
+      const long long q = end + threadIdx.x;
+      const int n = __syncthreads_count(q < p.chunks && p.sorted[min((q + 1) * p.len, p.T) - 1].x == v);
+      end += n;
+      all = n == 32 * kJoinWarps;
+    }
+    double sum[4] = {};
+    auto add = [&](const float* row) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (c0 + lane + 32 * i < p.C) sum[i] += (double)row[c0 + lane + 32 * i];
+    };
+    if (warp == 0) add(p.part + ((size_t)chunk * 2 + 1) * p.C);
 #pragma unroll 4
-    for (long long q = chunk + 1; q <= more; ++q) s += (double)p.part[(size_t)q * 2 * p.C + c];
-    static_cast<T*>(p.y)[(long long)v * p.ys + c] = from_f32<T>((float)(s * (double)p.scale));
+    for (long long q = chunk + 1 + warp; q < end; q += kJoinWarps) add(p.part + (size_t)q * 2 * p.C);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) red[warp][lane + 32 * i] = sum[i];
+    __syncthreads();
+    if (threadIdx.x < 128 && c0 + threadIdx.x < p.C) {
+      double s = 0.0;
+      for (int w = 0; w < kJoinWarps; ++w) s += red[w][threadIdx.x];
+      static_cast<T*>(p.y)[(long long)v * p.ys + c0 + threadIdx.x] = from_f32<T>((float)(s * (double)p.scale));
+    }
+    __syncthreads();
   }
 }
 
@@ -318,10 +384,14 @@ cudaError_t run_fwd(const EmbedParams& p, cudaStream_t st) {
 }
 template <typename T, int VEC>
 cudaError_t run_bwd(EmbedParams p, cudaStream_t st) {
+  // as few CTAs over the channels as there can be, with whole warps of equal parts
   p.slabs = (int)ceil_div(p.C, kSumThreads * VEC);
-  embed_sum<T, VEC><<<(unsigned)((p.chunks + ceil_div(p.V, kFill)) * p.slabs), kSumThreads, 0, st>>>(p);
-  p.slabs = (int)std::min<long long>(ceil_div(p.C, kSumThreads), 8);
-  embed_join<T><<<(unsigned)(p.chunks * p.slabs), kSumThreads, 0, st>>>(p);
+  const int threads = (int)ceil_div(ceil_div(ceil_div(p.C, VEC), p.slabs), 32) * 32;
+  embed_sum<T, VEC><<<(unsigned)((p.chunks + ceil_div(p.V, kFill)) * p.slabs), threads, 0, st>>>(p);
+  if (p.chunks > 1) {
+    const long long most = (p.chunks - 1) * ceil_div(p.C, 128);
+    embed_join<T><<<(unsigned)std::min<long long>(most, 148 * 4), 32 * kJoinWarps, 0, st>>>(p);
+  }
   return cudaGetLastError();
 }
 template <typename T>
@@ -393,7 +463,9 @@ int ssm_embedding_fwd(int64_t T, int64_t V, int64_t C, const void* idx, int32_t 
 int ssm_embedding_bwd_workspace_size(int64_t T, int64_t V, int64_t C, size_t* bytes) {
   if (bytes == nullptr) return fail(SSM_ERR_INVALID, "embedding: bytes is NULL");
   if (int rc = check_shape(T, V, C)) return rc;
-  *bytes = 2 * round256((size_t)T * sizeof(uint2)) + (size_t)ceil_div(T, chunk_len(T, C)) * 2 * C * sizeof(float) + 256;
+  const size_t chunks = (size_t)ceil_div(T, chunk_len(T, C));
+  *bytes = 2 * round256((size_t)T * sizeof(uint2)) + round256((chunks + 1) * sizeof(int)) +
+           round256((size_t)ceil_div(V, 32) * sizeof(int)) + chunks * 2 * C * sizeof(float) + 256;
   return SSM_OK;
 }
 
@@ -424,12 +496,16 @@ int ssm_embedding_bwd(int64_t T, int64_t V, int64_t C, const void* idx, int32_t 
   p.len = chunk_len(T, C);
   p.chunks = ceil_div(T, p.len);
   const int es = dy.dtype == SSM_BF16 ? 2 : 4, vec = width(C, es, dy, dweight);
-  if ((p.chunks + ceil_div(V, kFill)) * std::max<long long>(8, ceil_div(C, kSumThreads * vec)) > 0x7fffffffLL)
+  if ((p.chunks + ceil_div(V, kFill)) * ceil_div(C, kSumThreads * vec) > 0x7fffffffLL)
     return fail(SSM_ERR_INVALID, "embedding: shape out of range (tokens %lld, channels %lld)", T, C);
   unsigned char* at = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(workspace) + 255) & ~uintptr_t(255));
   uint2* a = reinterpret_cast<uint2*>(at);
   uint2* b = reinterpret_cast<uint2*>(at + round256((size_t)T * sizeof(uint2)));
-  p.part = reinterpret_cast<float*>(at + 2 * round256((size_t)T * sizeof(uint2)));
+  at += 2 * round256((size_t)T * sizeof(uint2));
+  p.joins = reinterpret_cast<int*>(at);
+  at += round256((size_t)(p.chunks + 1) * sizeof(int));
+  p.named = reinterpret_cast<uint32_t*>(at);
+  p.part = reinterpret_cast<float*>(at + round256((size_t)ceil_div(V, 32) * sizeof(int)));
   int passes = 1;                                      // of kDigit bits, for the ids 0 .. V (V: outside)
   while (passes * kDigit < 32 && (V >> (passes * kDigit)) > 0) ++passes;
   p.sorted = passes & 1 ? a : b;

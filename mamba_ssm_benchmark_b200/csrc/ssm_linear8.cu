@@ -225,13 +225,27 @@ __global__ void __launch_bounds__(kLinThreads) linear_e4m3(const __grid_constant
       const int n = first % p.tiles_n * kRowsW + 32 * warp + lane, m0 = first / p.tiles_n * TN;
       if (n < p.channels) {
         const float ws = p.w_scale[n], bias = p.bias != nullptr ? p.bias[n] : 0.0f;
-        for (int c = rank; c < TN && m0 + c < p.tokens; c += parts) {
-          const uint32_t at = smem_u32(smem) + (c * kRowsW + 32 * warp + lane) * 4;
-          float v = peer_load(at, 0);
-          for (int q = 1; q < parts; ++q) v += peer_load(at, q);
-          const long long m = m0 + c;
-          const float res = p.res != nullptr ? to_f32(static_cast<const TY*>(p.res)[m * p.rs + n]) : 0.0f;
-          static_cast<TY*>(p.y)[m * p.ys + n] = from_f32<TY>(finish(p, v, ws, p.x_scale[m], bias, res));
+        // this CTA's columns, kJoin at a time so that as many loads are on their way
+        constexpr int kJoin = TN >= 64 ? 8 : TN / 8;
+        const int own = TN / parts;
+        for (int c0 = rank * own; c0 < (rank + 1) * own && m0 + c0 < p.tokens; c0 += kJoin) {
+          float v[kJoin], res[kJoin], xs[kJoin];
+#pragma unroll
+          for (int i = 0; i < kJoin; ++i) {
+            const long long m = m0 + c0 + i;
+            const bool in = m < p.tokens;
+            xs[i] = in ? p.x_scale[m] : 0.0f;
+            res[i] = in && p.res != nullptr ? to_f32(static_cast<const TY*>(p.res)[m * p.rs + n]) : 0.0f;
+            v[i] = 0.0f;
+          }
+          for (int q = 0; q < parts; ++q) {
+#pragma unroll
+            for (int i = 0; i < kJoin; ++i) v[i] += peer_load(smem_u32(smem) + ((c0 + i) * kRowsW + 32 * warp + lane) * 4, q);
+          }
+#pragma unroll
+          for (int i = 0; i < kJoin; ++i)
+            if (m0 + c0 + i < p.tokens)
+              static_cast<TY*>(p.y)[(m0 + c0 + i) * p.ys + n] = from_f32<TY>(finish(p, v[i], ws, xs[i], bias, res[i]));
         }
       }
     }
@@ -274,7 +288,7 @@ cudaError_t run(LinearParams& p, cudaStream_t st) {
   p.tiles_n = ceil_div(p.channels, kRowsW);
   p.tiles = p.tiles_n * ceil_div(p.tokens, TN);
   const int room = 148 * (TN <= 64 ? 2 : 1);
-  int parts = 1;
+  int parts = 1;                                         // divides TN by kJoin or more
   while (parts < 8 && p.tiles * parts * 2 <= room && parts * 2 <= p.blocks) parts *= 2;
   if (parts > 1) return launch<TN, TY, true>(p, p.tiles * parts, parts, st);
   return launch<TN, TY, false>(p, std::min(p.tiles, room), 1, st);

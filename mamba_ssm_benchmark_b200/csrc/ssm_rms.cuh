@@ -4,9 +4,9 @@
 // t is a result, kept in the residual's type (the wider of the two), and what is normed: n comes from the rounded t, so
 // that a backward that reads t sees the forward's values.
 //
-// Memory bounds both directions.  A team of 1 to 8 warps holds a row in registers, K vectors of VEC values a
+// Memory bounds both directions.  A team of 1 to 16 warps holds a row in registers, K vectors of VEC values a
 // thread, and walks over rows; the rows ahead are on their way through slots of shared memory that only the thread
-// that reads them writes (cp.async, no barrier, no registers).  Sums are fp32: at most 32 values in a thread, then a
+// that reads them writes (cp.async, no barrier, no registers).  Sums are fp32: at most 16 values in a thread, then a
 // butterfly, then the warps in order.  Rows that no team holds take the kernels that pass over a row again.
 #pragma once
 
@@ -21,8 +21,9 @@
 
 namespace ssm {
 
-constexpr int kRmsThreads = 256;    // of a CTA
-constexpr int kRmsMost = 32;        // values of a row in a thread
+constexpr int kRmsMost = 16;        // values of a row in a thread: with more, registers leave too few rows to an SM
+constexpr int kRmsWarps = 16;       // of a team, at most
+constexpr int kRmsThreads = 32 * kRmsWarps;
 constexpr int kRmsChain = 256;      // rows that one fp32 sum of the weight's gradient takes; what joins them is fp64
 constexpr float kE4m3Max = 448.0f;
 constexpr float kRmsTiny = 1e-30f;  // rows whose largest value is below it share its scale: 1 / scale stays finite
@@ -36,6 +37,7 @@ struct RmsParams {
   int C, wbf16;
   float eps, inv_c;
   int norm;                           // 0: y = x, quantised
+  int wide8;                          // e4m3 rows start at multiples of 8
   // backward: t above is the normed sum, dy in y's place
   const void *dt;                     // gradient that arrives at t, or null
   void *dx, *dr;                      // dr null: the same tensor as dx
@@ -43,89 +45,189 @@ struct RmsParams {
   float* part;                        // partial rows of the weight's gradient, or null
 };
 
-// B bytes into shared memory, zeros unless ok; asynchronously where the hardware can (not two bytes).
-template <int B>
-__device__ __forceinline__ void fetch_piece(void* dst, const void* src, bool ok) {
-  if constexpr (B == 2)
-    *static_cast<uint16_t*>(dst) = ok ? *static_cast<const uint16_t*>(src) : (uint16_t)0;
-  else if constexpr (B == 16)
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(ok ? 16 : 0) : "memory");
-  else
-    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(smem_u32(dst)), "l"(src), "n"(B), "r"(ok ? B : 0)
-                 : "memory");
+// 16 bytes into shared memory, asynchronously: the first n of them from src, zeros behind.
+__device__ __forceinline__ void fetch_unit(void* dst, const void* src, int n) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(n) : "memory");
 }
-// A thread's slot of VEC values of T: units of at most 16 bytes, the same unit of all threads side by side.
-template <typename T, int VEC>
+// A warp's part of a row: VEC values to a lane, 32 VEC in a row from value c0 on, in 16-byte units of shared memory.
+// RAGGED: rows start anywhere and end anywhere; the units are those of memory that hold the values, a lane reads its own and
+// the next one and shifts.  (Loads of a value or two at a time, at 16384 x 2047 bf16: 515 us; this way 100.)
+// Values are float2 pairs: one instruction takes two.  Issue slots bound these kernels as much as memory does.
+template <typename T, int VEC, bool RAGGED>
 struct Slot {
-  static constexpr int kBytes = VEC * (int)sizeof(T), kUnit = kBytes > 16 ? 16 : kBytes, kStep = kUnit / (int)sizeof(T);
-  static __device__ __forceinline__ void fetch(unsigned char* at, const T* src, bool ok) {
-#pragma unroll
-    for (int i = 0; i < VEC / kStep; ++i) fetch_piece<kUnit>(at + (i * kRmsThreads + threadIdx.x) * kUnit, src + i * kStep, ok);
+  static constexpr int kLane = VEC * (int)sizeof(T), kUnits = kLane / 16, kWords = kLane / 4;
+  static constexpr int kWarp = 32 * kLane + (RAGGED ? 16 : 0);          // bytes
+  static_assert(kLane % 16 == 0, "whole units");
+  static __device__ __forceinline__ int offset(const T* row, int c0) {
+    return (int)(reinterpret_cast<uintptr_t>(row + c0) & 15);
   }
-  static __device__ __forceinline__ void read(const unsigned char* at, float (&v)[VEC]) {
+  // The warp's units of a row to `at`, which held zeros at first: what lies past the row's end stays zero.
+  static __device__ __forceinline__ void fetch(unsigned char* at, const T* row, int c0, int C, int lane) {
+    if constexpr (RAGGED) {
+      // a unit that holds a value of the row lies in the row's allocation up to that value: allocations start at multiples of 16
+      const int o = offset(row, c0);
+      const char* from = reinterpret_cast<const char*>(row + c0) - o;
+      const char* none = reinterpret_cast<const char*>(reinterpret_cast<uintptr_t>(row) & ~uintptr_t(15));
+      const int bytes = c0 < C ? (C - c0) * (int)sizeof(T) + o : 0;            // from the first unit to the row's end
 #pragma unroll
-    for (int i = 0; i < VEC / kStep; ++i) {
-      float part[kStep];
-      vec_load<T, kStep>(reinterpret_cast<const T*>(at + (i * kRmsThreads + threadIdx.x) * kUnit), part);
+      for (int i = 0; i <= kUnits; ++i) {
+        const int u = i * 32 + lane, n = min(16, bytes - 16 * u);
+        if (i < kUnits || lane == 0) fetch_unit(at + 16 * u, n > 0 ? from + 16 * u : none, max(n, 0));
+      }
+    } else {
 #pragma unroll
-      for (int j = 0; j < kStep; ++j) v[i * kStep + j] = part[j];
+      for (int i = 0; i < kUnits; ++i) {
+        const int c = c0 + (i * 32 + lane) * (16 / (int)sizeof(T));
+        if (c < C) fetch_unit(at + (i * 32 + lane) * 16, row + c, 16);
+      }
+    }
+  }
+  // two values to a word pair or word, and back
+  static __device__ __forceinline__ void pack(const float2 (&v)[VEC / 2], uint32_t (&w)[kWords]) {
+#pragma unroll
+    for (int i = 0; i < VEC / 2; ++i) {
+      if constexpr (sizeof(T) == 4) {
+        w[2 * i] = __float_as_uint(v[i].x);
+        w[2 * i + 1] = __float_as_uint(v[i].y);
+      } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(v[i].x, v[i].y);
+        w[i] = *reinterpret_cast<const uint32_t*>(&h);
+      }
+    }
+  }
+  static __device__ __forceinline__ void unpack(const uint32_t* w, float2 (&v)[VEC / 2]) {
+#pragma unroll
+    for (int i = 0; i < VEC / 2; ++i) {
+      if constexpr (sizeof(T) == 4)
+        v[i] = make_float2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+      else
+        v[i] = make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+    }
+  }
+  // the lane's values; zeros past the row's end
+  static __device__ __forceinline__ void read(const unsigned char* at, const T* row, int c0, int lane, float2 (&v)[VEC / 2]) {
+    constexpr int kHeld = kWords + (RAGGED ? 4 : 0);
+    uint32_t w[kHeld];
+#pragma unroll
+    for (int i = 0; i < kHeld / 4; ++i) {
+      const uint4 q = *reinterpret_cast<const uint4*>(at + (lane * kUnits + i) * 16);
+      w[4 * i] = q.x, w[4 * i + 1] = q.y, w[4 * i + 2] = q.z, w[4 * i + 3] = q.w;
+    }
+    if constexpr (RAGGED) {
+      const int o = offset(row, c0);
+#pragma unroll
+      for (int i = 0; i + 2 < kHeld; ++i) w[i] = o & 8 ? w[i + 2] : w[i];
+#pragma unroll
+      for (int i = 0; i + 3 < kHeld; ++i) w[i] = o & 4 ? w[i + 1] : w[i];
+      if constexpr (sizeof(T) == 2) {
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) w[i] = o & 2 ? __byte_perm(w[i], w[i + 1], 0x5432) : w[i];
+      }
+    }
+    unpack(w, v);
+  }
+  // the lane's words to the row; all lanes of a warp call it
+  static __device__ __forceinline__ void write(T* row, int c0, int C, int lane, const uint32_t (&own)[kWords]) {
+    constexpr int kVals = 16 / (int)sizeof(T);             // to a unit
+    const int n = C - c0;                                  // values of the row in this warp, and behind it
+    if constexpr (!RAGGED) {
+#pragma unroll
+      for (int i = 0; i < kUnits; ++i) {
+        const int first = (lane * kUnits + i) * kVals;
+        if (first < n)
+          *reinterpret_cast<uint4*>(row + c0 + first) = make_uint4(own[4 * i], own[4 * i + 1], own[4 * i + 2], own[4 * i + 3]);
+      }
+    } else {
+      const int o = offset(row, c0), before = o / (int)sizeof(T);
+      uint32_t w[kWords + 4];                              // the lane before's last unit, then this one's
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = __shfl_up_sync(0xffffffffu, own[kWords - 4 + i], 1);
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) w[4 + i] = own[i];
+      // towards the back by o bytes: w[4] becomes the first word of this lane's first unit of memory, whose front is the end
+      // of the lane before
+#pragma unroll
+      for (int i = kWords + 3; i >= 2; --i) w[i] = o & 8 ? w[i - 2] : w[i];
+#pragma unroll
+      for (int i = kWords + 3; i >= 3; --i) w[i] = o & 4 ? w[i - 1] : w[i];
+      if constexpr (sizeof(T) == 2) {
+#pragma unroll
+        for (int i = kWords + 3; i >= 4; --i) w[i] = o & 2 ? __byte_perm(w[i - 1], w[i], 0x5432) : w[i];
+      }
+#pragma unroll
+      for (int i = 0; i < kUnits; ++i) {
+        const int first = (lane * kUnits + i) * kVals - before;        // the unit's first value, from c0 on
+        T* to = row + c0 + first;
+        if (first >= 0 && first + kVals <= n)
+          *reinterpret_cast<uint4*>(to) = make_uint4(w[4 + 4 * i], w[5 + 4 * i], w[6 + 4 * i], w[7 + 4 * i]);
+        else
+          single(to, -first, n - first, &w[4 + 4 * i]);
+      }
+      // what the last lane's shift moved out: the end of its last unit
+      if (lane == 31 && before > 0) single(row + c0 + 32 * VEC - kVals, kVals - before, n - 32 * VEC + kVals, &own[kWords - 4]);
+    }
+  }
+  // values from .. to - 1 of a unit
+  static __device__ __forceinline__ void single(T* unit, int from, int to, const uint32_t* w) {
+#pragma unroll
+    for (int i = 0; i < 16 / (int)sizeof(T); ++i) {
+      if (i < from || i >= to) continue;
+      if constexpr (sizeof(T) == 4)
+        unit[i] = __uint_as_float(w[i]);
+      else
+        unit[i] = __ushort_as_bfloat16((unsigned short)(i & 1 ? w[i / 2] >> 16 : w[i / 2] & 0xffff));
     }
   }
 };
+// A CTA's queue to zeros, for what fetch does not write.
+__device__ __forceinline__ void clear_queue(unsigned char* queue, int bytes) {
+  for (int i = threadIdx.x * 16; i < bytes; i += blockDim.x * 16) *reinterpret_cast<uint4*>(queue + i) = make_uint4(0, 0, 0, 0);
+  __syncthreads();
+}
 __device__ __forceinline__ void queue_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void queue_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-template <typename T, int VEC>
-__device__ __forceinline__ void write_piece(T* dst, const float (&v)[VEC]) {
-  constexpr int kStep = VEC * sizeof(T) > 16 ? 16 / sizeof(T) : VEC;
-#pragma unroll
-  for (int i = 0; i < VEC; i += kStep) {
-    float part[kStep];
-#pragma unroll
-    for (int j = 0; j < kStep; ++j) part[j] = v[i + j];
-    vec_store<T, kStep>(dst + i, part);
-  }
-}
-// VEC values to e4m3, nearest even; NaN stays NaN.
+// VEC values to e4m3, nearest even (NaN stays NaN), the first n of them to dst; wide: dst is aligned to VEC bytes.
 template <int VEC>
-__device__ __forceinline__ void write_e4m3(uint8_t* dst, const float (&v)[VEC]) {
-  if constexpr (VEC == 1) {
-    dst[0] = __nv_cvt_float_to_fp8(v[0], __NV_SATFINITE, __NV_E4M3);
-  } else {
-    uint16_t h[VEC / 2];
+__device__ __forceinline__ void write_e4m3(uint8_t* dst, int n, bool wide, const float2 (&v)[VEC / 2]) {
+  uint16_t h[VEC / 2];
 #pragma unroll
-    for (int i = 0; i < VEC / 2; ++i)
-      h[i] = __nv_cvt_float2_to_fp8x2(make_float2(v[2 * i], v[2 * i + 1]), __NV_SATFINITE, __NV_E4M3);
-    if constexpr (VEC == 8) {
+  for (int i = 0; i < VEC / 2; ++i) h[i] = __nv_cvt_float2_to_fp8x2(v[i], __NV_SATFINITE, __NV_E4M3);
+  if (wide && n >= VEC) {
+    if constexpr (VEC == 8)
       *reinterpret_cast<uint2*>(dst) = make_uint2(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16);
-    } else if constexpr (VEC == 4) {
+    else
       *reinterpret_cast<uint32_t*>(dst) = h[0] | (uint32_t)h[1] << 16;
-    } else {
-      *reinterpret_cast<uint16_t*>(dst) = h[0];
-    }
-  }
-}
-
-template <int VEC>
-__device__ __forceinline__ void load_weight(const RmsParams& p, int c, float (&w)[VEC]) {
-  if (p.w == nullptr) {
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) w[v] = 1.0f;
-  } else if (p.wbf16) {
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) w[v] = to_f32(static_cast<const __nv_bfloat16*>(p.w)[c + v]);
   } else {
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) w[v] = static_cast<const float*>(p.w)[c + v];
+    for (int i = 0; i < VEC; ++i)
+      if (i < n) dst[i] = (uint8_t)(h[i / 2] >> (i & 1 ? 8 : 0));
   }
 }
 
-// The warps that share a row: `wpr` of a CTA's.  Sums alternate between two buffers: a thread that reads one is at most
-// one barrier behind those that write the other.
+// The first n of VEC weights from channel c on; zeros behind.
+template <int VEC>
+__device__ __forceinline__ void load_weight(const RmsParams& p, int c, int n, float2 (&w)[VEC / 2]) {
+  auto one = [&](int v) {
+    if (v >= n) return 0.0f;
+    return p.w == nullptr ? 1.0f
+           : p.wbf16      ? to_f32(static_cast<const __nv_bfloat16*>(p.w)[c + v])
+                          : static_cast<const float*>(p.w)[c + v];
+  };
+#pragma unroll
+  for (int v = 0; v < VEC / 2; ++v) w[v] = make_float2(one(2 * v), one(2 * v + 1));
+}
+__device__ __forceinline__ float weight_at(const RmsParams& p, int c) {
+  if (p.w == nullptr) return 1.0f;
+  return p.wbf16 ? to_f32(static_cast<const __nv_bfloat16*>(p.w)[c]) : static_cast<const float*>(p.w)[c];
+}
+
+// The warps that share a row: `wpr` of a CTA's.  Results of the warps alternate between two buffers: a thread that reads
+// one is at most one barrier behind those that write the other.
 struct Team {
   int wpr, id, lane, warp, tid, size, turn;
-  float2* red;                          // (2, wpr) of this team
+  float2* red;                          // (2, kRmsWarps) of this team
   __device__ Team(int wpr_, float2* buf) : wpr(wpr_), turn(0) {
     lane = threadIdx.x & 31;
     const int w = threadIdx.x >> 5;
@@ -133,57 +235,77 @@ struct Team {
     warp = w - id * wpr;
     size = wpr * 32;
     tid = warp * 32 + lane;
-    red = buf + id * 2 * wpr;
+    red = buf + id * 2 * kRmsWarps;
   }
-  template <typename F>
-  __device__ __forceinline__ float2 join(float2 v, F f) {
+  // every warp's value, in lane i that of warp i (`none` past the last)
+  __device__ __forceinline__ float2 exchange(float2 v, float2 none) {
+    float2* at = red + turn;
+    turn ^= kRmsWarps;
+    if (lane == 0) at[warp] = v;
+    asm volatile("bar.sync %0, %1;" ::"r"(1 + id), "r"(size) : "memory");
+    return lane < wpr ? at[lane] : none;
+  }
+  template <int LANES>
+  static __device__ __forceinline__ float2 add(float2 v) {
 #pragma unroll
-    for (int m = 16; m >= 1; m >>= 1)
-      v = f(v, make_float2(__shfl_xor_sync(0xffffffffu, v.x, m), __shfl_xor_sync(0xffffffffu, v.y, m)));
-    if (wpr > 1) {
-      float2* at = red + turn * wpr;
-      turn ^= 1;
-      if (lane == 0) at[warp] = v;
-      asm volatile("bar.sync %0, %1;" ::"r"(1 + id), "r"(size) : "memory");
-      v = at[0];
-      for (int i = 1; i < wpr; ++i) v = f(v, at[i]);
-    }
+    for (int m = LANES / 2; m >= 1; m /= 2)
+      v = add2(v, make_float2(__shfl_xor_sync(0xffffffffu, v.x, m), __shfl_xor_sync(0xffffffffu, v.y, m)));
     return v;
   }
-  __device__ __forceinline__ float2 sum(float a, float b) {
-    return join(make_float2(a, b), [](float2 u, float2 v) { return make_float2(u.x + v.x, u.y + v.y); });
+  __device__ __forceinline__ float2 sum(float2 v) {
+    v = add<32>(v);
+    if (wpr == 1) return v;
+    v = add<16>(exchange(v, make_float2(0.0f, 0.0f)));        // lanes 0 .. 15 hold the warps'
+    return make_float2(__shfl_sync(0xffffffffu, v.x, 0), __shfl_sync(0xffffffffu, v.y, 0));
   }
-  __device__ __forceinline__ float max(float a) {
-    return join(make_float2(a, 0.0f), [](float2 u, float2 v) { return make_float2(fmaxf(u.x, v.x), 0.0f); }).x;
+  __device__ __forceinline__ float sum(float v) {
+#pragma unroll
+    for (int m = 16; m >= 1; m /= 2) v += __shfl_xor_sync(0xffffffffu, v, m);
+    if (wpr == 1) return v;
+    v = exchange(make_float2(v, 0.0f), make_float2(0.0f, 0.0f)).x;
+#pragma unroll
+    for (int m = 8; m >= 1; m /= 2) v += __shfl_xor_sync(0xffffffffu, v, m);
+    return __shfl_sync(0xffffffffu, v, 0);
+  }
+  // of numbers that are not negative, which compare as their bits do
+  __device__ __forceinline__ float max(float v) {
+    uint32_t b = __reduce_max_sync(0xffffffffu, __float_as_uint(v));
+    if (wpr > 1) b = __reduce_max_sync(0xffffffffu, __float_as_uint(exchange(make_float2(__uint_as_float(b), 0.0f), make_float2(0.0f, 0.0f)).x));
+    return __uint_as_float(b);
   }
 };
+constexpr int kRmsRed = 2 * kRmsWarps * 8;       // floats2 of at most eight teams
 
-// Stages of a thread's queue of `bytes` bytes a row.
-constexpr int rms_depth(int bytes) { return bytes <= 48 ? 4 : bytes <= 256 ? 3 : 2; }
+// Rows on their way to a team: with more, fewer CTAs share an SM and wait for one another's barriers (16384 x 5120 bf16
+// backward: 179 us with four rows, 141 with three, 137 with two).
+constexpr int kRmsDepth = 2;
 
 // ---- host -----------------------------------------------------------------------------------
 inline long long rms_ceil(long long a, long long b) { return (a + b - 1) / b; }
 
-// Warps to a row and vectors a thread, or k = 0: no team holds the row.  The fewest warps whose threads take at most
-// `most` vectors: more rows side by side, fewer barriers.
+// Warps to a row and vectors a thread (one of `ks`, the largest first), or k = 0: no team holds the row.  The form that
+// wastes the fewest lanes (2560 bf16 values: five warps of two vectors), with the fewest warps.
 struct RmsForm {
   int wpr, k;
+  int teams() const { return std::max(1, 8 / wpr); }     // rows side by side in a CTA
+  int threads() const { return 32 * wpr * teams(); }
 };
-inline RmsForm rms_form(long long C, int vec, int most) {
-  for (int wpr = 1; wpr <= kRmsThreads / 32; wpr *= 2) {
-    const long long k = rms_ceil(rms_ceil(C, vec), 32 * wpr);
-    if (k <= most) return {wpr, (int)k};
+inline RmsForm rms_form(long long C, int vec, std::initializer_list<int> ks) {
+  RmsForm f = {0, 0};
+  for (int k : ks) {
+    const long long wpr = rms_ceil(C, 32LL * vec * k);
+    if (wpr <= kRmsWarps && (f.k == 0 || wpr * k < (long long)f.wpr * f.k)) f = {(int)wpr, k};
   }
-  return {0, 0};
+  return f;
 }
 
-// A tensor whose rows a kernel reads or writes in vectors.
+// A tensor whose rows a kernel reads or writes in units of 16 bytes.
 struct RmsSide {
   const void* ptr;
   long long stride;
   int bytes;
 };
-int rms_vec(long long C, int xbytes, std::initializer_list<RmsSide> sides);
+bool rms_aligned(long long C, int vec, std::initializer_list<RmsSide> sides);
 int rms_check(int64_t rows, int64_t C, const ssm_view& x, const ssm_view& residual, const void* weight, int32_t wdtype);
 
 }  // namespace ssm

@@ -15,81 +15,100 @@ int report_error(int code, const char* msg);
 
 namespace {
 
-template <typename TX, typename TR, int VEC, int K>
+template <typename TX, typename TR, int VEC, int K, bool RAGGED>
 __global__ void __launch_bounds__(kRmsThreads) rms_bwd(const __grid_constant__ RmsParams p, int wpr) {
-  constexpr int kT = Slot<TR, VEC>::kBytes, kG = Slot<TX, VEC>::kBytes, kRow = K * (2 * kT + kG), kDepth = rms_depth(kRow);
+  using ST = Slot<TR, VEC, RAGGED>;
+  using SG = Slot<TX, VEC, RAGGED>;
   extern __shared__ __align__(16) unsigned char queue[];
-  __shared__ float2 red[2 * kRmsThreads / 32];
+  __shared__ float2 red[kRmsRed];
   Team team(wpr, red);
-  constexpr int nt = kRmsThreads;
-  const int teams = nt / 32 / wpr;
+  const int warps = blockDim.x >> 5, teams = warps / wpr, lane = team.lane;
+  // this warp's bytes of a stage: K parts of t, of dy, of dt
+  constexpr int kG = K * ST::kWarp, kD = kG + K * SG::kWarp, kStage = kD + K * ST::kWarp;
+  clear_queue(queue, warps * kRmsDepth * kStage);
+  unsigned char* mine = queue + (threadIdx.x >> 5) * kRmsDepth * kStage;
   const long long step = (long long)gridDim.x * teams;
   long long row = (long long)blockIdx.x * teams + team.id;
-
+  const bool adds = p.dt != nullptr;
+  auto c0 = [&](int k) { return (team.warp * 32 + k * team.size) * VEC; };
   auto fetch = [&](long long r, int stage) {
-    unsigned char* at = queue + (size_t)stage * kRow * nt;
+    unsigned char* at = mine + stage * kStage;
+    if (r < p.rows) {
+      const TR* t = static_cast<const TR*>(p.t) + r * p.ts;
+      const TX* g = static_cast<const TX*>(p.y) + r * p.ys;
+      const TR* d = static_cast<const TR*>(p.dt) + r * p.dts;
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const int c = (team.tid + k * team.size) * VEC;
-      const bool ok = r < p.rows && c < p.C;
-      Slot<TR, VEC>::fetch(at + (size_t)k * kT * nt, static_cast<const TR*>(p.t) + (ok ? r * p.ts + c : 0), ok);
-      Slot<TX, VEC>::fetch(at + (size_t)(K * kT + k * kG) * nt, static_cast<const TX*>(p.y) + (ok ? r * p.ys + c : 0), ok);
-      if (p.dt != nullptr)
-        Slot<TR, VEC>::fetch(at + (size_t)(K * (kT + kG) + k * kT) * nt,
-                             static_cast<const TR*>(p.dt) + (ok ? r * p.dts + c : 0), ok);
+      for (int k = 0; k < K; ++k) {
+        ST::fetch(at + k * ST::kWarp, t, c0(k), p.C, lane);
+        SG::fetch(at + kG + k * SG::kWarp, g, c0(k), p.C, lane);
+        if (adds) ST::fetch(at + kD + k * ST::kWarp, d, c0(k), p.C, lane);
+      }
     }
     queue_commit();
   };
 #pragma unroll
-  for (int d = 0; d < kDepth; ++d) fetch(row + d * step, d);
-  float w[K][VEC], dw[K][VEC];
+  for (int d = 0; d < kRmsDepth; ++d) fetch(row + d * step, d);
+  float2 w[K][VEC / 2], dw[K][VEC / 2];
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    const int c = (team.tid + k * team.size) * VEC;
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) w[k][i] = dw[k][i] = 0.0f;
-    if (c < p.C) load_weight<VEC>(p, c, w[k]);
+    for (int i = 0; i < VEC / 2; ++i) dw[k][i] = make_float2(0.0f, 0.0f);
+    load_weight<VEC>(p, c0(k) + lane * VEC, p.C - c0(k) - lane * VEC, w[k]);
   }
   int stage = 0;
   for (; row < p.rows; row += step) {
-    float t[K][VEC], g[K][VEC], d[K][VEC];
-    float ss = 0.0f, gt = 0.0f;
-    queue_wait<kDepth - 1>();
-    const unsigned char* at = queue + (size_t)stage * kRow * nt;
+    // The row is read from its slots twice: kept in registers between the sums and their use, it left 8 warps to an SM
+    // (16384 x 5120 bf16: 150 us).
+    const TR* t_row = static_cast<const TR*>(p.t) + row * p.ts;
+    const TX* g_row = static_cast<const TX*>(p.y) + row * p.ys;
+    const TR* d_row = static_cast<const TR*>(p.dt) + row * p.dts;
+    float2 ss = make_float2(0.0f, 0.0f), gt = ss;
+    queue_wait<kRmsDepth - 1>();
+    __syncwarp();
+    const unsigned char* at = mine + stage * kStage;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      Slot<TR, VEC>::read(at + (size_t)k * kT * nt, t[k]);
-      Slot<TX, VEC>::read(at + (size_t)(K * kT + k * kG) * nt, g[k]);
-      if (p.dt != nullptr) {
-        Slot<TR, VEC>::read(at + (size_t)(K * (kT + kG) + k * kT) * nt, d[k]);
+      float2 t[VEC / 2], g[VEC / 2];
+      ST::read(at + k * ST::kWarp, t_row, c0(k), lane, t);
+      SG::read(at + kG + k * SG::kWarp, g_row, c0(k), lane, g);
+#pragma unroll
+      for (int i = 0; i < VEC / 2; ++i) {
+        ss = fma2(t[i], t[i], ss);
+        gt = fma2(mul2(g[i], w[k][i]), t[i], gt);
+      }
+    }
+    const float2 s = team.sum(make_float2(ss.x + ss.y, gt.x + gt.y));
+    const float rstd = 1.0f / sqrtf(s.x * p.inv_c + p.eps);
+    const float2 r2 = bc2(rstd), mean = bc2(-s.y * rstd * p.inv_c);      // minus that of g n
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      float2 t[VEC / 2], g[VEC / 2], d[VEC / 2];
+      ST::read(at + k * ST::kWarp, t_row, c0(k), lane, t);
+      SG::read(at + kG + k * SG::kWarp, g_row, c0(k), lane, g);
+      if (adds) {
+        ST::read(at + kD + k * ST::kWarp, d_row, c0(k), lane, d);
       } else {
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) d[k][i] = 0.0f;
+        for (int i = 0; i < VEC / 2; ++i) d[i] = make_float2(0.0f, 0.0f);
       }
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        ss = fmaf(t[k][i], t[k][i], ss);
-        gt = fmaf(g[k][i] * w[k][i], t[k][i], gt);
+      for (int i = 0; i < VEC / 2; ++i) {
+        const float2 n = mul2(t[i], r2);
+        dw[k][i] = fma2(g[i], n, dw[k][i]);
+        d[i] = fma2(r2, fma2(n, mean, mul2(g[i], w[k][i])), d[i]);
+      }
+      uint32_t dx[SG::kWords];
+      SG::pack(d, dx);
+      SG::write(static_cast<TX*>(p.dx) + row * p.dxs, c0(k), p.C, lane, dx);
+      if (p.dr != nullptr) {
+        uint32_t dr[ST::kWords];
+        ST::pack(d, dr);
+        ST::write(static_cast<TR*>(p.dr) + row * p.drs, c0(k), p.C, lane, dr);
       }
     }
-    fetch(row + kDepth * step, stage);
-    stage = stage + 1 == kDepth ? 0 : stage + 1;
-    const float2 s = team.sum(ss, gt);
-    const float rstd = 1.0f / sqrtf(s.x * p.inv_c + p.eps);
-    const float mean = s.y * rstd * p.inv_c;              // of g n
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const int c = (team.tid + k * team.size) * VEC;
-      if (c >= p.C) continue;
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        const float n = t[k][i] * rstd;
-        dw[k][i] = fmaf(g[k][i], n, dw[k][i]);
-        d[k][i] = fmaf(rstd, fmaf(-n, mean, g[k][i] * w[k][i]), d[k][i]);
-      }
-      write_piece<TX, VEC>(static_cast<TX*>(p.dx) + row * p.dxs + c, d[k]);
-      if (p.dr != nullptr) write_piece<TR, VEC>(static_cast<TR*>(p.dr) + row * p.drs + c, d[k]);
-    }
+    __syncwarp();
+    fetch(row + kRmsDepth * step, stage);
+    stage = stage + 1 == kRmsDepth ? 0 : stage + 1;
   }
   queue_wait<0>();
   if (p.part == nullptr) return;
@@ -103,43 +122,42 @@ __global__ void __launch_bounds__(kRmsThreads) rms_bwd(const __grid_constant__ R
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
           float& s = sum[(k * VEC + i) * team.size + team.tid];
-          s = q == 0 ? dw[k][i] : s + dw[k][i];
+          const float v = i & 1 ? dw[k][i / 2].y : dw[k][i / 2].x;
+          s = q == 0 ? v : s + v;
         }
     }
   }
   if (team.id == teams - 1) {
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const int c = (team.tid + k * team.size) * VEC;
-      if (c >= p.C) continue;
+    for (int k = 0; k < K; ++k)
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) p.part[(size_t)blockIdx.x * p.C + c + i] = sum[(k * VEC + i) * team.size + team.tid];
-    }
+      for (int i = 0; i < VEC; ++i) {
+        const int c = c0(k) + lane * VEC + i;
+        if (c < p.C) p.part[(size_t)blockIdx.x * p.C + c] = sum[(k * VEC + i) * team.size + team.tid];
+      }
   }
 }
 
 // Rows that no team holds: a CTA per row for the sums and d; rstd goes to `stat`.
 template <typename TX, typename TR>
-__global__ void __launch_bounds__(512) rms_bwd_long(const __grid_constant__ RmsParams p, float* stat) {
-  __shared__ float2 red[2 * 16];
-  Team team(16, red);
+__global__ void __launch_bounds__(kRmsThreads) rms_bwd_long(const __grid_constant__ RmsParams p, float* stat) {
+  __shared__ float2 red[kRmsRed];
+  Team team(kRmsWarps, red);
   for (long long row = blockIdx.x; row < p.rows; row += gridDim.x) {
     const TR* t = static_cast<const TR*>(p.t) + row * p.ts;
     const TX* dy = static_cast<const TX*>(p.y) + row * p.ys;
-    float ss = 0.0f, gt = 0.0f, w[1];
+    float ss = 0.0f, gt = 0.0f;
     for (int c = threadIdx.x; c < p.C; c += 512) {
-      load_weight<1>(p, c, w);
       const float v = to_f32(t[c]);
       ss = fmaf(v, v, ss);
-      gt = fmaf(to_f32(dy[c]) * w[0], v, gt);
+      gt = fmaf(to_f32(dy[c]) * weight_at(p, c), v, gt);
     }
-    const float2 s = team.sum(ss, gt);
+    const float2 s = team.sum(make_float2(ss, gt));
     const float rstd = 1.0f / sqrtf(s.x * p.inv_c + p.eps), mean = s.y * rstd * p.inv_c;
     if (threadIdx.x == 0) stat[row] = rstd;
     for (int c = threadIdx.x; c < p.C; c += 512) {
-      load_weight<1>(p, c, w);
       const float d0 = p.dt != nullptr ? to_f32(static_cast<const TR*>(p.dt)[row * p.dts + c]) : 0.0f;
-      const float d = fmaf(rstd, fmaf(-to_f32(t[c]) * rstd, mean, to_f32(dy[c]) * w[0]), d0);
+      const float d = fmaf(rstd, fmaf(-to_f32(t[c]) * rstd, mean, to_f32(dy[c]) * weight_at(p, c)), d0);
       static_cast<TX*>(p.dx)[row * p.dxs + c] = from_f32<TX>(d);
       if (p.dr != nullptr) static_cast<TR*>(p.dr)[row * p.drs + c] = from_f32<TR>(d);
     }
@@ -195,38 +213,31 @@ int fail(int code, const char* fmt, long long a = 0, long long b = 0) {
 constexpr long long kCtas = 148 * 8;
 long long most_parts(long long rows) { return std::max(kCtas, rms_ceil(rows, kRmsChain)); }
 
-template <typename TX, typename TR, int VEC, int K>
-cudaError_t launch(const RmsParams& p, int wpr, long long* parts, cudaStream_t st) {
-  constexpr int kRow = K * (2 * Slot<TR, VEC>::kBytes + Slot<TX, VEC>::kBytes);
-  constexpr auto kern = rms_bwd<TX, TR, VEC, K>;
-  const int teams = kRmsThreads / 32 / wpr;
-  const size_t smem = std::max((size_t)rms_depth(kRow) * kRow * kRmsThreads, (size_t)K * VEC * 4 * wpr * 32);
-  const int fit = std::min(8, ctas_per_sm<kern>(kRmsThreads, smem));
-  long long grid = std::min<long long>(rms_ceil(p.rows, teams), 148LL * std::max(fit, 1));
-  grid = std::max<long long>({1, grid, rms_ceil(p.rows, (long long)teams * kRmsChain)});
+template <typename TX, typename TR, int K, bool RAGGED>
+cudaError_t launch(const RmsParams& p, RmsForm f, long long* parts, cudaStream_t st) {
+  constexpr int VEC = 16 / sizeof(TX);
+  using ST = Slot<TR, VEC, RAGGED>;
+  using SG = Slot<TX, VEC, RAGGED>;
+  constexpr auto kern = rms_bwd<TX, TR, VEC, K, RAGGED>;
+  const int threads = f.threads(), teams = f.teams();
+  const size_t smem = std::max((size_t)kRmsDepth * K * (2 * ST::kWarp + SG::kWarp) * (threads / 32),
+                               (size_t)K * VEC * 4 * f.wpr * 32);
+  const int fit = std::min(8, std::max(1, ctas_per_sm_threads<kern>(threads, smem)));
+  // one wave, or as many as kRmsChain asks for
+  const long long grid = std::max(std::min<long long>(rms_ceil(p.rows, teams), 148LL * fit),
+                                  rms_ceil(p.rows, (long long)teams * kRmsChain));
   *parts = grid;
-  kern<<<(unsigned)grid, kRmsThreads, smem, st>>>(p, wpr);
+  kern<<<(unsigned)grid, threads, smem, st>>>(p, f.wpr);
   return cudaGetLastError();
 }
-template <typename TX, typename TR, int VEC>
-cudaError_t run_vec(const RmsParams& p, long long* parts, float* stat, cudaStream_t st) {
-  const RmsForm f = rms_form(p.C, VEC, kRmsMost / VEC);
-  if constexpr (VEC >= 4) {
-    if (f.k == 1) return launch<TX, TR, VEC, 1>(p, f.wpr, parts, st);
-    if (f.k == 2) return launch<TX, TR, VEC, 2>(p, f.wpr, parts, st);
-    if (f.k == 3) return launch<TX, TR, VEC, 3>(p, f.wpr, parts, st);
-    if (f.k == 4) return launch<TX, TR, VEC, 4>(p, f.wpr, parts, st);
-  }
-  if constexpr (VEC == 4) {
-    if (f.k == 5 || f.k == 6) return launch<TX, TR, VEC, 6>(p, f.wpr, parts, st);
-    if (f.k > 6) return launch<TX, TR, VEC, 8>(p, f.wpr, parts, st);
-  }
-  if constexpr (VEC <= 2) {
-    if (f.k > 0 && f.k * VEC <= 8) return launch<TX, TR, VEC, 8 / VEC>(p, f.wpr, parts, st);
-    if (f.k > 0 && f.k * VEC <= 16) return launch<TX, TR, VEC, 16 / VEC>(p, f.wpr, parts, st);
-    if (f.k > 0) return launch<TX, TR, VEC, 32 / VEC>(p, f.wpr, parts, st);
-  }
-  rms_bwd_long<TX, TR><<<(unsigned)std::min<long long>(p.rows, 148 * 4), 512, 0, st>>>(p, stat);
+template <typename TX, typename TR, bool RAGGED>
+cudaError_t run_form(const RmsParams& p, long long* parts, float* stat, cudaStream_t st) {
+  constexpr int VEC = 16 / sizeof(TX), kMany = kRmsMost / VEC;
+  const RmsForm f = rms_form(p.C, VEC, {kMany, kMany / 2, 1});
+  if (f.k == kMany) return launch<TX, TR, kMany, RAGGED>(p, f, parts, st);
+  if (VEC == 4 && f.k == 2) return launch<TX, TR, 2, RAGGED>(p, f, parts, st);
+  if (f.k == 1) return launch<TX, TR, 1, RAGGED>(p, f, parts, st);
+  rms_bwd_long<TX, TR><<<(unsigned)std::min<long long>(p.rows, 148 * 4), kRmsThreads, 0, st>>>(p, stat);
   if (p.part != nullptr) {
     *parts = rms_ceil(p.rows, kRmsChain);
     const dim3 grid((unsigned)rms_ceil(p.C, 32), (unsigned)std::min<long long>(*parts, 65535));
@@ -235,11 +246,8 @@ cudaError_t run_vec(const RmsParams& p, long long* parts, float* stat, cudaStrea
   return cudaGetLastError();
 }
 template <typename TX, typename TR>
-cudaError_t run(const RmsParams& p, int vec, long long* parts, float* stat, cudaStream_t st) {
-  constexpr int kFull = 16 / sizeof(TX);
-  if (vec >= kFull) return run_vec<TX, TR, kFull>(p, parts, stat, st);
-  if (vec >= 2) return run_vec<TX, TR, 2>(p, parts, stat, st);
-  return run_vec<TX, TR, 1>(p, parts, stat, st);
+cudaError_t run(const RmsParams& p, bool aligned, long long* parts, float* stat, cudaStream_t st) {
+  return aligned ? run_form<TX, TR, false>(p, parts, stat, st) : run_form<TX, TR, true>(p, parts, stat, st);
 }
 
 size_t round256(size_t x) { return (x + 255) & ~size_t(255); }
@@ -294,12 +302,12 @@ int ssm_rms_norm_bwd(int64_t rows, int64_t C, ssm_view total, const void* weight
   p.part = dweight != nullptr ? reinterpret_cast<float*>(at) : nullptr;
   float* stat = reinterpret_cast<float*>(at + round256((size_t)most_parts(rows) * C * 4));
   const int xb = dy.dtype == SSM_BF16 ? 2 : 4, tb = total.dtype == SSM_BF16 ? 2 : 4;
-  const int vec = rms_vec(C, xb, {{p.t, p.ts, tb}, {p.y, p.ys, xb}, {p.dt, p.dts, tb}, {p.dx, p.dxs, xb}, {p.dr, p.drs, tb}});
+  const bool aligned = rms_aligned(C, 16 / xb, {{p.t, p.ts, tb}, {p.y, p.ys, xb}, {p.dt, p.dts, tb}, {p.dx, p.dxs, xb}, {p.dr, p.drs, tb}});
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   long long parts = 0;
-  cudaError_t e = dy.dtype == SSM_F32      ? run<float, float>(p, vec, &parts, stat, st)
-                  : total.dtype == SSM_F32 ? run<__nv_bfloat16, float>(p, vec, &parts, stat, st)
-                                           : run<__nv_bfloat16, __nv_bfloat16>(p, vec, &parts, stat, st);
+  cudaError_t e = dy.dtype == SSM_F32      ? run<float, float>(p, aligned, &parts, stat, st)
+                  : total.dtype == SSM_F32 ? run<__nv_bfloat16, float>(p, aligned, &parts, stat, st)
+                                           : run<__nv_bfloat16, __nv_bfloat16>(p, aligned, &parts, stat, st);
   if (e == cudaSuccess && dweight != nullptr) {
     const unsigned grid = (unsigned)rms_ceil(C, 32);
     if (weight_dtype == SSM_BF16)

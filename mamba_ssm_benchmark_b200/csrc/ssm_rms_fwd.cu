@@ -12,89 +12,99 @@ int report_error(int code, const char* msg);
 
 namespace {
 
-template <typename TX, typename TR, int VEC, int K, bool FP8>
+template <typename TX, typename TR, int VEC, int K, bool FP8, bool RAGGED>
 __global__ void __launch_bounds__(kRmsThreads) rms_fwd(const __grid_constant__ RmsParams p, int wpr) {
-  constexpr int kRow = K * (Slot<TX, VEC>::kBytes + Slot<TR, VEC>::kBytes), kDepth = rms_depth(kRow);
+  using SX = Slot<TX, VEC, RAGGED>;
+  using SR = Slot<TR, VEC, RAGGED>;
   extern __shared__ __align__(16) unsigned char queue[];
-  __shared__ float2 red[2 * kRmsThreads / 32];
+  __shared__ float2 red[kRmsRed];
   Team team(wpr, red);
-  constexpr int nt = kRmsThreads;
-  const int teams = nt / 32 / wpr;
+  const int warps = blockDim.x >> 5, teams = warps / wpr, lane = team.lane;
+  constexpr int kStage = K * (SX::kWarp + SR::kWarp);     // a warp's bytes of a stage: K parts of x, K of the residual
+  clear_queue(queue, warps * kRmsDepth * kStage);
+  unsigned char* mine = queue + (threadIdx.x >> 5) * kRmsDepth * kStage;
   const long long step = (long long)gridDim.x * teams;
   long long row = (long long)blockIdx.x * teams + team.id;
-
+  const bool adds = p.r != nullptr;
+  auto c0 = [&](int k) { return (team.warp * 32 + k * team.size) * VEC; };
   auto fetch = [&](long long r, int stage) {
-    unsigned char* at = queue + (size_t)stage * kRow * nt;
+    unsigned char* at = mine + stage * kStage;
+    if (r < p.rows) {
+      const TX* x = static_cast<const TX*>(p.x) + r * p.xs;
+      const TR* res = static_cast<const TR*>(p.r) + r * p.rs;
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const int c = (team.tid + k * team.size) * VEC;
-      const bool ok = r < p.rows && c < p.C;
-      Slot<TX, VEC>::fetch(at + (size_t)k * Slot<TX, VEC>::kBytes * nt, static_cast<const TX*>(p.x) + (ok ? r * p.xs + c : 0), ok);
-      if (p.r != nullptr)
-        Slot<TR, VEC>::fetch(at + (size_t)(K * Slot<TX, VEC>::kBytes + k * Slot<TR, VEC>::kBytes) * nt,
-                             static_cast<const TR*>(p.r) + (ok ? r * p.rs + c : 0), ok);
+      for (int k = 0; k < K; ++k) {
+        SX::fetch(at + k * SX::kWarp, x, c0(k), p.C, lane);
+        if (adds) SR::fetch(at + K * SX::kWarp + k * SR::kWarp, res, c0(k), p.C, lane);
+      }
     }
     queue_commit();
   };
 #pragma unroll
-  for (int d = 0; d < kDepth; ++d) fetch(row + d * step, d);
-  float w[K][VEC];
+  for (int d = 0; d < kRmsDepth; ++d) fetch(row + d * step, d);
+  float2 w[K][VEC / 2];
 #pragma unroll
-  for (int k = 0; k < K; ++k) {
-    const int c = (team.tid + k * team.size) * VEC;
-    if (c < p.C) load_weight<VEC>(p, c, w[k]);
-  }
+  for (int k = 0; k < K; ++k) load_weight<VEC>(p, c0(k) + lane * VEC, p.C - c0(k) - lane * VEC, w[k]);
   int stage = 0;
   for (; row < p.rows; row += step) {             // the same count for all warps of a team
-    float v[K][VEC];
-    float ss = 0.0f;
-    queue_wait<kDepth - 1>();
-    const unsigned char* at = queue + (size_t)stage * kRow * nt;
+    const TX* x = static_cast<const TX*>(p.x) + row * p.xs;
+    const TR* res = static_cast<const TR*>(p.r) + row * p.rs;
+    float2 v[K][VEC / 2], ss = make_float2(0.0f, 0.0f);
+    queue_wait<kRmsDepth - 1>();
+    __syncwarp();                                 // a lane reads what others fetched
+    const unsigned char* at = mine + stage * kStage;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const int c = (team.tid + k * team.size) * VEC;
-      Slot<TX, VEC>::read(at + (size_t)k * Slot<TX, VEC>::kBytes * nt, v[k]);
-      if (p.r != nullptr) {
-        float r[VEC];
-        Slot<TR, VEC>::read(at + (size_t)(K * Slot<TX, VEC>::kBytes + k * Slot<TR, VEC>::kBytes) * nt, r);
+      SX::read(at + k * SX::kWarp, x, c0(k), lane, v[k]);
+      if (adds) {
+        float2 r[VEC / 2];
+        uint32_t t[SR::kWords];
+        SR::read(at + K * SX::kWarp + k * SR::kWarp, res, c0(k), lane, r);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) v[k][i] = to_f32(from_f32<TR>(v[k][i] + r[i]));   // t as it is kept
-        if (c < p.C) write_piece<TR, VEC>(static_cast<TR*>(p.t) + row * p.ts + c, v[k]);
+        for (int i = 0; i < VEC / 2; ++i) v[k][i] = add2(v[k][i], r[i]);
+        SR::pack(v[k], t);
+        SR::write(static_cast<TR*>(p.t) + row * p.ts, c0(k), p.C, lane, t);
+        SR::unpack(t, v[k]);                      // as it is kept
       }
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) ss = fmaf(v[k][i], v[k][i], ss);
+      for (int i = 0; i < VEC / 2; ++i) ss = fma2(v[k][i], v[k][i], ss);
     }
-    fetch(row + kDepth * step, stage);
-    stage = stage + 1 == kDepth ? 0 : stage + 1;
+    __syncwarp();
+    fetch(row + kRmsDepth * step, stage);
+    stage = stage + 1 == kRmsDepth ? 0 : stage + 1;
+    float rstd = 1.0f;
     if (!FP8 || p.norm) {
-      const float rstd = 1.0f / sqrtf(team.sum(ss, 0.0f).x * p.inv_c + p.eps);
+      rstd = 1.0f / sqrtf(team.sum(ss.x + ss.y) * p.inv_c + p.eps);
+      // in 8 bits rstd joins the scale: one product less
+      const float2 f = bc2(FP8 ? 1.0f : rstd);
 #pragma unroll
       for (int k = 0; k < K; ++k)
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) v[k][i] = v[k][i] * rstd * w[k][i];
+        for (int i = 0; i < VEC / 2; ++i) v[k][i] = FP8 ? mul2(v[k][i], w[k][i]) : mul2(mul2(v[k][i], f), w[k][i]);
     }
     if constexpr (FP8) {
       float big = 0.0f;
 #pragma unroll
       for (int k = 0; k < K; ++k)
-        if ((team.tid + k * team.size) * VEC < p.C) {
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) big = fmaxf(big, fabsf(v[k][i]));
-        }
-      const float scale = fmaxf(team.max(big), kRmsTiny) / kE4m3Max, inv = 1.0f / scale;
+        for (int i = 0; i < VEC / 2; ++i) big = fmaxf(big, fmaxf(fabsf(v[k][i].x), fabsf(v[k][i].y)));
+      // a zero row, and one whose root overflowed, is 0 (0 x inf is NaN and fmaxf passes over it)
+      const float scale = fmaxf(team.max(big) * rstd, kRmsTiny) / kE4m3Max;
+      const float2 inv = bc2(1.0f / scale), f = bc2(rstd);
       if (team.tid == 0) p.scale[row] = scale;
 #pragma unroll
       for (int k = 0; k < K; ++k) {
-        const int c = (team.tid + k * team.size) * VEC;
+        const int c = c0(k) + lane * VEC;
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) v[k][i] *= inv;
-        if (c < p.C) write_e4m3<VEC>(static_cast<uint8_t*>(p.y) + row * p.ys + c, v[k]);
+        for (int i = 0; i < VEC / 2; ++i) v[k][i] = mul2(mul2(v[k][i], f), inv);
+        if (c < p.C) write_e4m3<VEC>(static_cast<uint8_t*>(p.y) + row * p.ys + c, p.C - c, p.wide8, v[k]);
       }
     } else {
 #pragma unroll
       for (int k = 0; k < K; ++k) {
-        const int c = (team.tid + k * team.size) * VEC;
-        if (c < p.C) write_piece<TX, VEC>(static_cast<TX*>(p.y) + row * p.ys + c, v[k]);
+        uint32_t y[SX::kWords];
+        SX::pack(v[k], y);
+        SX::write(static_cast<TX*>(p.y) + row * p.ys, c0(k), p.C, lane, y);
       }
     }
   }
@@ -104,9 +114,9 @@ __global__ void __launch_bounds__(kRmsThreads) rms_fwd(const __grid_constant__ R
 // Rows that no team holds (above 8192 channels): a CTA passes over the row for the sum
 // of squares, for the largest value and for the result.
 template <typename TX, typename TR, bool FP8>
-__global__ void __launch_bounds__(512) rms_fwd_long(const __grid_constant__ RmsParams p) {
-  __shared__ float2 red[2 * 16];
-  Team team(16, red);
+__global__ void __launch_bounds__(kRmsThreads) rms_fwd_long(const __grid_constant__ RmsParams p) {
+  __shared__ float2 red[kRmsRed];
+  Team team(kRmsWarps, red);
   for (long long row = blockIdx.x; row < p.rows; row += gridDim.x) {
     const TX* x = static_cast<const TX*>(p.x) + row * p.xs;
     TR* t = static_cast<TR*>(p.t) + row * p.ts;
@@ -119,12 +129,10 @@ __global__ void __launch_bounds__(512) rms_fwd_long(const __grid_constant__ RmsP
       ss = fmaf(v, v, ss);
     }
     const bool norm = !FP8 || p.norm;
-    const float rstd = norm ? 1.0f / sqrtf(team.sum(ss, 0.0f).x * p.inv_c + p.eps) : 1.0f;
+    const float rstd = norm ? 1.0f / sqrtf(team.sum(ss) * p.inv_c + p.eps) : 1.0f;
     auto result = [&](int c) {
       if (!norm) return value(c);
-      float w[1];
-      load_weight<1>(p, c, w);
-      return value(c) * rstd * w[0];
+      return value(c) * rstd * weight_at(p, c);
     };
     if constexpr (FP8) {
       float big = 0.0f;
@@ -140,50 +148,37 @@ __global__ void __launch_bounds__(512) rms_fwd_long(const __grid_constant__ RmsP
 }
 
 // ---- host -----------------------------------------------------------------------------------
-template <typename TX, typename TR, int VEC, int K, bool FP8>
-cudaError_t launch(const RmsParams& p, int wpr, cudaStream_t st) {
-  constexpr int kRow = K * (Slot<TX, VEC>::kBytes + Slot<TR, VEC>::kBytes);
-  constexpr auto kern = rms_fwd<TX, TR, VEC, K, FP8>;
-  const int teams = kRmsThreads / 32 / wpr;
-  const size_t smem = (size_t)rms_depth(kRow) * kRow * kRmsThreads;
-  const int fit = ctas_per_sm<kern>(kRmsThreads, smem);
-  const long long grid = std::max<long long>(1, std::min<long long>(rms_ceil(p.rows, teams), 148LL * std::max(fit, 1)));
-  kern<<<(unsigned)grid, kRmsThreads, smem, st>>>(p, wpr);
+template <typename TX, typename TR, int K, bool FP8, bool RAGGED>
+cudaError_t launch(const RmsParams& p, RmsForm f, cudaStream_t st) {
+  constexpr int VEC = 16 / sizeof(TX);
+  using SX = Slot<TX, VEC, RAGGED>;
+  using SR = Slot<TR, VEC, RAGGED>;
+  constexpr auto kern = rms_fwd<TX, TR, VEC, K, FP8, RAGGED>;
+  const int threads = f.threads();
+  const size_t smem = (size_t)kRmsDepth * K * (SX::kWarp + SR::kWarp) * (threads / 32);
+  const int fit = std::max(1, ctas_per_sm_threads<kern>(threads, smem));
+  kern<<<(unsigned)std::min<long long>(rms_ceil(p.rows, f.teams()), 148LL * fit), threads, smem, st>>>(p, f.wpr);
   return cudaGetLastError();
 }
-template <typename TX, typename TR, int VEC, bool FP8>
-cudaError_t run_vec(const RmsParams& p, cudaStream_t st) {
-  const RmsForm f = rms_form(p.C, VEC, kRmsMost / VEC);
-  if constexpr (VEC >= 4) {
-    if (f.k == 1) return launch<TX, TR, VEC, 1, FP8>(p, f.wpr, st);
-    if (f.k == 2) return launch<TX, TR, VEC, 2, FP8>(p, f.wpr, st);
-    if (f.k == 3) return launch<TX, TR, VEC, 3, FP8>(p, f.wpr, st);
-    if (f.k == 4) return launch<TX, TR, VEC, 4, FP8>(p, f.wpr, st);
-  }
-  if constexpr (VEC == 4) {
-    if (f.k == 5 || f.k == 6) return launch<TX, TR, VEC, 6, FP8>(p, f.wpr, st);
-    if (f.k > 6) return launch<TX, TR, VEC, 8, FP8>(p, f.wpr, st);
-  }
-  if constexpr (VEC <= 2) {
-    if (f.k > 0 && f.k * VEC <= 8) return launch<TX, TR, VEC, 8 / VEC, FP8>(p, f.wpr, st);
-    if (f.k > 0 && f.k * VEC <= 16) return launch<TX, TR, VEC, 16 / VEC, FP8>(p, f.wpr, st);
-    if (f.k > 0) return launch<TX, TR, VEC, 32 / VEC, FP8>(p, f.wpr, st);
-  }
-  rms_fwd_long<TX, TR, FP8><<<(unsigned)std::min<long long>(p.rows, 148 * 4), 512, 0, st>>>(p);
+template <typename TX, typename TR, bool FP8, bool RAGGED>
+cudaError_t run_form(const RmsParams& p, cudaStream_t st) {
+  constexpr int VEC = 16 / sizeof(TX), kMany = kRmsMost / VEC;
+  const RmsForm f = rms_form(p.C, VEC, {kMany, kMany / 2, 1});
+  if (f.k == kMany) return launch<TX, TR, kMany, FP8, RAGGED>(p, f, st);
+  if (VEC == 4 && f.k == 2) return launch<TX, TR, 2, FP8, RAGGED>(p, f, st);
+  if (f.k == 1) return launch<TX, TR, 1, FP8, RAGGED>(p, f, st);
+  rms_fwd_long<TX, TR, FP8><<<(unsigned)std::min<long long>(p.rows, 148 * 4), kRmsThreads, 0, st>>>(p);
   return cudaGetLastError();
 }
 template <typename TX, typename TR, bool FP8>
-cudaError_t run(const RmsParams& p, int vec, cudaStream_t st) {
-  constexpr int kFull = 16 / sizeof(TX);
-  if (vec >= kFull) return run_vec<TX, TR, kFull, FP8>(p, st);
-  if (vec >= 2) return run_vec<TX, TR, 2, FP8>(p, st);
-  return run_vec<TX, TR, 1, FP8>(p, st);
+cudaError_t run(const RmsParams& p, bool aligned, cudaStream_t st) {
+  return aligned ? run_form<TX, TR, FP8, false>(p, st) : run_form<TX, TR, FP8, true>(p, st);
 }
 template <bool FP8>
-cudaError_t run_types(const RmsParams& p, int xd, int rd, int vec, cudaStream_t st) {
-  if (xd == SSM_F32) return run<float, float, FP8>(p, vec, st);
-  if (rd == SSM_F32) return run<__nv_bfloat16, float, FP8>(p, vec, st);
-  return run<__nv_bfloat16, __nv_bfloat16, FP8>(p, vec, st);
+cudaError_t run_types(const RmsParams& p, int xd, int rd, bool aligned, cudaStream_t st) {
+  if (xd == SSM_F32) return run<float, float, FP8>(p, aligned, st);
+  if (rd == SSM_F32) return run<__nv_bfloat16, float, FP8>(p, aligned, st);
+  return run<__nv_bfloat16, __nv_bfloat16, FP8>(p, aligned, st);
 }
 
 int fail(int code, const char* fmt, long long a = 0, long long b = 0) {
@@ -194,18 +189,12 @@ int fail(int code, const char* fmt, long long a = 0, long long b = 0) {
 
 }  // namespace
 
-// The widest vector (a power of two, at most 16 bytes of x) that divides the channels and at which every row starts
-// aligned to a vector, or to 16 bytes.
-int rms_vec(long long C, int xbytes, std::initializer_list<RmsSide> sides) {
-  int vec = 16 / xbytes;
-  while (C % vec != 0) vec /= 2;
-  for (const RmsSide& s : sides) {
-    if (s.ptr == nullptr) continue;
-    while (vec > 1 && (reinterpret_cast<uintptr_t>(s.ptr) % std::min(16, vec * s.bytes) != 0 ||
-                       s.stride * s.bytes % std::min(16, vec * s.bytes) != 0))
-      vec /= 2;
-  }
-  return vec;
+// Whether rows are whole vectors that start at multiples of 16 bytes.
+bool rms_aligned(long long C, int vec, std::initializer_list<RmsSide> sides) {
+  bool fits = C % vec == 0;
+  for (const RmsSide& s : sides)
+    fits = fits && (s.ptr == nullptr || (reinterpret_cast<uintptr_t>(s.ptr) % 16 == 0 && s.stride * s.bytes % 16 == 0));
+  return fits;
 }
 
 int rms_check(int64_t rows, int64_t C, const ssm_view& x, const ssm_view& residual, const void* weight, int32_t wdtype) {
@@ -251,10 +240,11 @@ static int forward(int64_t rows, int64_t C, ssm_view x, ssm_view residual, const
   p.inv_c = 1.0f / (float)C;
   p.norm = norm;
   const int xb = x.dtype == SSM_BF16 ? 2 : 4, rb = residual.dtype == SSM_BF16 ? 2 : 4;
-  const int vec = rms_vec(C, xb, {{x.ptr, p.xs, xb}, {p.r, p.rs, rb}, {p.t, p.ts, rb}, {p.y, p.ys, fp8 ? 1 : xb}});
+  const bool aligned = rms_aligned(C, 16 / xb, {{x.ptr, p.xs, xb}, {p.r, p.rs, rb}, {p.t, p.ts, rb}, {fp8 ? nullptr : p.y, p.ys, xb}});
+  p.wide8 = fp8 && ((reinterpret_cast<uintptr_t>(p.y) | (uintptr_t)p.ys) & 7) == 0;
   const int rd = residual.ptr != nullptr ? residual.dtype : x.dtype;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const cudaError_t e = fp8 ? run_types<true>(p, x.dtype, rd, vec, st) : run_types<false>(p, x.dtype, rd, vec, st);
+  const cudaError_t e = fp8 ? run_types<true>(p, x.dtype, rd, aligned, st) : run_types<false>(p, x.dtype, rd, aligned, st);
   if (e != cudaSuccess) return fail(SSM_ERR_CUDA, "rms_norm forward launch failed (error %lld)", (long long)e);
   return SSM_OK;
 }
