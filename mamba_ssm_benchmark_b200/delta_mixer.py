@@ -20,7 +20,7 @@ import torch.nn.functional as F
 
 from .conv import causal_conv1d
 from .delta import MAX_KEY_WIDTH, gated_delta_rule, gated_delta_state_update
-from .mixer import _Holder, _softplus_inverse
+from .mixer import _Holder, _softplus_inverse, project
 from .norm import group_norm
 
 
@@ -80,13 +80,14 @@ class GatedDeltaMixer(nn.Module):
                                ssm=torch.zeros(batch, self.heads, self.head_dim, self.head_dim, device=device,
                                                dtype=torch.float32))
 
-    def forward(self, u, state=None, pos=0):
+    def forward(self, u, state=None, pos=0, residual=None):
+        """The mixer of u, plus the residual where one is given; u as in ``MambaMixer.forward``."""
         del pos
-        Bsz, L, _ = u.shape
         H, d = self.heads, self.head_dim
-        xz = F.linear(u, self.in_proj.weight)
+        xz = project(self.in_proj, u)
+        Bsz, L, _ = xz.shape
         x, z = xz[..., :self.d_conv_in], xz[..., self.d_conv_in:]
-        gate = F.linear(u, self.gate_proj.weight).float()
+        gate = project(self.gate_proj, u).float()
         g = -torch.exp(self.A_log.float()) * F.softplus(gate[..., :H] + self.dt_bias.float())
         beta = torch.sigmoid(gate[..., H:])
         conv_state = None if state is None else state.conv
@@ -105,4 +106,4 @@ class GatedDeltaMixer(nn.Module):
                 state.ssm.copy_(last)
         o = group_norm(o.reshape(Bsz * L, self.d_inner), H, self.norm_weight, z=z.reshape(Bsz * L, self.d_inner),
                        center=False)
-        return F.linear(o.reshape(Bsz, L, self.d_inner), self.out_proj.weight)
+        return project(self.out_proj, o.reshape(Bsz, L, self.d_inner), residual)

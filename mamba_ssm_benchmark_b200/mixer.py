@@ -17,8 +17,9 @@ Per call the mixer runs one of three paths:
     and the final SSM state written back;
   * one token with a state (decode): ``causal_conv1d`` on the conv state plus
     ``selective_state_update``, both updating the state in place.
-The projections stay torch GEMMs.  ``GraphDecoder`` replays one decode step of a ``MambaLM`` as a
-CUDA graph.
+The projections stay torch GEMMs, unless ``MambaLM.quantize_fp8`` has put 8-bit weights in their places for
+answering (``linear_fp8`` on what ``rms_norm_fp8`` leaves).  The embedding, the norms with the residual's addition and the
+sampling run on this package's kernels too.  ``GraphDecoder`` replays one decode step of a ``MambaLM`` as a CUDA graph.
 """
 
 import math
@@ -29,8 +30,13 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from . import _native as nat
 from .conv import causal_conv1d
 from .decode import selective_state_update
+from .embed import embedding
+from .linear import Fp8Linear
+from .norm import rms_norm, rms_norm_fp8
+from .sampling import sample_tokens
 from .scan import selective_scan_fused
 
 
@@ -74,6 +80,15 @@ class _Holder(nn.Module):
         super().__init__()
         self.weight = nn.Parameter(torch.empty(weight_shape))
         self.bias = nn.Parameter(torch.empty(bias_shape)) if bias_shape is not None else None
+
+
+def project(holder, u, residual=None):
+    """u @ weight^T (+ residual).  With an 8-bit weight u may be the pair that ``rms_norm_fp8`` gives; the result is then in
+    the residual's dtype."""
+    if isinstance(holder, Fp8Linear):
+        return holder(u, residual=residual)
+    y = F.linear(u, holder.weight)
+    return y if residual is None else residual + y
 
 
 def _softplus_inverse(y):
@@ -163,15 +178,17 @@ class MambaMixer(nn.Module):
         return sum(t.numel() * t.element_size() for t in (state.conv, state.ssm))
 
     # -- forward --------------------------------------------------------------------------------
-    def forward(self, u, state=None, pos=0, return_delta=False):
+    def forward(self, u, state=None, pos=0, return_delta=False, residual=None):
+        """The mixer of u, plus the residual where one is given.  u: (B, L, d_model), or with 8-bit weights also the pair
+        (u8, scale) of ``rms_norm_fp8``."""
         del pos
-        xz = F.linear(u, self.in_proj.weight)
+        xz = project(self.in_proj, u)
         x, z = xz[..., :self.d_inner], xz[..., self.d_inner:]
-        if state is not None and u.shape[1] == 1:
+        if state is not None and xz.shape[1] == 1:
             y, delta = self._decode_step(x, z, state)
         else:
             y, delta = self._sequence(x, z, state, return_delta)
-        out = F.linear(y, self.out_proj.weight)
+        out = project(self.out_proj, y, residual)
         return (out, delta) if return_delta else out
 
     def _sequence(self, x, z, state, want_delta):
@@ -217,8 +234,36 @@ class RMSNorm(nn.Module):
         self.eps = eps
         self.weight = nn.Parameter(torch.ones(d))
 
+    def _fused(self, x):
+        """The kernels take x: on the GPU, in one of their types, which the weight has too."""
+        return x.is_cuda and x.dtype in nat.DTYPES and x.dtype == self.weight.dtype and x.numel() > 0
+
     def forward(self, x):
+        if self._fused(x):
+            return rms_norm(x, self.weight, eps=self.eps)
         return F.rms_norm(x.float(), (x.shape[-1],), eps=self.eps).to(x.dtype) * self.weight
+
+    def add(self, x, residual):
+        """(norm of x + residual, x + residual), in one pass over them."""
+        return rms_norm(x, self.weight, residual=residual, eps=self.eps)
+
+    def fp8(self, x):
+        """The norm of x in 8 bits: (values, scale of every row)."""
+        return rms_norm_fp8(x, self.weight, eps=self.eps)
+
+
+class TokenEmbedding(nn.Embedding):
+    """nn.Embedding whose lookup and gradient run on this package's kernels on the GPU."""
+
+    def forward(self, idx):
+        w = self.weight
+        if w.is_cuda and w.dtype in nat.DTYPES and idx.numel() > 0 and idx.device == w.device:
+            return embedding(idx, w)
+        return super().forward(idx)
+
+
+def _hooked(*modules):
+    return any(m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks for m in modules)
 
 
 def _delta_mixer(*args, **kw):
@@ -240,7 +285,20 @@ class MambaBlock(nn.Module):
         self.mlp = None
 
     def forward(self, x, state=None, pos=0):
+        if isinstance(self.mixer.in_proj, Fp8Linear):
+            return self.mixer(self.norm1.fp8(x), state, pos, residual=x)
         return x + self.mixer(self.norm1(x), state, pos)
+
+    def open(self, x):
+        """Whether ``inner`` computes what ``forward`` does of x and nobody watches the block's own result."""
+        return type(self) is MambaBlock and not isinstance(self.mixer.in_proj, Fp8Linear) and type(self.norm1) is RMSNorm \
+            and self.norm1._fused(x) and not _hooked(self, self.norm1)
+
+    def inner(self, h, x, state=None, pos=0):
+        """The block without its own addition: for the residual stream x + h (h None: x) the mixer's result and the stream,
+        so that the next norm adds them.  (h', x') with x' + h' what ``forward(x + h)`` gives."""
+        y, x = (self.norm1(x), x) if h is None else self.norm1.add(h, x)
+        return self.mixer(y, state, pos), x
 
 
 # ------------------------------------------------------------------------------------------------
@@ -265,7 +323,7 @@ class MambaLM(nn.Module):
                  discretization="zoh", selective=True, a_mode="s4d", mixer="mamba", head_dim=64):
         super().__init__()
         self.n_layers = n_layers
-        self.embed = nn.Embedding(vocab_size, d_model)
+        self.embed = TokenEmbedding(vocab_size, d_model)
         kw = dict(d_state=d_state, discretization=discretization, selective=selective, a_mode=a_mode) \
             if mixer == "mamba" else dict(head_dim=head_dim)
         self.blocks = nn.ModuleList(MambaBlock(d_model, mixer=mixer, expand=expand, d_conv=d_conv, **kw)
@@ -296,16 +354,45 @@ class MambaLM(nn.Module):
     def init_state(self, batch, max_len, device, dtype=torch.float32):
         return [block.mixer.init_state(batch, max_len, device, dtype) for block in self.blocks]
 
+    @torch.no_grad()
+    def quantize_fp8(self):
+        """Puts 8-bit weights (e4m3, a scale for every row) in the places of the blocks' projections and of the head, for
+        answering: decoding then reads a half or a quarter of the bytes.  In place; the model no longer trains.  The mixers'
+        small projections, convolutions and states and the embedding stay as they are.  Returns the model."""
+        for block in self.blocks:
+            for name in ("in_proj", "gate_proj", "out_proj"):
+                holder = getattr(block.mixer, name, None)
+                if holder is not None and not isinstance(holder, Fp8Linear):
+                    setattr(block.mixer, name, Fp8Linear(holder.weight))
+        if not isinstance(self.head, Fp8Linear):
+            self.head = Fp8Linear(self.head.weight)
+        return self
+
     def forward(self, idx, states=None, pos=0):
-        x = self.embed(idx)
+        x, h = self.embed(idx), None
+        state = (lambda i: None) if states is None else states.__getitem__
+        if all(isinstance(b, MambaBlock) and b.open(x) for b in self.blocks) and not _hooked(self.norm_f):
+            for i, block in enumerate(self.blocks):          # every norm adds what the mixer before it made
+                h, x = block.inner(h, x, state(i), pos)
+            return self.head(self.norm_f(x) if h is None else self.norm_f.add(h, x)[0])
         for i, block in enumerate(self.blocks):
-            x = block(x, states[i] if states is not None else None, pos)
+            x = block(x, state(i), pos)
+        if isinstance(self.head, Fp8Linear):
+            return self.head(self.norm_f.fp8(x), dtype=x.dtype)
         return self.head(self.norm_f(x))
 
     @torch.no_grad()
-    def generate(self, prompt, n_new, temperature=1.0, top_k=None, max_len=None, graph=False):
+    def generate(self, prompt, n_new, temperature=1.0, top_k=None, max_len=None, graph=False, top_p=None, min_p=None,
+                 uniforms=None):
         """Samples n_new tokens after ``prompt`` (B, T): one prefill pass with decode states, then one
-        decode step per token (a CUDA-graph replay each with ``graph=True``)."""
+        decode step per token (a CUDA-graph replay each with ``graph=True``).  With ``top_p``, ``min_p`` or ``uniforms`` ((B, n_new)
+        float32 in [0, 1): the random numbers of the answer) tokens come from ``sample_tokens``, whose settings may be given by row;
+        without, from ``torch.multinomial``."""
+        own = top_p is not None or min_p is not None or uniforms is not None
+        if own and uniforms is None:
+            uniforms = torch.rand(prompt.shape[0], n_new, device=prompt.device)
+        if uniforms is not None and tuple(uniforms.shape) != (prompt.shape[0], n_new):
+            raise ValueError(f"uniforms must be {(prompt.shape[0], n_new)}, got {tuple(uniforms.shape)}")
         Bsz, T = prompt.shape
         states = self.init_state(Bsz, max_len or T + n_new, prompt.device)
         logits = self(prompt, states, 0)
@@ -316,7 +403,10 @@ class MambaLM(nn.Module):
             advance = lambda tok, pos: self(tok, states, pos)
         tokens = [prompt]
         for i in range(n_new):
-            nxt = _sample(logits[:, -1], temperature, top_k)
+            if own:
+                nxt = sample_tokens(logits[:, -1], uniforms[:, i], temperature, top_k, top_p, min_p).unsqueeze(1)
+            else:
+                nxt = _sample(logits[:, -1], temperature, top_k)
             tokens.append(nxt)
             if i + 1 < n_new:
                 logits = advance(nxt, T + i)
