@@ -3,18 +3,22 @@
 // calls the C entry points of libssm_b200.so (include/ssm_b200.h).
 //
 // These operators are small enough in training and decoding that the host decides: as Python autograd functions
-// over ctypes a head norm of 8192 x 512 took 135 us forward and backward, 33 of them on the GPU; through here 85.  Arguments are
-// checked by the Python layer (delta.py, norm.py and so on); what arrives here has the right shapes, one device and unit
-// inner strides, except gradients, which autograd hands over as they are.
+// over ctypes a head norm of 8192 x 512 took 135 us forward and backward, 33 of them on the GPU; through here 85.  Arguments
+// of the delta rule and the group norm are checked by the Python layer (delta.py, norm.py); what arrives here has the right
+// shapes, one device and unit inner strides, except gradients, which autograd hands over as they are.
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/extension.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 
 #include <initializer_list>
+#include <limits>
 #include <optional>
 #include <string>
 #include <tuple>
+#include <type_traits>
+#include <variant>
+#include <vector>
 
 #include "ssm_b200.h"
 
@@ -29,8 +33,17 @@ void check(int rc, const char* what) {
   if (rc == SSM_OK) return;
   const std::string msg = std::string(what) + ": " + ssm_last_error_message();
   TORCH_CHECK_VALUE(rc != SSM_ERR_INVALID && rc != SSM_ERR_DTYPE, msg);
-  TORCH_CHECK(false, msg, " (status ", rc, ")");
+  TORCH_CHECK(false, msg + " (status " + std::to_string(rc) + ")");
 }
+// Messages are put together as strings: numbers written to a stream here end the process where the compiler's libstdc++ is
+// newer than the one that is loaded (its streams are then linked in, without the loaded one's locale).
+std::string text(at::IntArrayRef sizes) {
+  std::string s = "(";
+  for (size_t i = 0; i < sizes.size(); ++i) s += (i > 0 ? ", " : "") + std::to_string(sizes[i]);
+  return s + (sizes.size() == 1 ? ",)" : ")");
+}
+std::string text(const Tensor& t) { return t.defined() ? text(t.sizes()) : std::string("none"); }
+std::string text(at::ScalarType t) { return c10::toString(t); }
 
 int32_t code(const Tensor& t) { return t.scalar_type() == at::kBFloat16 ? SSM_BF16 : SSM_F32; }
 const void* data(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
@@ -235,6 +248,28 @@ Tensor gated_delta_step(const Tensor& state, const Tensor& q, const Tensor& k, c
   return o;
 }
 
+// ---- the operators around the mixers ------------------------------------------------------------------
+// Their arguments are checked here: in Python the checks of an 8-bit norm took longer than everything else (18 us a call for
+// a token, 10 this way).
+bool kernel_type(const Tensor& t) { return t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16; }
+Tensor kernel_typed(const Tensor& t) { return kernel_type(t) ? t : t.to(at::kFloat); }
+// unit stride along the last axis
+Tensor unit(const Tensor& t) { return t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous(); }
+Tensor as_rows(const Tensor& t) { return unit(t.dim() == 2 ? t : t.reshape({-1, t.size(-1)})); }
+Tensor shaped(const Tensor& t, at::IntArrayRef shape) { return t.sizes() == shape ? t : t.reshape(shape); }
+
+void needs_cuda(const char* what, const Tensor& t) {
+  TORCH_CHECK(t.is_cuda(), "the sm_100a ", what, " needs CUDA tensors (this package has no CPU path)");
+}
+void one_device(const Tensor& a, std::initializer_list<Tensor> others) {
+  for (const Tensor& t : others) TORCH_CHECK_VALUE(!t.defined() || t.device() == a.device(), "all tensors must be on one device");
+}
+void no_gradient(const char* what, std::initializer_list<Tensor> inputs) {
+  if (!at::GradMode::is_enabled()) return;
+  for (const Tensor& t : inputs)
+    TORCH_CHECK(!t.defined() || !t.requires_grad(), what, " has no gradient: call it under torch.no_grad()");
+}
+
 // ---- embedding ------------------------------------------------------------------------------------
 // idx: T dense ids; the result is (T, C).
 Tensor embedding_forward(const Tensor& idx, const Tensor& weight, double scale) {
@@ -271,13 +306,54 @@ struct Embedding : torch::autograd::Function<Embedding> {
 };
 
 Tensor embedding(const Tensor& idx, const Tensor& weight, double scale) {
+  TORCH_CHECK_VALUE(weight.dim() == 2 && weight.numel() > 0, "weight must be (vocabulary, channels) with no empty axis, got " + text(weight));
+  TORCH_CHECK_TYPE(idx.scalar_type() == at::kLong || idx.scalar_type() == at::kInt, "idx must be int64 or int32, got " + text(idx.scalar_type()));
+  TORCH_CHECK_VALUE(idx.numel() > 0, "idx must have no empty axis, got " + text(idx));
+  TORCH_CHECK_TYPE(kernel_type(weight), "weight must be float32 or bfloat16, got " + text(weight.scalar_type()));
+  needs_cuda("embedding", weight);
+  one_device(weight, {idx});
   plain("embedding", {weight});
-  return at::GradMode::is_enabled() && wants(weight) ? Embedding::apply(weight, idx, scale)
-                                                     : embedding_forward(idx, weight, scale);
+  const Tensor ids = idx.dim() == 1 && idx.is_contiguous() ? idx : idx.reshape({-1}).contiguous(), w = unit(weight);
+  const Tensor y = at::GradMode::is_enabled() && wants(w) ? Embedding::apply(w, ids, scale) : embedding_forward(ids, w, scale);
+  if (idx.dim() == 1) return y;
+  std::vector<int64_t> shape = idx.sizes().vec();
+  shape.push_back(weight.size(1));
+  return y.reshape(shape);
 }
 
 // ---- root-mean-square norm --------------------------------------------------------------------------
-// x, residual: (rows, C).  (y, total), total undefined without a residual.
+// The arguments as the kernels take them: x and residual (rows, C), the residual float32 or like x.
+struct RmsArgs {
+  Tensor x, residual, weight;
+  at::ScalarType y_type, total_type;          // what the caller gets
+  std::vector<int64_t> shape;
+  RmsArgs(const char* what, const Tensor& x0, const Maybe& w0, const Maybe& r0, double eps) {
+    TORCH_CHECK_VALUE(x0.dim() >= 1 && x0.numel() > 0, "x must be (..., C) with no empty axis, got " + text(x0));
+    const int64_t C = x0.size(-1);
+    residual = value(r0);
+    weight = value(w0);
+    TORCH_CHECK_VALUE(!residual.defined() || residual.sizes() == x0.sizes(), "residual must be shaped like x " + text(x0) + ", got " + text(residual));
+    TORCH_CHECK_VALUE(!weight.defined() || (weight.dim() == 1 && weight.size(0) == C), "weight must be (" + std::to_string(C) + ",), got " + text(weight));
+    TORCH_CHECK_VALUE(eps >= 0.0, "eps must not be negative, got " + std::to_string(eps));
+    for (const Tensor& t : {x0, residual, weight})
+      TORCH_CHECK_TYPE(!t.defined() || (t.is_floating_point() && t.scalar_type() != at::kDouble && t.element_size() > 1),
+                       "float64, 8-bit and integer tensors are not supported by the sm_100a kernels; use float32 or bfloat16");
+    needs_cuda(what, x0);
+    one_device(x0, {residual, weight});
+    y_type = total_type = x0.scalar_type();
+    shape = x0.sizes().vec();
+    x = as_rows(kernel_typed(x0));
+    if (residual.defined()) {
+      total_type = at::promote_types(y_type, residual.scalar_type());
+      if (residual.scalar_type() != at::kFloat && residual.scalar_type() != x.scalar_type()) residual = residual.to(at::kFloat);
+      residual = as_rows(residual);
+    }
+    if (weight.defined()) weight = kernel_typed(weight).contiguous();
+  }
+  static Tensor as(const Tensor& t, at::ScalarType type) { return t.scalar_type() == type ? t : t.to(type); }
+};
+
+// (y, total), total undefined without a residual.
 std::tuple<Tensor, Tensor> rms_forward(const Tensor& x, const Tensor& residual, const Tensor& weight, double eps) {
   const c10::cuda::CUDAGuard guard(x.device());
   const Tensor y = dense_like(x);
@@ -329,11 +405,21 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
   }
 };
 
-variable_list rms_norm(const Tensor& x, const Maybe& residual, const Maybe& weight, double eps) {
+// (y) or (y, total)
+variable_list rms_norm(const Tensor& x, const Maybe& weight, const Maybe& residual, double eps) {
+  const RmsArgs a("RMS norm", x, weight, residual, eps);
   plain("rms_norm", {x, value(residual), value(weight)});
-  if (at::GradMode::is_enabled() && (wants(x) || wants(residual) || wants(weight))) return RmsNorm::apply(x, residual, weight, eps);
-  const auto [y, total] = rms_forward(x, value(residual), value(weight), eps);
-  return total.defined() ? variable_list{y, total} : variable_list{y};
+  variable_list out;
+  if (at::GradMode::is_enabled() && (wants(a.x) || (a.residual.defined() && wants(a.residual)) || (a.weight.defined() && wants(a.weight)))) {
+    auto maybe = [](const Tensor& t) { return t.defined() ? Maybe(t) : Maybe(); };
+    out = RmsNorm::apply(a.x, maybe(a.residual), maybe(a.weight), eps);
+  } else {
+    const auto [y, total] = rms_forward(a.x, a.residual, a.weight, eps);
+    out = total.defined() ? variable_list{y, total} : variable_list{y};
+  }
+  out[0] = shaped(RmsArgs::as(out[0], a.y_type), a.shape);
+  if (out.size() > 1) out[1] = shaped(RmsArgs::as(out[1], a.total_type), a.shape);
+  return out;
 }
 
 // Rows of 8 bits start at multiples of 16 bytes, as ssm_linear_fp8 reads them.
@@ -343,23 +429,51 @@ Tensor rows8(int64_t rows, int64_t C, const Tensor& like) {
 }
 
 // (y8, scale) or (y8, scale, total)
-variable_list rms_norm_fp8(const Tensor& x, const Maybe& residual, const Maybe& weight, double eps, bool norm) {
-  plain(norm ? "rms_norm_fp8" : "quantize_fp8", {x, value(residual), value(weight)});
+variable_list rms_norm_fp8(const Tensor& x, const Maybe& weight, const Maybe& residual, double eps, bool norm) {
+  const char* what = norm ? "rms_norm_fp8" : "quantize_fp8";
+  no_gradient(what, {x, value(weight), value(residual)});
+  const RmsArgs a(what, x, weight, residual, eps);
+  plain(what, {x, a.residual, a.weight});
   const c10::cuda::CUDAGuard guard(x.device());
-  const Tensor r = value(residual), w = value(weight);
-  const Tensor y8 = rows8(x.size(0), x.size(1), x), scale = at::empty({x.size(0)}, x.options().dtype(at::kFloat));
-  Tensor total;
-  if (r.defined()) total = dense_like(r);
-  check(ssm_rms_norm_fp8(x.size(0), x.size(1), view(x), view(r), data(w), w.defined() ? code(w) : SSM_F32, (float)eps, norm,
-                         y8.mutable_data_ptr(), y8.stride(0), f32(scale), view(total), stream(x)),
+  const int64_t rows = a.x.size(0), C = a.x.size(1);
+  Tensor y8 = rows8(rows, C, a.x), scale = at::empty({rows}, a.x.options().dtype(at::kFloat)), total;
+  if (a.residual.defined()) total = dense_like(a.residual);
+  check(ssm_rms_norm_fp8(rows, C, view(a.x), view(a.residual), data(a.weight), a.weight.defined() ? code(a.weight) : SSM_F32,
+                         (float)eps, norm, y8.mutable_data_ptr(), y8.stride(0), f32(scale), view(total), stream(a.x)),
         "ssm_rms_norm_fp8");
-  return total.defined() ? variable_list{y8, scale, total} : variable_list{y8, scale};
+  if (a.shape.size() != 2) {
+    const std::vector<int64_t> outer(a.shape.begin(), a.shape.end() - 1);
+    y8 = outer.empty() ? y8.select(0, 0) : y8.unflatten(0, outer);
+    scale = scale.reshape(outer);
+  }
+  if (!total.defined()) return {y8, scale};
+  return {y8, scale, shaped(RmsArgs::as(total, a.total_type), a.shape)};
 }
 
 // ---- 8-bit products -----------------------------------------------------------------------------------
-Tensor linear_fp8(const Tensor& x8, const Tensor& x_scale, const Tensor& w8, const Tensor& w_scale, const Maybe& bias,
-                  const Maybe& residual, bool silu, bool bf16) {
-  plain("linear_fp8", {x8, x_scale, w8, w_scale, value(bias), value(residual)});
+Tensor linear_fp8(const Tensor& x8, const Tensor& x_scale, const Tensor& w8, const Tensor& w_scale, const Maybe& bias0, bool silu,
+                  const Maybe& residual0, std::optional<at::ScalarType> dtype) {
+  TORCH_CHECK_TYPE(x8.scalar_type() == at::kFloat8_e4m3fn && w8.scalar_type() == at::kFloat8_e4m3fn,
+                   "x8 and weight8 must be float8_e4m3fn, got " + text(x8.scalar_type()) + " and " + text(w8.scalar_type()));
+  TORCH_CHECK_VALUE(w8.dim() == 2 && x8.dim() >= 1 && x8.numel() > 0 && w8.numel() > 0,
+                    "x8 must be (..., K) and weight8 (N, K) with no empty axis, got " + text(x8) + " and " + text(w8));
+  const int64_t N = w8.size(0), K = w8.size(1);
+  TORCH_CHECK_VALUE(x8.size(-1) == K, "x8 must have weight8's " + std::to_string(K) + " columns, got " + text(x8));
+  const at::IntArrayRef outer = x8.sizes().slice(0, x8.dim() - 1);
+  TORCH_CHECK_VALUE(x_scale.sizes() == outer && w_scale.dim() == 1 && w_scale.size(0) == N, "the scales must be " + text(outer) + " and (" + std::to_string(N) + ",), got " + text(x_scale) + " and " + text(w_scale));
+  TORCH_CHECK_TYPE(x_scale.scalar_type() == at::kFloat && w_scale.scalar_type() == at::kFloat, "the scales must be float32");
+  Tensor bias = value(bias0), residual = value(residual0);
+  TORCH_CHECK_VALUE(!bias.defined() || (bias.dim() == 1 && bias.size(0) == N), "bias must be (" + std::to_string(N) + ",), got " + text(bias));
+  const at::ScalarType type = dtype.has_value() ? *dtype : residual.defined() ? residual.scalar_type() : at::kBFloat16;
+  TORCH_CHECK_TYPE(type == at::kFloat || type == at::kBFloat16, "dtype must be float32 or bfloat16, got " + text(type));
+  std::vector<int64_t> shape = outer.vec();
+  shape.push_back(N);
+  TORCH_CHECK_VALUE(!residual.defined() || (residual.sizes() == at::IntArrayRef(shape) && residual.scalar_type() == type),
+                    "residual must be " + text(shape) + " in " + text(type) + ", got " + text(residual));
+  no_gradient("linear_fp8", {x_scale, w_scale, bias, residual});
+  needs_cuda("products", x8);
+  one_device(x8, {x_scale, w8, w_scale, bias, residual});
+  plain("linear_fp8", {x8, x_scale, w8, w_scale, bias, residual});
   const c10::cuda::CUDAGuard guard(x8.device());
   auto rows = [](const Tensor& t) {                  // rows that start at multiples of 16 bytes
     const bool fits = (t.stride(1) == 1 || t.size(1) == 1) && (t.size(0) == 1 || (t.stride(0) % 16 == 0 && t.stride(0) >= t.size(1))) &&
@@ -370,25 +484,59 @@ Tensor linear_fp8(const Tensor& x8, const Tensor& x_scale, const Tensor& w8, con
     return u;
   };
   auto stride = [](const Tensor& t) { return t.size(0) == 1 ? (t.size(1) + 15) / 16 * 16 : t.stride(0); };
-  const Tensor x = rows(x8), w = rows(w8);
-  const Tensor y = at::empty({x.size(0), w.size(0)}, x_scale.options().dtype(bf16 ? at::kBFloat16 : at::kFloat));
-  check(ssm_linear_fp8(x.size(0), w.size(0), x.size(1), x.const_data_ptr(), stride(x), f32(x_scale), w.const_data_ptr(),
-                       stride(w), f32(w_scale), f32(value(bias)), silu, view(value(residual)), view(y), stream(x)),
+  const Tensor x = rows(x8.dim() == 2 ? x8 : x8.reshape({-1, K})), w = rows(w8), xs = x_scale.contiguous(), ws = w_scale.contiguous();
+  if (bias.defined()) bias = bias.to(at::kFloat).contiguous();
+  if (residual.defined()) residual = as_rows(residual);
+  const Tensor y = at::empty({x.size(0), N}, x_scale.options().dtype(type));
+  check(ssm_linear_fp8(x.size(0), N, K, x.const_data_ptr(), stride(x), f32(xs), w.const_data_ptr(), stride(w), f32(ws), f32(bias), silu,
+                       view(residual), view(y), stream(x)),
         "ssm_linear_fp8");
-  return y;
+  return shaped(y, shape);
 }
 
 // ---- sampling -------------------------------------------------------------------------------------
-// Settings: (B) float64 (top_k: int64) tensors, or the numbers beside them.
-Tensor sample_tokens(const Tensor& logits, const Tensor& uniforms, const Maybe& temperature, double temperature0, const Maybe& top_k,
-                     int64_t top_k0, const Maybe& top_p, double top_p0, const Maybe& min_p, double min_p0) {
-  plain("sample_tokens", {logits, uniforms});
-  const c10::cuda::CUDAGuard guard(logits.device());
-  const Tensor tokens = at::empty({logits.size(0)}, logits.options().dtype(at::kLong));
-  auto by_row = [](const Maybe& t) { return t.has_value() ? t->const_data_ptr<double>() : nullptr; };
-  check(ssm_sample_tokens(logits.size(0), logits.size(1), view(logits), uniforms.const_data_ptr<float>(), by_row(temperature),
-                          temperature0, top_k.has_value() ? top_k->const_data_ptr<int64_t>() : nullptr, top_k0, by_row(top_p),
-                          top_p0, by_row(min_p), min_p0, tokens.mutable_data_ptr<int64_t>(), stream(logits)),
+// A setting: none, a number, or a tensor with one for every row.
+template <typename N>
+using Setting = std::optional<std::variant<Tensor, N>>;
+template <typename N>
+struct Given {
+  Tensor rows;
+  N one;
+  Given(const char* name, const Setting<N>& s, const Tensor& logits, N none, N lo, N hi) : one(none) {
+    if (!s.has_value()) return;
+    if (const Tensor* t = std::get_if<Tensor>(&*s)) {
+      TORCH_CHECK_VALUE(t->dim() == 1 && t->size(0) == logits.size(0), std::string(name) + " must be a number or a (" + std::to_string(logits.size(0)) + ",) tensor, got " + text(*t));
+      one_device(logits, {*t});
+      rows = t->detach().to(std::is_same_v<N, double> ? at::kDouble : at::kLong).contiguous();
+    } else {
+      one = std::get<N>(*s);
+      TORCH_CHECK_VALUE(one >= lo && one <= hi, std::string(name) + " must be in " + std::to_string(lo) + " .. " + std::to_string(hi) + ", got " + std::to_string(one));
+    }
+  }
+  const N* by_row() const { return rows.defined() ? static_cast<const N*>(rows.const_data_ptr()) : nullptr; }
+};
+
+Tensor sample_tokens(const Tensor& logits0, const Tensor& uniforms, const Setting<double>& temperature, const Setting<int64_t>& top_k,
+                     const Setting<double>& top_p, const Setting<double>& min_p) {
+  TORCH_CHECK_VALUE(logits0.dim() == 2 && logits0.numel() > 0, "logits must be (B, V) with no empty axis, got " + text(logits0));
+  const int64_t B = logits0.size(0), V = logits0.size(1), most = 1 << 20;
+  TORCH_CHECK_VALUE(V <= most, "the vocabulary must be at most " + std::to_string(most) + ", got " + std::to_string(V));
+  TORCH_CHECK_VALUE(uniforms.dim() == 1 && uniforms.size(0) == B, "uniforms must be (" + std::to_string(B) + ",), got " + text(uniforms));
+  TORCH_CHECK_TYPE(logits0.is_floating_point() && logits0.scalar_type() != at::kDouble && logits0.element_size() > 1 &&
+                       uniforms.scalar_type() == at::kFloat,
+                   "logits must be float32 or bfloat16 and uniforms float32, got " + text(logits0.scalar_type()) + " and " + text(uniforms.scalar_type()));
+  const double inf = std::numeric_limits<double>::infinity();
+  const Given<double> t("temperature", temperature, logits0, 1.0, 0.0, inf), p("top_p", top_p, logits0, 1.0, 0.0, 1.0),
+      m("min_p", min_p, logits0, 0.0, 0.0, 1.0);
+  const Given<int64_t> k("top_k", top_k, logits0, 0, 0, (int64_t)1 << 62);
+  needs_cuda("sampling", logits0);
+  one_device(logits0, {uniforms});
+  plain("sample_tokens", {logits0, uniforms});
+  const c10::cuda::CUDAGuard guard(logits0.device());
+  const Tensor logits = unit(kernel_typed(logits0.detach())), u = uniforms.contiguous();
+  const Tensor tokens = at::empty({B}, logits.options().dtype(at::kLong));
+  check(ssm_sample_tokens(B, V, view(logits), u.const_data_ptr<float>(), t.by_row(), t.one, k.by_row(), k.one, p.by_row(), p.one,
+                          m.by_row(), m.one, tokens.mutable_data_ptr<int64_t>(), stream(logits)),
         "ssm_sample_tokens");
   return tokens;
 }

@@ -10,7 +10,7 @@ import torch
 import torch.nn as nn
 
 from . import _native as nat
-from .norm import _dense, quantize_fp8
+from .norm import quantize_fp8
 
 E4M3 = torch.float8_e4m3fn
 
@@ -21,43 +21,9 @@ def linear_fp8(x8, x_scale, weight8, weight_scale, bias=None, activation=None, r
     x8: (..., K) and weight8: (N, K) in float8_e4m3fn, rows that start at multiples of 16 bytes as ``quantize_fp8`` lays them
     out (others are copied); x_scale: (...), weight_scale: (N) float32; bias: (N) or None; activation: None or "silu";
     residual: shaped like y and in its dtype, or None.  Sums are float32."""
-    if x8.dtype != E4M3 or weight8.dtype != E4M3:
-        raise TypeError(f"x8 and weight8 must be float8_e4m3fn, got {x8.dtype} and {weight8.dtype}")
-    if weight8.dim() != 2 or x8.dim() < 1 or x8.numel() == 0 or weight8.numel() == 0:
-        raise ValueError(f"x8 must be (..., K) and weight8 (N, K) with no empty axis, got {tuple(x8.shape)} and {tuple(weight8.shape)}")
-    N, K = weight8.shape
-    shape = x8.shape[:-1]
-    if x8.shape[-1] != K:
-        raise ValueError(f"x8 must have weight8's {K} columns, got {tuple(x8.shape)}")
-    if x_scale.shape != shape or weight_scale.shape != (N,):
-        raise ValueError(f"the scales must be {tuple(shape)} and ({N},), got {tuple(x_scale.shape)} and {tuple(weight_scale.shape)}")
-    if x_scale.dtype != torch.float32 or weight_scale.dtype != torch.float32:
-        raise TypeError("the scales must be float32")
     if activation not in (None, "silu"):
         raise ValueError(f"activation must be 'silu' or None, got {activation!r}")
-    if bias is not None and bias.shape != (N,):
-        raise ValueError(f"bias must be ({N},), got {tuple(bias.shape)}")
-    if dtype is None:
-        dtype = residual.dtype if residual is not None else torch.bfloat16
-    if dtype not in nat.DTYPES:
-        raise TypeError(f"dtype must be float32 or bfloat16, got {dtype}")
-    if residual is not None and (residual.shape != (*shape, N) or residual.dtype != dtype):
-        raise ValueError(f"residual must be {(*shape, N)} in {dtype}, got {tuple(residual.shape)} in {residual.dtype}")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x_scale, weight_scale, bias, residual)):
-        raise RuntimeError("linear_fp8 has no gradient: call it under torch.no_grad()")
-    if not x8.is_cuda:
-        raise RuntimeError("the sm_100a products need CUDA tensors (this package has no CPU path)")
-    dev = x8.device
-    for t in (x_scale, weight8, weight_scale, bias, residual):
-        if t is not None and t.device != dev:
-            raise ValueError("all tensors must be on one device")
-    if bias is not None:
-        bias = bias.to(torch.float32).contiguous()
-    if residual is not None:
-        residual = _dense(residual.reshape(-1, N))
-    y = nat.glue().linear_fp8(x8.reshape(-1, K), x_scale.reshape(-1).contiguous(), weight8, weight_scale.contiguous(), bias,
-                              residual, activation == "silu", dtype == torch.bfloat16)
-    return y if len(shape) == 1 else y.reshape(*shape, N)
+    return nat.glue().linear_fp8(x8, x_scale, weight8, weight_scale, bias, activation is not None, residual, dtype)
 
 
 class Fp8Linear(nn.Module):

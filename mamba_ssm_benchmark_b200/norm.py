@@ -85,37 +85,6 @@ def group_norm(x, groups, weight=None, bias=None, eps=1e-5, activation=None, z=N
     return y if in_dtype == dtype else y.to(in_dtype)
 
 
-def _rows(x, weight, residual, eps, what):
-    """Checks shared by the RMS norms; (x, weight, residual) as the kernels take them, and the sum's dtype."""
-    if x.dim() < 1 or x.numel() == 0:
-        raise ValueError(f"x must be (..., C) with no empty axis, got {tuple(x.shape)}")
-    C = x.shape[-1]
-    if residual is not None and residual.shape != x.shape:
-        raise ValueError(f"residual must be shaped like x {tuple(x.shape)}, got {tuple(residual.shape)}")
-    if weight is not None and tuple(weight.shape) != (C,):
-        raise ValueError(f"weight must be ({C},), got {tuple(weight.shape)}")
-    if not eps >= 0.0:
-        raise ValueError(f"eps must not be negative, got {eps!r}")
-    for t in (x, residual):
-        if t is not None and (t.dtype == torch.float64 or not t.is_floating_point()):
-            raise TypeError(f"{t.dtype} is not supported by the sm_100a kernels; use float32 or bfloat16")
-    if not x.is_cuda:
-        raise RuntimeError(f"the sm_100a {what} needs CUDA tensors (this package has no CPU path)")
-    for t in (weight, residual):
-        if t is not None and t.device != x.device:
-            raise ValueError("all tensors must be on one device")
-    total = x.dtype if residual is None or residual.dtype == x.dtype else torch.promote_types(x.dtype, residual.dtype)
-    # the residual is float32 or like x: a narrower one is widened
-    x = x if x.dtype in nat.DTYPES else x.to(torch.float32)
-    if residual is not None:
-        if residual.dtype != torch.float32 and residual.dtype != x.dtype:
-            residual = residual.to(torch.float32)
-        residual = _dense(residual.reshape(-1, C))
-    if weight is not None:
-        weight = (weight if weight.dtype in nat.DTYPES else weight.to(torch.float32)).contiguous()
-    return _dense(x.reshape(-1, C)), weight, residual, total
-
-
 def rms_norm(x, weight=None, residual=None, eps=1e-5):
     """total = x + residual, y = total / sqrt(mean(total^2) + eps) * weight: y without a residual, (y, total) with one.
 
@@ -123,30 +92,8 @@ def rms_norm(x, weight=None, residual=None, eps=1e-5):
     weight: (C) or None.  y is in x's dtype, total in the wider of x's and the residual's; what is normed is total as it is
     kept.  Differentiable with respect to x, weight and residual, whose gradients are one tensor where x and residual
     have one dtype (as those of x + residual are)."""
-    shape, dtype = x.shape, x.dtype
-    x, weight, residual, wide = _rows(x, weight, residual, eps, "RMS norm")
-    out = nat.glue().rms_norm(x, residual, weight, float(eps))
-    y = out[0] if len(shape) == 2 else out[0].reshape(shape)
-    y = y if y.dtype == dtype else y.to(dtype)
-    if residual is None:
-        return y
-    total = out[1] if len(shape) == 2 else out[1].reshape(shape)
-    return y, total if total.dtype == wide else total.to(wide)
-
-
-def _fp8(x, weight, residual, eps, norm, what):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, residual)):
-        raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad()")
-    shape = x.shape
-    x, weight, residual, wide = _rows(x, weight, residual, eps, what)
-    out = nat.glue().rms_norm_fp8(x, residual, weight, float(eps), norm)
-    y8, scale = out[0], out[1]
-    if len(shape) != 2:
-        y8, scale = y8.unflatten(0, shape[:-1]) if len(shape) > 1 else y8[0], scale.reshape(shape[:-1])
-    if residual is None:
-        return y8, scale
-    total = out[2].reshape(shape)
-    return y8, scale, total if total.dtype == wide else total.to(wide)
+    out = nat.glue().rms_norm(x, weight, residual, eps)
+    return out[0] if residual is None else tuple(out)
 
 
 def rms_norm_fp8(x, weight=None, residual=None, eps=1e-5):
@@ -154,9 +101,9 @@ def rms_norm_fp8(x, weight=None, residual=None, eps=1e-5):
 
     y8: float8_e4m3fn, shaped like x, rows that start at multiples of 16 bytes; scale: (...) float32, the row's largest |y|
     (at least 1e-30) / 448; y is about y8 * scale.  No gradient."""
-    return _fp8(x, weight, residual, eps, True, "rms_norm_fp8")
+    return tuple(nat.glue().rms_norm_fp8(x, weight, residual, eps, True))
 
 
 def quantize_fp8(x):
     """x (..., C) in 8 bits with a scale for every row: (x8, scale) as ``rms_norm_fp8`` gives them.  No gradient."""
-    return _fp8(x, None, None, 0.0, False, "quantize_fp8")
+    return tuple(nat.glue().rms_norm_fp8(x, None, None, 0.0, False))
