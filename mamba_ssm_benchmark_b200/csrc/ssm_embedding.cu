@@ -14,7 +14,7 @@
 
 #include "ssm_b200.h"
 #include "ssm_launch.cuh"
-#include "ssm_vec.cuh"
+#include "ssm_rows.cuh"
 
 namespace cg = cooperative_groups;
 
@@ -25,10 +25,12 @@ int* device_error_word();
 
 namespace {
 
-using ssm::Raw;
+using ssm::Slot;
+using ssm::add2;
+using ssm::bc2;
+using ssm::mul2;
 using ssm::from_f32;
 using ssm::to_f32;
-using ssm::vec_store;
 
 constexpr int kBadToken = 2;        // bit of the device error word
 
@@ -57,43 +59,39 @@ __device__ __forceinline__ long long token_at(const EmbedParams& p, long long t)
 }
 
 // ---- forward ----------------------------------------------------------------------------------
-// A warp takes kAhead vectors a lane of one row, so that as many loads are on their way; a row has `pieces` warps.
+// A warp takes kAhead units a lane of one row, so that as many loads are on their way; a row has `pieces` warps.
 constexpr int kAhead = 4;
-template <typename T, int VEC, bool SCALE>
+template <typename T, bool RAGGED, bool SCALE>
 __global__ void __launch_bounds__(256) embed_fwd(const __grid_constant__ EmbedParams p, int pieces) {
+  constexpr int VEC = 16 / sizeof(T);
+  using Part = Slot<T, VEC, RAGGED>;
   const long long item = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
   const long long t = item / pieces;
   if (t >= p.T) return;
-  const int lane = threadIdx.x & 31, c0 = ((int)(item - t * pieces) * kAhead * 32 + lane) * VEC;
+  const int lane = threadIdx.x & 31, c0 = (int)(item - t * pieces) * kAhead * Part::kTaken;
   const long long v = token_at(p, t);
   const bool bad = v < 0 || v >= p.V;
+  if (bad && lane == 0 && p.err != nullptr) atomicOr(p.err, kBadToken);
+  const T* row = static_cast<const T*>(p.w) + (bad ? 0 : v) * p.ws;
   T* out = static_cast<T*>(p.y) + t * p.ys;
-  if (bad) {
-    if (lane == 0 && p.err != nullptr) atomicOr(p.err, kBadToken);
+  uint4 raw[kAhead];
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k)
-      for (int i = 0; i < VEC; ++i)
-        if (c0 + k * 32 * VEC + i < p.C) out[c0 + k * 32 * VEC + i] = from_f32<T>(__int_as_float(0x7fc00000));
-    return;
-  }
-  const T* row = static_cast<const T*>(p.w) + v * p.ws;
-  Raw<T, VEC> raw[kAhead];
-#pragma unroll
-  for (int k = 0; k < kAhead; ++k)
-    if (c0 + k * 32 * VEC < p.C) raw[k].load(row + c0 + k * 32 * VEC);
+  for (int k = 0; k < kAhead; ++k) raw[k] = Part::take(row, c0 + k * Part::kTaken, p.C, lane);
 #pragma unroll
   for (int k = 0; k < kAhead; ++k) {
-    const int c = c0 + k * 32 * VEC;
-    if (c >= p.C) continue;
-    if constexpr (SCALE) {
-      float x[VEC];
-      raw[k].widen(x);
+    const int c = c0 + k * Part::kTaken;
+    if (c >= p.C) continue;                            // the same for the warp
+    uint32_t w[4];
+    Part::taken(raw[k], row, c, w);
+    if (SCALE || bad) {
+      float2 x[VEC / 2];
+      Part::unpack(w, x);
+      const float2 scale = bc2(bad ? __int_as_float(0x7fc00000) : p.scale);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) x[i] *= p.scale;
-      vec_store<T, VEC>(out + c, x);
-    } else {
-      *reinterpret_cast<Raw<T, VEC>*>(out + c) = raw[k];
+      for (int i = 0; i < VEC / 2; ++i) x[i] = bad ? scale : mul2(x[i], scale);
+      Part::pack(x, w);
     }
+    Part::write(out, c, min(p.C, c + Part::kTaken), lane, w);
   }
 }
 
@@ -216,11 +214,15 @@ constexpr int kSumThreads = 256, kLongest = 64, kRows = 8, kFill = 32;      // k
 // Chunk q starts at the first place from q len on where another token begins, or at q len inside a run of more than len.
 // The sum of a run of equal tokens goes to the table where the chunk holds all of it, else to the chunk's partial
 // rows: 0 where the run comes from the chunk before, 1 where it starts here and goes on.
-template <typename T, int VEC>
+template <typename T, bool RAGGED>
 __global__ void __launch_bounds__(kSumThreads) embed_sum(const __grid_constant__ EmbedParams p) {
   __shared__ uint2 near[2 * kLongest + 1];             // from the place before the chunk's first possible one
   __shared__ int bound[2];
-  const int c = ((int)(blockIdx.x % p.slabs) * blockDim.x + threadIdx.x) * VEC;
+  constexpr int VEC = 16 / sizeof(T);
+  using Part = Slot<T, VEC, RAGGED>;
+  const int lane = threadIdx.x & 31;
+  const int c0 = ((int)(blockIdx.x % p.slabs) * (blockDim.x >> 5) + (threadIdx.x >> 5)) * Part::kTaken;      // the warp's channels
+  const int c1 = min(p.C, c0 + Part::kTaken);
   const long long item = blockIdx.x / p.slabs;
   constexpr uint32_t kNone = 0xffffffffu;
   // Chunks to sum and rows to zero take turns, so that reads and writes mix.
@@ -229,10 +231,10 @@ __global__ void __launch_bounds__(kSumThreads) embed_sum(const __grid_constant__
   if ((item + 1) * fills / items > fill) {             // rows without a token
     const uint32_t named = p.named[fill];
     const int rows = (int)min((long long)kFill, p.V - fill * kFill);
-    const float zero[VEC] = {};
-    if (c < p.C)
+    const uint32_t zero[4] = {0, 0, 0, 0};
+    if (c0 < p.C)
       for (int i = 0; i < rows; ++i)
-        if (!(named >> i & 1)) vec_store<T, VEC>(static_cast<T*>(p.y) + (fill * kFill + i) * p.ys + c, zero);
+        if (!(named >> i & 1)) Part::write(static_cast<T*>(p.y) + (fill * kFill + i) * p.ys, c0, c1, lane, zero);
     return;
   }
   const long long t0 = chunk * p.len;
@@ -258,40 +260,49 @@ __global__ void __launch_bounds__(kSumThreads) embed_sum(const __grid_constant__
     const uint32_t v = at[n - 1].x;
     if (v < p.V && outer[1] == v && !(at[0].x == v && outer[0] == v)) p.joins[1 + atomicAdd(p.joins, 1)] = (int)chunk;
   }
-  if (c >= p.C) return;
-  float acc[VEC] = {};
+  if (c0 >= p.C) return;
+  float2 acc[VEC / 2] = {};
   int start = 0;                                       // of the run
   auto flush = [&](int end) {
     const uint32_t v = at[start].x;
     if (v < p.V) {
       const bool from = start == 0 && outer[0] == v, to = end == n && outer[1] == v;
       if (!from && !to) {
+        uint32_t w[4];
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) acc[i] *= p.scale;
-        vec_store<T, VEC>(static_cast<T*>(p.y) + (long long)v * p.ys + c, acc);
+        for (int i = 0; i < VEC / 2; ++i) acc[i] = mul2(acc[i], bc2(p.scale));
+        Part::pack(acc, w);
+        Part::write(static_cast<T*>(p.y) + (long long)v * p.ys, c0, c1, lane, w);
       } else {
-        float* out = p.part + ((size_t)chunk * 2 + (from ? 0 : 1)) * p.C + c;
+        float* out = p.part + ((size_t)chunk * 2 + (from ? 0 : 1)) * p.C;
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) out[i] = acc[i];
+        for (int i = 0; i < VEC / 2; ++i) {
+          const int c = c0 + lane * VEC + 2 * i;
+          if (c < c1) out[c] = acc[i].x;
+          if (c + 1 < c1) out[c + 1] = acc[i].y;
+        }
       }
     }
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) acc[i] = 0.0f;
+    for (int i = 0; i < VEC / 2; ++i) acc[i] = make_float2(0.0f, 0.0f);
     start = end;
   };
+  auto row = [&](int i) { return static_cast<const T*>(p.w) + (long long)at[i].y * p.ws; };
   for (int i0 = 0; i0 < n; i0 += kRows) {
-    Raw<T, VEC> raw[kRows];
+    uint4 raw[kRows];
 #pragma unroll
     for (int i = 0; i < kRows; ++i)
-      if (i0 + i < n) raw[i].load(static_cast<const T*>(p.w) + (long long)at[i0 + i].y * p.ws + c);
+      if (i0 + i < n) raw[i] = Part::take(row(i0 + i), c0, p.C, lane);
 #pragma unroll
     for (int i = 0; i < kRows; ++i) {
       if (i0 + i >= n) break;
       if (at[i0 + i].x != at[start].x) flush(i0 + i);
-      float x[VEC];
-      raw[i].widen(x);
+      uint32_t w[4];
+      float2 x[VEC / 2];
+      Part::taken(raw[i], row(i0 + i), c0, w);
+      Part::unpack(w, x);
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) acc[j] += x[j];
+      for (int j = 0; j < VEC / 2; ++j) acc[j] = add2(acc[j], x[j]);
     }
   }
   flush(n);
@@ -364,30 +375,29 @@ int check_side(const char* what, const ssm_view& v) {
   }
   return SSM_OK;
 }
-// The widest vector, at most 16 bytes, that divides the channels and at which the rows of both tensors start aligned.
-int width(int64_t C, int es, const ssm_view& a, const ssm_view& b) {
-  int vec = 16 / es;
-  auto fits = [&](const ssm_view& v) {
-    return reinterpret_cast<uintptr_t>(v.ptr) % (vec * es) == 0 && v.batch_stride % vec == 0;
-  };
-  while (vec > 1 && (C % vec != 0 || !fits(a) || !fits(b))) vec /= 2;
-  return vec;
+// Whether the rows of both tensors are whole 16 bytes that start at multiples of 16.
+bool aligned(int64_t C, int es, const ssm_view& a, const ssm_view& b) {
+  auto fits = [&](const ssm_view& v) { return reinterpret_cast<uintptr_t>(v.ptr) % 16 == 0 && v.batch_stride * es % 16 == 0; };
+  return C * es % 16 == 0 && fits(a) && fits(b);
 }
+// Channels of a warp, by a unit of 16 bytes to a lane.
+int warp_channels(int es, bool ragged) { return (ragged ? 31 : 32) * 16 / es; }
 
-template <typename T, int VEC>
+template <typename T, bool RAGGED>
 cudaError_t run_fwd(const EmbedParams& p, cudaStream_t st) {
-  const int pieces = (int)ceil_div(p.C, 32 * VEC * kAhead);
+  const int pieces = (int)ceil_div(p.C, warp_channels(sizeof(T), RAGGED) * kAhead);
   const unsigned grid = (unsigned)ceil_div(p.T * pieces, 8);
-  if (p.scale == 1.0f) embed_fwd<T, VEC, false><<<grid, 256, 0, st>>>(p, pieces);
-  else embed_fwd<T, VEC, true><<<grid, 256, 0, st>>>(p, pieces);
+  if (p.scale == 1.0f) embed_fwd<T, RAGGED, false><<<grid, 256, 0, st>>>(p, pieces);
+  else embed_fwd<T, RAGGED, true><<<grid, 256, 0, st>>>(p, pieces);
   return cudaGetLastError();
 }
-template <typename T, int VEC>
+template <typename T, bool RAGGED>
 cudaError_t run_bwd(EmbedParams p, cudaStream_t st) {
-  // as few CTAs over the channels as there can be, with whole warps of equal parts
-  p.slabs = (int)ceil_div(p.C, kSumThreads * VEC);
-  const int threads = (int)ceil_div(ceil_div(ceil_div(p.C, VEC), p.slabs), 32) * 32;
-  embed_sum<T, VEC><<<(unsigned)((p.chunks + ceil_div(p.V, kFill)) * p.slabs), threads, 0, st>>>(p);
+  // as few CTAs over the channels as there can be, with warps in equal parts
+  const long long warps = ceil_div(p.C, warp_channels(sizeof(T), RAGGED));
+  p.slabs = (int)ceil_div(warps, kSumThreads / 32);
+  const int threads = (int)ceil_div(warps, p.slabs) * 32;
+  embed_sum<T, RAGGED><<<(unsigned)((p.chunks + ceil_div(p.V, kFill)) * p.slabs), threads, 0, st>>>(p);
   if (p.chunks > 1) {
     const long long most = (p.chunks - 1) * ceil_div(p.C, 128);
     embed_join<T><<<(unsigned)std::min<long long>(most, 148 * 4), 32 * kJoinWarps, 0, st>>>(p);
@@ -395,12 +405,9 @@ cudaError_t run_bwd(EmbedParams p, cudaStream_t st) {
   return cudaGetLastError();
 }
 template <typename T>
-cudaError_t run(const EmbedParams& p, bool bwd, int vec, cudaStream_t st) {
-  if constexpr (sizeof(T) == 2)
-    if (vec == 8) return bwd ? run_bwd<T, 8>(p, st) : run_fwd<T, 8>(p, st);
-  if (vec == 4) return bwd ? run_bwd<T, 4>(p, st) : run_fwd<T, 4>(p, st);
-  if (vec == 2) return bwd ? run_bwd<T, 2>(p, st) : run_fwd<T, 2>(p, st);
-  return bwd ? run_bwd<T, 1>(p, st) : run_fwd<T, 1>(p, st);
+cudaError_t run(const EmbedParams& p, bool bwd, bool ragged, cudaStream_t st) {
+  if (ragged) return bwd ? run_bwd<T, true>(p, st) : run_fwd<T, true>(p, st);
+  return bwd ? run_bwd<T, false>(p, st) : run_fwd<T, false>(p, st);
 }
 
 // Places to a chunk: as many as leave every SM a dozen CTAs, 8 to kLongest.
@@ -452,11 +459,12 @@ int ssm_embedding_fwd(int64_t T, int64_t V, int64_t C, const void* idx, int32_t 
   p.C = (int)C;
   p.scale = scale;
   p.err = ssm::device_error_word();
-  const int es = weight.dtype == SSM_BF16 ? 2 : 4, vec = width(C, es, weight, y);
-  if (ceil_div(T * ceil_div(C, 32 * vec * kAhead), 8) > 0x7fffffffLL)
+  const int es = weight.dtype == SSM_BF16 ? 2 : 4;
+  const bool ragged = !aligned(C, es, weight, y);
+  if (ceil_div(T * ceil_div(C, warp_channels(es, ragged) * kAhead), 8) > 0x7fffffffLL)
     return fail(SSM_ERR_INVALID, "embedding: shape out of range (tokens %lld, channels %lld)", T, C);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const cudaError_t e = es == 2 ? run<__nv_bfloat16>(p, false, vec, st) : run<float>(p, false, vec, st);
+  const cudaError_t e = es == 2 ? run<__nv_bfloat16>(p, false, ragged, st) : run<float>(p, false, ragged, st);
   return e == cudaSuccess ? SSM_OK : fail(SSM_ERR_CUDA, "embedding forward launch failed (error %lld)", (long long)e);
 }
 
@@ -495,8 +503,9 @@ int ssm_embedding_bwd(int64_t T, int64_t V, int64_t C, const void* idx, int32_t 
   p.scale = scale;
   p.len = chunk_len(T, C);
   p.chunks = ceil_div(T, p.len);
-  const int es = dy.dtype == SSM_BF16 ? 2 : 4, vec = width(C, es, dy, dweight);
-  if ((p.chunks + ceil_div(V, kFill)) * ceil_div(C, kSumThreads * vec) > 0x7fffffffLL)
+  const int es = dy.dtype == SSM_BF16 ? 2 : 4;
+  const bool ragged = !aligned(C, es, dy, dweight);
+  if ((p.chunks + ceil_div(V, kFill)) * ceil_div(C, warp_channels(es, ragged)) > 0x7fffffffLL)
     return fail(SSM_ERR_INVALID, "embedding: shape out of range (tokens %lld, channels %lld)", T, C);
   unsigned char* at = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(workspace) + 255) & ~uintptr_t(255));
   uint2* a = reinterpret_cast<uint2*>(at);
@@ -511,7 +520,7 @@ int ssm_embedding_bwd(int64_t T, int64_t V, int64_t C, const void* idx, int32_t 
   p.sorted = passes & 1 ? a : b;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (int rc = run_sort(p, a, b, passes, st)) return rc;
-  const cudaError_t e = es == 2 ? run<__nv_bfloat16>(p, true, vec, st) : run<float>(p, true, vec, st);
+  const cudaError_t e = es == 2 ? run<__nv_bfloat16>(p, true, ragged, st) : run<float>(p, true, ragged, st);
   return e == cudaSuccess ? SSM_OK : fail(SSM_ERR_CUDA, "embedding backward launch failed (error %lld)", (long long)e);
 }
 

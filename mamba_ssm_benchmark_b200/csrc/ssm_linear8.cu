@@ -517,12 +517,15 @@ int ssm_linear_fp8(int64_t tokens, int64_t channels, int64_t K, const void* x8, 
   // Columns of a tile: the fewest that hold the tokens, where these are few (or y's rows do not allow the other form); else as
   // many channels as leave every SM a tile.
   const bool by_token = tokens > 64 && aligned(16) && channels * es % 16 == 0;
-  int tn = by_token ? 256 : 16;
-  if (by_token) {
-    while (tn > 64 && (channels + tn - 1) / tn * ((tokens + kRows - 1) / kRows) < 148) tn /= 2;
+  const int64_t cols = by_token ? channels : tokens, lanes = by_token ? tokens : channels;
+  int tn = 16;
+  if (cols > 64) {
+    tn = 256;
+    while (tn > 64 && (cols + tn - 1) / tn * ((lanes + kRows - 1) / kRows) < 148) tn /= 2;
   } else {
-    while (tn < 256 && tn < tokens) tn *= 2;
+    while (tn < cols) tn *= 2;
   }
+  if (by_token && tn < 64) tn = 64;
   p.wide = aligned(32);
   const bool made = by_token ? encode_rows8(&p.ta, x8, tokens, K, x_stride, kRows) && encode_rows8(&p.tb, w8, channels, K, w_stride, tn)
                              : encode_rows8(&p.ta, w8, channels, K, w_stride, kRows) && encode_rows8(&p.tb, x8, tokens, K, x_stride, tn);
