@@ -17,6 +17,7 @@
 
 #include <algorithm>
 #include <cstdio>
+#include <type_traits>
 
 #include "ssm_b200.h"
 #include "ssm_launch.cuh"
@@ -59,14 +60,14 @@ constexpr int kMargins = 4;
 
 struct SampleSmem {
   double exp2[kTable];
-  u64 part[32], slot[2];
+  u64 part[32], part2[kWarps], slot[2], slot2[2];
   u64 list[kList];
   u64 kept[kWarps];                   // by warp: the weight of its kept tokens
-  u64 slot2[2];
   uint32_t count[kBins], upto[kBins];
   int size;                           // of the list
   int first[1 + 2 * kMargins];        // the first bin at which a sum over the bins passes a value
-  u64 cut;
+  u64 cut, rest;                      // rest: what the drawn token's place is short of where its warp's tokens start
+  int owner;                          // that warp
   alignas(16) float logits[4];        // the slice
 };
 
@@ -80,25 +81,28 @@ __device__ __forceinline__ float key_logit(u64 key) {
   return __uint_as_float(b & 0x80000000u ? b & 0x7fffffffu : ~b);
 }
 
-// A weight in whole units: 2^42 2^y, y = (l - top) rate.  2^y = 2^k 2^(j/1024) 2^r, |r| <= 2^-11: the Taylor polynomial of
-// degree 3 is within (ln 2 / 2048)^4 / 24 = 6e-16 of 2^r.  No branch: y is held above -60, where the weight is zero (a NaN,
-// of infinities, is too), and the largest logit's weight is set.  Ten operations in double, a quarter of the instructions.
+// A weight in whole units: 2^42 2^y, y = (l - top) rate, for finite top and l <= top.  2^y = 2^k 2^(j/1024) 2^r, |r| <= 2^-11:
+// the Taylor polynomial of degree 3 is within (ln 2 / 2048)^4 / 24 = 6e-16 of 2^r.  y is held above -60, where the weight is
+// zero, by its high word: of two negative numbers the larger has the smaller one.
 struct Weights {
   const double* table;
-  float top;                          // the largest logit
-  double top2, rate;                  // the same; log2(e) / temperature
-  __device__ u64 operator()(float l) const {
+  double top, rate;                   // the largest logit; log2(e) / temperature, held within 1e-290 .. 1e290
+  __device__ void set(float top_, double temperature) {
+    top = top_;
+    rate = fmin(fmax(1.4426950408889634 / temperature, 1e-290), 1e290);
+  }
+  __device__ __forceinline__ u64 operator()(float l) const {
     constexpr double kLn2 = 0.69314718055994531, kC2 = kLn2 * kLn2 / 2, kC3 = kLn2 * kLn2 * kLn2 / 6;
     constexpr double kShift = 6755399441055744.0 / kTable;   // 1.5 2^52 / 1024: y is rounded to 1024ths
-    const double y = fmax(((double)l - top2) * rate, -60.0);
+    const double raw = ((double)l - top) * rate;
+    const double y = __hiloint2double((int)min((uint32_t)__double2hiint(raw), 0xc04e0000u), __double2loint(raw));      // -60
     const double t = y + kShift;
     const int i = __double2loint(t);                       // 1024 y, rounded
     const double r = y - (t - kShift);
     const double q = fma(r, fma(r, fma(r, kC3, kC2), kLn2), 1.0);
     const double step = table[i & (kTable - 1)];
     const double scaled = __hiloint2double(__double2hiint(step) + (((i >> 10) + kBits) << 20), __double2loint(step));
-    const u64 units = (u64)__double_as_longlong(fma(scaled, q, 4503599627370496.0)) & ((1ull << 52) - 1);
-    return l == top ? kOne : units;
+    return (u64)__double_as_longlong(fma(scaled, q, 4503599627370496.0)) & ((1ull << 52) - 1);
   }
 };
 
@@ -232,9 +236,10 @@ struct Sampler {
   const T* logits;                    // of the row
   int row, ctas, lane, warp, base, per, first, last, turn;
   Weights weight;
-  float bin_rate;                     // bins to a logit
+  float top, bin_rate;                // the largest logit; bins to a logit
+  bool infinite;
 
-  __device__ Sampler(const SampleParams& p_, SampleSmem& s_) : p(p_), s(s_), cluster(cg::this_cluster()), turn(0) {
+  __device__ Sampler(const SampleParams& p_, SampleSmem& s_) : p(p_), s(s_), cluster(cg::this_cluster()), turn(0), infinite(false) {
     ctas = (int)cluster.num_blocks();
     row = (int)blockIdx.x / ctas;
     logits = static_cast<const T*>(p.logits) + row * p.stride;
@@ -248,15 +253,22 @@ struct Sampler {
     last = min(end, first + per);
     weight.table = s.exp2;
   }
-  // Four logits from i on; -inf past the warp's last.
+  // Four logits from i on; -inf past the warp's last.  In a row with infinite logits these alone count (`infinite`): 0, and -inf
+  // the others.
   __device__ void load(int i, float (&l)[4]) const {
+    constexpr float kInf = __builtin_huge_valf();
     if (p.wide && i + 4 <= last) {
       ssm::load4(logits + i, l);
     } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) l[j] = i + j < last ? ssm::to_f32(logits[i + j]) : -__int_as_float(0x7f800000);
+      for (int j = 0; j < 4; ++j) l[j] = i + j < last ? ssm::to_f32(logits[i + j]) : -kInf;
+    }
+    if (infinite) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) l[j] = l[j] == kInf ? 0.0f : -kInf;
     }
   }
+  __device__ void keep(int i, const float (&l)[4]) { *reinterpret_cast<float4*>(s.logits + (i - base)) = make_float4(l[0], l[1], l[2], l[3]); }
   // f(i, l[4]) for this lane's tokens
   template <typename F>
   __device__ __forceinline__ void each(F f) {
@@ -275,13 +287,19 @@ struct Sampler {
       if (HALVES) return (u64)max((uint32_t)(a >> 32), (uint32_t)(b >> 32)) << 32 | max((uint32_t)a, (uint32_t)b);
       return MAX ? max(a, b) : a + b;
     };
+    auto of_warp = [&](u64 v) {
+      if constexpr (HALVES) {
+        return (u64)__reduce_max_sync(0xffffffffu, (uint32_t)(v >> 32)) << 32 | __reduce_max_sync(0xffffffffu, (uint32_t)v);
+      } else {
 #pragma unroll
-    for (int m = 16; m >= 1; m /= 2) v = f(v, __shfl_xor_sync(0xffffffffu, v, m));
+        for (int m = 16; m >= 1; m /= 2) v = f(v, __shfl_xor_sync(0xffffffffu, v, m));
+        return v;
+      }
+    };
+    v = of_warp(v);
     if (lane == 0) s.part[warp] = v;
     __syncthreads();
-    v = lane < kWarps ? s.part[lane] : 0;
-#pragma unroll
-    for (int m = 16; m >= 1; m /= 2) v = f(v, __shfl_xor_sync(0xffffffffu, v, m));
+    v = of_warp(lane < kWarps ? s.part[lane] : 0);
     if (ctas == 1) {
       __syncthreads();
       return v;
@@ -293,31 +311,15 @@ struct Sampler {
     turn ^= 1;
     return v;
   }
-  // Two sums at once.
-  __device__ void join2(u64& x, u64& y) {
-    u64 all;
-    block_scan(x, s.part, &all);
-    x = all;
-    block_scan(y, s.part, &all);
-    y = all;
-    if (ctas == 1) return;
-    if (threadIdx.x == 0) s.slot[turn] = x, s.slot2[turn] = y;
-    cluster.sync();
-    x = y = 0;
-    for (int r = 0; r < ctas; ++r) {
-      x += *cluster.map_shared_rank(&s.slot[turn], r);
-      y += *cluster.map_shared_rank(&s.slot2[turn], r);
-    }
-    turn ^= 1;
-  }
   __device__ void sync() {
     if (ctas == 1) __syncthreads();
     else cluster.sync();
   }
 
+  __device__ __forceinline__ float distance(float l) const { return (top - l) * bin_rate; }
   // The bin of a logit by its distance to the largest; kBins: so far below that its weight is zero.
   __device__ int bin(float l) const {
-    const float z = l == weight.top ? 0.0f : (weight.top - l) * bin_rate;
+    const float z = distance(l);
     return z < (float)kBins ? (int)z : kBins;
   }
 
@@ -370,36 +372,78 @@ struct Sampler {
       n[3] += c.w;
     }
   }
-  // The tokens of bins lo .. hi that rank at least as high as `cut`, in the first CTA's list (in any order); f(l, bin, in)
-  // for four tokens at a time, `in` where they rank so.
-  template <typename F>
-  __device__ void gather(int lo, int hi, u64 cut, F f) {
+  // The tokens of bins lo .. hi that rank at least as high as `cut` to the first CTA's list (in any order).  SUMS: of the tokens
+  // that rank so, the weight of all and of those in bins below lo.
+  template <bool SUMS>
+  __device__ void gather(int lo, int hi, u64 cut, u64& total, u64& before) {
     int* size = cluster.map_shared_rank(&s.size, 0);
     u64* list = cluster.map_shared_rank(s.list, 0);
-    each([&](int i, const float (&l)[4]) {
-      int b[4];
-      bool in[4];
+    const float from = (float)lo, to = (float)(hi + 1);
+    total = before = 0;
+    auto body = [&](int i, const float (&l)[4], auto cuts) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        b[j] = bin(l[j]);
-        in[j] = b[j] < kBins && (cut == 0 || rank_key(l[j], i + j) >= cut);
-        if (b[j] >= lo && b[j] <= hi && in[j]) {
+        const float z = distance(l[j]);
+        const bool in = !cuts || rank_key(l[j], i + j) >= cut;
+        if (SUMS) {
+          const u64 w = weight(l[j]);
+          if (in) total += w;
+          if (in && z < from) before += w;
+        }
+        if (z >= from && z < to && in) {
           const int at = atomicAdd(size, 1);
           if (at < kList) list[at] = rank_key(l[j], i + j);
         }
       }
-      f(l, b, in);
-    });
+    };
+    if (cut != 0) each([&](int i, const float (&l)[4]) { body(i, l, std::true_type()); });
+    else each([&](int i, const float (&l)[4]) { body(i, l, std::false_type()); });
   }
-  // This thread's token of the first CTA's list, largest first (0: none); for all CTAs of the cluster to call.
-  __device__ u64 sorted() {
-    sync();                               // the list is written
-    const int n = min(s.size, kList);     // 0 but in the first CTA
-    int pow2 = 32;
-    while (pow2 < n) pow2 *= 2;
-    const u64 key = (int)threadIdx.x < n ? s.list[threadIdx.x] : 0;
+  // x and y summed over the cluster, once the list is written: one barrier of the cluster for both.
+  __device__ void sums(u64& x, u64& y) {
+#pragma unroll
+    for (int m = 16; m >= 1; m /= 2) {
+      x += __shfl_xor_sync(0xffffffffu, x, m);
+      y += __shfl_xor_sync(0xffffffffu, y, m);
+    }
+    if (lane == 0) s.part[warp] = x, s.part2[warp] = y;
     __syncthreads();
-    return block_sort(key, s.list, pow2);
+    if (warp == 0) {
+      x = lane < kWarps ? s.part[lane] : 0;
+      y = lane < kWarps ? s.part2[lane] : 0;
+#pragma unroll
+      for (int m = 16; m >= 1; m /= 2) {
+        x += __shfl_xor_sync(0xffffffffu, x, m);
+        y += __shfl_xor_sync(0xffffffffu, y, m);
+      }
+      if (lane == 0) s.slot[turn] = x, s.slot2[turn] = y;
+    }
+    sync();                               // the list and the sums are written
+    x = y = 0;
+    for (int r = 0; r < ctas; ++r) {
+      x += *cluster.map_shared_rank(&s.slot[turn], r);
+      y += *cluster.map_shared_rank(&s.slot2[turn], r);
+    }
+    turn ^= 1;
+  }
+  // This thread's token of the first CTA's list, which is written, largest first (0: none; in the other CTAs all).
+  __device__ u64 sorted() {
+    const int n = min(s.size, kList);
+    const u64 key = (int)threadIdx.x < n ? s.list[threadIdx.x] : 0;
+    if (n > 128) {
+      int pow2 = 256;
+      while (pow2 < n) pow2 *= 2;
+      __syncthreads();
+      return block_sort(key, s.list, pow2);
+    }
+    // few: every token's rank by comparing it with all
+    int rank = 0;
+    if (key != 0)
+      for (int i = 0; i < n; ++i) rank += s.list[i] > key;
+    __syncthreads();
+    if (key != 0) s.list[rank] = key;
+    __syncthreads();
+    return (int)threadIdx.x < n ? s.list[threadIdx.x] : 0;
   }
 };
 
@@ -419,7 +463,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_many(const __grid_constant
   for (int i = a.first + 4 * a.lane; i < a.last; i += 128) {
     float l[4];
     a.load(i, l);
-    if (p.cached) *reinterpret_cast<float4*>(s.logits + (i - a.base)) = make_float4(l[0], l[1], l[2], l[3]);
+    if (p.cached) a.keep(i, l);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       high = fmaxf(high, l[j]);
@@ -430,7 +474,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_many(const __grid_constant
   // both in one: the largest, and the smallest as the largest of the negated
   const u64 ends = a.template join<true, true>(nan ? ~0ull : (rank_key(high, 0) >> 32) << 32 | rank_key(-low, 0) >> 32);
   const bool none = no_token(ends, set.temperature);
-  a.weight.top = key_logit(ends);
+  a.top = key_logit(ends);
   if (none || !(set.temperature > 0.0)) {                 // the same for the whole cluster
     u64 best = 0;
     if (!none)
@@ -444,15 +488,24 @@ __global__ void __launch_bounds__(kThreads, 2) sample_many(const __grid_constant
     a.sync();                                             // peers read this CTA's slots until here
     return;
   }
-  a.weight.top2 = a.weight.top;
-  a.weight.rate = 1.4426950408889634 / set.temperature;
+  float spread = a.top + key_logit(ends << 32);           // between the largest and the smallest above -inf
+  if (a.top == kInf) {
+    a.infinite = true;
+    a.top = spread = 0.0f;
+    for (int i = a.first + 4 * a.lane; p.cached && i < a.last; i += 128) {
+      float l[4];
+      a.load(i, l);
+      a.keep(i, l);
+    }
+  }
+  a.weight.set(a.top, set.temperature);
   const bool top_k = set.top_k > 0 && set.top_k < p.V, top_p = set.top_p < 1.0;
   u64 cut = 0;
   bool summed = false;                                    // s.kept is known
   if (top_k || top_p) {
     // 31 temperatures below the largest a weight is zero
-    const float range = fminf(31.0f * (float)set.temperature, a.weight.top + key_logit(ends << 32));
-    a.bin_rate = ((float)kBins - 0.01f) / range;
+    const float range = fminf(31.0f * (float)set.temperature, spread);
+    a.bin_rate = fminf(((float)kBins - 0.01f) / range, 3e38f);
     uint32_t n[kPer];
     a.count_bins(n);
     u64 all, run = block_scan((u64)n[0] + n[1] + n[2] + n[3], s.part, &all) - n[0] - n[1] - n[2] - n[3];
@@ -468,10 +521,11 @@ __global__ void __launch_bounds__(kThreads, 2) sample_many(const __grid_constant
     if (borders) last = s.first[0];
     const int listed = (int)s.upto[last];                 // tokens up to it
     if (listed <= kList) {                                // what is kept of the top_k: all in the list
-      a.gather(0, last, 0, [](const float (&)[4], const int (&)[4], const bool (&)[4]) {});
-      u64 key = a.sorted();
+      u64 none0, none1;
+      a.template gather<false>(0, last, 0, none0, none1);
       a.sync();
-      if (!leader) return;
+      if (!leader) return;                                // nobody reads this CTA's memory any more
+      u64 key = a.sorted();
       const long long k = top_k ? set.top_k : p.V;
       u64 w = key != 0 && t < k ? a.weight(key_logit(key)) : 0, total;
       run = block_scan(w, s.part, &total);
@@ -491,7 +545,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_many(const __grid_constant
       if (listed - before > kList) {
         cut = a.template bisect<false>(0, (u64)set.top_k);
       } else {
-        a.gather(last, last, 0, [](const float (&)[4], const int (&)[4], const bool (&)[4]) {});
+        u64 none0, none1;
+        a.template gather<false>(last, last, 0, none0, none1);
+        a.sync();
         const u64 key = a.sorted();
         if (leader && t == (int)set.top_k - before - 1) s.cut = key;
         a.sync();
@@ -537,22 +593,14 @@ __global__ void __launch_bounds__(kThreads, 2) sample_many(const __grid_constant
           fits = (int)(s.upto[hi] - (lo > 0 ? s.upto[lo - 1] : 0)) <= most;
         }
         if (!fits) continue;
-        total = 0;
-        u64 before = 0;
-        a.gather(lo, hi, cut, [&](const float (&l)[4], const int (&bin)[4], const bool (&in)[4]) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const u64 w = a.weight(l[j]);
-            total += in[j] ? w : 0;
-            before += in[j] && bin[j] < lo ? w : 0;
-          }
-        });
+        u64 before;
+        a.template gather<true>(lo, hi, cut, total, before);
         u64 mine = before;                                // of this warp
 #pragma unroll
         for (int m = 16; m >= 1; m /= 2) mine += __shfl_xor_sync(0xffffffffu, mine, m);
         if (a.lane == 0) s.kept[a.warp] = mine;
+        a.sums(total, before);
         u64 key = a.sorted();
-        a.join2(total, before);
         const u64 reach = set.reach(total), w = key != 0 ? a.weight(key_logit(key)) : 0;
         u64 sum;
         upto = before + block_scan(w, s.part, &sum);
@@ -571,7 +619,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_many(const __grid_constant
           if (key >= cut && at >= 0 && at < p.slice) atomicAdd(&s.kept[at / a.per], a.weight(key_logit(key)));
           summed = a.weight(key_logit(cut)) >= set.least;  // min_p cuts nothing off
         }
-        a.sync();
+        __syncthreads();
       }
       if (!found) {
         total = a.template above<true>(cut, 0);
@@ -608,39 +656,37 @@ __global__ void __launch_bounds__(kThreads, 2) sample_many(const __grid_constant
       total += v;
     }
   }
+  // the warp whose tokens hold the drawn one; its CTA goes over them together
   const u64 target = set.draw(total);
-  if (before <= target && target < before + sum) {        // one warp of the cluster
-    for (int i0 = a.first; i0 < a.last; i0 += 128) {
-      const int i = i0 + 4 * a.lane;
-      float l[4];
-      if (i >= a.last) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) l[j] = -kInf;
-      } else if (p.cached) {
-        ssm::load4(s.logits + (i - a.base), l);
+  if (t == 0) s.owner = -1;
+  __syncthreads();
+  if (a.lane == 0 && before <= target && target < before + sum) {
+    s.owner = a.warp;
+    s.rest = target - before;
+  }
+  __syncthreads();
+  if (s.owner >= 0) {
+    const int begin = a.base + s.owner * a.per, end = min(min(p.V, a.base + p.slice), begin + a.per), each = (a.per + kThreads - 1) / kThreads;
+    const u64 rest = s.rest;
+    auto at = [&](int j) -> u64 {                         // of this thread's j-th token
+      const int i = begin + t * each + j;
+      if (i >= end) return 0;
+      float l;
+      if (p.cached) {
+        l = s.logits[i - a.base];
       } else {
-        a.load(i, l);
+        l = ssm::to_f32(a.logits[i]);
+        if (a.infinite) l = l == kInf ? 0.0f : -kInf;
       }
-      u64 w[4], mine = 0;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) mine += w[j] = kept(i + j, l[j]);
-      u64 run = mine;
-#pragma unroll
-      for (int m = 1; m < 32; m *= 2) {
-        const u64 up = __shfl_up_sync(0xffffffffu, run, m);
-        if (a.lane >= m) run += up;
-      }
-      const uint32_t passed = __ballot_sync(0xffffffffu, before + run > target);
-      if (passed != 0) {
-        if (a.lane == __ffs(passed) - 1) {
-          u64 at = before + run - mine;
-          int j = 0;
-          while (j < 3 && at + w[j] <= target) at += w[j++];
-          p.token[a.row] = i + j;
-        }
-        break;
-      }
-      before += __shfl_sync(0xffffffffu, run, 31);
+      const u64 w = a.weight(l);
+      return (cut == 0 || rank_key(l, i) >= cut) && w >= set.least ? w : 0;
+    };
+    u64 own = 0, all;
+    for (int j = 0; j < each; ++j) own += at(j);
+    u64 run = block_scan(own, s.part, &all) - own;
+    for (int j = 0; run <= rest && j < each; ++j) {
+      run += at(j);
+      if (run > rest) p.token[a.row] = begin + t * each + j;
     }
   }
   a.sync();
