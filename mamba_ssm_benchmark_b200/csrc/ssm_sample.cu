@@ -9,7 +9,7 @@
 // is off by at most 2^-43 of the largest; what rounds to zero is never drawn.
 //
 // Up to kFew tokens: a thread each, sorted by rank in registers.  More: a cluster of up to eight CTAs shares a row, a slice
-// of tokens each, kept in shared memory where it fits.  A histogram of the logits' distance to the largest says which
+// of tokens each, kept in shared memory where two CTAs to an SM have the room.  A histogram of the logits' distance to the largest says which
 // bins can hold the border of top_k (exactly) or of top_p (the bins' masses to a part in ten thousand); the few tokens
 // of these bins are sorted by one CTA, against exact sums of what lies before them.  Where a bin holds more than kList
 // tokens (thousands of equal logits) the border is found by bisection of the rank.
@@ -272,11 +272,20 @@ struct Sampler {
   // f(i, l[4]) for this lane's tokens
   template <typename F>
   __device__ __forceinline__ void each(F f) {
-    for (int i = first + 4 * lane; i < last; i += 128) {
-      float l[4];
-      if (p.cached) ssm::load4(s.logits + (i - base), l);
-      else load(i, l);
-      f(i, l);
+    if (p.cached) {
+      for (int i = first + 4 * lane; i < last; i += 128) {
+        float l[4];
+        ssm::load4(s.logits + (i - base), l);
+        f(i, l);
+      }
+    } else {                              // from L2 or memory: the next ones on their way
+      float next[4];
+      load(first + 4 * lane, next);
+      for (int i = first + 4 * lane; i < last; i += 128) {
+        const float l[4] = {next[0], next[1], next[2], next[3]};
+        load(i + 128, next);
+        f(i, l);
+      }
     }
   }
 
@@ -698,8 +707,7 @@ int fail(int code, const char* fmt, long long a = 0, long long b = 0) {
   snprintf(msg, sizeof(msg), fmt, a, b);
   return ssm::report_error(code, msg);
 }
-constexpr int kCached = 45 * 1024;    // logits that a CTA keeps (180 KB)
-constexpr int kTwo = 19 * 1024;       // logits that each of two CTAs on an SM keeps
+constexpr int kCached = 19 * 1024;    // logits that each of two CTAs on an SM keeps (76 KB); more are read again
 
 }  // namespace
 
@@ -737,10 +745,10 @@ extern "C" int ssm_sample_tokens(int64_t B, int64_t V, ssm_view logits, const fl
     const cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? SSM_OK : fail(SSM_ERR_CUDA, "sample_tokens launch failed (error %lld)", (long long)e);
   }
-  // CTAs to a row: what lets two on an SM keep their slices in shared memory, and more where few rows leave SMs idle
+  // CTAs to a row: as many as run at once.  A cluster's barriers cost a row as much as its passes (256 x 131072 by top-p: 300 us
+  // with eight CTAs to a row, 158 with one).
   int ctas = 1;
-  while (ctas < 8 && V > (int64_t)ctas * kTwo) ctas *= 2;
-  while (ctas < 8 && V >= (int64_t)ctas * 4096 && B * ctas * 2 <= 148) ctas *= 2;
+  while (ctas < 8 && V >= (int64_t)ctas * 4096 && B * ctas * 2 <= 296) ctas *= 2;
   p.slice = (int)((V + ctas - 1) / ctas + 3) & ~3;
   p.cached = p.slice <= kCached;
   const int unit = p.bf16 ? 8 : 16;                        // bytes of four logits
