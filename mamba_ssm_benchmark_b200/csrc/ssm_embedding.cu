@@ -132,15 +132,11 @@ __global__ void __launch_bounds__(1024) embed_sort(const __grid_constant__ Embed
     uint2 x[kHeld];
     if (held) {
 #pragma unroll
-      for (int i = 0; i < kHeld; ++i)
-        if (first + 32 * i + lane < last) x[i] = item(first + 32 * i + lane);
+      for (int i = 0; i < kHeld; ++i) x[i] = item(min(first + 32 * i + lane, p.T - 1));      // no branch between the loads
     }
     for (int i = threadIdx.x; i < kSortWarps * kBins / 4; i += 1024) reinterpret_cast<uint4*>(s.count)[i] = make_uint4(0, 0, 0, 0);
     __syncthreads();
-    auto count = [&](uint32_t token) {
-      atomicAdd(&s.count[warp][token >> shift & (kBins - 1)], 1u);
-      if (pass == 0 && token < p.V) atomicOr(p.named + (token >> 5), 1u << (token & 31));
-    };
+    auto count = [&](uint32_t token) { atomicAdd(&s.count[warp][token >> shift & (kBins - 1)], 1u); };
     if (held) {
 #pragma unroll
       for (int i = 0; i < kHeld; ++i)
@@ -185,7 +181,14 @@ __global__ void __launch_bounds__(1024) embed_sort(const __grid_constant__ Embed
     __syncthreads();
     auto place = [&](bool live, uint2 v) {
       const uint32_t bin = live ? v.x >> shift & (kBins - 1) : kBins;      // lanes past the end share a bin of their own
-      const uint32_t same = __match_any_sync(0xffffffffu, bin);
+      // the lanes of the same bin, bit by bit (__match_any_sync takes its time by the number of values: 65536 places of
+      // mostly different bins 8.2 us, this way 6.3)
+      uint32_t same = 0xffffffffu;
+#pragma unroll
+      for (int i = 0; i <= kDigit; ++i) {
+        const uint32_t set = __ballot_sync(0xffffffffu, bin >> i & 1);
+        same &= bin >> i & 1 ? set : ~set;
+      }
       const uint32_t to = live ? s.count[warp][bin] + __popc(same & ((1u << lane) - 1)) : 0;
       __syncwarp();
       if (live && lane == __ffs(same) - 1) s.count[warp][bin] += __popc(same);
@@ -205,6 +208,13 @@ __global__ void __launch_bounds__(1024) embed_sort(const __grid_constant__ Embed
     }
     __threadfence();
     cluster.sync();                                    // the next pass reads what every CTA wrote, and counts anew
+  }
+  // a bit for every token that occurs, where its places start
+  const uint2* out = passes & 1 ? a : b;
+  const uint32_t none = 0xffffffffu;
+  for (long long t = rank * 1024 + threadIdx.x; t < p.T; t += ctas * 1024) {
+    const uint32_t v = out[t].x, before = t > 0 ? out[t - 1].x : none;
+    if (v != before && v < p.V) atomicOr(p.named + (v >> 5), 1u << (v & 31));
   }
 }
 
@@ -417,9 +427,14 @@ int chunk_len(int64_t T, int64_t C) {
 }
 
 int run_sort(const EmbedParams& p, uint2* a, uint2* b, int passes, cudaStream_t st) {
-  // the barriers of a cluster cost more than its CTAs save while one CTA's warps take a few dozen places each
-  const int ctas = p.T <= 4096 ? 1 : 8;
+  // The barriers of a cluster cost more than its CTAs save while one CTA's warps take a few dozen places each; with many
+  // places their scattered stores, one a clock and SM, take most of the time.
+  const int ctas = p.T <= 4096 ? 1 : p.T <= 16384 ? 8 : 16;
   ssm::ctas_per_sm<embed_sort>(1024, sizeof(SortSmem));
+  if (ctas > 8) {
+    const cudaError_t e = cudaFuncSetAttribute(embed_sort, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) return fail(SSM_ERR_CUDA, "embedding: the sort's cluster is refused (error %lld)", (long long)e);
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ctas);
   cfg.blockDim = dim3(1024);
