@@ -78,7 +78,7 @@ __global__ void __launch_bounds__(kRmsThreads) rms_bwd(const __grid_constant__ R
       }
     }
     const float2 s = team.sum(make_float2(ss.x + ss.y, gt.x + gt.y));
-    const float rstd = 1.0f / sqrtf(s.x * p.inv_c + p.eps);
+    const float rstd = rsqrtf(s.x * p.inv_c + p.eps);
     const float2 r2 = bc2(rstd), mean = bc2(-s.y * rstd * p.inv_c);      // minus that of g n
 #pragma unroll
     for (int k = 0; k < K; ++k) {
@@ -153,7 +153,7 @@ __global__ void __launch_bounds__(kRmsThreads) rms_bwd_long(const __grid_constan
       gt = fmaf(to_f32(dy[c]) * weight_at(p, c), v, gt);
     }
     const float2 s = team.sum(make_float2(ss, gt));
-    const float rstd = 1.0f / sqrtf(s.x * p.inv_c + p.eps), mean = s.y * rstd * p.inv_c;
+    const float rstd = rsqrtf(s.x * p.inv_c + p.eps), mean = s.y * rstd * p.inv_c;
     if (threadIdx.x == 0) stat[row] = rstd;
     for (int c = threadIdx.x; c < p.C; c += 512) {
       const float d0 = p.dt != nullptr ? to_f32(static_cast<const TR*>(p.dt)[row * p.dts + c]) : 0.0f;
@@ -211,7 +211,7 @@ int fail(int code, const char* fmt, long long a = 0, long long b = 0) {
 
 // Partial rows: a CTA each, of teams that take at most kRmsChain rows; or a slab of kRmsChain rows each.
 constexpr long long kCtas = 148 * 8;
-long long most_parts(long long rows) { return std::max(kCtas, rms_ceil(rows, kRmsChain)); }
+long long most_parts(long long rows) { return std::min(rows, std::max(kCtas, rms_ceil(rows, kRmsChain))); }
 
 template <typename TX, typename TR, int K, bool RAGGED>
 cudaError_t launch(const RmsParams& p, RmsForm f, long long* parts, cudaStream_t st) {

@@ -12,6 +12,13 @@ int report_error(int code, const char* msg);
 
 namespace {
 
+// the largest; a NaN only where all are
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
 template <typename TX, typename TR, int VEC, int K, bool FP8, bool RAGGED>
 __global__ void __launch_bounds__(kRmsThreads) rms_fwd(const __grid_constant__ RmsParams p, int wpr) {
   using SX = Slot<TX, VEC, RAGGED>;
@@ -74,7 +81,7 @@ __global__ void __launch_bounds__(kRmsThreads) rms_fwd(const __grid_constant__ R
     stage = stage + 1 == kRmsDepth ? 0 : stage + 1;
     float rstd = 1.0f;
     if (!FP8 || p.norm) {
-      rstd = 1.0f / sqrtf(team.sum(ss.x + ss.y) * p.inv_c + p.eps);
+      rstd = rsqrtf(team.sum(ss.x + ss.y) * p.inv_c + p.eps);      // within 2 ulp; a root and a quotient cost a row 40 instructions
       // in 8 bits rstd joins the scale: one product less
       const float2 f = bc2(FP8 ? 1.0f : rstd);
 #pragma unroll
@@ -87,16 +94,23 @@ __global__ void __launch_bounds__(kRmsThreads) rms_fwd(const __grid_constant__ R
 #pragma unroll
       for (int k = 0; k < K; ++k)
 #pragma unroll
-        for (int i = 0; i < VEC / 2; ++i) big = fmaxf(big, fmaxf(fabsf(v[k][i].x), fabsf(v[k][i].y)));
+        for (int i = 0; i < VEC / 2; ++i) big = max3(big, fabsf(v[k][i].x), fabsf(v[k][i].y));
       // a zero row, and one whose root overflowed, is 0 (0 x inf is NaN and fmaxf passes over it)
-      const float scale = fmaxf(team.max(big) * rstd, kRmsTiny) / kE4m3Max;
-      const float2 inv = bc2(1.0f / scale), f = bc2(rstd);
+      const float scale = fmaxf(team.max(big) * rstd, kRmsTiny) / kE4m3Max, inv = rcp(scale);
       if (team.tid == 0) p.scale[row] = scale;
+      float f = rstd * inv;
+      if (f > 1e38f) {                            // of a row about as small as kRmsTiny: one factor after the other
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+          for (int i = 0; i < VEC / 2; ++i) v[k][i] = mul2(v[k][i], bc2(rstd));
+        f = inv;
+      }
 #pragma unroll
       for (int k = 0; k < K; ++k) {
         const int c = c0(k) + lane * VEC;
 #pragma unroll
-        for (int i = 0; i < VEC / 2; ++i) v[k][i] = mul2(mul2(v[k][i], f), inv);
+        for (int i = 0; i < VEC / 2; ++i) v[k][i] = mul2(v[k][i], bc2(f));
         if (c < p.C) write_e4m3<VEC>(static_cast<uint8_t*>(p.y) + row * p.ys + c, p.C - c, p.wide8, v[k]);
       }
     } else {
@@ -129,7 +143,7 @@ __global__ void __launch_bounds__(kRmsThreads) rms_fwd_long(const __grid_constan
       ss = fmaf(v, v, ss);
     }
     const bool norm = !FP8 || p.norm;
-    const float rstd = norm ? 1.0f / sqrtf(team.sum(ss) * p.inv_c + p.eps) : 1.0f;
+    const float rstd = norm ? rsqrtf(team.sum(ss) * p.inv_c + p.eps) : 1.0f;
     auto result = [&](int c) {
       if (!norm) return value(c);
       return value(c) * rstd * weight_at(p, c);
@@ -137,7 +151,7 @@ __global__ void __launch_bounds__(kRmsThreads) rms_fwd_long(const __grid_constan
     if constexpr (FP8) {
       float big = 0.0f;
       for (int c = threadIdx.x; c < p.C; c += 512) big = fmaxf(big, fabsf(result(c)));
-      const float scale = fmaxf(team.max(big), kRmsTiny) / kE4m3Max, inv = 1.0f / scale;
+      const float scale = fmaxf(team.max(big), kRmsTiny) / kE4m3Max, inv = rcp(scale);
       if (threadIdx.x == 0) p.scale[row] = scale;
       for (int c = threadIdx.x; c < p.C; c += 512)
         static_cast<uint8_t*>(p.y)[row * p.ys + c] = __nv_cvt_float_to_fp8(result(c) * inv, __NV_SATFINITE, __NV_E4M3);
