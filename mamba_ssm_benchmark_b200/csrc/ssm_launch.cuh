@@ -24,21 +24,17 @@ int ctas_per_sm(int threads, size_t smem) {
   return n;
 }
 
-// The same for a kernel that is launched with different numbers of threads (whole warps, up to 32), with as much shared
-// memory each time as `smem` says for these.
+// The same for a kernel that is launched with different numbers of threads (whole warps, up to 32) and `smem` bytes for
+// these; `most`: the largest of all its launches, to which the limit is set every time (two host threads may be here at once).
 template <auto Kern>
-int ctas_per_sm_threads(int threads, size_t smem) {
+int ctas_per_sm_threads(int threads, size_t smem, size_t most) {
   static std::atomic<int> known[64][33];
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return 0;
   if (dev < 64)
     if (const int n = known[dev][threads / 32].load(std::memory_order_relaxed)) return n;
   int n = 0;
-  cudaFuncAttributes now;
-  if (cudaFuncGetAttributes(&now, Kern) != cudaSuccess) return 0;
-  if ((size_t)now.maxDynamicSharedSizeBytes < smem &&
-      cudaFuncSetAttribute(Kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
-    return 0;
+  if (cudaFuncSetAttribute(Kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most) != cudaSuccess) return 0;
   if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, Kern, threads, smem) != cudaSuccess) return 0;
   if (dev < 64) known[dev][threads / 32].store(n, std::memory_order_relaxed);
   return n;

@@ -220,9 +220,11 @@ cudaError_t launch(const RmsParams& p, RmsForm f, long long* parts, cudaStream_t
   using SG = Slot<TX, VEC, RAGGED>;
   constexpr auto kern = rms_bwd<TX, TR, VEC, K, RAGGED>;
   const int threads = f.threads(), teams = f.teams();
-  const size_t smem = std::max((size_t)kRmsDepth * K * (2 * ST::kWarp + SG::kWarp) * (threads / 32),
-                               (size_t)K * VEC * 4 * f.wpr * 32);
-  const int fit = std::min(8, std::max(1, ctas_per_sm_threads<kern>(threads, smem)));
+  // the queue, which is larger than what the teams leave one another at the end
+  constexpr size_t warp = (size_t)kRmsDepth * K * (2 * ST::kWarp + SG::kWarp);
+  static_assert(warp >= (size_t)K * VEC * 4 * 32, "a team's gradients fit its part of the queue");
+  const size_t smem = warp * (threads / 32);
+  const int fit = std::min(8, std::max(1, ctas_per_sm_threads<kern>(threads, smem, warp * kRmsWarps)));
   // one wave, or as many as kRmsChain asks for
   const long long grid = std::max(std::min<long long>(rms_ceil(p.rows, teams), 148LL * fit),
                                   rms_ceil(p.rows, (long long)teams * kRmsChain));

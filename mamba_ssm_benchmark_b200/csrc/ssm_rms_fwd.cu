@@ -169,8 +169,9 @@ cudaError_t launch(const RmsParams& p, RmsForm f, cudaStream_t st) {
   using SR = Slot<TR, VEC, RAGGED>;
   constexpr auto kern = rms_fwd<TX, TR, VEC, K, FP8, RAGGED>;
   const int threads = f.threads();
-  const size_t smem = (size_t)kRmsDepth * K * (SX::kWarp + SR::kWarp) * (threads / 32);
-  const int fit = std::max(1, ctas_per_sm_threads<kern>(threads, smem));
+  constexpr size_t warp = (size_t)kRmsDepth * K * (SX::kWarp + SR::kWarp);
+  const size_t smem = warp * (threads / 32);
+  const int fit = std::max(1, ctas_per_sm_threads<kern>(threads, smem, warp * kRmsWarps));
   kern<<<(unsigned)std::min<long long>(rms_ceil(p.rows, f.teams()), 148LL * fit), threads, smem, st>>>(p, f.wpr);
   return cudaGetLastError();
 }

@@ -8,11 +8,16 @@
 // units of 2^-42, formed in double, and every sum is a 64-bit whole number, exact in any order (up to 2^20 tokens).  A weight
 // is off by at most 2^-43 of the largest; what rounds to zero is never drawn.
 //
-// Up to kFew tokens: a thread each, sorted by rank in registers.  More: a cluster of up to eight CTAs shares a row, a slice
-// of tokens each, kept in shared memory where two CTAs to an SM have the room.  A histogram of the logits' distance to the largest says which
-// bins can hold the border of top_k (exactly) or of top_p (the bins' masses to a part in ten thousand); the few tokens
-// of these bins are sorted by one CTA, against exact sums of what lies before them.  Where a bin holds more than kList
-// tokens (thousands of equal logits) the border is found by bisection of the rank.
+// Up to kFew tokens: a thread each, sorted by rank in registers (a byte of one sequence: 7 us, most of it the launch).
+// More: a cluster of up to eight CTAs shares a row, a slice of tokens each, kept in shared memory where two CTAs to an SM have
+// the room.  A histogram of the logits' distance to the largest says which bins can hold the border of top_k (exactly) or
+// of top_p (the bins' masses to a part in ten thousand); the few tokens of these bins are sorted by one CTA, against exact
+// sums of what lies before them.  Where a bin holds more than kList tokens (hundreds of equal logits) the border is found by
+// bisection of the rank, fifty passes instead of two.
+//
+// 256 x 131072 fp32 by top-p: 162 us, 0.4 GB of DRAM (three passes over what does not stay in L2) at 30 % of its rate; 57 % of
+// the issue slots, forty instructions to a weight, bound it.  64 x 50257 bf16 with all rules: 18 us, the barriers of
+// passes of 1 to 3 us each.  Bisection alone, the first form, took 6690 and 518 us.
 #include <cooperative_groups.h>
 
 #include <algorithm>

@@ -253,17 +253,19 @@ class RMSNorm(nn.Module):
 
 
 class TokenEmbedding(nn.Embedding):
-    """nn.Embedding whose lookup and gradient run on this package's kernels on the GPU."""
+    """nn.Embedding whose lookup and gradient run on this package's kernels on the GPU, where none of its options is used."""
 
     def forward(self, idx):
         w = self.weight
-        if w.is_cuda and w.dtype in nat.DTYPES and idx.numel() > 0 and idx.device == w.device:
+        plain = self.padding_idx is None and self.max_norm is None and not self.scale_grad_by_freq and not self.sparse
+        if plain and w.is_cuda and w.dtype in nat.DTYPES and idx.numel() > 0 and idx.device == w.device:
             return embedding(idx, w)
         return super().forward(idx)
 
 
 def _hooked(*modules):
-    return any(m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks for m in modules)
+    return torch.nn.modules.module._has_any_global_hook() or any(
+        m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks for m in modules)
 
 
 def _delta_mixer(*args, **kw):

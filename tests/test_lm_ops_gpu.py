@@ -70,6 +70,17 @@ def test_embedding_one_token_everywhere():
         assert not dw.any()
 
 
+@pytest.mark.parametrize("T", [4095, 4097, 16385, 131072, 131073, 300001])
+def test_embedding_of_many_tokens(T):
+    """Every form of the sort: one CTA, eight, sixteen, more places than stay in registers.  Whole numbers: sums are exact."""
+    V = 3000
+    idx = (torch.rand(T, device=DEV, generator=_gen(T)) ** 4 * V).long().clamp_max(V - 1)
+    W = torch.zeros(V, 8, device=DEV, requires_grad=True)
+    dy = torch.randint(-4, 5, (T, 8), device=DEV, generator=_gen(1)).float()
+    dw, = torch.autograd.grad(embedding(idx.int(), W), W, dy)
+    assert torch.equal(dw.double(), O.embedding_grad(idx, dy, V, 1.0)[0])
+
+
 @pytest.mark.parametrize("V", [511, 512, 513, 262143, 262144, 300000])
 def test_embedding_sorts_every_digit(V):
     """Places by token where a pass more or less is needed, the first and last ids among them."""
@@ -452,6 +463,30 @@ def test_sample_special_rows():
     odd = torch.tensor([nan, 2.0, -1.0, 1.0, 0.0, 0.99999994, 0.5], device=DEV)     # numbers outside [0, 1)
     flat = torch.zeros(7, 4, device=DEV)
     assert sample_tokens(flat, odd).tolist() == [0, 3, 0, 3, 0, 3, 2]
+
+
+@pytest.mark.parametrize("B,V", [(6, 3000), (300, 30000), (6, 400000)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_sample_special_rows_of_many_tokens(B, V, dtype):
+    """Rows shared by CTAs, by one, and read again instead of kept: infinities, NaN, nothing left, one left, ties, settings at
+    their ends."""
+    inf = float("inf")
+    logits = (2 * _randn(B, V, seed=1)).to(dtype)
+    u = torch.rand(B, device=DEV, generator=_gen(2))
+    logits[0, [7, V // 2, V - 1]] = inf
+    logits[1] = -inf
+    logits[2, V - 2] = float("nan")
+    logits[3] = -inf
+    logits[3, V - 3] = -5.0
+    logits[4] = logits[4].round()
+    want = None
+    for kw in (dict(), dict(top_k=2), dict(top_k=700), dict(top_p=0.9), dict(top_p=0.5, top_k=2000, min_p=0.01), dict(temperature=1e-30, top_p=0.7),
+               dict(temperature=1e30, top_p=0.7), dict(temperature=inf, top_k=5), dict(temperature=0.0)):
+        got = sample_tokens(logits, u, **kw).tolist()
+        rows = list(range(6)) + list(range(6, B, 37))
+        want = [_sample_rows(logits[b:b + 1], u[b:b + 1], **kw)[0] for b in rows]
+        assert [got[b] for b in rows] == want, kw
+    assert want[:4] == [7, -1, -1, V - 3]
 
 
 def test_sample_layouts():

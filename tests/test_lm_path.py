@@ -33,6 +33,21 @@ def test_embedding_and_norm_are_what_they_were_on_the_cpu():
     assert torch.equal(n(x), F.rms_norm(x, (16,), eps=1e-5) * n.weight)
 
 
+@pytest.mark.gpu
+def test_embedding_options_keep_torchs_way():
+    """padding_idx has no gradient, max_norm shortens rows: the kernels know neither."""
+    idx = torch.tensor([0, 1, 1, 3], device=DEV)
+    for kw in (dict(padding_idx=1), dict(max_norm=0.5), dict(scale_grad_by_freq=True)):
+        torch.manual_seed(0)
+        a = torch.nn.Embedding(5, 8, device=DEV, **kw)
+        b = TokenEmbedding(5, 8, device=DEV, **kw)
+        b.load_state_dict(a.state_dict())
+        ya, yb = a(idx), b(idx)
+        assert torch.equal(ya, yb)
+        ga, gb = (torch.autograd.grad(y.square().sum(), m.weight)[0] for y, m in ((ya, a), (yb, b)))
+        assert torch.equal(ga, gb)
+
+
 def test_refusals():
     with pytest.raises(RuntimeError, match="CUDA"):
         _lm().quantize_fp8()
