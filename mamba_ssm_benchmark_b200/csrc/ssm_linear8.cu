@@ -148,7 +148,8 @@ __device__ __forceinline__ void finish16(const LinearParams& p, const uint32_t (
     const float4 s = *reinterpret_cast<const float4*>(scale + 2 * i);
     float4 b = make_float4(lb.x, lb.x, lb.x, lb.x);
     if (bias != nullptr) b = *reinterpret_cast<const float4*>(bias + 2 * i);
-    r[i] = fma2(mul2(make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), ls), make_float2(s.x, s.y), make_float2(b.x, b.y));
+    r[i] = fma2(mul2(make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), ls), make_float2(s.x, s.y),
+                make_float2(b.x, b.y));
     r[i + 1] = fma2(mul2(make_float2(__uint_as_float(v[2 * i + 2]), __uint_as_float(v[2 * i + 3])), ls), make_float2(s.z, s.w),
                     make_float2(b.z, b.w));
   }
@@ -236,8 +237,8 @@ struct TokenRow {
 // Results of a tile whose lanes are channels: this lane's channel n, COLS tokens from m0 on, 16 at a time; 32 lanes store 32
 // neighbours.  The next tokens' residuals are on their way.
 template <int COLS, typename TY>
-__device__ __forceinline__ void finish_channel(const LinearParams& p, uint32_t acc, int m0, int n, const float* x_scale, float w_scale,
-                                               float bias) {
+__device__ __forceinline__ void finish_channel(const LinearParams& p, uint32_t acc, int m0, int n, const float* x_scale,
+                                               float w_scale, float bias) {
   const int left = n < p.channels ? min(COLS, p.tokens - m0) : 0;
   const TY* rp = static_cast<const TY*>(p.res) + (long long)m0 * p.rs + n;
   TY* yp = static_cast<TY*>(p.y) + (long long)m0 * p.ys + n;
@@ -386,14 +387,16 @@ __global__ void __launch_bounds__(kLinThreads, TN <= 64 ? 2 : 1) linear_e4m3(con
           wait(&bar.acc_full[buf], bpar);
           wait.dead = __any_sync(0xffffffffu, wait.dead);
           tc_fence_after();
-          if (!wait.dead) out.finish(my + buf * TN + half, xs, bar.scale[buf] + half, p.bias != nullptr ? bar.bias[buf] + half : nullptr);
+          const float* bias = p.bias != nullptr ? bar.bias[buf] + half : nullptr;
+          if (!wait.dead) out.finish(my + buf * TN + half, xs, bar.scale[buf] + half, bias);
         } else {
           const int n = n0 + row;
           const float ws = n < p.channels ? p.w_scale[n] : 0.0f, bias = n < p.channels && p.bias != nullptr ? p.bias[n] : 0.0f;
           wait(&bar.acc_full[buf], bpar);
           wait.dead = __any_sync(0xffffffffu, wait.dead);
           tc_fence_after();
-          if (!wait.dead && works) finish_channel<kCols, TY>(p, my + buf * TN + half, m0 + half, n, bar.scale[buf] + half, ws, bias);
+          if (!wait.dead && works)
+            finish_channel<kCols, TY>(p, my + buf * TN + half, m0 + half, n, bar.scale[buf] + half, ws, bias);
         }
         tc_fence_before();
         __syncwarp();
@@ -532,9 +535,9 @@ int ssm_linear_fp8(int64_t tokens, int64_t channels, int64_t K, const void* x8, 
   }
   if (by_token && tn < 64) tn = 64;
   p.wide = aligned(32);
-  const bool made = by_token ? encode_rows8(&p.ta, x8, tokens, K, x_stride, kRows) && encode_rows8(&p.tb, w8, channels, K, w_stride, tn)
-                             : encode_rows8(&p.ta, w8, channels, K, w_stride, kRows) && encode_rows8(&p.tb, x8, tokens, K, x_stride, tn);
-  if (!made) return fail(SSM_ERR_CUDA, "linear_fp8: the tensor maps could not be made");
+  CUtensorMap &mx = by_token ? p.ta : p.tb, &mw = by_token ? p.tb : p.ta;
+  if (!encode_rows8(&mx, x8, tokens, K, x_stride, by_token ? kRows : tn) ||
+      !encode_rows8(&mw, w8, channels, K, w_stride, by_token ? tn : kRows)) return fail(SSM_ERR_CUDA, "linear_fp8: the tensor maps could not be made");
   p.w_scale = w_scale;
   p.x_scale = x_scale;
   p.bias = bias;

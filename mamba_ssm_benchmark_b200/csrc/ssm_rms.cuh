@@ -136,7 +136,10 @@ struct Team {
   // of numbers that are not negative, which compare as their bits do
   __device__ __forceinline__ float max(float v) {
     uint32_t b = __reduce_max_sync(0xffffffffu, __float_as_uint(v));
-    if (wpr > 1) b = __reduce_max_sync(0xffffffffu, __float_as_uint(exchange(make_float2(__uint_as_float(b), 0.0f), make_float2(0.0f, 0.0f)).x));
+    if (wpr > 1) {
+      const float2 zero = make_float2(0.0f, 0.0f);
+      b = __reduce_max_sync(0xffffffffu, __float_as_uint(exchange(make_float2(__uint_as_float(b), 0.0f), zero).x));
+    }
     return __uint_as_float(b);
   }
 };

@@ -304,7 +304,8 @@ int ssm_rms_norm_bwd(int64_t rows, int64_t C, ssm_view total, const void* weight
   p.part = dweight != nullptr ? reinterpret_cast<float*>(at) : nullptr;
   float* stat = reinterpret_cast<float*>(at + round256((size_t)most_parts(rows) * C * 4));
   const int xb = dy.dtype == SSM_BF16 ? 2 : 4, tb = total.dtype == SSM_BF16 ? 2 : 4;
-  const bool aligned = rms_aligned(C, 16 / xb, {{p.t, p.ts, tb}, {p.y, p.ys, xb}, {p.dt, p.dts, tb}, {p.dx, p.dxs, xb}, {p.dr, p.drs, tb}});
+  const bool aligned = rms_aligned(
+      C, 16 / xb, {{p.t, p.ts, tb}, {p.y, p.ys, xb}, {p.dt, p.dts, tb}, {p.dx, p.dxs, xb}, {p.dr, p.drs, tb}});
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   long long parts = 0;
   cudaError_t e = dy.dtype == SSM_F32      ? run<float, float>(p, aligned, &parts, stat, st)

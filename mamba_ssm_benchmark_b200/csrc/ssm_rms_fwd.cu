@@ -255,7 +255,8 @@ static int forward(int64_t rows, int64_t C, ssm_view x, ssm_view residual, const
   p.inv_c = 1.0f / (float)C;
   p.norm = norm;
   const int xb = x.dtype == SSM_BF16 ? 2 : 4, rb = residual.dtype == SSM_BF16 ? 2 : 4;
-  const bool aligned = rms_aligned(C, 16 / xb, {{x.ptr, p.xs, xb}, {p.r, p.rs, rb}, {p.t, p.ts, rb}, {fp8 ? nullptr : p.y, p.ys, xb}});
+  const RmsSide out = {fp8 ? nullptr : p.y, p.ys, xb};
+  const bool aligned = rms_aligned(C, 16 / xb, {{x.ptr, p.xs, xb}, {p.r, p.rs, rb}, {p.t, p.ts, rb}, out});
   p.wide8 = fp8 && ((reinterpret_cast<uintptr_t>(p.y) | (uintptr_t)p.ys) & 7) == 0;
   const int rd = residual.ptr != nullptr ? residual.dtype : x.dtype;
   cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -273,7 +273,9 @@ struct Sampler {
       for (int j = 0; j < 4; ++j) l[j] = l[j] == kInf ? 0.0f : -kInf;
     }
   }
-  __device__ void keep(int i, const float (&l)[4]) { *reinterpret_cast<float4*>(s.logits + (i - base)) = make_float4(l[0], l[1], l[2], l[3]); }
+  __device__ void keep(int i, const float (&l)[4]) {
+    *reinterpret_cast<float4*>(s.logits + (i - base)) = make_float4(l[0], l[1], l[2], l[3]);
+  }
   // f(i, l[4]) for this lane's tokens
   template <typename F>
   __device__ __forceinline__ void each(F f) {
@@ -680,7 +682,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_many(const __grid_constant
   }
   __syncthreads();
   if (s.owner >= 0) {
-    const int begin = a.base + s.owner * a.per, end = min(min(p.V, a.base + p.slice), begin + a.per), each = (a.per + kThreads - 1) / kThreads;
+    const int begin = a.base + s.owner * a.per, end = min(min(p.V, a.base + p.slice), begin + a.per);
+    const int each = (a.per + kThreads - 1) / kThreads;
     const u64 rest = s.rest;
     auto at = [&](int j) -> u64 {                         // of this thread's j-th token
       const int i = begin + t * each + j;

@@ -306,8 +306,10 @@ struct Embedding : torch::autograd::Function<Embedding> {
 };
 
 Tensor embedding(const Tensor& idx, const Tensor& weight, double scale) {
-  TORCH_CHECK_VALUE(weight.dim() == 2 && weight.numel() > 0, "weight must be (vocabulary, channels) with no empty axis, got " + text(weight));
-  TORCH_CHECK_TYPE(idx.scalar_type() == at::kLong || idx.scalar_type() == at::kInt, "idx must be int64 or int32, got " + text(idx.scalar_type()));
+  TORCH_CHECK_VALUE(weight.dim() == 2 && weight.numel() > 0,
+                    "weight must be (vocabulary, channels) with no empty axis, got " + text(weight));
+  TORCH_CHECK_TYPE(idx.scalar_type() == at::kLong || idx.scalar_type() == at::kInt,
+                   "idx must be int64 or int32, got " + text(idx.scalar_type()));
   TORCH_CHECK_VALUE(idx.numel() > 0, "idx must have no empty axis, got " + text(idx));
   TORCH_CHECK_TYPE(kernel_type(weight), "weight must be float32 or bfloat16, got " + text(weight.scalar_type()));
   needs_cuda("embedding", weight);
@@ -332,8 +334,10 @@ struct RmsArgs {
     const int64_t C = x0.size(-1);
     residual = value(r0);
     weight = value(w0);
-    TORCH_CHECK_VALUE(!residual.defined() || residual.sizes() == x0.sizes(), "residual must be shaped like x " + text(x0) + ", got " + text(residual));
-    TORCH_CHECK_VALUE(!weight.defined() || (weight.dim() == 1 && weight.size(0) == C), "weight must be (" + std::to_string(C) + ",), got " + text(weight));
+    TORCH_CHECK_VALUE(!residual.defined() || residual.sizes() == x0.sizes(),
+                      "residual must be shaped like x " + text(x0) + ", got " + text(residual));
+    TORCH_CHECK_VALUE(!weight.defined() || (weight.dim() == 1 && weight.size(0) == C),
+                      "weight must be (" + std::to_string(C) + ",), got " + text(weight));
     TORCH_CHECK_VALUE(eps >= 0.0, "eps must not be negative, got " + std::to_string(eps));
     for (const Tensor& t : {x0, residual, weight})
       TORCH_CHECK_TYPE(!t.defined() || (t.is_floating_point() && t.scalar_type() != at::kDouble && t.element_size() > 1),
@@ -410,7 +414,8 @@ variable_list rms_norm(const Tensor& x, const Maybe& weight, const Maybe& residu
   const RmsArgs a("RMS norm", x, weight, residual, eps);
   plain("rms_norm", {x, value(residual), value(weight)});
   variable_list out;
-  if (at::GradMode::is_enabled() && (wants(a.x) || (a.residual.defined() && wants(a.residual)) || (a.weight.defined() && wants(a.weight)))) {
+  const bool wanted = wants(a.x) || (a.residual.defined() && wants(a.residual)) || (a.weight.defined() && wants(a.weight));
+  if (at::GradMode::is_enabled() && wanted) {
     auto maybe = [](const Tensor& t) { return t.defined() ? Maybe(t) : Maybe(); };
     out = RmsNorm::apply(a.x, maybe(a.residual), maybe(a.weight), eps);
   } else {
@@ -460,10 +465,13 @@ Tensor linear_fp8(const Tensor& x8, const Tensor& x_scale, const Tensor& w8, con
   const int64_t N = w8.size(0), K = w8.size(1);
   TORCH_CHECK_VALUE(x8.size(-1) == K, "x8 must have weight8's " + std::to_string(K) + " columns, got " + text(x8));
   const at::IntArrayRef outer = x8.sizes().slice(0, x8.dim() - 1);
-  TORCH_CHECK_VALUE(x_scale.sizes() == outer && w_scale.dim() == 1 && w_scale.size(0) == N, "the scales must be " + text(outer) + " and (" + std::to_string(N) + ",), got " + text(x_scale) + " and " + text(w_scale));
+  TORCH_CHECK_VALUE(x_scale.sizes() == outer && w_scale.dim() == 1 && w_scale.size(0) == N,
+                    "the scales must be " + text(outer) + " and (" + std::to_string(N) + ",), got " + text(x_scale) + " and " +
+                        text(w_scale));
   TORCH_CHECK_TYPE(x_scale.scalar_type() == at::kFloat && w_scale.scalar_type() == at::kFloat, "the scales must be float32");
   Tensor bias = value(bias0), residual = value(residual0);
-  TORCH_CHECK_VALUE(!bias.defined() || (bias.dim() == 1 && bias.size(0) == N), "bias must be (" + std::to_string(N) + ",), got " + text(bias));
+  TORCH_CHECK_VALUE(!bias.defined() || (bias.dim() == 1 && bias.size(0) == N),
+                    "bias must be (" + std::to_string(N) + ",), got " + text(bias));
   const at::ScalarType type = dtype.has_value() ? *dtype : residual.defined() ? residual.scalar_type() : at::kBFloat16;
   TORCH_CHECK_TYPE(type == at::kFloat || type == at::kBFloat16, "dtype must be float32 or bfloat16, got " + text(type));
   std::vector<int64_t> shape = outer.vec();
@@ -476,20 +484,20 @@ Tensor linear_fp8(const Tensor& x8, const Tensor& x_scale, const Tensor& w8, con
   plain("linear_fp8", {x8, x_scale, w8, w_scale, bias, residual});
   const c10::cuda::CUDAGuard guard(x8.device());
   auto rows = [](const Tensor& t) {                  // rows that start at multiples of 16 bytes
-    const bool fits = (t.stride(1) == 1 || t.size(1) == 1) && (t.size(0) == 1 || (t.stride(0) % 16 == 0 && t.stride(0) >= t.size(1))) &&
-                      reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0;
-    if (fits) return t;
+    const bool fits = (t.stride(1) == 1 || t.size(1) == 1) && reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0;
+    if (fits && (t.size(0) == 1 || (t.stride(0) % 16 == 0 && t.stride(0) >= t.size(1)))) return t;
     const Tensor u = rows8(t.size(0), t.size(1), t);
     u.copy_(t);
     return u;
   };
   auto stride = [](const Tensor& t) { return t.size(0) == 1 ? (t.size(1) + 15) / 16 * 16 : t.stride(0); };
-  const Tensor x = rows(x8.dim() == 2 ? x8 : x8.reshape({-1, K})), w = rows(w8), xs = x_scale.contiguous(), ws = w_scale.contiguous();
+  const Tensor x = rows(x8.dim() == 2 ? x8 : x8.reshape({-1, K})), w = rows(w8);
+  const Tensor xs = x_scale.contiguous(), ws = w_scale.contiguous();
   if (bias.defined()) bias = bias.to(at::kFloat).contiguous();
   if (residual.defined()) residual = as_rows(residual);
   const Tensor y = at::empty({x.size(0), N}, x_scale.options().dtype(type));
-  check(ssm_linear_fp8(x.size(0), N, K, x.const_data_ptr(), stride(x), f32(xs), w.const_data_ptr(), stride(w), f32(ws), f32(bias), silu,
-                       view(residual), view(y), stream(x)),
+  check(ssm_linear_fp8(x.size(0), N, K, x.const_data_ptr(), stride(x), f32(xs), w.const_data_ptr(), stride(w), f32(ws), f32(bias),
+                       silu, view(residual), view(y), stream(x)),
         "ssm_linear_fp8");
   return shaped(y, shape);
 }
@@ -505,26 +513,30 @@ struct Given {
   Given(const char* name, const Setting<N>& s, const Tensor& logits, N none, N lo, N hi) : one(none) {
     if (!s.has_value()) return;
     if (const Tensor* t = std::get_if<Tensor>(&*s)) {
-      TORCH_CHECK_VALUE(t->dim() == 1 && t->size(0) == logits.size(0), std::string(name) + " must be a number or a (" + std::to_string(logits.size(0)) + ",) tensor, got " + text(*t));
+      TORCH_CHECK_VALUE(t->dim() == 1 && t->size(0) == logits.size(0),
+                        std::string(name) + " must be a number or a (" + std::to_string(logits.size(0)) + ",) tensor, got " + text(*t));
       one_device(logits, {*t});
       rows = t->detach().to(std::is_same_v<N, double> ? at::kDouble : at::kLong).contiguous();
     } else {
       one = std::get<N>(*s);
-      TORCH_CHECK_VALUE(one >= lo && one <= hi, std::string(name) + " must be in " + std::to_string(lo) + " .. " + std::to_string(hi) + ", got " + std::to_string(one));
+      TORCH_CHECK_VALUE(one >= lo && one <= hi, std::string(name) + " must be in " + std::to_string(lo) + " .. " + std::to_string(hi) +
+                                                    ", got " + std::to_string(one));
     }
   }
   const N* by_row() const { return rows.defined() ? static_cast<const N*>(rows.const_data_ptr()) : nullptr; }
 };
 
-Tensor sample_tokens(const Tensor& logits0, const Tensor& uniforms, const Setting<double>& temperature, const Setting<int64_t>& top_k,
-                     const Setting<double>& top_p, const Setting<double>& min_p) {
+Tensor sample_tokens(const Tensor& logits0, const Tensor& uniforms, const Setting<double>& temperature,
+                     const Setting<int64_t>& top_k, const Setting<double>& top_p, const Setting<double>& min_p) {
   TORCH_CHECK_VALUE(logits0.dim() == 2 && logits0.numel() > 0, "logits must be (B, V) with no empty axis, got " + text(logits0));
   const int64_t B = logits0.size(0), V = logits0.size(1), most = 1 << 20;
   TORCH_CHECK_VALUE(V <= most, "the vocabulary must be at most " + std::to_string(most) + ", got " + std::to_string(V));
-  TORCH_CHECK_VALUE(uniforms.dim() == 1 && uniforms.size(0) == B, "uniforms must be (" + std::to_string(B) + ",), got " + text(uniforms));
+  TORCH_CHECK_VALUE(uniforms.dim() == 1 && uniforms.size(0) == B,
+                    "uniforms must be (" + std::to_string(B) + ",), got " + text(uniforms));
   TORCH_CHECK_TYPE(logits0.is_floating_point() && logits0.scalar_type() != at::kDouble && logits0.element_size() > 1 &&
                        uniforms.scalar_type() == at::kFloat,
-                   "logits must be float32 or bfloat16 and uniforms float32, got " + text(logits0.scalar_type()) + " and " + text(uniforms.scalar_type()));
+                   "logits must be float32 or bfloat16 and uniforms float32, got " + text(logits0.scalar_type()) + " and " +
+                       text(uniforms.scalar_type()));
   const double inf = std::numeric_limits<double>::infinity();
   const Given<double> t("temperature", temperature, logits0, 1.0, 0.0, inf), p("top_p", top_p, logits0, 1.0, 0.0, 1.0),
       m("min_p", min_p, logits0, 0.0, 0.0, 1.0);
