@@ -248,24 +248,33 @@ __device__ __forceinline__ uint32_t smem_u32(const void* p) {
 // and its writes are visible, so the kernel sees exactly what a plain launch would see.
 // pdl_launch_dependents() at a kernel's top lets the next launch_pdl kernel be scheduled once all
 // of this grid's CTAs are running.  Kernels from other libraries that follow are launched
-// normally.  Measured at config 1 (fwd + bwd + finalize): 173.3 -> 171.3 us per step.
+// normally.  A cluster's size, when it is above 0, is given with the launch.  Measured at config 1
+// (fwd + bwd + finalize): 173.3 -> 171.3 us per step.
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 template <typename... KArgs, typename... Args>
-cudaError_t launch_pdl(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
-                       Args&&... args) {
+cudaError_t launch_pdl_cluster(void (*kern)(KArgs...), dim3 grid, dim3 block, unsigned cluster, size_t smem,
+                               cudaStream_t stream, Args&&... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = block;
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = cluster > 0 ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...);
+}
+template <typename... KArgs, typename... Args>
+cudaError_t launch_pdl(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
+                       Args&&... args) {
+  return launch_pdl_cluster(kern, grid, block, 0, smem, stream, std::forward<Args>(args)...);
 }
 
 __device__ __forceinline__ void mbar_init(uint64_t* bar, uint32_t count) {

@@ -69,6 +69,8 @@ template <typename T, bool RAGGED, bool SCALE>
 __global__ void __launch_bounds__(256) embed_fwd(const __grid_constant__ EmbedParams p, int pieces) {
   constexpr int VEC = 16 / sizeof(T);
   using Part = Slot<T, VEC, RAGGED>;
+  ssm::pdl_launch_dependents();
+  ssm::pdl_wait();
   const long long item = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
   const long long t = item / pieces;
   if (t >= p.T) return;
@@ -113,6 +115,8 @@ struct SortSmem {
 __global__ void __launch_bounds__(1024) embed_sort(const __grid_constant__ EmbedParams p, uint2* a, uint2* b, int passes) {
   extern __shared__ __align__(16) unsigned char raw[];
   SortSmem& s = *reinterpret_cast<SortSmem*>(raw);
+  ssm::pdl_launch_dependents();
+  ssm::pdl_wait();
   cg::cluster_group cluster = cg::this_cluster();
   const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -232,6 +236,8 @@ template <typename T, bool RAGGED>
 __global__ void __launch_bounds__(kSumThreads) embed_sum(const __grid_constant__ EmbedParams p) {
   __shared__ uint2 near[2 * kLongest + 1];             // from the place before the chunk's first possible one
   __shared__ int bound[2];
+  ssm::pdl_launch_dependents();
+  ssm::pdl_wait();
   constexpr int VEC = 16 / sizeof(T);
   using Part = Slot<T, VEC, RAGGED>;
   const int lane = threadIdx.x & 31;
@@ -328,6 +334,8 @@ constexpr int kJoinWarps = 8;
 template <typename T>
 __global__ void __launch_bounds__(32 * kJoinWarps) embed_join(const __grid_constant__ EmbedParams p) {
   __shared__ double red[kJoinWarps][128];
+  ssm::pdl_launch_dependents();
+  ssm::pdl_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, pieces = (p.C + 127) / 128;
   const long long items = (long long)p.joins[0] * pieces;
   for (long long item = blockIdx.x; item < items; item += gridDim.x) {
@@ -401,9 +409,7 @@ template <typename T, bool RAGGED>
 cudaError_t run_fwd(const EmbedParams& p, cudaStream_t st) {
   const int pieces = (int)ceil_div(p.C, warp_channels(sizeof(T), RAGGED) * kAhead);
   const unsigned grid = (unsigned)ceil_div(p.T * pieces, 8);
-  if (p.scale == 1.0f) embed_fwd<T, RAGGED, false><<<grid, 256, 0, st>>>(p, pieces);
-  else embed_fwd<T, RAGGED, true><<<grid, 256, 0, st>>>(p, pieces);
-  return cudaGetLastError();
+  return ssm::launch_pdl(p.scale == 1.0f ? embed_fwd<T, RAGGED, false> : embed_fwd<T, RAGGED, true>, grid, 256, 0, st, p, pieces);
 }
 template <typename T, bool RAGGED>
 cudaError_t run_bwd(EmbedParams p, cudaStream_t st) {
@@ -411,12 +417,13 @@ cudaError_t run_bwd(EmbedParams p, cudaStream_t st) {
   const long long warps = ceil_div(p.C, warp_channels(sizeof(T), RAGGED));
   p.slabs = (int)ceil_div(warps, kSumThreads / 32);
   const int threads = (int)ceil_div(warps, p.slabs) * 32;
-  embed_sum<T, RAGGED><<<(unsigned)((p.chunks + ceil_div(p.V, kFill)) * p.slabs), threads, 0, st>>>(p);
-  if (p.chunks > 1) {
+  const unsigned grid = (unsigned)((p.chunks + ceil_div(p.V, kFill)) * p.slabs);
+  cudaError_t e = ssm::launch_pdl(embed_sum<T, RAGGED>, grid, threads, 0, st, p);
+  if (e == cudaSuccess && p.chunks > 1) {
     const long long most = (p.chunks - 1) * ceil_div(p.C, 128);
-    embed_join<T><<<(unsigned)std::min<long long>(most, 148 * 4), 32 * kJoinWarps, 0, st>>>(p);
+    e = ssm::launch_pdl(embed_join<T>, (unsigned)std::min<long long>(most, 148 * 4), 32 * kJoinWarps, 0, st, p);
   }
-  return cudaGetLastError();
+  return e;
 }
 template <typename T>
 cudaError_t run(const EmbedParams& p, bool bwd, bool ragged, cudaStream_t st) {
@@ -439,18 +446,7 @@ int run_sort(const EmbedParams& p, uint2* a, uint2* b, int passes, cudaStream_t 
     const cudaError_t e = cudaFuncSetAttribute(embed_sort, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) return fail(SSM_ERR_CUDA, "embedding: the sort's cluster is refused (error %lld)", (long long)e);
   }
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(ctas);
-  cfg.blockDim = dim3(1024);
-  cfg.dynamicSmemBytes = sizeof(SortSmem);
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = ctas;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, embed_sort, p, a, b, passes);
+  const cudaError_t e = ssm::launch_pdl_cluster(embed_sort, ctas, 1024, ctas, sizeof(SortSmem), st, p, a, b, passes);
   return e == cudaSuccess ? SSM_OK : fail(SSM_ERR_CUDA, "embedding: the sort's launch failed (error %lld)", (long long)e);
 }
 

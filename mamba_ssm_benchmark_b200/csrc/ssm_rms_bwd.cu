@@ -26,6 +26,8 @@ __global__ void __launch_bounds__(kRmsThreads) rms_bwd(const __grid_constant__ R
   // this warp's bytes of a stage: K parts of t, of dy, of dt
   constexpr int kG = K * ST::kWarp, kD = kG + K * SG::kWarp, kStage = kD + K * ST::kWarp;
   clear_queue(queue, warps * kRmsDepth * kStage);
+  pdl_launch_dependents();
+  pdl_wait();
   unsigned char* mine = queue + (threadIdx.x >> 5) * kRmsDepth * kStage;
   const long long step = (long long)gridDim.x * teams;
   long long row = (long long)blockIdx.x * teams + team.id;
@@ -141,6 +143,8 @@ __global__ void __launch_bounds__(kRmsThreads) rms_bwd(const __grid_constant__ R
 // Rows that no team holds: a CTA per row for the sums and d; rstd goes to `stat`.
 template <typename TX, typename TR>
 __global__ void __launch_bounds__(kRmsThreads) rms_bwd_long(const __grid_constant__ RmsParams p, float* stat) {
+  pdl_launch_dependents();
+  pdl_wait();
   __shared__ float2 red[kRmsRed];
   Team team(kRmsWarps, red);
   for (long long row = blockIdx.x; row < p.rows; row += gridDim.x) {
@@ -166,6 +170,8 @@ __global__ void __launch_bounds__(kRmsThreads) rms_bwd_long(const __grid_constan
 // Their gradient of the weight: 32 channels and kRmsChain rows to a CTA, eight rows side by side.
 template <typename TX, typename TR>
 __global__ void __launch_bounds__(256) rms_bwd_cols(const __grid_constant__ RmsParams p, const float* stat) {
+  pdl_launch_dependents();
+  pdl_wait();
   __shared__ float red[8][32];
   const long long c = (long long)blockIdx.x * 32 + threadIdx.x;
   for (long long slab = blockIdx.y; slab * kRmsChain < p.rows; slab += gridDim.y) {
@@ -187,6 +193,8 @@ __global__ void __launch_bounds__(256) rms_bwd_cols(const __grid_constant__ RmsP
 // The partial rows in a fixed order: a warp takes every eighth, the warps' sums are added in order.
 template <typename TW>
 __global__ void __launch_bounds__(256) rms_dweight(const float* part, long long nparts, int C, TW* dw) {
+  pdl_launch_dependents();
+  pdl_wait();
   __shared__ double red[8][32];
   const long long c = (long long)blockIdx.x * 32 + threadIdx.x;
   double s = 0.0;
@@ -229,8 +237,7 @@ cudaError_t launch(const RmsParams& p, RmsForm f, long long* parts, cudaStream_t
   const long long grid = std::max(std::min<long long>(rms_ceil(p.rows, teams), 148LL * fit),
                                   rms_ceil(p.rows, (long long)teams * kRmsChain));
   *parts = grid;
-  kern<<<(unsigned)grid, threads, smem, st>>>(p, f.wpr);
-  return cudaGetLastError();
+  return launch_pdl(kern, (unsigned)grid, threads, smem, st, p, f.wpr);
 }
 template <typename TX, typename TR, bool RAGGED>
 cudaError_t run_form(const RmsParams& p, long long* parts, float* stat, cudaStream_t st) {
@@ -239,13 +246,13 @@ cudaError_t run_form(const RmsParams& p, long long* parts, float* stat, cudaStre
   if (f.k == kMany) return launch<TX, TR, kMany, RAGGED>(p, f, parts, st);
   if (VEC == 4 && f.k == 2) return launch<TX, TR, 2, RAGGED>(p, f, parts, st);
   if (f.k == 1) return launch<TX, TR, 1, RAGGED>(p, f, parts, st);
-  rms_bwd_long<TX, TR><<<(unsigned)std::min<long long>(p.rows, 148 * 4), kRmsThreads, 0, st>>>(p, stat);
-  if (p.part != nullptr) {
+  cudaError_t e = launch_pdl(rms_bwd_long<TX, TR>, (unsigned)std::min<long long>(p.rows, 148 * 4), kRmsThreads, 0, st, p, stat);
+  if (e == cudaSuccess && p.part != nullptr) {
     *parts = rms_ceil(p.rows, kRmsChain);
     const dim3 grid((unsigned)rms_ceil(p.C, 32), (unsigned)std::min<long long>(*parts, 65535));
-    rms_bwd_cols<TX, TR><<<grid, dim3(32, 8), 0, st>>>(p, stat);
+    e = launch_pdl(rms_bwd_cols<TX, TR>, grid, dim3(32, 8), 0, st, p, stat);
   }
-  return cudaGetLastError();
+  return e;
 }
 template <typename TX, typename TR>
 cudaError_t run(const RmsParams& p, bool aligned, long long* parts, float* stat, cudaStream_t st) {
@@ -313,11 +320,9 @@ int ssm_rms_norm_bwd(int64_t rows, int64_t C, ssm_view total, const void* weight
                                            : run<__nv_bfloat16, __nv_bfloat16>(p, aligned, &parts, stat, st);
   if (e == cudaSuccess && dweight != nullptr) {
     const unsigned grid = (unsigned)rms_ceil(C, 32);
-    if (weight_dtype == SSM_BF16)
-      rms_dweight<<<grid, dim3(32, 8), 0, st>>>(p.part, parts, p.C, static_cast<__nv_bfloat16*>(dweight));
-    else
-      rms_dweight<<<grid, dim3(32, 8), 0, st>>>(p.part, parts, p.C, static_cast<float*>(dweight));
-    e = cudaGetLastError();
+    e = weight_dtype == SSM_BF16
+            ? launch_pdl(rms_dweight<__nv_bfloat16>, grid, dim3(32, 8), 0, st, p.part, parts, p.C, static_cast<__nv_bfloat16*>(dweight))
+            : launch_pdl(rms_dweight<float>, grid, dim3(32, 8), 0, st, p.part, parts, p.C, static_cast<float*>(dweight));
   }
   if (e != cudaSuccess) return fail(SSM_ERR_CUDA, "rms_norm backward launch failed (error %lld)", (long long)e);
   return SSM_OK;

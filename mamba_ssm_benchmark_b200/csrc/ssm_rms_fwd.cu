@@ -29,6 +29,8 @@ __global__ void __launch_bounds__(kRmsThreads) rms_fwd(const __grid_constant__ R
   const int warps = blockDim.x >> 5, teams = warps / wpr, lane = team.lane;
   constexpr int kStage = K * (SX::kWarp + SR::kWarp);     // a warp's bytes of a stage: K parts of x, K of the residual
   clear_queue(queue, warps * kRmsDepth * kStage);
+  pdl_launch_dependents();
+  pdl_wait();
   unsigned char* mine = queue + (threadIdx.x >> 5) * kRmsDepth * kStage;
   const long long step = (long long)gridDim.x * teams;
   long long row = (long long)blockIdx.x * teams + team.id;
@@ -129,6 +131,8 @@ __global__ void __launch_bounds__(kRmsThreads) rms_fwd(const __grid_constant__ R
 // of squares, for the largest value and for the result.
 template <typename TX, typename TR, bool FP8>
 __global__ void __launch_bounds__(kRmsThreads) rms_fwd_long(const __grid_constant__ RmsParams p) {
+  pdl_launch_dependents();
+  pdl_wait();
   __shared__ float2 red[kRmsRed];
   Team team(kRmsWarps, red);
   for (long long row = blockIdx.x; row < p.rows; row += gridDim.x) {
@@ -172,8 +176,8 @@ cudaError_t launch(const RmsParams& p, RmsForm f, cudaStream_t st) {
   constexpr size_t warp = (size_t)kRmsDepth * K * (SX::kWarp + SR::kWarp);
   const size_t smem = warp * (threads / 32);
   const int fit = std::max(1, ctas_per_sm_threads<kern>(threads, smem, warp * kRmsWarps));
-  kern<<<(unsigned)std::min<long long>(rms_ceil(p.rows, f.teams()), 148LL * fit), threads, smem, st>>>(p, f.wpr);
-  return cudaGetLastError();
+  const long long grid = std::min<long long>(rms_ceil(p.rows, f.teams()), 148LL * fit);
+  return launch_pdl(kern, (unsigned)grid, threads, smem, st, p, f.wpr);
 }
 template <typename TX, typename TR, bool FP8, bool RAGGED>
 cudaError_t run_form(const RmsParams& p, cudaStream_t st) {
@@ -182,8 +186,7 @@ cudaError_t run_form(const RmsParams& p, cudaStream_t st) {
   if (f.k == kMany) return launch<TX, TR, kMany, FP8, RAGGED>(p, f, st);
   if (VEC == 4 && f.k == 2) return launch<TX, TR, 2, FP8, RAGGED>(p, f, st);
   if (f.k == 1) return launch<TX, TR, 1, FP8, RAGGED>(p, f, st);
-  rms_fwd_long<TX, TR, FP8><<<(unsigned)std::min<long long>(p.rows, 148 * 4), kRmsThreads, 0, st>>>(p);
-  return cudaGetLastError();
+  return launch_pdl(rms_fwd_long<TX, TR, FP8>, (unsigned)std::min<long long>(p.rows, 148 * 4), kRmsThreads, 0, st, p);
 }
 template <typename TX, typename TR, bool FP8>
 cudaError_t run(const RmsParams& p, bool aligned, cudaStream_t st) {

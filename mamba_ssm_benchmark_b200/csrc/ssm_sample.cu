@@ -200,6 +200,8 @@ __device__ __forceinline__ u64 block_sort(u64 v, u64* buf, int n) {
 template <typename T>
 __global__ void __launch_bounds__(kFew) sample_few(const __grid_constant__ SampleParams p) {
   __shared__ u64 part[32], buf[kFew];
+  ssm::pdl_launch_dependents();
+  ssm::pdl_wait();
   const int row = (int)blockIdx.x, i = threadIdx.x;
   const Settings set(p, row);
   const float l = i < p.V ? ssm::to_f32(static_cast<const T*>(p.logits)[row * p.stride + i]) : 0.0f;
@@ -467,11 +469,13 @@ template <typename T>
 __global__ void __launch_bounds__(kThreads, 2) sample_many(const __grid_constant__ SampleParams p) {
   extern __shared__ __align__(16) unsigned char raw[];
   SampleSmem& s = *reinterpret_cast<SampleSmem*>(raw);
+  const int t = threadIdx.x;
+  for (int i = t; i < kTable; i += kThreads) s.exp2[i] = exp2((double)i / kTable);
+  ssm::pdl_launch_dependents();
+  ssm::pdl_wait();
   Sampler<T> a(p, s);
   const Settings set(p, a.row);
-  const int t = threadIdx.x;
   const bool leader = a.cluster.block_rank() == 0;
-  for (int i = t; i < kTable; i += kThreads) s.exp2[i] = exp2((double)i / kTable);
   constexpr float kInf = __builtin_huge_valf();
   float high = -kInf, low = kInf;                         // of the logits above -inf
   bool nan = false;
@@ -748,9 +752,7 @@ extern "C" int ssm_sample_tokens(int64_t B, int64_t V, ssm_view logits, const fl
   if (V <= kFew) {
     int threads = 64;                                      // a power of two: one token to a thread
     while (threads < V) threads *= 2;
-    if (p.bf16) sample_few<__nv_bfloat16><<<(unsigned)B, threads, 0, st>>>(p);
-    else sample_few<float><<<(unsigned)B, threads, 0, st>>>(p);
-    const cudaError_t e = cudaGetLastError();
+    const cudaError_t e = ssm::launch_pdl(p.bf16 ? sample_few<__nv_bfloat16> : sample_few<float>, (unsigned)B, threads, 0, st, p);
     return e == cudaSuccess ? SSM_OK : fail(SSM_ERR_CUDA, "sample_tokens launch failed (error %lld)", (long long)e);
   }
   // CTAs to a row: as many as run at once.  A cluster's barriers cost a row as much as its passes (256 x 131072 by top-p: 300 us
@@ -764,18 +766,8 @@ extern "C" int ssm_sample_tokens(int64_t B, int64_t V, ssm_view logits, const fl
   const size_t most = sizeof(SampleSmem) + kCached * sizeof(float);
   if (p.bf16) ssm::ctas_per_sm<sample_many<__nv_bfloat16>>(kThreads, most);
   else ssm::ctas_per_sm<sample_many<float>>(kThreads, most);
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(B * ctas));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = sizeof(SampleSmem) + (p.cached ? p.slice * sizeof(float) : 0);
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)ctas;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  const cudaError_t e = p.bf16 ? cudaLaunchKernelEx(&cfg, sample_many<__nv_bfloat16>, p)
-                                : cudaLaunchKernelEx(&cfg, sample_many<float>, p);
+  const size_t smem = sizeof(SampleSmem) + (p.cached ? p.slice * sizeof(float) : 0);
+  const cudaError_t e = ssm::launch_pdl_cluster(p.bf16 ? sample_many<__nv_bfloat16> : sample_many<float>, (unsigned)(B * ctas), kThreads,
+                                                (unsigned)ctas, smem, st, p);
   return e == cudaSuccess ? SSM_OK : fail(SSM_ERR_CUDA, "sample_tokens launch failed (error %lld)", (long long)e);
 }
