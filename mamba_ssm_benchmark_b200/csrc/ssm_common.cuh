@@ -252,6 +252,8 @@ __device__ __forceinline__ uint32_t smem_u32(const void* p) {
 // (fwd + bwd + finalize): 173.3 -> 171.3 us per step.
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+// A line of 128 bytes to L2: allowed ahead of pdl_wait(), for L2 is where all writes meet.
+__device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p) : "memory"); }
 
 template <typename... KArgs, typename... Args>
 cudaError_t launch_pdl_cluster(void (*kern)(KArgs...), dim3 grid, dim3 block, unsigned cluster, size_t smem,

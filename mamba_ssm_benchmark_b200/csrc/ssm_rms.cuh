@@ -72,6 +72,11 @@ __device__ __forceinline__ void write_e4m3(uint8_t* dst, int n, bool wide, const
   }
 }
 
+// The weight to L2 while the kernel before still runs; the grid's first threads take a line each.
+__device__ __forceinline__ void prefetch_weight(const RmsParams& p) {
+  const long long at = ((long long)blockIdx.x * blockDim.x + threadIdx.x) * 128;
+  if (p.w != nullptr && at < (long long)p.C * (p.wbf16 ? 2 : 4)) prefetch_l2(static_cast<const char*>(p.w) + at);
+}
 // The first n of VEC weights from channel c on; zeros behind.
 template <int VEC>
 __device__ __forceinline__ void load_weight(const RmsParams& p, int c, int n, float2 (&w)[VEC / 2]) {

@@ -28,6 +28,7 @@ __global__ void __launch_bounds__(kRmsThreads) rms_fwd(const __grid_constant__ R
   Team team(wpr, red);
   const int warps = blockDim.x >> 5, teams = warps / wpr, lane = team.lane;
   constexpr int kStage = K * (SX::kWarp + SR::kWarp);     // a warp's bytes of a stage: K parts of x, K of the residual
+  prefetch_weight(p);
   clear_queue(queue, warps * kRmsDepth * kStage);
   pdl_launch_dependents();
   pdl_wait();
