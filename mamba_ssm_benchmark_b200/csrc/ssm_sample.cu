@@ -12,8 +12,8 @@
 // More: a cluster of up to eight CTAs shares a row, a slice of tokens each, kept in shared memory where two CTAs to an SM have
 // the room.  A histogram of the logits' distance to the largest says which bins can hold the border of top_k (exactly) or
 // of top_p (the bins' masses to a part in ten thousand); the few tokens of these bins are sorted by one CTA, against exact
-// sums of what lies before them.  Where a bin holds more than kList tokens (hundreds of equal logits) the border is found by
-// bisection of the rank, fifty passes instead of two.
+// sums of what lies before them.  Where the bins' masses mislead, the exact sum at the list's edge says where to look next; where
+// a bin holds more than kList tokens (hundreds of equal logits) a pass over the row takes eleven bits of the border's rank.
 //
 // 256 x 131072 fp32 by top-p: 162 us, 0.4 GB of DRAM (three passes over what does not stay in L2) at 30 % of its rate; 57 % of
 // the issue slots, forty instructions to a weight, bound it.  64 x 50257 bf16 with all rules: 18 us, the barriers of
@@ -55,13 +55,17 @@ struct SampleParams {
 
 constexpr int kBits = 42;
 constexpr u64 kOne = 1ull << kBits;
-constexpr int kTable = 1024;          // steps of the table of 2^x
+constexpr int kTable = 1024;          // steps of the table of 2^x; 2^10
 constexpr int kFew = 1024;            // tokens that one CTA takes, one to a thread
 constexpr int kThreads = 512;         // of a CTA that shares a row: two of them to an SM, so that one waits while one works
 constexpr int kWarps = kThreads / 32;
 constexpr int kList = kThreads;       // tokens that are sorted: one to a thread
 constexpr int kPer = 4, kBins = kPer * kThreads;
 constexpr int kMargins = 4;
+constexpr int kDepth = 4;              // loads of a thread on their way, where a row is not kept
+
+// What a gather adds up: nothing, all weights and those before a bin, those of some bins.
+enum Adds { kNothing, kAll, kSome };
 
 struct SampleSmem {
   double exp2[kTable];
@@ -73,7 +77,7 @@ struct SampleSmem {
   int first[1 + 2 * kMargins];        // the first bin at which a sum over the bins passes a value
   u64 cut, rest;                      // rest: what the drawn token's place is short of where its warp's tokens start
   int owner;                          // that warp
-  alignas(16) float logits[4];        // the slice
+  alignas(16) float logits[4];        // the slice, or kDepth slots of 16 bytes to a thread
 };
 
 // A whole number that orders floats as they compare (-0 as 0); the index decides among equal ones, the lowest first.
@@ -85,18 +89,25 @@ __device__ __forceinline__ float key_logit(u64 key) {
   const uint32_t b = (uint32_t)(key >> 32);
   return __uint_as_float(b & 0x80000000u ? b & 0x7fffffffu : ~b);
 }
+__device__ __forceinline__ int key_token(u64 key) { return (int)(0xffffffffu - (uint32_t)key); }
 
 // A weight in whole units: 2^42 2^y, y = (l - top) rate, for finite top and l <= top.  2^y = 2^k 2^(j/1024) 2^r, |r| <= 2^-11:
 // the Taylor polynomial of degree 3 is within (ln 2 / 2048)^4 / 24 = 6e-16 of 2^r.  y is held above -60, where the weight is
 // zero, by its high word: of two negative numbers the larger has the smaller one.
 struct Weights {
-  const double* table;
+  static constexpr double kRaised = 4503599627370496.0;
+  const double* table;                // 2^(42 + j / 1024), its high word less j 2^10: adding 1024 y 2^10 adds k to the exponent
   double top, rate;                   // the largest logit; log2(e) / temperature, held within 1e-290 .. 1e290
   __device__ void set(float top_, double temperature) {
     top = top_;
     rate = fmin(fmax(1.4426950408889634 / temperature, 1e-290), 1e290);
   }
-  __device__ __forceinline__ u64 operator()(float l) const {
+  static __device__ double entry(int j) {
+    const double v = exp2((double)j / kTable + kBits);
+    return __hiloint2double(__double2hiint(v) - (j << 10), __double2loint(v));
+  }
+  // 2^52 and the weight, rounded
+  __device__ __forceinline__ double raised(float l) const {
     constexpr double kLn2 = 0.69314718055994531, kC2 = kLn2 * kLn2 / 2, kC3 = kLn2 * kLn2 * kLn2 / 6;
     constexpr double kShift = 6755399441055744.0 / kTable;   // 1.5 2^52 / 1024: y is rounded to 1024ths
     const double raw = ((double)l - top) * rate;
@@ -106,9 +117,24 @@ struct Weights {
     const double r = y - (t - kShift);
     const double q = fma(r, fma(r, fma(r, kC3, kC2), kLn2), 1.0);
     const double step = table[i & (kTable - 1)];
-    const double scaled = __hiloint2double(__double2hiint(step) + (((i >> 10) + kBits) << 20), __double2loint(step));
-    return (u64)__double_as_longlong(fma(scaled, q, 4503599627370496.0)) & ((1ull << 52) - 1);
+    const double scaled = __hiloint2double(__double2hiint(step) + i * kTable, __double2loint(step));
+    return fma(scaled, q, kRaised);
   }
+  __device__ __forceinline__ u64 operator()(float l) const {
+    return (u64)__double_as_longlong(raised(l)) & ((1ull << 52) - 1);
+  }
+  // The same as a double, which holds a thread's sums too, all of them below 2^53: the passes over whole rows are bound by what
+  // works on whole numbers, not by the arithmetic in double.
+  __device__ __forceinline__ double units(float l) const { return raised(l) - kRaised; }
+};
+
+// Whether a token ranks at least as high as one with this key.
+struct Border {
+  float l;
+  int i;
+  __device__ explicit Border(u64 key)
+      : l(key != 0 ? key_logit(key) : -__builtin_huge_valf()), i(key != 0 ? key_token(key) : 0x7fffffff) {}
+  __device__ __forceinline__ bool operator()(float v, int at) const { return v > l || (v == l && at <= i); }
 };
 
 struct Settings {
@@ -137,10 +163,16 @@ struct Settings {
 
 // The rank of a logit as it came: a NaN above all.
 __device__ __forceinline__ u64 raw_key(float l, int i) { return l != l ? ~0ull : rank_key(l, i); }
-__device__ __forceinline__ int key_token(u64 key) { return (int)(0xffffffffu - (uint32_t)key); }
 // Neither a token nor a choice: no logit above -inf, a NaN, a NaN temperature.
 __device__ __forceinline__ bool no_token(u64 best, double temperature) {
   return best == ~0ull || key_logit(best) == -__int_as_float(0x7f800000) || temperature != temperature;
+}
+
+// The larger one, or NaN.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
 }
 
 // ---- a CTA's threads, a value each ------------------------------------------------------------------
@@ -260,6 +292,11 @@ struct Sampler {
     last = min(end, first + per);
     weight.table = s.exp2;
   }
+  static __device__ void finite(float (&l)[4]) {
+    constexpr float kInf = __builtin_huge_valf();
+#pragma unroll
+    for (int j = 0; j < 4; ++j) l[j] = l[j] == kInf ? 0.0f : -kInf;
+  }
   // Four logits from i on; -inf past the warp's last.  In a row with infinite logits these alone count (`infinite`): 0, and -inf
   // the others.
   __device__ void load(int i, float (&l)[4]) const {
@@ -270,10 +307,7 @@ struct Sampler {
 #pragma unroll
       for (int j = 0; j < 4; ++j) l[j] = i + j < last ? ssm::to_f32(logits[i + j]) : -kInf;
     }
-    if (infinite) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) l[j] = l[j] == kInf ? 0.0f : -kInf;
-    }
+    if (infinite) finite(l);
   }
   __device__ void keep(int i, const float (&l)[4]) {
     *reinterpret_cast<float4*>(s.logits + (i - base)) = make_float4(l[0], l[1], l[2], l[3]);
@@ -287,12 +321,34 @@ struct Sampler {
         ssm::load4(s.logits + (i - base), l);
         f(i, l);
       }
-    } else {                              // from L2 or memory: the next ones on their way
-      float next[4];
-      load(first + 4 * lane, next);
+    } else if (p.wide) {                  // from L2 or memory: the next ones on their way to this thread's slots
+      uint4* slots = reinterpret_cast<uint4*>(s.logits) + threadIdx.x;
+      auto fetch = [&](int i, int slot) {
+        if (i + 4 <= last)
+          asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(ssm::smem_u32(slots + slot * kThreads)), "l"(logits + i),
+                       "n"(4 * sizeof(T))
+                       : "memory");
+        asm volatile("cp.async.commit_group;" ::: "memory");
+      };
+      int i = first + 4 * lane;
+#pragma unroll
+      for (int d = 0; d < kDepth; ++d) fetch(i + 128 * d, d);
+      for (int slot = 0; i < last; i += 128, slot = (slot + 1) % kDepth) {
+        float l[4];
+        asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory");
+        if (i + 4 <= last) {
+          ssm::load4(reinterpret_cast<const T*>(slots + slot * kThreads), l);
+          if (infinite) finite(l);
+        } else {
+          load(i, l);
+        }
+        f(i, l);
+        fetch(i + 128 * kDepth, slot);
+      }
+    } else {
       for (int i = first + 4 * lane; i < last; i += 128) {
-        const float l[4] = {next[0], next[1], next[2], next[3]};
-        load(i + 128, next);
+        float l[4];
+        load(i, l);
         f(i, l);
       }
     }
@@ -341,29 +397,70 @@ struct Sampler {
     return z < (float)kBins ? (int)z : kBins;
   }
 
-  // How many tokens (or what weight) rank at least as high as both keys.
-  template <bool MASS>
-  __device__ u64 above(u64 cut, u64 key) {
-    u64 n = 0;
-    const u64 least = max(cut, key);
-    each([&](int i, const float (&l)[4]) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (i + j < last && rank_key(l[j], i + j) >= least) n += MASS ? weight(l[j]) : 1;
-    });
-    return join<false>(n);
-  }
-  // The key of the token, by rank, at which the count (or weight) of those that rank at least as high as `cut`
-  // reaches `target`; one that has all of them where it does not.
-  template <bool MASS>
-  __device__ u64 bisect(u64 cut, u64 target) {
-    u64 lo = 0, hi = ~0ull;               // above(lo) >= target (or lo = 0), above(hi + 1) < target
-    while (lo < hi) {
-      const u64 mid = lo + (hi - lo) / 2 + 1;
-      if (above<MASS>(cut, mid) >= target) lo = mid;
-      else hi = mid - 1;
+  // The largest key of a logit that is `b` bins or more from the largest: a search over the floats, by every thread.
+  __device__ u64 highest_key(int b) const {
+    if (b == 0) return ~0ull;
+    uint32_t lo = 0x007fffffu, hi = (uint32_t)(rank_key(top, 0) >> 32);     // -inf is that far, the largest is not
+    while (hi - lo > 1) {
+      const uint32_t mid = lo + (hi - lo) / 2;
+      if (distance(key_logit((u64)mid << 32)) >= (float)b) lo = mid;
+      else hi = mid;
     }
-    return lo;
+    return (u64)lo << 32 | 0xffffffffu;
+  }
+  // The key lo <= key <= hi of the token, by rank, with which the count (or weight) of those from hi on, and `before`, reaches
+  // `target`.  A pass takes eleven bits of the range: a bin to each part of it, exact sums in the bins.  False: all of them do not
+  // reach it; lo is the key, `before` their sum.
+  template <bool MASS>
+  __device__ bool search(u64& lo, u64 hi, u64& before, u64 target) {
+    using Bin = std::conditional_t<MASS, u64, uint32_t>;
+    Bin* bins = reinterpret_cast<Bin*>(s.count);          // sums take the place of `upto` too
+    while (lo < hi) {
+      const int shift = max(0, 64 - __clzll((long long)(hi - lo)) - 11);
+      sync();                                             // the bins are no longer read
+      for (int b = threadIdx.x; b < kBins; b += kThreads) bins[b] = 0;
+      if (threadIdx.x == 0) s.first[0] = -1;
+      __syncthreads();
+      each([&](int i, const float (&l)[4]) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const u64 key = rank_key(l[j], i + j);
+          if (i + j < last && key >= lo && key <= hi) {
+            if constexpr (MASS) atomicAdd(&bins[(hi - key) >> shift], weight(l[j]));
+            else atomicAdd(&bins[(hi - key) >> shift], 1u);
+          }
+        }
+      });
+      sync();
+      u64 n[kPer] = {}, mine = 0, all;
+      for (int r = 0; r < ctas; ++r) {
+        const Bin* of = cluster.map_shared_rank(bins, r) + kPer * threadIdx.x;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) n[i] += of[i];
+      }
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) mine += n[i];
+      u64 upto = before + block_scan(mine, s.part, &all) - mine;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        if (upto < target && upto + n[i] >= target) {
+          s.first[0] = kPer * threadIdx.x + i;
+          s.rest = upto;
+        }
+        upto += n[i];
+      }
+      __syncthreads();
+      const int bin = s.first[0];
+      if (bin < 0) {
+        before += all;
+        return false;
+      }
+      before = s.rest;
+      hi -= (u64)bin << shift;
+      const u64 span = (1ull << shift) - 1;
+      if (hi - lo > span) lo = hi - span;
+    }
+    return true;
   }
 
   // Every bin's count over the cluster, in registers: kPer bins to a thread.
@@ -390,25 +487,34 @@ struct Sampler {
       n[3] += c.w;
     }
   }
-  // The tokens of bins lo .. hi that rank at least as high as `cut` to the first CTA's list (in any order).  SUMS: of the tokens
-  // that rank so, the weight of all and of those in bins below lo.
-  template <bool SUMS>
-  __device__ void gather(int lo, int hi, u64 cut, u64& total, u64& before) {
+  // The tokens of bins lo .. hi that rank at least as high as `cut` to the first CTA's list (in any order).  kAll: of the tokens
+  // that rank so, the weight of all and of those in bins below lo.  kSome: of those in bins from .. to - 1.
+  template <Adds ADDS>
+  __device__ void gather(int lo, int hi, u64 cut, u64& total, u64& before, int from = 0, int to = 0) {
     int* size = cluster.map_shared_rank(&s.size, 0);
     u64* list = cluster.map_shared_rank(s.list, 0);
-    const float from = (float)lo, to = (float)(hi + 1);
-    total = before = 0;
+    const float begin = (float)lo, end = (float)(hi + 1), some = (float)from, others = (float)to;
+    const Border border(cut);
+    double all = 0.0, higher = 0.0;
     auto body = [&](int i, const float (&l)[4], auto cuts) {
+      bool here[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const float z = distance(l[j]);
-        const bool in = !cuts || rank_key(l[j], i + j) >= cut;
-        if (SUMS) {
-          const u64 w = weight(l[j]);
-          if (in) total += w;
-          if (in && z < from) before += w;
+        const bool in = !cuts || border(l[j], i + j);
+        if constexpr (ADDS == kAll) {
+          const double w = weight.units(in ? l[j] : -__builtin_huge_valf());
+          all += w;
+          if (z < begin) higher += w;
+        } else if constexpr (ADDS == kSome) {
+          if (in && z >= some && z < others) higher += weight.units(l[j]);
         }
-        if (z >= from && z < to && in) {
+        here[j] = z >= begin && z < end && in;
+      }
+      if (here[0] || here[1] || here[2] || here[3]) {     // one branch to four tokens, after their weights
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (!here[j]) continue;
           const int at = atomicAdd(size, 1);
           if (at < kList) list[at] = rank_key(l[j], i + j);
         }
@@ -416,6 +522,8 @@ struct Sampler {
     };
     if (cut != 0) each([&](int i, const float (&l)[4]) { body(i, l, std::true_type()); });
     else each([&](int i, const float (&l)[4]) { body(i, l, std::false_type()); });
+    total = (u64)all;
+    before = (u64)higher;
   }
   // x and y summed over the cluster, once the list is written: one barrier of the cluster for both.
   __device__ void sums(u64& x, u64& y) {
@@ -470,7 +578,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_many(const __grid_constant
   extern __shared__ __align__(16) unsigned char raw[];
   SampleSmem& s = *reinterpret_cast<SampleSmem*>(raw);
   const int t = threadIdx.x;
-  for (int i = t; i < kTable; i += kThreads) s.exp2[i] = exp2((double)i / kTable);
+  for (int i = t; i < kTable; i += kThreads) s.exp2[i] = Weights::entry(i);
   ssm::pdl_launch_dependents();
   ssm::pdl_wait();
   Sampler<T> a(p, s);
@@ -478,7 +586,6 @@ __global__ void __launch_bounds__(kThreads, 2) sample_many(const __grid_constant
   const bool leader = a.cluster.block_rank() == 0;
   constexpr float kInf = __builtin_huge_valf();
   float high = -kInf, low = kInf;                         // of the logits above -inf
-  bool nan = false;
 #pragma unroll 4
   for (int i = a.first + 4 * a.lane; i < a.last; i += 128) {
     float l[4];
@@ -486,13 +593,12 @@ __global__ void __launch_bounds__(kThreads, 2) sample_many(const __grid_constant
     if (p.cached) a.keep(i, l);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      high = fmaxf(high, l[j]);
+      high = max_nan(high, l[j]);
       low = fminf(low, l[j] > -kInf ? l[j] : kInf);
-      nan |= l[j] != l[j];
     }
   }
   // both in one: the largest, and the smallest as the largest of the negated
-  const u64 ends = a.template join<true, true>(nan ? ~0ull : (rank_key(high, 0) >> 32) << 32 | rank_key(-low, 0) >> 32);
+  const u64 ends = a.template join<true, true>(high != high ? ~0ull : (rank_key(high, 0) >> 32) << 32 | rank_key(-low, 0) >> 32);
   const bool none = no_token(ends, set.temperature);
   a.top = key_logit(ends);
   if (none || !(set.temperature > 0.0)) {                 // the same for the whole cluster
@@ -542,7 +648,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_many(const __grid_constant
     const int listed = (int)s.upto[last];                 // tokens up to it
     if (listed <= kList) {                                // what is kept of the top_k: all in the list
       u64 none0, none1;
-      a.template gather<false>(0, last, 0, none0, none1);
+      a.template gather<kNothing>(0, last, 0, none0, none1);
       a.sync();
       if (!leader) return;                                // nobody reads this CTA's memory any more
       u64 key = a.sorted();
@@ -563,10 +669,12 @@ __global__ void __launch_bounds__(kThreads, 2) sample_many(const __grid_constant
     if (borders) {                                        // the border of top_k lies in bin `last`
       const int before = last > 0 ? (int)s.upto[last - 1] : 0;
       if (listed - before > kList) {
-        cut = a.template bisect<false>(0, (u64)set.top_k);
+        cut = a.highest_key(last + 1) + 1;
+        u64 upto = before;
+        a.template search<false>(cut, a.highest_key(last), upto, (u64)set.top_k);
       } else {
         u64 none0, none1;
-        a.template gather<false>(last, last, 0, none0, none1);
+        a.template gather<kNothing>(last, last, 0, none0, none1);
         a.sync();
         const u64 key = a.sorted();
         if (leader && t == (int)set.top_k - before - 1) s.cut = key;
@@ -577,16 +685,24 @@ __global__ void __launch_bounds__(kThreads, 2) sample_many(const __grid_constant
       }
     }
     if (top_p) {
-      // the bins' masses, about: as many weights as it has tokens, from its middle
+      // The masses of this thread's bins, about: as many weights as a bin has tokens, from its middle, in units of 2^-24.  They
+      // are made anew when they are needed again, which is rare: held over the pass in between they cost it registers.
       const float step = range / ((float)kBins - 0.01f) / (float)set.temperature;
-      u64 unit[kPer], mass, upto = 0;
+      auto masses = [&](u64 (&unit)[kPer], u64& upto) {   // upto: before the first of the thread's bins.  The mass of all.
+        u64 mine = 0, mass;
+        uint32_t seen = b0 > 0 ? s.upto[b0 - 1] : 0;
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        if (borders && b0 + i == last) n[i] = (uint32_t)set.top_k - (last > 0 ? s.upto[last - 1] : 0);
-        unit[i] = b0 + i <= last ? (u64)((float)n[i] * __expf(-step * ((float)(b0 + i) + 0.5f)) * 16777216.0f) : 0;
-        upto += unit[i];
-      }
-      upto = block_scan(upto, s.part, &mass) - upto;      // before the first of this thread's bins
+        for (int i = 0; i < kPer; ++i) {
+          const uint32_t now = borders && b0 + i == last ? (uint32_t)set.top_k : s.upto[b0 + i];
+          unit[i] = b0 + i <= last ? (u64)((float)(now - seen) * __expf(-step * ((float)(b0 + i) + 0.5f)) * 16777216.0f) : 0;
+          mine += unit[i];
+          seen = now;
+        }
+        upto = block_scan(mine, s.part, &mass) - mine;
+        return mass;
+      };
+      u64 unit[kPer], upto;
+      const u64 mass = masses(unit, upto);
       // the first bin at which the sum is above (top_p - margin), and (top_p + margin), of the mass
       const double margins[kMargins] = {0.008, 0.001, 0.0001, 0.0};
 #pragma unroll
@@ -601,34 +717,48 @@ __global__ void __launch_bounds__(kThreads, 2) sample_many(const __grid_constant
         }
       }
       __syncthreads();
-      // the widest margin with few tokens; where the border is not between them after all, with as many as fit
-      bool found = false;
-      u64 total = 0;
-      for (int most = kList / 4; most <= kList && !found; most *= 4) {
-        int lo = 0, hi = 0;
-        bool fits = false;
-        for (int i = 0; i < kMargins && !fits; ++i) {
+      // the widest margin with few tokens, else the widest with as many as fit, else the widest of all
+      auto tokens = [&](int lo, int hi) { return (int)(s.upto[hi] - (lo > 0 ? s.upto[lo - 1] : 0)); };
+      int lo = 0, hi = 0;
+      bool fits = false;
+      for (int most = kList / 4; most <= kList && !fits; most *= 4)
+        for (int i = 0; i < kMargins - (most < kList) && !fits; ++i) {
           lo = s.first[1 + 2 * i];
           hi = min(last, s.first[2 + 2 * i]);
-          fits = (int)(s.upto[hi] - (lo > 0 ? s.upto[lo - 1] : 0)) <= most;
+          fits = tokens(lo, hi) <= most;
         }
-        if (!fits) continue;
-        u64 before;
-        a.template gather<true>(lo, hi, cut, total, before);
-        u64 mine = before;                                // of this warp
+      if (!fits) {
+        lo = s.first[1];
+        hi = min(last, s.first[2]);
+      }
+      u64 total, before;                                  // before: the weight of what lies before bin lo
+      a.template gather<kAll>(lo, hi, cut, total, before);
+      auto of_warp = [](u64 v) {
 #pragma unroll
-        for (int m = 16; m >= 1; m /= 2) mine += __shfl_xor_sync(0xffffffffu, mine, m);
-        if (a.lane == 0) s.kept[a.warp] = mine;
-        a.sums(total, before);
+        for (int m = 16; m >= 1; m /= 2) v += __shfl_xor_sync(0xffffffffu, v, m);
+        return v;
+      };
+      u64 mine = of_warp(before);
+      if (a.lane == 0) s.kept[a.warp] = mine;
+      a.sums(total, before);
+      const u64 reach = set.reach(total);
+      bool found = false;
+      // where the border is if it is not found: between these bins, with so much before them
+      int from = lo, to = hi;
+      u64 start = before;
+      for (int turn = 0; fits; ++turn) {
         u64 key = a.sorted();
-        const u64 reach = set.reach(total), w = key != 0 ? a.weight(key_logit(key)) : 0;
+        const u64 w = key != 0 ? a.weight(key_logit(key)) : 0;
         u64 sum;
-        upto = before + block_scan(w, s.part, &sum);
+        const u64 run = before + block_scan(w, s.part, &sum);
         // the border is in the list: the last token that the sum before it leaves short
-        if (t == 0) s.cut = s.size = 0;
+        if (t == 0) {
+          s.cut = s.size = 0;
+          s.rest = sum;
+        }
         s.list[t] = key;
         __syncthreads();
-        if (leader && key != 0 && upto - w < reach && upto >= reach) s.cut = key;
+        if (leader && key != 0 && run - w < reach && run >= reach) s.cut = key;
         a.sync();
         const u64 border = *a.cluster.map_shared_rank(&s.cut, 0);
         found = border != 0;
@@ -639,26 +769,90 @@ __global__ void __launch_bounds__(kThreads, 2) sample_many(const __grid_constant
           if (key >= cut && at >= 0 && at < p.slice) atomicAdd(&s.kept[at / a.per], a.weight(key_logit(key)));
           summed = a.weight(key_logit(cut)) >= set.least;  // min_p cuts nothing off
         }
+        __syncthreads();                                  // s.kept is written; s.first and s.part2 are no longer read
+        if (found || turn == 1) break;
+        // It is off by a known weight from an edge of the list: where the bins' masses say, from there on.
+        const bool after = reach > before;
+        const u64 edge = after ? before + *a.cluster.map_shared_rank(&s.rest, 0) : before;
+        from = after ? hi + 1 : 0;
+        to = after ? last : lo - 1;
+        start = after ? edge : 0;
+        const int old = lo, at = after ? hi + 1 : lo;
+        masses(unit, upto);
+        u64 e = upto;
+        if (t < 4) s.first[1 + t] = last;
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+          if (b0 + j == at) s.part2[0] = e;
+          e += unit[j];
+        }
         __syncthreads();
+        if (from > to) break;                             // no such bin
+        const long long off = ((long long)reach - (long long)edge) >> (kBits - 24), slack = (off < 0 ? -off : off) / 32 + 8;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const long long value = max(0ll, (long long)s.part2[0] + off + (i == 0 ? -slack : i == 1 ? slack : 0));
+          long long e2 = (long long)upto;
+#pragma unroll
+          for (int j = 0; j < kPer; ++j) {
+            if (e2 <= value && e2 + (long long)unit[j] > value) s.first[1 + i] = b0 + j;
+            e2 += (long long)unit[j];
+          }
+        }
+        __syncthreads();
+        fits = false;
+        for (int i = 0; i < 4 && !fits; i += 2) {
+          lo = min(max(s.first[1 + i], from), to);
+          hi = max(min(s.first[2 + i], to), lo);
+          fits = tokens(lo, hi) <= kList;
+        }
+        if (!fits) break;
+        u64 none0;
+        a.template gather<kSome>(lo, hi, cut, none0, mine, min(lo, old), max(lo, old));
+        u64 part = mine, none1 = 0;
+        mine = of_warp(mine);
+        if (a.lane == 0) s.kept[a.warp] += after ? mine : 0 - mine;
+        a.sums(part, none1);
+        before += after ? part : 0 - part;
       }
       if (!found) {
-        total = a.template above<true>(cut, 0);
-        cut = max(cut, a.template bisect<true>(cut, set.reach(total)));
+        u64 lowest = max(cut, a.highest_key(to + 1) + 1), highest = a.highest_key(from);
+        if (reach <= start) {
+          highest = ~0ull;
+          lowest = max(cut, a.highest_key(from) + 1);
+          start = 0;
+        }
+        u64 key = lowest;
+        if (!a.template search<true>(key, highest, start, reach) && lowest > cut) {
+          key = cut;
+          a.template search<true>(key, lowest - 1, start, reach);
+        }
+        cut = key;
       }
     }
   }
-  auto kept = [&](int i, float l) -> u64 {
-    const u64 w = a.weight(l);
-    return i < a.last && (cut == 0 || rank_key(l, i) >= cut) && w >= set.least ? w : 0;
-  };
+  const Border border(cut);
   u64 sum = 0;
   if (summed) {
     sum = s.kept[a.warp];
   } else {
-    a.each([&](int i, const float (&l)[4]) {
+    double kept = 0.0;                                    // past the warp's last token l is -inf, its weight zero
+    if (cut == 0 && set.least == 0) {
+      a.each([&](int, const float (&l)[4]) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) sum += kept(i + j, l[j]);
-    });
+        for (int j = 0; j < 4; ++j) kept += a.weight.units(l[j]);
+      });
+    } else {
+      const double least = (double)set.least;
+      a.each([&](int i, const float (&l)[4]) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const double w = a.weight.units(l[j]);
+          if (border(l[j], i + j) && w >= least) kept += w;
+        }
+      });
+    }
+    sum = (u64)kept;
 #pragma unroll
     for (int m = 16; m >= 1; m /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, m);
   }
@@ -687,27 +881,29 @@ __global__ void __launch_bounds__(kThreads, 2) sample_many(const __grid_constant
   __syncthreads();
   if (s.owner >= 0) {
     const int begin = a.base + s.owner * a.per, end = min(min(p.V, a.base + p.slice), begin + a.per);
-    const int each = (a.per + kThreads - 1) / kThreads;
-    const u64 rest = s.rest;
-    auto at = [&](int j) -> u64 {                         // of this thread's j-th token
-      const int i = begin + t * each + j;
-      if (i >= end) return 0;
-      float l;
-      if (p.cached) {
-        l = s.logits[i - a.base];
-      } else {
-        l = ssm::to_f32(a.logits[i]);
-        if (a.infinite) l = l == kInf ? 0.0f : -kInf;
+    u64 rest = s.rest;
+    for (int at = begin; at < end; at += 4 * kThreads) {  // four tokens to a thread
+      const int i = at + 4 * t;
+      u64 w[4], own = 0, all;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float l = -kInf;
+        if (i + j < end) {
+          l = p.cached ? s.logits[i + j - a.base] : ssm::to_f32(a.logits[i + j]);
+          if (a.infinite && !p.cached) l = l == kInf ? 0.0f : -kInf;
+        }
+        w[j] = a.weight(l);
+        if (!border(l, i + j) || w[j] < set.least) w[j] = 0;
+        own += w[j];
       }
-      const u64 w = a.weight(l);
-      return (cut == 0 || rank_key(l, i) >= cut) && w >= set.least ? w : 0;
-    };
-    u64 own = 0, all;
-    for (int j = 0; j < each; ++j) own += at(j);
-    u64 run = block_scan(own, s.part, &all) - own;
-    for (int j = 0; run <= rest && j < each; ++j) {
-      run += at(j);
-      if (run > rest) p.token[a.row] = begin + t * each + j;
+      u64 run = block_scan(own, s.part, &all) - own;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (run <= rest && run + w[j] > rest) p.token[a.row] = i + j;
+        run += w[j];
+      }
+      if (rest < all) break;
+      rest -= all;
     }
   }
   a.sync();
@@ -766,7 +962,7 @@ extern "C" int ssm_sample_tokens(int64_t B, int64_t V, ssm_view logits, const fl
   const size_t most = sizeof(SampleSmem) + kCached * sizeof(float);
   if (p.bf16) ssm::ctas_per_sm<sample_many<__nv_bfloat16>>(kThreads, most);
   else ssm::ctas_per_sm<sample_many<float>>(kThreads, most);
-  const size_t smem = sizeof(SampleSmem) + (p.cached ? p.slice * sizeof(float) : 0);
+  const size_t smem = sizeof(SampleSmem) + (p.cached ? p.slice * sizeof(float) : kDepth * kThreads * sizeof(uint4));
   const cudaError_t e = ssm::launch_pdl_cluster(p.bf16 ? sample_many<__nv_bfloat16> : sample_many<float>, (unsigned)(B * ctas), kThreads,
                                                 (unsigned)ctas, smem, st, p);
   return e == cudaSuccess ? SSM_OK : fail(SSM_ERR_CUDA, "sample_tokens launch failed (error %lld)", (long long)e);

@@ -500,6 +500,30 @@ def test_sample_layouts():
     assert [int(sample_tokens(wide[b:b + 1], u[b:b + 1], top_k=50)) for b in range(9)] == same.tolist()
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("B,V", [(3, 5003), (3, 50257), (3, 131072), (200, 131072), (3, 300001), (2, 1 << 20)])
+def test_sample_borders_of_dense_rows(B, V, dtype):
+    """The border itself: rows in rising order drawn at 0 give the first token by index, the lowest that is kept; falling ones, just
+    below 1, the last.  Borders fall where few tokens are and where thousands share a value.
+
+    A weight is a whole number of 2^-42 of the largest, off by 2^-43 at most, and a sum of V of them by E = V 2^-43.  With R a running
+    sum and T the place that is drawn: R[want - 1] <= T < R[want], and the same of got in whole numbers, each side off by E.  So
+    what lies between the two tokens weighs less than 2 E; the border of top_p, a place in such sums too, adds as much."""
+    rows = [0, 1, B - 1]
+    for width in (0.3, 1.0, 3.0, 5.0):
+        up = (width * _randn(B, V, seed=V)).to(dtype).sort(-1).values
+        for logits, at in ((up, 0.0), (up.flip(-1).contiguous(), 1 - 2.0 ** -24)):
+            u = torch.full((B,), at, device=DEV)
+            for kw in (dict(top_p=0.5), dict(top_p=0.9), dict(top_p=0.95), dict(top_p=0.999), dict(top_k=V // 2), dict(top_k=3000, top_p=0.95),
+                       dict(top_p=0.95, temperature=0.6)):
+                got = sample_tokens(logits, u, **kw).tolist()
+                for b in rows:
+                    want = _sample_rows(logits[b:b + 1], u[b:b + 1], **kw)[0]
+                    l = logits[b].double()
+                    between = torch.exp((l[min(got[b], want) + 1:max(got[b], want)] - l.max()) / kw.get("temperature", 1.0))
+                    assert got[b] == want or float(between.sum()) < 4 * V * 2.0 ** -43, (width, at, kw, got[b], want)
+
+
 def test_sample_the_largest_vocabulary():
     V = 1 << 20
     logits = 3 * _randn(2, V, seed=1)
