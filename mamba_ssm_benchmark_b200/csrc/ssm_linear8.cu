@@ -281,9 +281,10 @@ __global__ void __launch_bounds__(kLinThreads, TN <= 64 ? 2 : 1) linear_e4m3(con
   const int first = SPLIT ? (int)blockIdx.x / parts : (int)blockIdx.x, step = SPLIT ? p.tiles : (int)gridDim.x;
   const int k0 = SPLIT ? (int)((long long)p.blocks * rank / parts) : 0;
   const int k1 = SPLIT ? (int)((long long)p.blocks * (rank + 1) / parts) : p.blocks;
-  // What the first tile reads of the weight goes to L2 while the kernel before still runs (L2 is where all
-  // writes meet, so a weight that this kernel writes is not read stale): a layer as below with 64 tokens takes 24.3 us for 27.3,
-  // with 16 tokens 18.3 for 21.0, with one 18.8 for 19.7.  With tokens in the lanes it gained 1 % of a layer of 128 and lost as much of one of 512.
+  // What the first tile reads of the weight goes to L2 while the kernel before still runs (L2 is where all writes meet, so a
+  // weight that this kernel writes is not read stale): a layer as below with 64 tokens takes 24.3 us for 27.3, with 16 tokens
+  // 18.3 for 21.0, with one 18.8 for 19.7.  With tokens in the lanes it gained 1 % of a layer of 128 and lost as much of one
+  // of 512.
   if (!TOKENS && warp == kOutWarps) {
     const int row = first % p.tiles_n * kRows;
     for (int k = k0 + lane; k < k1; k += 32) tma_prefetch_2d(&p.ta, k * kBlockK, row);
@@ -546,7 +547,8 @@ int ssm_linear_fp8(int64_t tokens, int64_t channels, int64_t K, const void* x8, 
   p.wide = aligned(32);
   CUtensorMap &mx = by_token ? p.ta : p.tb, &mw = by_token ? p.tb : p.ta;
   if (!encode_rows8(&mx, x8, tokens, K, x_stride, by_token ? kRows : tn) ||
-      !encode_rows8(&mw, w8, channels, K, w_stride, by_token ? tn : kRows)) return fail(SSM_ERR_CUDA, "linear_fp8: the tensor maps could not be made");
+      !encode_rows8(&mw, w8, channels, K, w_stride, by_token ? tn : kRows))
+    return fail(SSM_ERR_CUDA, "linear_fp8: the tensor maps could not be made");
   p.w_scale = w_scale;
   p.x_scale = x_scale;
   p.bias = bias;

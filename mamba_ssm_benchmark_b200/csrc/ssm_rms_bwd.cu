@@ -320,9 +320,10 @@ int ssm_rms_norm_bwd(int64_t rows, int64_t C, ssm_view total, const void* weight
                                            : run<__nv_bfloat16, __nv_bfloat16>(p, aligned, &parts, stat, st);
   if (e == cudaSuccess && dweight != nullptr) {
     const unsigned grid = (unsigned)rms_ceil(C, 32);
+    const dim3 block(32, 8);
     e = weight_dtype == SSM_BF16
-            ? launch_pdl(rms_dweight<__nv_bfloat16>, grid, dim3(32, 8), 0, st, p.part, parts, p.C, static_cast<__nv_bfloat16*>(dweight))
-            : launch_pdl(rms_dweight<float>, grid, dim3(32, 8), 0, st, p.part, parts, p.C, static_cast<float*>(dweight));
+            ? launch_pdl(rms_dweight<__nv_bfloat16>, grid, block, 0, st, p.part, parts, p.C, static_cast<__nv_bfloat16*>(dweight))
+            : launch_pdl(rms_dweight<float>, grid, block, 0, st, p.part, parts, p.C, static_cast<float*>(dweight));
   }
   if (e != cudaSuccess) return fail(SSM_ERR_CUDA, "rms_norm backward launch failed (error %lld)", (long long)e);
   return SSM_OK;

@@ -6,7 +6,7 @@
 //
 // A token must not depend on how sums are split, nor change when a sum's rounding does: weights are whole numbers in
 // units of 2^-42, formed in double, and every sum is a 64-bit whole number, exact in any order (up to 2^20 tokens).  A weight
-// is off by at most 2^-43 of the largest; what rounds to zero is never drawn.
+// is cut down by less than 2^-42 of the largest; what is less than that is never drawn.
 //
 // Up to kFew tokens: a thread each, sorted by rank in registers (a byte of one sequence: 7 us, most of it the launch).
 // More: a cluster of up to eight CTAs shares a row, a slice of tokens each, kept in shared memory where two CTAs to an SM have
@@ -15,9 +15,10 @@
 // sums of what lies before them.  Where the bins' masses mislead, the exact sum at the list's edge says where to look next; where
 // a bin holds more than kList tokens (hundreds of equal logits) a pass over the row takes eleven bits of the border's rank.
 //
-// 256 x 131072 fp32 by top-p: 162 us, 0.4 GB of DRAM (three passes over what does not stay in L2) at 30 % of its rate; 57 % of
-// the issue slots, forty instructions to a weight, bound it.  64 x 50257 bf16 with all rules: 18 us, the barriers of
-// passes of 1 to 3 us each.  Bisection alone, the first form, took 6690 and 518 us.
+// 256 x 131072 fp32 by top-p: 138 us, 0.4 GB of DRAM in three passes, whose loads are four ahead in slots of shared memory; the
+// instructions they issue bound them, on the 108 SMs that have two rows (clocks in the kernel: maximum 38 thousand,
+// histogram 64, list and sums 115, all else 45).  By temperature alone 72 us, by top-k 75.  64 x 50257 bf16 with all rules: 18 us,
+// the barriers of passes of 1 to 3 us each.  Bisection of the rank, the first form, took 6690 and 518 us.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -91,9 +92,13 @@ __device__ __forceinline__ float key_logit(u64 key) {
 }
 __device__ __forceinline__ int key_token(u64 key) { return (int)(0xffffffffu - (uint32_t)key); }
 
-// A weight in whole units: 2^42 2^y, y = (l - top) rate, for finite top and l <= top.  2^y = 2^k 2^(j/1024) 2^r, |r| <= 2^-11:
-// the Taylor polynomial of degree 3 is within (ln 2 / 2048)^4 / 24 = 6e-16 of 2^r.  y is held above -60, where the weight is
-// zero, by its high word: of two negative numbers the larger has the smaller one.
+// ln 2, its square by 2, its cube by 6: from constant memory an operand of the instruction, not two moves before it.
+constexpr double kLn2 = 0.69314718055994531;
+__constant__ double kTaylor[3] = {kLn2, kLn2 * kLn2 / 2, kLn2 * kLn2 * kLn2 / 6};
+
+// A weight in whole units: 2^42 2^y cut to a whole number, y = (l - top) rate, for finite top and l <= top.  2^y = 2^k 2^(j/1024)
+// 2^r, |r| <= 2^-11: the Taylor polynomial of degree 3 is within (ln 2 / 2048)^4 / 24 = 6e-16 of 2^r.  y is held above -60, where
+// the weight is zero, by its high word: of two negative numbers the larger has the smaller one.
 struct Weights {
   static constexpr double kRaised = 4503599627370496.0;
   const double* table;                // 2^(42 + j / 1024), its high word less j 2^10: adding 1024 y 2^10 adds k to the exponent
@@ -106,26 +111,25 @@ struct Weights {
     const double v = exp2((double)j / kTable + kBits);
     return __hiloint2double(__double2hiint(v) - (j << 10), __double2loint(v));
   }
-  // 2^52 and the weight, rounded
-  __device__ __forceinline__ double raised(float l) const {
-    constexpr double kLn2 = 0.69314718055994531, kC2 = kLn2 * kLn2 / 2, kC3 = kLn2 * kLn2 * kLn2 / 6;
+  // The sum and the weight, cut to a whole number by the addition itself: the sum is a whole number of 2^52 up to 2^53, where
+  // doubles are a unit apart, and rounding down is the same whatever it is added to.  A thread starts its sum at kRaised
+  // and has up to 2^10 tokens.  The passes over whole rows are bound by the instructions they issue: this takes two off.
+  __device__ __forceinline__ double add(float l, double sum) const {
     constexpr double kShift = 6755399441055744.0 / kTable;   // 1.5 2^52 / 1024: y is rounded to 1024ths
     const double raw = ((double)l - top) * rate;
     const double y = __hiloint2double((int)min((uint32_t)__double2hiint(raw), 0xc04e0000u), __double2loint(raw));      // -60
     const double t = y + kShift;
     const int i = __double2loint(t);                       // 1024 y, rounded
     const double r = y - (t - kShift);
-    const double q = fma(r, fma(r, fma(r, kC3, kC2), kLn2), 1.0);
+    const double q = fma(r, fma(r, fma(r, kTaylor[2], kTaylor[1]), kTaylor[0]), 1.0);
     const double step = table[i & (kTable - 1)];
     const double scaled = __hiloint2double(__double2hiint(step) + i * kTable, __double2loint(step));
-    return fma(scaled, q, kRaised);
+    return __fma_rd(scaled, q, sum);
   }
   __device__ __forceinline__ u64 operator()(float l) const {
-    return (u64)__double_as_longlong(raised(l)) & ((1ull << 52) - 1);
+    return (u64)__double_as_longlong(add(l, kRaised)) & ((1ull << 52) - 1);
   }
-  // The same as a double, which holds a thread's sums too, all of them below 2^53: the passes over whole rows are bound by what
-  // works on whole numbers, not by the arithmetic in double.
-  __device__ __forceinline__ double units(float l) const { return raised(l) - kRaised; }
+  static __device__ u64 whole(double sum) { return (u64)(sum - kRaised); }
 };
 
 // Whether a token ranks at least as high as one with this key.
@@ -247,7 +251,7 @@ __global__ void __launch_bounds__(kFew) sample_few(const __grid_constant__ Sampl
   const double top = key_logit(best), rate = 1.4426950408889634 / set.temperature;
   auto weight = [&](float v) {                            // as in Weights, by the library's function: no table to make
     const double y = ((double)v - top) * rate;
-    return v == key_logit(best) ? kOne : y > -60.0 ? (u64)__double2ll_rn(exp2(y) * (double)kOne) : 0;
+    return v == key_logit(best) ? kOne : y > -60.0 ? (u64)__double2ll_rd(exp2(y) * (double)kOne) : 0;
   };
   u64 total, w = 0;
   const bool top_k = set.top_k > 0 && set.top_k < p.V;
@@ -321,29 +325,34 @@ struct Sampler {
         ssm::load4(s.logits + (i - base), l);
         f(i, l);
       }
-    } else if (p.wide) {                  // from L2 or memory: the next ones on their way to this thread's slots
-      uint4* slots = reinterpret_cast<uint4*>(s.logits) + threadIdx.x;
-      auto fetch = [&](int i, int slot) {
-        if (i + 4 <= last)
-          asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(ssm::smem_u32(slots + slot * kThreads)), "l"(logits + i),
-                       "n"(4 * sizeof(T))
-                       : "memory");
+    } else if (p.wide && !infinite) {     // from L2 or memory: the next ones on their way to this thread's slots
+      constexpr uint32_t kStep = kThreads * 16, kRing = kDepth * kStep;
+      const uint32_t ring = ssm::smem_u32(s.logits) + threadIdx.x * 16;
+      const T* from = logits + first + 4 * lane;
+      const int steps = (last - first) >> 7;              // that are whole for the warp
+      auto fetch = [&](int step, const T* src, uint32_t at) {
+        if (step < steps)
+          asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(ring + at), "l"(src), "n"(4 * sizeof(T)) : "memory");
         asm volatile("cp.async.commit_group;" ::: "memory");
       };
-      int i = first + 4 * lane;
 #pragma unroll
-      for (int d = 0; d < kDepth; ++d) fetch(i + 128 * d, d);
-      for (int slot = 0; i < last; i += 128, slot = (slot + 1) % kDepth) {
+      for (int d = 0; d < kDepth; ++d) fetch(d, from + 128 * d, d * kStep);
+      int i = first + 4 * lane;
+      uint32_t at = 0;
+      for (int step = 0; step < steps; ++step) {
         float l[4];
         asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory");
-        if (i + 4 <= last) {
-          ssm::load4(reinterpret_cast<const T*>(slots + slot * kThreads), l);
-          if (infinite) finite(l);
-        } else {
-          load(i, l);
-        }
+        ssm::load4(reinterpret_cast<const T*>(reinterpret_cast<const char*>(s.logits) + threadIdx.x * 16 + at), l);
         f(i, l);
-        fetch(i + 128 * kDepth, slot);
+        fetch(step + kDepth, from + 128 * kDepth, at);
+        from += 128;
+        i += 128;
+        at = (at + kStep) & (kRing - 1);
+      }
+      if (i < last) {
+        float l[4];
+        load(i, l);
+        f(i, l);
       }
     } else {
       for (int i = first + 4 * lane; i < last; i += 128) {
@@ -495,7 +504,7 @@ struct Sampler {
     u64* list = cluster.map_shared_rank(s.list, 0);
     const float begin = (float)lo, end = (float)(hi + 1), some = (float)from, others = (float)to;
     const Border border(cut);
-    double all = 0.0, higher = 0.0;
+    double all = Weights::kRaised, higher = Weights::kRaised;
     auto body = [&](int i, const float (&l)[4], auto cuts) {
       bool here[4];
 #pragma unroll
@@ -503,11 +512,11 @@ struct Sampler {
         const float z = distance(l[j]);
         const bool in = !cuts || border(l[j], i + j);
         if constexpr (ADDS == kAll) {
-          const double w = weight.units(in ? l[j] : -__builtin_huge_valf());
-          all += w;
-          if (z < begin) higher += w;
+          const float v = in ? l[j] : -__builtin_huge_valf();
+          all = weight.add(v, all);
+          if (z < begin) higher = weight.add(v, higher);
         } else if constexpr (ADDS == kSome) {
-          if (in && z >= some && z < others) higher += weight.units(l[j]);
+          if (in && z >= some && z < others) higher = weight.add(l[j], higher);
         }
         here[j] = z >= begin && z < end && in;
       }
@@ -522,8 +531,8 @@ struct Sampler {
     };
     if (cut != 0) each([&](int i, const float (&l)[4]) { body(i, l, std::true_type()); });
     else each([&](int i, const float (&l)[4]) { body(i, l, std::false_type()); });
-    total = (u64)all;
-    before = (u64)higher;
+    total = Weights::whole(all);
+    before = Weights::whole(higher);
   }
   // x and y summed over the cluster, once the list is written: one barrier of the cluster for both.
   __device__ void sums(u64& x, u64& y) {
@@ -836,23 +845,23 @@ __global__ void __launch_bounds__(kThreads, 2) sample_many(const __grid_constant
   if (summed) {
     sum = s.kept[a.warp];
   } else {
-    double kept = 0.0;                                    // past the warp's last token l is -inf, its weight zero
+    double kept = Weights::kRaised;                                    // past the warp's last token l is -inf, its weight zero
     if (cut == 0 && set.least == 0) {
       a.each([&](int, const float (&l)[4]) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) kept += a.weight.units(l[j]);
+        for (int j = 0; j < 4; ++j) kept = a.weight.add(l[j], kept);
       });
     } else {
       const double least = (double)set.least;
       a.each([&](int i, const float (&l)[4]) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const double w = a.weight.units(l[j]);
-          if (border(l[j], i + j) && w >= least) kept += w;
+          const double next = a.weight.add(l[j], kept);
+          if (border(l[j], i + j) && next - kept >= least) kept = next;
         }
       });
     }
-    sum = (u64)kept;
+    sum = Weights::whole(kept);
 #pragma unroll
     for (int m = 16; m >= 1; m /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, m);
   }
@@ -951,10 +960,10 @@ extern "C" int ssm_sample_tokens(int64_t B, int64_t V, ssm_view logits, const fl
     const cudaError_t e = ssm::launch_pdl(p.bf16 ? sample_few<__nv_bfloat16> : sample_few<float>, (unsigned)B, threads, 0, st, p);
     return e == cudaSuccess ? SSM_OK : fail(SSM_ERR_CUDA, "sample_tokens launch failed (error %lld)", (long long)e);
   }
-  // CTAs to a row: as many as run at once.  A cluster's barriers cost a row as much as its passes (256 x 131072 by top-p: 300 us
-  // with eight CTAs to a row, 158 with one).
+  // CTAs to a row: as many as run at once, and so many that a thread has up to 2^10 tokens (Weights::add).  A cluster's barriers
+  // cost a row as much as its passes (256 x 131072 by top-p: 300 us with eight CTAs to a row, 158 with one).
   int ctas = 1;
-  while (ctas < 8 && V >= (int64_t)ctas * 4096 && B * ctas * 2 <= 296) ctas *= 2;
+  while (ctas < 8 && V >= (int64_t)ctas * 4096 && (B * ctas * 2 <= 296 || V > (int64_t)ctas << 19)) ctas *= 2;
   p.slice = (int)((V + ctas - 1) / ctas + 3) & ~3;
   p.cached = p.slice <= kCached;
   const int unit = p.bf16 ? 8 : 16;                        // bytes of four logits
@@ -963,7 +972,7 @@ extern "C" int ssm_sample_tokens(int64_t B, int64_t V, ssm_view logits, const fl
   if (p.bf16) ssm::ctas_per_sm<sample_many<__nv_bfloat16>>(kThreads, most);
   else ssm::ctas_per_sm<sample_many<float>>(kThreads, most);
   const size_t smem = sizeof(SampleSmem) + (p.cached ? p.slice * sizeof(float) : kDepth * kThreads * sizeof(uint4));
-  const cudaError_t e = ssm::launch_pdl_cluster(p.bf16 ? sample_many<__nv_bfloat16> : sample_many<float>, (unsigned)(B * ctas), kThreads,
-                                                (unsigned)ctas, smem, st, p);
+  const auto kern = p.bf16 ? sample_many<__nv_bfloat16> : sample_many<float>;
+  const cudaError_t e = ssm::launch_pdl_cluster(kern, (unsigned)(B * ctas), kThreads, (unsigned)ctas, smem, st, p);
   return e == cudaSuccess ? SSM_OK : fail(SSM_ERR_CUDA, "sample_tokens launch failed (error %lld)", (long long)e);
 }
