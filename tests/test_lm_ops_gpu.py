@@ -543,6 +543,61 @@ def _chain(idx, W, w, p8, ps, u):
     return sample_tokens(logits, u, temperature=0.8, top_k=40, top_p=0.9), total, logits
 
 
+@pytest.mark.parametrize("tokens", [1, 17, 64, 200])
+def test_parameters_written_just_before(tokens):
+    """A weight that the kernel right before writes, into the memory of the last one: what is fetched early is not used stale."""
+    x8, xs = _rows8(tokens, 640, 1)
+    x = _randn(tokens, 640, seed=2)
+    tables = [_randn(512, 640, seed=3 + i) * (1 + i) for i in range(4)]
+    first = torch.zeros(1, dtype=torch.int64, device=DEV)
+    own = [quantize_fp8(t) for t in tables]
+    torch.cuda.synchronize()
+    products = [linear_fp8(x8, xs, *o) for o in own]
+    norms = [rms_norm(x, t[0].clone()) for t in tables]
+    places = set()
+    for turn in range(40):
+        i = turn % 4
+        w8, ws = quantize_fp8(tables[i])
+        y = linear_fp8(x8, xs, w8, ws)
+        places.add(w8.data_ptr())
+        z = rms_norm(x, embedding(first, tables[i])[0])
+        assert torch.equal(y, products[i]) and torch.equal(z, norms[i]), turn
+        del w8, ws
+    assert len(places) < 40                                     # the memory did come again
+
+
+def test_two_streams_at_once():
+    """Kernels that are launched early, on two streams: products of every form share the SMs' tensor memory with those that wait."""
+    rows = {n: _rows8(n, 640, n) for n in (1, 20, 64, 130, 700, 5000)}
+    w8, ws = _rows8(640, 640, 9)
+    wide8, wides = _rows8(3000, 640, 10)
+    g = 1 + 0.1 * _randn(640, seed=11)
+    u = torch.rand(64, device=DEV, generator=_gen(12))
+
+    def run(sizes):
+        out = []
+        for n in sizes:
+            h = linear_fp8(*rows[n], w8, ws, dtype=BF16)
+            q, scale = rms_norm_fp8(h, g)
+            logits = linear_fp8(q, scale, wide8, wides, dtype=BF16)
+            out += [h, logits, sample_tokens(logits[:64], u[:min(n, 64)], top_k=30, top_p=0.9)]
+        return out
+
+    orders = [(1, 5000, 64, 20, 700, 130), (700, 1, 130, 5000, 20, 64)]
+    want = [run(order) for order in orders]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for _ in range(5):
+        for i in (0, 1):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(run(orders[i]))
+    torch.cuda.synchronize()
+    for i in (0, 1):
+        for one in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(one, want[i]))
+
+
 def test_graph_and_stream():
     """The operators after one another, captured with two graphs alive, and on a stream of their own."""
     W, w = _randn(500, 96, seed=1), 1 + 0.1 * _randn(96, seed=2)
