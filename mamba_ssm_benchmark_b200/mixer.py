@@ -263,9 +263,18 @@ class TokenEmbedding(nn.Embedding):
         return super().forward(idx)
 
 
-def _hooked(*modules):
-    return torch.nn.modules.module._has_any_global_hook() or any(
-        m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks for m in modules)
+def _untouched(module, cls):
+    """Whether module is a cls as it comes from here: no subclass, no method replaced on the instance, nothing hooked.  Only then
+    may its work be done without calling it."""
+    own = module.__dict__
+    return type(module) is cls and not ("forward" in own or "add" in own or "fp8" in own or "inner" in own) and not (
+        module._forward_hooks or module._forward_pre_hooks or module._backward_hooks or module._backward_pre_hooks
+        or torch.nn.modules.module._has_any_global_hook())
+
+
+def _adds(norm, x):
+    """Whether ``norm.add`` of x and a residual is what ``norm`` gives of their sum."""
+    return _untouched(norm, RMSNorm) and norm._fused(x)
 
 
 def _delta_mixer(*args, **kw):
@@ -292,9 +301,8 @@ class MambaBlock(nn.Module):
         return x + self.mixer(self.norm1(x), state, pos)
 
     def open(self, x):
-        """Whether ``inner`` computes what ``forward`` does of x and nobody watches the block's own result."""
-        return type(self) is MambaBlock and not isinstance(self.mixer.in_proj, Fp8Linear) and type(self.norm1) is RMSNorm \
-            and self.norm1._fused(x) and not _hooked(self, self.norm1)
+        """Whether ``inner`` computes what ``forward`` does of x and nobody watches or replaces the block's own result."""
+        return _untouched(self, MambaBlock) and not isinstance(self.mixer.in_proj, Fp8Linear) and _adds(self.norm1, x)
 
     def inner(self, h, x, state=None, pos=0):
         """The block without its own addition: for the residual stream x + h (h None: x) the mixer's result and the stream,
@@ -373,7 +381,7 @@ class MambaLM(nn.Module):
     def forward(self, idx, states=None, pos=0):
         x, h = self.embed(idx), None
         state = (lambda i: None) if states is None else states.__getitem__
-        if all(isinstance(b, MambaBlock) and b.open(x) for b in self.blocks) and not _hooked(self.norm_f):
+        if all(isinstance(b, MambaBlock) and b.open(x) for b in self.blocks) and _adds(self.norm_f, x):
             for i, block in enumerate(self.blocks):          # every norm adds what the mixer before it made
                 h, x = block.inner(h, x, state(i), pos)
             return self.head(self.norm_f(x) if h is None else self.norm_f.add(h, x)[0])
