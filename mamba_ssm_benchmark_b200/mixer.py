@@ -295,14 +295,18 @@ class MambaBlock(nn.Module):
         self.mixer = MambaMixer(d_model, **mixer_kw) if mixer == "mamba" else _delta_mixer(d_model, **mixer_kw)
         self.mlp = None
 
+    def _fp8(self):
+        """Whether the mixer takes its input in 8 bits; one of another kind need not have the projection."""
+        return isinstance(getattr(self.mixer, "in_proj", None), Fp8Linear)
+
     def forward(self, x, state=None, pos=0):
-        if isinstance(self.mixer.in_proj, Fp8Linear):
+        if self._fp8():
             return self.mixer(self.norm1.fp8(x), state, pos, residual=x)
         return x + self.mixer(self.norm1(x), state, pos)
 
     def open(self, x):
         """Whether ``inner`` computes what ``forward`` does of x and nobody watches or replaces the block's own result."""
-        return _untouched(self, MambaBlock) and not isinstance(self.mixer.in_proj, Fp8Linear) and _adds(self.norm1, x)
+        return _untouched(self, MambaBlock) and not self._fp8() and _adds(self.norm1, x)
 
     def inner(self, h, x, state=None, pos=0):
         """The block without its own addition: for the residual stream x + h (h None: x) the mixer's result and the stream,

@@ -95,3 +95,18 @@ def test_a_float32_end_of_a_bf16_model(kw):
     with torch.no_grad():
         got, want = lm(idx), _one_by_one(lm, idx)
     assert got.dtype == torch.float32 and torch.equal(got, want)
+
+
+def test_a_mixer_of_another_kind():
+    """A block around a module that takes (u, state, pos) and has no projections of the mixers' names."""
+    class Half(nn.Module):
+        def forward(self, u, state=None, pos=0):
+            return 0.5 * u
+
+    lm, idx = _lm(), _ids()
+    for block in lm.blocks:
+        block.mixer = Half()
+    with torch.no_grad():
+        assert _near(lm(idx), _one_by_one(lm, idx), 1e-5)
+        x = torch.randn(2, 3, 64, device=DEV)
+        assert torch.equal(lm.blocks[0](x), x + 0.5 * lm.blocks[0].norm1(x))
