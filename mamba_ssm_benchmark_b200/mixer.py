@@ -244,7 +244,12 @@ class RMSNorm(nn.Module):
         return F.rms_norm(x.float(), (x.shape[-1],), eps=self.eps).to(x.dtype) * self.weight
 
     def add(self, x, residual):
-        """(norm of x + residual, x + residual), in one pass over them."""
+        """(norm of x + residual, x + residual), in one pass over them.  Both are in the type of the sum, the wider of the two."""
+        if x.shape != residual.shape or x.dtype not in nat.DTYPES or residual.dtype not in nat.DTYPES:
+            total = x + residual
+            return self(total), total
+        if residual.dtype != x.dtype and x.dtype != torch.float32:      # rms_norm's result is in its first argument's
+            x, residual = residual, x
         return rms_norm(x, self.weight, residual=residual, eps=self.eps)
 
     def fp8(self, x):

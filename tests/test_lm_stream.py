@@ -110,3 +110,54 @@ def test_a_mixer_of_another_kind():
         assert _near(lm(idx), _one_by_one(lm, idx), 1e-5)
         x = torch.randn(2, 3, 64, device=DEV)
         assert torch.equal(lm.blocks[0](x), x + 0.5 * lm.blocks[0].norm1(x))
+
+
+class Cast(nn.Module):
+    """A mixer's result in another type, as one that computes in it gives; looks at what it is given."""
+
+    def __init__(self, mixer, given, to):
+        super().__init__()
+        self.mixer, self.given, self.to_type = mixer, given, to
+
+    def forward(self, u, state=None, pos=0):
+        assert u.dtype == self.given
+        return self.mixer(u, state, pos).to(self.to_type)
+
+
+@pytest.mark.parametrize("kw", KINDS)
+@pytest.mark.parametrize("to", [torch.bfloat16, torch.float16, torch.float64])
+def test_mixers_whose_results_have_another_type(kw, to):
+    """The stream and its norms are in the wider type, as those of x + mixer(norm(x)).  Where the additions are fused, the mixers
+    see the same float32 values but for the order of a norm's sums: 2^-20; a result of a mixer may then round the other way, a step
+    of its type (2^-7 of bf16) of few values: 1e-3 of the logits' norm."""
+    lm, idx = _lm(**kw), _ids()
+    wide = torch.promote_types(torch.float32, to)
+    for i, block in enumerate(lm.blocks):
+        block.mixer = Cast(block.mixer, wide if i > 0 and to == torch.float64 else torch.float32, to)
+    if to == torch.float64:                                 # the kernels' mixers take what the stream's second type gives as float32
+        for block in lm.blocks:
+            run = block.mixer.mixer.forward
+            block.mixer.mixer.forward = lambda u, *a, run=run: run(u.float(), *a)
+        lm.head = nn.Linear(64, 256, bias=False, dtype=torch.float64).to(DEV)
+    with torch.no_grad():
+        assert _near(lm(idx), _one_by_one(lm, idx), 1e-3)
+    n = RMSNorm(64).to(DEV)
+    x, h = torch.randn(5, 64, device=DEV), torch.randn(5, 64, device=DEV).to(to)
+    for a, b in ((x, h), (h, x), (x, h[:1])):
+        y, total = n.add(a, b)
+        assert torch.equal(total, a + b) and _near(y, n(a + b), 1e-6)
+
+
+@pytest.mark.parametrize("kw", KINDS)
+def test_autocast(kw):
+    """Under autocast the mixers give bf16 and the stream stays float32; logits and gradients as block by block, where a product's
+    input may round the other way: 2^-8 of few values, 1e-2 of a gradient's norm."""
+    lm, idx = _lm(**kw), _ids()
+
+    def run(forward):
+        with torch.autocast(DEV, torch.bfloat16):
+            logits = forward(idx)
+        return [logits, *torch.autograd.grad(logits.float().logsumexp(-1).mean(), list(lm.parameters()), allow_unused=True)]
+
+    for a, b in zip(run(lm), run(lambda i: _one_by_one(lm, i))):
+        assert (a is None and b is None) or _near(a, b, 1e-2)
