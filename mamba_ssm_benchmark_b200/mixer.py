@@ -35,7 +35,7 @@ from .conv import causal_conv1d
 from .decode import selective_state_update
 from .embed import embedding
 from .linear import Fp8Linear
-from .norm import rms_norm, rms_norm_fp8
+from .norm import quantize_fp8, rms_norm, rms_norm_fp8
 from .sampling import sample_tokens
 from .scan import selective_scan_fused
 
@@ -282,6 +282,11 @@ def _adds(norm, x):
     return _untouched(norm, RMSNorm) and norm._fused(x)
 
 
+def _normed8(norm, x):
+    """What ``norm`` gives of x, in 8 bits: from the kernel that norms and rounds, where norm is an RMSNorm that nobody touched."""
+    return norm.fp8(x) if _untouched(norm, RMSNorm) else quantize_fp8(norm(x))
+
+
 def _delta_mixer(*args, **kw):
     from .delta_mixer import GatedDeltaMixer        # which builds on this module
     return GatedDeltaMixer(*args, **kw)
@@ -306,7 +311,7 @@ class MambaBlock(nn.Module):
 
     def forward(self, x, state=None, pos=0):
         if self._fp8():
-            return self.mixer(self.norm1.fp8(x), state, pos, residual=x)
+            return self.mixer(_normed8(self.norm1, x), state, pos, residual=x)
         return x + self.mixer(self.norm1(x), state, pos)
 
     def open(self, x):
@@ -397,7 +402,7 @@ class MambaLM(nn.Module):
         for i, block in enumerate(self.blocks):
             x = block(x, state(i), pos)
         if isinstance(self.head, Fp8Linear):
-            return self.head(self.norm_f.fp8(x), dtype=x.dtype)
+            return self.head(_normed8(self.norm_f, x), dtype=x.dtype)
         return self.head(self.norm_f(x))
 
     @torch.no_grad()

@@ -161,3 +161,33 @@ def test_autocast(kw):
 
     for a, b in zip(run(lm), run(lambda i: _one_by_one(lm, i))):
         assert (a is None and b is None) or _near(a, b, 1e-2)
+
+
+@pytest.mark.parametrize("kw", KINDS)
+@pytest.mark.parametrize("what", ["norm1", "norm_f"])
+def test_norms_of_an_8_bit_model_have_their_say(kw, what):
+    """Hooks run and their results count, and so do subclasses.  A hook that changes nothing moves an e4m3 value only where the
+    norm's rounding to float32 before 8 bits does: one in 10^5 by an eighth, below 2e-3 of the logits' norm."""
+    lm, idx, seen = _lm(**kw).quantize_fp8(), _ids(), []
+    place = lm.norm_f if what == "norm_f" else lm.blocks[1].norm1
+    with torch.no_grad():
+        plain = lm(idx)
+        handle = place.register_forward_hook(lambda m, i, o: seen.append(o.shape))
+        assert _near(lm(idx), plain, 2e-3) and seen == [(2, 20, 64)]
+        handle.remove()
+        handle = place.register_forward_hook(lambda m, i, o: 2 * o)
+        twice = lm(idx)
+        handle.remove()
+        assert torch.equal(lm(idx), plain)
+        other = Twice(64).to(DEV)
+        if what == "norm_f":
+            lm.norm_f = other
+            assert _near(twice, 2 * plain, 2e-3)
+        else:
+            lm.blocks[1].norm1 = other
+        assert torch.equal(lm(idx), twice) and not _near(twice, plain, 1e-2)
+        if what == "norm_f":
+            lm.norm_f = nn.LayerNorm(64).to(DEV)
+        else:
+            lm.blocks[1].norm1 = nn.LayerNorm(64).to(DEV)
+        assert not _near(lm(idx), plain, 1e-3)
