@@ -256,6 +256,17 @@ Tensor kernel_typed(const Tensor& t) { return kernel_type(t) ? t : t.to(at::kFlo
 // unit stride along the last axis
 Tensor unit(const Tensor& t) { return t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous(); }
 Tensor as_rows(const Tensor& t) { return unit(t.dim() == 2 ? t : t.reshape({-1, t.size(-1)})); }
+// a layout that is (rows, C) without a copy
+Tensor row_layout(const Tensor& t) {
+  bool fits = t.stride(-1) == 1 || t.size(-1) == 1;
+  int64_t next = -1;                          // the stride that the axis before needs
+  for (int64_t i = t.dim() - 2; i >= 0; --i) {
+    if (t.size(i) == 1) continue;
+    fits = fits && (next < 0 || t.stride(i) == next);
+    next = t.stride(i) * t.size(i);
+  }
+  return fits ? t : t.contiguous();
+}
 Tensor shaped(const Tensor& t, at::IntArrayRef shape) { return t.sizes() == shape ? t : t.reshape(shape); }
 
 void needs_cuda(const char* what, const Tensor& t) {
@@ -324,11 +335,12 @@ Tensor embedding(const Tensor& idx, const Tensor& weight, double scale) {
 }
 
 // ---- root-mean-square norm --------------------------------------------------------------------------
-// The arguments as the kernels take them: x and residual (rows, C), the residual float32 or like x.
+// The arguments as the kernels take them, but in the caller's shape: x and residual are (rows, C) without a copy, the residual is
+// float32 or like x.  They become rows inside the autograd function: a reshape in front of it would hand x and residual
+// two views of their one gradient, which leaves would both keep and add the next one to, each to the memory of the other.
 struct RmsArgs {
   Tensor x, residual, weight;
   at::ScalarType y_type, total_type;          // what the caller gets
-  std::vector<int64_t> shape;
   RmsArgs(const char* what, const Tensor& x0, const Maybe& w0, const Maybe& r0, double eps) {
     TORCH_CHECK_VALUE(x0.dim() >= 1 && x0.numel() > 0, "x must be (..., C) with no empty axis, got " + text(x0));
     const int64_t C = x0.size(-1);
@@ -345,17 +357,19 @@ struct RmsArgs {
     needs_cuda(what, x0);
     one_device(x0, {residual, weight});
     y_type = total_type = x0.scalar_type();
-    shape = x0.sizes().vec();
-    x = as_rows(kernel_typed(x0));
+    x = row_layout(kernel_typed(x0));
     if (residual.defined()) {
       total_type = at::promote_types(y_type, residual.scalar_type());
       if (residual.scalar_type() != at::kFloat && residual.scalar_type() != x.scalar_type()) residual = residual.to(at::kFloat);
-      residual = as_rows(residual);
+      residual = row_layout(residual);
     }
     if (weight.defined()) weight = kernel_typed(weight).contiguous();
   }
   static Tensor as(const Tensor& t, at::ScalarType type) { return t.scalar_type() == type ? t : t.to(type); }
 };
+
+// of what row_layout gives: never a copy, whose memory would be free before the launch
+ssm_view rows_view(const Tensor& t) { return view(!t.defined() || t.dim() == 2 ? t : t.view({-1, t.size(-1)})); }
 
 // (y, total), total undefined without a residual.
 std::tuple<Tensor, Tensor> rms_forward(const Tensor& x, const Tensor& residual, const Tensor& weight, double eps) {
@@ -363,8 +377,9 @@ std::tuple<Tensor, Tensor> rms_forward(const Tensor& x, const Tensor& residual, 
   const Tensor y = dense_like(x);
   Tensor total;
   if (residual.defined()) total = dense_like(residual);
-  check(ssm_rms_norm_fwd(x.size(0), x.size(1), view(x), view(residual), data(weight), weight.defined() ? code(weight) : SSM_F32,
-                         (float)eps, view(y), view(total), stream(x)),
+  const int64_t C = x.size(-1);
+  check(ssm_rms_norm_fwd(x.numel() / C, C, rows_view(x), rows_view(residual), data(weight),
+                         weight.defined() ? code(weight) : SSM_F32, (float)eps, rows_view(y), rows_view(total), stream(x)),
         "ssm_rms_norm_fwd");
   return {y, total};
 }
@@ -393,18 +408,20 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
       if (weight.defined()) dw = at::zeros(weight.sizes(), weight.options());
       return {dtotal.defined() ? dtotal.to(type) : Tensor(), dtotal, dw, Tensor()};
     }
-    const Tensor dy = dense(grads[0], type), dx = at::empty(total.sizes(), total.options().dtype(type));
+    const Tensor dy = row_layout(dense(grads[0], type)), dx = at::empty(total.sizes(), total.options().dtype(type));
+    if (dtotal.defined()) dtotal = row_layout(dtotal);
     Tensor dr, dw;
     if (residual && total.scalar_type() != type) dr = dense_like(total);
     if (weight.defined()) dw = dense_like(weight);
+    const int64_t C = dy.size(-1), rows = dy.numel() / C;
     size_t need = 0;
-    check(ssm_rms_norm_bwd_workspace_size(dy.size(0), dy.size(1), &need), "ssm_rms_norm_bwd_workspace_size");
+    check(ssm_rms_norm_bwd_workspace_size(rows, C, &need), "ssm_rms_norm_bwd_workspace_size");
     const Tensor ws = bytes(need, dy);
-    check(ssm_rms_norm_bwd(dy.size(0), dy.size(1), view(total), data(weight), weight.defined() ? code(weight) : SSM_F32,
-                           (float)ctx->saved_data["eps"].toDouble(), view(dy), view(dtotal), view(dx), view(dr),
+    check(ssm_rms_norm_bwd(rows, C, rows_view(total), data(weight), weight.defined() ? code(weight) : SSM_F32,
+                           (float)ctx->saved_data["eps"].toDouble(), rows_view(dy), rows_view(dtotal), rows_view(dx), rows_view(dr),
                            dw.defined() ? dw.mutable_data_ptr() : nullptr, ws.mutable_data_ptr(), need, stream(dy)),
           "ssm_rms_norm_bwd");
-    // in one type the two inputs' gradients are one tensor, as those of a sum of two tensors are
+    // in one type the two inputs' gradients are one tensor, as those of a sum of two tensors are; leaves then keep a copy and it
     return {dx, !residual ? Tensor() : dr.defined() ? dr : dx, dw, Tensor()};
   }
 };
@@ -422,8 +439,8 @@ variable_list rms_norm(const Tensor& x, const Maybe& weight, const Maybe& residu
     const auto [y, total] = rms_forward(a.x, a.residual, a.weight, eps);
     out = total.defined() ? variable_list{y, total} : variable_list{y};
   }
-  out[0] = shaped(RmsArgs::as(out[0], a.y_type), a.shape);
-  if (out.size() > 1) out[1] = shaped(RmsArgs::as(out[1], a.total_type), a.shape);
+  out[0] = RmsArgs::as(out[0], a.y_type);
+  if (out.size() > 1) out[1] = RmsArgs::as(out[1], a.total_type);
   return out;
 }
 
@@ -440,19 +457,19 @@ variable_list rms_norm_fp8(const Tensor& x, const Maybe& weight, const Maybe& re
   const RmsArgs a(what, x, weight, residual, eps);
   plain(what, {x, a.residual, a.weight});
   const c10::cuda::CUDAGuard guard(x.device());
-  const int64_t rows = a.x.size(0), C = a.x.size(1);
+  const int64_t C = x.size(-1), rows = x.numel() / C;
   Tensor y8 = rows8(rows, C, a.x), scale = at::empty({rows}, a.x.options().dtype(at::kFloat)), total;
   if (a.residual.defined()) total = dense_like(a.residual);
-  check(ssm_rms_norm_fp8(rows, C, view(a.x), view(a.residual), data(a.weight), a.weight.defined() ? code(a.weight) : SSM_F32,
-                         (float)eps, norm, y8.mutable_data_ptr(), y8.stride(0), f32(scale), view(total), stream(a.x)),
+  check(ssm_rms_norm_fp8(rows, C, rows_view(a.x), rows_view(a.residual), data(a.weight), a.weight.defined() ? code(a.weight) : SSM_F32,
+                         (float)eps, norm, y8.mutable_data_ptr(), y8.stride(0), f32(scale), rows_view(total), stream(a.x)),
         "ssm_rms_norm_fp8");
-  if (a.shape.size() != 2) {
-    const std::vector<int64_t> outer(a.shape.begin(), a.shape.end() - 1);
+  if (x.dim() != 2) {
+    const std::vector<int64_t> outer(x.sizes().begin(), x.sizes().end() - 1);
     y8 = outer.empty() ? y8.select(0, 0) : y8.unflatten(0, outer);
     scale = scale.reshape(outer);
   }
   if (!total.defined()) return {y8, scale};
-  return {y8, scale, shaped(RmsArgs::as(total, a.total_type), a.shape)};
+  return {y8, scale, RmsArgs::as(total, a.total_type)};
 }
 
 // ---- 8-bit products -----------------------------------------------------------------------------------

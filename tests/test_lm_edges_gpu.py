@@ -1,0 +1,67 @@
+"""Edges of the operators around a language model's mixers that their other tests pass by.  u = 2^-24."""
+
+import pytest
+import torch
+
+from mamba_ssm_benchmark_b200 import rms_norm, rms_norm_fp8
+from oracle import lm_oracle as O
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+U = 2.0 ** -24
+F32, BF16 = torch.float32, torch.bfloat16
+HALF = {F32: U, BF16: 2.0 ** -8}
+
+
+def _randn(*shape, seed=0, dtype=F32):
+    return torch.randn(*shape, device=DEV, generator=torch.Generator(device=DEV).manual_seed(seed)).to(dtype)
+
+
+@pytest.mark.parametrize("shape", [(8,), (4, 8), (2, 4, 8), (2, 3, 2, 24), (1, 1, 8), (3, 5, 1)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_gradients_of_leaves_do_not_share_memory(shape, dtype):
+    """x and residual have one gradient; kept by leaves of any number of axes, each adds the next one to its own memory."""
+    x, r = (_randn(*shape, seed=i, dtype=dtype).requires_grad_() for i in (1, 2))
+    w = torch.ones(shape[-1], device=DEV)
+
+    def step():
+        y, total = rms_norm(x, w, residual=r)
+        assert y.shape == total.shape == x.shape
+        (y.float().sum() + total.float().square().sum()).backward()
+
+    step()
+    first = x.grad.clone()
+    assert torch.equal(r.grad, first) and x.grad.data_ptr() != r.grad.data_ptr()
+    step()
+    assert torch.equal(x.grad, 2 * first) and torch.equal(r.grad, 2 * first)
+    x.grad.zero_()
+    assert torch.equal(r.grad, 2 * first)
+    x.grad = r.grad = None
+    rms_norm(x, w, residual=r)[1].sum().backward()          # only the sum is used
+    assert x.grad.data_ptr() != r.grad.data_ptr()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_rms_norm_of_any_layout(dtype):
+    """Axes in another order, broadcast, cut and stepped over, as x, residual and gradients: as of dense copies."""
+    a = _randn(4, 6, 5, 48, seed=1, dtype=dtype)
+    views = [a[:, :, 0], a[:, 2], a[1:, ::2, 1:4], a.transpose(0, 2), a.transpose(1, 3), a[..., 3:40], a[:, :1].expand(4, 6, 5, 48),
+             a[0, 0, 0].expand(7, 3, 48), a[:, :, :, :1], a[:, :, :1, :1], a[0, :1, 0], a[..., 1], a[0].movedim(0, -1), a.flip(0)[None]]
+    for i, v in enumerate(views):
+        dense = v.contiguous().clone()
+        C = v.shape[-1]
+        w = 1 + 0.1 * _randn(C, seed=2)
+        dy = _randn(*v.shape[::-1], seed=3, dtype=dtype).permute(*range(v.dim() - 1, -1, -1))
+        results = []
+        for x, r, g in ((v, v, dy), (dense, dense, dy.contiguous())):
+            x, r, wl = (t.detach().requires_grad_() for t in (x, r, w))
+            y, total = rms_norm(x, wl, residual=r)
+            alone = rms_norm(x, wl)
+            with torch.no_grad():
+                y8, scale, t8 = rms_norm_fp8(x, wl, residual=r)
+            results.append([y.detach(), total.detach(), alone.detach(), y8.float(), scale, t8, *torch.autograd.grad([y, total, alone], [x, r, wl], [g, g, g])])
+        for k, (p, q) in enumerate(zip(*results)):
+            # a layout that is not aligned adds a row's values in another order: 2 x 27 u, then a step of the type
+            tol = 54 * U + 2 * HALF[p.dtype] if k != 3 else 2.0 ** -3
+            assert p.shape == q.shape and p.dtype == q.dtype, (i, k)
+            assert float((p.double() - q.double()).norm()) <= tol * float(q.double().norm()), (i, k)
