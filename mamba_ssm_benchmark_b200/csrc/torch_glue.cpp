@@ -292,31 +292,53 @@ Tensor embedding_forward(const Tensor& idx, const Tensor& weight, double scale) 
   return y;
 }
 
+// idx: T dense ids, dy: (T, C); the result is (V, C).
+Tensor embedding_backward(const Tensor& idx, const Tensor& dy0, int64_t V, double scale) {
+  const c10::cuda::CUDAGuard guard(dy0.device());
+  const Tensor dy = dense(dy0, dy0.scalar_type()), dw = at::empty({V, dy.size(1)}, dy.options());
+  size_t need = 0;
+  check(ssm_embedding_bwd_workspace_size(dy.size(0), V, dy.size(1), &need), "ssm_embedding_bwd_workspace_size");
+  const Tensor ws = bytes(need, dy);
+  check(ssm_embedding_bwd(dy.size(0), V, dy.size(1), idx.const_data_ptr(), (int)idx.element_size(), (float)scale, view(dy), view(dw),
+                          ws.mutable_data_ptr(), need, stream(dy)),
+        "ssm_embedding_bwd");
+  return dw;
+}
+
+// again: the gradient can be differentiated once more, and so on; both directions are linear, and each is the other's.
 struct Embedding : torch::autograd::Function<Embedding> {
-  static Tensor forward(AutogradContext* ctx, const Tensor& weight, const Tensor& idx, double scale) {
+  static Tensor forward(AutogradContext* ctx, const Tensor& weight, const Tensor& idx, double scale, bool again) {
     ctx->save_for_backward({idx});
     ctx->saved_data["vocab"] = weight.size(0);
     ctx->saved_data["scale"] = scale;
-    return embedding_forward(idx, weight, scale);
+    ctx->saved_data["again"] = again;
+    return embedding_forward(idx, unit(weight), scale);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads);
+};
+struct EmbeddingGrad : torch::autograd::Function<EmbeddingGrad> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& dy, const Tensor& idx, int64_t V, double scale) {
+    ctx->save_for_backward({idx});
+    ctx->saved_data["scale"] = scale;
+    return embedding_backward(idx, dy, V, scale);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    once("embedding");
     const Tensor idx = ctx->get_saved_variables()[0];
-    const int64_t V = ctx->saved_data["vocab"].toInt();
-    const c10::cuda::CUDAGuard guard(grads[0].device());
-    const Tensor dy = dense(grads[0], grads[0].scalar_type()), dw = at::empty({V, dy.size(1)}, dy.options());
-    size_t need = 0;
-    check(ssm_embedding_bwd_workspace_size(dy.size(0), V, dy.size(1), &need), "ssm_embedding_bwd_workspace_size");
-    const Tensor ws = bytes(need, dy);
-    check(ssm_embedding_bwd(dy.size(0), V, dy.size(1), idx.const_data_ptr(), (int)idx.element_size(),
-                            (float)ctx->saved_data["scale"].toDouble(), view(dy), view(dw), ws.mutable_data_ptr(), need,
-                            stream(dy)),
-          "ssm_embedding_bwd");
-    return {dw, Tensor(), Tensor()};
+    return {Embedding::apply(grads[0], idx, ctx->saved_data["scale"].toDouble(), true), Tensor(), Tensor(), Tensor()};
   }
 };
+variable_list Embedding::backward(AutogradContext* ctx, variable_list grads) {
+  const bool again = ctx->saved_data["again"].toBool();
+  if (!again) once("embedding");
+  const Tensor idx = ctx->get_saved_variables()[0];
+  const int64_t V = ctx->saved_data["vocab"].toInt();
+  const double scale = ctx->saved_data["scale"].toDouble();
+  const Tensor dw = at::GradMode::is_enabled() ? EmbeddingGrad::apply(grads[0], idx, V, scale)
+                                               : embedding_backward(idx, grads[0], V, scale);
+  return {dw, Tensor(), Tensor(), Tensor()};
+}
 
-Tensor embedding(const Tensor& idx, const Tensor& weight, double scale) {
+Tensor embedding(const Tensor& idx, const Tensor& weight, double scale, bool again) {
   TORCH_CHECK_VALUE(weight.dim() == 2 && weight.numel() > 0,
                     "weight must be (vocabulary, channels) with no empty axis, got " + text(weight));
   TORCH_CHECK_TYPE(idx.scalar_type() == at::kLong || idx.scalar_type() == at::kInt,
@@ -327,7 +349,8 @@ Tensor embedding(const Tensor& idx, const Tensor& weight, double scale) {
   one_device(weight, {idx});
   plain("embedding", {weight});
   const Tensor ids = idx.dim() == 1 && idx.is_contiguous() ? idx : idx.reshape({-1}).contiguous(), w = unit(weight);
-  const Tensor y = at::GradMode::is_enabled() && wants(w) ? Embedding::apply(w, ids, scale) : embedding_forward(ids, w, scale);
+  const Tensor y = at::GradMode::is_enabled() && wants(w) ? Embedding::apply(w, ids, scale, again)
+                                                              : embedding_forward(ids, w, scale);
   if (idx.dim() == 1) return y;
   std::vector<int64_t> shape = idx.sizes().vec();
   shape.push_back(weight.size(1));
@@ -384,18 +407,31 @@ std::tuple<Tensor, Tensor> rms_forward(const Tensor& x, const Tensor& residual, 
   return {y, total};
 }
 
+// The gradients by torch's operators, which can be differentiated again: what the kernels do of the same tensors.
+variable_list rms_gradients(const Tensor& total, const Tensor& weight, const Tensor& dy, const Tensor& dtotal, double eps,
+                            at::ScalarType type, bool residual) {
+  const Tensor t = total.to(at::kFloat), g0 = dy.to(at::kFloat), rstd = (t.square().mean(-1, true) + eps).rsqrt(), n = t * rstd;
+  const Tensor g = weight.defined() ? g0 * weight.to(at::kFloat) : g0;
+  Tensor d = rstd * (g - n * (g * n).mean(-1, true)), dw;
+  if (dtotal.defined()) d = d + dtotal.to(at::kFloat);
+  if (weight.defined()) dw = (g0 * n).reshape({-1, t.size(-1)}).sum(0).to(weight.scalar_type());
+  return {d.to(type), residual ? d.to(total.scalar_type()) : Tensor(), dw, Tensor(), Tensor()};
+}
+
 struct RmsNorm : torch::autograd::Function<RmsNorm> {
-  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Maybe& residual, const Maybe& weight, double eps) {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Maybe& residual, const Maybe& weight, double eps,
+                               bool again) {
     const auto [y, total] = rms_forward(x, value(residual), value(weight), eps);
     ctx->save_for_backward({total.defined() ? total : x, value(weight)});
     ctx->saved_data["eps"] = eps;
+    ctx->saved_data["again"] = again;
     ctx->saved_data["bf16"] = x.scalar_type() == at::kBFloat16;
     ctx->saved_data["residual"] = total.defined();
     ctx->set_materialize_grads(false);
     return total.defined() ? variable_list{y, total} : variable_list{y};
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    once("rms_norm");
+    if (!ctx->saved_data["again"].toBool()) once("rms_norm");
     const variable_list saved = ctx->get_saved_variables();
     const Tensor &total = saved[0], &weight = saved[1];
     const bool residual = ctx->saved_data["residual"].toBool();
@@ -406,8 +442,10 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
     if (!grads[0].defined()) {                       // only the sum was used
       Tensor dw;
       if (weight.defined()) dw = at::zeros(weight.sizes(), weight.options());
-      return {dtotal.defined() ? dtotal.to(type) : Tensor(), dtotal, dw, Tensor()};
+      return {dtotal.defined() ? dtotal.to(type) : Tensor(), dtotal, dw, Tensor(), Tensor()};
     }
+    if (at::GradMode::is_enabled())
+      return rms_gradients(total, weight, grads[0], dtotal, ctx->saved_data["eps"].toDouble(), type, residual);
     const Tensor dy = row_layout(dense(grads[0], type)), dx = at::empty(total.sizes(), total.options().dtype(type));
     if (dtotal.defined()) dtotal = row_layout(dtotal);
     Tensor dr, dw;
@@ -422,19 +460,19 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
                            dw.defined() ? dw.mutable_data_ptr() : nullptr, ws.mutable_data_ptr(), need, stream(dy)),
           "ssm_rms_norm_bwd");
     // in one type the two inputs' gradients are one tensor, as those of a sum of two tensors are; leaves then keep a copy and it
-    return {dx, !residual ? Tensor() : dr.defined() ? dr : dx, dw, Tensor()};
+    return {dx, !residual ? Tensor() : dr.defined() ? dr : dx, dw, Tensor(), Tensor()};
   }
 };
 
 // (y) or (y, total)
-variable_list rms_norm(const Tensor& x, const Maybe& weight, const Maybe& residual, double eps) {
+variable_list rms_norm(const Tensor& x, const Maybe& weight, const Maybe& residual, double eps, bool again) {
   const RmsArgs a("RMS norm", x, weight, residual, eps);
   plain("rms_norm", {x, value(residual), value(weight)});
   variable_list out;
   const bool wanted = wants(a.x) || (a.residual.defined() && wants(a.residual)) || (a.weight.defined() && wants(a.weight));
   if (at::GradMode::is_enabled() && wanted) {
     auto maybe = [](const Tensor& t) { return t.defined() ? Maybe(t) : Maybe(); };
-    out = RmsNorm::apply(a.x, maybe(a.residual), maybe(a.weight), eps);
+    out = RmsNorm::apply(a.x, maybe(a.residual), maybe(a.weight), eps, again);
   } else {
     const auto [y, total] = rms_forward(a.x, a.residual, a.weight, eps);
     out = total.defined() ? variable_list{y, total} : variable_list{y};

@@ -14,4 +14,4 @@ def embedding(idx, weight, scale=1.0):
     idx: int64 or int32 token ids of any shape; weight: (V, C) float32 or bfloat16, unit stride along C (other layouts
     are copied); scale: a number.  Differentiable with respect to weight.  An id outside 0 .. V-1 gives a row of NaN and no
     gradient, and sets a bit of the device error word."""
-    return nat.glue().embedding(idx, weight, scale)
+    return nat.glue().embedding(idx, weight, scale, False)

@@ -29,13 +29,13 @@ from types import SimpleNamespace
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+from torch.autograd import forward_ad
 
 from . import _native as nat
 from .conv import causal_conv1d
 from .decode import selective_state_update
-from .embed import embedding
 from .linear import Fp8Linear
-from .norm import quantize_fp8, rms_norm, rms_norm_fp8
+from .norm import quantize_fp8, rms_norm_fp8
 from .sampling import sample_tokens
 from .scan import selective_scan_fused
 
@@ -226,8 +226,19 @@ class MambaMixer(nn.Module):
         return y.unsqueeze(1), delta
 
 
+_TENSORS = (torch.Tensor, nn.Parameter)
+
+
+def _runs_now(a, b):
+    """Whether a and b are tensors that a kernel can be given, and the call is nothing but a call: not one of ``torch.compile``, export
+    or ``torch.jit.trace``, of forward-mode derivatives or of ``torch.func``.  All of these go through torch's own operators."""
+    return not (torch.compiler.is_compiling() or torch.jit.is_tracing() or forward_ad._current_level >= 0
+                or torch._C._functorch.peek_interpreter_stack() is not None) and type(a) in _TENSORS and type(b) in _TENSORS
+
+
 class RMSNorm(nn.Module):
-    """Root-mean-square normalisation in float32, then a learned per-feature scale."""
+    """Root-mean-square normalisation in float32, then a learned per-feature scale.  On the GPU by this package's kernels, which it
+    can be differentiated through any number of times."""
 
     def __init__(self, d, eps=1e-5):
         super().__init__()
@@ -236,11 +247,12 @@ class RMSNorm(nn.Module):
 
     def _fused(self, x):
         """The kernels take x: on the GPU, in one of their types, which the weight has too."""
-        return x.is_cuda and x.dtype in nat.DTYPES and x.dtype == self.weight.dtype and x.numel() > 0
+        return x.is_cuda and x.dtype in nat.DTYPES and x.dtype == self.weight.dtype and x.numel() > 0 and _runs_now(x, self.weight)
 
     def forward(self, x):
-        if self._fused(x):
-            return rms_norm(x, self.weight, eps=self.eps)
+        if not torch.jit.is_scripting():
+            if self._fused(x):
+                return nat.glue().rms_norm(x, self.weight, None, self.eps, True)[0]
         return F.rms_norm(x.float(), (x.shape[-1],), eps=self.eps).to(x.dtype) * self.weight
 
     def add(self, x, residual):
@@ -250,7 +262,7 @@ class RMSNorm(nn.Module):
             return self(total), total
         if residual.dtype != x.dtype and x.dtype != torch.float32:      # rms_norm's result is in its first argument's
             x, residual = residual, x
-        return rms_norm(x, self.weight, residual=residual, eps=self.eps)
+        return tuple(nat.glue().rms_norm(x, self.weight, residual, self.eps, True))
 
     def fp8(self, x):
         """The norm of x in 8 bits: (values, scale of every row)."""
@@ -258,14 +270,18 @@ class RMSNorm(nn.Module):
 
 
 class TokenEmbedding(nn.Embedding):
-    """nn.Embedding whose lookup and gradient run on this package's kernels on the GPU, where none of its options is used."""
+    """nn.Embedding whose lookup and gradients run on this package's kernels on the GPU, where none of its options is used."""
 
-    def forward(self, idx):
+    def _fused(self, idx):
         w = self.weight
         plain = self.padding_idx is None and self.max_norm is None and not self.scale_grad_by_freq and not self.sparse
-        if plain and w.is_cuda and w.dtype in nat.DTYPES and idx.numel() > 0 and idx.device == w.device:
-            return embedding(idx, w)
-        return super().forward(idx)
+        return plain and w.is_cuda and w.dtype in nat.DTYPES and idx.numel() > 0 and idx.device == w.device and _runs_now(w, idx)
+
+    def forward(self, idx):
+        if not torch.jit.is_scripting():
+            if self._fused(idx):
+                return nat.glue().embedding(idx, self.weight, 1.0, True)
+        return F.embedding(idx, self.weight, self.padding_idx, self.max_norm, self.norm_type, self.scale_grad_by_freq, self.sparse)
 
 
 def _untouched(module, cls):

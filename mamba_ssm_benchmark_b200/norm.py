@@ -92,7 +92,7 @@ def rms_norm(x, weight=None, residual=None, eps=1e-5):
     weight: (C) or None.  y is in x's dtype, total in the wider of x's and the residual's; what is normed is total as it is
     kept.  Differentiable with respect to x, weight and residual, whose gradients are one tensor where x and residual
     have one dtype (as those of x + residual are)."""
-    out = nat.glue().rms_norm(x, weight, residual, eps)
+    out = nat.glue().rms_norm(x, weight, residual, eps, False)
     return out[0] if residual is None else tuple(out)
 
 
