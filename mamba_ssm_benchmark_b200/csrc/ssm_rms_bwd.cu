@@ -150,13 +150,18 @@ __global__ void __launch_bounds__(kRmsThreads) rms_bwd_long(const __grid_constan
   for (long long row = blockIdx.x; row < p.rows; row += gridDim.x) {
     const TR* t = static_cast<const TR*>(p.t) + row * p.ts;
     const TX* dy = static_cast<const TX*>(p.y) + row * p.ys;
-    float ss = 0.0f, gt = 0.0f;
-    for (int c = threadIdx.x; c < p.C; c += 512) {
-      const float v = to_f32(t[c]);
-      ss = fmaf(v, v, ss);
-      gt = fmaf(to_f32(dy[c]) * weight_at(p, c), v, gt);
+    double ss = 0.0, gt = 0.0;
+    for (int c0 = threadIdx.x; c0 < p.C; c0 += 512 * kRmsMost) {
+      float2 part = make_float2(0.0f, 0.0f);
+      for (int c = c0; c < min(p.C, c0 + 512 * kRmsMost); c += 512) {
+        const float v = to_f32(t[c]);
+        part.x = fmaf(v, v, part.x);
+        part.y = fmaf(to_f32(dy[c]) * weight_at(p, c), v, part.y);
+      }
+      ss += (double)part.x;
+      gt += (double)part.y;
     }
-    const float2 s = team.sum(make_float2(ss, gt));
+    const float2 s = team.sum(make_float2((float)ss, (float)gt));
     const float rstd = rsqrtf(s.x * p.inv_c + p.eps), mean = s.y * rstd * p.inv_c;
     if (threadIdx.x == 0) stat[row] = rstd;
     for (int c = threadIdx.x; c < p.C; c += 512) {

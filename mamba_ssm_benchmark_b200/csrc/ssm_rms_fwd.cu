@@ -141,14 +141,18 @@ __global__ void __launch_bounds__(kRmsThreads) rms_fwd_long(const __grid_constan
     TR* t = static_cast<TR*>(p.t) + row * p.ts;
     // a thread reads the sums that it wrote itself
     auto value = [&](int c) { return p.r != nullptr ? to_f32(t[c]) : to_f32(x[c]); };
-    float ss = 0.0f;
-    for (int c = threadIdx.x; c < p.C; c += 512) {
-      if (p.r != nullptr) t[c] = from_f32<TR>(to_f32(x[c]) + to_f32(static_cast<const TR*>(p.r)[row * p.rs + c]));
-      const float v = value(c);
-      ss = fmaf(v, v, ss);
+    double ss = 0.0;
+    for (int c0 = threadIdx.x; c0 < p.C; c0 += 512 * kRmsMost) {
+      float part = 0.0f;
+      for (int c = c0; c < min(p.C, c0 + 512 * kRmsMost); c += 512) {
+        if (p.r != nullptr) t[c] = from_f32<TR>(to_f32(x[c]) + to_f32(static_cast<const TR*>(p.r)[row * p.rs + c]));
+        const float v = value(c);
+        part = fmaf(v, v, part);
+      }
+      ss += (double)part;
     }
     const bool norm = !FP8 || p.norm;
-    const float rstd = norm ? rsqrtf(team.sum(ss) * p.inv_c + p.eps) : 1.0f;
+    const float rstd = norm ? rsqrtf(team.sum((float)ss) * p.inv_c + p.eps) : 1.0f;
     auto result = [&](int c) {
       if (!norm) return value(c);
       return value(c) * rstd * weight_at(p, c);

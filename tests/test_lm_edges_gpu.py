@@ -17,6 +17,13 @@ def _randn(*shape, seed=0, dtype=F32):
     return torch.randn(*shape, device=DEV, generator=torch.Generator(device=DEV).manual_seed(seed)).to(dtype)
 
 
+def _within(got, want, bound):
+    """|got - want| <= bound, element by element."""
+    assert got.shape == want.shape
+    off = (got.detach().double() - want).abs()
+    assert bool((off <= bound).all()), float((off / bound.clamp_min(1e-300)).max())
+
+
 @pytest.mark.parametrize("shape", [(8,), (4, 8), (2, 4, 8), (2, 3, 2, 24), (1, 1, 8), (3, 5, 1)])
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_gradients_of_leaves_do_not_share_memory(shape, dtype):
@@ -65,3 +72,35 @@ def test_rms_norm_of_any_layout(dtype):
             tol = 54 * U + 2 * HALF[p.dtype] if k != 3 else 2.0 ** -3
             assert p.shape == q.shape and p.dtype == q.dtype, (i, k)
             assert float((p.double() - q.double()).norm()) <= tol * float(q.double().norm()), (i, k)
+
+
+@pytest.mark.parametrize("C", [8200, 20001, 1 << 17, 1 << 20, 1 << 24])
+@pytest.mark.parametrize("xd,rd", [(F32, None), (F32, F32), (BF16, F32)])
+def test_rms_norm_of_very_long_rows(C, xd, rd):
+    """Equal values, whose roundings add up instead of cancelling.  A sum passes 16 additions of a thread, a rounding of those in
+    float64 and 9 of the warps': 26 u, of which half reaches the root; the root (4 u), inv_c and two products: 27 u of a value as of any
+    row; of a gradient 64 u of its terms' sizes."""
+    x = torch.full((1, C), 1.7, device=DEV, dtype=xd)
+    r = None if rd is None else torch.full((1, C), 0.6, device=DEV, dtype=rd)
+    w = torch.full((C,), 1.1, device=DEV)
+    dy = torch.full((1, C), 0.3, device=DEV)
+    dy[:, ::2] = 0.9
+    dy = dy.to(xd)
+    lv = [t.clone().requires_grad_() for t in (x, w)] + ([] if r is None else [r.clone().requires_grad_()])
+    out = rms_norm(lv[0], lv[1], residual=lv[2] if r is not None else None)
+    y, total = out if r is not None else (out, x)
+    grads = torch.autograd.grad(y, lv, dy)
+    t = total.detach().double()
+    rstd = (t.square().mean() + 1e-5).rsqrt()
+    n, g = t * rstd, dy.double() * w.double()
+    _within(y, n * w.double(), (27 * U + HALF[xd]) * (n * w.double()).abs())
+    mean = (g * n).mean()
+    dx, size = rstd * (g - n * mean), rstd * (g.abs() + n.abs() * mean.abs())
+    _within(grads[0], dx, 64 * U * size + HALF[xd] * dx.abs())
+    _within(grads[1], dy.double()[0] * n[0], 64 * U * (dy.double()[0] * n[0]).abs())
+    if r is not None:
+        _within(grads[2], dx, 64 * U * size + U * dx.abs())
+    y8, scale = rms_norm_fp8(total.detach(), w)
+    want = float((n * w.double()).abs().max()) / 448
+    assert abs(float(scale) / want - 1) <= 29 * U
+    assert bool((y8.float() == 448).all())
