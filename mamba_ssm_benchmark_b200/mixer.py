@@ -426,8 +426,8 @@ class MambaLM(nn.Module):
                  uniforms=None):
         """Samples n_new tokens after ``prompt`` (B, T): one prefill pass with decode states, then one
         decode step per token (a CUDA-graph replay each with ``graph=True``).  With ``top_p``, ``min_p`` or ``uniforms`` ((B, n_new)
-        float32 in [0, 1): the random numbers of the answer) tokens come from ``sample_tokens``, whose settings may be given by row;
-        without, from ``torch.multinomial``."""
+        float32 in [0, 1): the random numbers of the answer) tokens come from ``sample_tokens``, whose settings may be given by row, and
+        logits that leave no token (a NaN) are an error at the end; without, tokens come from ``torch.multinomial``."""
         own = top_p is not None or min_p is not None or uniforms is not None
         if own and uniforms is None:
             uniforms = torch.rand(prompt.shape[0], n_new, device=prompt.device)
@@ -450,7 +450,10 @@ class MambaLM(nn.Module):
             tokens.append(nxt)
             if i + 1 < n_new:
                 logits = advance(nxt, T + i)
-        return torch.cat(tokens, dim=1)
+        out = torch.cat(tokens, dim=1)
+        if own and not torch.cuda.is_current_stream_capturing() and bool((out[:, T:] < 0).any()):
+            raise RuntimeError("logits without a token: a NaN, or nothing above -inf (an id outside the vocabulary in the prompt gives NaN)")
+        return out
 
 
 class GraphDecoder:

@@ -5,6 +5,7 @@ import pytest
 import torch
 import torch.nn as nn
 
+from mamba_ssm_benchmark_b200 import _native as nat
 from mamba_ssm_benchmark_b200 import mixer as mix
 from mamba_ssm_benchmark_b200.mixer import MambaLM, RMSNorm
 
@@ -191,3 +192,20 @@ def test_norms_of_an_8_bit_model_have_their_say(kw, what):
         else:
             lm.blocks[1].norm1 = nn.LayerNorm(64).to(DEV)
         assert not _near(lm(idx), plain, 1e-3)
+
+
+@pytest.mark.parametrize("graph", [False, True])
+def test_answers_without_a_token_are_refused(graph):
+    """An id outside the vocabulary makes NaN of a row's logits, for which sample_tokens gives -1: no answer, and no id to go on from."""
+    lm, prompt = _lm(), _ids()
+    u = torch.rand(2, 4, device=DEV)
+    want = lm.generate(prompt, 4, uniforms=u, graph=graph)
+    bad = prompt.clone()
+    bad[0, 3] = 300
+    with pytest.raises(RuntimeError, match="without a token"):
+        lm.generate(bad, 4, uniforms=u, graph=graph)
+    with pytest.raises(RuntimeError, match="without a token"):
+        lm.generate(bad, 1, top_p=0.9)
+    assert nat.read_device_error() == 2
+    assert torch.equal(lm.generate(prompt, 4, uniforms=u, graph=graph), want)
+    assert torch.equal(lm.generate(prompt, 0, uniforms=u[:, :0]), prompt)
