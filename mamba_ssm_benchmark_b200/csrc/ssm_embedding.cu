@@ -3,8 +3,9 @@
 //   y[t] = scale W[idx[t]],   dW[v] = scale sum over t with idx[t] = v of dy[t]
 // Both directions are bound by memory: the rows that are read and written.  The gradient's places are sorted by token
 // (stable, so that a token's places stay in order), cut into chunks of nearly equal length whatever the tokens'
-// frequencies, and summed chunk by chunk: fp32 within a chunk, fp64 over the chunks that a frequent token spans.  No atomics on
-// floats, a fixed order: results are reproducible.  Rows that no token names are zeroed by CTAs of the same launch.
+// frequencies, and summed chunk by chunk: fp32 within a chunk (up to 127 places, below), fp64 over the chunks that a frequent
+// token spans.  No atomics on floats, a fixed order: results are reproducible.  Rows that no token names are zeroed by CTAs of
+// the same launch.
 //
 // 65536 x 2560 bf16 of 50257 words: forward 68 us (5.7 TB/s of what is read from memory and written), sort 21, sums 103 (DRAM
 // at 67 % of its rate, 5.5 TB/s), long runs 12.  One CTA to a token instead of chunks would have the most frequent one, a
@@ -229,7 +230,8 @@ __global__ void __launch_bounds__(1024) embed_sort(const __grid_constant__ Embed
 // ---- sums of the sorted places ---------------------------------------------------------------------
 constexpr int kSumThreads = 256, kLongest = 64, kRows = 8, kFill = 32;      // kFill: a word of `named`
 
-// Chunk q starts at the first place from q len on where another token begins, or at q len inside a run of more than len.
+// Chunk q starts at the first place from q len on where another token begins, or at q len inside a run of more than len: it has
+// up to 2 len - 1 places, all of which may be one token's, 126 additions of a fp32 sum.
 // The sum of a run of equal tokens goes to the table where the chunk holds all of it, else to the chunk's partial
 // rows: 0 where the run comes from the chunk before, 1 where it starts here and goes on.
 template <typename T, bool RAGGED>

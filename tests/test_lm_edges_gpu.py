@@ -3,7 +3,7 @@
 import pytest
 import torch
 
-from mamba_ssm_benchmark_b200 import rms_norm, rms_norm_fp8
+from mamba_ssm_benchmark_b200 import embedding, rms_norm, rms_norm_fp8
 from oracle import lm_oracle as O
 
 pytestmark = pytest.mark.gpu
@@ -104,3 +104,21 @@ def test_rms_norm_of_very_long_rows(C, xd, rd):
     want = float((n * w.double()).abs().max()) / 448
     assert abs(float(scale) / want - 1) <= 29 * U
     assert bool((y8.float() == 448).all())
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("longest", [64, 127])
+def test_embedding_gradient_of_the_longest_chunks(longest, dtype):
+    """Runs of 127 places and of one in turn: with as many places as here a chunk is nominally 64 long and ends where a run does, so
+    a whole run of 127 is one chunk.  Equal values: 126 additions whose roundings add up, u of the sum each, then the scale and half
+    a step."""
+    turns, C = 1200, 48
+    count = torch.tensor([longest, 128 - longest], device=DEV).repeat(turns)
+    idx = torch.repeat_interleave(torch.arange(2 * turns, device=DEV), count)
+    assert len(idx) == 128 * turns >= 64 * 148 * 12
+    W = torch.zeros(2 * turns, C, device=DEV, dtype=dtype, requires_grad=True)
+    dy = torch.full((len(idx), C), 1 / 3, device=DEV).to(dtype)
+    dw, = torch.autograd.grad(embedding(idx, W, 1.7), W, dy)
+    want = count[:, None].double() * float(dy[0, 0].double()) * 1.7
+    _within(dw, want.expand(-1, C), ((126 + 2) * U + HALF[dtype]) * want)
+    assert torch.equal(dw, torch.autograd.grad(embedding(idx, W, 1.7), W, dy)[0])
