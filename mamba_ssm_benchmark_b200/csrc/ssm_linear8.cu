@@ -271,6 +271,7 @@ __device__ __forceinline__ void finish_channel(const LinearParams& p, uint32_t a
 // CTAs a part of K each.
 template <int TN, typename TY, bool TOKENS, bool SPLIT>
 __global__ void __launch_bounds__(kLinThreads, TN <= 64 ? 2 : 1) linear_e4m3(const __grid_constant__ LinearParams p, int parts) {
+  static_assert(!SPLIT || TN <= 64, "parts of K are for few tiles, which are narrow");
   using Form = LinearForm<TN>;
   constexpr int kStages = Form::kStages;
   extern __shared__ unsigned char raw[];
@@ -431,7 +432,7 @@ __global__ void __launch_bounds__(kLinThreads, TN <= 64 ? 2 : 1) linear_e4m3(con
     __syncwarp();
     cluster_arrive_wait();
     // this CTA's tokens; a warp takes kJoin of them and 32 channels at a time, so that as many loads are on their way
-    constexpr int kPitch = TOKENS ? TN + 1 : kRows, kJoin = kTileM >= 64 ? 8 : kTileM / 8;
+    constexpr int kPitch = TOKENS ? TN + 1 : kRows, kJoin = TOKENS ? 8 : TN / 8;
     const int own = kTileM / parts, m0 = tile_m(first), n0 = tile_n(first);
     for (int item = warp; item < own / kJoin * (kTileN / 32); item += kLinThreads / 32) {
       const int c0 = rank * own + item / (kTileN / 32) * kJoin, col = item % (kTileN / 32) * 32 + lane, n = n0 + col;
@@ -487,9 +488,12 @@ template <int TN, typename TY, bool TOKENS>
 cudaError_t run(LinearParams& p, cudaStream_t st) {
   p.tiles_n = ceil_div(p.channels, TOKENS ? TN : kRows);
   p.tiles = p.tiles_n * ceil_div(p.tokens, TOKENS ? kRows : TN);
-  int parts = 1;
-  while (parts < 8 && p.tiles * parts * 2 <= room(TN) && parts * 2 <= p.blocks) parts *= 2;
-  if (parts > 1) return launch<TN, TY, TOKENS, true>(p, p.tiles * parts, parts, st);
+  // wider tiles are taken where there are 148 of them or more: one to an SM, which leaves no room for parts of K
+  if constexpr (TN <= 64) {
+    int parts = 1;
+    while (parts < 8 && p.tiles * parts * 2 <= room(TN) && parts * 2 <= p.blocks) parts *= 2;
+    if (parts > 1) return launch<TN, TY, TOKENS, true>(p, p.tiles * parts, parts, st);
+  }
   return launch<TN, TY, TOKENS, false>(p, std::min(p.tiles, room(TN)), 1, st);
 }
 template <typename TY>
