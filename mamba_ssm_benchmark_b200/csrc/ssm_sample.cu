@@ -78,6 +78,7 @@ struct SampleSmem {
   int first[1 + 2 * kMargins];        // the first bin at which a sum over the bins passes a value
   u64 cut, rest;                      // rest: what the drawn token's place is short of where its warp's tokens start
   int owner;                          // that warp
+  int half;                           // see Sampler::form
   alignas(16) float logits[4];        // the slice, or kDepth slots of 16 bytes to a thread
 };
 
@@ -280,9 +281,9 @@ struct Sampler {
   int row, ctas, lane, warp, base, per, first, last, turn;
   Weights weight;
   float top, bin_rate;                // the largest logit; bins to a logit
-  bool infinite;
+  bool formed;                        // the passes work on other values than the logits
 
-  __device__ Sampler(const SampleParams& p_, SampleSmem& s_) : p(p_), s(s_), cluster(cg::this_cluster()), turn(0), infinite(false) {
+  __device__ Sampler(const SampleParams& p_, SampleSmem& s_) : p(p_), s(s_), cluster(cg::this_cluster()), turn(0), formed(false) {
     ctas = (int)cluster.num_blocks();
     row = (int)blockIdx.x / ctas;
     logits = static_cast<const T*>(p.logits) + row * p.stride;
@@ -296,13 +297,13 @@ struct Sampler {
     last = min(end, first + per);
     weight.table = s.exp2;
   }
-  static __device__ void finite(float (&l)[4]) {
+  // In a row with infinite logits these alone count: 0, and -inf the others.  Where a float does not hold how far logits are apart and
+  // the temperature is so high that it matters, halves of both (exact but for logits below 2^-125, which are then one to any weight).
+  __device__ __forceinline__ float form(float l) const {
     constexpr float kInf = __builtin_huge_valf();
-#pragma unroll
-    for (int j = 0; j < 4; ++j) l[j] = l[j] == kInf ? 0.0f : -kInf;
+    return s.half ? 0.5f * l : l == kInf ? 0.0f : -kInf;
   }
-  // Four logits from i on; -inf past the warp's last.  In a row with infinite logits these alone count (`infinite`): 0, and -inf
-  // the others.
+  // Four logits from i on; -inf past the warp's last.
   __device__ void load(int i, float (&l)[4]) const {
     constexpr float kInf = __builtin_huge_valf();
     if (p.wide && i + 4 <= last) {
@@ -311,7 +312,10 @@ struct Sampler {
 #pragma unroll
       for (int j = 0; j < 4; ++j) l[j] = i + j < last ? ssm::to_f32(logits[i + j]) : -kInf;
     }
-    if (infinite) finite(l);
+    if (formed) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) l[j] = form(l[j]);
+    }
   }
   __device__ void keep(int i, const float (&l)[4]) {
     *reinterpret_cast<float4*>(s.logits + (i - base)) = make_float4(l[0], l[1], l[2], l[3]);
@@ -325,7 +329,7 @@ struct Sampler {
         ssm::load4(s.logits + (i - base), l);
         f(i, l);
       }
-    } else if (p.wide && !infinite) {     // from L2 or memory: the next ones on their way to this thread's slots
+    } else if (p.wide && !formed) {       // from L2 or memory: the next ones on their way to this thread's slots
       constexpr uint32_t kStep = kThreads * 16, kRing = kDepth * kStep;
       const uint32_t ring = ssm::smem_u32(s.logits) + threadIdx.x * 16;
       const T* from = logits + first + 4 * lane;
@@ -624,22 +628,29 @@ __global__ void __launch_bounds__(kThreads, 2) sample_many(const __grid_constant
     return;
   }
   float spread = a.top + key_logit(ends << 32);           // between the largest and the smallest above -inf
-  if (a.top == kInf) {
-    a.infinite = true;
-    a.top = spread = 0.0f;
+  float heat = (float)set.temperature;                    // held as a float, which is enough for the bins
+  double temperature = set.temperature;
+  if (a.top == kInf || (spread == kInf && 31.0f * heat == kInf)) {
+    const bool half = a.top < kInf;
+    s.half = half;                                        // by every thread, before it reads it
+    a.formed = true;
+    spread = half ? 0.5f * a.top + 0.5f * key_logit(ends << 32) : 0.0f;
+    a.top = half ? 0.5f * a.top : 0.0f;
+    if (half) temperature *= 0.5;
+    heat = (float)temperature;
     for (int i = a.first + 4 * a.lane; p.cached && i < a.last; i += 128) {
       float l[4];
       a.load(i, l);
       a.keep(i, l);
     }
   }
-  a.weight.set(a.top, set.temperature);
+  a.weight.set(a.top, temperature);
   const bool top_k = set.top_k > 0 && set.top_k < p.V, top_p = set.top_p < 1.0;
   u64 cut = 0;
   bool summed = false;                                    // s.kept is known
   if (top_k || top_p) {
     // 31 temperatures below the largest a weight is zero
-    const float range = fminf(31.0f * (float)set.temperature, spread);
+    const float range = fminf(31.0f * heat, spread);
     a.bin_rate = fminf(((float)kBins - 0.01f) / range, 3e38f);
     uint32_t n[kPer];
     a.count_bins(n);
@@ -696,7 +707,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_many(const __grid_constant
     if (top_p) {
       // The masses of this thread's bins, about: as many weights as a bin has tokens, from its middle, in units of 2^-24.  They
       // are made anew when they are needed again, which is rare: held over the pass in between they cost it registers.
-      const float step = range / ((float)kBins - 0.01f) / (float)set.temperature;
+      const float step = range / ((float)kBins - 0.01f) / heat;
       auto masses = [&](u64 (&unit)[kPer], u64& upto) {   // upto: before the first of the thread's bins.  The mass of all.
         u64 mine = 0, mass;
         uint32_t seen = b0 > 0 ? s.upto[b0 - 1] : 0;
@@ -899,7 +910,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_many(const __grid_constant
         float l = -kInf;
         if (i + j < end) {
           l = p.cached ? s.logits[i + j - a.base] : ssm::to_f32(a.logits[i + j]);
-          if (a.infinite && !p.cached) l = l == kInf ? 0.0f : -kInf;
+          if (a.formed && !p.cached) l = a.form(l);
         }
         w[j] = a.weight(l);
         if (!border(l, i + j) || w[j] < set.least) w[j] = 0;

@@ -3,7 +3,7 @@
 import pytest
 import torch
 
-from mamba_ssm_benchmark_b200 import embedding, rms_norm, rms_norm_fp8
+from mamba_ssm_benchmark_b200 import embedding, rms_norm, rms_norm_fp8, sample_tokens
 from oracle import lm_oracle as O
 
 pytestmark = pytest.mark.gpu
@@ -122,3 +122,24 @@ def test_embedding_gradient_of_the_longest_chunks(longest, dtype):
     want = count[:, None].double() * float(dy[0, 0].double()) * 1.7
     _within(dw, want.expand(-1, C), ((126 + 2) * U + HALF[dtype]) * want)
     assert torch.equal(dw, torch.autograd.grad(embedding(idx, W, 1.7), W, dy)[0])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("V", [4, 900, 3000, 60000, 400000])
+def test_sample_the_widest_range(V, dtype):
+    """Logits from the type's lowest value to its highest, whose distances a float32 does not hold, at temperatures where they matter
+    and at ones where they do not; some masked.  Up to 2 V 2^-42 of the largest weight may lie between two tokens at a border."""
+    g = torch.Generator(device=DEV).manual_seed(V)
+    logits = torch.linspace(-1, 1, V, device=DEV).double()[torch.randperm(V, device=DEV, generator=g)] * torch.finfo(dtype).max
+    logits = torch.stack([logits.to(dtype), logits.to(dtype).masked_fill(torch.rand(V, device=DEV, generator=g) < 0.3, float("-inf"))])
+    logits[1, V // 2] = torch.finfo(dtype).max
+    u = torch.tensor([0.03, 0.97], device=DEV)
+    for at in (u, u.flip(0)):
+        for T in (1.0, 1e36, 1e37, 2e37, 1e39, 1e300, float("inf")):
+            for kw in (dict(), dict(top_k=V - 2), dict(top_p=0.9), dict(top_k=V // 2, top_p=0.9), dict(top_k=600), dict(min_p=0.9), dict(top_p=0.01)):
+                got = sample_tokens(logits, at, temperature=T, **kw).tolist()
+                for b in range(2):
+                    l = logits[b].double()
+                    want = O.sample(l, float(at[b].double()), temperature=T, **kw)
+                    between = torch.exp((l[min(got[b], want) + 1:max(got[b], want)] - l.max()) / T).nan_to_num(0.0)
+                    assert got[b] == want or float(between.sum()) < 2 * V * 2.0 ** -42, (T, kw, b, got[b], want)
