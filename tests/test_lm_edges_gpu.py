@@ -143,3 +143,65 @@ def test_sample_the_widest_range(V, dtype):
                     want = O.sample(l, float(at[b].double()), temperature=T, **kw)
                     between = torch.exp((l[min(got[b], want) + 1:max(got[b], want)] - l.max()) / T).nan_to_num(0.0)
                     assert got[b] == want or float(between.sum()) < 2 * V * 2.0 ** -42, (T, kw, b, got[b], want)
+
+
+@pytest.mark.parametrize("residual", [False, True])
+def test_rms_norm_gradient_against_differences_of_its_own_forward(residual):
+    """Along random directions, x, residual and weight together and each alone: (f(+h) - f(-h)) / 2h of the float32 forward.
+    Each f is off by 28 u of every |y c| (27 u and the rounding) and u of every |total c|, so the quotient by that over h; the step
+    itself by what the same quotient of the float64 definition is off at h against h / 1000, whose own error is (h / 1000)^2; a gradient by
+    64 u of its terms' sizes, at most 64 u (|g| + |n| mean|g n|) rstd <= 1000 u here."""
+    rows, C, h = 6, 96, 2.0 ** -6
+    x, w, r = _randn(rows, C, seed=1), 1 + 0.1 * _randn(C, seed=2), 2 * _randn(rows, C, seed=3)
+    cy, ct = _randn(rows, C, seed=4), _randn(rows, C, seed=5)
+    leaves = [x, w] + ([r] if residual else [])
+
+    def loss(norm, at):
+        out = norm(at[0], at[1], *at[2:])
+        y, total = out if residual else (out, None)
+        return float((y.double() * cy.double()).sum() + ((total.double() * ct.double()).sum() if residual else 0.0))
+
+    own = lambda x, w, r=None: rms_norm(x, w, residual=r)
+    exact = lambda x, w, r=None: O.rms_norm(x, w, r) if residual else O.rms_norm(x, w)[0]
+    out = own(*leaves)
+    y, total = (t.double() for t in out) if residual else (out.double(), None)
+    noise = float(28 * U * (y.abs() * cy.abs()).sum() + (U * (total.abs() * ct.abs()).sum() if residual else 0.0)) / h
+    for moved in [tuple(range(len(leaves)))] + [(i,) for i in range(len(leaves))]:
+        d = [_randn(*t.shape, seed=20 + i) if i in moved else torch.zeros_like(t) for i, t in enumerate(leaves)]
+        quotient = lambda norm, at, d, h: (loss(norm, [a + h * b for a, b in zip(at, d)]) - loss(norm, [a - h * b for a, b in zip(at, d)])) / (2 * h)
+        # the points as float32 has them, exactly h d to either side
+        at = [(t * 2 ** 10).round() / 2 ** 10 for t in leaves]
+        d = [(t * 2 ** 10).round() / 2 ** 10 for t in d]
+        lv = [t.clone().requires_grad_() for t in at]
+        grads = torch.autograd.grad(own(*lv), lv, (cy, ct) if residual else cy)
+        wide = [t.double() for t in at], [t.double() for t in d]
+        step = abs(quotient(exact, *wide, h) - quotient(exact, *wide, h / 1000))
+        got = sum(float((g.double() * b.double()).sum()) for g, b in zip(grads, d))
+        size = sum(float(b.abs().double().sum()) for b in d)
+        assert abs(got - quotient(own, at, d, h)) <= noise + step + 1e-5 + 1000 * U * size, moved
+
+
+@pytest.mark.parametrize("xd,rd", [(BF16, None), (BF16, BF16), (BF16, F32), (F32, F32)])
+def test_rms_norm_gradient_along_the_row(xd, rd):
+    """The norm does not change as its row grows: the mean of g n takes away what g has along the row, and without it the
+    derivative would be the sum of g n, ten times the bound in bf16 and more in float32.  That is left by eps and dtotal, exactly known; the bound is the gradient's
+    own rounding and 64 u of its terms."""
+    rows, C = 5, 1000
+    x, w = _randn(rows, C, seed=1, dtype=xd), 1 + 0.1 * _randn(C, seed=2)
+    r = None if rd is None else _randn(rows, C, seed=3).to(rd)
+    lv = [x.clone().requires_grad_()] + ([] if r is None else [r.clone().requires_grad_()])
+    out = rms_norm(lv[0], w, residual=lv[1] if r is not None else None)
+    y, total = out if r is not None else (out, x)
+    t = total.detach().double()
+    rstd = (t.square().mean(-1, keepdim=True) + 1e-5).rsqrt()
+    n = t * rstd
+    dy = (n + 0.3 * _randn(rows, C, seed=4)).to(xd)
+    ct = 0.01 * _randn(rows, C, seed=5).to(total.dtype)
+    grads = torch.autograd.grad(out, lv, (dy, ct) if r is not None else dy)
+    g = dy.double() * w.double()
+    want = (g * n * 1e-5 * rstd.square()).sum(-1) + (0.0 if r is None else (ct.double() * t).sum(-1))
+    size = rstd * (g.abs() + n.abs() * (g * n).abs().mean(-1, keepdim=True)) + (0.0 if r is None else ct.double().abs())
+    for d in grads:
+        bound = ((64 * U * size + HALF[d.dtype] * d.double().abs()) * t.abs()).sum(-1)
+        _within((d.double() * t).sum(-1), want, bound)
+        assert bool(((g * n).sum(-1) > 100 * bound).all() if d.dtype == F32 else ((g * n).sum(-1) > 10 * bound).all())
