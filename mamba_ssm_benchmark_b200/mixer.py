@@ -246,8 +246,13 @@ class RMSNorm(nn.Module):
         self.weight = nn.Parameter(torch.ones(d))
 
     def _fused(self, x):
-        """The kernels take x: on the GPU, in one of their types, which the weight has too."""
-        return x.is_cuda and x.dtype in nat.DTYPES and x.dtype == self.weight.dtype and x.numel() > 0 and _runs_now(x, self.weight)
+        """The kernels take x: on the GPU, in one of their types, which the weight has too, a weight to a channel."""
+        w = self.weight
+        return x.is_cuda and x.dtype in nat.DTYPES and x.dtype == w.dtype and x.numel() > 0 and self._per_channel(x) and _runs_now(x, w)
+
+    def _per_channel(self, x):
+        """What the kernels and torch's form have in common; the latter also broadcasts the weight and knows eps = None."""
+        return self.weight.shape == x.shape[-1:] and self.eps is not None and self.eps >= 0.0
 
     def forward(self, x):
         if not torch.jit.is_scripting():
@@ -300,7 +305,7 @@ def _adds(norm, x):
 
 def _normed8(norm, x):
     """What ``norm`` gives of x, in 8 bits: from the kernel that norms and rounds, where norm is an RMSNorm that nobody touched."""
-    return norm.fp8(x) if _untouched(norm, RMSNorm) else quantize_fp8(norm(x))
+    return norm.fp8(x) if _untouched(norm, RMSNorm) and norm._per_channel(x) else quantize_fp8(norm(x))
 
 
 def _delta_mixer(*args, **kw):

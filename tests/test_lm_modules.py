@@ -110,3 +110,16 @@ def test_the_sum_and_its_norm_are_differentiated_twice(dev):
             res.append([*g, *h, *torch.autograd.grad(only[0].sum() + only[1].float().sum(), [a, b])])
         for k, (p, q) in enumerate(zip(*res)):
             assert _near(p, q, 1e-5 if rd == torch.float32 else 6 * 2.0 ** -8), (rd, k)
+
+
+def test_weights_that_broadcast_and_no_eps(dev):
+    """What torch's form knows and the kernels do not."""
+    x = torch.randn(2, 3, 16, device=dev)
+    one, heads, none = RMSNorm(1).to(dev), RMSNorm(16).to(dev), RMSNorm(16, eps=None).to(dev)
+    with torch.no_grad():
+        one.weight.fill_(3.0)
+    heads.weight = torch.nn.Parameter(torch.randn(3, 16, device=dev))
+    n = F.rms_norm(x, (16,), eps=1e-5)
+    assert _near(one(x), 3 * n) and _near(heads(x), n * heads.weight) and _near(none(x), F.rms_norm(x, (16,)))
+    with torch.inference_mode():
+        assert _near(RMSNorm(16).to(dev)(x), n)

@@ -209,3 +209,21 @@ def test_answers_without_a_token_are_refused(graph):
     assert nat.read_device_error() == 2
     assert torch.equal(lm.generate(prompt, 4, uniforms=u, graph=graph), want)
     assert torch.equal(lm.generate(prompt, 0, uniforms=u[:, :0]), prompt)
+
+
+@pytest.mark.parametrize("eight", [False, True])
+def test_norms_with_one_weight_for_all_channels(eight):
+    """Such a norm is torch's; 2e-3 as for a hooked norm of an 8-bit model."""
+    lm, idx = _lm(), _ids()
+    for norm in (lm.blocks[1].norm1, lm.norm_f):
+        norm.weight = nn.Parameter(torch.full((1,), 1.5, device=DEV))
+    with torch.no_grad():
+        want = _one_by_one(lm, idx)
+        if not eight:
+            assert _near(lm(idx), want, 1e-5)
+            return
+        lm.quantize_fp8()
+        got = lm(idx)
+        for norm in (lm.blocks[1].norm1, lm.norm_f):
+            norm.weight = nn.Parameter(torch.full((64,), 1.5, device=DEV))
+        assert _near(got, lm(idx), 2e-3)
