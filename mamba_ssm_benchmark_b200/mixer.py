@@ -402,14 +402,16 @@ class MambaLM(nn.Module):
     @torch.no_grad()
     def quantize_fp8(self):
         """Puts 8-bit weights (e4m3, a scale for every row) in the places of the blocks' projections and of the head, for
-        answering: decoding then reads a half or a quarter of the bytes.  In place; the model no longer trains.  The mixers'
-        small projections, convolutions and states and the embedding stay as they are.  Returns the model."""
+        answering: decoding then reads a half or a quarter of the bytes of these.  What they multiply (the norms' results, the
+        mixers' inner activations) is put into 8 bits too, row by row, also for the gates of a delta mixer.  In place; the model no
+        longer trains.  The mixers' small projections, convolutions and states, the embedding and a head that is more than a
+        weight (a bias, another module, hooks) stay as they are.  Returns the model."""
         for block in self.blocks:
             for name in ("in_proj", "gate_proj", "out_proj"):
                 holder = getattr(block.mixer, name, None)
                 if holder is not None and not isinstance(holder, Fp8Linear):
                     setattr(block.mixer, name, Fp8Linear(holder.weight))
-        if not isinstance(self.head, Fp8Linear):
+        if _untouched(self.head, nn.Linear) and self.head.bias is None:
             self.head = Fp8Linear(self.head.weight)
         return self
 

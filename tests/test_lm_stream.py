@@ -7,6 +7,7 @@ import torch.nn as nn
 
 from mamba_ssm_benchmark_b200 import _native as nat
 from mamba_ssm_benchmark_b200 import mixer as mix
+from mamba_ssm_benchmark_b200.linear import Fp8Linear
 from mamba_ssm_benchmark_b200.mixer import MambaLM, RMSNorm
 
 pytestmark = pytest.mark.gpu
@@ -227,3 +228,28 @@ def test_norms_with_one_weight_for_all_channels(eight):
         for norm in (lm.blocks[1].norm1, lm.norm_f):
             norm.weight = nn.Parameter(torch.full((64,), 1.5, device=DEV))
         assert _near(got, lm(idx), 2e-3)
+
+
+@pytest.mark.parametrize("what", ["bias", "two layers", "hook", "patched"])
+def test_a_head_that_is_more_than_a_weight_stays(what):
+    """quantize_fp8 leaves it as it is; the logits are those of the head on the norm of the 8-bit blocks' stream, bit by bit."""
+    lm, idx, seen = _lm(), _ids(), []
+    if what == "bias":
+        lm.head = nn.Linear(64, 256).to(DEV)
+        with torch.no_grad():
+            lm.head.bias += 3.0
+    elif what == "two layers":
+        lm.head = nn.Sequential(nn.Linear(64, 32), nn.Linear(32, 256)).to(DEV)
+    elif what == "hook":
+        lm.head.register_forward_hook(lambda m, i, o: o + 3.0)
+    else:
+        _patched(lm.head, seen)
+    head = lm.head
+    with torch.no_grad():
+        assert lm.quantize_fp8().head is head
+        got = lm(idx)
+        x = lm.embed(idx)
+        for block in lm.blocks:
+            assert isinstance(block.mixer.out_proj, Fp8Linear)
+            x = block(x)
+        assert torch.equal(got, head(lm.norm_f(x)))
