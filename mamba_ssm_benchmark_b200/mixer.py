@@ -409,7 +409,7 @@ class MambaLM(nn.Module):
         for block in self.blocks:
             for name in ("in_proj", "gate_proj", "out_proj"):
                 holder = getattr(block.mixer, name, None)
-                if holder is not None and not isinstance(holder, Fp8Linear):
+                if isinstance(holder, _Holder):              # a mixer of another kind keeps what it has
                     setattr(block.mixer, name, Fp8Linear(holder.weight))
         if _untouched(self.head, nn.Linear) and self.head.bias is None:
             self.head = Fp8Linear(self.head.weight)

@@ -253,3 +253,23 @@ def test_a_head_that_is_more_than_a_weight_stays(what):
             assert isinstance(block.mixer.out_proj, Fp8Linear)
             x = block(x)
         assert torch.equal(got, head(lm.norm_f(x)))
+
+
+def test_mixers_of_another_kind_keep_their_weights():
+    """quantize_fp8 knows the projections of this package's mixers; a module that calls its own by the same names goes on as it was."""
+    class Own(nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.in_proj, self.out_proj = nn.Linear(64, 32), nn.Linear(32, 64)
+
+        def forward(self, u, state=None, pos=0):
+            return self.out_proj(torch.tanh(self.in_proj(u)))
+
+    lm, idx = _lm(), _ids()
+    lm.blocks[1].mixer = Own().to(DEV)
+    x = torch.randn(2, 5, 64, device=DEV)
+    with torch.no_grad():
+        want = lm.blocks[1](x)
+        lm.quantize_fp8()
+        assert torch.equal(lm.blocks[1](x), want) and isinstance(lm.blocks[0].mixer.in_proj, Fp8Linear)
+        assert bool(lm(idx).isfinite().all())
