@@ -262,7 +262,8 @@ class RMSNorm(nn.Module):
 
     def add(self, x, residual):
         """(norm of x + residual, x + residual), in one pass over them.  Both are in the type of the sum, the wider of the two."""
-        if x.shape != residual.shape or x.dtype not in nat.DTYPES or residual.dtype not in nat.DTYPES:
+        if x.shape != residual.shape or x.dtype not in nat.DTYPES or residual.dtype not in nat.DTYPES \
+                or type(x) not in _TENSORS or type(residual) not in _TENSORS:
             total = x + residual
             return self(total), total
         if residual.dtype != x.dtype and x.dtype != torch.float32:      # rms_norm's result is in its first argument's

@@ -273,3 +273,26 @@ def test_mixers_of_another_kind_keep_their_weights():
         lm.quantize_fp8()
         assert torch.equal(lm.blocks[1](x), want) and isinstance(lm.blocks[0].mixer.in_proj, Fp8Linear)
         assert bool(lm(idx).isfinite().all())
+
+
+class Tagged(torch.Tensor):
+    pass
+
+
+def test_mixers_that_give_a_tensor_of_another_class():
+    """A subclass of torch.Tensor goes through the stream as through the blocks one by one."""
+    class As(nn.Module):
+        def __init__(self, mixer):
+            super().__init__()
+            self.mixer = mixer
+
+        def forward(self, u, state=None, pos=0):
+            return self.mixer(u.as_subclass(torch.Tensor), state, pos).as_subclass(Tagged)
+
+    lm, idx = _lm(), _ids()
+    for block in lm.blocks:
+        block.mixer = As(block.mixer)
+    with torch.no_grad():
+        got, want = lm(idx), _one_by_one(lm, idx)
+        assert type(want) is Tagged and type(got) is Tagged
+        assert _near(got.as_subclass(torch.Tensor), want.as_subclass(torch.Tensor), 1e-5)
