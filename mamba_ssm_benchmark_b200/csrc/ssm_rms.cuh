@@ -8,13 +8,14 @@
 // thread, and walks over rows; the rows ahead are on their way through slots of shared memory that only the thread
 // that reads them writes (cp.async, no barrier, no registers).  Sums are fp32: at most 16 values in a thread, then a
 // butterfly over the warp and one over the warps.  Rows that no team holds take the kernels that pass over a row again; a thread
-// has more than 16 values there and joins their sums of 16 in fp64 (in one fp32 chain a row of 2^24 equal values was off by 2^-13).
+// has more than 16 values there and joins sums of four in fp64 (in one fp32 chain a row of 2^24 equal values was off by 2^-13).
 #pragma once
 
 #include <cuda_fp8.h>
 
 #include <algorithm>
 #include <initializer_list>
+#include <type_traits>
 
 #include "ssm_b200.h"
 #include "ssm_launch.cuh"
@@ -93,6 +94,14 @@ __device__ __forceinline__ void load_weight(const RmsParams& p, int c, int n, fl
 __device__ __forceinline__ float weight_at(const RmsParams& p, int c) {
   if (p.w == nullptr) return 1.0f;
   return p.wbf16 ? to_f32(static_cast<const __nv_bfloat16*>(p.w)[c]) : static_cast<const float*>(p.w)[c];
+}
+
+// f(c, n) for the channels c, c + 512 .. of this one of a CTA's threads: n (a constant) of them at once, four and the rest singly.
+template <typename F>
+__device__ __forceinline__ void by_fours(int C, F f) {
+  int c = threadIdx.x;
+  for (; c + 3 * kRmsThreads < C; c += 4 * kRmsThreads) f(c, std::integral_constant<int, 4>());
+  for (; c < C; c += kRmsThreads) f(c, std::integral_constant<int, 1>());
 }
 
 // The warps that share a row: `wpr` of a CTA's.  Results of the warps alternate between two buffers: a thread that reads

@@ -142,7 +142,7 @@ __global__ void __launch_bounds__(kRmsThreads) rms_bwd(const __grid_constant__ R
 
 // Rows that no team holds: a CTA per row for the sums and d; rstd goes to `stat`.
 template <typename TX, typename TR>
-__global__ void __launch_bounds__(kRmsThreads) rms_bwd_long(const __grid_constant__ RmsParams p, float* stat) {
+__global__ void __launch_bounds__(kRmsThreads, 4) rms_bwd_long(const __grid_constant__ RmsParams p, float* stat) {
   pdl_launch_dependents();
   pdl_wait();
   __shared__ float2 red[kRmsRed];
@@ -151,16 +151,19 @@ __global__ void __launch_bounds__(kRmsThreads) rms_bwd_long(const __grid_constan
     const TR* t = static_cast<const TR*>(p.t) + row * p.ts;
     const TX* dy = static_cast<const TX*>(p.y) + row * p.ys;
     double ss = 0.0, gt = 0.0;
-    for (int c0 = threadIdx.x; c0 < p.C; c0 += 512 * kRmsMost) {
+    by_fours(p.C, [&](int c, auto n) {
+      float v[n], g[n];
       float2 part = make_float2(0.0f, 0.0f);
-      for (int c = c0; c < min(p.C, c0 + 512 * kRmsMost); c += 512) {
-        const float v = to_f32(t[c]);
-        part.x = fmaf(v, v, part.x);
-        part.y = fmaf(to_f32(dy[c]) * weight_at(p, c), v, part.y);
+#pragma unroll
+      for (int i = 0; i < n; ++i) {
+        v[i] = to_f32(t[c + i * kRmsThreads]);
+        g[i] = to_f32(dy[c + i * kRmsThreads]) * weight_at(p, c + i * kRmsThreads);
       }
+#pragma unroll
+      for (int i = 0; i < n; ++i) part = make_float2(fmaf(v[i], v[i], part.x), fmaf(g[i], v[i], part.y));
       ss += (double)part.x;
       gt += (double)part.y;
-    }
+    });
     const float2 s = team.sum(make_float2((float)ss, (float)gt));
     const float rstd = rsqrtf(s.x * p.inv_c + p.eps), mean = s.y * rstd * p.inv_c;
     if (threadIdx.x == 0) stat[row] = rstd;

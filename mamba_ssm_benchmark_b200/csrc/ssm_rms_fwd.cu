@@ -142,15 +142,30 @@ __global__ void __launch_bounds__(kRmsThreads) rms_fwd_long(const __grid_constan
     // a thread reads the sums that it wrote itself
     auto value = [&](int c) { return p.r != nullptr ? to_f32(t[c]) : to_f32(x[c]); };
     double ss = 0.0;
-    for (int c0 = threadIdx.x; c0 < p.C; c0 += 512 * kRmsMost) {
+    by_fours(p.C, [&](int c, auto n) {
       float part = 0.0f;
-      for (int c = c0; c < min(p.C, c0 + 512 * kRmsMost); c += 512) {
-        if (p.r != nullptr) t[c] = from_f32<TR>(to_f32(x[c]) + to_f32(static_cast<const TR*>(p.r)[row * p.rs + c]));
-        const float v = value(c);
+      auto one = [&](int c, float v) {
+        if (p.r != nullptr) {
+          const TR sum = from_f32<TR>(v + to_f32(static_cast<const TR*>(p.r)[row * p.rs + c]));
+          t[c] = sum;
+          v = to_f32(sum);
+        }
         part = fmaf(v, v, part);
+      };
+      // Loads ahead of the sums' stores; in 8 bits, where two more passes want registers, four at once leave fewer CTAs to an SM or
+      // shorter loops (512 x 65536 bf16: 162 us, this way 141; plain 97, one after another 104).
+      if constexpr (FP8) {
+#pragma unroll
+        for (int i = 0; i < n; ++i) one(c + i * kRmsThreads, to_f32(x[c + i * kRmsThreads]));
+      } else {
+        float v[n];
+#pragma unroll
+        for (int i = 0; i < n; ++i) v[i] = to_f32(x[c + i * kRmsThreads]);
+#pragma unroll
+        for (int i = 0; i < n; ++i) one(c + i * kRmsThreads, v[i]);
       }
       ss += (double)part;
-    }
+    });
     const bool norm = !FP8 || p.norm;
     const float rstd = norm ? rsqrtf(team.sum((float)ss) * p.inv_c + p.eps) : 1.0f;
     auto result = [&](int c) {
