@@ -232,7 +232,7 @@ _TENSORS = (torch.Tensor, nn.Parameter)
 def _runs_now(a, b):
     """Whether a and b are tensors that a kernel can be given, and the call is nothing but a call: not one of ``torch.compile``, export
     or ``torch.jit.trace``, of forward-mode derivatives or of ``torch.func``.  All of these go through torch's own operators."""
-    return not (torch.compiler.is_compiling() or torch.jit.is_tracing() or forward_ad._current_level >= 0
+    return not (torch.compiler.is_compiling() or torch._C._is_tracing() or forward_ad._current_level >= 0
                 or torch._C._functorch.peek_interpreter_stack() is not None) and type(a) in _TENSORS and type(b) in _TENSORS
 
 
@@ -248,11 +248,12 @@ class RMSNorm(nn.Module):
     def _fused(self, x):
         """The kernels take x: on the GPU, in one of their types, which the weight has too, a weight to a channel."""
         w = self.weight
-        return x.is_cuda and x.dtype in nat.DTYPES and x.dtype == w.dtype and x.numel() > 0 and self._per_channel(x) and _runs_now(x, w)
+        return x.is_cuda and x.dtype in nat.DTYPES and x.dtype == w.dtype and x.numel() > 0 and self._per_channel(x, w) and _runs_now(x, w)
 
-    def _per_channel(self, x):
+    def _per_channel(self, x, w):
         """What the kernels and torch's form have in common; the latter also broadcasts the weight and knows eps = None."""
-        return self.weight.shape == x.shape[-1:] and self.eps is not None and self.eps >= 0.0
+        eps = self.eps
+        return w.shape == x.shape[-1:] and eps is not None and eps >= 0.0
 
     def forward(self, x):
         if not torch.jit.is_scripting():
@@ -306,7 +307,7 @@ def _adds(norm, x):
 
 def _normed8(norm, x):
     """What ``norm`` gives of x, in 8 bits: from the kernel that norms and rounds, where norm is an RMSNorm that nobody touched."""
-    return norm.fp8(x) if _untouched(norm, RMSNorm) and norm._per_channel(x) else quantize_fp8(norm(x))
+    return norm.fp8(x) if _untouched(norm, RMSNorm) and norm._per_channel(x, norm.weight) else quantize_fp8(norm(x))
 
 
 def _delta_mixer(*args, **kw):
