@@ -440,9 +440,11 @@ int chunk_len(int64_t T, int64_t C) {
 }
 
 int run_sort(const EmbedParams& p, uint2* a, uint2* b, int passes, cudaStream_t st) {
-  // The barriers of a cluster cost more than its CTAs save while one CTA's warps take a few dozen places each; with many
-  // places their scattered stores, one a clock and SM, take most of the time.
-  const int ctas = p.T <= 4096 ? 1 : p.T <= 16384 ? 8 : 16;
+  // With few places the barriers of a cluster cost as much as its CTAs save; with many their scattered stores, one a clock and SM,
+  // take most of the time.  Forward and gradient of 50257 words of 16 channels in a graph, us with one, eight and sixteen CTAs:
+  // 512 places 20.5, 21.9, 23.6; 1024: 22.6, 22.7, 24.6; 4096: 28.7, 24.6, 26.7; 16384: 68.9, 29.6, 29.9; 32768: 122, 39.1, 37.3;
+  // 65536: 225, 57, 51.
+  const int ctas = p.T <= 1024 ? 1 : p.T <= 16384 ? 8 : 16;
   ssm::ctas_per_sm<embed_sort>(1024, sizeof(SortSmem));
   if (ctas > 8) {
     const cudaError_t e = cudaFuncSetAttribute(embed_sort, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);

@@ -205,3 +205,15 @@ def test_rms_norm_gradient_along_the_row(xd, rd):
         bound = ((64 * U * size + HALF[d.dtype] * d.double().abs()) * t.abs()).sum(-1)
         _within((d.double() * t).sum(-1), want, bound)
         assert bool(((g * n).sum(-1) > 100 * bound).all() if d.dtype == F32 else ((g * n).sum(-1) > 10 * bound).all())
+
+
+@pytest.mark.parametrize("T", [1, 31, 1023, 1024, 1025, 1500, 2048, 4096, 16384, 16385])
+@pytest.mark.parametrize("V", [3, 511, 512, 70000])
+def test_embedding_gradient_on_both_sides_of_the_sorts_borders(T, V):
+    """One CTA, eight and sixteen, a pass or two: whole numbers, whose sums are exact."""
+    g = torch.Generator(device=DEV).manual_seed(T)
+    idx = torch.randint(0, V, (T,), device=DEV, generator=g)
+    W = torch.zeros(V, 8, device=DEV, requires_grad=True)
+    dy = torch.randint(-4, 5, (T, 8), device=DEV, generator=g).float()
+    dw, = torch.autograd.grad(embedding(idx, W), W, dy)
+    assert torch.equal(dw.double(), O.embedding_grad(idx, dy, V, 1.0)[0])
