@@ -19,6 +19,28 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return r;
 }
 
+// Of a row whose largest |t w| is `big`: the scale, and what t w is multiplied by for e4m3.  y / scale is t w 448 / big, which
+// the root does not enter: four roundings, 4 u.  With the product of the root and the scale's reciprocal, within 2 and 1 ulp, more
+// values next to a border between two e4m3 went to the wrong one (8192 x 2560: 0.72 of a million, this way 0.57), and 8 bits of
+// 16384 x 5120 without a residual took 81 us for 74.  A zero row, and one whose root overflowed, is 0 (0 x inf is NaN and fmaxf
+// passes over it).
+__device__ __forceinline__ float row_scale(float big, float rstd) { return fmaxf(big * rstd, kRmsTiny) / kE4m3Max; }
+// false: t w is multiplied by rstd first, for the product of the two factors is out of range (a row about as small as kRmsTiny)
+__device__ __forceinline__ bool row_factor(float big, float rstd, float& f) {
+  const float top = big * rstd;
+  if (top > kRmsTiny && top < __int_as_float(0x7f800000) && big > 1e-35f) {
+    // 448 / big: a reciprocal of normal size, and one step of Newton's
+    const float r = rcp(big * (1.0f / kE4m3Max));
+    f = fmaf(fmaf(-r, big, kE4m3Max), r * (1.0f / kE4m3Max), r);
+    return true;
+  }
+  const float inv = rcp(row_scale(big, rstd));
+  f = rstd * inv;
+  const bool fits = !(f > 1e38f);
+  if (!fits) f = inv;
+  return fits;
+}
+
 template <typename TX, typename TR, int VEC, int K, bool FP8, bool RAGGED>
 __global__ void __launch_bounds__(kRmsThreads) rms_fwd(const __grid_constant__ RmsParams p, int wpr) {
   using SX = Slot<TX, VEC, RAGGED>;
@@ -98,16 +120,14 @@ __global__ void __launch_bounds__(kRmsThreads) rms_fwd(const __grid_constant__ R
       for (int k = 0; k < K; ++k)
 #pragma unroll
         for (int i = 0; i < VEC / 2; ++i) big = max3(big, fabsf(v[k][i].x), fabsf(v[k][i].y));
-      // a zero row, and one whose root overflowed, is 0 (0 x inf is NaN and fmaxf passes over it)
-      const float scale = fmaxf(team.max(big) * rstd, kRmsTiny) / kE4m3Max, inv = rcp(scale);
-      if (team.tid == 0) p.scale[row] = scale;
-      float f = rstd * inv;
-      if (f > 1e38f) {                            // of a row about as small as kRmsTiny: one factor after the other
+      big = team.max(big);
+      if (team.tid == 0) p.scale[row] = row_scale(big, rstd);
+      float f;
+      if (!row_factor(big, rstd, f)) {            // one factor after the other
 #pragma unroll
         for (int k = 0; k < K; ++k)
 #pragma unroll
           for (int i = 0; i < VEC / 2; ++i) v[k][i] = mul2(v[k][i], bc2(rstd));
-        f = inv;
       }
 #pragma unroll
       for (int k = 0; k < K; ++k) {
@@ -131,7 +151,7 @@ __global__ void __launch_bounds__(kRmsThreads) rms_fwd(const __grid_constant__ R
 // Rows that no team holds (above 8192 channels): a CTA passes over the row for the sum
 // of squares, for the largest value and for the result.
 template <typename TX, typename TR, bool FP8>
-__global__ void __launch_bounds__(kRmsThreads) rms_fwd_long(const __grid_constant__ RmsParams p) {
+__global__ void __launch_bounds__(kRmsThreads, 4) rms_fwd_long(const __grid_constant__ RmsParams p) {
   pdl_launch_dependents();
   pdl_wait();
   __shared__ float2 red[kRmsRed];
@@ -152,8 +172,8 @@ __global__ void __launch_bounds__(kRmsThreads) rms_fwd_long(const __grid_constan
         }
         part = fmaf(v, v, part);
       };
-      // Loads ahead of the sums' stores; in 8 bits, where two more passes want registers, four at once leave fewer CTAs to an SM or
-      // shorter loops (512 x 65536 bf16: 162 us, this way 141; plain 97, one after another 104).
+      // Loads ahead of the sums' stores (512 x 65536 bf16 95 us, one after another 104); in 8 bits the two more passes want their
+      // registers (162 us, one after another 131).
       if constexpr (FP8) {
 #pragma unroll
         for (int i = 0; i < n; ++i) one(c + i * kRmsThreads, to_f32(x[c + i * kRmsThreads]));
@@ -168,17 +188,19 @@ __global__ void __launch_bounds__(kRmsThreads) rms_fwd_long(const __grid_constan
     });
     const bool norm = !FP8 || p.norm;
     const float rstd = norm ? rsqrtf(team.sum((float)ss) * p.inv_c + p.eps) : 1.0f;
+    // in 8 bits without rstd, which joins the scale
     auto result = [&](int c) {
       if (!norm) return value(c);
-      return value(c) * rstd * weight_at(p, c);
+      return FP8 ? value(c) * weight_at(p, c) : value(c) * rstd * weight_at(p, c);
     };
     if constexpr (FP8) {
-      float big = 0.0f;
+      float big = 0.0f, f;
       for (int c = threadIdx.x; c < p.C; c += 512) big = fmaxf(big, fabsf(result(c)));
-      const float scale = fmaxf(team.max(big), kRmsTiny) / kE4m3Max, inv = rcp(scale);
-      if (threadIdx.x == 0) p.scale[row] = scale;
+      big = team.max(big);
+      if (threadIdx.x == 0) p.scale[row] = row_scale(big, rstd);
+      const float first = row_factor(big, rstd, f) ? 1.0f : rstd;
       for (int c = threadIdx.x; c < p.C; c += 512)
-        static_cast<uint8_t*>(p.y)[row * p.ys + c] = __nv_cvt_float_to_fp8(result(c) * inv, __NV_SATFINITE, __NV_E4M3);
+        static_cast<uint8_t*>(p.y)[row * p.ys + c] = __nv_cvt_float_to_fp8(result(c) * first * f, __NV_SATFINITE, __NV_E4M3);
     } else {
       for (int c = threadIdx.x; c < p.C; c += 512) static_cast<TX*>(p.y)[row * p.ys + c] = from_f32<TX>(result(c));
     }

@@ -3,7 +3,7 @@
 import pytest
 import torch
 
-from mamba_ssm_benchmark_b200 import embedding, rms_norm, rms_norm_fp8, sample_tokens
+from mamba_ssm_benchmark_b200 import embedding, quantize_fp8, rms_norm, rms_norm_fp8, sample_tokens
 from oracle import lm_oracle as O
 
 pytestmark = pytest.mark.gpu
@@ -217,3 +217,31 @@ def test_embedding_gradient_on_both_sides_of_the_sorts_borders(T, V):
     dy = torch.randint(-4, 5, (T, 8), device=DEV, generator=g).float()
     dw, = torch.autograd.grad(embedding(idx, W), W, dy)
     assert torch.equal(dw.double(), O.embedding_grad(idx, dy, V, 1.0)[0])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("norm", [False, True])
+@pytest.mark.parametrize("C", [96, 2560, 9000])
+def test_values_next_to_the_borders_of_e4m3(C, norm, dtype):
+    """Rows full of values near the middle between two e4m3, off it by up to 16 float32 steps.  y / scale = t w 448 / max|t w|: the
+    products t w (of the value and of the largest one), the quotient and the last product round, u each; a value further than that from the middle
+    goes to its nearest."""
+    g = torch.Generator(device=DEV).manual_seed(C)
+    rows = 300
+    mids = torch.tensor([(8 + k + 0.5) * 2.0 ** e for e in range(-4, 5) for k in range(8)], device=DEV).double()
+    mids = mids[mids < 440]
+    big = torch.exp(4 * torch.randn(rows, 1, device=DEV, generator=g)).to(dtype)
+    off = torch.randint(-16, 17, (rows, C), device=DEV, generator=g).double() * 2.0 ** -23
+    w = 1 + 0.1 * torch.randn(C, device=DEV, generator=g) if norm else torch.ones(C, device=DEV)
+    v = mids[torch.randint(0, len(mids), (rows, C), device=DEV, generator=g)] * (1 + off) * (1 - 2 * torch.randint(0, 2, (rows, C), device=DEV, generator=g))
+    x = (v * big.double() / 448 / w.double()).to(dtype)
+    x[:, 5] = big[:, 0]
+    x[:, 5] *= 2
+    y8, scale = rms_norm_fp8(x, w) if norm else quantize_fp8(x)
+    t = x.double() * w.double()
+    v = t * 448 / t.abs().amax(-1, keepdim=True)
+    half = torch.exp2(torch.floor(torch.log2(v.abs().clamp_min(2.0 ** -6))) - 4)
+    _within(y8.double(), v, half + (4 if norm else 2) * U * (1 + 2 * U) * v.abs())
+    y = O.rms_norm(x.double(), w.double())[0] if norm else t
+    want = y.abs().amax(-1) / 448
+    _within(scale, want, (27 + 2) * U * want)
