@@ -10,9 +10,10 @@
 // multiplies, eight warps read the accumulators of one tile while the next is multiplied.  Few tiles: the CTAs of a
 // cluster take a part of K each and add their sums, in order, through distributed shared memory.
 //
-// 16384 x 5120 x 2560 with bias and residual: 163 us alone (2.6 PFLOP/s, tensor pipe 77 % active), 207 in a stream of calls, where
-// the card's power decides; cuBLAS with row scales and neither bias nor residual took 167 alone.  64 x 2560 x 10240: 12.4 us
-// for 26 MB of weights: prologue 1.5, two parts of K 3.0, their joining 2.8, barriers and the end 2 (clocks in the kernel).
+// 16384 x 5120 x 2560 with bias and residual: 163 us alone behind a cleared L2 (2.6 PFLOP/s, tensor pipe 77 % active), 196 to 207
+// in a stream of calls, where the card's power decides.  Without them 156 and 179; so cuBLAS 171 and 182 with row scales, 164 and
+// 154 with one scale.  64 x 2560 x 10240: 11.9 us for 26 MB of weights: prologue 1.5, two parts of K 3.0, their joining 2.8,
+// barriers and the end 2 (clocks in the kernel).
 // Wider joins (16 tokens, or 16 bytes a lane, at a time) were no faster.
 #include <algorithm>
 #include <cstdio>

@@ -15,9 +15,11 @@
 // sums of what lies before them.  Where the bins' masses mislead, the exact sum at the list's edge says where to look next; where
 // a bin holds more than kList tokens (hundreds of equal logits) a pass over the row takes eleven bits of the border's rank.
 //
-// 256 x 131072 fp32 by top-p: 138 us, 0.4 GB of DRAM in three passes, whose loads are four ahead in slots of shared memory; the
-// instructions they issue bound them, on the 108 SMs that have two rows (clocks in the kernel: maximum 38 thousand,
-// histogram 64, list and sums 115, all else 45).  By temperature alone 72 us, by top-k 75.  64 x 50257 bf16 with all rules: 18 us,
+// 256 x 131072 fp32 by top-p: 138 us, 0.4 GB of DRAM in three passes, whose loads are four ahead in slots of shared memory.  The
+// 108 SMs that have two rows decide (263 thousand clocks: maximum 38, histogram 64, list and sums 115, all else 45); a row
+// that has its SM alone takes 218, so what bounds a row is the latency of its passes' chains (a load, the table, a weight's double
+// arithmetic), and only the fifth that the second row adds is issue slots, 55 % of which are used over the GPU.  By temperature
+// alone 72 us, by top-k 75.  64 x 50257 bf16 with all rules: 18 us,
 // the barriers of passes of 1 to 3 us each.  Bisection of the rank, the first form, took 6690 and 518 us.
 #include <cooperative_groups.h>
 
