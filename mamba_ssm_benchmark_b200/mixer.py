@@ -292,10 +292,10 @@ class TokenEmbedding(nn.Embedding):
 
 
 def _untouched(module, cls):
-    """Whether module is a cls as it comes from here: no subclass, no method replaced on the instance, nothing hooked.  Only then
-    may its work be done without calling it."""
+    """Whether module is a cls as it comes from here: no subclass, no method replaced on the instance, no forward on the class,
+    nothing hooked.  Only then may its work be done without calling it."""
     own = module.__dict__
-    return type(module) is cls and not ("forward" in own or "add" in own or "fp8" in own or "inner" in own) and not (
+    return type(module) is cls and cls.forward is _FORWARD[cls] and not ("forward" in own or "add" in own or "fp8" in own or "inner" in own) and not (
         module._forward_hooks or module._forward_pre_hooks or module._backward_hooks or module._backward_pre_hooks
         or torch.nn.modules.module._has_any_global_hook())
 
@@ -346,6 +346,9 @@ class MambaBlock(nn.Module):
         so that the next norm adds them.  (h', x') with x' + h' what ``forward(x + h)`` gives."""
         y, x = (self.norm1(x), x) if h is None else self.norm1.add(h, x)
         return self.mixer(y, state, pos), x
+
+
+_FORWARD = {cls: cls.forward for cls in (RMSNorm, MambaBlock, nn.Linear)}
 
 
 # ------------------------------------------------------------------------------------------------
